@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define ML_ABI_VERSION 11
+#define ML_ABI_VERSION 12
 
 /* dtype tags */
 #define ML_F32 0
@@ -157,6 +157,52 @@ int ml_swiglu_fwd(const void* gate, const void* up, void* out, int64_t n, int dt
  */
 int ml_swiglu_bwd(const void* gate, const void* up, const void* dy, void* dgate, void* dup,
                   int64_t n, int dtype, void* stream);
+
+/* ------------------------------------------------------------------ dropout
+ * No reference counterpart (nn.Dropout, which its models keep). For n
+ * contiguous elements, numbered from 0:
+ *
+ *   out_i = kept_i ? scale * x_i : 0   (+ residual_i)
+ *
+ * threshold = round(65536 p), 0..65536; scale: 65536 / (65536 - threshold) for
+ * dropout, 1 for its mask alone. kept_i: the (i mod 8)-th 16-bit part
+ * (low halves first) of the four words of Philox4x32 with 7 rounds at the
+ * counter (i div 8 as 64 bits, stream_id, 0) and the key *seed is at least
+ * threshold. seed: one int64 in DEVICE memory; stream_id: 32 bits, so that one
+ * seed serves several masks. The gradient of x is the same call over the
+ * gradient of out (without residual). residual may be NULL; out may be x or
+ * residual. A dropped element contributes 0 whatever x holds there.
+ */
+int ml_dropout(const void* x, const void* residual, void* out, int64_t n, int64_t threshold,
+               float scale, const int64_t* seed, int64_t stream_id, int dtype, void* stream);
+
+/* ---------------------------------------------------------------- embedding
+ * No reference counterpart (nn.Embedding, which its models keep). ids: n
+ * integers of id_bytes (4 or 8), in DEVICE memory; weight [vocab, hidden], row
+ * stride ldw; out [n, hidden] dense:
+ *
+ *   out[k] = scale * weight[ids[k]]
+ *
+ * An id outside 0..vocab-1 gives a row of NaN.
+ */
+int ml_embedding_fwd(const void* ids, int id_bytes, int64_t n, const void* weight, int64_t ldw,
+                     void* out, int64_t vocab, int64_t hidden, float scale, int dtype,
+                     void* stream);
+
+/*
+ * The gradient of the table, dense [vocab, hidden]:
+ *
+ *   dweight[v] = scale * sum of dy[k] over the k with ids[k] = v
+ *
+ * summed in fp32 in an order that the ids alone decide (bit-reproducible);
+ * zero for rows that no id names and for padding_idx (-1: none). Ids outside
+ * the table are skipped. dy [n, hidden], row stride lddy.
+ */
+size_t ml_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t hidden);
+int ml_embedding_bwd(const void* ids, int id_bytes, int64_t n, const void* dy, int64_t lddy,
+                     void* dweight, int64_t vocab, int64_t hidden, int64_t padding_idx,
+                     float scale, void* workspace, size_t workspace_bytes, int dtype,
+                     void* stream);
 
 /* --------------------------------------------------------------------- RoPE
  * Rotate-half rotary embedding over one or two [B, H, S, D] tensors (q and,

@@ -19,6 +19,8 @@ _SUBMODULES = (
     "ops.fused_rope",
     "ops.fused_linear_cross_entropy",
     "ops.fused_lora",
+    "ops.fused_dropout",
+    "ops.fused_embedding",
     "patch",
     "_torch_library",
     "_compile",

@@ -14,6 +14,8 @@ from metal_liger_amd.ops.fused_rms_norm import MetalLigerRMSNorm  # noqa: E402
 from metal_liger_amd.ops.fused_swiglu import MetalLigerSwiGLU  # noqa: E402
 from metal_liger_amd.ops.fused_rope import MetalLigerRoPE  # noqa: E402
 from metal_liger_amd.ops.fused_linear_cross_entropy import MetalLigerFusedLinearCrossEntropy  # noqa: E402
+from metal_liger_amd.ops.fused_dropout import MetalLigerDropout, fused_dropout  # noqa: E402
+from metal_liger_amd.ops.fused_embedding import MetalLigerEmbedding, fused_embedding  # noqa: E402
 from metal_liger_amd.ops.fused_lora import (  # noqa: E402
     apply_fused_lora_mlp,
     apply_fused_lora_qkv,
@@ -30,6 +32,10 @@ __all__ = [
     "MetalLigerSwiGLU",
     "MetalLigerRoPE",
     "MetalLigerFusedLinearCrossEntropy",
+    "MetalLigerDropout",
+    "MetalLigerEmbedding",
+    "fused_dropout",
+    "fused_embedding",
     "apply_metal_liger_to_qwen3vl",
     "apply_fused_lora_qkv",
     "apply_fused_lora_mlp",

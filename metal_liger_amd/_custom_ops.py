@@ -312,8 +312,8 @@ def _(x2, w):
     return x2.new_empty((x2.shape[0], w.shape[0]), dtype=torch.bfloat16)
 
 
-# The packing and unpacking of adapters, registered without custom_op's wrapper:
-# the wrapper costs the host 4.7 us a call with lists of tensors (7.9 against 3.2
+# Dropout, the embedding and the packing and unpacking of adapters, registered
+# without custom_op's wrapper: the wrapper costs the host 4.7 us a call with lists of tensors (7.9 against 3.2
 # for an op that only allocates), which made few-token passes slower than the
 # tensor operations that each of these replaces ([205, 1024] to 1024 at rank 8, a
 # pass on one thread: 186 us by those operations, 202 through custom_op).
@@ -338,6 +338,18 @@ def _define(schema: str, fn, fake):
     _LIB.impl(name, torch.library.fallthrough_kernel, "Autograd")
     torch.library.register_fake(f"{NS}::{name}", fake, lib=_LIB)
     return getattr(getattr(torch.ops, NS), name).default
+
+
+dropout = _define("dropout(Tensor x, Tensor? residual, Tensor seed, SymInt threshold, SymInt stream, "
+                  "float scale) -> Tensor", hip_ops.dropout,
+                  lambda x, residual, seed, threshold, stream, scale: x.new_empty(x.shape))
+embedding_fwd = _define("embedding_fwd(Tensor ids, Tensor weight, float scale) -> Tensor",
+                        hip_ops.embedding_fwd,
+                        lambda ids, weight, scale: weight.new_empty((*ids.shape, weight.shape[1])))
+embedding_bwd = _define("embedding_bwd(Tensor ids, Tensor dy, SymInt vocab, SymInt padding_idx, "
+                        "float scale) -> Tensor", hip_ops.embedding_bwd,
+                        lambda ids, dy, vocab, padding_idx, scale:
+                        dy.new_empty((vocab, dy.shape[-1])))
 
 
 def _lora_pack_fake(As, Bs, scales, rank):

@@ -52,6 +52,12 @@ SIGNATURES: dict[str, tuple] = {
     ),
     "ml_swiglu_fwd": (_i32, [_p, _p, _p, _i64, _i32, _p]),
     "ml_swiglu_bwd": (_i32, [_p, _p, _p, _p, _p, _i64, _i32, _p]),
+    "ml_dropout": (_i32, [_p, _p, _p, _i64, _i64, _f32, _p, _i64, _i32, _p]),
+    "ml_embedding_fwd": (_i32, [_p, _i32, _i64, _p, _i64, _p, _i64, _i64, _f32, _i32, _p]),
+    "ml_embedding_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "ml_embedding_bwd": (
+        _i32, [_p, _i32, _i64, _p, _i64, _p, _i64, _i64, _i64, _f32, _p, _sz, _i32, _p],
+    ),
     "ml_rope_table": (
         _i32,
         [_p, _p, _i64p, _p, _p, _i64p, _i64, _p, _p, _i64p, _f32, _i32, _i32, _i32, _p],
@@ -170,7 +176,7 @@ SIGNATURES: dict[str, tuple] = {
     ),
 }
 
-ABI_VERSION = 11
+ABI_VERSION = 12
 
 _lib = None
 _lock = threading.Lock()

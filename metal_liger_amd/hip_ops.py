@@ -153,6 +153,92 @@ def swiglu_bwd(gate: torch.Tensor, up: torch.Tensor, dy: torch.Tensor):
     return dg, du
 
 
+# ----------------------------------------------------------------- dropout --
+
+
+def drop_threshold(p: float) -> int:
+    """The 16-bit threshold of a rate: round(65536 p). Refuses p outside [0, 1]."""
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError(f"dropout: the rate must be between 0 and 1 (got {p})")
+    return int(p * 65536 + 0.5)
+
+
+def drop_scale(threshold: int) -> float:
+    """The factor of kept elements: the inverse of the rate that is applied."""
+    return 65536.0 / (65536 - threshold) if threshold < 65536 else 0.0
+
+
+def check_seed(seed: torch.Tensor) -> None:
+    if seed.dtype != torch.int64 or seed.numel() != 1:
+        raise TypeError("dropout: the seed must be one int64 "
+                        f"(got {seed.dtype} of shape {tuple(seed.shape)})")
+
+
+def dropout(x: torch.Tensor, residual: torch.Tensor | None, seed: torch.Tensor, threshold: int,
+            stream: int, scale: float) -> torch.Tensor:
+    """scale * x where kept, else 0, + residual (ml_dropout's masks over x's
+    elements in row-major order, whatever its strides); contiguous, x's dtype."""
+    ensure_rocm_device(x, residual, seed)
+    check_seed(seed)
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError(f"dropout: residual {tuple(residual.shape)} {residual.dtype} does not "
+                             f"match x {tuple(x.shape)} {x.dtype}")
+        residual = residual.contiguous()
+    x = x.contiguous()
+    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    call("ml_dropout", ptr(x), ptr(residual), ptr(out), x.numel(), threshold, float(scale), ptr(seed),
+         stream, dtype_tag(x, "x"), stream_of(x))
+    return out
+
+
+# --------------------------------------------------------------- embedding --
+
+
+def _ids(ids: torch.Tensor) -> torch.Tensor:
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"embedding: ids must be int64 or int32 (got {ids.dtype})")
+    return ids.contiguous()
+
+
+def embedding_fwd(ids: torch.Tensor, weight: torch.Tensor, scale: float) -> torch.Tensor:
+    """scale * weight[ids] -> [*ids.shape, hidden] in weight's dtype; an id outside
+    the table gives a row of NaN."""
+    ensure_rocm_device(ids, weight)
+    if weight.dim() != 2 or 0 in weight.shape:
+        raise ValueError(f"embedding: the table must be [vocab, hidden] (got {tuple(weight.shape)})")
+    V, H = weight.shape
+    if weight.stride(1) != 1 or weight.stride(0) < H:
+        weight = weight.contiguous()
+    ids = _ids(ids)
+    out = torch.empty((*ids.shape, H), dtype=weight.dtype, device=weight.device)
+    call("ml_embedding_fwd", ptr(ids), ids.element_size(), ids.numel(), ptr(weight),
+         row_stride(weight), ptr(out), V, H, float(scale), dtype_tag(weight, "weight"),
+         stream_of(weight))
+    return out
+
+
+def embedding_bwd(ids: torch.Tensor, dy: torch.Tensor, vocab: int, padding_idx: int,
+                  scale: float) -> torch.Tensor:
+    """The gradient [vocab, hidden] of the table, in dy's dtype: scale times the
+    sums (fp32, in an order that the ids decide) of the rows of dy that name each
+    entry; zero for padding_idx (-1: none)."""
+    ensure_rocm_device(ids, dy)
+    if dy.shape[:-1] != ids.shape:
+        raise ValueError(f"embedding backward: grad shape {tuple(dy.shape)} does not match ids "
+                         f"{tuple(ids.shape)}")
+    H, n = dy.shape[-1], ids.numel()
+    ids = _ids(ids)
+    dw = torch.empty(vocab, H, dtype=dy.dtype, device=dy.device)
+    dy2 = rows_view(dy) if n > 0 else dy.reshape(0, H)
+    wsb = _hip.query("ml_embedding_bwd_workspace_bytes", n, vocab, H)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dy.device) if wsb else None
+    call("ml_embedding_bwd", ptr(ids), ids.element_size(), n, ptr(dy2), row_stride(dy2), ptr(dw),
+         vocab, H, padding_idx, float(scale), ptr(ws), wsb, dtype_tag(dy, "grad"), stream_of(dy))
+    return dw
+
+
 # -------------------------------------------------------------------- RoPE --
 
 

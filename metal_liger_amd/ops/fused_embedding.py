@@ -1,0 +1,108 @@
+"""Fused token embedding on MI355X: the lookup with its scaling, and the gradient
+of the table (no counterpart in the reference, whose models keep nn.Embedding).
+
+The gradient sums the tokens' rows in fp32 in an order that the ids alone decide,
+so that it is bit-reproducible, and rounds once.
+"""
+
+from __future__ import annotations
+
+import logging
+
+import torch
+import torch.nn as nn
+
+from metal_liger_amd import _custom_ops as cops
+
+logger = logging.getLogger(__name__)
+
+
+class _FusedEmbeddingFunction(torch.autograd.Function):
+    """scale * weight[ids]; saves the ids alone."""
+
+    @staticmethod
+    def forward(ctx, ids, weight, scale: float, padding_idx: int):
+        ctx.save_for_backward(ids)
+        ctx.scale, ctx.padding_idx = scale, padding_idx
+        ctx.vocab, ctx.dtype = weight.shape[0], weight.dtype
+        return cops.embedding_fwd(ids, weight, scale)
+
+    @staticmethod
+    def backward(ctx, dy):
+        ids, = ctx.saved_tensors
+        if dy.dtype != ctx.dtype:
+            dy = dy.to(ctx.dtype)
+        return None, cops.embedding_bwd(ids, dy, ctx.vocab, ctx.padding_idx, ctx.scale), None, None
+
+
+def fused_embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
+                    padding_idx: int | None = None) -> torch.Tensor:
+    """scale * weight[ids]: ids int64 or int32 of any shape, weight [vocab, hidden]
+    of fp32, bf16 or fp16; returns [*ids.shape, hidden] in weight's dtype.
+
+    padding_idx (negative: counted from the end): the row that gets no gradient.
+    An id outside the table gives a row of NaN and no gradient (nn.Embedding ends
+    the process there).
+    """
+    vocab = weight.shape[0]
+    if padding_idx is None:
+        padding_idx = -1
+    elif not -vocab <= padding_idx < vocab:
+        raise ValueError(f"embedding: padding_idx {padding_idx} outside a table of {vocab} rows")
+    else:
+        padding_idx %= vocab
+    return _FusedEmbeddingFunction.apply(ids, weight, float(scale), padding_idx)
+
+
+def _fusable(module: nn.Module) -> bool:
+    """An nn.Embedding as it is (a subclass may compute something else), without
+    the options that the fused op does not have."""
+    return (type(module) is nn.Embedding and module.max_norm is None and not module.sparse
+            and not module.scale_grad_by_freq)
+
+
+class MetalLigerEmbedding(nn.Module):
+    """Drop-in for an nn.Embedding, whose parameter it shares (state_dict keys and
+    tied weights are unchanged); `scale` multiplies the output."""
+
+    def __init__(self, original: nn.Embedding, scale: float = 1.0):
+        super().__init__()
+        if not _fusable(original):
+            raise ValueError("MetalLigerEmbedding: a plain nn.Embedding without max_norm, sparse or "
+                             f"scale_grad_by_freq is needed (got {original})")
+        self.weight = original.weight
+        self.num_embeddings, self.embedding_dim = original.weight.shape
+        self.padding_idx, self.scale = original.padding_idx, scale
+
+    def forward(self, ids: torch.Tensor) -> torch.Tensor:
+        return fused_embedding(ids, self.weight, self.scale, self.padding_idx)
+
+    def extra_repr(self) -> str:
+        return f"{self.num_embeddings}, {self.embedding_dim}, scale={self.scale}"
+
+
+class _FusedEmbeddingForward:
+    """Forward of a routed nn.Embedding."""
+
+    def __init__(self, module: nn.Embedding):
+        self.module = module
+
+    def __call__(self, ids):
+        return fused_embedding(ids, self.module.weight, padding_idx=self.module.padding_idx)
+
+
+def patch_embedding(model: nn.Module) -> int:
+    """Routes the model's token embeddings (plain nn.Embedding modules called
+    ``embed_tokens``, or inside a wrapper of that name as PEFT's modules_to_save
+    makes one) through the fused op and returns how many were routed. Only the
+    instances' ``forward`` changes; modules already routed are left as they are."""
+    routed = 0
+    for name, module in model.named_modules():
+        if "embed_tokens" not in name.split(".") or not _fusable(module):
+            continue
+        if getattr(module, "_metal_liger_fused_embedding", False):
+            continue
+        module.forward = _FusedEmbeddingForward(module)
+        module._metal_liger_fused_embedding = True
+        routed += 1
+    return routed

@@ -21,7 +21,7 @@ matrices (saved for the backward, where the reference recomputed it) and
 each output as one GEMM over [X | X A^T] x [W; s B]^T.
 
 Semantics kept from the reference (ops/fused_lora.py:43-421): PEFT parameter
-layout (first adapter only, dropout ignored), A/B cast to the activation
+layout (first adapter only, dropout ignored unless asked for), A/B cast to the activation
 dtype, dA/dB returned in fp32, no gradient for the frozen base weights, and
 the patcher shadows q/k/v_proj without replacing modules (state_dict keys
 unchanged). bf16 activations run the bf16 MFMA kernels above; fp32 (and,
@@ -38,6 +38,8 @@ import torch.nn as nn
 from metal_liger_amd import _custom_ops as cops
 from metal_liger_amd import hip_ops
 from metal_liger_amd._model_walk import find_layers, shadowed
+from metal_liger_amd.ops.fused_dropout import MetalLigerDropout, seed_tensor
+from metal_liger_amd.ops.fused_swiglu import fused_swiglu
 
 logger = logging.getLogger(__name__)
 
@@ -426,19 +428,146 @@ class _LoRA_W(torch.autograd.Function):
         return dX.view(*ctx.orig_shape), None, dA, dB, None
 
 
-def apply_fused_lora_linear(linear, X: torch.Tensor) -> torch.Tensor:
+# ------------------------------------------------------- dropout on X --
+# PEFT drops elements of the adapter's input, with a mask M_i of its own for each
+# projection, and scales the others by c_i = 1 / (1 - q_i):
+#   y_i  = X W_i^T + s_i XA_i B_i^T      XA_i = c_i (M_i X) A_i^T
+#   P_i  = c_i s_i dY_i B_i              dB_i = s_i dY_i^T XA_i
+#   dA_i = P_i^T (M_i X)                 dX   = sum_i dY_i W_i + M_i (P_i A_i)
+# c_i goes into the rank-r products, whose sums are fp32, so that the dropped X is X
+# or 0 and no element of it is rounded. Projection i of a block takes stream i of one
+# seed (ops/fused_dropout.py); the backward forms the masks again.
+
+class _LoRA_Dropout(torch.autograd.Function):
+    """Projections of one X whose adapters read it through dropout: `thresholds`
+    (round(65536 p), one per projection) and streams first .. of `seed`; params
+    W, A, B, S of each. Returns their outputs."""
+
+    @staticmethod
+    def forward(ctx, X, seed, thresholds, first: int, *params):
+        _check_float(X, "LoRA with dropout")
+        Ws, As, Bs = params[0::4], params[1::4], params[2::4]
+        scales = [float(s) for s in params[3::4]]
+        shape = X.shape
+        hip_ops.check_adapters([shape[-1]] * len(Ws), Ws, As, Bs)
+        fp32 = _fp32_path(X, shape[-1], *(W.shape[0] for W in Ws))
+        if fp32:
+            X2, rp = _rows_f32(X), 0
+            Ac, Bc, sB = [_f32(A) for A in As], [_f32(B) for B in Bs], \
+                [_f32(B) * s for B, s in zip(Bs, scales)]
+            Wc, kept = [_f32(W) for W in Ws], [t.detach() for t in (*Ws, *As, *Bs)]
+        else:
+            X2, rp = hip_ops._bf16_rows(X.reshape(-1, shape[-1])), _pad_rank(max(A.shape[0] for A in As))
+            flat, a_views, Bc, sB = _packed([shape[-1]] * len(Ws), Ws, As, Bs, scales, rp)
+            Ac, Wc = [_view(flat, v) for v in a_views], [hip_ops._bf16_rows(W.detach()) for W in Ws]
+            kept = [*Wc, flat]
+        outs, xas = [], []
+        for i, t in enumerate(thresholds):
+            xa = _product([cops.dropout(X2, None, seed, t, first + i, 1.0)], [Ac[i]], True,
+                          alpha=hip_ops.drop_scale(t))
+            outs.append(cops.gemm_f32([X2, xa], [Wc[i], sB[i]], False, True, 1.0) if fp32
+                        else cops.lora_linear_out(X2, Wc[i], xa, sB[i]))
+            xas.append(xa)
+        ctx.save_for_backward(X2, seed, *xas, *kept)
+        ctx.scales, ctx.thresholds, ctx.first = scales, thresholds, first
+        ctx.fp32, ctx.rank_p, ctx.orig_shape, ctx.x_dtype = fp32, rp, shape, X.dtype
+        ctx.outs = [W.shape[0] for W in Ws]
+        ctx.ranks = [A.shape[0] for A in As]
+        ctx.param_dtypes = [(A.dtype, B.dtype) for A, B in zip(As, Bs)]
+        return tuple(o.to(X.dtype).view(*shape[:-1], o.shape[-1]) for o in outs)
+
+    @staticmethod
+    def backward(ctx, *dYs):
+        X2, seed, *rest = ctx.saved_tensors
+        n, rp = len(ctx.scales), ctx.rank_p
+        xas, Ws, adapters = rest[:n], rest[n:2 * n], rest[2 * n:]
+        if ctx.fp32:
+            dys, Ws = [_rows_f32(d) for d in dYs], [_f32(W) for W in Ws]
+            As, Bs = [_f32(t) for t in adapters[:n]], [_f32(t) for t in adapters[n:]]
+        else:
+            dys = [hip_ops._bf16_rows(d.reshape(-1, d.shape[-1])) for d in dYs]
+            As, Bs = _unpack_views(adapters[0], X2.shape[1], ctx.outs, rp)
+        dX, grads = _product(dys, Ws, False), []
+        for i, t in enumerate(ctx.thresholds):
+            s, stream, r = ctx.scales[i], ctx.first + i, ctx.ranks[i]
+            P = _product([dys[i]], [Bs[i]], False, alpha=s * hip_ops.drop_scale(t))
+            dA = _product([P], [cops.dropout(X2, None, seed, t, stream, 1.0)], False, a_t=True,
+                          f32=True)
+            dB = _product([dys[i]], [xas[i]], False, a_t=True, f32=True, alpha=s)
+            dX = cops.dropout(_product([P], [As[i]], False), dX, seed, t, stream, 1.0)
+            ta, tb = ctx.param_dtypes[i]
+            grads += [None, dA[:r].to(ta), dB[:, :r].to(tb), None]
+        return (dX.to(ctx.x_dtype).view(*ctx.orig_shape), None, None, None, *grads)
+
+
+def _unpack_views(flat, in_f, outs, rp: int):
+    """The A_i [rp, in] and B_i [out_i, rp] of _packed's buffer."""
+    As = [_view(flat, (i * rp * in_f, rp, in_f)) for i in range(len(outs))]
+    off, Bs = len(outs) * rp * in_f, []
+    for o in outs:
+        Bs.append(_view(flat, (off, o, rp)))
+        off += o * rp
+    return As, Bs
+
+
+def _product(a_list, b_list, b_t: bool, a_t: bool = False, alpha: float = 1.0, f32: bool = False):
+    """alpha * sum_s op(a_s) op(b_s) in the operands' dtype (f32: in fp32)."""
+    if a_list[0].dtype == torch.float32:
+        return cops.gemm_f32(a_list, b_list, a_t, b_t, alpha)
+    out = None
+    for a, b in zip(a_list, b_list):
+        p = hip_ops.matmul(a, b, a_t=a_t, b_t=b_t, alpha=alpha)
+        out = p if out is None else out.add_(p)
+    return out if f32 else out.to(torch.bfloat16)
+
+
+def _drop_threshold(linear) -> int:
+    """The dropout threshold of a PEFT LoRA Linear's first adapter: 0 in eval mode,
+    where it has none (nn.Identity), and without the attribute."""
+    dropouts = getattr(linear, "lora_dropout", None)
+    if dropouts is None:
+        return 0
+    module = dropouts[list(linear.lora_A.keys())[0]]
+    if isinstance(module, nn.Identity) or not module.training:
+        return 0
+    if not isinstance(module, (nn.Dropout, MetalLigerDropout)):
+        raise TypeError(f"LoRA dropout: nn.Dropout or nn.Identity is needed (got {module})")
+    return hip_ops.drop_threshold(module.p)
+
+
+def _dropped(linears, X, seed, first: int = 0):
+    """The projections of X with their adapters' dropout, or None where none drops."""
+    thresholds = [_drop_threshold(m) for m in linears]
+    if not any(thresholds):
+        return None
+    hip_ops.ensure_rocm_device(X)
+    params = [t for m in linears for t in _get_lora_params(m)]
+    return _LoRA_Dropout.apply(X, seed_tensor(seed, X.device), tuple(thresholds), first, *params)
+
+
+def apply_fused_lora_linear(linear, X: torch.Tensor, lora_dropout: bool = False,
+                            seed=None) -> torch.Tensor:
     """One LoRA projection (e.g. o_proj) through _LoRA_W; the module's own
-    forward when it has no LoRA adapter."""
+    forward when it has no LoRA adapter. lora_dropout, seed: as in
+    apply_fused_lora_qkv."""
     W, A, B, S = _get_lora_params(linear)
     if A is None:
         return linear(X)
+    if lora_dropout:
+        out = _dropped([linear], X, seed)
+        if out is not None:
+            return out[0]
     return _LoRA_W.apply(X, W, A, B, S)
 
 
-def apply_fused_lora_qkv(attn_module, X: torch.Tensor):
+def apply_fused_lora_qkv(attn_module, X: torch.Tensor, lora_dropout: bool = False, seed=None):
     """Fused Q+K+V LoRA projections of an attention module
     (ops/fused_lora.py:269-295); plain module calls when any projection has
-    no LoRA adapter."""
+    no LoRA adapter.
+
+    lora_dropout: the adapters read X through their own lora_dropout modules (in
+    training mode), which the reference ignores; projection i on stream i of one
+    seed (ops/fused_dropout.py), given or drawn at each call."""
     QW, QA, QB, QS = _get_lora_params(attn_module.q_proj)
     KW, KA, KB, KS = _get_lora_params(attn_module.k_proj)
     VW, VA, VB, VS = _get_lora_params(attn_module.v_proj)
@@ -449,6 +578,10 @@ def apply_fused_lora_qkv(attn_module, X: torch.Tensor):
         V = attn_module.v_proj(X)
         return Q, K, V
 
+    if lora_dropout:
+        outs = _dropped([attn_module.q_proj, attn_module.k_proj, attn_module.v_proj], X, seed)
+        if outs is not None:
+            return outs
     return _LoRA_QKV.apply(
         X,
         QW, QA, QB, QS,
@@ -457,9 +590,13 @@ def apply_fused_lora_qkv(attn_module, X: torch.Tensor):
     )
 
 
-def apply_fused_lora_mlp(mlp_module, X: torch.Tensor) -> torch.Tensor:
+def apply_fused_lora_mlp(mlp_module, X: torch.Tensor, lora_dropout: bool = False,
+                         seed=None) -> torch.Tensor:
     """Fused gate+up+down LoRA MLP (ops/fused_lora.py:298-320); the module's
-    own forward when any projection has no LoRA adapter."""
+    own forward when any projection has no LoRA adapter.
+
+    lora_dropout, seed: as in apply_fused_lora_qkv (streams 0, 1, 2 for gate, up,
+    down); the block is then gate and up together, SwiGLU, and down."""
     GW, GA, GB, GS = _get_lora_params(mlp_module.gate_proj)
     UW, UA, UB, US = _get_lora_params(mlp_module.up_proj)
     DW, DA, DB, DS = _get_lora_params(mlp_module.down_proj)
@@ -467,6 +604,15 @@ def apply_fused_lora_mlp(mlp_module, X: torch.Tensor) -> torch.Tensor:
     if GA is None or UA is None or DA is None:
         return mlp_module(X)
 
+    projections = [mlp_module.gate_proj, mlp_module.up_proj, mlp_module.down_proj]
+    if lora_dropout and any(_drop_threshold(m) for m in projections):
+        hip_ops.ensure_rocm_device(X)
+        seed = seed_tensor(seed, X.device)
+        gate, up = _dropped(projections[:2], X, seed) or (
+            apply_fused_lora_linear(m, X) for m in projections[:2])
+        h = fused_swiglu(gate, up)
+        down = _dropped(projections[2:], h, seed, first=2)
+        return down[0] if down is not None else _LoRA_W.apply(h, DW, DA, DB, DS)
     return _LoRA_MLP.apply(
         X,
         GW, GA, GB, GS,
@@ -503,18 +649,19 @@ class _FusedAttentionForward:
     results (o_proj by _LoRA_W when it carries LoRA too, which the
     reference's patcher leaves to PEFT)."""
 
-    def __init__(self, attn: nn.Module, original):
+    def __init__(self, attn: nn.Module, original, lora_dropout: bool = False):
         self.attn = attn
         self.original = original
+        self.lora_dropout = lora_dropout
         o_proj = getattr(attn, "o_proj", None)
         self.o_proj = o_proj if _all_lora(attn, ("o_proj",)) else None
 
     def __call__(self, hidden_states, *args, **kwargs):
-        q, k, v = apply_fused_lora_qkv(self.attn, hidden_states)
+        q, k, v = apply_fused_lora_qkv(self.attn, hidden_states, self.lora_dropout)
         subs = dict(zip(_QKV_PROJ, (_Returns(q), _Returns(k), _Returns(v))))
         if self.o_proj is not None:
             o_proj = self.o_proj
-            subs["o_proj"] = lambda x: apply_fused_lora_linear(o_proj, x)
+            subs["o_proj"] = lambda x: apply_fused_lora_linear(o_proj, x, self.lora_dropout)
         with shadowed(self.attn, **subs):
             return self.original(hidden_states, *args, **kwargs)
 
@@ -523,14 +670,15 @@ class _FusedMLPForward:
     """Forward of an MLP whose gate/up/down projections all carry LoRA: the
     whole block is one _LoRA_MLP call."""
 
-    def __init__(self, mlp: nn.Module):
+    def __init__(self, mlp: nn.Module, lora_dropout: bool = False):
         self.mlp = mlp
+        self.lora_dropout = lora_dropout
 
     def __call__(self, x):
-        return apply_fused_lora_mlp(self.mlp, x)
+        return apply_fused_lora_mlp(self.mlp, x, self.lora_dropout)
 
 
-def patch_fused_lora(model: nn.Module) -> int:
+def patch_fused_lora(model: nn.Module, lora_dropout: bool = False) -> int:
     """Routes every decoder layer's attention and MLP whose three
     projections all carry LoRA through _LoRA_QKV / _LoRA_MLP and returns how
     many modules were routed (ops/fused_lora.py:323-421).
@@ -540,15 +688,20 @@ def patch_fused_lora(model: nn.Module) -> int:
     state_dict keys and checkpoints are unaffected. The decoder layers are
     found as the model patcher finds them (PEFT's base_model.model, a bare
     HF model or decoder, Qwen3-VL's language_model); modules already routed
-    are left as they are, so a second call returns 0."""
+    are left as they are, so a second call returns 0.
+
+    lora_dropout: in training mode the adapters read their input through their
+    lora_dropout modules, as PEFT's own forward does (the reference ignores it)."""
     layers = find_layers(model)
     if layers is None:
         logger.warning("MetalLiger fused LoRA: could not find transformer layers")
         return 0
     routed = 0
     for layer in layers:
-        for attr, names, make in (("self_attn", _QKV_PROJ, lambda m: _FusedAttentionForward(m, m.forward)),
-                                  ("mlp", _MLP_PROJ, _FusedMLPForward)):
+        for attr, names, make in (
+                ("self_attn", _QKV_PROJ,
+                 lambda m: _FusedAttentionForward(m, m.forward, lora_dropout)),
+                ("mlp", _MLP_PROJ, lambda m: _FusedMLPForward(m, lora_dropout))):
             mod = getattr(layer, attr, None)
             if mod is None or getattr(mod, "_metal_liger_fused_lora", False):
                 continue

@@ -16,6 +16,7 @@ import torch.nn as nn
 
 from metal_liger_amd._model_walk import find_final_norm, find_layers
 from metal_liger_amd.ops.fused_add_rms_norm import patch_residual_add_norm
+from metal_liger_amd.ops.fused_embedding import patch_embedding
 from metal_liger_amd.ops.fused_linear_cross_entropy import patch_causal_lm_loss
 from metal_liger_amd.ops.fused_lora import patch_fused_lora
 from metal_liger_amd.ops.fused_qk_norm_rope import patch_qk_norm_rope
@@ -82,6 +83,8 @@ def apply_metal_liger_to_qwen3vl(
     fuse_qk_norm_rope: bool = False,
     fuse_lm_loss: bool = False,
     efficient_attention: bool = False,
+    lora_dropout: bool = False,
+    fuse_embedding: bool = False,
 ) -> nn.Module:
     """Apply the fused operations to a Qwen3 / Qwen3-VL model in place and
     return it (patch.py:181-240).
@@ -106,6 +109,11 @@ def apply_metal_liger_to_qwen3vl(
     "sdpa" implementation run SDPA's memory-efficient kernel over repeated
     key / value heads instead of the flash kernel with GQA
     (ops/gqa_attention.py).
+    lora_dropout: with fuse_lora, the adapters' lora_dropout is applied in
+    training mode, as PEFT applies it and the reference does not
+    (ops/fused_lora.py, ops/fused_dropout.py).
+    fuse_embedding: the token embedding and the gradient of its table
+    (ops/fused_embedding.py).
     use_optimized_generator is not part of metal_liger_amd (inference path).
     """
     stats = {}
@@ -127,13 +135,17 @@ def apply_metal_liger_to_qwen3vl(
         stats["qk_norm_rope"] = n
         logger.info(f"MetalLiger: fused q/k norm + RoPE on {n} attention modules")
     if fuse_lora:
-        n = patch_fused_lora(model)
+        n = patch_fused_lora(model, lora_dropout)
         stats["fused_lora"] = n
         logger.info(f"MetalLiger: fused LoRA QKV+MLP marked {n} modules")
     if fuse_lm_loss:
         n = patch_causal_lm_loss(model)
         stats["lm_loss"] = n
         logger.info(f"MetalLiger: fused linear cross-entropy loss on {n} causal LM heads")
+    if fuse_embedding:
+        n = patch_embedding(model)
+        stats["embedding"] = n
+        logger.info(f"MetalLiger: fused {n} token embeddings")
     if efficient_attention:
         n = patch_efficient_attention(model)
         stats["efficient_attention"] = n
