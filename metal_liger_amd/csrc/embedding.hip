@@ -11,7 +11,7 @@
 // The gradient of a table of 151936 rows is mostly zeros (622 MB of bf16 at 2048
 // columns, of which 8192 tokens name 33 MB at most), so that its fill is the bound
 // and everything else is kept beside it:
-//   sort   tiles of 8192 tokens, one workgroup each, by (id, position), while the
+//   sort   tiles of up to 16384 tokens, one workgroup each, by (id, position), while the
 //          other workgroups of the launch fill dW with zeros;
 //   merge  up to 8 sorted runs at a time (none for one tile);
 //   sum    chunks of the sorted order: a run of equal ids inside a chunk is summed
@@ -68,20 +68,47 @@ __global__ __launch_bounds__(kThreads) void embedding_rows(const void* ids, bool
 }
 
 // -------------------------------------------------------------------- sort --
-// One workgroup sorts a tile by a radix sort of 6-bit digits in LDS: wave w holds
-// elements 512 w .. of the current order, 64 at a time; a lane's rank within its
-// digit is the number of lanes below it that share the digit (six ballots) plus
-// the wave's count of the digit so far, and a scan over (digit, wave) places them.
-constexpr int kTile = 8192, kSortThreads = 1024, kWaves = kSortThreads / 64;
-constexpr int kItems = kTile / kSortThreads, kDigitBits = 6, kDigits = 1 << kDigitBits;
+// One workgroup sorts a tile by a radix sort of 6-bit digits between two buffers of
+// LDS, an entry being one word: the id above the position in the tile. Wave w holds
+// the w-th part of the current order, 64 entries at a time. A lane's entry goes to
+// the number of entries with smaller digits, plus those of the same digit in earlier
+// waves (a scan over (digit, wave) of what each wave counted), in the wave's earlier
+// rounds and in lower lanes; lanes that share a digit find each other by six ballots.
+// (Entries, ranks and predicates held in registers spilled 452 bytes a lane and took
+// 95 us for 8192 ids.)
+constexpr int kSortThreads = 1024, kWaves = kSortThreads / 64;
+constexpr int kDigitBits = 6, kDigits = 1 << kDigitBits;
 static_assert(kWaves * kDigits == kSortThreads, "a counter per thread");
 
+// Ids below 2^18 go in 32 bits beside 14 bits of position, others in 64 beside 13.
+template <typename W>
+constexpr int pos_bits() { return sizeof(W) == 4 ? 14 : 13; }
+template <typename W>
+constexpr int tile_of() { return 1 << pos_bits<W>(); }
+constexpr int64_t kNarrowVocab = (1 << 18) - 1;  // the key of "no gradient" is the vocabulary
+
+// The lanes (of those that are `in`) whose digit is this lane's.
+__device__ __forceinline__ uint64_t same_digit(uint32_t d, bool in) {
+  uint64_t same = __ballot(in);
+#pragma unroll
+  for (int b = 0; b < kDigitBits; ++b) {
+    const bool bit = (d >> b) & 1;
+    const uint64_t has = __ballot(bit);
+    same &= bit ? has : ~has;
+  }
+  return same;
+}
+
+// Zeros, by one wave in each of `blocks` workgroups. One wave per CU keeps what is
+// being written within 256 KB: 622 MB take 96 us beside the sort, and 85 in a launch
+// of 64-thread workgroups of their own, which would wait for the sort instead; with
+// 512 to 2048 threads per CU, 105 to 140.
 __device__ __forceinline__ void fill_zero(char* p, int64_t bytes, int64_t block, int64_t blocks) {
+  if (threadIdx.x >= 64) return;
   const int64_t head = std::min<int64_t>(bytes, (16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15);
   const int64_t vecs = (bytes - head) / 16, tail = head + vecs * 16;
   u32x4_t* v = reinterpret_cast<u32x4_t*>(p + head);
-  const int64_t stride = blocks * kSortThreads;
-  for (int64_t i = block * kSortThreads + threadIdx.x; i < vecs; i += stride)
+  for (int64_t i = block * 64 + threadIdx.x; i < vecs; i += blocks * 64)
     __builtin_nontemporal_store(u32x4_t{0, 0, 0, 0}, v + i);
   if (block == 0 && threadIdx.x < 16) {
     if (threadIdx.x < head) p[threadIdx.x] = 0;
@@ -89,6 +116,7 @@ __device__ __forceinline__ void fill_zero(char* p, int64_t bytes, int64_t block,
   }
 }
 
+template <typename W>
 __global__ __launch_bounds__(kSortThreads) void sort_tiles(const void* ids, bool wide, int64_t N,
                                                            int tiles, int64_t V, int64_t skip,
                                                            int passes, uint64_t* sorted, char* dW,
@@ -97,43 +125,33 @@ __global__ __launch_bounds__(kSortThreads) void sort_tiles(const void* ids, bool
     fill_zero(dW, bytes, blockIdx.x - tiles, gridDim.x - tiles);
     return;
   }
-  __shared__ uint32_t keys[kTile];
-  __shared__ uint16_t from[kTile];
+  constexpr int kTile = tile_of<W>(), kPos = pos_bits<W>();
+  __shared__ W buf[2][kTile];
   __shared__ uint32_t count[kDigits * kWaves];  // [digit][wave]
-  __shared__ uint32_t wave_sum_[kWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ uint32_t totals[kWaves];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int64_t first = (int64_t)blockIdx.x * kTile;
-  const int64_t below = (1ULL << lane) - 1;
-  uint32_t key[kItems], pos[kItems], rank[kItems];
-#pragma unroll
-  for (int r = 0; r < kItems; ++r) {
-    pos[r] = wave * (kItems * 64) + r * 64 + lane;
-    const int64_t n = first + pos[r];
-    key[r] = 0xFFFFFFFFu;  // past the end: after every key of the tile
-    if (n < N) {
-      const int64_t id = id_at(ids, n, wide);
-      key[r] = id >= 0 && id < V && id != skip ? (uint32_t)id : (uint32_t)V;  // no gradient: last
-    }
+  const int size = (int)std::min<int64_t>(kTile, N - first);
+  const int part = (size + kSortThreads - 1) / kSortThreads * 64;  // entries per wave
+  const int begin = wave * part, end = std::min(begin + part, size);
+  const uint64_t below = (1ULL << lane) - 1;
+  for (int i = tid; i < size; i += kSortThreads) {
+    const int64_t id = id_at(ids, first + i, wide);
+    const bool ok = id >= 0 && id < V && id != skip;
+    buf[0][i] = (W)(ok ? id : V) << kPos | (W)i;  // no gradient: after all others
   }
+  W *src = buf[0], *dst = buf[1];
   for (int p = 0; p < passes; ++p) {
-    const int shift = p * kDigitBits;
+    const int shift = kPos + p * kDigitBits;
     count[tid] = 0;
     __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kItems; ++r) {
-      const uint32_t d = (key[r] >> shift) & (kDigits - 1);
-      uint64_t same = ~0ULL;
-#pragma unroll
-      for (int b = 0; b < kDigitBits; ++b) {
-        const bool bit = (d >> b) & 1;
-        const uint64_t has = __ballot(bit);
-        same &= bit ? has : ~has;
-      }
+    for (int i = begin; i < end; i += 64) {
+      const bool in = i + lane < end;
+      const uint32_t d = in ? (uint32_t)(src[i + lane] >> shift) & (kDigits - 1) : 0;
+      const uint64_t same = same_digit(d, in);
       volatile uint32_t* c = count + d * kWaves + wave;  // this wave's own, in order
-      const uint32_t before = *c;
-      rank[r] = before + __popcll(same & below);
-      if ((same & below) == 0) *c = before + __popcll(same);
-      __builtin_amdgcn_wave_barrier();
+      if (in && (same & below) == 0) *c = *c + __popcll(same);
     }
     __syncthreads();
     // exclusive scan of the counters in (digit, wave) order, one per thread
@@ -144,31 +162,33 @@ __global__ __launch_bounds__(kSortThreads) void sort_tiles(const void* ids, bool
       const uint32_t up = __shfl_up(sum, off, 64);
       if (lane >= off) sum += up;
     }
-    if (lane == 63) wave_sum_[wave] = sum;
+    if (lane == 63) totals[wave] = sum;
     __syncthreads();
-    uint32_t base = 0;
-    for (int w = 0; w < wave; ++w) base += wave_sum_[w];
-    count[tid] = base + sum - own;
-    __syncthreads();
+    sum -= own;
 #pragma unroll
-    for (int r = 0; r < kItems; ++r) {
-      const uint32_t at = count[((key[r] >> shift) & (kDigits - 1)) * kWaves + wave] + rank[r];
-      keys[at] = key[r];
-      from[at] = (uint16_t)pos[r];
+    for (int w = 0; w < kWaves; ++w) sum += w < wave ? totals[w] : 0;
+    count[tid] = sum;
+    __syncthreads();
+    for (int i = begin; i < end; i += 64) {
+      const bool in = i + lane < end;
+      const W e = in ? src[i + lane] : 0;
+      const uint32_t d = (uint32_t)(e >> shift) & (kDigits - 1);
+      const uint64_t same = same_digit(d, in);
+      volatile uint32_t* c = count + d * kWaves + wave;
+      const uint32_t before = *c;
+      if (in) {
+        if ((same & below) == 0) *c = before + __popcll(same);
+        dst[before + __popcll(same & below)] = e;
+      }
     }
     __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kItems; ++r) {
-      const int i = wave * (kItems * 64) + r * 64 + lane;
-      key[r] = keys[i];
-      pos[r] = from[i];
-    }
-    __syncthreads();
+    W* const done = dst;
+    dst = src;
+    src = done;
   }
-#pragma unroll
-  for (int r = 0; r < kItems; ++r) {
-    const int64_t n = first + wave * (kItems * 64) + r * 64 + lane;
-    if (n < N) sorted[n] = (uint64_t)key[r] << 32 | (uint64_t)(first + pos[r]);
+  for (int i = tid; i < size; i += kSortThreads) {
+    const W e = src[i];
+    sorted[first + i] = (uint64_t)(e >> kPos) << 32 | (uint64_t)(first + (e & (kTile - 1)));
   }
 }
 
@@ -217,10 +237,12 @@ __device__ __forceinline__ uint32_t key_of(uint64_t e) { return (uint32_t)(e >> 
 // the chunk holds of a run that began before it; [1]: of a run that begins in it and
 // goes on after it.
 template <typename T, int VEC>
-__global__ __launch_bounds__(kThreads) void sum_chunks(const uint64_t* sorted, int64_t N, int chunk,
-                                                       const T* dy, int64_t ldy, T* dW, int64_t V,
-                                                       int64_t H, float* parts, float scale) {
-  constexpr int U = 8;  // rows in flight
+__global__ __launch_bounds__(kThreads) void sum_chunks(const uint64_t* __restrict__ sorted,
+                                                       int64_t N, int chunk,
+                                                       const T* __restrict__ dy, int64_t ldy,
+                                                       T* __restrict__ dW, int64_t V, int64_t H,
+                                                       float* __restrict__ parts, float scale) {
+  constexpr int U = 16;  // rows in flight: the shortest chunk
   const int64_t s = (int64_t)blockIdx.x * chunk, e = std::min<int64_t>(s + chunk, N);
   const int64_t c = ((int64_t)blockIdx.y * kThreads + threadIdx.x) * VEC;
   const bool live = c < H;
@@ -249,13 +271,14 @@ __global__ __launch_bounds__(kThreads) void sum_chunks(const uint64_t* sorted, i
   };
   for (int64_t i = s; i < e; i += U) {
     uint64_t en[U];
-    float x[U][VEC];
+    Pack<T, VEC> x[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) en[u] = sorted[i + u < e ? i + u : e - 1];
     if (key_of(en[0]) >= V) break;  // no gradient from here on
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      load_n<T, VEC>(dy + (int64_t)(uint32_t)en[u] * ldy + (live ? c : 0), x[u]);
+      x[u] = *reinterpret_cast<const Pack<T, VEC>*>(dy + (int64_t)(uint32_t)en[u] * ldy +
+                                                    (live ? c : 0));
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (i + u < e) {
@@ -268,7 +291,7 @@ __global__ __launch_bounds__(kThreads) void sum_chunks(const uint64_t* sorted, i
           for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
         }
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] += x[u][j];
+        for (int j = 0; j < VEC; ++j) acc[j] += to_f32(x[u].v[j]);
       }
     }
   }
@@ -279,80 +302,151 @@ __global__ __launch_bounds__(kThreads) void sum_chunks(const uint64_t* sorted, i
     finish();
 }
 
-// The runs that cross chunks: the workgroup of the chunk in which a run begins adds
-// the partials of the chunks it covers. kJoin groups of lanes take every kJoin-th
-// chunk and meet in LDS in a fixed order.
-constexpr int kJoin = 8, kJoinCols = 32;  // 4 columns a lane: 128 a workgroup
+// The runs that cross chunks: their partials added in the chunks' order. Every workgroup lists the chunks in which such a run begins (a thread a
+// chunk) and takes its share of the (run, column slice) items: a wave sums a run of a
+// few chunks, 256 columns at a time; a long one (an image's or a padding token) takes
+// the workgroup, 64 columns at a time, whose waves add every 16th chunk and meet in LDS
+// in a fixed order.
+// (A workgroup for every chunk and slice took 39 us where a run covers 700 chunks of
+// 16384 tokens and 7.5 us where it had next to nothing to do.)
+constexpr int kJoinThreads = 1024, kJoinWaves = kJoinThreads / 64, kShortCols = 4;
+constexpr int kMaxChunks = kJoinThreads, kLongRun = 16;
 
-__device__ __forceinline__ void add4(float (&s)[4], const float* p, int64_t c, int64_t H,
-                                     bool vec) {
-  if (vec) {
-    float x[4];
-    load_n<float, 4>(p, x);
+// Adds the partials k, k + step .. up to `last`, U loads in flight (those past the
+// last read it again and add nothing: a loop over what is left would wait for each).
+template <int U>
+__device__ __forceinline__ void add_parts(float& sum, const float* __restrict__ p, int k, int step,
+                                          int last, int64_t H) {
+  for (; k <= last; k += U * step) {
+    float x[U];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] += x[j];
-  } else {
+    for (int u = 0; u < U; ++u) {
+      const int at = k + u * step;
+      x[u] = p[(int64_t)(at < last ? at : last) * 2 * H];
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c + j < H) s[j] += p[j];
+    for (int u = 0; u < U; ++u) sum += k + u * step <= last ? x[u] : 0.f;
   }
 }
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void join_chunks(const uint64_t* sorted, int64_t N, int chunk,
-                                                        int chunks, T* dW, int64_t V, int64_t H,
-                                                        const float* parts, float scale) {
-  __shared__ float met[kJoin][kJoinCols * 4];
-  const int b = blockIdx.x;
-  const int64_t s = (int64_t)b * chunk, e = s + chunk;
-  if (e >= N) return;
-  const uint32_t key = key_of(sorted[e]);
-  if (key >= V || key_of(sorted[e - 1]) != key) return;
-  if (s > 0 && key_of(sorted[s - 1]) == key) return;  // it began earlier
-  int span = 0;  // chunks after this one that it reaches
-  for (;;) {
-    const int64_t at = (int64_t)(b + 1 + span + threadIdx.x) * chunk;
-    const int n = __syncthreads_count(at < N && key_of(sorted[at]) == key);
-    span += n;
-    if (n < kThreads) break;
+__global__ __launch_bounds__(kJoinThreads) void join_chunks(const uint64_t* __restrict__ sorted,
+                                                            int64_t N, int chunk, int chunks,
+                                                            T* __restrict__ dW, int64_t V,
+                                                            int64_t H,
+                                                            const float* __restrict__ parts,
+                                                            float scale) {
+  __shared__ uint32_t first[kMaxChunks + 1];  // a chunk's first key
+  __shared__ uint32_t list[2][kMaxChunks];    // chunks in which short / long runs begin
+  __shared__ uint16_t spans[kMaxChunks];      // how many chunks more the run reaches
+  __shared__ int counts[2][kJoinWaves];
+  __shared__ float met[kJoinWaves][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t s = (int64_t)tid * chunk, e = s + chunk;
+  uint32_t before = 0xFFFFFFFFu, last = 0xFFFFFFFFu;
+  first[tid] = 0xFFFFFFFFu;
+  if (tid < chunks) {
+    first[tid] = key_of(sorted[s]);
+    if (tid > 0) before = key_of(sorted[s - 1]);
+    if (e < N) last = key_of(sorted[e - 1]);
   }
-  const int g = threadIdx.x / kJoinCols, l = threadIdx.x % kJoinCols;
-  const int64_t c = ((int64_t)blockIdx.y * kJoinCols + l) * 4;
-  const bool vec = H % 4 == 0;
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
-  if (c < H) {
-    if (g == 0) add4(sum, parts + ((int64_t)b * 2 + 1) * H + c, c, H, vec);
-#pragma unroll 8
-    for (int k = g; k < span; k += kJoin)
-      add4(sum, parts + (int64_t)(b + 1 + k) * 2 * H + c, c, H, vec);
-  }
-#pragma unroll
-  for (int j = 0; j < 4; ++j) met[g][l * 4 + j] = sum[j];
+  if (tid == 0) first[kMaxChunks] = 0xFFFFFFFFu;
   __syncthreads();
-  const int col = threadIdx.x;
-  const int64_t oc = (int64_t)blockIdx.y * kJoinCols * 4 + col;
-  if (col < kJoinCols * 4 && oc < H) {
-    float t = 0.f;
+  // a run goes on after this chunk, and did not come into it
+  const bool owner =
+      last < V && first[tid + 1] == last && !(first[tid] == last && before == last);
+  int span = 0;
+  if (owner) {
+    int lo = tid + 1, hi = chunks;  // the first chunk after it that begins with another key
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (first[mid] == last)
+        lo = mid + 1;
+      else
+        hi = mid;
+    }
+    span = lo - tid - 1;
+    spans[tid] = (uint16_t)span;
+  }
+  // every workgroup makes the same lists, in the chunks' order
+  const uint64_t has[2] = {__ballot(owner && span <= kLongRun), __ballot(owner && span > kLongRun)};
+  if (lane < 2) counts[lane][wave] = __popcll(lane == 0 ? has[0] : has[1]);
+  __syncthreads();
+  int found[2] = {0, 0}, at[2] = {0, 0};
 #pragma unroll
-    for (int k = 0; k < kJoin; ++k) t += met[k][col];
-    dW[(int64_t)key * H + oc] = from_f32<T>(t * scale);
+  for (int k = 0; k < 2; ++k)
+    for (int w = 0; w < kJoinWaves; ++w) {
+      if (w == wave) at[k] = found[k];
+      found[k] += counts[k][w];
+    }
+  if (owner) {
+    const int k = span > kLongRun;
+    const uint64_t mine = k ? has[1] : has[0];
+    list[k][(k ? at[1] : at[0]) + __popcll(mine & ((1ULL << lane) - 1))] = tid;
+  }
+  __syncthreads();
+  const int wide = (int)((H + 64 * kShortCols - 1) / (64 * kShortCols));
+  const int shorts = found[0] * wide;
+  for (int i = blockIdx.x * kJoinWaves + wave; i < shorts; i += gridDim.x * kJoinWaves) {
+    const int b = list[0][i / wide], span = spans[b];
+    const float* p = parts + (int64_t)b * 2 * H;
+    int64_t c[kShortCols];
+    float sum[kShortCols];
+#pragma unroll
+    for (int j = 0; j < kShortCols; ++j) {
+      c[j] = (int64_t)(i % wide * kShortCols + j) * 64 + lane;
+      sum[j] = p[H + (c[j] < H ? c[j] : 0)];
+    }
+    for (int k = 1; k <= span; k += 2) {  // two chunks of every column in flight
+      float x[2][kShortCols];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int j = 0; j < kShortCols; ++j)
+          x[u][j] = p[(int64_t)(k + u < span ? k + u : span) * 2 * H + (c[j] < H ? c[j] : 0)];
+#pragma unroll
+      for (int j = 0; j < kShortCols; ++j) sum[j] += x[0][j] + (k < span ? x[1][j] : 0.f);
+    }
+#pragma unroll
+    for (int j = 0; j < kShortCols; ++j)
+      if (c[j] < H) dW[(int64_t)first[b + 1] * H + c[j]] = from_f32<T>(sum[j] * scale);
+  }
+  const int narrow = (int)((H + 63) / 64), longs = found[1] * narrow;
+  for (int i = blockIdx.x; i < longs; i += gridDim.x) {
+    const int b = list[1][i / narrow], span = spans[b];
+    const int64_t c = (int64_t)(i % narrow) * 64 + lane;
+    float sum = 0.f;
+    if (c < H) {
+      if (wave == 0) sum = parts[((int64_t)b * 2 + 1) * H + c];
+      add_parts<16>(sum, parts + (int64_t)b * 2 * H + c, 1 + wave, kJoinWaves, span, H);
+    }
+    __syncthreads();  // the previous item's sums have been read
+    met[wave][lane] = sum;
+    __syncthreads();
+    if (wave == 0 && c < H) {
+      float total = 0.f;
+#pragma unroll
+      for (int w = 0; w < kJoinWaves; ++w) total += met[w][lane];
+      dW[(int64_t)first[b + 1] * H + c] = from_f32<T>(total * scale);
+    }
   }
 }
 
 struct Plan {
-  int tiles, chunk, chunks, merges;
+  int tile, tiles, chunk, chunks, merges;
   size_t entries, parts;  // bytes of one copy of the sorted entries, and of the partials
 };
 
 size_t align256(size_t b) { return (b + 255) / 256 * 256; }
 
 // Chunks of 16 tokens until they are 1024, then longer ones: enough workgroups to
-// fill the GPU and few enough partials to join.
-Plan plan_of(int64_t n, int64_t hidden) {
+// fill the GPU, and a thread for each in the join.
+Plan plan_of(int64_t n, int64_t vocab, int64_t hidden) {
   Plan p{};
-  p.tiles = (int)((n + kTile - 1) / kTile);
-  for (int64_t run = kTile; run < n; run *= kWay) ++p.merges;
-  p.chunk = (int)std::max<int64_t>(16, (n + 1023) / 1024);
+  p.tile = vocab <= kNarrowVocab ? tile_of<uint32_t>() : tile_of<uint64_t>();
+  p.tiles = (int)((n + p.tile - 1) / p.tile);
+  for (int64_t run = p.tile; run < n; run *= kWay) ++p.merges;
+  p.chunk = (int)std::max<int64_t>(16, (n + kMaxChunks - 1) / kMaxChunks);
   p.chunks = (int)((n + p.chunk - 1) / p.chunk);
   p.entries = align256((size_t)n * 8);
   p.parts = align256((size_t)p.chunks * 2 * hidden * 4);
@@ -409,7 +503,7 @@ extern "C" int ml_embedding_fwd(const void* ids, int id_bytes, int64_t n, const 
 
 extern "C" size_t ml_embedding_bwd_workspace_bytes(int64_t n, int64_t vocab, int64_t hidden) {
   if (n <= 0 || vocab <= 0 || hidden <= 0 || n >= (1LL << 31) || hidden >= (1LL << 22)) return 0;
-  return bytes_of(plan_of(n, hidden));
+  return bytes_of(plan_of(n, vocab, hidden));
 }
 
 extern "C" int ml_embedding_bwd(const void* ids, int id_bytes, int64_t n, const void* dy,
@@ -421,7 +515,7 @@ extern "C" int ml_embedding_bwd(const void* ids, int id_bytes, int64_t n, const 
   ML_CHECK(padding_idx >= -1 && padding_idx < vocab, "embedding backward: bad padding index %lld",
            (long long)padding_idx);
   ML_CHECK(dweight && ((ids && dy) || n == 0), "embedding backward: null pointer");
-  const Plan p = plan_of(n, hidden);
+  const Plan p = plan_of(n, vocab, hidden);
   ML_CHECK(n == 0 || (workspace && aligned16(workspace) && workspace_bytes >= bytes_of(p)),
            "embedding backward: workspace too small or misaligned (%zu < %zu)", workspace_bytes,
            bytes_of(p));
@@ -431,20 +525,28 @@ extern "C" int ml_embedding_bwd(const void* ids, int id_bytes, int64_t n, const 
     constexpr int VEC = vec16<T>();
     T* dw = static_cast<T*>(dweight);
     const int64_t bytes = vocab * hidden * (int64_t)sizeof(T);
-    const int64_t per_block = (int64_t)kSortThreads * 16 * 4;
-    const int64_t fill = std::min<int64_t>((bytes + per_block - 1) / per_block, num_cus() * 8);
+    // one workgroup of this launch fits a CU (its LDS): those that fill leave room for
+    // those that sort, so that none starts late
+    const int64_t fill = std::min<int64_t>((bytes + 1023) / 1024,
+                                           std::max(num_cus() - p.tiles, num_cus() / 4));
     int passes = 0;
     while (passes * kDigitBits < 32 && (vocab >> (passes * kDigitBits)) > 0) ++passes;
     char* ws = static_cast<char*>(workspace);
     uint64_t* a = reinterpret_cast<uint64_t*>(ws);
     uint64_t* b = reinterpret_cast<uint64_t*>(ws + p.entries);
     float* parts = reinterpret_cast<float*>(ws + p.entries * (p.merges ? 2 : 1));
-    sort_tiles<<<dim3((unsigned)(p.tiles + fill)), kSortThreads, 0, st>>>(
-        ids, id_bytes == 8, n, p.tiles, vocab, padding_idx, passes, a,
-        static_cast<char*>(dweight), bytes);
+    const dim3 sg((unsigned)(p.tiles + fill));
+    if (vocab <= kNarrowVocab)
+      sort_tiles<uint32_t><<<sg, kSortThreads, 0, st>>>(ids, id_bytes == 8, n, p.tiles, vocab,
+                                                        padding_idx, passes, a,
+                                                        static_cast<char*>(dweight), bytes);
+    else
+      sort_tiles<uint64_t><<<sg, kSortThreads, 0, st>>>(ids, id_bytes == 8, n, p.tiles, vocab,
+                                                        padding_idx, passes, a,
+                                                        static_cast<char*>(dweight), bytes);
     ML_LAUNCH_CHECK();
     if (n == 0) return ML_OK;
-    int64_t run = kTile;
+    int64_t run = p.tile;
     for (int k = 0; k < p.merges; ++k, run *= kWay) {
       merge_runs<<<dim3((unsigned)((n + kThreads - 1) / kThreads)), kThreads, 0, st>>>(a, b, n,
                                                                                       run);
@@ -463,10 +565,8 @@ extern "C" int ml_embedding_bwd(const void* ids, int id_bytes, int64_t n, const 
                                                   scale);
     ML_LAUNCH_CHECK();
     if (p.chunks > 1) {
-      const dim3 jg((unsigned)p.chunks,
-                    (unsigned)((hidden + kJoinCols * 4 - 1) / (kJoinCols * 4)));
-      join_chunks<T><<<jg, kThreads, 0, st>>>(a, n, p.chunk, p.chunks, dw, vocab, hidden, parts,
-                                              scale);
+      join_chunks<T><<<dim3((unsigned)num_cus()), kJoinThreads, 0, st>>>(
+          a, n, p.chunk, p.chunks, dw, vocab, hidden, parts, scale);
       ML_LAUNCH_CHECK();
     }
     return ML_OK;
