@@ -487,6 +487,36 @@ int ml_lora_unpack(int count, const float* const* src, const int64_t* geometry, 
 int ml_lora_xa(const void* X, int64_t n_tokens, int64_t in_features, int64_t ldx, const void* A,
                int64_t rank_total, void* XA, int64_t ldo, void* stream);
 
+/* LoRA with dropout on the adapters' input (lora_dropout of PEFT, which the
+ * reference ignores), for nadp (1..3) adapters that share X [n_tokens,
+ * in_features] (bf16). Adapter i drops by ml_dropout's mask M_i over X's elements
+ * in row-major order: threshold thresholds[i], stream first_stream + i, *seed (one
+ * int64 in DEVICE memory); c_i = 65536 / (65536 - threshold), 0 at 65536. rank (16,
+ * 32, 48 or 64) of every adapter; in_features a multiple of 8.
+ *
+ * ml_lora_dropout_xa: XA [n_tokens, nadp rank] (row stride ldo), column block i =
+ * c_i (M_i X) A_i^T; A_stack [nadp rank, in_features] dense; X of row stride ldx (a
+ * multiple of 8). X and A 16-byte aligned.
+ *
+ * ml_lora_dropout_bwd: as ml_lora_qkv_bwd, XA being ml_lora_dropout_xa's:
+ *   dX   = sum_i dY_i W_i + M_i (P_i A_i),  P_i = c_i s_i dY_i B_i  (P in bf16; the
+ *          sum of the dY_i W_i is rounded to bf16 before the adapters' part is added)
+ *   dA_i = P_i^T (M_i X)        dB_i = s_i dY_i^T XA_i
+ * every operand dense and 16-byte aligned.
+ */
+int ml_lora_dropout_xa(int nadp, const void* X, int64_t n_tokens, int64_t in_features, int64_t ldx,
+                       const void* A_stack, int64_t rank, const int64_t* thresholds,
+                       const int64_t* seed, int64_t first_stream, void* XA, int64_t ldo,
+                       void* stream);
+size_t ml_lora_dropout_bwd_workspace_bytes(int nadp, int64_t n_tokens, int64_t in_features,
+                                           const int64_t* out_features, int64_t rank);
+int ml_lora_dropout_bwd(int nadp, const void* X, int64_t n_tokens, int64_t in_features,
+                        const void* const* dY, const int64_t* out_features, const void* const* W,
+                        const void* A_stack, const void* const* B, const float* scale,
+                        const void* XA, int64_t rank, const int64_t* thresholds,
+                        const int64_t* seed, int64_t first_stream, void* dX, float* dA,
+                        float* const* dB, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Grouped-query attention's key / value heads (no reference counterpart: its
  * models run transformers' attention, whose repeat_kv these replace), for
  * `count` (1..2: k and v) tensors in one launch. geometry[10 i ..] = B, H

@@ -312,8 +312,8 @@ def _(x2, w):
     return x2.new_empty((x2.shape[0], w.shape[0]), dtype=torch.bfloat16)
 
 
-# Dropout, the embedding and the packing and unpacking of adapters, registered
-# without custom_op's wrapper: the wrapper costs the host 4.7 us a call with lists of tensors (7.9 against 3.2
+# Dropout, the embedding, LoRA with dropout and the packing and unpacking of
+# adapters, registered without custom_op's wrapper: the wrapper costs the host 4.7 us a call with lists of tensors (7.9 against 3.2
 # for an op that only allocates), which made few-token passes slower than the
 # tensor operations that each of these replaces ([205, 1024] to 1024 at rank 8, a
 # pass on one thread: 186 us by those operations, 202 through custom_op).
@@ -365,6 +365,36 @@ lora_pack = _define("lora_pack(Tensor[] As, Tensor[] Bs, float[] scales, SymInt 
                     hip_ops.lora_pack, _lora_pack_fake)
 lora_unpack = _define("lora_unpack(Tensor flat, SymInt[] spec, ScalarType dtype) -> Tensor",
                       hip_ops.lora_unpack, _lora_unpack_fake)
+
+
+def _lora_dropout_fwd_fake(x2, ws, As, Bs, scales, rank, seed, thresholds, first):
+    new = lambda *s: x2.new_empty(s, dtype=torch.bfloat16)  # noqa: E731
+    return [*(new(x2.shape[0], w.shape[0]) for w in ws), new(x2.shape[0], len(ws) * rank),
+            _lora_pack_fake(As, Bs, scales, rank)]
+
+
+def _lora_dropout_bwd_fake(x2, dys, ws, packed, scales, xa, rank, seed, thresholds, first, spec,
+                           dtype):
+    shapes = hip_ops.lora_dropout_grad_shapes(x2.shape[1], [d.shape[1] for d in dys], rank)
+    grads = x2.new_empty((max(hip_ops.unpack_layout(spec)[1], 1),), dtype=dtype) if spec else \
+        _grads_fake(x2, shapes)
+    return x2.new_empty(x2.shape, dtype=torch.bfloat16), grads
+
+
+_LORA_DROPOUT_FWD = ("(Tensor x2, Tensor[] ws, Tensor[] As, Tensor[] Bs, float[] scales, "
+                     "SymInt rank, Tensor seed, SymInt[] thresholds, SymInt first) -> Tensor[]")
+_LORA_DROPOUT_BWD = ("(Tensor x2, Tensor[] dys, Tensor[] ws, Tensor packed, float[] scales, "
+                     "Tensor xa, SymInt rank, Tensor seed, SymInt[] thresholds, SymInt first, "
+                     "SymInt[] spec, ScalarType dtype) -> (Tensor, Tensor)")
+# ranks up to 64, and above (wide)
+lora_dropout_fwd = _define("lora_dropout_fwd" + _LORA_DROPOUT_FWD, hip_ops.lora_dropout_fwd,
+                           _lora_dropout_fwd_fake)
+lora_dropout_bwd = _define("lora_dropout_bwd" + _LORA_DROPOUT_BWD, hip_ops.lora_dropout_bwd,
+                           _lora_dropout_bwd_fake)
+lora_dropout_wide_fwd = _define("lora_dropout_wide_fwd" + _LORA_DROPOUT_FWD,
+                                hip_ops.lora_dropout_wide_fwd, _lora_dropout_fwd_fake)
+lora_dropout_wide_bwd = _define("lora_dropout_wide_bwd" + _LORA_DROPOUT_BWD,
+                                hip_ops.lora_dropout_wide_bwd, _lora_dropout_bwd_fake)
 
 
 @torch.library.custom_op(f"{NS}::lora_xa", mutates_args=(), device_types=_DEV)

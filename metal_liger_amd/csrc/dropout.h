@@ -62,6 +62,11 @@ inline DropRate drop_rate(int64_t threshold) {
   return DropRate{t | (t << 16), threshold > 0 ? 0u : ~0u};
 }
 
+// The factor of kept elements; 0 where nothing is kept.
+inline float drop_scale(int64_t threshold) {
+  return threshold < kDropAll ? 65536.f / (float)(kDropAll - threshold) : 0.f;
+}
+
 // All ones in the halves whose elements are kept, zeros in the others. (Written
 // out: from vectors of 16 bits the compiler makes two compares, two selects and a
 // permute of it.)

@@ -22,6 +22,7 @@
 // bit-reproducible.
 #include <algorithm>
 
+#include "dropout.h"
 #include "gemm_core.h"
 #include "swiglu_math.h"
 
@@ -329,7 +330,7 @@ struct DyJob {
   int64_t ldb;
   const bf16* xa;
   int64_t ldxa;
-  float scale;
+  float scale, pscale;  // of dB, of P
   bf16* p;
   int64_t ldp;
   float* db;
@@ -388,7 +389,7 @@ inline int dy_pass(int N, const DyJob* jobs, int n, char* ws, size_t ws_bytes, h
   for (int i = 0; i < n; ++i) {
     const DyJob& j = jobs[i];
     const DyAdapter& a = args.ad[i];
-    red.job[2 * i] = DyReduceJob{a.ppart, a.ctiles, N, j.p, j.ldp, j.scale, 0};
+    red.job[2 * i] = DyReduceJob{a.ppart, a.ctiles, N, j.p, j.ldp, j.pscale, 0};
     red.job[2 * i + 1] =
         DyReduceJob{a.dbpart, dy_rtiles(N, args.rows), j.O, j.db, j.lddb, j.scale, 1};
   }
@@ -1106,6 +1107,8 @@ __global__ __launch_bounds__(64 * kXaWaves) void xa_kernel(const bf16* __restric
   }
 }
 
+#include "lora_dropout.h"
+
 }  // namespace
 }  // namespace lora
 }  // namespace mla
@@ -1303,7 +1306,7 @@ static int adapters_bwd(const char* what, int nadp, const void* X, int64_t n_tok
       n += lora::dy_jobs(jobs + n,
                          lora::DyJob{static_cast<const bf16*>(dY[i]), out_features[i],
                                      (int)out_features[i], static_cast<const bf16*>(B[i]), R,
-                                     xa + i * R, RS, scale[i], P + i * R, RS, dB[i], R}, R);
+                                     xa + i * R, RS, scale[i], scale[i], P + i * R, RS, dB[i], R}, R);
     rc = lora::dy_pass(N, jobs, n, reinterpret_cast<char*>(part), part_bytes, st);
     if (rc) return rc;
   }
@@ -1378,6 +1381,126 @@ extern "C" int ml_lora_linear_bwd(const void* X, int64_t n_tokens, int64_t in_fe
   return adapters_bwd("lora linear", 1, X, n_tokens, in_features, dys, &out_features, ws_, A, bs,
                       &scale, XA, rank, dX, dA, dbs, workspace, workspace_bytes,
                       (hipStream_t)stream);
+}
+
+// ---------------------------------------------------------------- dropout --
+
+static int drop_rates(const char* what, int n, const int64_t* thresholds, const int64_t* seed,
+                      int64_t first_stream, lora::DropRates& r) {
+  ML_CHECK(n >= 1 && n <= lora::kDropMaxAdapters, "%s: 1..%d adapters (got %d)", what,
+           lora::kDropMaxAdapters, n);
+  ML_CHECK(thresholds && seed, "%s: null pointer", what);
+  ML_CHECK(first_stream >= 0 && first_stream + n - 1 <= 0xFFFFFFFFLL,
+           "%s: stream id outside 32 bits", what);
+  for (int i = 0; i < n; ++i) {
+    ML_CHECK(thresholds[i] >= 0 && thresholds[i] <= kDropAll,
+             "%s: threshold %lld outside 0..65536", what, (long long)thresholds[i]);
+    r.rate[i] = drop_rate(thresholds[i]);
+    r.stream[i] = (uint32_t)(first_stream + i);
+    r.scale[i] = drop_scale(thresholds[i]);
+  }
+  return ML_OK;
+}
+
+extern "C" int ml_lora_dropout_xa(int nadp, const void* X, int64_t n_tokens, int64_t in_features,
+                                  int64_t ldx, const void* A_stack, int64_t rank,
+                                  const int64_t* thresholds, const int64_t* seed,
+                                  int64_t first_stream, void* XA, int64_t ldo, void* stream) {
+  lora::DropRates rates{};
+  int rc = drop_rates("lora dropout xa", nadp, thresholds, seed, first_stream, rates);
+  if (rc) return rc;
+  ML_CHECK(n_tokens >= 0 && n_tokens < (1LL << 31), "lora dropout xa: bad token count");
+  ML_CHECK(in_features >= 8 && in_features % 8 == 0 && in_features < (1LL << 31),
+           "lora dropout xa: in_features must be a positive multiple of 8");
+  ML_CHECK(lora::pass_rank(rank) && rank > 0, "lora dropout xa: rank 16, 32, 48 or 64 (got %lld)",
+           (long long)rank);
+  ML_CHECK(ldx >= in_features && ldx % 8 == 0 && ldo >= nadp * rank,
+           "lora dropout xa: bad leading dimensions");
+  if (n_tokens == 0) return ML_OK;
+  ML_CHECK(X && A_stack && XA, "lora dropout xa: null pointer");
+  ML_CHECK(aligned16(X) && aligned16(A_stack),
+           "lora dropout xa: X and A must be 16-byte aligned");
+  return lora::drop_xa((int)n_tokens, (int)in_features, static_cast<const bf16*>(X), ldx,
+                       static_cast<const bf16*>(A_stack), nadp, (int)rank, seed, rates,
+                       static_cast<bf16*>(XA), ldo, (hipStream_t)stream);
+}
+
+extern "C" size_t ml_lora_dropout_bwd_workspace_bytes(int nadp, int64_t n_tokens,
+                                                      int64_t in_features,
+                                                      const int64_t* out_features, int64_t rank) {
+  if (nadp < 1 || nadp > lora::kDropMaxAdapters || n_tokens <= 0 || in_features <= 0 ||
+      rank <= 0 || !lora::pass_rank(rank) || !out_features)
+    return 0;
+  const int N = (int)n_tokens, IN = (int)in_features, R = (int)rank;
+  int O[lora::kDropMaxAdapters], kt = 0;
+  for (int i = 0; i < nadp; ++i) {
+    if (out_features[i] <= 0) return 0;
+    O[i] = (int)out_features[i];
+    kt += lora::ktiles(O[i]);
+  }
+  size_t m = lora::dy_pass_ws_bytes(N, O, nadp, R / lora::kDyRank);
+  m = std::max(m, product_ws_bytes(N, IN, kt));
+  m = std::max(m, lora::drop_bwd_ws_bytes(N, nadp * R, IN));
+  return lora::align256((size_t)n_tokens * nadp * rank * 2) + m;
+}
+
+extern "C" int ml_lora_dropout_bwd(int nadp, const void* X, int64_t n_tokens, int64_t in_features,
+                                   const void* const* dY, const int64_t* out_features,
+                                   const void* const* W, const void* A_stack,
+                                   const void* const* B, const float* scale, const void* XA,
+                                   int64_t rank, const int64_t* thresholds, const int64_t* seed,
+                                   int64_t first_stream, void* dX, float* dA, float* const* dB,
+                                   void* workspace, size_t workspace_bytes, void* stream) {
+  const char* what = "lora dropout";
+  lora::DropRates rates{};
+  int rc = drop_rates(what, nadp, thresholds, seed, first_stream, rates);
+  if (rc) return rc;
+  ML_CHECK(n_tokens > 0 && n_tokens < (1LL << 31), "%s: bad token count", what);
+  ML_CHECK(in_features >= 8 && in_features % 8 == 0 && in_features < (1LL << 31),
+           "%s: in_features must be a positive multiple of 8", what);
+  ML_CHECK(rank > 0 && lora::pass_rank(rank), "%s: rank 16, 32, 48 or 64 (got %lld)", what,
+           (long long)rank);
+  ML_CHECK(X && dY && out_features && W && A_stack && B && scale && XA && dX && dA && dB,
+           "%s: null pointer", what);
+  for (int i = 0; i < nadp; ++i) {
+    ML_CHECK(dY[i] && W[i] && B[i] && dB[i], "%s: null pointer for adapter %d", what, i);
+    ML_CHECK(out_features[i] > 0 && out_features[i] % 8 == 0 && out_features[i] < (1LL << 31),
+             "%s: out_features[%d] must be a positive multiple of 8", what, i);
+    ML_CHECK(aligned16(dY[i]) && aligned16(W[i]) && aligned16(B[i]),
+             "%s: dY, W and B of adapter %d must be 16-byte aligned", what, i);
+  }
+  ML_CHECK(all_aligned16({X, A_stack, XA, dX}), "%s: X, A, XA and dX must be 16-byte aligned",
+           what);
+  const size_t need = ml_lora_dropout_bwd_workspace_bytes(nadp, n_tokens, in_features,
+                                                          out_features, rank);
+  ML_CHECK(workspace && aligned16(workspace) && workspace_bytes >= need,
+           "%s: workspace too small or misaligned (%zu < %zu)", what, workspace_bytes, need);
+  const int N = (int)n_tokens, IN = (int)in_features, R = (int)rank, RT = nadp * R;
+  hipStream_t st = (hipStream_t)stream;
+  char* ws = static_cast<char*>(workspace);
+  bf16* P = reinterpret_cast<bf16*>(ws);  // [N, nadp r], column block i = c_i s_i dY_i B_i
+  char* part = ws + lora::align256((size_t)N * RT * 2);
+  const size_t part_bytes = workspace_bytes - (size_t)(part - ws);
+  const bf16* xa = static_cast<const bf16*>(XA);
+  lora::DyJob jobs[lora::kDyMaxJobs];
+  Segment segs[lora::kDropMaxAdapters];
+  int n = 0;
+  for (int i = 0; i < nadp; ++i) {
+    const bf16* dy = static_cast<const bf16*>(dY[i]);
+    const int O = (int)out_features[i];
+    n += lora::dy_jobs(jobs + n,
+                       lora::DyJob{dy, O, O, static_cast<const bf16*>(B[i]), R, xa + i * R, RT,
+                                   scale[i], scale[i] * rates.scale[i], P + i * R, RT, dB[i], R},
+                       R);
+    segs[i] = Segment{{dy, O}, {static_cast<const bf16*>(W[i]), IN}, O};
+  }
+  rc = lora::dy_pass(N, jobs, n, part, part_bytes, st);
+  if (rc) return rc;
+  rc = run_product(N, IN, nadp, segs, kMNMajor, static_cast<bf16*>(dX), IN, 1.0f, 0.0f,
+                   reinterpret_cast<float*>(part), part_bytes, st);
+  if (rc) return rc;
+  return lora::drop_bwd(N, IN, static_cast<const bf16*>(X), P, static_cast<const bf16*>(A_stack),
+                        nadp, R, seed, rates, static_cast<bf16*>(dX), dA, part, part_bytes, st);
 }
 
 // ------------------------------------------------------------------- MLP --
@@ -1463,7 +1586,7 @@ extern "C" int ml_lora_mlp_bwd(const void* X, int64_t n_tokens, int64_t hidden,
   if (passes) {  // P_D and dB_D in one pass over dY
     const int n = lora::dy_jobs(jobs, lora::DyJob{dy, H, H, static_cast<const bf16*>(BD), R,
                                                   static_cast<const bf16*>(hA_D), R, scale[2],
-                                                  PD, R, dB_D, R}, R);
+                                                  scale[2], PD, R, dB_D, R}, R);
     rc = lora::dy_pass(N, jobs, n, reinterpret_cast<char*>(part), part_bytes, st);
     if (rc) return rc;
   } else {
@@ -1529,8 +1652,8 @@ extern "C" int ml_lora_mlp_bwd(const void* X, int64_t n_tokens, int64_t hidden,
     int n = 0;
     for (int i = 0; i < 2; ++i)
       n += lora::dy_jobs(jobs + n, lora::DyJob{dgu[i], I, I, static_cast<const bf16*>(Bs[i]), R,
-                                               xa + i * R, R2, scale[i], PGU + i * R, R2, dBs[i],
-                                               R}, R);
+                                               xa + i * R, R2, scale[i], scale[i], PGU + i * R,
+                                               R2, dBs[i], R}, R);
     rc = lora::dy_pass(N, jobs, n, reinterpret_cast<char*>(part), part_bytes, st);
     if (rc) return rc;
   }

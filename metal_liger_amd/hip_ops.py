@@ -1143,6 +1143,122 @@ def lora_qkv_fwd(x2: torch.Tensor, ws, As, Bs, scales, rank: int):
     return _lora_outs(x2, ws, xa, sbs, [rank] * n, rank), xa, packed
 
 
+def lora_dropout_fwd(x2: torch.Tensor, ws, As, Bs, scales, rank: int, seed: torch.Tensor,
+                     thresholds, first: int) -> list:
+    """Projections of x2 whose adapters read it through dropout (ml_lora_dropout_xa:
+    adapter i by stream first + i of `seed`, threshold thresholds[i]), from the
+    adapters as they are; rank, 16 to 64, is what theirs are padded to. Returns
+    [*outs, XA [N, n rank], the packed adapters]."""
+    check_adapters([x2.shape[1]] * len(ws), ws, As, Bs)
+    ensure_rocm_device(x2, *ws, *As, *Bs, seed)
+    check_seed(seed)
+    x2 = _al16(x2)
+    ws = [_al16(w) for w in ws]
+    (N, IN), n = x2.shape, len(ws)
+    packed = lora_pack(As, Bs, scales, rank)
+    xa = torch.empty(N, n * rank, dtype=torch.bfloat16, device=x2.device)
+    base = packed.data_ptr()
+    call("ml_lora_dropout_xa", n, ptr(x2), N, IN, row_stride(x2), base, rank, geom(thresholds),
+         ptr(seed), first, ptr(xa), n * rank, stream_of(x2))
+    at, sbs = base + 2 * rank * (n * IN + sum(b.shape[0] for b in Bs)), []
+    for b in Bs:
+        sbs.append(at)
+        at += 2 * rank * b.shape[0]
+    if n > 1:
+        outs = _lora_outs(x2, ws, xa, sbs, [rank] * n, rank)
+    else:
+        off = (sbs[0] - base) // 2
+        outs = [lora_linear_out(x2, ws[0], xa,
+                                packed[off:off + ws[0].shape[0] * rank].view(-1, rank))]
+    return [*outs, xa, packed]
+
+
+def lora_dropout_bwd(x2, dys, ws_, packed, scales, xa, rank: int, seed, thresholds, first: int,
+                     spec, dtype):
+    """The backward of lora_dropout_fwd: (dX, the adapters' gradients as
+    lora_unpack(grads, spec, dtype), or in fp32 as laid out by
+    grad_layout(lora_dropout_grad_shapes(...)) where spec is empty)."""
+    ensure_rocm_device(x2, *dys, *ws_, packed, xa, seed)
+    x2 = _dense16(x2)
+    dys, ws_ = [list(_dense16(*t, None))[:-1] for t in (dys, ws_)]
+    (N, IN), n, dev = x2.shape, len(dys), x2.device
+    outs = [int(d.shape[1]) for d in dys]
+    dX = torch.empty(N, IN, dtype=torch.bfloat16, device=dev)
+    offs, total = grad_layout(lora_dropout_grad_shapes(IN, outs, rank))
+    flat = torch.empty(max(total, 1), dtype=torch.float32, device=dev)
+    if N == 0:
+        flat.zero_()
+    else:
+        base, g = packed.data_ptr(), flat.data_ptr()
+        at, b_ptrs = base + 2 * rank * n * IN, []
+        for o in outs:
+            b_ptrs.append(at)
+            at += 2 * rank * o
+        out_geom = geom(outs)
+        wsb = _hip.query("ml_lora_dropout_bwd_workspace_bytes", n, N, IN, out_geom, rank)
+        ws = torch.empty(max(wsb, 16), dtype=torch.uint8, device=dev)
+        call(
+            "ml_lora_dropout_bwd", n, x2.data_ptr(), N, IN, _hip.ptrs([d.data_ptr() for d in dys]),
+            out_geom, _hip.ptrs([w.data_ptr() for w in ws_]), base, _hip.ptrs(b_ptrs),
+            _hip.floats(scales), xa.data_ptr(), rank, geom(thresholds), seed.data_ptr(), first,
+            dX.data_ptr(), g, _hip.ptrs([g + 4 * o for o in offs[1:]]), ws.data_ptr(), ws.numel(),
+            stream_of(x2),
+        )
+    return dX, lora_unpack(flat, spec, dtype) if spec else flat
+
+
+def lora_dropout_wide_fwd(x2, ws, As, Bs, scales, rank: int, seed, thresholds, first: int) -> list:
+    """lora_dropout_fwd at ranks that the masked passes do not take: masked copies of
+    x2 through the plain products."""
+    check_adapters([x2.shape[1]] * len(ws), ws, As, Bs)
+    ensure_rocm_device(x2, *ws, *As, *Bs, seed)
+    (N, IN), n, bf = x2.shape, len(ws), torch.bfloat16
+    packed = lora_pack(As, Bs, scales, rank)
+    a_stack = packed[:n * rank * IN].view(n, rank, IN)
+    off, outs = rank * (n * IN + sum(b.shape[0] for b in Bs)), []
+    xa = torch.empty(N, n * rank, dtype=bf, device=x2.device)
+    for i, (w, b, t) in enumerate(zip(ws, Bs, thresholds)):
+        cols = xa[:, i * rank:(i + 1) * rank]
+        if N > 0:
+            matmul(dropout(x2, None, seed, t, first + i, 1.0), a_stack[i], b_t=True, out=cols,
+                   alpha=drop_scale(t))
+        o = b.shape[0]
+        outs.append(lora_linear_out(x2, w, cols, packed[off:off + o * rank].view(o, rank)))
+        off += o * rank
+    return [*outs, xa, packed]
+
+
+def lora_dropout_wide_bwd(x2, dys, ws_, packed, scales, xa, rank: int, seed, thresholds, first: int,
+                          spec, dtype):
+    """The backward of lora_dropout_wide_fwd, as lora_dropout_bwd."""
+    ensure_rocm_device(x2, *dys, *ws_, packed, xa, seed)
+    (N, IN), n, bf, dev = x2.shape, len(dys), torch.bfloat16, x2.device
+    shapes = lora_dropout_grad_shapes(IN, [d.shape[1] for d in dys], rank)
+    flat, (dA, *dBs) = _grad_buffer(shapes, dev)
+    if N == 0:
+        flat.zero_()
+        dX = torch.empty(0, IN, dtype=bf, device=dev)
+        return dX, lora_unpack(flat, spec, dtype) if spec else flat
+    a_stack = packed[:n * rank * IN].view(n, rank, IN)
+    off, dX = n * rank * IN, None
+    for dy, w in zip(dys, ws_):  # the large products' sum in fp32, rounded once
+        dX = matmul(dy, w, out=dX, beta=0.0 if dX is None else 1.0)
+    dX = dX.to(bf)
+    for i, (dy, t) in enumerate(zip(dys, thresholds)):
+        o = dy.shape[1]
+        b, off = packed[off:off + o * rank].view(o, rank), off + o * rank
+        P = matmul(dy, b, out_dtype=bf, alpha=scales[i] * drop_scale(t))
+        matmul(P, dropout(x2, None, seed, t, first + i, 1.0), a_t=True,
+               out=dA[i * rank:(i + 1) * rank])
+        matmul(dy, xa[:, i * rank:(i + 1) * rank], a_t=True, out=dBs[i], alpha=scales[i])
+        dX = dropout(matmul(P, a_stack[i], out_dtype=bf), dX, seed, t, first + i, 1.0)
+    return dX, lora_unpack(flat, spec, dtype) if spec else flat
+
+
+def lora_dropout_grad_shapes(IN, outs, rank):
+    return [(len(outs) * rank, IN), *((int(o), rank) for o in outs)]
+
+
 # The adapter gradients of one LoRA backward call live in one fp32 buffer:
 # each gradient starts on a 256-byte boundary, in the order the call lists
 # them. A caller that wants them in the parameters' dtype converts the buffer

@@ -441,7 +441,8 @@ class _LoRA_W(torch.autograd.Function):
 class _LoRA_Dropout(torch.autograd.Function):
     """Projections of one X whose adapters read it through dropout: `thresholds`
     (round(65536 p), one per projection) and streams first .. of `seed`; params
-    W, A, B, S of each. Returns their outputs."""
+    W, A, B, S of each. Returns their outputs. One op each way for bf16 and
+    ranks up to 64."""
 
     @staticmethod
     def forward(ctx, X, seed, thresholds, first: int, *params):
@@ -450,75 +451,76 @@ class _LoRA_Dropout(torch.autograd.Function):
         scales = [float(s) for s in params[3::4]]
         shape = X.shape
         hip_ops.check_adapters([shape[-1]] * len(Ws), Ws, As, Bs)
-        fp32 = _fp32_path(X, shape[-1], *(W.shape[0] for W in Ws))
-        if fp32:
-            X2, rp = _rows_f32(X), 0
-            Ac, Bc, sB = [_f32(A) for A in As], [_f32(B) for B in Bs], \
-                [_f32(B) * s for B, s in zip(Bs, scales)]
-            Wc, kept = [_f32(W) for W in Ws], [t.detach() for t in (*Ws, *As, *Bs)]
-        else:
-            X2, rp = hip_ops._bf16_rows(X.reshape(-1, shape[-1])), _pad_rank(max(A.shape[0] for A in As))
-            flat, a_views, Bc, sB = _packed([shape[-1]] * len(Ws), Ws, As, Bs, scales, rp)
-            Ac, Wc = [_view(flat, v) for v in a_views], [hip_ops._bf16_rows(W.detach()) for W in Ws]
-            kept = [*Wc, flat]
-        outs, xas = [], []
-        for i, t in enumerate(thresholds):
-            xa = _product([cops.dropout(X2, None, seed, t, first + i, 1.0)], [Ac[i]], True,
-                          alpha=hip_ops.drop_scale(t))
-            outs.append(cops.gemm_f32([X2, xa], [Wc[i], sB[i]], False, True, 1.0) if fp32
-                        else cops.lora_linear_out(X2, Wc[i], xa, sB[i]))
-            xas.append(xa)
-        ctx.save_for_backward(X2, seed, *xas, *kept)
         ctx.scales, ctx.thresholds, ctx.first = scales, thresholds, first
-        ctx.fp32, ctx.rank_p, ctx.orig_shape, ctx.x_dtype = fp32, rp, shape, X.dtype
-        ctx.outs = [W.shape[0] for W in Ws]
+        ctx.orig_shape, ctx.x_dtype = shape, X.dtype
         ctx.ranks = [A.shape[0] for A in As]
-        ctx.param_dtypes = [(A.dtype, B.dtype) for A, B in zip(As, Bs)]
-        return tuple(o.to(X.dtype).view(*shape[:-1], o.shape[-1]) for o in outs)
+        ctx.param_dtypes = [t.dtype for AB in zip(As, Bs) for t in AB]
+        ctx.rank_p = _pad_rank(max(ctx.ranks))
+        ctx.fp32 = _fp32_path(X, shape[-1], *(W.shape[0] for W in Ws))
+        if ctx.fp32:
+            X2 = _rows_f32(X)
+            Ac, Bc = [_f32(A) for A in As], [_f32(B) for B in Bs]
+            outs, xas = _dropped_f32(X2, [_f32(W) for W in Ws], Ac, [B * s for B, s in zip(Bc, scales)],
+                                     seed, thresholds, first)
+            ctx.save_for_backward(X2, seed, *xas, *(t.detach() for t in (*Ws, *As, *Bs)))
+            return tuple(o.to(X.dtype).view(*shape[:-1], o.shape[-1]) for o in outs)
+        X2 = hip_ops._bf16_rows(X.reshape(-1, shape[-1]))
+        Wc = [hip_ops._bf16_rows(W.detach()) for W in Ws]
+        op = cops.lora_dropout_fwd if ctx.rank_p <= 64 else cops.lora_dropout_wide_fwd
+        *outs, xa, packed = op(X2, Wc, list(As), list(Bs), scales, ctx.rank_p, seed, thresholds,
+                               first)
+        ctx.save_for_backward(X2, seed, xa, packed, *Wc)
+        return tuple(o.view(*shape[:-1], o.shape[-1]) for o in outs)
 
     @staticmethod
     def backward(ctx, *dYs):
         X2, seed, *rest = ctx.saved_tensors
-        n, rp = len(ctx.scales), ctx.rank_p
-        xas, Ws, adapters = rest[:n], rest[n:2 * n], rest[2 * n:]
+        n, ranks, dtypes = len(ctx.scales), ctx.ranks, ctx.param_dtypes
         if ctx.fp32:
-            dys, Ws = [_rows_f32(d) for d in dYs], [_f32(W) for W in Ws]
-            As, Bs = [_f32(t) for t in adapters[:n]], [_f32(t) for t in adapters[n:]]
+            xas, params = rest[:n], [_f32(t) for t in rest[n:]]
+            dX, grads = _dropped_grads_f32(X2, [_rows_f32(d) for d in dYs], params[:n],
+                                           params[n:2 * n], params[2 * n:], ctx.scales, xas, seed,
+                                           ctx.thresholds, ctx.first)
+            grads = [g.to(t) for g, t in zip(grads, dtypes)]
         else:
+            xa, packed, *Ws = rest
             dys = [hip_ops._bf16_rows(d.reshape(-1, d.shape[-1])) for d in dYs]
-            As, Bs = _unpack_views(adapters[0], X2.shape[1], ctx.outs, rp)
-        dX, grads = _product(dys, Ws, False), []
-        for i, t in enumerate(ctx.thresholds):
-            s, stream, r = ctx.scales[i], ctx.first + i, ctx.ranks[i]
-            P = _product([dys[i]], [Bs[i]], False, alpha=s * hip_ops.drop_scale(t))
-            dA = _product([P], [cops.dropout(X2, None, seed, t, stream, 1.0)], False, a_t=True,
-                          f32=True)
-            dB = _product([dys[i]], [xas[i]], False, a_t=True, f32=True, alpha=s)
-            dX = cops.dropout(_product([P], [As[i]], False), dX, seed, t, stream, 1.0)
-            ta, tb = ctx.param_dtypes[i]
-            grads += [None, dA[:r].to(ta), dB[:, :r].to(tb), None]
-        return (dX.to(ctx.x_dtype).view(*ctx.orig_shape), None, None, None, *grads)
+            rp, in_f = ctx.rank_p, X2.shape[1]
+            shapes = hip_ops.lora_dropout_grad_shapes(in_f, [d.shape[1] for d in dys], rp)
+            parts = [p for i, r in enumerate(ranks)
+                     for p in ((0, i * rp, r, in_f), (1 + i, 0, dys[i].shape[1], r))]
+            spec, unpack = _grad_spec(shapes, parts, dtypes)
+            op = cops.lora_dropout_bwd if rp <= 64 else cops.lora_dropout_wide_bwd
+            dX, flat = op(X2, dys, Ws, packed, ctx.scales, xa, rp, seed, ctx.thresholds, ctx.first,
+                          spec if unpack else [], dtypes[0] if unpack else torch.float32)
+            grads = _unpacked_views(flat, spec) if unpack else \
+                [g.to(t) for g, t in zip(_grad_views(flat, spec), dtypes)]
+        out = [dX.to(ctx.x_dtype).view(*ctx.orig_shape), None, None, None]
+        for i in range(n):
+            out += [None, grads[2 * i], grads[2 * i + 1], None]
+        return tuple(out)
 
 
-def _unpack_views(flat, in_f, outs, rp: int):
-    """The A_i [rp, in] and B_i [out_i, rp] of _packed's buffer."""
-    As = [_view(flat, (i * rp * in_f, rp, in_f)) for i in range(len(outs))]
-    off, Bs = len(outs) * rp * in_f, []
-    for o in outs:
-        Bs.append(_view(flat, (off, o, rp)))
-        off += o * rp
-    return As, Bs
+def _dropped_f32(X2, Ws, As, sBs, seed, thresholds, first: int):
+    """The outputs and the XA_i, in fp32."""
+    outs, xas = [], []
+    for i, (W, A, sB, t) in enumerate(zip(Ws, As, sBs, thresholds)):
+        xm = cops.dropout(X2, None, seed, t, first + i, 1.0)
+        xas.append(cops.gemm_f32([xm], [A], False, True, hip_ops.drop_scale(t)))
+        outs.append(cops.gemm_f32([X2, xas[-1]], [W, sB], False, True, 1.0))
+    return outs, xas
 
 
-def _product(a_list, b_list, b_t: bool, a_t: bool = False, alpha: float = 1.0, f32: bool = False):
-    """alpha * sum_s op(a_s) op(b_s) in the operands' dtype (f32: in fp32)."""
-    if a_list[0].dtype == torch.float32:
-        return cops.gemm_f32(a_list, b_list, a_t, b_t, alpha)
-    out = None
-    for a, b in zip(a_list, b_list):
-        p = hip_ops.matmul(a, b, a_t=a_t, b_t=b_t, alpha=alpha)
-        out = p if out is None else out.add_(p)
-    return out if f32 else out.to(torch.bfloat16)
+def _dropped_grads_f32(X2, dys, Ws, As, Bs, scales, xas, seed, thresholds, first: int):
+    """dX and [dA_i, dB_i, ...] in fp32."""
+    dX, grads = cops.gemm_f32(dys, Ws, False, False, 1.0), []
+    for i, (dy, A, B, s, xa, t) in enumerate(zip(dys, As, Bs, scales, xas, thresholds)):
+        P = cops.gemm_f32([dy], [B], False, False, s * hip_ops.drop_scale(t))
+        xm = cops.dropout(X2, None, seed, t, first + i, 1.0)
+        grads += [cops.gemm_f32([P], [xm], True, False, 1.0),
+                  cops.gemm_f32([dy], [xa], True, False, s)]
+        dX = cops.dropout(cops.gemm_f32([P], [A], False, False, 1.0), dX, seed, t, first + i, 1.0)
+    return dX, grads
 
 
 def _drop_threshold(linear) -> int:
