@@ -397,6 +397,26 @@ lora_dropout_wide_bwd = _define("lora_dropout_wide_bwd" + _LORA_DROPOUT_BWD,
                                 hip_ops.lora_dropout_wide_bwd, _lora_dropout_bwd_fake)
 
 
+def _lora_dropout_f32_fwd_fake(x2, ws, As, Bs, scales, seed, thresholds, first):
+    new = lambda *s: x2.new_empty(s, dtype=torch.float32)  # noqa: E731
+    return [new(x2.shape[0], m.shape[0]) for m in (*ws, *As)]
+
+
+def _lora_dropout_f32_bwd_fake(x2, dys, ws, As, Bs, scales, xas, seed, thresholds, first):
+    new = lambda s: x2.new_empty(s, dtype=torch.float32)  # noqa: E731
+    return [new(x2.shape), *(new(t.shape) for AB in zip(As, Bs) for t in AB)]
+
+
+lora_dropout_f32_fwd = _define(
+    "lora_dropout_f32_fwd(Tensor x2, Tensor[] ws, Tensor[] As, Tensor[] Bs, float[] scales, "
+    "Tensor seed, SymInt[] thresholds, SymInt first) -> Tensor[]",
+    hip_ops.lora_dropout_f32_fwd, _lora_dropout_f32_fwd_fake)
+lora_dropout_f32_bwd = _define(
+    "lora_dropout_f32_bwd(Tensor x2, Tensor[] dys, Tensor[] ws, Tensor[] As, Tensor[] Bs, "
+    "float[] scales, Tensor[] xas, Tensor seed, SymInt[] thresholds, SymInt first) -> Tensor[]",
+    hip_ops.lora_dropout_f32_bwd, _lora_dropout_f32_bwd_fake)
+
+
 @torch.library.custom_op(f"{NS}::lora_xa", mutates_args=(), device_types=_DEV)
 def lora_xa(x2: Tensor, a_stack: Tensor) -> Tensor:
     return hip_ops.lora_xa(x2, a_stack)

@@ -1255,6 +1255,30 @@ def lora_dropout_wide_bwd(x2, dys, ws_, packed, scales, xa, rank: int, seed, thr
     return dX, lora_unpack(flat, spec, dtype) if spec else flat
 
 
+def lora_dropout_f32_fwd(x2, ws, As, Bs, scales, seed, thresholds, first: int) -> list:
+    """The projections in fp32, by the fp32 products over masked copies of x2:
+    [*outs, *XA_i]."""
+    ensure_rocm_device(x2, *ws, *As, *Bs, seed)
+    outs, xas = [], []
+    for i, (w, a, b, s, t) in enumerate(zip(ws, As, Bs, scales, thresholds)):
+        xm = dropout(x2, None, seed, t, first + i, 1.0)
+        xas.append(gemm_f32([xm], [a], b_t=True, alpha=drop_scale(t)))
+        outs.append(gemm_f32([x2, xas[-1]], [w, b.float() * s], b_t=True))
+    return [*outs, *xas]
+
+
+def lora_dropout_f32_bwd(x2, dys, ws, As, Bs, scales, xas, seed, thresholds, first: int) -> list:
+    """The backward of lora_dropout_f32_fwd in fp32: [dX, dA_0, dB_0, dA_1, ...]."""
+    ensure_rocm_device(x2, *dys, *ws, *As, *Bs, *xas, seed)
+    dX, grads = gemm_f32(dys, ws), []
+    for i, (dy, a, b, s, xa, t) in enumerate(zip(dys, As, Bs, scales, xas, thresholds)):
+        P = gemm_f32([dy], [b], alpha=s * drop_scale(t))
+        xm = dropout(x2, None, seed, t, first + i, 1.0)
+        grads += [gemm_f32([P], [xm], a_t=True), gemm_f32([dy], [xa], a_t=True, alpha=s)]
+        dX = dropout(gemm_f32([P], [a]), dX, seed, t, first + i, 1.0)
+    return [dX, *grads]
+
+
 def lora_dropout_grad_shapes(IN, outs, rank):
     return [(len(outs) * rank, IN), *((int(o), rank) for o in outs)]
 

@@ -458,12 +458,12 @@ class _LoRA_Dropout(torch.autograd.Function):
         ctx.rank_p = _pad_rank(max(ctx.ranks))
         ctx.fp32 = _fp32_path(X, shape[-1], *(W.shape[0] for W in Ws))
         if ctx.fp32:
-            X2 = _rows_f32(X)
-            Ac, Bc = [_f32(A) for A in As], [_f32(B) for B in Bs]
-            outs, xas = _dropped_f32(X2, [_f32(W) for W in Ws], Ac, [B * s for B, s in zip(Bc, scales)],
-                                     seed, thresholds, first)
-            ctx.save_for_backward(X2, seed, *xas, *(t.detach() for t in (*Ws, *As, *Bs)))
-            return tuple(o.to(X.dtype).view(*shape[:-1], o.shape[-1]) for o in outs)
+            X2, params = _rows_f32(X), [t.detach() for t in (*Ws, *As, *Bs)]
+            n = len(Ws)
+            res = cops.lora_dropout_f32_fwd(X2, params[:n], params[n:2 * n], params[2 * n:], scales,
+                                            seed, thresholds, first)
+            ctx.save_for_backward(X2, seed, *res[n:], *params)
+            return tuple(o.to(X.dtype).view(*shape[:-1], o.shape[-1]) for o in res[:n])
         X2 = hip_ops._bf16_rows(X.reshape(-1, shape[-1]))
         Wc = [hip_ops._bf16_rows(W.detach()) for W in Ws]
         op = cops.lora_dropout_fwd if ctx.rank_p <= 64 else cops.lora_dropout_wide_fwd
@@ -477,10 +477,9 @@ class _LoRA_Dropout(torch.autograd.Function):
         X2, seed, *rest = ctx.saved_tensors
         n, ranks, dtypes = len(ctx.scales), ctx.ranks, ctx.param_dtypes
         if ctx.fp32:
-            xas, params = rest[:n], [_f32(t) for t in rest[n:]]
-            dX, grads = _dropped_grads_f32(X2, [_rows_f32(d) for d in dYs], params[:n],
-                                           params[n:2 * n], params[2 * n:], ctx.scales, xas, seed,
-                                           ctx.thresholds, ctx.first)
+            xas, Ws, As, Bs = (list(rest[k * n:(k + 1) * n]) for k in range(4))
+            dX, *grads = cops.lora_dropout_f32_bwd(X2, [_rows_f32(d) for d in dYs], Ws, As, Bs,
+                                                   ctx.scales, xas, seed, ctx.thresholds, ctx.first)
             grads = [g.to(t) for g, t in zip(grads, dtypes)]
         else:
             xa, packed, *Ws = rest
@@ -499,28 +498,6 @@ class _LoRA_Dropout(torch.autograd.Function):
         for i in range(n):
             out += [None, grads[2 * i], grads[2 * i + 1], None]
         return tuple(out)
-
-
-def _dropped_f32(X2, Ws, As, sBs, seed, thresholds, first: int):
-    """The outputs and the XA_i, in fp32."""
-    outs, xas = [], []
-    for i, (W, A, sB, t) in enumerate(zip(Ws, As, sBs, thresholds)):
-        xm = cops.dropout(X2, None, seed, t, first + i, 1.0)
-        xas.append(cops.gemm_f32([xm], [A], False, True, hip_ops.drop_scale(t)))
-        outs.append(cops.gemm_f32([X2, xas[-1]], [W, sB], False, True, 1.0))
-    return outs, xas
-
-
-def _dropped_grads_f32(X2, dys, Ws, As, Bs, scales, xas, seed, thresholds, first: int):
-    """dX and [dA_i, dB_i, ...] in fp32."""
-    dX, grads = cops.gemm_f32(dys, Ws, False, False, 1.0), []
-    for i, (dy, A, B, s, xa, t) in enumerate(zip(dys, As, Bs, scales, xas, thresholds)):
-        P = cops.gemm_f32([dy], [B], False, False, s * hip_ops.drop_scale(t))
-        xm = cops.dropout(X2, None, seed, t, first + i, 1.0)
-        grads += [cops.gemm_f32([P], [xm], True, False, 1.0),
-                  cops.gemm_f32([dy], [xa], True, False, s)]
-        dX = cops.dropout(cops.gemm_f32([P], [A], False, False, 1.0), dX, seed, t, first + i, 1.0)
-    return dX, grads
 
 
 def _drop_threshold(linear) -> int:
