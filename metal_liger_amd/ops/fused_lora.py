@@ -450,7 +450,6 @@ class _LoRA_Dropout(torch.autograd.Function):
         Ws, As, Bs = params[0::4], params[1::4], params[2::4]
         scales = [float(s) for s in params[3::4]]
         shape = X.shape
-        hip_ops.check_adapters([shape[-1]] * len(Ws), Ws, As, Bs)
         ctx.scales, ctx.thresholds, ctx.first = scales, thresholds, first
         ctx.orig_shape, ctx.x_dtype = shape, X.dtype
         ctx.ranks = [A.shape[0] for A in As]
@@ -460,6 +459,7 @@ class _LoRA_Dropout(torch.autograd.Function):
         if ctx.fp32:
             X2, params = _rows_f32(X), [t.detach() for t in (*Ws, *As, *Bs)]
             n = len(Ws)
+            hip_ops.check_adapters([shape[-1]] * n, Ws, As, Bs)
             res = cops.lora_dropout_f32_fwd(X2, params[:n], params[n:2 * n], params[2 * n:], scales,
                                             seed, thresholds, first)
             ctx.save_for_backward(X2, seed, *res[n:], *params)
@@ -506,7 +506,7 @@ def _drop_threshold(linear) -> int:
     dropouts = getattr(linear, "lora_dropout", None)
     if dropouts is None:
         return 0
-    module = dropouts[list(linear.lora_A.keys())[0]]
+    module = dropouts[next(iter(linear.lora_A.keys()))]
     if isinstance(module, nn.Identity) or not module.training:
         return 0
     if not isinstance(module, (nn.Dropout, MetalLigerDropout)):
@@ -514,13 +514,15 @@ def _drop_threshold(linear) -> int:
     return hip_ops.drop_threshold(module.p)
 
 
-def _dropped(linears, X, seed, first: int = 0):
-    """The projections of X with their adapters' dropout, or None where none drops."""
+def _dropped(linears, X, seed, first: int = 0, params=None):
+    """The projections of X with their adapters' dropout, or None where none drops.
+    params: W, A, B, S of each, if they are at hand."""
     thresholds = [_drop_threshold(m) for m in linears]
     if not any(thresholds):
         return None
     hip_ops.ensure_rocm_device(X)
-    params = [t for m in linears for t in _get_lora_params(m)]
+    if params is None:
+        params = [t for m in linears for t in _get_lora_params(m)]
     return _LoRA_Dropout.apply(X, seed_tensor(seed, X.device), tuple(thresholds), first, *params)
 
 
@@ -533,7 +535,7 @@ def apply_fused_lora_linear(linear, X: torch.Tensor, lora_dropout: bool = False,
     if A is None:
         return linear(X)
     if lora_dropout:
-        out = _dropped([linear], X, seed)
+        out = _dropped([linear], X, seed, params=(W, A, B, S))
         if out is not None:
             return out[0]
     return _LoRA_W.apply(X, W, A, B, S)
@@ -558,7 +560,8 @@ def apply_fused_lora_qkv(attn_module, X: torch.Tensor, lora_dropout: bool = Fals
         return Q, K, V
 
     if lora_dropout:
-        outs = _dropped([attn_module.q_proj, attn_module.k_proj, attn_module.v_proj], X, seed)
+        outs = _dropped([attn_module.q_proj, attn_module.k_proj, attn_module.v_proj], X, seed,
+                        params=(QW, QA, QB, QS, KW, KA, KB, KS, VW, VA, VB, VS))
         if outs is not None:
             return outs
     return _LoRA_QKV.apply(
@@ -587,10 +590,10 @@ def apply_fused_lora_mlp(mlp_module, X: torch.Tensor, lora_dropout: bool = False
     if lora_dropout and any(_drop_threshold(m) for m in projections):
         hip_ops.ensure_rocm_device(X)
         seed = seed_tensor(seed, X.device)
-        gate, up = _dropped(projections[:2], X, seed) or (
+        gate, up = _dropped(projections[:2], X, seed, 0, (GW, GA, GB, GS, UW, UA, UB, US)) or (
             apply_fused_lora_linear(m, X) for m in projections[:2])
         h = fused_swiglu(gate, up)
-        down = _dropped(projections[2:], h, seed, first=2)
+        down = _dropped(projections[2:], h, seed, 2, (DW, DA, DB, DS))
         return down[0] if down is not None else _LoRA_W.apply(h, DW, DA, DB, DS)
     return _LoRA_MLP.apply(
         X,
