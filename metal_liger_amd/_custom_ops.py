@@ -397,6 +397,32 @@ lora_dropout_wide_bwd = _define("lora_dropout_wide_bwd" + _LORA_DROPOUT_BWD,
                                 hip_ops.lora_dropout_wide_bwd, _lora_dropout_bwd_fake)
 
 
+def _lora_dropout_mlp_fwd_fake(x2, ws, As, Bs, scales, rank, seed, thresholds):
+    new = lambda n: x2.new_empty((x2.shape[0], n), dtype=torch.bfloat16)  # noqa: E731
+    inter = ws[0].shape[0]
+    return [new(ws[2].shape[0]), new(inter), new(inter), new(inter), new(2 * rank), new(rank),
+            _lora_pack_fake(As, Bs, scales, rank)]
+
+
+def _lora_dropout_mlp_bwd_fake(x2, gate, up, h, dy, ws, packed, scales, xa, xa_d, rank, seed,
+                               thresholds, spec, dtype):
+    shapes = hip_ops.lora_mlp_grad_shapes(x2.shape[1], gate.shape[1], rank)
+    grads = x2.new_empty((max(hip_ops.unpack_layout(spec)[1], 1),), dtype=dtype) if spec else \
+        _grads_fake(x2, shapes)
+    return x2.new_empty(x2.shape, dtype=torch.bfloat16), grads
+
+
+lora_dropout_mlp_fwd = _define(
+    "lora_dropout_mlp_fwd(Tensor x2, Tensor[] ws, Tensor[] As, Tensor[] Bs, float[] scales, "
+    "SymInt rank, Tensor seed, SymInt[] thresholds) -> Tensor[]",
+    hip_ops.lora_dropout_mlp_fwd, _lora_dropout_mlp_fwd_fake)
+lora_dropout_mlp_bwd = _define(
+    "lora_dropout_mlp_bwd(Tensor x2, Tensor gate, Tensor up, Tensor h, Tensor dy, Tensor[] ws, "
+    "Tensor packed, float[] scales, Tensor xa, Tensor xa_d, SymInt rank, Tensor seed, "
+    "SymInt[] thresholds, SymInt[] spec, ScalarType dtype) -> (Tensor, Tensor)",
+    hip_ops.lora_dropout_mlp_bwd, _lora_dropout_mlp_bwd_fake)
+
+
 def _lora_dropout_f32_fwd_fake(x2, ws, As, Bs, scales, seed, thresholds, first):
     new = lambda *s: x2.new_empty(s, dtype=torch.float32)  # noqa: E731
     return [new(x2.shape[0], m.shape[0]) for m in (*ws, *As)]

@@ -1073,6 +1073,10 @@ def lora_linear_out(x2: torch.Tensor, w: torch.Tensor, xa: torch.Tensor,
     """X W^T + XA (s B)^T as ONE K-concatenated GEMM -> [N, out] bf16."""
     ensure_rocm_device(x2, w, xa, sb)
     x2, w, xa, sb = _al16(x2, w, xa, sb)
+    return _lora_out(x2, w, xa, sb.data_ptr(), sb.stride(0))
+
+
+def _lora_out(x2, w, xa, sb_ptr: int, sb_stride: int) -> torch.Tensor:
     N, K = x2.shape
     out_f = w.shape[0]
     r = xa.shape[1]
@@ -1084,8 +1088,8 @@ def lora_linear_out(x2: torch.Tensor, w: torch.Tensor, xa: torch.Tensor,
     ws = torch.empty(wsb, dtype=torch.uint8, device=x2.device) if wsb else None
     call(
         "ml_gemm_bf16_segments_ws", N, out_f, 2, k_lens, _hip.ptrs([x2.data_ptr(), xa.data_ptr()]),
-        geom([x2.stride(0), xa.stride(0)]), _hip.ptrs([w.data_ptr(), sb.data_ptr()]),
-        geom([w.stride(0), sb.stride(0)]), 0, 0, ptr(out), out.stride(0), dtype_tag(out, "out"),
+        geom([x2.stride(0), xa.stride(0)]), _hip.ptrs([w.data_ptr(), sb_ptr]),
+        geom([w.stride(0), sb_stride]), 0, 0, ptr(out), out.stride(0), dtype_tag(out, "out"),
         1.0, 0.0, ptr(ws), wsb, stream_of(x2),
     )
     return out
@@ -1143,34 +1147,65 @@ def lora_qkv_fwd(x2: torch.Tensor, ws, As, Bs, scales, rank: int):
     return _lora_outs(x2, ws, xa, sbs, [rank] * n, rank), xa, packed
 
 
+def _packed_ptrs(packed, ins, outs, rank: int):
+    """The addresses of lora_pack's A_i, B_i and s_i B_i."""
+    at, ptrs = packed.data_ptr(), []
+    for n in (*ins, *outs, *outs):
+        ptrs.append(at)
+        at += 2 * rank * n
+    n = len(ins)
+    return ptrs[:n], ptrs[n:2 * n], ptrs[2 * n:]
+
+
+def _drop_xa(x2, a_ptr: int, n: int, rank: int, seed, thresholds, first: int) -> torch.Tensor:
+    """ml_lora_dropout_xa for the n adapters whose stacked A lies at a_ptr."""
+    N, IN = x2.shape
+    xa = torch.empty(N, n * rank, dtype=torch.bfloat16, device=x2.device)
+    call("ml_lora_dropout_xa", n, ptr(x2), N, IN, row_stride(x2), a_ptr, rank, geom(thresholds),
+         ptr(seed), first, ptr(xa), n * rank, stream_of(x2))
+    return xa
+
+
 def lora_dropout_fwd(x2: torch.Tensor, ws, As, Bs, scales, rank: int, seed: torch.Tensor,
                      thresholds, first: int) -> list:
     """Projections of x2 whose adapters read it through dropout (ml_lora_dropout_xa:
     adapter i by stream first + i of `seed`, threshold thresholds[i]), from the
     adapters as they are; rank, 16 to 64, is what theirs are padded to. Returns
     [*outs, XA [N, n rank], the packed adapters]."""
-    check_adapters([x2.shape[1]] * len(ws), ws, As, Bs)
+    n, ins = len(ws), [x2.shape[1]] * len(ws)
+    check_adapters(ins, ws, As, Bs)
     ensure_rocm_device(x2, *ws, *As, *Bs, seed)
     check_seed(seed)
     x2 = _al16(x2)
     ws = [_al16(w) for w in ws]
-    (N, IN), n = x2.shape, len(ws)
     packed = lora_pack(As, Bs, scales, rank)
-    xa = torch.empty(N, n * rank, dtype=torch.bfloat16, device=x2.device)
-    base = packed.data_ptr()
-    call("ml_lora_dropout_xa", n, ptr(x2), N, IN, row_stride(x2), base, rank, geom(thresholds),
-         ptr(seed), first, ptr(xa), n * rank, stream_of(x2))
-    at, sbs = base + 2 * rank * (n * IN + sum(b.shape[0] for b in Bs)), []
-    for b in Bs:
-        sbs.append(at)
-        at += 2 * rank * b.shape[0]
+    a_ptrs, _, sbs = _packed_ptrs(packed, ins, [w.shape[0] for w in ws], rank)
+    xa = _drop_xa(x2, a_ptrs[0], n, rank, seed, thresholds, first)
     if n > 1:
         outs = _lora_outs(x2, ws, xa, sbs, [rank] * n, rank)
     else:
-        off = (sbs[0] - base) // 2
-        outs = [lora_linear_out(x2, ws[0], xa,
-                                packed[off:off + ws[0].shape[0] * rank].view(-1, rank))]
+        outs = [_lora_out(x2, ws[0], xa, sbs[0], rank)]
     return [*outs, xa, packed]
+
+
+def _lora_dropout_bwd(x2, dys, ws_, a_ptr: int, b_ptrs, scales, xa, rank: int, seed, thresholds,
+                      first: int, da_ptr: int, db_ptrs) -> torch.Tensor:
+    """ml_lora_dropout_bwd for at least one token; the gradients go to the given
+    fp32 buffers. Returns dX."""
+    x2 = _dense16(x2)
+    dys, ws_ = [list(_dense16(*t, None))[:-1] for t in (dys, ws_)]
+    (N, IN), n, dev = x2.shape, len(dys), x2.device
+    dX = torch.empty(N, IN, dtype=torch.bfloat16, device=dev)
+    out_geom = geom([d.shape[1] for d in dys])
+    wsb = _hip.query("ml_lora_dropout_bwd_workspace_bytes", n, N, IN, out_geom, rank)
+    ws = torch.empty(max(wsb, 16), dtype=torch.uint8, device=dev)
+    call(
+        "ml_lora_dropout_bwd", n, x2.data_ptr(), N, IN, _hip.ptrs([d.data_ptr() for d in dys]),
+        out_geom, _hip.ptrs([w.data_ptr() for w in ws_]), a_ptr, _hip.ptrs(b_ptrs),
+        _hip.floats(scales), xa.data_ptr(), rank, geom(thresholds), seed.data_ptr(), first,
+        dX.data_ptr(), da_ptr, _hip.ptrs(db_ptrs), ws.data_ptr(), wsb, stream_of(x2),
+    )
+    return dX
 
 
 def lora_dropout_bwd(x2, dys, ws_, packed, scales, xa, rank: int, seed, thresholds, first: int,
@@ -1179,31 +1214,57 @@ def lora_dropout_bwd(x2, dys, ws_, packed, scales, xa, rank: int, seed, threshol
     lora_unpack(grads, spec, dtype), or in fp32 as laid out by
     grad_layout(lora_dropout_grad_shapes(...)) where spec is empty)."""
     ensure_rocm_device(x2, *dys, *ws_, packed, xa, seed)
-    x2 = _dense16(x2)
-    dys, ws_ = [list(_dense16(*t, None))[:-1] for t in (dys, ws_)]
-    (N, IN), n, dev = x2.shape, len(dys), x2.device
-    outs = [int(d.shape[1]) for d in dys]
-    dX = torch.empty(N, IN, dtype=torch.bfloat16, device=dev)
+    (N, IN), outs = x2.shape, [int(d.shape[1]) for d in dys]
     offs, total = grad_layout(lora_dropout_grad_shapes(IN, outs, rank))
-    flat = torch.empty(max(total, 1), dtype=torch.float32, device=dev)
+    flat = torch.empty(max(total, 1), dtype=torch.float32, device=x2.device)
     if N == 0:
         flat.zero_()
+        dX = torch.empty(0, IN, dtype=torch.bfloat16, device=x2.device)
     else:
-        base, g = packed.data_ptr(), flat.data_ptr()
-        at, b_ptrs = base + 2 * rank * n * IN, []
-        for o in outs:
-            b_ptrs.append(at)
-            at += 2 * rank * o
-        out_geom = geom(outs)
-        wsb = _hip.query("ml_lora_dropout_bwd_workspace_bytes", n, N, IN, out_geom, rank)
-        ws = torch.empty(max(wsb, 16), dtype=torch.uint8, device=dev)
-        call(
-            "ml_lora_dropout_bwd", n, x2.data_ptr(), N, IN, _hip.ptrs([d.data_ptr() for d in dys]),
-            out_geom, _hip.ptrs([w.data_ptr() for w in ws_]), base, _hip.ptrs(b_ptrs),
-            _hip.floats(scales), xa.data_ptr(), rank, geom(thresholds), seed.data_ptr(), first,
-            dX.data_ptr(), g, _hip.ptrs([g + 4 * o for o in offs[1:]]), ws.data_ptr(), ws.numel(),
-            stream_of(x2),
-        )
+        a_ptrs, b_ptrs, _ = _packed_ptrs(packed, [IN] * len(outs), outs, rank)
+        g = flat.data_ptr()
+        dX = _lora_dropout_bwd(x2, dys, ws_, a_ptrs[0], b_ptrs, scales, xa, rank, seed, thresholds,
+                               first, g, [g + 4 * o for o in offs[1:]])
+    return dX, lora_unpack(flat, spec, dtype) if spec else flat
+
+
+def lora_dropout_mlp_fwd(x2, ws, As, Bs, scales, rank: int, seed, thresholds) -> list:
+    """The MLP block whose gate, up and down adapters read their inputs through
+    dropout (streams 0, 1, 2): [out, gate, up, h, XA_GU, XA_D, the packed adapters]."""
+    ins, outs = [x2.shape[1]] * 2 + [ws[0].shape[0]], [w.shape[0] for w in ws]
+    check_adapters(ins, ws, As, Bs)
+    ensure_rocm_device(x2, *ws, *As, *Bs, seed)
+    check_seed(seed)
+    x2 = _al16(x2)
+    ws = [_al16(w) for w in ws]
+    packed = lora_pack(As, Bs, scales, rank)
+    a_ptrs, _, sbs = _packed_ptrs(packed, ins, outs, rank)
+    xa = _drop_xa(x2, a_ptrs[0], 2, rank, seed, thresholds[:2], 0)
+    gate, up = _lora_outs(x2, ws[:2], xa, sbs[:2], [rank] * 2, rank)
+    h = swiglu_fwd(gate, up)
+    xa_d = _drop_xa(h, a_ptrs[2], 1, rank, seed, thresholds[2:], 2)
+    return [_lora_out(h, ws[2], xa_d, sbs[2], rank), gate, up, h, xa, xa_d, packed]
+
+
+def lora_dropout_mlp_bwd(x2, gate, up, h, dy, ws_, packed, scales, xa, xa_d, rank: int, seed,
+                         thresholds, spec, dtype):
+    """The backward of lora_dropout_mlp_fwd, as lora_dropout_bwd; the gradients'
+    layout is that of lora_mlp_grad_shapes."""
+    ensure_rocm_device(x2, gate, up, h, dy, *ws_, packed, xa, xa_d, seed)
+    (N, H), I = x2.shape, gate.shape[1]  # noqa: E741
+    offs, total = grad_layout(lora_mlp_grad_shapes(H, I, rank))
+    flat = torch.empty(max(total, 1), dtype=torch.float32, device=x2.device)
+    if N == 0:
+        flat.zero_()
+        dX = torch.empty(0, H, dtype=torch.bfloat16, device=x2.device)
+        return dX, lora_unpack(flat, spec, dtype) if spec else flat
+    a_ptrs, b_ptrs, _ = _packed_ptrs(packed, [H, H, I], [I, I, H], rank)
+    da_gu, da_d, db_g, db_u, db_d = (flat.data_ptr() + 4 * o for o in offs)
+    dh = _lora_dropout_bwd(h, [dy], ws_[2:], a_ptrs[2], b_ptrs[2:], scales[2:], xa_d, rank, seed,
+                           thresholds[2:], 2, da_d, [db_d])
+    dgate, dup = swiglu_bwd(gate, up, dh)
+    dX = _lora_dropout_bwd(x2, [dgate, dup], ws_[:2], a_ptrs[0], b_ptrs[:2], scales[:2], xa, rank,
+                           seed, thresholds[:2], 0, da_gu, [db_g, db_u])
     return dX, lora_unpack(flat, spec, dtype) if spec else flat
 
 

@@ -500,6 +500,46 @@ class _LoRA_Dropout(torch.autograd.Function):
         return tuple(out)
 
 
+class _LoRA_Dropout_MLP(torch.autograd.Function):
+    """gate + up + down with dropout on each adapter's input (streams 0, 1, 2 of
+    `seed`) and SwiGLU, for bf16 and ranks up to 64: one op each way. h is saved,
+    as the down adapter's input."""
+
+    @staticmethod
+    def forward(ctx, X, seed, thresholds, *params):
+        Ws, As, Bs = params[0::4], params[1::4], params[2::4]
+        ctx.scales, ctx.thresholds = [float(s) for s in params[3::4]], thresholds
+        ctx.ranks = [A.shape[0] for A in As]
+        ctx.rank_p = _pad_rank(max(ctx.ranks))
+        ctx.param_dtypes = [t.dtype for t in (*As, *Bs)]
+        X2 = hip_ops._bf16_rows(X.reshape(-1, X.shape[-1]))
+        Wc = [hip_ops._bf16_rows(W.detach()) for W in Ws]
+        out, *saved = cops.lora_dropout_mlp_fwd(X2, Wc, list(As), list(Bs), ctx.scales, ctx.rank_p,
+                                                seed, thresholds)
+        ctx.save_for_backward(X2, seed, *saved, *Wc)
+        ctx.orig_shape = X.shape
+        return out.view(*X.shape[:-1], out.shape[-1])
+
+    @staticmethod
+    def backward(ctx, dY):
+        X2, seed, gate, up, h, xa, xa_d, packed, *Ws = ctx.saved_tensors
+        (rg, ru, rd), rp, dtypes = ctx.ranks, ctx.rank_p, ctx.param_dtypes
+        dy = hip_ops._bf16_rows(dY.reshape(-1, dY.shape[-1]))
+        H, I = X2.shape[1], gate.shape[1]  # noqa: E741
+        parts = [(0, 0, rg, H), (0, rp, ru, H), (1, 0, rd, I), (2, 0, I, rg), (3, 0, I, ru),
+                 (4, 0, dy.shape[1], rd)]
+        spec, unpack = _grad_spec(hip_ops.lora_mlp_grad_shapes(H, I, rp), parts, dtypes)
+        dX, flat = cops.lora_dropout_mlp_bwd(X2, gate, up, h, dy, Ws, packed, ctx.scales, xa, xa_d,
+                                             rp, seed, ctx.thresholds, spec if unpack else [],
+                                             dtypes[0] if unpack else torch.float32)
+        grads = _unpacked_views(flat, spec) if unpack else \
+            [g.to(t) for g, t in zip(_grad_views(flat, spec), dtypes)]
+        out = [dX.view(*ctx.orig_shape), None, None]
+        for A, B in zip(grads[:3], grads[3:]):
+            out += [None, A, B, None]
+        return tuple(out)
+
+
 def _drop_threshold(linear) -> int:
     """The dropout threshold of a PEFT LoRA Linear's first adapter: 0 in eval mode,
     where it has none (nn.Identity), and without the attribute."""
@@ -578,7 +618,7 @@ def apply_fused_lora_mlp(mlp_module, X: torch.Tensor, lora_dropout: bool = False
     own forward when any projection has no LoRA adapter.
 
     lora_dropout, seed: as in apply_fused_lora_qkv (streams 0, 1, 2 for gate, up,
-    down); the block is then gate and up together, SwiGLU, and down."""
+    down)."""
     GW, GA, GB, GS = _get_lora_params(mlp_module.gate_proj)
     UW, UA, UB, US = _get_lora_params(mlp_module.up_proj)
     DW, DA, DB, DS = _get_lora_params(mlp_module.down_proj)
@@ -586,15 +626,20 @@ def apply_fused_lora_mlp(mlp_module, X: torch.Tensor, lora_dropout: bool = False
     if GA is None or UA is None or DA is None:
         return mlp_module(X)
 
-    projections = [mlp_module.gate_proj, mlp_module.up_proj, mlp_module.down_proj]
-    if lora_dropout and any(_drop_threshold(m) for m in projections):
-        hip_ops.ensure_rocm_device(X)
-        seed = seed_tensor(seed, X.device)
-        gate, up = _dropped(projections[:2], X, seed, 0, (GW, GA, GB, GS, UW, UA, UB, US)) or (
-            apply_fused_lora_linear(m, X) for m in projections[:2])
-        h = fused_swiglu(gate, up)
-        down = _dropped(projections[2:], h, seed, 2, (DW, DA, DB, DS))
-        return down[0] if down is not None else _LoRA_W.apply(h, DW, DA, DB, DS)
+    if lora_dropout:
+        projections = [mlp_module.gate_proj, mlp_module.up_proj, mlp_module.down_proj]
+        thresholds = tuple(_drop_threshold(m) for m in projections)
+        if any(thresholds):
+            _check_float(X, "LoRA MLP")
+            hip_ops.ensure_rocm_device(X)
+            seed = seed_tensor(seed, X.device)
+            if not _fp32_path(X, X.shape[-1], GW.shape[0], DW.shape[0]) \
+                    and max(GA.shape[0], UA.shape[0], DA.shape[0]) <= 64:
+                return _LoRA_Dropout_MLP.apply(X, seed, thresholds, GW, GA, GB, GS, UW, UA, UB, US,
+                                               DW, DA, DB, DS)
+            gate, up = _LoRA_Dropout.apply(X, seed, thresholds[:2], 0, GW, GA, GB, GS, UW, UA, UB, US)
+            return _LoRA_Dropout.apply(fused_swiglu(gate, up), seed, thresholds[2:], 2,
+                                       DW, DA, DB, DS)[0]
     return _LoRA_MLP.apply(
         X,
         GW, GA, GB, GS,
