@@ -18,6 +18,8 @@ between replays gives each its own masks. An int is the same mask at each call.
 
 from __future__ import annotations
 
+import operator
+
 import torch
 import torch.nn as nn
 
@@ -32,7 +34,7 @@ def seed_tensor(seed, device) -> torch.Tensor:
         return torch.randint(-(2 ** 63), 2 ** 63 - 1, (1,), dtype=torch.int64, device=device)
     if isinstance(seed, torch.Tensor):
         return seed
-    wrapped = (int(seed) + 2 ** 63) % 2 ** 64 - 2 ** 63
+    wrapped = (operator.index(seed) + 2 ** 63) % 2 ** 64 - 2 ** 63
     return torch.full((1,), wrapped, dtype=torch.int64, device=device)
 
 
@@ -75,12 +77,15 @@ def fused_dropout(x: torch.Tensor, p: float = 0.5, training: bool = True,
 
 
 class MetalLigerDropout(nn.Module):
-    """Drop-in for nn.Dropout; forward also takes a residual to add."""
+    """Drop-in for nn.Dropout; forward also takes a residual to add. (There is no
+    in-place form: inplace=True is refused.)"""
 
-    def __init__(self, p: float = 0.5):
+    def __init__(self, p: float = 0.5, inplace: bool = False):
         super().__init__()
         hip_ops.drop_threshold(p)
-        self.p = p
+        if inplace:
+            raise ValueError("MetalLigerDropout: inplace is not supported")
+        self.p, self.inplace = p, False
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
         return fused_dropout(x, self.p, self.training, residual)

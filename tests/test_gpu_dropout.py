@@ -136,6 +136,26 @@ def test_module_and_checkpointing(dev):
     assert torch.equal(drop(x, residual=x), x + x)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [4099, 4096])
+def test_in_place_through_the_c_abi(dev, dtype, n):
+    """out may be x or residual, aligned or not; what lies behind stays as it was."""
+    from metal_liger_amd import _hip
+    for shift in (0, 1):
+        buf = [seeded((n + 16,), k, dtype).to(dev) for k in (1, 2)]
+        seed = torch.tensor([4], device=dev)
+        x, res = (b[shift:shift + n] for b in buf)
+        want = _op()(x, 0.3, residual=res, seed=4)
+        for out in (0, 1):
+            t = [b.clone() for b in buf]
+            p = [b[shift:].data_ptr() for b in t]
+            _hip.call("ml_dropout", p[0], p[1], p[out], n, 19661, 65536 / (65536 - 19661),
+                      seed.data_ptr(), 0, _hip.DTYPE_TAG[dtype], _hip.stream_of(seed))
+            assert torch.equal(t[out][shift:shift + n], want)
+            assert torch.equal(t[out][shift + n:], buf[out][shift + n:])
+            assert torch.equal(t[1 - out], buf[1 - out])
+
+
 def test_other_stream(dev):
     x = seeded((512, 512), 8).to(dev)
     want = _op()(x, 0.3, seed=1)

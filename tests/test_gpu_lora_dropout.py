@@ -190,18 +190,30 @@ def test_entry_points_and_streams(dev):
         assert torch.equal(a, b)
 
 
-@pytest.mark.parametrize("dtype, tol", [(F32, 2e-5), (BF, 2e-2)])
-def test_mlp(dev, dtype, tol):
+def _mlp(dev, dtype, ranks, ps, H=256, I=512, adapter=None):  # noqa: E741
+    shapes = ((H, I), (H, I), (I, H))
+    lins = [_linear(dev, i, o, r, p, dtype, 10 * k, adapter)
+            for k, ((i, o), r, p) in enumerate(zip(shapes, ranks, ps))]
+    return lins, _block(gate_proj=lins[0], up_proj=lins[1], down_proj=lins[2])
+
+
+@pytest.mark.parametrize("dtype, tokens, ranks, ps", [
+    (F32, 300, (16, 16, 16), (0.2, 0.2, 0.2)), (BF, 300, (16, 16, 16), (0.2, 0.2, 0.2)),
+    (BF, 1, (8, 8, 8), (0.5, 0.5, 0.5)), (BF, 777, (32, 16, 12), (0.1, 0.3, 0.2)),
+    (BF, 65, (64, 64, 64), (0.1, 0.1, 0.1)), (BF, 130, (96, 16, 16), (0.2, 0.1, 0.3)),
+    (BF, 200, (16, 16, 16), (0.0, 0.0, 0.4)), (BF, 200, (16, 16, 16), (0.4, 0.0, 0.0)),
+    (torch.float16, 90, (8, 8, 8), (0.2, 0.2, 0.2))])
+def test_mlp(dev, dtype, tokens, ranks, ps):
     """The MLP block: streams 0, 1, 2 for gate, up, down. Its inner tensors are
     rounded to the activation dtype, so that the norms of the errors are compared:
-    about ten roundings of eps / 2 each in bf16, sums of 256 to 512 terms in fp32."""
+    about ten roundings of eps / 2 each in bf16 and fp16's fp32 products (rounded
+    between), sums of 256 to 512 terms in fp32."""
     from metal_liger_amd import apply_fused_lora_mlp
-    H, I, N = 256, 512, 300  # noqa: E741
-    shapes = ((H, I), (H, I), (I, H))
-    lins = [_linear(dev, i, o, 16, 0.2, dtype, 10 * k) for k, (i, o) in enumerate(shapes)]
-    mlp = _block(gate_proj=lins[0], up_proj=lins[1], down_proj=lins[2])
-    x = seeded((N, H), 1, dtype)
-    dy = seeded((N, H), 2, dtype)
+    tol = {F32: 2e-5, BF: 2e-2, torch.float16: 2.5e-3}[dtype]
+    lins, mlp = _mlp(dev, dtype, ranks, ps, adapter=F32 if dtype == torch.float16 else None)
+    H = 256
+    x = seeded((tokens, H), 1, dtype)
+    dy = seeded((tokens, H), 2, dtype)
     xd = x.to(dev).requires_grad_()
     adapters = [t for m in lins for t in (m.lora_A["default"].weight, m.lora_B["default"].weight)]
     y = apply_fused_lora_mlp(mlp, xd, lora_dropout=True, seed=11)
@@ -215,11 +227,129 @@ def test_mlp(dev, dtype, tol):
         a, b = (v.double().requires_grad_() for v in (a, b))
         leaves += [a, b]
         t = out[0] * torch.sigmoid(out[0]) * out[1] if k == 2 else x64
-        f = ref.dropout_factors(tuple(t.shape), 0.2, 11, k)
+        f = ref.dropout_factors(tuple(t.shape), ps[k], 11, k)
         out.append(t @ w.double().t() + s * ((t * f) @ a.t()) @ b.t())
     want = [out[2], *torch.autograd.grad(out[2], [x64, *leaves], dy.double())]
+    assert y.dtype == dtype and [g.dtype for g in got[2:]] == [t.dtype for t in adapters]
     for g, w in zip(got, want):
         assert (g.double().cpu() - w).norm() <= tol * w.norm()
+
+
+def test_mlp_without_dropout_is_the_plain_block(dev):
+    from metal_liger_amd import apply_fused_lora_mlp
+    _, mlp = _mlp(dev, BF, (16, 16, 16), (0.3, 0.3, 0.3))
+    x = seeded((70, 256), 1, BF).to(dev)
+    want = apply_fused_lora_mlp(mlp, x)
+    assert not torch.equal(apply_fused_lora_mlp(mlp, x, lora_dropout=True), want)
+    assert torch.equal(apply_fused_lora_mlp(mlp.eval(), x, lora_dropout=True), want)
+
+
+def test_mlp_empty_batch(dev):
+    from metal_liger_amd import apply_fused_lora_mlp
+    lins, mlp = _mlp(dev, BF, (16, 16, 16), (0.3, 0.3, 0.3))
+    x = torch.empty(0, 256, dtype=BF, device=dev, requires_grad=True)
+    y = apply_fused_lora_mlp(mlp, x, lora_dropout=True)
+    dx, db = torch.autograd.grad(y, [x, lins[2].lora_B["default"].weight], torch.empty_like(y))
+    assert y.shape == dx.shape == (0, 256) and not db.any()
+
+
+def test_dropped_infinities_stay_out_of_the_adapters(dev):
+    """An element that every mask drops reaches no adapter, whatever it holds: XA and
+    dA are those of a zero there."""
+    from metal_liger_amd import hip_ops
+    lins = [_linear(dev, 256, 64, 16, 0.5, BF, 10 * k) for k in range(2)]
+    x = seeded((40, 256), 1, BF).to(dev)
+    fs = [ref.dropout_factors((40, 256), 0.5, 21, k) for k in range(2)]
+    gone = ((fs[0] == 0) & (fs[1] == 0)).to(dev)
+    bad = torch.where(gone, torch.tensor(float("inf"), dtype=BF, device=dev), x)
+    zero = torch.where(gone, torch.zeros((), dtype=BF, device=dev), x)
+    seed = torch.tensor([21], device=dev)
+    args = [[m.base_layer.weight.detach() for m in lins],
+            [m.lora_A["default"].weight.detach() for m in lins],
+            [m.lora_B["default"].weight.detach() for m in lins], [2.0, 2.0], 16, seed,
+            [32768, 32768], 0]
+    (*_, xa, packed), (*_, xa0, _) = (hip_ops.lora_dropout_fwd(t, *args) for t in (bad, zero))
+    assert torch.equal(xa, xa0)
+    dys = [seeded((40, 64), 2, BF).to(dev)] * 2
+    _, g = hip_ops.lora_dropout_bwd(bad, dys, args[0], packed, [2.0, 2.0], xa, 16, seed,
+                                    [32768, 32768], 0, [], BF)
+    _, g0 = hip_ops.lora_dropout_bwd(zero, dys, args[0], packed, [2.0, 2.0], xa, 16, seed,
+                                     [32768, 32768], 0, [], BF)
+    assert torch.equal(g, g0)
+
+
+@pytest.mark.parametrize("rank", [16, 96])
+def test_strided_and_misaligned_operands(dev, rank):
+    from metal_liger_amd.ops.fused_lora import _LoRA_Dropout
+    lin = _linear(dev, 128, 64, rank, 0.3, BF, 0)
+    seed = torch.tensor([4], device=dev)
+    base = seeded((60, 300), 1, BF).to(dev)
+    dys = seeded((60, 200), 2, BF).to(dev)
+    w, a, b, s = (lin.base_layer.weight, lin.lora_A["default"].weight,
+                  lin.lora_B["default"].weight, 2.0)
+
+    def step(x, dy, w):
+        x = x.detach().requires_grad_()
+        y, = _LoRA_Dropout.apply(x, seed, (19661,), 0, w, a, b, s)
+        return [y, *torch.autograd.grad(y, [x, a, b], dy)]
+
+    x, dy = base[:, 3:131], dys[:, 5:69]
+    want = step(x.contiguous(), dy.contiguous(), w)
+    wide = torch.zeros(64, 140, dtype=BF, device=dev)
+    wide[:, 1:129] = w.detach()
+    for args in ((x, dy, w), (x.t().contiguous().t(), dy, w), (x, dy, wide[:, 1:129])):
+        for got, ref_ in zip(step(*args), want):
+            assert torch.equal(got, ref_)
+
+
+def test_compile_and_opcheck(dev):
+    from metal_liger_amd import _custom_ops as cops
+    from metal_liger_amd import apply_fused_lora_mlp, apply_fused_lora_qkv, hip_ops
+    lins = [_linear(dev, 128, o, 16, 0.4, BF, 10 * k) for k, o in enumerate((128, 64, 64))]
+    attn = _block(q_proj=lins[0], k_proj=lins[1], v_proj=lins[2])
+    mlp_lins, mlp = _mlp(dev, BF, (16, 16, 16), (0.3, 0.3, 0.3), 128, 256)
+    x = seeded((50, 128), 1, BF).to(dev).requires_grad_()
+    seed = torch.tensor([7], device=dev)
+    for fn, ms in ((lambda t: apply_fused_lora_qkv(attn, t, lora_dropout=True, seed=seed), lins),
+                   (lambda t: (apply_fused_lora_mlp(mlp, t, lora_dropout=True, seed=seed),),
+                    mlp_lins)):
+        leaves = [x, *(w for m in ms for w in (m.lora_A["default"].weight,
+                                              m.lora_B["default"].weight))]
+        want = fn(x)
+        got = torch.compile(fn, fullgraph=True, backend="aot_eager")(x)
+        dys = [seeded(tuple(y.shape), 3, BF).to(dev) for y in want]
+        for p, q in zip([*got, *torch.autograd.grad(got, leaves, dys)],
+                        [*want, *torch.autograd.grad(want, leaves, dys)]):
+            assert torch.equal(p, q)
+    checks = ("test_schema", "test_faketensor", "test_aot_dispatch_dynamic")
+    xd = x.detach()
+    for rank, fwd, bwd in ((16, cops.lora_dropout_fwd, cops.lora_dropout_bwd),
+                           (72, cops.lora_dropout_wide_fwd, cops.lora_dropout_wide_bwd)):
+        m = _linear(dev, 128, 64, rank, 0.4, BF, 3)
+        args = (xd, [m.base_layer.weight.detach()], [m.lora_A["default"].weight.detach()],
+                [m.lora_B["default"].weight.detach()], [2.0], rank, seed, [1000], 1)
+        torch.library.opcheck(fwd, args, test_utils=checks)
+        y, xa, packed = fwd(*args)
+        for spec in ([], [0, rank, 128, 128]):
+            torch.library.opcheck(bwd, (xd, [y], args[1], packed, [2.0], xa, rank, seed, [1000], 1,
+                                        spec, BF), test_utils=checks)
+    args = (xd, [m.base_layer.weight.detach() for m in mlp_lins],
+            [m.lora_A["default"].weight.detach() for m in mlp_lins],
+            [m.lora_B["default"].weight.detach() for m in mlp_lins], [2.0] * 3, 16, seed, [1000] * 3)
+    torch.library.opcheck(cops.lora_dropout_mlp_fwd, args, test_utils=checks)
+    y, gate, up, h, xa, xa_d, packed = cops.lora_dropout_mlp_fwd(*args)
+    torch.library.opcheck(cops.lora_dropout_mlp_bwd,
+                          (xd, gate, up, h, y, args[1], packed, [2.0] * 3, xa, xa_d, 16, seed,
+                           [1000] * 3, [], BF), test_utils=checks)
+    f32 = [t.float() for t in (xd, lins[0].base_layer.weight.detach(),
+                               lins[0].lora_A["default"].weight.detach(),
+                               lins[0].lora_B["default"].weight.detach())]
+    args = (f32[0], [f32[1]], [f32[2]], [f32[3]], [2.0], seed, [1000], 0)
+    torch.library.opcheck(cops.lora_dropout_f32_fwd, args, test_utils=checks)
+    y, xa = cops.lora_dropout_f32_fwd(*args)
+    torch.library.opcheck(cops.lora_dropout_f32_bwd, (f32[0], [y], [f32[1]], [f32[2]], [f32[3]], [2.0],
+                                                      [xa], seed, [1000], 0), test_utils=checks)
+    assert hip_ops.drop_scale(65536) == 0.0
 
 
 def test_drawn_seeds(dev):

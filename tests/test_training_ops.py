@@ -90,6 +90,17 @@ def test_dropout_refuses_rates(p):
         MetalLigerDropout(p)
 
 
+def test_dropout_refuses_inplace_and_seeds_that_are_no_integers():
+    from metal_liger_amd import MetalLigerDropout
+    from metal_liger_amd.ops.fused_dropout import seed_tensor
+    with pytest.raises(ValueError, match="inplace"):
+        MetalLigerDropout(0.1, inplace=True)
+    with pytest.raises(TypeError):
+        seed_tensor(1.5, "cpu")
+    assert seed_tensor(2 ** 64 - 1, "cpu").tolist() == [-1]
+    assert seed_tensor(None, "cpu").dtype == torch.int64
+
+
 def test_dropout_refuses_streams_and_cpu_tensors():
     from metal_liger_amd import fused_dropout
     for stream in (-1, 1 << 32):
@@ -150,8 +161,50 @@ def test_host_side_argument_errors():
     refused(L.ml_embedding_fwd(None, 8, 1, 4096, 4, 4096, 8, 4, 1.0, 0, None), b"null pointer")
     refused(L.ml_embedding_bwd(4096, 8, 1, 4096, 4, 4096, 8, 4, 8, 1.0, 4096, 1 << 20, 0, None),
             b"padding index")
+    refused(L.ml_embedding_bwd(4096, 8, 1, 4096, 4, 4096, 8, 4, -1, 1.0, None, 1 << 20, 0, None),
+            b"workspace")
+    refused(L.ml_embedding_bwd(4096, 8, 1, 4096, 4, 4096, 8, 4, -1, 1.0, 4096, 16, 0, None),
+            b"workspace")
+    refused(L.ml_embedding_bwd(4096, 8, 1, 4096, 4, 4096, 8, 4, -1, 1.0, 4100, 1 << 20, 0, None),
+            b"misaligned")
     refused(L.ml_embedding_bwd(4096, 8, 1, None, 4, 4096, 8, 4, -1, 1.0, 4096, 1 << 20, 0, None),
             b"null pointer")
+
+
+def test_lora_dropout_host_side_argument_errors():
+    from metal_liger_amd import _hip
+    L = _hip.lib()
+    p = 4096  # (never read: every call is refused on the host)
+
+    def xa(n=1, tokens=4, width=64, ldx=64, rank=16, thresholds=(0, 0, 0), first=0, ldo=48, x=p,
+           seed=p):
+        return L.ml_lora_dropout_xa(n, x, tokens, width, ldx, p, rank, _hip.geom(thresholds), seed,
+                                    first, p, ldo, None)
+
+    for kw, text in ((dict(n=4), b"1..3 adapters"), (dict(n=0), b"1..3 adapters"),
+                     (dict(seed=None), b"null pointer"), (dict(thresholds=(65537,)), b"threshold"),
+                     (dict(n=2, thresholds=(0, -1)), b"threshold"), (dict(first=-1), b"stream id"),
+                     (dict(n=2, first=(1 << 32) - 1), b"stream id"), (dict(width=60), b"multiple of 8"),
+                     (dict(rank=24), b"rank 16, 32, 48 or 64"), (dict(rank=80), b"rank 16"),
+                     (dict(ldx=56), b"leading"), (dict(ldo=8), b"leading"),
+                     (dict(x=None), b"null pointer"), (dict(x=p + 2), b"16-byte aligned")):
+        assert xa(**kw) == 1 and text in L.ml_last_error(), (kw, L.ml_last_error())
+
+    def bwd(n=1, tokens=4, width=64, outs=(64, 64, 64), rank=16, dx=p, w=p, ws=p, ws_bytes=1 << 30):
+        ptrs = _hip.ptrs([p] * 3)
+        return L.ml_lora_dropout_bwd(n, p, tokens, width, ptrs, _hip.geom(outs), _hip.ptrs([w] * 3), p,
+                                     ptrs, _hip.floats([1.0] * 3), p, rank, _hip.geom([0] * 3), p, 0,
+                                     dx, p, ptrs, ws, ws_bytes, None)
+
+    for kw, text in ((dict(n=0), b"1..3 adapters"), (dict(tokens=0), b"token count"),
+                     (dict(width=4), b"multiple of 8"), (dict(outs=(60,)), b"multiple of 8"),
+                     (dict(rank=72), b"rank 16"), (dict(dx=None), b"null pointer"),
+                     (dict(w=None), b"null pointer"), (dict(w=p + 8), b"16-byte aligned"),
+                     (dict(dx=p + 2), b"16-byte aligned"), (dict(ws=None), b"workspace"),
+                     (dict(ws_bytes=64), b"workspace"), (dict(ws=p + 4), b"workspace")):
+        assert bwd(**kw) == 1 and text in L.ml_last_error(), (kw, L.ml_last_error())
+    assert L.ml_lora_dropout_bwd_workspace_bytes(4, 4, 64, _hip.geom([64] * 4), 16) == 0
+    assert L.ml_lora_dropout_bwd_workspace_bytes(1, 4, 64, _hip.geom([64]), 72) == 0
 
 
 # ----------------------------------------------------------------- fake kernels
@@ -171,6 +224,16 @@ def test_fake_kernels():
         assert ops.embedding_fwd(ids, e(10, 4), 1.0).shape == (2, 3, 4)
         dw = ops.embedding_bwd(ids, e(2, 3, 4, dtype=F32), 10, -1, 1.0)
         assert dw.shape == (10, 4) and dw.dtype == F32
+        x, ws, As, Bs = e(96, 128), [e(64, 128), e(32, 128)], [e(12, 128), e(16, 128)], [e(64, 12),
+                                                                                       e(32, 16)]
+        for rank, fwd, bwd in ((16, ops.lora_dropout_fwd, ops.lora_dropout_bwd),
+                               (72, ops.lora_dropout_wide_fwd, ops.lora_dropout_wide_bwd)):
+            q, k, xa, packed = fwd(x, ws, As, Bs, [2.0] * 2, rank, seed, [100, 0], 0)
+            assert q.shape == (96, 64) and k.shape == (96, 32) and xa.shape == (96, 2 * rank)
+            assert packed.shape == (rank * (2 * 128 + 2 * 96),)
+            dx, g = bwd(x, [q, k], ws, packed, [2.0] * 2, xa, rank, seed, [100, 0], 0, [], BF)
+            assert dx.shape == (96, 128) and g.dtype == F32
+            assert g.shape == (2 * rank * 128 + 64 * rank + 32 * rank,)
 
 
 # ------------------------------------------------------------------ the patcher
