@@ -495,15 +495,23 @@ int ml_lora_xa(const void* X, int64_t n_tokens, int64_t in_features, int64_t ldx
  * 32, 48 or 64) of every adapter; in_features a multiple of 8.
  *
  * ml_lora_dropout_xa: XA [n_tokens, nadp rank] (row stride ldo), column block i =
- * c_i (M_i X) A_i^T; A_stack [nadp rank, in_features] dense; X of row stride ldx (a
- * multiple of 8). X and A 16-byte aligned.
+ * c_i (M_i X) A_i^T; A_stack as ml_lora_dropout_pack lays down A_0 .. one after
+ * another; X of row stride ldx (a multiple of 8). X and A 16-byte aligned.
+ *
+ * ml_lora_dropout_pack: ml_lora_pack with the first nadp matrices (the A_i, padded to
+ * rank rows and to a multiple of 32 columns) in the order of the kernels' operands: for
+ * every 32 columns and 16 rows of those, 64 times 8 elements, the l-th of row l mod 16,
+ * columns 8 (l div 16) .. of the block; A_i takes rank times the padded columns.
  *
  * ml_lora_dropout_bwd: as ml_lora_qkv_bwd, XA being ml_lora_dropout_xa's:
  *   dX   = sum_i dY_i W_i + M_i (P_i A_i),  P_i = c_i s_i dY_i B_i  (P in bf16; the
  *          sum of the dY_i W_i is rounded to bf16 before the adapters' part is added)
  *   dA_i = P_i^T (M_i X)        dB_i = s_i dY_i^T XA_i
- * every operand dense and 16-byte aligned.
+ * A_stack as above, every other operand dense; all 16-byte aligned.
  */
+int ml_lora_dropout_pack(int count, int nadp, const void* const* src, const int64_t* geometry,
+                         const int* dtypes, const float* scales, void* const* dst,
+                         void* const* scaled, void* stream);
 int ml_lora_dropout_xa(int nadp, const void* X, int64_t n_tokens, int64_t in_features, int64_t ldx,
                        const void* A_stack, int64_t rank, const int64_t* thresholds,
                        const int64_t* seed, int64_t first_stream, void* XA, int64_t ldo,

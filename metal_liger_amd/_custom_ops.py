@@ -367,10 +367,20 @@ lora_unpack = _define("lora_unpack(Tensor flat, SymInt[] spec, ScalarType dtype)
                       hip_ops.lora_unpack, _lora_unpack_fake)
 
 
+def _lora_pack_frag_fake(As, Bs, rank):
+    n = rank * (sum(hip_ops.frag_cols(a.shape[1]) for a in As) + 2 * sum(b.shape[0] for b in Bs))
+    return As[0].new_empty((n,), dtype=torch.bfloat16)
+
+
 def _lora_dropout_fwd_fake(x2, ws, As, Bs, scales, rank, seed, thresholds, first):
     new = lambda *s: x2.new_empty(s, dtype=torch.bfloat16)  # noqa: E731
     return [*(new(x2.shape[0], w.shape[0]) for w in ws), new(x2.shape[0], len(ws) * rank),
-            _lora_pack_fake(As, Bs, scales, rank)]
+            _lora_pack_frag_fake(As, Bs, rank)]
+
+
+def _lora_dropout_wide_fwd_fake(x2, ws, As, Bs, scales, rank, seed, thresholds, first):
+    *outs, _ = _lora_dropout_fwd_fake(x2, ws, As, Bs, scales, rank, seed, thresholds, first)
+    return [*outs, _lora_pack_fake(As, Bs, scales, rank)]
 
 
 def _lora_dropout_bwd_fake(x2, dys, ws, packed, scales, xa, rank, seed, thresholds, first, spec,
@@ -392,7 +402,7 @@ lora_dropout_fwd = _define("lora_dropout_fwd" + _LORA_DROPOUT_FWD, hip_ops.lora_
 lora_dropout_bwd = _define("lora_dropout_bwd" + _LORA_DROPOUT_BWD, hip_ops.lora_dropout_bwd,
                            _lora_dropout_bwd_fake)
 lora_dropout_wide_fwd = _define("lora_dropout_wide_fwd" + _LORA_DROPOUT_FWD,
-                                hip_ops.lora_dropout_wide_fwd, _lora_dropout_fwd_fake)
+                                hip_ops.lora_dropout_wide_fwd, _lora_dropout_wide_fwd_fake)
 lora_dropout_wide_bwd = _define("lora_dropout_wide_bwd" + _LORA_DROPOUT_BWD,
                                 hip_ops.lora_dropout_wide_bwd, _lora_dropout_bwd_fake)
 
@@ -401,7 +411,7 @@ def _lora_dropout_mlp_fwd_fake(x2, ws, As, Bs, scales, rank, seed, thresholds):
     new = lambda n: x2.new_empty((x2.shape[0], n), dtype=torch.bfloat16)  # noqa: E731
     inter = ws[0].shape[0]
     return [new(ws[2].shape[0]), new(inter), new(inter), new(inter), new(2 * rank), new(rank),
-            _lora_pack_fake(As, Bs, scales, rank)]
+            _lora_pack_frag_fake(As, Bs, rank)]
 
 
 def _lora_dropout_mlp_bwd_fake(x2, gate, up, h, dy, ws, packed, scales, xa, xa_d, rank, seed,

@@ -168,6 +168,11 @@ SIGNATURES: dict[str, tuple] = {
         _i32,
         [_p, _i64, _i64, _p, _i64, _p, _p, _p, _f32, _p, _i64, _p, _p, _p, _p, _sz, _p],
     ),
+    "ml_lora_dropout_pack": (
+        _i32,
+        [_i32, _i32, ctypes.POINTER(_p), _i64p, ctypes.POINTER(_i32), ctypes.POINTER(_f32),
+         ctypes.POINTER(_p), ctypes.POINTER(_p), _p],
+    ),
     "ml_lora_dropout_xa": (
         _i32, [_i32, _p, _i64, _i64, _i64, _p, _i64, _i64p, _p, _i64, _p, _i64, _p],
     ),

@@ -100,7 +100,7 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t d, bool in) {
 }
 
 // Zeros, by one wave in each of `blocks` workgroups. One wave per CU keeps what is
-// being written within 256 KB: 622 MB take 96 us beside the sort, and 85 in a launch
+// being written within 256 KB: 622 MB take 100 us beside the sort, and 85 in a launch
 // of 64-thread workgroups of their own, which would wait for the sort instead; with
 // 512 to 2048 threads per CU, 105 to 140.
 __device__ __forceinline__ void fill_zero(char* p, int64_t bytes, int64_t block, int64_t blocks) {

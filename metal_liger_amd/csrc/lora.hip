@@ -943,11 +943,22 @@ struct PackJob {
   int64_t ld;
   int rows, cols, drows, dcols, dtype;
   float scale;
+  int frag;  // dst in fragment order
 };
 constexpr int kMaxPack = 6;
 struct PackArgs {
   PackJob job[kMaxPack];
 };
+
+// Where 8 elements of row r from column c lie in fragment order: what a wave's lanes
+// hold of 16 rows and 32 columns in the MFMA operand layout (lane l: row l % 16,
+// columns 8 (l / 16) ..) is 1 KB in one piece, the rows' 16-row slices of a 32-column
+// step behind one another. A wave's load of a fragment is then a row of memory instead
+// of 16 pieces of 64 bytes (X A^T under dropout, [1777, 6144] x 32: 18.5 -> 13.3 us).
+__device__ __forceinline__ int64_t frag_offset(int r, int c, int rows) {
+  const int lane = (r & 15) + 16 * ((c >> 3) & 3);
+  return (((int64_t)(c >> 5) * (rows >> 4) + (r >> 4)) * 64 + lane) * 8;
+}
 
 template <typename T>
 __device__ __forceinline__ void pack_load(const PackJob& j, int r, int c, float (&x)[8]) {
@@ -979,7 +990,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const PackArgs args) {
       x[k] = to_f32(from_f32<bf16>(x[k]));
       y[k] = j.scale * x[k];
     }
-    const int64_t o = (int64_t)r * j.dcols + c;
+    const int64_t o = j.frag ? frag_offset(r, c, j.drows) : (int64_t)r * j.dcols + c;
     store_n<bf16, 8>(j.dst + o, x);
     if (j.scaled) store_n<bf16, 8>(j.scaled + o, y);
   }
@@ -1118,9 +1129,9 @@ using namespace mla::gemm;
 
 // ---------------------------------------------------------- adapter pack --
 
-extern "C" int ml_lora_pack(int count, const void* const* src, const int64_t* geometry,
-                            const int* dtypes, const float* scales, void* const* dst,
-                            void* const* scaled, void* stream) {
+static int pack_matrices(int count, int nfrag, const void* const* src, const int64_t* geometry,
+                         const int* dtypes, const float* scales, void* const* dst,
+                         void* const* scaled, void* stream) {
   ML_CHECK(count >= 1 && count <= lora::kMaxPack, "lora pack: 1..%d matrices (got %d)",
            lora::kMaxPack, count);
   ML_CHECK(src && geometry && dtypes && scales && dst && scaled, "lora pack: null argument arrays");
@@ -1131,13 +1142,15 @@ extern "C" int ml_lora_pack(int count, const void* const* src, const int64_t* ge
     ML_CHECK(g[0] >= 0 && g[1] >= 0 && g[2] >= g[1] && g[3] >= g[0] && g[4] >= g[1] &&
                  g[4] % 8 == 0 && g[3] < (1LL << 31) && g[4] < (1LL << 31),
              "lora pack: bad geometry of matrix %d", i);
+    ML_CHECK(i >= nfrag || (g[3] % 16 == 0 && g[4] % 32 == 0),
+             "lora pack: matrix %d in fragment order needs 16 x 32 blocks", i);
     ML_CHECK(dtypes[i] == ML_F32 || dtypes[i] == ML_BF16 || dtypes[i] == ML_F16,
              "lora pack: matrix %d must be fp32, bf16 or fp16", i);
     ML_CHECK(dst[i] && aligned16(dst[i]) && aligned16(scaled[i]) && (src[i] || g[0] * g[1] == 0),
              "lora pack: null or misaligned pointer for matrix %d", i);
     a.job[i] = lora::PackJob{src[i], static_cast<bf16*>(dst[i]), static_cast<bf16*>(scaled[i]),
                              g[2], (int)g[0], (int)g[1], (int)g[3], (int)g[4], dtypes[i],
-                             scales[i]};
+                             scales[i], i < nfrag};
     most = std::max(most, g[3] * (g[4] / 8));
   }
   if (most == 0) return ML_OK;
@@ -1145,6 +1158,21 @@ extern "C" int ml_lora_pack(int count, const void* const* src, const int64_t* ge
   lora::pack_kernel<<<dim3((unsigned)blocks, (unsigned)count), 256, 0, (hipStream_t)stream>>>(a);
   ML_LAUNCH_CHECK();
   return ML_OK;
+}
+
+extern "C" int ml_lora_pack(int count, const void* const* src, const int64_t* geometry,
+                            const int* dtypes, const float* scales, void* const* dst,
+                            void* const* scaled, void* stream) {
+  return pack_matrices(count, 0, src, geometry, dtypes, scales, dst, scaled, stream);
+}
+
+extern "C" int ml_lora_dropout_pack(int count, int nadp, const void* const* src,
+                                    const int64_t* geometry, const int* dtypes,
+                                    const float* scales, void* const* dst, void* const* scaled,
+                                    void* stream) {
+  ML_CHECK(nadp >= 0 && nadp <= count, "lora pack: %d of %d matrices in fragment order", nadp,
+           count);
+  return pack_matrices(count, nadp, src, geometry, dtypes, scales, dst, scaled, stream);
 }
 
 extern "C" int ml_lora_unpack(int count, const float* const* src, const int64_t* geometry,

@@ -15,6 +15,16 @@
 
 constexpr int kDropMaxAdapters = 3;
 
+// A_i is packed in fragment order (frag_offset): its elements, and the fragment of
+// 16-rank slice r at columns 32 s ...
+__host__ __device__ inline int64_t frag_size(int rank, int K) {
+  return (int64_t)rank * ((K + 31) / 32 * 32);
+}
+template <int RS>
+__device__ __forceinline__ bf16x8_t frag_of(const bf16* A, int s, int r, int lane) {
+  return *reinterpret_cast<const bf16x8_t*>(A + ((int64_t)(s * RS + r) * 64 + lane) * 8);
+}
+
 struct DropRates {
   DropRate rate[kDropMaxAdapters];
   uint32_t stream[kDropMaxAdapters];
@@ -26,8 +36,8 @@ __device__ __forceinline__ bf16x8_t masked8(u32x4_t x, u32x4_t m) {
 }
 
 // ----------------------------------------------------------------- forward --
-// As xa_kernel (16 MT rows a workgroup, eight waves splitting K, operands loaded in
-// the MFMA layout), with every 8 elements of X that a lane holds masked once for each
+// As xa_kernel (16 MT rows a workgroup, eight waves splitting K, X loaded in the MFMA
+// layout and A lying in it), with every 8 elements of X that a lane holds masked once for each
 // of NA adapters: a lane's operand is one counter's block of 8 elements, so that a mask
 // costs one Philox call. RS 16-rank tiles per adapter; blockIdx.y takes the next NA.
 template <int NA, int RS, int MT>
@@ -39,7 +49,7 @@ __global__ __launch_bounds__(64 * kXaWaves) void drop_xa_kernel(
   constexpr int W = 16 * MT * 16 * NT;  // one wave's sums
   __shared__ float red[kXaWaves * W];
   const int ad0 = blockIdx.y * NA;
-  A += (int64_t)ad0 * 16 * RS * K;
+  A += ad0 * frag_size(16 * RS, K);
   XA += ad0 * 16 * RS;
   const DropKey key = drop_key(seed);
   const int tid = threadIdx.x, lane = tid & 63;
@@ -75,8 +85,9 @@ __global__ __launch_bounds__(64 * kXaWaves) void drop_xa_kernel(
 #pragma unroll
       for (int t = 0; t < MT; ++t) a[u][t] = *reinterpret_cast<const u32x4_t*>(xp[t] + kc[u]);
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-        b[u][j] = *reinterpret_cast<const bf16x8_t*>(A + (int64_t)(16 * j + lr) * K + kc[u]);
+      for (int j = 0; j < NT; ++j)  // zeros past K
+        b[u][j] = frag_of<RS>(A + j / RS * frag_size(16 * RS, K), s0 + u < ke ? s0 + u : kb, j % RS,
+                              lane);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -91,7 +102,7 @@ __global__ __launch_bounds__(64 * kXaWaves) void drop_xa_kernel(
 #pragma unroll
           for (int r = 0; r < RS; ++r)
             acc[t][i * RS + r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                xm, ok[u] ? b[u][i * RS + r] : bf16x8_t{}, acc[t][i * RS + r], 0, 0, 0);
+                xm, b[u][i * RS + r], acc[t][i * RS + r], 0, 0, 0);
         }
       }
     }
@@ -208,18 +219,18 @@ __global__ __launch_bounds__(64 * kDbWaves) void drop_bwd_kernel(
   const bool okc = cc < IN;  // IN % 8 == 0: a lane's columns are all inside or all outside
   const int ccl = okc ? cc : 0;
 
-  // A fragments of the wave's columns: lane (m = lane % 16, k = 4 (lane / 16) + j)
+  // A fragments of the wave's columns, lane (m = lane % 16, k = 4 (lane / 16) + j): the
+  // packed ones (rank = lane % 16, 8 columns) laid down in LDS and read transposed
   i16x4_t af[S][2];
 #pragma unroll
   for (int s = 0; s < S; ++s)
+    *reinterpret_cast<bf16x8_t*>(pl + s * kPBytes + lr * 64 + lg * 16) =
+        frag_of<RS>(A + s / RS * frag_size(16 * RS, IN), c0 / kDbCols, s % RS, lane);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = c0 + 8 * (lr >> 2) + 4 * h + (lr & 3);
+  for (int s = 0; s < S; ++s)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        af[s][h][j] = c < IN ? __builtin_bit_cast(short, A[(int64_t)(16 * s + 4 * lg + j) * IN + c])
-                             : (short)0;
-    }
+    for (int h = 0; h < 2; ++h)
+      af[s][h] = tr_read(pl + s * kPBytes + (4 * lg + (lr >> 2)) * 64 + (lr & 3) * 16 + 8 * h);
 
   // LDS offsets: this lane's 16 bytes of masked X (rows lr and lr + 16: the same chunk
   // swizzle), the transposing reads of X (two column tiles, two groups of 4 rows) and

@@ -990,11 +990,17 @@ def check_adapters(ins, ws, As, Bs) -> None:
                              f"{tuple(w)} do not fit {n} input features")
 
 
-def lora_pack(As, Bs, scales, rank: int) -> torch.Tensor:
+def frag_cols(n: int) -> int:
+    """Columns of an A_i of n input features in the order of the masked passes."""
+    return -(-n // 32) * 32
+
+
+def lora_pack(As, Bs, scales, rank: int, frag: bool = False) -> torch.Tensor:
     """The adapters' parameters in bf16 with ranks padded by zeros to `rank`,
     in one buffer and one launch: every A_i [rank, in_i], then every B_i
     [out_i, rank], then every s_i B_i. A_i [r_i, in_i], B_i [out_i, r_i] of any
-    float dtype; in_i and out_i multiples of 8."""
+    float dtype; in_i and out_i multiples of 8. frag: the A_i as the masked passes
+    read them (ml_lora_dropout_pack), of frag_cols(in_i) columns."""
     dev = ensure_rocm_device(*As, *Bs)
     srcs, dims, tags = [], [], []
     for i, t in enumerate((*As, *Bs)):
@@ -1004,7 +1010,8 @@ def lora_pack(As, Bs, scales, rank: int) -> torch.Tensor:
             t = t.contiguous()
         r, c = t.shape
         srcs.append(t)
-        dims += (r, c, max(t.stride(0), c), *((rank, c) if i < len(As) else (r, rank)))
+        pad = (rank, frag_cols(c) if frag else c) if i < len(As) else (r, rank)
+        dims += (r, c, max(t.stride(0), c), *pad)
         tags.append(_hip.DTYPE_TAG[t.dtype])
     sizes = [dims[5 * i + 3] * dims[5 * i + 4] for i in range(len(srcs))]
     n_a, n_all = sum(sizes[:len(As)]), sum(sizes)
@@ -1014,8 +1021,9 @@ def lora_pack(As, Bs, scales, rank: int) -> torch.Tensor:
         dst.append(base + 2 * off)
         off += n
     scaled = [None] * len(As) + [p + 2 * (n_all - n_a) for p in dst[len(As):]]
-    call("ml_lora_pack", len(srcs), _hip.ptrs([t.data_ptr() for t in srcs]), geom(dims),
-         _hip.ints(tags), _hip.floats([1.0] * len(As) + list(scales)), _hip.ptrs(dst),
+    name, head = ("ml_lora_dropout_pack", (len(srcs), len(As))) if frag else ("ml_lora_pack",
+                                                                             (len(srcs),))
+    call(name, *head, _hip.ptrs([t.data_ptr() for t in srcs]), geom(dims), _hip.ints(tags), _hip.floats([1.0] * len(As) + list(scales)), _hip.ptrs(dst),
          _hip.ptrs(scaled), stream_of(flat))
     return flat
 
@@ -1148,9 +1156,9 @@ def lora_qkv_fwd(x2: torch.Tensor, ws, As, Bs, scales, rank: int):
 
 
 def _packed_ptrs(packed, ins, outs, rank: int):
-    """The addresses of lora_pack's A_i, B_i and s_i B_i."""
+    """The addresses of lora_pack's A_i, B_i and s_i B_i (frag)."""
     at, ptrs = packed.data_ptr(), []
-    for n in (*ins, *outs, *outs):
+    for n in (*(frag_cols(i) for i in ins), *outs, *outs):
         ptrs.append(at)
         at += 2 * rank * n
     n = len(ins)
@@ -1178,7 +1186,7 @@ def lora_dropout_fwd(x2: torch.Tensor, ws, As, Bs, scales, rank: int, seed: torc
     check_seed(seed)
     x2 = _al16(x2)
     ws = [_al16(w) for w in ws]
-    packed = lora_pack(As, Bs, scales, rank)
+    packed = lora_pack(As, Bs, scales, rank, frag=True)
     a_ptrs, _, sbs = _packed_ptrs(packed, ins, [w.shape[0] for w in ws], rank)
     xa = _drop_xa(x2, a_ptrs[0], n, rank, seed, thresholds, first)
     if n > 1:
@@ -1237,7 +1245,7 @@ def lora_dropout_mlp_fwd(x2, ws, As, Bs, scales, rank: int, seed, thresholds) ->
     check_seed(seed)
     x2 = _al16(x2)
     ws = [_al16(w) for w in ws]
-    packed = lora_pack(As, Bs, scales, rank)
+    packed = lora_pack(As, Bs, scales, rank, frag=True)
     a_ptrs, _, sbs = _packed_ptrs(packed, ins, outs, rank)
     xa = _drop_xa(x2, a_ptrs[0], 2, rank, seed, thresholds[:2], 0)
     gate, up = _lora_outs(x2, ws[:2], xa, sbs[:2], [rank] * 2, rank)

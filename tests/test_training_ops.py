@@ -176,6 +176,14 @@ def test_lora_dropout_host_side_argument_errors():
     L = _hip.lib()
     p = 4096  # (never read: every call is refused on the host)
 
+    one = lambda *v: _hip.ptrs(v)  # noqa: E731
+    for nadp, geometry, text in ((2, (16, 64, 64, 16, 64), b"fragment order"),
+                                 (1, (8, 64, 64, 8, 64), b"16 x 32"),
+                                 (1, (16, 40, 40, 16, 40), b"16 x 32")):
+        rc = L.ml_lora_dropout_pack(1, nadp, one(p), _hip.geom(geometry), _hip.ints([1]),
+                                    _hip.floats([1.0]), one(p), one(None), None)
+        assert rc == 1 and text in L.ml_last_error(), L.ml_last_error()
+
     def xa(n=1, tokens=4, width=64, ldx=64, rank=16, thresholds=(0, 0, 0), first=0, ldo=48, x=p,
            seed=p):
         return L.ml_lora_dropout_xa(n, x, tokens, width, ldx, p, rank, _hip.geom(thresholds), seed,
