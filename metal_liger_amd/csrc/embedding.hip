@@ -302,11 +302,12 @@ __global__ __launch_bounds__(kThreads) void sum_chunks(const uint64_t* __restric
     finish();
 }
 
-// The runs that cross chunks: their partials added in the chunks' order. Every workgroup lists the chunks in which such a run begins (a thread a
-// chunk) and takes its share of the (run, column slice) items: a wave sums a run of a
-// few chunks, 256 columns at a time; a long one (an image's or a padding token) takes
-// the workgroup, 64 columns at a time, whose waves add every 16th chunk and meet in LDS
-// in a fixed order.
+// The runs that cross chunks: their partials added in the chunks' order. Every
+// workgroup lists the chunks in which such a run begins (a thread a chunk) and takes
+// its share of the (run, column slice) items: a wave sums a run of a few chunks, 256
+// columns at a time; a long one (an image's or a padding token) takes the workgroup, 64
+// columns at a time, whose waves add every 16th chunk and meet in LDS in a fixed order:
+// 9 us after 8192 tokens of text, 10 where one run covers 700 chunks of 16384 tokens.
 // (A workgroup for every chunk and slice took 39 us where a run covers 700 chunks of
 // 16384 tokens and 7.5 us where it had next to nothing to do.)
 constexpr int kJoinThreads = 1024, kJoinWaves = kJoinThreads / 64, kShortCols = 4;
