@@ -506,7 +506,8 @@ int ml_lora_xa(const void* X, int64_t n_tokens, int64_t in_features, int64_t ldx
  * ml_lora_dropout_bwd: as ml_lora_qkv_bwd, XA being ml_lora_dropout_xa's:
  *   dX   = sum_i dY_i W_i + M_i (P_i A_i),  P_i = c_i s_i dY_i B_i  (P in bf16; the
  *          sum of the dY_i W_i is rounded to bf16 before the adapters' part is added)
- *   dA_i = P_i^T (M_i X)        dB_i = s_i dY_i^T XA_i
+ *   dA_i = P_i^T (M_i X)        dB_i = s_i dY_i^T XA_i   (grad_dtype: ML_F32, or
+ *          ML_BF16: the fp32 sums rounded once; [rank, in] and [out, rank])
  * A_stack as above, every other operand dense; all 16-byte aligned.
  */
 int ml_lora_dropout_pack(int count, int nadp, const void* const* src, const int64_t* geometry,
@@ -522,8 +523,9 @@ int ml_lora_dropout_bwd(int nadp, const void* X, int64_t n_tokens, int64_t in_fe
                         const void* const* dY, const int64_t* out_features, const void* const* W,
                         const void* A_stack, const void* const* B, const float* scale,
                         const void* XA, int64_t rank, const int64_t* thresholds,
-                        const int64_t* seed, int64_t first_stream, void* dX, float* dA,
-                        float* const* dB, void* workspace, size_t workspace_bytes, void* stream);
+                        const int64_t* seed, int64_t first_stream, void* dX, void* dA,
+                        void* const* dB, int grad_dtype, void* workspace, size_t workspace_bytes,
+                        void* stream);
 
 /* Grouped-query attention's key / value heads (no reference counterpart: its
  * models run transformers' attention, whose repeat_kv these replace), for

@@ -383,12 +383,16 @@ def _lora_dropout_wide_fwd_fake(x2, ws, As, Bs, scales, rank, seed, thresholds, 
     return [*outs, _lora_pack_fake(As, Bs, scales, rank)]
 
 
+def _drop_grads_fake(x2, shapes, spec, dtype):
+    n = hip_ops.unpack_layout(spec)[1] if spec else hip_ops.grad_layout(shapes)[1]
+    return x2.new_empty((max(n, 1),), dtype=dtype)
+
+
 def _lora_dropout_bwd_fake(x2, dys, ws, packed, scales, xa, rank, seed, thresholds, first, spec,
                            dtype):
     shapes = hip_ops.lora_dropout_grad_shapes(x2.shape[1], [d.shape[1] for d in dys], rank)
-    grads = x2.new_empty((max(hip_ops.unpack_layout(spec)[1], 1),), dtype=dtype) if spec else \
-        _grads_fake(x2, shapes)
-    return x2.new_empty(x2.shape, dtype=torch.bfloat16), grads
+    return (x2.new_empty(x2.shape, dtype=torch.bfloat16),
+            _drop_grads_fake(x2, shapes, spec, dtype))
 
 
 _LORA_DROPOUT_FWD = ("(Tensor x2, Tensor[] ws, Tensor[] As, Tensor[] Bs, float[] scales, "
@@ -417,9 +421,8 @@ def _lora_dropout_mlp_fwd_fake(x2, ws, As, Bs, scales, rank, seed, thresholds):
 def _lora_dropout_mlp_bwd_fake(x2, gate, up, h, dy, ws, packed, scales, xa, xa_d, rank, seed,
                                thresholds, spec, dtype):
     shapes = hip_ops.lora_mlp_grad_shapes(x2.shape[1], gate.shape[1], rank)
-    grads = x2.new_empty((max(hip_ops.unpack_layout(spec)[1], 1),), dtype=dtype) if spec else \
-        _grads_fake(x2, shapes)
-    return x2.new_empty(x2.shape, dtype=torch.bfloat16), grads
+    return (x2.new_empty(x2.shape, dtype=torch.bfloat16),
+            _drop_grads_fake(x2, shapes, spec, dtype))
 
 
 lora_dropout_mlp_fwd = _define(

@@ -181,7 +181,7 @@ SIGNATURES: dict[str, tuple] = {
         _i32,
         [_i32, _p, _i64, _i64, ctypes.POINTER(_p), _i64p, ctypes.POINTER(_p), _p,
          ctypes.POINTER(_p), ctypes.POINTER(_f32), _p, _i64, _i64p, _p, _i64, _p, _p,
-         ctypes.POINTER(_p), _p, _sz, _p],
+         ctypes.POINTER(_p), _i32, _p, _sz, _p],
     ),
     "ml_lora_mlp_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64]),
     "ml_lora_mlp_bwd": (

@@ -333,8 +333,9 @@ struct DyJob {
   float scale, pscale;  // of dB, of P
   bf16* p;
   int64_t ldp;
-  float* db;
+  void* db;  // fp32, or bf16 where db_f32 is 0
   int64_t lddb;
+  int db_f32 = 1;
 };
 
 // Tile rows of a dY pass over n outputs, `slices` jobs each, and its partials.
@@ -391,7 +392,7 @@ inline int dy_pass(int N, const DyJob* jobs, int n, char* ws, size_t ws_bytes, h
     const DyAdapter& a = args.ad[i];
     red.job[2 * i] = DyReduceJob{a.ppart, a.ctiles, N, j.p, j.ldp, j.pscale, 0};
     red.job[2 * i + 1] =
-        DyReduceJob{a.dbpart, dy_rtiles(N, args.rows), j.O, j.db, j.lddb, j.scale, 1};
+        DyReduceJob{a.dbpart, dy_rtiles(N, args.rows), j.O, j.db, j.lddb, j.scale, j.db_f32};
   }
   dy_reduce_kernel<<<dim3(128, (unsigned)(2 * n)), 256, 0, st>>>(red);
   ML_LAUNCH_CHECK();
@@ -405,7 +406,7 @@ inline int dy_jobs(DyJob* jobs, const DyJob& j, int R) {
     jobs[s].b += s * kDyRank;
     jobs[s].xa += s * kDyRank;
     jobs[s].p += s * kDyRank;
-    jobs[s].db += s * kDyRank;
+    jobs[s].db = static_cast<char*>(j.db) + s * kDyRank * (j.db_f32 ? 4 : 2);
   }
   return R / kDyRank;
 }
@@ -1477,8 +1478,9 @@ extern "C" int ml_lora_dropout_bwd(int nadp, const void* X, int64_t n_tokens, in
                                    const void* const* W, const void* A_stack,
                                    const void* const* B, const float* scale, const void* XA,
                                    int64_t rank, const int64_t* thresholds, const int64_t* seed,
-                                   int64_t first_stream, void* dX, float* dA, float* const* dB,
-                                   void* workspace, size_t workspace_bytes, void* stream) {
+                                   int64_t first_stream, void* dX, void* dA, void* const* dB,
+                                   int grad_dtype, void* workspace, size_t workspace_bytes,
+                                   void* stream) {
   const char* what = "lora dropout";
   lora::DropRates rates{};
   int rc = drop_rates(what, nadp, thresholds, seed, first_stream, rates);
@@ -1488,6 +1490,8 @@ extern "C" int ml_lora_dropout_bwd(int nadp, const void* X, int64_t n_tokens, in
            "%s: in_features must be a positive multiple of 8", what);
   ML_CHECK(rank > 0 && lora::pass_rank(rank), "%s: rank 16, 32, 48 or 64 (got %lld)", what,
            (long long)rank);
+  ML_CHECK(grad_dtype == ML_F32 || grad_dtype == ML_BF16, "%s: gradients in fp32 or bf16 (got %d)",
+           what, grad_dtype);
   ML_CHECK(X && dY && out_features && W && A_stack && B && scale && XA && dX && dA && dB,
            "%s: null pointer", what);
   for (int i = 0; i < nadp; ++i) {
@@ -1518,7 +1522,8 @@ extern "C" int ml_lora_dropout_bwd(int nadp, const void* X, int64_t n_tokens, in
     const int O = (int)out_features[i];
     n += lora::dy_jobs(jobs + n,
                        lora::DyJob{dy, O, O, static_cast<const bf16*>(B[i]), R, xa + i * R, RT,
-                                   scale[i], scale[i] * rates.scale[i], P + i * R, RT, dB[i], R},
+                                   scale[i], scale[i] * rates.scale[i], P + i * R, RT, dB[i], R,
+                                   grad_dtype == ML_F32},
                        R);
     segs[i] = Segment{{dy, O}, {static_cast<const bf16*>(W[i]), IN}, O};
   }
@@ -1527,8 +1532,11 @@ extern "C" int ml_lora_dropout_bwd(int nadp, const void* X, int64_t n_tokens, in
   rc = run_product(N, IN, nadp, segs, kMNMajor, static_cast<bf16*>(dX), IN, 1.0f, 0.0f,
                    reinterpret_cast<float*>(part), part_bytes, st);
   if (rc) return rc;
-  return lora::drop_bwd(N, IN, static_cast<const bf16*>(X), P, static_cast<const bf16*>(A_stack),
-                        nadp, R, seed, rates, static_cast<bf16*>(dX), dA, part, part_bytes, st);
+  auto finish = [&](auto* da) {
+    return lora::drop_bwd(N, IN, static_cast<const bf16*>(X), P, static_cast<const bf16*>(A_stack),
+                          nadp, R, seed, rates, static_cast<bf16*>(dX), da, part, part_bytes, st);
+  };
+  return grad_dtype == ML_F32 ? finish(static_cast<float*>(dA)) : finish(static_cast<bf16*>(dA));
 }
 
 // ------------------------------------------------------------------- MLP --

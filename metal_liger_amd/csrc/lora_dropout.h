@@ -353,9 +353,10 @@ __global__ __launch_bounds__(64 * kDbWaves) void drop_bwd_kernel(
     }
 }
 
-// dX [N, IN] += the adapters' part, dA [n rank, IN] (fp32, dense).
+// dX [N, IN] += the adapters' part, dA [n rank, IN] (fp32 or bf16, dense).
+template <typename TG>
 inline int drop_bwd(int N, int IN, const bf16* X, const bf16* P, const bf16* A, int n, int rank,
-                    const int64_t* seed, const DropRates& rates, bf16* dX, float* dA, char* ws,
+                    const int64_t* seed, const DropRates& rates, bf16* dX, TG* dA, char* ws,
                     size_t ws_bytes, hipStream_t st) {
   const int rs = rank / 16, RT = n * rank, rows = drop_bwd_rows(N, IN);
   ML_CHECK(drop_bwd_ws_bytes(N, RT, IN) <= ws_bytes, "lora dropout: workspace too small");
@@ -373,7 +374,7 @@ inline int drop_bwd(int N, int IN, const bf16* X, const bf16* P, const bf16* A, 
 #undef ML_DROP_BWD4
 #undef ML_DROP_BWD
   ML_LAUNCH_CHECK();
-  reduce_partials_kernel<float><<<dim3(256), 256, 0, st>>>(part, rtiles, RT, IN, dA, IN, 1.0f, 0.f);
+  reduce_partials_kernel<TG><<<dim3(256), 256, 0, st>>>(part, rtiles, RT, IN, dA, IN, 1.0f, 0.f);
   ML_LAUNCH_CHECK();
   return ML_OK;
 }

@@ -1196,43 +1196,58 @@ def lora_dropout_fwd(x2: torch.Tensor, ws, As, Bs, scales, rank: int, seed: torc
     return [*outs, xa, packed]
 
 
+@functools.lru_cache(maxsize=256)
+def _lora_dropout_ws_bytes(N: int, IN: int, rank: int, *outs: int) -> int:
+    return _hip.query("ml_lora_dropout_bwd_workspace_bytes", len(outs), N, IN, geom(outs), rank)
+
+
 def _lora_dropout_bwd(x2, dys, ws_, a_ptr: int, b_ptrs, scales, xa, rank: int, seed, thresholds,
-                      first: int, da_ptr: int, db_ptrs) -> torch.Tensor:
+                      first: int, da_ptr: int, db_ptrs, tag: int) -> torch.Tensor:
     """ml_lora_dropout_bwd for at least one token; the gradients go to the given
-    fp32 buffers. Returns dX."""
+    buffers, of the type that `tag` names. Returns dX."""
     x2 = _dense16(x2)
     dys, ws_ = [list(_dense16(*t, None))[:-1] for t in (dys, ws_)]
     (N, IN), n, dev = x2.shape, len(dys), x2.device
     dX = torch.empty(N, IN, dtype=torch.bfloat16, device=dev)
-    out_geom = geom([d.shape[1] for d in dys])
-    wsb = _hip.query("ml_lora_dropout_bwd_workspace_bytes", n, N, IN, out_geom, rank)
+    outs = [d.shape[1] for d in dys]
+    wsb = _lora_dropout_ws_bytes(N, IN, rank, *outs)
     ws = torch.empty(max(wsb, 16), dtype=torch.uint8, device=dev)
     call(
         "ml_lora_dropout_bwd", n, x2.data_ptr(), N, IN, _hip.ptrs([d.data_ptr() for d in dys]),
-        out_geom, _hip.ptrs([w.data_ptr() for w in ws_]), a_ptr, _hip.ptrs(b_ptrs),
+        geom(outs), _hip.ptrs([w.data_ptr() for w in ws_]), a_ptr, _hip.ptrs(b_ptrs),
         _hip.floats(scales), xa.data_ptr(), rank, geom(thresholds), seed.data_ptr(), first,
-        dX.data_ptr(), da_ptr, _hip.ptrs(db_ptrs), ws.data_ptr(), wsb, stream_of(x2),
+        dX.data_ptr(), da_ptr, _hip.ptrs(db_ptrs), tag, ws.data_ptr(), wsb, stream_of(x2),
     )
     return dX
+
+
+def _drop_grads(shapes, spec, dtype, dev):
+    """The buffer of a masked backward's gradients and their addresses and type: fp32
+    where they are unpacked by spec, else `dtype` (fp32 or bf16)."""
+    offs, total = grad_layout(shapes)
+    t = torch.float32 if spec else dtype
+    flat = torch.empty(max(total, 1), dtype=t, device=dev)
+    base, size = flat.data_ptr(), flat.element_size()
+    return flat, [base + size * o for o in offs], _hip.DTYPE_TAG[t]
 
 
 def lora_dropout_bwd(x2, dys, ws_, packed, scales, xa, rank: int, seed, thresholds, first: int,
                      spec, dtype):
     """The backward of lora_dropout_fwd: (dX, the adapters' gradients as
-    lora_unpack(grads, spec, dtype), or in fp32 as laid out by
-    grad_layout(lora_dropout_grad_shapes(...)) where spec is empty)."""
+    lora_unpack(grads, spec, dtype), or as laid out by
+    grad_layout(lora_dropout_grad_shapes(...)) in `dtype`, fp32 or bf16, where spec is
+    empty)."""
     ensure_rocm_device(x2, *dys, *ws_, packed, xa, seed)
     (N, IN), outs = x2.shape, [int(d.shape[1]) for d in dys]
-    offs, total = grad_layout(lora_dropout_grad_shapes(IN, outs, rank))
-    flat = torch.empty(max(total, 1), dtype=torch.float32, device=x2.device)
+    flat, (da, *dbs), tag = _drop_grads(lora_dropout_grad_shapes(IN, outs, rank), spec, dtype,
+                                        x2.device)
     if N == 0:
         flat.zero_()
         dX = torch.empty(0, IN, dtype=torch.bfloat16, device=x2.device)
     else:
         a_ptrs, b_ptrs, _ = _packed_ptrs(packed, [IN] * len(outs), outs, rank)
-        g = flat.data_ptr()
         dX = _lora_dropout_bwd(x2, dys, ws_, a_ptrs[0], b_ptrs, scales, xa, rank, seed, thresholds,
-                               first, g, [g + 4 * o for o in offs[1:]])
+                               first, da, dbs, tag)
     return dX, lora_unpack(flat, spec, dtype) if spec else flat
 
 
@@ -1260,19 +1275,18 @@ def lora_dropout_mlp_bwd(x2, gate, up, h, dy, ws_, packed, scales, xa, xa_d, ran
     layout is that of lora_mlp_grad_shapes."""
     ensure_rocm_device(x2, gate, up, h, dy, *ws_, packed, xa, xa_d, seed)
     (N, H), I = x2.shape, gate.shape[1]  # noqa: E741
-    offs, total = grad_layout(lora_mlp_grad_shapes(H, I, rank))
-    flat = torch.empty(max(total, 1), dtype=torch.float32, device=x2.device)
+    flat, (da_gu, da_d, db_g, db_u, db_d), tag = _drop_grads(lora_mlp_grad_shapes(H, I, rank), spec,
+                                                             dtype, x2.device)
     if N == 0:
         flat.zero_()
         dX = torch.empty(0, H, dtype=torch.bfloat16, device=x2.device)
         return dX, lora_unpack(flat, spec, dtype) if spec else flat
     a_ptrs, b_ptrs, _ = _packed_ptrs(packed, [H, H, I], [I, I, H], rank)
-    da_gu, da_d, db_g, db_u, db_d = (flat.data_ptr() + 4 * o for o in offs)
     dh = _lora_dropout_bwd(h, [dy], ws_[2:], a_ptrs[2], b_ptrs[2:], scales[2:], xa_d, rank, seed,
-                           thresholds[2:], 2, da_d, [db_d])
+                           thresholds[2:], 2, da_d, [db_d], tag)
     dgate, dup = swiglu_bwd(gate, up, dh)
     dX = _lora_dropout_bwd(x2, [dgate, dup], ws_[:2], a_ptrs[0], b_ptrs[:2], scales[:2], xa, rank,
-                           seed, thresholds[:2], 0, da_gu, [db_g, db_u])
+                           seed, thresholds[:2], 0, da_gu, [db_g, db_u], tag)
     return dX, lora_unpack(flat, spec, dtype) if spec else flat
 
 
@@ -1299,7 +1313,8 @@ def lora_dropout_wide_fwd(x2, ws, As, Bs, scales, rank: int, seed, thresholds, f
 
 def lora_dropout_wide_bwd(x2, dys, ws_, packed, scales, xa, rank: int, seed, thresholds, first: int,
                           spec, dtype):
-    """The backward of lora_dropout_wide_fwd, as lora_dropout_bwd."""
+    """The backward of lora_dropout_wide_fwd, as lora_dropout_bwd (dtype fp32 where
+    spec is empty)."""
     ensure_rocm_device(x2, *dys, *ws_, packed, xa, seed)
     (N, IN), n, bf, dev = x2.shape, len(dys), torch.bfloat16, x2.device
     shapes = lora_dropout_grad_shapes(IN, [d.shape[1] for d in dys], rank)

@@ -30,6 +30,7 @@ formulas (gemm_f32: forward [X | X A^T] x [W; s B]^T, backward P = s dY B,
 dA = P^T X, dB = s dY^T (X A^T), dX one K-concatenated product).
 """
 
+import functools
 import logging
 
 import torch
@@ -429,6 +430,38 @@ class _LoRA_W(torch.autograd.Function):
 
 
 # ------------------------------------------------------- dropout on X --
+@functools.lru_cache(maxsize=256)
+def _drop_grad_plan(shapes, parts, ranks, rp: int, dtypes):
+    """How a masked backward's gradients reach the adapters' shapes and types: (the
+    op's spec, the dtype it returns, where each lies in that: (offset, rows, cols, row
+    stride)). Written in place where all adapters are bf16, or fp32, of the padded rank;
+    unpacked where they share another type or a rank is padded; cast one by one where
+    their types differ."""
+    spec, unpack = _grad_spec(shapes, parts, dtypes)
+    same = len(set(dtypes)) == 1
+    if same and dtypes[0] in (torch.bfloat16, torch.float32) and rp <= 64 and set(ranks) == {rp}:
+        spec_arg, dtype, unpack = [], dtypes[0], False
+    else:
+        spec_arg, dtype = (spec, dtypes[0]) if unpack else ([], torch.float32)
+    at = hip_ops.unpack_layout(spec)[0]
+    views = [(at[k], *spec[4 * k + 1:4 * k + 3], spec[4 * k + 2]) if unpack
+             else tuple(spec[4 * k:4 * k + 4]) for k in range(len(at))]
+    return spec_arg, dtype, views
+
+
+def _drop_grad_views(flat, views, dtypes):
+    out = []
+    for (off, rows, cols, ld), t in zip(views, dtypes):
+        g = flat.as_strided((rows, cols), (ld, 1), off)
+        out.append(g if g.dtype == t else g.to(t))
+    return out
+
+
+def _rows(t):
+    """[..., C] -> [R, C]"""
+    return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+
+
 # PEFT drops elements of the adapter's input, with a mask M_i of its own for each
 # projection, and scales the others by c_i = 1 / (1 - q_i):
 #   y_i  = X W_i^T + s_i XA_i B_i^T      XA_i = c_i (M_i X) A_i^T
@@ -464,12 +497,14 @@ class _LoRA_Dropout(torch.autograd.Function):
                                             seed, thresholds, first)
             ctx.save_for_backward(X2, seed, *res[n:], *params)
             return tuple(o.to(X.dtype).view(*shape[:-1], o.shape[-1]) for o in res[:n])
-        X2 = hip_ops._bf16_rows(X.reshape(-1, shape[-1]))
+        X2 = hip_ops._bf16_rows(_rows(X))
         Wc = [hip_ops._bf16_rows(W.detach()) for W in Ws]
         op = cops.lora_dropout_fwd if ctx.rank_p <= 64 else cops.lora_dropout_wide_fwd
         *outs, xa, packed = op(X2, Wc, list(As), list(Bs), scales, ctx.rank_p, seed, thresholds,
                                first)
         ctx.save_for_backward(X2, seed, xa, packed, *Wc)
+        if len(shape) == 2:
+            return tuple(outs)
         return tuple(o.view(*shape[:-1], o.shape[-1]) for o in outs)
 
     @staticmethod
@@ -483,18 +518,19 @@ class _LoRA_Dropout(torch.autograd.Function):
             grads = [g.to(t) for g, t in zip(grads, dtypes)]
         else:
             xa, packed, *Ws = rest
-            dys = [hip_ops._bf16_rows(d.reshape(-1, d.shape[-1])) for d in dYs]
-            rp, in_f = ctx.rank_p, X2.shape[1]
-            shapes = hip_ops.lora_dropout_grad_shapes(in_f, [d.shape[1] for d in dys], rp)
-            parts = [p for i, r in enumerate(ranks)
-                     for p in ((0, i * rp, r, in_f), (1 + i, 0, dys[i].shape[1], r))]
-            spec, unpack = _grad_spec(shapes, parts, dtypes)
+            dys = [hip_ops._bf16_rows(_rows(d)) for d in dYs]
+            rp, in_f, outs = ctx.rank_p, X2.shape[1], [W.shape[0] for W in Ws]
+            shapes = tuple(hip_ops.lora_dropout_grad_shapes(in_f, outs, rp))
+            parts = tuple(p for i, (r, o) in enumerate(zip(ranks, outs))
+                          for p in ((0, i * rp, r, in_f), (1 + i, 0, o, r)))
+            spec, dtype, views = _drop_grad_plan(shapes, parts, tuple(ranks), rp, tuple(dtypes))
             op = cops.lora_dropout_bwd if rp <= 64 else cops.lora_dropout_wide_bwd
             dX, flat = op(X2, dys, Ws, packed, ctx.scales, xa, rp, seed, ctx.thresholds, ctx.first,
-                          spec if unpack else [], dtypes[0] if unpack else torch.float32)
-            grads = _unpacked_views(flat, spec) if unpack else \
-                [g.to(t) for g, t in zip(_grad_views(flat, spec), dtypes)]
-        out = [dX.to(ctx.x_dtype).view(*ctx.orig_shape), None, None, None]
+                          spec, dtype)
+            grads = _drop_grad_views(flat, views, dtypes)
+        if dX.dtype != ctx.x_dtype or len(ctx.orig_shape) != 2:
+            dX = dX.to(ctx.x_dtype).view(*ctx.orig_shape)
+        out = [dX, None, None, None]
         for i in range(n):
             out += [None, grads[2 * i], grads[2 * i + 1], None]
         return tuple(out)
@@ -512,7 +548,7 @@ class _LoRA_Dropout_MLP(torch.autograd.Function):
         ctx.ranks = [A.shape[0] for A in As]
         ctx.rank_p = _pad_rank(max(ctx.ranks))
         ctx.param_dtypes = [t.dtype for t in (*As, *Bs)]
-        X2 = hip_ops._bf16_rows(X.reshape(-1, X.shape[-1]))
+        X2 = hip_ops._bf16_rows(_rows(X))
         Wc = [hip_ops._bf16_rows(W.detach()) for W in Ws]
         out, *saved = cops.lora_dropout_mlp_fwd(X2, Wc, list(As), list(Bs), ctx.scales, ctx.rank_p,
                                                 seed, thresholds)
@@ -524,16 +560,15 @@ class _LoRA_Dropout_MLP(torch.autograd.Function):
     def backward(ctx, dY):
         X2, seed, gate, up, h, xa, xa_d, packed, *Ws = ctx.saved_tensors
         (rg, ru, rd), rp, dtypes = ctx.ranks, ctx.rank_p, ctx.param_dtypes
-        dy = hip_ops._bf16_rows(dY.reshape(-1, dY.shape[-1]))
+        dy = hip_ops._bf16_rows(_rows(dY))
         H, I = X2.shape[1], gate.shape[1]  # noqa: E741
-        parts = [(0, 0, rg, H), (0, rp, ru, H), (1, 0, rd, I), (2, 0, I, rg), (3, 0, I, ru),
-                 (4, 0, dy.shape[1], rd)]
-        spec, unpack = _grad_spec(hip_ops.lora_mlp_grad_shapes(H, I, rp), parts, dtypes)
+        parts = ((0, 0, rg, H), (0, rp, ru, H), (1, 0, rd, I), (2, 0, I, rg), (3, 0, I, ru),
+                 (4, 0, dy.shape[1], rd))
+        spec, dtype, views = _drop_grad_plan(tuple(hip_ops.lora_mlp_grad_shapes(H, I, rp)), parts,
+                                             tuple(ctx.ranks), rp, tuple(dtypes))
         dX, flat = cops.lora_dropout_mlp_bwd(X2, gate, up, h, dy, Ws, packed, ctx.scales, xa, xa_d,
-                                             rp, seed, ctx.thresholds, spec if unpack else [],
-                                             dtypes[0] if unpack else torch.float32)
-        grads = _unpacked_views(flat, spec) if unpack else \
-            [g.to(t) for g, t in zip(_grad_views(flat, spec), dtypes)]
+                                             rp, seed, ctx.thresholds, spec, dtype)
+        grads = _drop_grad_views(flat, views, dtypes)
         out = [dX.view(*ctx.orig_shape), None, None]
         for A, B in zip(grads[:3], grads[3:]):
             out += [None, A, B, None]

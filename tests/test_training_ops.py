@@ -198,17 +198,19 @@ def test_lora_dropout_host_side_argument_errors():
                      (dict(x=None), b"null pointer"), (dict(x=p + 2), b"16-byte aligned")):
         assert xa(**kw) == 1 and text in L.ml_last_error(), (kw, L.ml_last_error())
 
-    def bwd(n=1, tokens=4, width=64, outs=(64, 64, 64), rank=16, dx=p, w=p, ws=p, ws_bytes=1 << 30):
+    def bwd(n=1, tokens=4, width=64, outs=(64, 64, 64), rank=16, dx=p, w=p, ws=p, ws_bytes=1 << 30,
+            grad=0):
         ptrs = _hip.ptrs([p] * 3)
         return L.ml_lora_dropout_bwd(n, p, tokens, width, ptrs, _hip.geom(outs), _hip.ptrs([w] * 3), p,
                                      ptrs, _hip.floats([1.0] * 3), p, rank, _hip.geom([0] * 3), p, 0,
-                                     dx, p, ptrs, ws, ws_bytes, None)
+                                     dx, p, ptrs, grad, ws, ws_bytes, None)
 
     for kw, text in ((dict(n=0), b"1..3 adapters"), (dict(tokens=0), b"token count"),
                      (dict(width=4), b"multiple of 8"), (dict(outs=(60,)), b"multiple of 8"),
                      (dict(rank=72), b"rank 16"), (dict(dx=None), b"null pointer"),
                      (dict(w=None), b"null pointer"), (dict(w=p + 8), b"16-byte aligned"),
                      (dict(dx=p + 2), b"16-byte aligned"), (dict(ws=None), b"workspace"),
+                     (dict(grad=2), b"fp32 or bf16"),
                      (dict(ws_bytes=64), b"workspace"), (dict(ws=p + 4), b"workspace")):
         assert bwd(**kw) == 1 and text in L.ml_last_error(), (kw, L.ml_last_error())
     assert L.ml_lora_dropout_bwd_workspace_bytes(4, 4, 64, _hip.geom([64] * 4), 16) == 0
@@ -239,7 +241,7 @@ def test_fake_kernels():
             q, k, xa, packed = fwd(x, ws, As, Bs, [2.0] * 2, rank, seed, [100, 0], 0)
             assert q.shape == (96, 64) and k.shape == (96, 32) and xa.shape == (96, 2 * rank)
             assert packed.shape == (rank * (2 * 128 + 2 * 96),)
-            dx, g = bwd(x, [q, k], ws, packed, [2.0] * 2, xa, rank, seed, [100, 0], 0, [], BF)
+            dx, g = bwd(x, [q, k], ws, packed, [2.0] * 2, xa, rank, seed, [100, 0], 0, [], F32)
             assert dx.shape == (96, 128) and g.dtype == F32
             assert g.shape == (2 * rank * 128 + 64 * rank + 32 * rank,)
 
