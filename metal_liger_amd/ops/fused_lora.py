@@ -539,7 +539,10 @@ class _LoRA_Dropout(torch.autograd.Function):
 class _LoRA_Dropout_MLP(torch.autograd.Function):
     """gate + up + down with dropout on each adapter's input (streams 0, 1, 2 of
     `seed`) and SwiGLU, for bf16 and ranks up to 64: one op each way. h is saved,
-    as the down adapter's input."""
+    as the down adapter's input. gate, up, h and their gradients are rounded to bf16
+    between the products, which read them on the bf16 matrix cores, as in the block
+    without dropout: the results are off by 4.2e-3 of their norm, with fp32 there by
+    1.7e-3."""
 
     @staticmethod
     def forward(ctx, X, seed, thresholds, *params):
