@@ -671,13 +671,17 @@ def apply_fused_lora_mlp(mlp_module, X: torch.Tensor, lora_dropout: bool = False
             _check_float(X, "LoRA MLP")
             hip_ops.ensure_rocm_device(X)
             seed = seed_tensor(seed, X.device)
-            if not _fp32_path(X, X.shape[-1], GW.shape[0], DW.shape[0]) \
-                    and max(GA.shape[0], UA.shape[0], DA.shape[0]) <= 64:
+            fp32 = _fp32_path(X, X.shape[-1], GW.shape[0], DW.shape[0])
+            if not fp32 and max(GA.shape[0], UA.shape[0], DA.shape[0]) <= 64:
                 return _LoRA_Dropout_MLP.apply(X, seed, thresholds, GW, GA, GB, GS, UW, UA, UB, US,
                                                DW, DA, DB, DS)
-            gate, up = _LoRA_Dropout.apply(X, seed, thresholds[:2], 0, GW, GA, GB, GS, UW, UA, UB, US)
+            # on the fp32 products gate, up, h and their gradients stay in fp32, as in
+            # _LoRA_MLP: rounded to fp16 between the projections, h would overflow
+            # where the block without dropout does not
+            x = X.float() if fp32 else X
+            gate, up = _LoRA_Dropout.apply(x, seed, thresholds[:2], 0, GW, GA, GB, GS, UW, UA, UB, US)
             return _LoRA_Dropout.apply(fused_swiglu(gate, up), seed, thresholds[2:], 2,
-                                       DW, DA, DB, DS)[0]
+                                       DW, DA, DB, DS)[0].to(X.dtype)
     return _LoRA_MLP.apply(
         X,
         GW, GA, GB, GS,

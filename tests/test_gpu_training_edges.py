@@ -1,0 +1,77 @@
+"""Dropout, LoRA dropout and the embedding where two of their paths meet: the types
+that one projection hands to the next, evaluation beside training, rows of unusual
+strides, second derivatives, sizes past the limits of one launch and ids that need
+several levels of merging. Bounds as in the operators' own tests."""
+
+import pytest
+import torch
+
+from oracle import training_ops as ref
+from tests.parity import seeded
+from tests.test_gpu_lora_dropout import (
+    _half,
+    _linear,
+    _mlp,
+    _params,
+)
+
+pytestmark = pytest.mark.gpu
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+# ------------------------------------------------- the MLP on the fp32 products
+
+def _mlp_grads(dev, mlp, lins, x, dy, ps, seed=11):
+    """(y, dx, adapters' gradients) of the block and the same in 64 bits, with the
+    largest |h| of its inner activations."""
+    from metal_liger_amd import apply_fused_lora_mlp
+    xd = x.to(dev).requires_grad_()
+    adapters = [t for m in lins for t in (m.lora_A["default"].weight, m.lora_B["default"].weight)]
+    y = apply_fused_lora_mlp(mlp, xd, lora_dropout=True, seed=seed)
+    got = [y, *torch.autograd.grad(y, [xd, *adapters], dy.to(dev))]
+    x64 = x.double().requires_grad_()
+    leaves, out, h = [], [], 0.0
+    for k, m in enumerate(lins):
+        w, a, b, s = _params(m)
+        a, b = (v.double().requires_grad_() for v in (a, b))
+        leaves += [a, b]
+        t = out[0] * torch.sigmoid(out[0]) * out[1] if k == 2 else x64
+        h = t.detach().abs().max().item()
+        f = ref.dropout_factors(tuple(t.shape), ps[k], seed, k)
+        out.append(t @ w.double().t() + s * ((t * f) @ a.t()) @ b.t())
+    return got, [out[2], *torch.autograd.grad(out[2], [x64, *leaves], dy.double())], h
+
+
+@pytest.mark.parametrize("dtype, H, I", [(F16, 256, 512), (F16, 99, 203), (BF, 99, 203)])
+def test_mlp_holds_its_inner_tensors_in_fp32(dev, dtype, H, I):  # noqa: E741
+    """On the fp32 products only the block's output and dX are rounded to the
+    activations' type (norms: eps / 2 of them), as in the block without dropout; the
+    adapters' gradients, in fp32, are sums of at most 512 terms (2e-5 of their norms,
+    as where the activations are fp32 too)."""
+    ps = (0.2, 0.1, 0.3)
+    lins, mlp = _mlp(dev, dtype, (8, 8, 8), ps, H, I, adapter=F32)
+    x, dy = (seeded((90, H), k, dtype) for k in (1, 2))
+    got, want, _ = _mlp_grads(dev, mlp, lins, x, dy, ps)
+    assert got[0].dtype == got[1].dtype == dtype
+    for k, (g, w) in enumerate(zip(got, want)):
+        tol = 2e-5 + (_half(dtype) if k < 2 else 0.0)
+        assert (g.double().cpu() - w).norm() <= tol * w.norm(), k
+
+
+def test_mlp_inner_activations_past_fp16(dev):
+    """silu(gate) * up beyond 65504 under a down projection that brings it back: the
+    fp16 block is finite and near the 64-bit form (output rounded once, sums of 512
+    terms in fp32), with dropout as without."""
+    from metal_liger_amd import apply_fused_lora_mlp
+    ps = (0.1, 0.1, 0.1)
+    lins, mlp = _mlp(dev, F16, (8, 8, 8), ps, adapter=F32)
+    with torch.no_grad():
+        lins[2].base_layer.weight.mul_(2.0 ** -7)
+        lins[2].lora_B["default"].weight.mul_(2.0 ** -7)
+    x, dy = seeded((40, 256), 1, F16, scale=400.0), seeded((40, 256), 2, F16)
+    got, want, h = _mlp_grads(dev, mlp, lins, x, dy, ps)
+    assert h > 65504 and want[0].abs().max() < 65504
+    assert torch.isfinite(apply_fused_lora_mlp(mlp, x.to(dev))).all()
+    for k, (g, w) in enumerate(zip(got, want)):
+        tol = 2e-5 + (_half(F16) if k < 2 else 0.0)
+        assert torch.isfinite(g).all() and (g.double().cpu() - w).norm() <= tol * w.norm(), k
