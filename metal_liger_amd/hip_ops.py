@@ -610,14 +610,23 @@ def kv_reduce(dk: torch.Tensor, dv: torch.Tensor, groups: int):
 # -------------------------------------------------------------------- GEMM --
 
 
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """The matrix with its width as row stride. (contiguous() returns a matrix of one
+    row as it is, whatever its row stride, which the products would refuse.)"""
+    t = t.contiguous()
+    if t.stride(0) != t.shape[-1]:
+        t = t.clone(memory_format=torch.contiguous_format)
+    return t
+
+
 def _gemm_operand(t: torch.Tensor, what: str) -> torch.Tensor:
     if t.dtype != torch.bfloat16:
         raise TypeError(f"gemm: {what} must be bfloat16 (got {t.dtype})")
     if t.dim() != 2:
         raise ValueError(f"gemm: {what} must be 2-D")
-    if t.stride(1) != 1 or t.stride(0) % 8 != 0 or t.data_ptr() % 16 != 0:
-        t = t.contiguous()
-    return t
+    if t.stride(1) != 1 or t.stride(0) % 8 != 0:
+        t = _dense(t)
+    return _al16(t)
 
 
 def matmul(a: torch.Tensor, b: torch.Tensor, *, a_t: bool = False, b_t: bool = False,
@@ -672,7 +681,7 @@ def _f32_2d(t: torch.Tensor) -> torch.Tensor:
     if t.dtype != torch.float32:
         t = t.float()
     if t.dim() != 2 or t.stride(1) != 1 or t.stride(0) < t.shape[1]:
-        t = t.contiguous()
+        t = _dense(t)
     return t
 
 
@@ -728,8 +737,10 @@ def _flce_operands(hidden, weight, labels, bias):
         raise ValueError(f"flce: labels shape {tuple(labels.shape)} != ({hidden.shape[0]},)")
 
     def rowmajor(t):
-        ok = t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.data_ptr() % 16 == 0
-        return t if ok and t.shape[0] > 0 else t.contiguous()
+        ok = t.stride(1) == 1 and t.stride(0) % 8 == 0 and t.shape[0] > 0
+        t = t if ok else _dense(t)
+        # (fp32 takes any alignment; other widths in bf16 are padded below)
+        return _al16(t) if t.dtype == torch.bfloat16 and t.shape[1] % 8 == 0 else t
 
     hidden = rowmajor(hidden)
     weight = rowmajor(weight)
@@ -943,7 +954,7 @@ def _bf16_rows(t: torch.Tensor) -> torch.Tensor:
     if t.dtype != torch.bfloat16:
         t = t.to(torch.bfloat16)
     if t.dim() != 2 or t.stride(1) != 1 or t.stride(0) % 8 != 0 or t.stride(0) < t.shape[1]:
-        t = t.contiguous()
+        t = _dense(t)
     return t
 
 

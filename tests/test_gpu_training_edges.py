@@ -9,6 +9,7 @@ import torch
 from oracle import training_ops as ref
 from tests.parity import seeded
 from tests.test_gpu_lora_dropout import (
+    _block,
     _half,
     _linear,
     _mlp,
@@ -75,3 +76,67 @@ def test_mlp_inner_activations_past_fp16(dev):
     for k, (g, w) in enumerate(zip(got, want)):
         tol = 2e-5 + (_half(F16) if k < 2 else 0.0)
         assert torch.isfinite(g).all() and (g.double().cpu() - w).norm() <= tol * w.norm(), k
+
+
+# ------------------------------------------------------------------ odd strides
+
+@pytest.mark.parametrize("rank", [16, 96])
+def test_one_row_of_an_odd_stride(dev, rank):
+    """A batch of one token cut out of a wider buffer: its row stride, which no access
+    uses, need not be a multiple of 8."""
+    from metal_liger_amd import apply_fused_lora_mlp, apply_fused_lora_qkv
+    from metal_liger_amd.ops.fused_lora import _lora_linear, apply_fused_lora_linear
+    lins = [_linear(dev, 128, o, rank, 0.4, BF, 10 * k) for k, o in enumerate((128, 64, 64))]
+    attn = _block(q_proj=lins[0], k_proj=lins[1], v_proj=lins[2])
+    _, mlp = _mlp(dev, BF, (rank,) * 3, (0.3,) * 3, 128, 256)
+    wide = seeded((3, 131), 1, BF).to(dev)
+    w, a, b, s = (lins[0].base_layer.weight, lins[0].lora_A["default"].weight,
+                  lins[0].lora_B["default"].weight, 2.0)
+    calls = [lambda x, drop=drop, f=f: f(x, drop) for drop in (True, False) for f in (
+        lambda x, drop: apply_fused_lora_qkv(attn, x, lora_dropout=drop, seed=3),
+        lambda x, drop: (apply_fused_lora_mlp(mlp, x, lora_dropout=drop, seed=3),),
+        lambda x, drop: (apply_fused_lora_linear(lins[0], x, lora_dropout=drop, seed=3),),
+        lambda x, drop: (_lora_linear(x, w, a, b, s),),
+        lambda x, drop: (_lora_linear(x, w, None, None, s),))]
+    for i, call in enumerate(calls):
+        odd = wide[1:2, :128]
+        assert odd.stride(0) == 131
+        for x in (odd, odd.unsqueeze(0), wide[:1, :128]):
+            runs = []
+            for dense in (False, True):
+                t = x.clone(memory_format=torch.contiguous_format) if dense else x
+                t = t.detach().requires_grad_()
+                assert t.stride(-2) == (128 if dense else 131)
+                ys = call(t)
+                dys = [wide.flatten()[5:5 + y.numel()].view(y.shape) for y in ys]
+                dx = () if i % 5 > 2 else torch.autograd.grad(ys, t, dys)  # (_lora_linear: none)
+                runs.append([*ys, *dx])
+            assert all(torch.equal(p, q) for p, q in zip(*runs)), i
+
+
+def test_one_row_of_an_odd_stride_through_the_loss(dev):
+    """As above for the fused cross-entropy's hidden state and the products."""
+    from metal_liger_amd import hip_ops
+    from metal_liger_amd.ops.fused_linear_cross_entropy import MetalLigerFusedLinearCrossEntropy
+    wide = seeded((3, 131), 1, BF).to(dev)
+    x = wide[1:2, :128]
+    weight = seeded((64, 128), 2, BF, scale=0.1).to(dev)
+    labels = torch.tensor([5], device=dev)
+    head = torch.nn.Linear(128, 64, bias=False)
+    head.weight = torch.nn.Parameter(weight)
+    loss = MetalLigerFusedLinearCrossEntropy(head)
+    dense = x.clone(memory_format=torch.contiguous_format)
+    runs = []
+    for t in (x, dense, wide[:1, :128], wide[:1, :128].clone(memory_format=torch.contiguous_format)):
+        t = t.detach().requires_grad_()
+        y = loss(t, labels)
+        runs.append([y, *torch.autograd.grad(y, [t, head.weight])])
+    for k in (0, 2):
+        assert all(torch.equal(p, q) for p, q in zip(runs[k], runs[k + 1]))
+    assert torch.equal(hip_ops.matmul(x, weight, b_t=True), hip_ops.matmul(dense, weight, b_t=True))
+    f = wide.float()[1:2, :128]
+    flat = torch.ones(128, device=dev).as_strided((1, 128), (1, 1))
+    for t in (f, flat):
+        assert torch.equal(hip_ops.gemm_f32([t], [weight.float()], b_t=True),
+                           hip_ops.gemm_f32([t.clone(memory_format=torch.contiguous_format)],
+                                            [weight.float()], b_t=True))
