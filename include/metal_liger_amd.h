@@ -168,10 +168,11 @@ int ml_swiglu_bwd(const void* gate, const void* up, const void* dy, void* dgate,
  * dropout, 1 for its mask alone. kept_i: the (i mod 8)-th 16-bit part
  * (low halves first) of the four words of Philox4x32 with 7 rounds at the
  * counter (i div 8 as 64 bits, stream_id, 0) and the key *seed is at least
- * threshold. seed: one int64 in DEVICE memory; stream_id: 32 bits, so that one
- * seed serves several masks. The gradient of x is the same call over the
- * gradient of out (without residual). residual may be NULL; out may be x or
- * residual. A dropped element contributes 0 whatever x holds there.
+ * threshold. seed: one int64 in DEVICE memory (NULL where threshold is 0);
+ * stream_id: 32 bits, so that one seed serves several masks. The gradient of x
+ * is the same call over the gradient of out (without residual). residual may be
+ * NULL; out may be x or residual. A dropped element contributes 0 whatever x
+ * holds there.
  */
 int ml_dropout(const void* x, const void* residual, void* out, int64_t n, int64_t threshold,
                float scale, const int64_t* seed, int64_t stream_id, int dtype, void* stream);

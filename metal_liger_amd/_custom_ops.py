@@ -340,7 +340,7 @@ def _define(schema: str, fn, fake):
     return getattr(getattr(torch.ops, NS), name).default
 
 
-dropout = _define("dropout(Tensor x, Tensor? residual, Tensor seed, SymInt threshold, SymInt stream, "
+dropout = _define("dropout(Tensor x, Tensor? residual, Tensor? seed, SymInt threshold, SymInt stream, "
                   "float scale) -> Tensor", hip_ops.dropout,
                   lambda x, residual, seed, threshold, stream, scale: x.new_empty(x.shape))
 embedding_fwd = _define("embedding_fwd(Tensor ids, Tensor weight, float scale) -> Tensor",

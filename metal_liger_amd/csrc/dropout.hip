@@ -35,7 +35,7 @@ __global__ __launch_bounds__(kThreads) void dropout_scalar(const T* x, const T* 
                                                            int64_t n, const int64_t* seed,
                                                            uint32_t stream, DropRate rate,
                                                            float scale) {
-  const DropKey key = drop_key(seed);
+  const DropKey key = seed ? drop_key(seed) : DropKey{};  // (none where nothing is dropped)
   for (int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kDropBlock; i < n;
        i += (int64_t)gridDim.x * kThreads * kDropBlock)
     drop_block<T>(x, RES ? res : nullptr, out, i, n, key, stream, rate, scale);
@@ -68,7 +68,7 @@ __global__ __launch_bounds__(kThreads) void dropout_vec(const T* x, const T* res
   constexpr int VEC = vec16<T>();
   const int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * VEC;
   const int64_t block = i / kDropBlock;
-  const DropKey key = drop_key(seed);
+  const DropKey key = seed ? drop_key(seed) : DropKey{};  // (none where nothing is dropped)
   if ((block + 1) * kDropBlock <= n) {
     const Pack<T, VEC> v = load_pack_nt<T, VEC>(x + i);
     Pack<T, VEC> r{};
@@ -95,7 +95,7 @@ extern "C" int ml_dropout(const void* x, const void* residual, void* out, int64_
            (long long)threshold);
   ML_CHECK(stream_id >= 0 && stream_id <= 0xFFFFFFFFLL, "dropout: stream id outside 32 bits");
   if (n == 0) return ML_OK;
-  ML_CHECK(x && out && seed, "dropout: null pointer");
+  ML_CHECK(x && out && (seed || threshold == 0), "dropout: null pointer");
   ML_CHECK(n < (1LL << 40), "dropout: too many elements (%lld)", (long long)n);
   hipStream_t st = (hipStream_t)stream;
   const DropRate rate = drop_rate(threshold);

@@ -175,12 +175,14 @@ def check_seed(seed: torch.Tensor) -> None:
                         f"(got {seed.dtype} of shape {tuple(seed.shape)})")
 
 
-def dropout(x: torch.Tensor, residual: torch.Tensor | None, seed: torch.Tensor, threshold: int,
-            stream: int, scale: float) -> torch.Tensor:
+def dropout(x: torch.Tensor, residual: torch.Tensor | None, seed: torch.Tensor | None,
+            threshold: int, stream: int, scale: float) -> torch.Tensor:
     """scale * x where kept, else 0, + residual (ml_dropout's masks over x's
-    elements in row-major order, whatever its strides); contiguous, x's dtype."""
+    elements in row-major order, whatever its strides); contiguous, x's dtype.
+    seed: None only where threshold is 0."""
     ensure_rocm_device(x, residual, seed)
-    check_seed(seed)
+    if seed is not None:
+        check_seed(seed)
     if residual is not None:
         if residual.shape != x.shape or residual.dtype != x.dtype:
             raise ValueError(f"dropout: residual {tuple(residual.shape)} {residual.dtype} does not "

@@ -51,7 +51,9 @@ class _FusedDropoutFunction(torch.autograd.Function):
     def backward(ctx, dy):
         seed, = ctx.saved_tensors
         dx = None
-        if ctx.needs_input_grad[0]:
+        if ctx.needs_input_grad[0] and ctx.threshold == 0:
+            dx = dy
+        elif ctx.needs_input_grad[0]:
             dx = cops.dropout(dy, None, seed, ctx.threshold, ctx.stream,
                               hip_ops.drop_scale(ctx.threshold))
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
@@ -65,7 +67,8 @@ def fused_dropout(x: torch.Tensor, p: float = 0.5, training: bool = True,
 
     x of fp32, bf16 or fp16 and any shape and strides; the mask goes by row-major
     order. seed: one int64 on x's device, an int, or None (module docstring);
-    stream: 0 .. 2^32 - 1, for several masks of one seed. Not training: x (+ residual).
+    stream: 0 .. 2^32 - 1, for several masks of one seed. Not training: x (+ residual),
+    and no seed is drawn.
     """
     threshold = hip_ops.drop_threshold(p) if training else 0
     if not 0 <= stream < 2 ** 32:
@@ -73,7 +76,8 @@ def fused_dropout(x: torch.Tensor, p: float = 0.5, training: bool = True,
     if threshold == 0 and residual is None:
         return x
     hip_ops.ensure_rocm_device(x, residual)
-    return _FusedDropoutFunction.apply(x, residual, seed_tensor(seed, x.device), threshold, stream)
+    seed = seed_tensor(seed, x.device) if threshold else None
+    return _FusedDropoutFunction.apply(x, residual, seed, threshold, stream)
 
 
 class MetalLigerDropout(nn.Module):

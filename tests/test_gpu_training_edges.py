@@ -140,3 +140,27 @@ def test_one_row_of_an_odd_stride_through_the_loss(dev):
         assert torch.equal(hip_ops.gemm_f32([t], [weight.float()], b_t=True),
                            hip_ops.gemm_f32([t.clone(memory_format=torch.contiguous_format)],
                                             [weight.float()], b_t=True))
+
+
+# ------------------------------------------------------------------ evaluation
+
+def test_evaluation_with_a_residual_draws_no_seed(dev):
+    """Nothing is dropped: torch's generator stays where it was, the sum is the one
+    rounding of x + residual, and both gradients are dy's values."""
+    from metal_liger_amd import MetalLigerDropout, fused_dropout
+    for dtype in (F32, BF, F16):
+        x, res, dy = (seeded((33, 65), k, dtype).to(dev).requires_grad_() for k in (1, 2, 3))
+        torch.manual_seed(3)
+        state = torch.cuda.get_rng_state()
+        for y in (fused_dropout(x, 0.5, training=False, residual=res),
+                  fused_dropout(x, 1e-7, residual=res), MetalLigerDropout(0.5).eval()(x, res)):
+            assert torch.equal(y, x + res) and y.is_contiguous()
+            dx, dr = torch.autograd.grad(y, [x, res], dy)
+            assert torch.equal(dx, dy) and torch.equal(dr, dy)
+        assert torch.equal(torch.cuda.get_rng_state(), state)
+    with pytest.raises(ValueError, match="residual"):
+        fused_dropout(x, 0.5, training=False, residual=res[:1])
+    with pytest.raises(ValueError, match="residual"):
+        fused_dropout(x, 0.5, training=False, residual=res.float())
+    with pytest.raises(TypeError, match="dtype"):
+        fused_dropout(x.double(), 0.5, training=False, residual=res.double())
