@@ -164,3 +164,19 @@ def test_evaluation_with_a_residual_draws_no_seed(dev):
         fused_dropout(x, 0.5, training=False, residual=res.float())
     with pytest.raises(TypeError, match="dtype"):
         fused_dropout(x.double(), 0.5, training=False, residual=res.double())
+
+
+# ------------------------------------------------- sizes past one launch's threads
+
+def test_dropout_past_one_launch(dev):
+    """More blocks of 16 bytes than a launch has threads (2^35 elements of 16 bits and
+    some, in place): the ends, and both sides of where the second launch begins."""
+    from metal_liger_amd import _hip
+    n = 2 ** 35 + 1003
+    x = torch.ones(n, dtype=BF, device=dev)
+    seed = torch.tensor([10], device=dev)
+    _hip.call("ml_dropout", x.data_ptr(), None, x.data_ptr(), n, 32768, 2.0, seed.data_ptr(), 7,
+              _hip.DTYPE_TAG[BF], _hip.stream_of(x))
+    for first in (0, 2 ** 34 - 512, 2 ** 35 - 512, n - 1003):
+        f = ref.dropout_factors((1003,), 0.5, 10, 7, first=first)
+        assert torch.equal(x[first:first + 1003].double().cpu(), f), first
