@@ -37,6 +37,7 @@ __device__ __forceinline__ int64_t id_at(const void* ids, int64_t n, bool wide) 
 // A row is VEC-element vectors; LPR lanes (a power of two, 1..256) walk a row and
 // 256 / LPR rows go side by side, kRows of them in flight per lane.
 constexpr int kRows = 4;
+constexpr int64_t kMaxBlocks = 1 << 23;  // a launch holds fewer than 2^32 threads along x
 
 template <typename T, int VEC>
 __global__ __launch_bounds__(kThreads) void embedding_rows(const void* ids, bool wide, int64_t N,
@@ -487,16 +488,20 @@ extern "C" int ml_embedding_fwd(const void* ids, int id_bytes, int64_t n, const 
     int lpr = 1;
     while (lpr < per_row && lpr < kThreads) lpr *= 2;
     const int rows = kThreads / lpr * kRows;
-    const dim3 grid((unsigned)((n + rows - 1) / rows), (unsigned)((per_row + lpr - 1) / lpr));
     const T* w = static_cast<const T*>(weight);
-    T* o = static_cast<T*>(out);
     hipStream_t st = (hipStream_t)stream;
-    if (vec)
-      embedding_rows<T, VEC><<<grid, kThreads, 0, st>>>(ids, id_bytes == 8, n, w, ldw, o, vocab,
+    for (int64_t first = 0; first < n; first += kMaxBlocks * rows) {
+      const int64_t count = std::min(n - first, kMaxBlocks * rows);
+      const dim3 grid((unsigned)((count + rows - 1) / rows), (unsigned)((per_row + lpr - 1) / lpr));
+      const char* p = static_cast<const char*>(ids) + first * id_bytes;
+      T* o = static_cast<T*>(out) + first * hidden;
+      if (vec)
+        embedding_rows<T, VEC><<<grid, kThreads, 0, st>>>(p, id_bytes == 8, count, w, ldw, o, vocab,
+                                                          hidden, lpr, scale);
+      else
+        embedding_rows<T, 1><<<grid, kThreads, 0, st>>>(p, id_bytes == 8, count, w, ldw, o, vocab,
                                                         hidden, lpr, scale);
-    else
-      embedding_rows<T, 1><<<grid, kThreads, 0, st>>>(ids, id_bytes == 8, n, w, ldw, o, vocab,
-                                                      hidden, lpr, scale);
+    }
     ML_LAUNCH_CHECK();
     return ML_OK;
   });

@@ -180,3 +180,15 @@ def test_dropout_past_one_launch(dev):
     for first in (0, 2 ** 34 - 512, 2 ** 35 - 512, n - 1003):
         f = ref.dropout_factors((1003,), 0.5, 10, 7, first=first)
         assert torch.equal(x[first:first + 1003].double().cpu(), f), first
+
+
+def test_lookup_past_one_launch(dev):
+    """More workgroups of four rows than a launch holds."""
+    from metal_liger_amd import fused_embedding
+    n, vocab, hidden = 2 ** 26 + 1029, 501, 129
+    w = seeded((vocab, hidden), 1, F16).to(dev)
+    ids = (torch.arange(n, dtype=torch.int32, device=dev) * 7) % vocab
+    y = fused_embedding(ids, w)
+    for first in (0, 2 ** 25 - 4096, n - 8192):
+        part = slice(first, first + 8192)
+        assert torch.equal(y[part], w[ids[part].long()]), first
