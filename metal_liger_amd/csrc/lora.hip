@@ -1438,7 +1438,8 @@ extern "C" int ml_lora_dropout_xa(int nadp, const void* X, int64_t n_tokens, int
   lora::DropRates rates{};
   int rc = drop_rates("lora dropout xa", nadp, thresholds, seed, first_stream, rates);
   if (rc) return rc;
-  ML_CHECK(n_tokens >= 0 && n_tokens < (1LL << 31), "lora dropout xa: bad token count");
+  // (32 tokens a workgroup of 512 threads, of which a launch holds fewer than 2^32)
+  ML_CHECK(n_tokens >= 0 && n_tokens <= (1LL << 28) - 32, "lora dropout xa: bad token count");
   ML_CHECK(in_features >= 8 && in_features % 8 == 0 && in_features < (1LL << 31),
            "lora dropout xa: in_features must be a positive multiple of 8");
   ML_CHECK(lora::pass_rank(rank) && rank > 0, "lora dropout xa: rank 16, 32, 48 or 64 (got %lld)",
