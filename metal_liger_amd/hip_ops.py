@@ -1327,7 +1327,8 @@ def lora_dropout_wide_fwd(x2, ws, As, Bs, scales, rank: int, seed, thresholds, f
 def lora_dropout_wide_bwd(x2, dys, ws_, packed, scales, xa, rank: int, seed, thresholds, first: int,
                           spec, dtype):
     """The backward of lora_dropout_wide_fwd, as lora_dropout_bwd (dtype fp32 where
-    spec is empty)."""
+    spec is empty). P is rounded to bf16, as the products' operand; dX is summed in
+    fp32 and rounded once."""
     ensure_rocm_device(x2, *dys, *ws_, packed, xa, seed)
     (N, IN), n, bf, dev = x2.shape, len(dys), torch.bfloat16, x2.device
     shapes = lora_dropout_grad_shapes(IN, [d.shape[1] for d in dys], rank)
@@ -1338,9 +1339,8 @@ def lora_dropout_wide_bwd(x2, dys, ws_, packed, scales, xa, rank: int, seed, thr
         return dX, lora_unpack(flat, spec, dtype) if spec else flat
     a_stack = packed[:n * rank * IN].view(n, rank, IN)
     off, dX = n * rank * IN, None
-    for dy, w in zip(dys, ws_):  # the large products' sum in fp32, rounded once
+    for dy, w in zip(dys, ws_):
         dX = matmul(dy, w, out=dX, beta=0.0 if dX is None else 1.0)
-    dX = dX.to(bf)
     for i, (dy, t) in enumerate(zip(dys, thresholds)):
         o = dy.shape[1]
         b, off = packed[off:off + o * rank].view(o, rank), off + o * rank
@@ -1348,7 +1348,8 @@ def lora_dropout_wide_bwd(x2, dys, ws_, packed, scales, xa, rank: int, seed, thr
         matmul(P, dropout(x2, None, seed, t, first + i, 1.0), a_t=True,
                out=dA[i * rank:(i + 1) * rank])
         matmul(dy, xa[:, i * rank:(i + 1) * rank], a_t=True, out=dBs[i], alpha=scales[i])
-        dX = dropout(matmul(P, a_stack[i], out_dtype=bf), dX, seed, t, first + i, 1.0)
+        dX = dropout(matmul(P, a_stack[i]), dX, seed, t, first + i, 1.0)
+    dX = dX.to(bf)
     return dX, lora_unpack(flat, spec, dtype) if spec else flat
 
 

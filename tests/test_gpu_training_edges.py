@@ -192,3 +192,32 @@ def test_lookup_past_one_launch(dev):
     for first in (0, 2 ** 25 - 4096, n - 8192):
         part = slice(first, first + 8192)
         assert torch.equal(y[part], w[ids[part].long()]), first
+
+
+# --------------------------------------------------------------- ranks above 64
+
+@pytest.mark.parametrize("n", [1, 3])
+def test_wide_ranks_round_dx_once(dev, n):
+    """dX at ranks above 64, from whole numbers whose products and sums are exact in
+    fp32 and whose P = c s dY B is exact in bf16 (at most 2 x 3 x 40 in magnitude): the
+    large products' sum and every adapter's part, rounded once."""
+    from metal_liger_amd.ops.fused_lora import _dropped
+    outs, rank = (192, 64, 72)[:n], 96
+    lins = [_linear(dev, 320, o, rank, 0.5, BF, 10 * k, alpha=float(rank)) for k, o in
+            enumerate(outs)]
+    g = torch.Generator().manual_seed(1)
+    whole = lambda *s: torch.randint(-3, 4, s, generator=g).to(BF)  # noqa: E731
+    with torch.no_grad():
+        for lin, o in zip(lins, outs):
+            lin.base_layer.weight.copy_(whole(o, 320))
+            lin.lora_A["default"].weight.copy_(whole(rank, 320))
+            b = torch.zeros(o, rank)
+            b[:40] = whole(40, rank).sign()
+            lin.lora_B["default"].weight.copy_(b)
+    x, dys = whole(130, 320), [whole(130, o) for o in outs]
+    xd = x.to(dev).requires_grad_()
+    dx, = torch.autograd.grad(_dropped(lins, xd, 5), xd, [d.to(dev) for d in dys])
+    fs = [ref.dropout_factors((130, 320), 0.5, 5, k) for k in range(n)]
+    _, want, _ = ref.lora_dropout(x, [_params(m) for m in lins], dys, fs)
+    assert want.abs().max() < 2 ** 24
+    assert torch.equal(dx.cpu(), want.to(BF))
