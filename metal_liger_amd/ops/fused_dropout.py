@@ -53,6 +53,8 @@ class _FusedDropoutFunction(torch.autograd.Function):
         dx = None
         if ctx.needs_input_grad[0] and ctx.threshold == 0:
             dx = dy
+        elif ctx.needs_input_grad[0] and torch.is_grad_enabled():  # create_graph
+            dx = _FusedDropoutFunction.apply(dy, None, seed, ctx.threshold, ctx.stream)
         elif ctx.needs_input_grad[0]:
             dx = cops.dropout(dy, None, seed, ctx.threshold, ctx.stream,
                               hip_ops.drop_scale(ctx.threshold))

@@ -32,7 +32,28 @@ class _FusedEmbeddingFunction(torch.autograd.Function):
         ids, = ctx.saved_tensors
         if dy.dtype != ctx.dtype:
             dy = dy.to(ctx.dtype)
-        return None, cops.embedding_bwd(ids, dy, ctx.vocab, ctx.padding_idx, ctx.scale), None, None
+        args = (ids, dy, ctx.vocab, ctx.padding_idx, ctx.scale)
+        grad = _EmbeddingGradFunction.apply if torch.is_grad_enabled() else cops.embedding_bwd
+        return None, grad(*args), None, None
+
+
+class _EmbeddingGradFunction(torch.autograd.Function):
+    """The table's gradient, itself differentiable (create_graph): linear in dy, whose
+    gradient is the lookup of the table that arrives, zero where an id gives none."""
+
+    @staticmethod
+    def forward(ctx, ids, dy, vocab: int, padding_idx: int, scale: float):
+        ctx.save_for_backward(ids)
+        ctx.vocab, ctx.padding_idx, ctx.scale = vocab, padding_idx, scale
+        return cops.embedding_bwd(ids, dy, vocab, padding_idx, scale)
+
+    @staticmethod
+    def backward(ctx, ddw):
+        ids, = ctx.saved_tensors
+        keep = (ids >= 0) & (ids < ctx.vocab) & (ids != ctx.padding_idx)
+        y = _FusedEmbeddingFunction.apply(ids, ddw, ctx.scale, ctx.padding_idx)
+        ddy = torch.where(keep.unsqueeze(-1), y, torch.zeros((), dtype=y.dtype, device=y.device))
+        return None, ddy, None, None, None
 
 
 def fused_embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,

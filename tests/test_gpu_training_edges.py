@@ -8,6 +8,7 @@ import torch
 
 from oracle import training_ops as ref
 from tests.parity import seeded
+from tests.test_gpu_embedding import _check_grad, _ids
 from tests.test_gpu_lora_dropout import (
     _block,
     _half,
@@ -221,3 +222,35 @@ def test_wide_ranks_round_dx_once(dev, n):
     _, want, _ = ref.lora_dropout(x, [_params(m) for m in lins], dys, fs)
     assert want.abs().max() < 2 ** 24
     assert torch.equal(dx.cpu(), want.to(BF))
+
+
+# ------------------------------------------------------------ second derivatives
+
+@pytest.mark.parametrize("training", [True, False])
+def test_dropout_twice_differentiable(dev, training):
+    """d/dy of dx's product with v is the mask over v (and v for the residual)."""
+    from metal_liger_amd import fused_dropout
+    x, res, dy, v = (seeded((33, 65), k).to(dev).requires_grad_() for k in (1, 2, 3, 4))
+    y = fused_dropout(x, 0.3, training, res, seed=77, stream=5)
+    dx, dr = torch.autograd.grad(y, [x, res], dy, create_graph=True)
+    ddy, = torch.autograd.grad([dx, dr], dy, [v, v])
+    f = ref.dropout_factors((33, 65), 0.3, 77, 5).to(dev) if training else 1.0
+    want = v.double() * f + v.double()
+    assert bool(((ddy - want).abs() <= 4 * 2.0 ** -24 * (want.abs() + v.abs())).all())
+
+
+def test_embedding_twice_differentiable(dev):
+    """d/d(dy) of the table's gradient's product with v is the lookup of v: zero for
+    the padding index and for ids outside the table; a third derivative follows."""
+    from metal_liger_amd import fused_embedding
+    w, v = (seeded((20, 24), k).to(dev).requires_grad_() for k in (1, 2))
+    ids = torch.tensor([[3, -1, 20], [5, 7, 3]], device=dev)
+    dy = seeded((2, 3, 24), 3).to(dev).requires_grad_()
+    dw, = torch.autograd.grad(fused_embedding(ids, w, 1.5, 7), w, dy, create_graph=True)
+    _check_grad(dw, ids, dy.detach(), 20, 1.5, 7)
+    ddy, = torch.autograd.grad(dw, dy, v, create_graph=True)
+    keep = torch.tensor([[1, 0, 0], [1, 0, 1]], device=dev, dtype=torch.bool)
+    want = torch.where(keep[..., None], 1.5 * v[ids.clamp(0, 19)], torch.zeros((), device=dev))
+    assert torch.equal(ddy, want)
+    u = seeded((2, 3, 24), 4).to(dev)
+    _check_grad(torch.autograd.grad(ddy, v, u)[0], ids, u, 20, 1.5, 7)
