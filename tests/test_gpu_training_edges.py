@@ -254,3 +254,35 @@ def test_embedding_twice_differentiable(dev):
     assert torch.equal(ddy, want)
     u = seeded((2, 3, 24), 4).to(dev)
     _check_grad(torch.autograd.grad(ddy, v, u)[0], ids, u, 20, 1.5, 7)
+
+
+# -------------------------------------------------------------- compiled, drawn
+
+def test_compile_with_a_drawn_seed(dev):
+    """The seed is drawn inside the compiled step: one mask both ways, another at the
+    next call, and the same again from the same state of torch's generator."""
+    from metal_liger_amd import apply_fused_lora_qkv, fused_dropout
+    x = torch.ones(64, 128, device=dev, requires_grad=True)
+    step = torch.compile(lambda t: fused_dropout(t, 0.5), fullgraph=True, backend="aot_eager")
+    torch.manual_seed(1)
+    a, b = step(x), step(x)
+    for y in (a, b):
+        dx, = torch.autograd.grad(y, x, torch.ones_like(y))
+        assert torch.equal(dx, y)
+        assert set(y.unique().tolist()) == {0.0, 2.0}
+    torch.manual_seed(1)
+    assert torch.equal(step(x), a) and not torch.equal(a, b)
+
+    lins = [_linear(dev, 128, o, 16, 0.4, BF, 10 * k) for k, o in enumerate((128, 64, 64))]
+    attn = _block(q_proj=lins[0], k_proj=lins[1], v_proj=lins[2])
+    xb = seeded((50, 128), 1, BF).to(dev).requires_grad_()
+    fn = torch.compile(lambda t: apply_fused_lora_qkv(attn, t, lora_dropout=True), fullgraph=True,
+                       backend="aot_eager")
+    dys = [seeded((50, o), 2, BF).to(dev) for o in (128, 64, 64)]
+    runs = []
+    for _ in range(2):
+        torch.manual_seed(2)
+        ys = fn(xb)
+        runs.append([*ys, *torch.autograd.grad(ys, xb, dys)])
+    assert all(torch.equal(p, q) for p, q in zip(*runs))
+    assert not torch.equal(fn(xb)[0], runs[0][0])
