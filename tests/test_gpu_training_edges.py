@@ -286,3 +286,36 @@ def test_compile_with_a_drawn_seed(dev):
         runs.append([*ys, *torch.autograd.grad(ys, xb, dys)])
     assert all(torch.equal(p, q) for p, q in zip(*runs))
     assert not torch.equal(fn(xb)[0], runs[0][0])
+
+
+# ----------------------------------------------- several tiles of ids, and merges
+
+@pytest.mark.parametrize("kind", ["uniform", "same", "half"])
+@pytest.mark.parametrize("vocab, tokens", [
+    (262144, 8193), (262145, 70001),          # 64-bit entries: two tiles, a full merge
+    (30011, 140003), (262143, 131073),        # 32-bit entries, two levels of merging
+    (262144, 65537), (300007, 150001)])       # 64-bit entries, two levels
+def test_merged_orders(dev, vocab, tokens, kind):
+    """Scattered ids over more tokens than one sorted tile, or one merge, holds; every
+    token's row is another one, so that a wrong or repeated position shows."""
+    ids = _ids(kind, tokens, vocab, seed=tokens)
+    dy = seeded((tokens, 8), 2)
+    dw = torch.ops.metal_liger_amd.embedding_bwd(ids.to(dev), dy.to(dev), vocab, -1, 1.0)
+    _check_grad(dw, ids, dy, vocab)
+
+
+def test_offsets_of_a_gradient_past_32_bits(dev):
+    """An output's gradient of more than 2^31 elements with scattered ids: the rows
+    past that, and those that a wrapped offset would read instead, have values of
+    their own."""
+    n, hidden, vocab = (1 << 19) + 3, 4104, 5003
+    dy = torch.zeros(n, hidden, dtype=BF, device=dev)
+    special = torch.tensor([0, 1, 2, 777, (1 << 31) // hidden - 1, (1 << 31) // hidden,
+                            (1 << 31) // hidden + 1, n - 3, n - 2, n - 1])
+    for k, t in enumerate(special.tolist()):
+        dy[t] = float(k + 1)
+    ids = _ids("uniform", n, vocab, seed=9)
+    dw = torch.ops.metal_liger_amd.embedding_bwd(ids.to(dev), dy, vocab, -1, 1.0)
+    want = torch.zeros(vocab)                           # sums of small whole numbers: exact
+    want.index_add_(0, ids[special], torch.arange(1.0, len(special) + 1))
+    assert torch.equal(dw.float().cpu(), want[:, None].expand(vocab, hidden))
