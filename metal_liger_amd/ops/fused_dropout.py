@@ -93,8 +93,8 @@ class MetalLigerDropout(nn.Module):
             raise ValueError("MetalLigerDropout: inplace is not supported")
         self.p, self.inplace = p, False
 
-    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
-        return fused_dropout(x, self.p, self.training, residual)
+    def forward(self, input: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        return fused_dropout(input, self.p, self.training, residual)
 
     def extra_repr(self) -> str:
         return f"p={self.p}"

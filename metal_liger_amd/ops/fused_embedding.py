@@ -95,8 +95,8 @@ class MetalLigerEmbedding(nn.Module):
         self.num_embeddings, self.embedding_dim = original.weight.shape
         self.padding_idx, self.scale = original.padding_idx, scale
 
-    def forward(self, ids: torch.Tensor) -> torch.Tensor:
-        return fused_embedding(ids, self.weight, self.scale, self.padding_idx)
+    def forward(self, input: torch.Tensor) -> torch.Tensor:
+        return fused_embedding(input, self.weight, self.scale, self.padding_idx)
 
     def extra_repr(self) -> str:
         return f"{self.num_embeddings}, {self.embedding_dim}, scale={self.scale}"
@@ -108,8 +108,8 @@ class _FusedEmbeddingForward:
     def __init__(self, module: nn.Embedding):
         self.module = module
 
-    def __call__(self, ids):
-        return fused_embedding(ids, self.module.weight, padding_idx=self.module.padding_idx)
+    def __call__(self, input):
+        return fused_embedding(input, self.module.weight, padding_idx=self.module.padding_idx)
 
 
 def patch_embedding(model: nn.Module) -> int:

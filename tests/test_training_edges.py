@@ -1,6 +1,10 @@
 """Dropout, LoRA dropout and the embedding without a GPU: sizes that a launch cannot
 hold, and what the drop-in modules and the patcher leave as torch has it."""
 
+import pytest
+import torch
+import torch.nn as nn
+
 
 def test_lora_dropout_refuses_more_tokens_than_a_launch_holds():
     from metal_liger_amd import _hip
@@ -9,3 +13,20 @@ def test_lora_dropout_refuses_more_tokens_than_a_launch_holds():
     for tokens in (-1, (1 << 28) - 31, 1 << 28, (1 << 31) - 1):
         rc = L.ml_lora_dropout_xa(1, p, tokens, 64, 64, p, 16, _hip.geom([100]), p, 0, p, 16, None)
         assert rc == 1 and b"token count" in L.ml_last_error(), (tokens, L.ml_last_error())
+
+
+def test_the_modules_take_their_argument_by_torch_s_name():
+    """(On the CPU the call gets as far as the check of the device.)"""
+    from metal_liger_amd import MetalLigerDropout, MetalLigerEmbedding
+    from metal_liger_amd.ops.fused_embedding import patch_embedding
+    root = nn.Module()
+    root.embed_tokens = nn.Embedding(8, 4)
+    assert patch_embedding(root) == 1
+    x, ids = torch.zeros(4), torch.zeros(3, dtype=torch.long)
+    for call in (lambda: MetalLigerDropout(0.5)(input=x),
+                 lambda: MetalLigerDropout(0.5)(input=x, residual=x),
+                 lambda: MetalLigerEmbedding(nn.Embedding(8, 4))(input=ids),
+                 lambda: root.embed_tokens(input=ids)):
+        with pytest.raises(ValueError, match="ROCm GPU"):
+            call()
+    assert MetalLigerDropout(0.5).eval()(input=x) is x
