@@ -256,6 +256,26 @@ def test_embedding_twice_differentiable(dev):
     _check_grad(torch.autograd.grad(ddy, v, u)[0], ids, u, 20, 1.5, 7)
 
 
+def test_lookup_without_a_gradient(dev):
+    """A frozen table, or a trained one where no gradient is formed: the same values,
+    nothing kept for a backward; a routed module follows its table."""
+    from metal_liger_amd import fused_embedding
+    from metal_liger_amd.ops.fused_embedding import patch_embedding
+    root = torch.nn.Module()
+    root.embed_tokens = torch.nn.Embedding(50, 24, device=dev)
+    assert patch_embedding(root) == 1
+    w, ids = root.embed_tokens.weight, torch.randint(0, 50, (3, 7), device=dev)
+    y = root.embed_tokens(ids)
+    assert "FusedEmbedding" in type(y.grad_fn).__name__ and torch.equal(y, w[ids])
+    with torch.no_grad():
+        assert torch.equal(fused_embedding(ids, w, 2.0), 2 * w[ids])
+    w.requires_grad_(False)
+    for y in (fused_embedding(ids, w), root.embed_tokens(ids)):
+        assert y.grad_fn is None and torch.equal(y, w[ids])
+    step = torch.compile(lambda i: fused_embedding(i, w, 2.0), fullgraph=True, backend="aot_eager")
+    assert torch.equal(step(ids), 2 * w[ids])
+
+
 # -------------------------------------------------------------- compiled, drawn
 
 def test_compile_with_a_drawn_seed(dev):

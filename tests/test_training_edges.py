@@ -30,3 +30,15 @@ def test_the_modules_take_their_argument_by_torch_s_name():
         with pytest.raises(ValueError, match="ROCm GPU"):
             call()
     assert MetalLigerDropout(0.5).eval()(input=x) is x
+
+
+def test_a_routed_embedding_is_torch_s_own_while_its_table_is_frozen():
+    from metal_liger_amd.ops.fused_embedding import patch_embedding
+    root = nn.Module()
+    root.embed_tokens = nn.Embedding(8, 4, padding_idx=2).requires_grad_(False)
+    assert patch_embedding(root) == 1
+    ids = torch.tensor([[1, 2], [7, 1]])
+    assert torch.equal(root.embed_tokens(ids), root.embed_tokens.weight[ids])
+    root.embed_tokens.requires_grad_(True)               # trained from here on
+    with pytest.raises(ValueError, match="ROCm GPU"):
+        root.embed_tokens(ids)
