@@ -493,7 +493,8 @@ int ml_lora_xa(const void* X, int64_t n_tokens, int64_t in_features, int64_t ldx
  * in_features] (bf16). Adapter i drops by ml_dropout's mask M_i over X's elements
  * in row-major order: threshold thresholds[i], stream first_stream + i, *seed (one
  * int64 in DEVICE memory); c_i = 65536 / (65536 - threshold), 0 at 65536. rank (16,
- * 32, 48 or 64) of every adapter; in_features a multiple of 8.
+ * 32, 48 or 64) of every adapter; in_features a multiple of 8; n_tokens at most
+ * 2^28 - 32.
  *
  * ml_lora_dropout_xa: XA [n_tokens, nadp rank] (row stride ldo), column block i =
  * c_i (M_i X) A_i^T; A_stack as ml_lora_dropout_pack lays down A_0 .. one after

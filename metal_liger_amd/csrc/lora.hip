@@ -1414,6 +1414,10 @@ extern "C" int ml_lora_linear_bwd(const void* X, int64_t n_tokens, int64_t in_fe
 
 // ---------------------------------------------------------------- dropout --
 
+// X A^T takes 32 tokens a workgroup of 512 threads, of which a launch holds fewer than
+// 2^32; the passes count rows in 32 bits.
+constexpr int64_t kDropMaxTokens = (1LL << 28) - 32;
+
 static int drop_rates(const char* what, int n, const int64_t* thresholds, const int64_t* seed,
                       int64_t first_stream, lora::DropRates& r) {
   ML_CHECK(n >= 1 && n <= lora::kDropMaxAdapters, "%s: 1..%d adapters (got %d)", what,
@@ -1438,8 +1442,7 @@ extern "C" int ml_lora_dropout_xa(int nadp, const void* X, int64_t n_tokens, int
   lora::DropRates rates{};
   int rc = drop_rates("lora dropout xa", nadp, thresholds, seed, first_stream, rates);
   if (rc) return rc;
-  // (32 tokens a workgroup of 512 threads, of which a launch holds fewer than 2^32)
-  ML_CHECK(n_tokens >= 0 && n_tokens <= (1LL << 28) - 32, "lora dropout xa: bad token count");
+  ML_CHECK(n_tokens >= 0 && n_tokens <= kDropMaxTokens, "lora dropout xa: bad token count");
   ML_CHECK(in_features >= 8 && in_features % 8 == 0 && in_features < (1LL << 31),
            "lora dropout xa: in_features must be a positive multiple of 8");
   ML_CHECK(lora::pass_rank(rank) && rank > 0, "lora dropout xa: rank 16, 32, 48 or 64 (got %lld)",
@@ -1486,7 +1489,7 @@ extern "C" int ml_lora_dropout_bwd(int nadp, const void* X, int64_t n_tokens, in
   lora::DropRates rates{};
   int rc = drop_rates(what, nadp, thresholds, seed, first_stream, rates);
   if (rc) return rc;
-  ML_CHECK(n_tokens > 0 && n_tokens < (1LL << 31), "%s: bad token count", what);
+  ML_CHECK(n_tokens > 0 && n_tokens <= kDropMaxTokens, "%s: bad token count", what);
   ML_CHECK(in_features >= 8 && in_features % 8 == 0 && in_features < (1LL << 31),
            "%s: in_features must be a positive multiple of 8", what);
   ML_CHECK(rank > 0 && lora::pass_rank(rank), "%s: rank 16, 32, 48 or 64 (got %lld)", what,

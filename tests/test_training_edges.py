@@ -13,6 +13,11 @@ def test_lora_dropout_refuses_more_tokens_than_a_launch_holds():
     for tokens in (-1, (1 << 28) - 31, 1 << 28, (1 << 31) - 1):
         rc = L.ml_lora_dropout_xa(1, p, tokens, 64, 64, p, 16, _hip.geom([100]), p, 0, p, 16, None)
         assert rc == 1 and b"token count" in L.ml_last_error(), (tokens, L.ml_last_error())
+        one = _hip.ptrs([p])
+        rc = L.ml_lora_dropout_bwd(1, p, tokens, 64, one, _hip.geom([64]), one, p, one,
+                                   _hip.floats([1.0]), p, 16, _hip.geom([100]), p, 0, p, p, one, 0,
+                                   p, 16, None)
+        assert rc == 1 and b"token count" in L.ml_last_error(), (tokens, L.ml_last_error())
 
 
 def test_the_modules_take_their_argument_by_torch_s_name():
