@@ -313,10 +313,11 @@ def _(x2, w):
 
 
 # Dropout, the embedding, LoRA with dropout and the packing and unpacking of
-# adapters, registered without custom_op's wrapper: the wrapper costs the host 4.7 us a call with lists of tensors (7.9 against 3.2
-# for an op that only allocates), which made few-token passes slower than the
-# tensor operations that each of these replaces ([205, 1024] to 1024 at rank 8, a
-# pass on one thread: 186 us by those operations, 202 through custom_op).
+# adapters are registered without custom_op's wrapper, which costs the host 4.7 us a
+# call with lists of tensors (7.9 against 3.2 for an op that only allocates). Through
+# it, the packing and unpacking made few-token passes slower than the tensor
+# operations that they replace ([205, 1024] to 1024 at rank 8, a pass on one thread:
+# 186 us by those operations, 202 through custom_op).
 _LIB = torch.library.Library(NS, "FRAGMENT")
 
 
@@ -340,8 +341,8 @@ def _define(schema: str, fn, fake):
     return getattr(getattr(torch.ops, NS), name).default
 
 
-dropout = _define("dropout(Tensor x, Tensor? residual, Tensor? seed, SymInt threshold, SymInt stream, "
-                  "float scale) -> Tensor", hip_ops.dropout,
+dropout = _define("dropout(Tensor x, Tensor? residual, Tensor? seed, SymInt threshold, "
+                  "SymInt stream, float scale) -> Tensor", hip_ops.dropout,
                   lambda x, residual, seed, threshold, stream, scale: x.new_empty(x.shape))
 embedding_fwd = _define("embedding_fwd(Tensor ids, Tensor weight, float scale) -> Tensor",
                         hip_ops.embedding_fwd,

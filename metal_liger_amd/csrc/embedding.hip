@@ -2,9 +2,10 @@
 // reference counterpart: nn.Embedding is left to torch there).
 //
 //   y[n]  = scale * W[id_n]
-//   dW[v] = scale * sum over the n with id_n = v, in ascending order, of dy[n]
+//   dW[v] = scale * sum over the n with id_n = v of dy[n]
 //
-// Sums are held in fp32 and rounded once. An id outside the table gives a row of
+// Sums are held in fp32 and rounded once; their order (below) follows from the ids and
+// their number alone. An id outside the table gives a row of
 // NaN and no gradient; rows of dW that no token names, and the row of the padding
 // index, are zero.
 //
@@ -16,8 +17,9 @@
 //   merge  up to 8 sorted runs at a time (none for one tile);
 //   sum    chunks of the sorted order: a run of equal ids inside a chunk is summed
 //          and stored; what crosses a chunk's end is left as an fp32 partial;
-//   join   the partials of each such run, in the chunks' order.
-// Chunks and order follow from the ids alone, so that the sums do too.
+//   join   the partials of each such run.
+// A chunk adds its tokens in ascending order; a run of up to 16 chunks more adds their
+// partials two by two, a longer one every 16th chunk to one of 16 sums, then those.
 #include <math.h>
 
 #include <algorithm>
@@ -303,7 +305,7 @@ __global__ __launch_bounds__(kThreads) void sum_chunks(const uint64_t* __restric
     finish();
 }
 
-// The runs that cross chunks: their partials added in the chunks' order. Every
+// The runs that cross chunks: their partials added in a fixed order. Every
 // workgroup lists the chunks in which such a run begins (a thread a chunk) and takes
 // its share of the (run, column slice) items: a wave sums a run of a few chunks, 256
 // columns at a time; a long one (an image's or a padding token) takes the workgroup, 64

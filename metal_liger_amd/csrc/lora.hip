@@ -270,12 +270,12 @@ __global__ __launch_bounds__(256) void dy_pass_kernel(const DyArgs args) {
 }
 
 // The fixed-order partial sums of a dY pass, every adapter's P (bf16) and dB
-// (fp32) in one launch: blockIdx.y picks the job. Same arithmetic as
+// (fp32, or bf16: rounded once) in one launch: blockIdx.y picks the job. Same arithmetic as
 // reduce_partials_kernel (splits summed in order, then scaled); N = 16.
 struct DyReduceJob {
   const float* part;
   int splits, rows;
-  void* out;  // bf16 (P) or fp32 (dB), row stride ld
+  void* out;  // fp32 where out_f32 (dB), else bf16 (P, or dB); row stride ld
   int64_t ld;
   float scale;
   int out_f32;
@@ -320,8 +320,8 @@ __global__ __launch_bounds__(256) void dy_reduce_kernel(const DyReduceArgs args)
 }
 
 // Host side of the dY pass for up to kDyMaxJobs jobs of one layer. ws holds
-// every job's partials; P_i (bf16, row stride ldp) and dB_i (fp32 [O_i,
-// ldb_out]) receive s_i times the sums.
+// every job's partials; P_i (bf16, row stride ldp) receives pscale times its sums
+// (s_i, under dropout c_i s_i) and dB_i (fp32 or bf16, row stride lddb) scale times.
 struct DyJob {
   const bf16* dy;
   int64_t ldy;
@@ -955,7 +955,8 @@ struct PackArgs {
 // hold of 16 rows and 32 columns in the MFMA operand layout (lane l: row l % 16,
 // columns 8 (l / 16) ..) is 1 KB in one piece, the rows' 16-row slices of a 32-column
 // step behind one another. A wave's load of a fragment is then a row of memory instead
-// of 16 pieces of 64 bytes (X A^T under dropout, [1777, 6144] x 32: 18.5 -> 13.3 us).
+// of 16 pieces of 64 bytes (X A^T under dropout inside a pass, [1777, 6144] x 32: 24 ->
+// 19 us; over the same X again and again 14).
 __device__ __forceinline__ int64_t frag_offset(int r, int c, int rows) {
   const int lane = (r & 15) + 16 * ((c >> 3) & 3);
   return (((int64_t)(c >> 5) * (rows >> 4) + (r >> 4)) * 64 + lane) * 8;

@@ -190,8 +190,8 @@ def dropout(x: torch.Tensor, residual: torch.Tensor | None, seed: torch.Tensor |
         residual = residual.contiguous()
     x = x.contiguous()
     out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    call("ml_dropout", ptr(x), ptr(residual), ptr(out), x.numel(), threshold, float(scale), ptr(seed),
-         stream, dtype_tag(x, "x"), stream_of(x))
+    call("ml_dropout", ptr(x), ptr(residual), ptr(out), x.numel(), threshold, float(scale),
+         ptr(seed), stream, dtype_tag(x, "x"), stream_of(x))
     return out
 
 
@@ -1036,8 +1036,9 @@ def lora_pack(As, Bs, scales, rank: int, frag: bool = False) -> torch.Tensor:
     scaled = [None] * len(As) + [p + 2 * (n_all - n_a) for p in dst[len(As):]]
     name, head = ("ml_lora_dropout_pack", (len(srcs), len(As))) if frag else ("ml_lora_pack",
                                                                              (len(srcs),))
-    call(name, *head, _hip.ptrs([t.data_ptr() for t in srcs]), geom(dims), _hip.ints(tags), _hip.floats([1.0] * len(As) + list(scales)), _hip.ptrs(dst),
-         _hip.ptrs(scaled), stream_of(flat))
+    call(name, *head, _hip.ptrs([t.data_ptr() for t in srcs]), geom(dims), _hip.ints(tags),
+         _hip.floats([1.0] * len(As) + list(scales)), _hip.ptrs(dst), _hip.ptrs(scaled),
+         stream_of(flat))
     return flat
 
 

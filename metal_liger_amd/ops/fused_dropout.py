@@ -11,9 +11,13 @@ that.
 The seed is one int64 on the GPU. By default each call draws it from torch's
 generator of the device, so that torch.manual_seed reproduces a run, activation
 checkpointing recomputes the same mask and a captured step gets a new one at each
-replay. A seed given as a tensor is read when the kernels run: changing it between
-a forward and its backward is an error that autograd reports, and changing it
-between replays gives each its own masks. An int is the same mask at each call.
+replay; where nothing is dropped none is drawn. A seed given as a tensor is read when
+the kernels run: changing it between a forward and its backward is an error that
+autograd reports, and changing it between replays gives each its own masks. An int is
+the same mask at each call.
+
+The backward can be differentiated again; forward mode and torch.func's transforms
+are refused.
 """
 
 from __future__ import annotations

@@ -1,20 +1,17 @@
 """Fused token embedding on MI355X: the lookup with its scaling, and the gradient
 of the table (no counterpart in the reference, whose models keep nn.Embedding).
 
-The gradient sums the tokens' rows in fp32 in an order that the ids alone decide,
-so that it is bit-reproducible, and rounds once.
+The gradient sums the tokens' rows in fp32 in an order that the ids and their number
+alone decide, so that it is bit-reproducible, and rounds once. Both directions can be
+differentiated again; forward mode and torch.func's transforms are refused.
 """
 
 from __future__ import annotations
-
-import logging
 
 import torch
 import torch.nn as nn
 
 from metal_liger_amd import _custom_ops as cops
-
-logger = logging.getLogger(__name__)
 
 
 class _FusedEmbeddingFunction(torch.autograd.Function):
@@ -89,8 +86,8 @@ class MetalLigerEmbedding(nn.Module):
     def __init__(self, original: nn.Embedding, scale: float = 1.0):
         super().__init__()
         if not _fusable(original):
-            raise ValueError("MetalLigerEmbedding: a plain nn.Embedding without max_norm, sparse or "
-                             f"scale_grad_by_freq is needed (got {original})")
+            raise ValueError("MetalLigerEmbedding: a plain nn.Embedding without max_norm, sparse "
+                             f"or scale_grad_by_freq is needed (got {original})")
         self.weight = original.weight
         self.num_embeddings, self.embedding_dim = original.weight.shape
         self.padding_idx, self.scale = original.padding_idx, scale

@@ -679,7 +679,8 @@ def apply_fused_lora_mlp(mlp_module, X: torch.Tensor, lora_dropout: bool = False
             # _LoRA_MLP: rounded to fp16 between the projections, h would overflow
             # where the block without dropout does not
             x = X.float() if fp32 else X
-            gate, up = _LoRA_Dropout.apply(x, seed, thresholds[:2], 0, GW, GA, GB, GS, UW, UA, UB, US)
+            gate, up = _LoRA_Dropout.apply(x, seed, thresholds[:2], 0, GW, GA, GB, GS,
+                                           UW, UA, UB, US)
             return _LoRA_Dropout.apply(fused_swiglu(gate, up), seed, thresholds[2:], 2,
                                        DW, DA, DB, DS)[0].to(X.dtype)
     return _LoRA_MLP.apply(

@@ -128,7 +128,8 @@ def test_one_row_of_an_odd_stride_through_the_loss(dev):
     loss = MetalLigerFusedLinearCrossEntropy(head)
     dense = x.clone(memory_format=torch.contiguous_format)
     runs = []
-    for t in (x, dense, wide[:1, :128], wide[:1, :128].clone(memory_format=torch.contiguous_format)):
+    first = wide[:1, :128]
+    for t in (x, dense, first, first.clone(memory_format=torch.contiguous_format)):
         t = t.detach().requires_grad_()
         y = loss(t, labels)
         runs.append([y, *torch.autograd.grad(y, [t, head.weight])])
@@ -254,6 +255,21 @@ def test_embedding_twice_differentiable(dev):
     assert torch.equal(ddy, want)
     u = seeded((2, 3, 24), 4).to(dev)
     _check_grad(torch.autograd.grad(ddy, v, u)[0], ids, u, 20, 1.5, 7)
+
+
+def test_other_derivatives_are_refused(dev):
+    """Forward mode and torch.func say so instead of leaving a derivative out."""
+    import torch.autograd.forward_ad as fw
+
+    from metal_liger_amd import fused_dropout, fused_embedding
+    x = seeded((20, 24), 1).to(dev)
+    ids = torch.tensor([3, 5], device=dev)
+    for fn in (lambda t: fused_dropout(t, 0.5, seed=3), lambda t: fused_embedding(ids, t),
+               lambda t: fused_dropout(t, 0.5, training=False, residual=x)):
+        with pytest.raises(RuntimeError):
+            torch.func.grad(lambda t: fn(t).sum())(x)
+        with fw.dual_level(), pytest.raises((RuntimeError, NotImplementedError)):
+            fn(fw.make_dual(x, torch.ones_like(x)))
 
 
 def test_lookup_without_a_gradient(dev):
