@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define ML_ABI_VERSION 12
+#define ML_ABI_VERSION 13
 
 /* dtype tags */
 #define ML_F32 0

@@ -191,7 +191,7 @@ SIGNATURES: dict[str, tuple] = {
     ),
 }
 
-ABI_VERSION = 12
+ABI_VERSION = 13
 
 _lib = None
 _lock = threading.Lock()

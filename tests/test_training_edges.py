@@ -47,3 +47,14 @@ def test_a_routed_embedding_is_torch_s_own_while_its_table_is_frozen():
     root.embed_tokens.requires_grad_(True)               # trained from here on
     with pytest.raises(ValueError, match="ROCm GPU"):
         root.embed_tokens(ids)
+
+
+def test_a_seed_may_be_missing_only_where_nothing_is_dropped():
+    from metal_liger_amd import _hip
+    L = _hip.lib()
+    assert L.ml_abi_version() >= 13
+    assert L.ml_dropout(4096, None, 4096, 0, 0, 1.0, None, 0, 0, None) == 0    # nothing to do
+    rc = L.ml_dropout(4096, None, 4096, 8, 1, 1.0, None, 0, 0, None)
+    assert rc == 1 and b"null pointer" in L.ml_last_error()
+    rc = L.ml_dropout(4096, None, 4096, 8, 0, 1.0, None, 0, 9, None)           # past the pointers
+    assert rc == 1 and b"dtype" in L.ml_last_error()
