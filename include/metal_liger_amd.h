@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define ML_ABI_VERSION 13
+#define ML_ABI_VERSION 14
 
 /* dtype tags */
 #define ML_F32 0
@@ -637,6 +637,92 @@ int ml_gemm_f32_segments_ws(int64_t M, int64_t N, int nseg, const int64_t* k_len
                             const void* const* b_ptrs, const int64_t* ldbs, int a_layout,
                             int b_layout, float* C, int64_t ldc, float alpha, float beta,
                             void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------ feed-forward
+ * Linear layers with what surrounds them, and the gated block, forward and
+ * backward (no reference counterpart: its models keep nn.Linear, and its SwiGLU
+ * fuses the activation step only, ops/fused_swiglu.py:59-75). dtype ML_F32 or
+ * ML_BF16; bf16 operands of a product have 16-byte aligned bases, and columns and
+ * row strides in multiples of 8.
+ *
+ * What a backward needs of its forward's inner tensors is kept as `keep` says:
+ * ML_KEEP_SAME, dense in dtype; ML_KEEP_FP8, one byte an element [rows, cols] and
+ * one scale byte for every 32 columns of a row [rows, ceil(cols / 32)]: with
+ * e = max(floor(log2 m) - 7, -126) for the largest finite magnitude m of the 32
+ * (m = 0: -126) the scale's byte is e + 127, an element's is e4m3 of v / 2^e
+ * (nearest, ties to even; NaN where v is not finite). The bits are formed of the
+ * fp32 values, before any other rounding. Buffers are 16-byte aligned.
+ */
+#define ML_KEEP_NONE 0
+#define ML_KEEP_SAME 1
+#define ML_KEEP_FP8 2
+
+/* activations: z, z sigmoid(z), z Phi(z), and the latter by tanh */
+#define ML_ACT_NONE 0
+#define ML_ACT_SILU 1
+#define ML_ACT_GELU 2
+#define ML_ACT_GELU_TANH 3
+
+/*
+ *   z = x W^T + bias, y = act(z) + residual
+ * x [M, K] (ldx), W [N, K] (ldw), bias [N] or NULL, residual [M, N] (ldr) or NULL,
+ * y [M, N] (ldy); z kept in z (and zscale) as keep says. fp32 sums, y rounded once.
+ */
+size_t ml_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype);
+int ml_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                  const void* residual, int64_t ldr, int act, void* y, int64_t ldy, int keep,
+                  void* z, void* zscale, int64_t M, int64_t N, int64_t K, void* workspace,
+                  size_t workspace_bytes, int dtype, void* stream);
+
+/*
+ * Its backward, of dy [M, N] (ldy) and the kept z (act not ML_ACT_NONE):
+ *   dz = dy act'(z), dx = dz W [M, K], dw = dz^T x [N, K], db = column sums of dz [N]
+ * each dense, or NULL where it is not wanted (then w, or x, may be NULL as well).
+ * db is summed in fp32 before dz is rounded, in a fixed order.
+ */
+size_t ml_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int act, int dtype);
+int ml_linear_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* dy,
+                  int64_t ldy, int act, int keep, const void* z, const void* zscale, void* dx,
+                  void* dw, void* db, int64_t M, int64_t N, int64_t K, void* workspace,
+                  size_t workspace_bytes, int dtype, void* stream);
+
+/*
+ *   g = x Wg^T, u = x Wu^T, h = silu(g) u, y = h Wd^T + residual
+ * x [M, H], Wg and Wu [I, H], Wd [O, I], residual [M, O] or NULL, y [M, O] dense;
+ * g and u kept as keep says. h is rounded to dtype between the products.
+ */
+size_t ml_swiglu_mlp_fwd_workspace_bytes(int64_t M, int64_t H, int64_t I, int64_t O, int dtype);
+int ml_swiglu_mlp_fwd(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu,
+                      int64_t ldu, const void* wd, int64_t ldd, const void* residual, int64_t ldr,
+                      void* y, int keep, void* gate, void* gate_scale, void* up, void* up_scale,
+                      int64_t M, int64_t H, int64_t I, int64_t O, void* workspace,
+                      size_t workspace_bytes, int dtype, void* stream);
+
+/*
+ * Its backward, of dy [M, O] (ldy) and the kept g and u: dx [M, H], dwg and dwu
+ * [I, H], dwd [O, I], each dense, or NULL where it is not wanted. h is formed again
+ * of the kept g and u; dg, du and h are rounded to dtype between the products.
+ */
+size_t ml_swiglu_mlp_bwd_workspace_bytes(int64_t M, int64_t H, int64_t I, int64_t O, int dtype);
+int ml_swiglu_mlp_bwd(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu,
+                      int64_t ldu, const void* wd, int64_t ldd, const void* dy, int64_t ldy,
+                      int keep, const void* gate, const void* gate_scale, const void* up,
+                      const void* up_scale, void* dx, void* dwg, void* dwu, void* dwd, int64_t M,
+                      int64_t H, int64_t I, int64_t O, void* workspace, size_t workspace_bytes,
+                      int dtype, void* stream);
+
+/*
+ * SwiGLU whose backward reads gate and up as 8 bits hold them (ops/fused_swiglu.py:
+ * 26-50 keeps them whole): out = silu(gate) up of the inputs themselves, gate and up
+ * [rows, cols] written to *_q and *_scale as ML_KEEP_FP8; all dense, any dtype and
+ * alignment of gate, up and out. The backward: dgate and dup of dy.
+ */
+int ml_swiglu_kept_fwd(const void* gate, const void* up, void* out, void* gate_q,
+                       void* gate_scale, void* up_q, void* up_scale, int64_t rows, int64_t cols,
+                       int dtype, void* stream);
+int ml_swiglu_kept_bwd(const void* gate_q, const void* gate_scale, const void* up_q,
+                       const void* up_scale, const void* dy, void* dgate, void* dup, int64_t rows,
+                       int64_t cols, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

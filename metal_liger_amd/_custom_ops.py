@@ -353,6 +353,62 @@ embedding_bwd = _define("embedding_bwd(Tensor ids, Tensor dy, SymInt vocab, SymI
                         dy.new_empty((vocab, dy.shape[-1])))
 
 
+def _kept_fake(x2, cols, keep):
+    rows = x2.shape[0]
+    if keep == hip_ops.KEEP_FP8:
+        return [x2.new_empty(s, dtype=torch.uint8) for s in hip_ops.kept_shapes((rows, cols))]
+    return [x2.new_empty((rows, cols) if keep == hip_ops.KEEP_SAME else (0,)),
+            x2.new_empty((0,), dtype=torch.uint8)]
+
+
+def _swiglu_kept_fake(gate, up):
+    shapes = 2 * hip_ops.kept_shapes(gate.shape)
+    return (gate.new_empty(gate.shape), *(gate.new_empty(s, dtype=torch.uint8) for s in shapes))
+
+
+def _linear_fwd_fake(x2, w, bias, residual, act, keep):
+    N = w.shape[0]
+    return (x2.new_empty((x2.shape[0], N)), *_kept_fake(x2, N, keep))
+
+
+def _linear_bwd_fake(x2, w, dy, act, keep, z, zscale, N, K, need_dx, need_dw, need_db):
+    return (dy.new_empty((dy.shape[0], K) if need_dx else (0,)),
+            dy.new_empty((N, K) if need_dw else (0,)), dy.new_empty((N,) if need_db else (0,)))
+
+
+def _swiglu_mlp_fwd_fake(x2, wg, wu, wd, residual, keep):
+    return (x2.new_empty((x2.shape[0], wd.shape[0])), *_kept_fake(x2, wd.shape[1], keep),
+            *_kept_fake(x2, wd.shape[1], keep))
+
+
+def _swiglu_mlp_bwd_fake(x2, wg, wu, wd, dy, keep, gate, gate_scale, up, up_scale, *needs):
+    shapes = (x2.shape, wg.shape, wu.shape, wd.shape)
+    return tuple(x2.new_empty(s if need else (0,)) for s, need in zip(shapes, needs))
+
+
+swiglu_kept_fwd = _define("swiglu_kept_fwd(Tensor gate, Tensor up) -> "
+                          "(Tensor, Tensor, Tensor, Tensor, Tensor)", hip_ops.swiglu_kept_fwd,
+                          _swiglu_kept_fake)
+swiglu_kept_bwd = _define("swiglu_kept_bwd(Tensor gate_q, Tensor gate_scale, Tensor up_q, "
+                          "Tensor up_scale, Tensor dy, ScalarType gate_dtype, ScalarType up_dtype)"
+                          " -> (Tensor, Tensor)", hip_ops.swiglu_kept_bwd,
+                          lambda gq, gs, uq, us, dy, gt, ut: (dy.new_empty(dy.shape, dtype=gt),
+                                                              dy.new_empty(dy.shape, dtype=ut)))
+linear_fwd = _define("linear_fwd(Tensor x2, Tensor w, Tensor? bias, Tensor? residual, int act, "
+                     "int keep) -> (Tensor, Tensor, Tensor)", hip_ops.linear_fwd, _linear_fwd_fake)
+linear_bwd = _define("linear_bwd(Tensor? x2, Tensor? w, Tensor dy, int act, int keep, Tensor z, "
+                     "Tensor zscale, SymInt N, SymInt K, bool need_dx, bool need_dw, bool need_db)"
+                     " -> (Tensor, Tensor, Tensor)", hip_ops.linear_bwd, _linear_bwd_fake)
+swiglu_mlp_fwd = _define("swiglu_mlp_fwd(Tensor x2, Tensor wg, Tensor wu, Tensor wd, "
+                         "Tensor? residual, int keep) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
+                         hip_ops.swiglu_mlp_fwd, _swiglu_mlp_fwd_fake)
+swiglu_mlp_bwd = _define("swiglu_mlp_bwd(Tensor x2, Tensor wg, Tensor wu, Tensor wd, Tensor dy, "
+                         "int keep, Tensor gate, Tensor gate_scale, Tensor up, Tensor up_scale, "
+                         "bool need_dx, bool need_dwg, bool need_dwu, bool need_dwd) -> "
+                         "(Tensor, Tensor, Tensor, Tensor)", hip_ops.swiglu_mlp_bwd,
+                         _swiglu_mlp_bwd_fake)
+
+
 def _lora_pack_fake(As, Bs, scales, rank):
     n = rank * (sum(a.shape[1] for a in As) + 2 * sum(b.shape[0] for b in Bs))
     return As[0].new_empty((n,), dtype=torch.bfloat16)

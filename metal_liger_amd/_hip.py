@@ -52,6 +52,32 @@ SIGNATURES: dict[str, tuple] = {
     ),
     "ml_swiglu_fwd": (_i32, [_p, _p, _p, _i64, _i32, _p]),
     "ml_swiglu_bwd": (_i32, [_p, _p, _p, _p, _p, _i64, _i32, _p]),
+    "ml_swiglu_kept_fwd": (_i32, [_p] * 7 + [_i64, _i64, _i32, _p]),
+    "ml_swiglu_kept_bwd": (_i32, [_p] * 7 + [_i64, _i64, _i32, _p]),
+    "ml_linear_fwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32]),
+    "ml_linear_fwd": (
+        _i32,
+        [_p, _i64, _p, _i64, _p, _p, _i64, _i32, _p, _i64, _i32, _p, _p, _i64, _i64, _i64, _p, _sz,
+         _i32, _p],
+    ),
+    "ml_linear_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32, _i32]),
+    "ml_linear_bwd": (
+        _i32,
+        [_p, _i64, _p, _i64, _p, _i64, _i32, _i32, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _sz,
+         _i32, _p],
+    ),
+    "ml_swiglu_mlp_fwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i32]),
+    "ml_swiglu_mlp_fwd": (
+        _i32,
+        [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i32, _p, _p, _p, _p, _i64, _i64,
+         _i64, _i64, _p, _sz, _i32, _p],
+    ),
+    "ml_swiglu_mlp_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i32]),
+    "ml_swiglu_mlp_bwd": (
+        _i32,
+        [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _p, _p, _p, _p, _p, _p, _p, _p,
+         _i64, _i64, _i64, _i64, _p, _sz, _i32, _p],
+    ),
     "ml_dropout": (_i32, [_p, _p, _p, _i64, _i64, _f32, _p, _i64, _i32, _p]),
     "ml_embedding_fwd": (_i32, [_p, _i32, _i64, _p, _i64, _p, _i64, _i64, _f32, _i32, _p]),
     "ml_embedding_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64]),
@@ -191,7 +217,7 @@ SIGNATURES: dict[str, tuple] = {
     ),
 }
 
-ABI_VERSION = 13
+ABI_VERSION = 14
 
 _lib = None
 _lock = threading.Lock()

@@ -1,0 +1,614 @@
+// The feed-forward operators: a linear layer with bias, activation and residual in its
+// epilogue, the gated block (both projections, SiLU, the product, the projection
+// back), SwiGLU with its inputs kept in 8 bits; forward and backward. The mathematics
+// of the steps between the products is in ffn_rows.h, the 8 bits in held8.h.
+//
+//   linear  z = x W^T + b, y = act(z) + residual
+//           dz = dy act'(z), dx = dz W, dW = dz^T x, db = column sums of dz
+//   gated   g = x Wg^T, u = x Wu^T, h = silu(g) u, y = h Wd^T + residual
+//           dh = dy Wd, dg = dh u silu'(g), du = dh silu(g),
+//           dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
+//
+// bf16 runs on the bf16 matrix cores (gemm_core.h), fp32 on the fp32 ones.
+#include "ffn_rows.h"
+#include "gemm_core.h"
+
+namespace mla {
+namespace ffn {
+namespace {
+
+using gemm::kKMajor;
+using gemm::kMNMajor;
+
+// A workspace taken apart front to back; with a null base it only counts.
+struct Arena {
+  char* base;
+  size_t used = 0;
+
+  template <typename P>
+  P* take(size_t n) {
+    used = (used + 255) / 256 * 256;
+    P* p = base ? reinterpret_cast<P*>(base + used) : nullptr;
+    used += n * sizeof(P);
+    return p;
+  }
+};
+
+bool aligned_rows(const void* p, int64_t ld) { return !p || (aligned16(p) && ld % 8 == 0); }
+
+int ktiles(int64_t k) { return (int)((k + gemm::kBK - 1) / gemm::kBK); }
+
+// The products of each type.
+//   raw:    fp32 sums [splits][M][N] of A B^T (B [N, K]) or A B (B [K, N], b_mn)
+//   store:  sum over segments of A_s B_s (B [K_s, N]), rounded to T
+//   wgrad:  A^T B (A [K, M], B [K, N]), rounded to T
+template <typename T>
+struct Products;
+
+template <>
+struct Products<bf16> {
+  static gemm::Plan plan(int64_t M, int64_t N, int64_t K) {
+    const int m = (int)M, n = (int)N, kt = ktiles(K);
+    return gemm::plan_products(1, &m, &n, &kt, true);
+  }
+
+  static size_t raw_floats(int64_t M, int64_t N, int64_t K) {
+    return (size_t)plan(M, N, K).ksplit * M * N;
+  }
+
+  template <class CF>
+  static int raw_cfg(int64_t M, int64_t N, const gemm::Segment& s, bool b_mn, int ksplit,
+                     float* out, int& splits, hipStream_t st) {
+    gemm::Problem pb;
+    const int rc = gemm::make_problem<CF>(pb, (int)M, (int)N, 1, &s, kKMajor,
+                                          b_mn ? kMNMajor : kKMajor, 0, ksplit);
+    if (rc) return rc;
+    splits = pb.ksplit;
+    const gemm::EpiPartial epi{out, pb.M, pb.N};
+    const dim3 grid(gemm::grid_blocks(pb));
+    if (b_mn)
+      gemm::gemm_kernel<CF, kKMajor, kMNMajor, gemm::EpiPartial><<<grid, CF::THREADS, 0, st>>>(pb, epi);
+    else
+      gemm::gemm_kernel<CF, kKMajor, kKMajor, gemm::EpiPartial><<<grid, CF::THREADS, 0, st>>>(pb, epi);
+    ML_LAUNCH_CHECK();
+    return ML_OK;
+  }
+
+  static int raw(int64_t M, int64_t N, int64_t K, const bf16* a, int64_t lda, const bf16* b,
+                 int64_t ldb, bool b_mn, float* out, int& splits, hipStream_t st) {
+    const gemm::Segment s{{a, lda}, {b, ldb}, (int)K};
+    const gemm::Plan p = plan(M, N, K);
+    return p.tile == 128 ? raw_cfg<gemm::R4SCfg>(M, N, s, b_mn, p.ksplit, out, splits, st)
+                         : raw_cfg<gemm::R4Cfg>(M, N, s, b_mn, p.ksplit, out, splits, st);
+  }
+
+  static size_t store_bytes(int64_t M, int64_t N, int64_t K) {
+    return gemm::product_ws_bytes((int)M, (int)N, ktiles(K));
+  }
+
+  static int store(int64_t M, int64_t N, int nseg, const int64_t* K, const bf16* const* a,
+                   const int64_t* lda, const bf16* const* b, const int64_t* ldb, bf16* out,
+                   void* ws, size_t wsb, hipStream_t st) {
+    gemm::Segment s[2];
+    for (int i = 0; i < nseg; ++i) s[i] = gemm::Segment{{a[i], lda[i]}, {b[i], ldb[i]}, (int)K[i]};
+    return gemm::run_product((int)M, (int)N, nseg, s, kMNMajor, out, N, 1.f, 0.f,
+                             wsb ? static_cast<float*>(ws) : nullptr, wsb, st);
+  }
+
+  static size_t wgrad_bytes(int64_t, int64_t, int64_t) { return 0; }
+
+  static int wgrad(int64_t M, int64_t N, int64_t K, const bf16* a, int64_t lda, const bf16* b,
+                   int64_t ldb, bf16* out, void*, size_t, hipStream_t st) {
+    const gemm::Segment s{{a, lda}, {b, ldb}, (int)K};
+    gemm::Problem pb;
+    const int rc = gemm::make_problem<gemm::BigCfg>(pb, (int)M, (int)N, 1, &s, kMNMajor, kMNMajor, 0);
+    if (rc) return rc;
+    return gemm::launch_store<bf16>(pb, kMNMajor, kMNMajor, out, N, 1.f, 0.f, st);
+  }
+
+  static int check(const void* a, int64_t lda, int64_t cols, const char* what) {
+    ML_CHECK(aligned16(a) && lda % 8 == 0 && cols % 8 == 0,
+             "ffn: bf16 %s needs a 16-byte aligned base, and columns and row stride in multiples "
+             "of 8 (%lld, %lld)", what, (long long)cols, (long long)lda);
+    return ML_OK;
+  }
+};
+
+template <>
+struct Products<float> {
+  static size_t split_bytes(int64_t M, int64_t N, int64_t K) {
+    return ml_gemm_f32_workspace_bytes(M, N, K);
+  }
+
+  static size_t raw_floats(int64_t M, int64_t N, int64_t K) {
+    return (size_t)M * N + (split_bytes(M, N, K) + 3) / 4;
+  }
+
+  static int run(int64_t M, int64_t N, int nseg, const int64_t* K, const float* const* a,
+                 const int64_t* lda, const float* const* b, const int64_t* ldb, int la, int lb,
+                 float* out, void* ws, size_t wsb, hipStream_t st) {
+    const void *ap[2], *bp[2];
+    for (int i = 0; i < nseg; ++i) {
+      ap[i] = a[i];
+      bp[i] = b[i];
+    }
+    return ml_gemm_f32_segments_ws(M, N, nseg, K, ap, lda, bp, ldb, la, lb, out, N, 1.f, 0.f, ws,
+                                   wsb, st);
+  }
+
+  static int raw(int64_t M, int64_t N, int64_t K, const float* a, int64_t lda, const float* b,
+                 int64_t ldb, bool b_mn, float* out, int& splits, hipStream_t st) {
+    splits = 1;
+    const size_t wsb = split_bytes(M, N, K);
+    return run(M, N, 1, &K, &a, &lda, &b, &ldb, kKMajor, b_mn ? kMNMajor : kKMajor, out,
+               wsb ? out + (size_t)M * N : nullptr, wsb, st);
+  }
+
+  static size_t store_bytes(int64_t M, int64_t N, int64_t K) { return split_bytes(M, N, K); }
+
+  static int store(int64_t M, int64_t N, int nseg, const int64_t* K, const float* const* a,
+                   const int64_t* lda, const float* const* b, const int64_t* ldb, float* out,
+                   void* ws, size_t wsb, hipStream_t st) {
+    return run(M, N, nseg, K, a, lda, b, ldb, kKMajor, kMNMajor, out, ws, wsb, st);
+  }
+
+  static size_t wgrad_bytes(int64_t M, int64_t N, int64_t K) { return split_bytes(M, N, K); }
+
+  static int wgrad(int64_t M, int64_t N, int64_t K, const float* a, int64_t lda, const float* b,
+                   int64_t ldb, float* out, void* ws, size_t wsb, hipStream_t st) {
+    return run(M, N, 1, &K, &a, &lda, &b, &ldb, kMNMajor, kMNMajor, out, ws, wsb, st);
+  }
+
+  static int check(const void*, int64_t, int64_t, const char*) { return ML_OK; }
+};
+
+template <typename F>
+int dispatch(int dtype, F&& f) {
+  if (dtype == ML_F32) return f(float{});
+  if (dtype == ML_BF16) return f(bf16{});
+  set_error("ffn: dtype tag %d not supported (fp32 or bf16)", dtype);
+  return ML_ERR_INVALID;
+}
+
+int check_sizes(int64_t M, int64_t N, int64_t K) {
+  constexpr int64_t kMax = 1LL << 31;
+  ML_CHECK(M > 0 && N > 0 && K > 0 && M < kMax && N < kMax && K < kMax,
+           "ffn: bad sizes (rows %lld, columns %lld, %lld)", (long long)M, (long long)N,
+           (long long)K);
+  return ML_OK;
+}
+
+int check_kept(int keep, const void* v, const void* scale, const char* what) {
+  ML_CHECK(keep >= kKeepNone && keep <= kKeepFp8, "ffn: bad way to keep %s (%d)", what, keep);
+  ML_CHECK(keep == kKeepNone || v, "ffn: %s is kept but its buffer is null", what);
+  ML_CHECK(keep != kKeepFp8 || scale, "ffn: %s is kept in 8 bits but its scales are null", what);
+  ML_CHECK(!v || aligned16(v), "ffn: the buffer of %s must be 16-byte aligned", what);
+  return ML_OK;
+}
+
+// ------------------------------------------------------------------- linear --
+
+template <typename T>
+int linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const LinearStep<T>& step,
+               int64_t M, int64_t N, int64_t K, Arena& ws, bool run, hipStream_t st) {
+  float* sums = ws.take<float>(Products<T>::raw_floats(M, N, K));
+  if (!run) return ML_OK;
+  int splits = 1;
+  const int rc = Products<T>::raw(M, N, K, static_cast<const T*>(x), ldx,
+                                  static_cast<const T*>(w), ldw, false, sums, splits, st);
+  if (rc) return rc;
+  const bool vec = N % 8 == 0 && aligned_rows(step.bias, 0) && aligned_rows(step.residual, step.ldr) &&
+                   aligned_rows(step.y, step.ldy);
+  return launch_rows(vec, PartialSource{sums, splits, M * N, N}, NoSource{}, step, M, N, st);
+}
+
+struct GradGrid {
+  int64_t x, y, rows_per;
+};
+
+GradGrid grad_grid(int64_t rows, int64_t cols, bool vec) {
+  const int64_t x = (cols + (vec ? 255 : 31)) / (vec ? 256 : 32);
+  int64_t want = (4 * 256 + x - 1) / x;  // four workgroups a CU
+  const int64_t most = (rows + 7) / 8;
+  want = want < most ? want : most;
+  want = want > 0 ? want : 1;
+  const int64_t per = ((rows + want - 1) / want + 7) / 8 * 8;
+  return {x, (rows + per - 1) / per, per};
+}
+
+// dz (act) and db; ws counts what the partial sums take.
+template <typename T>
+int linear_grad(const T* dy, int64_t ldy, const Kept<T>& z, int act, T* dz, T* db, int64_t M,
+                int64_t N, Arena& ws, bool run, hipStream_t st) {
+  const bool vec = N % 8 == 0 && aligned_rows(dy, ldy) && aligned_rows(dz, 0);
+  // (the row ranges of the wider grid: a count that holds for both)
+  const int64_t most = grad_grid(M, N, true).y > grad_grid(M, N, false).y
+                           ? grad_grid(M, N, true).y : grad_grid(M, N, false).y;
+  float* partial = db || !run ? ws.take<float>((size_t)(most * N)) : nullptr;
+  if (!run) return ML_OK;
+  const GradGrid g = grad_grid(M, N, vec);
+  const dim3 grid((unsigned)g.x, (unsigned)g.y);
+  if (vec)
+    linear_grad_kernel<8, T><<<grid, kThreads, 0, st>>>(dy, ldy, z, act, dz, partial, M, N, g.rows_per);
+  else
+    linear_grad_kernel<1, T><<<grid, kThreads, 0, st>>>(dy, ldy, z, act, dz, partial, M, N, g.rows_per);
+  ML_LAUNCH_CHECK();
+  if (db) {
+    column_sum_kernel<T><<<dim3((unsigned)((N + kThreads - 1) / kThreads)), kThreads, 0, st>>>(
+        partial, (int)g.y, N, db);
+    ML_LAUNCH_CHECK();
+  }
+  return ML_OK;
+}
+
+struct LinearBwd {
+  const void *x, *w, *dy;
+  int64_t ldx, ldw, ldy;
+  int act, keep;
+  const void *z, *zscale;
+  void *dx, *dw, *db;
+  int64_t M, N, K;
+};
+
+size_t larger(size_t a, size_t b) { return a > b ? a : b; }
+
+template <typename T>
+int linear_bwd(const LinearBwd& p, Arena& ws, bool run, hipStream_t st) {
+  const T* dy = static_cast<const T*>(p.dy);
+  T* dz = p.act != kActNone ? ws.take<T>((size_t)(p.M * p.N)) : nullptr;
+  const Kept<T> z = make_kept<T>(p.keep, p.z, p.zscale, p.N);
+  if (dz || p.db || !run) {
+    const int rc = linear_grad<T>(dy, p.ldy, z, p.act, dz, static_cast<T*>(p.db), p.M, p.N, ws, run,
+                                  st);
+    if (rc) return rc;
+  }
+  const size_t wsb = larger(Products<T>::store_bytes(p.M, p.K, p.N),
+                            Products<T>::wgrad_bytes(p.N, p.K, p.M));
+  char* pws = ws.take<char>(wsb);
+  if (!run) return ML_OK;
+  const T* g = dz ? dz : dy;
+  const int64_t ldg = dz ? p.N : p.ldy;
+  const T* w = static_cast<const T*>(p.w);
+  if (p.dx) {
+    const int rc = Products<T>::store(p.M, p.K, 1, &p.N, &g, &ldg, &w, &p.ldw, static_cast<T*>(p.dx),
+                                      pws, wsb, st);
+    if (rc) return rc;
+  }
+  if (p.dw) {
+    const int rc = Products<T>::wgrad(p.N, p.K, p.M, g, ldg, static_cast<const T*>(p.x), p.ldx,
+                                      static_cast<T*>(p.dw), pws, wsb, st);
+    if (rc) return rc;
+  }
+  return ML_OK;
+}
+
+// -------------------------------------------------------------- gated block --
+
+struct MlpFwd {
+  const void *x, *wg, *wu, *wd, *residual;
+  int64_t ldx, ldg, ldu, ldd, ldr;
+  void* y;
+  int keep;
+  void *gate, *gscale, *up, *uscale;
+  int64_t M, H, I, O;
+};
+
+template <typename T>
+int mlp_fwd(const MlpFwd& p, Arena& ws, bool run, hipStream_t st) {
+  T* h = ws.take<T>((size_t)(p.M * p.I));
+  const size_t n_in = Products<T>::raw_floats(p.M, p.I, p.H);
+  float* sums = ws.take<float>(larger(2 * n_in, Products<T>::raw_floats(p.M, p.O, p.I)));
+  if (!run) return ML_OK;
+  const T* x = static_cast<const T*>(p.x);
+  int splits = 1;
+  int rc = Products<T>::raw(p.M, p.I, p.H, x, p.ldx, static_cast<const T*>(p.wg), p.ldg, false,
+                            sums, splits, st);
+  if (rc) return rc;
+  rc = Products<T>::raw(p.M, p.I, p.H, x, p.ldx, static_cast<const T*>(p.wu), p.ldu, false,
+                        sums + n_in, splits, st);
+  if (rc) return rc;
+  const GatedStep<T> step{h, p.I, make_kept<T>(p.keep, p.gate, p.gscale, p.I),
+                          make_kept<T>(p.keep, p.up, p.uscale, p.I)};
+  const int64_t mi = p.M * p.I;
+  rc = launch_rows(p.I % 8 == 0, PartialSource{sums, splits, mi, p.I},
+                   PartialSource{sums + n_in, splits, mi, p.I}, step, p.M, p.I, st);
+  if (rc) return rc;
+  rc = Products<T>::raw(p.M, p.O, p.I, h, p.I, static_cast<const T*>(p.wd), p.ldd, false, sums,
+                        splits, st);
+  if (rc) return rc;
+  const LinearStep<T> out{nullptr, static_cast<const T*>(p.residual), static_cast<T*>(p.y), p.ldr,
+                          p.O, kActNone, Kept<T>{}};
+  return launch_rows(p.O % 8 == 0 && aligned_rows(p.residual, p.ldr) && aligned_rows(p.y, p.O),
+                     PartialSource{sums, splits, p.M * p.O, p.O}, NoSource{}, out, p.M, p.O, st);
+}
+
+struct MlpBwd {
+  const void *x, *wg, *wu, *wd, *dy;
+  int64_t ldx, ldg, ldu, ldd, ldy;
+  int keep;
+  const void *gate, *gscale, *up, *uscale;
+  void *dx, *dwg, *dwu, *dwd;
+  int64_t M, H, I, O;
+};
+
+template <typename T>
+int mlp_bwd(const MlpBwd& p, Arena& ws, bool run, hipStream_t st) {
+  const size_t mi = (size_t)(p.M * p.I);
+  T* dg = ws.take<T>(mi);
+  T* du = ws.take<T>(mi);
+  T* h = ws.take<T>(mi);
+  float* sums = ws.take<float>(Products<T>::raw_floats(p.M, p.I, p.O));
+  size_t wsb = larger(Products<T>::store_bytes(p.M, p.H, 2 * p.I), Products<T>::wgrad_bytes(p.I, p.H, p.M));
+  wsb = larger(wsb, Products<T>::wgrad_bytes(p.O, p.I, p.M));
+  char* pws = ws.take<char>(wsb);
+  if (!run) return ML_OK;
+  const T* x = static_cast<const T*>(p.x);
+  const T* dy = static_cast<const T*>(p.dy);
+  int splits = 1;
+  int rc = Products<T>::raw(p.M, p.I, p.O, dy, p.ldy, static_cast<const T*>(p.wd), p.ldd, true,
+                            sums, splits, st);
+  if (rc) return rc;
+  const GatedGradStep<T> step{dg, du, p.dwd ? h : nullptr, p.I,
+                              make_kept<T>(p.keep, p.gate, p.gscale, p.I),
+                              make_kept<T>(p.keep, p.up, p.uscale, p.I)};
+  rc = launch_rows(p.I % 8 == 0, PartialSource{sums, splits, p.M * p.I, p.I}, NoSource{}, step, p.M,
+                   p.I, st);
+  if (rc) return rc;
+  if (p.dx) {
+    const int64_t ks[2] = {p.I, p.I}, la[2] = {p.I, p.I}, lb[2] = {p.ldg, p.ldu};
+    const T* a[2] = {dg, du};
+    const T* b[2] = {static_cast<const T*>(p.wg), static_cast<const T*>(p.wu)};
+    rc = Products<T>::store(p.M, p.H, 2, ks, a, la, b, lb, static_cast<T*>(p.dx), pws, wsb, st);
+    if (rc) return rc;
+  }
+  auto wgrad = [&](int64_t rows, int64_t cols, const T* a, int64_t lda, const T* b, int64_t ldb,
+                   void* out) {
+    return out ? Products<T>::wgrad(rows, cols, p.M, a, lda, b, ldb, static_cast<T*>(out), pws, wsb,
+                                    st)
+               : (int)ML_OK;
+  };
+  rc = wgrad(p.I, p.H, dg, p.I, x, p.ldx, p.dwg);
+  if (rc) return rc;
+  rc = wgrad(p.I, p.H, du, p.I, x, p.ldx, p.dwu);
+  if (rc) return rc;
+  return wgrad(p.O, p.I, dy, p.ldy, h, p.I, p.dwd);
+}
+
+}  // namespace
+}  // namespace ffn
+}  // namespace mla
+
+using namespace mla;
+
+#define ML_TRY(call)        \
+  do {                      \
+    const int rc_ = (call); \
+    if (rc_) return rc_;    \
+  } while (0)
+
+extern "C" size_t ml_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
+  if (ffn::check_sizes(M, N, K)) return 0;
+  ffn::Arena ws{nullptr};
+  ffn::dispatch(dtype, [&](auto t) {
+    using T = decltype(t);
+    return ffn::linear_fwd<T>(nullptr, 0, nullptr, 0, ffn::LinearStep<T>{}, M, N, K, ws, false, nullptr);
+  });
+  return ws.used;
+}
+
+extern "C" int ml_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                             const void* bias, const void* residual, int64_t ldr, int act,
+                             void* y, int64_t ldy, int keep, void* z, void* zscale, int64_t M,
+                             int64_t N, int64_t K, void* workspace, size_t workspace_bytes,
+                             int dtype, void* stream) {
+  ML_TRY(ffn::check_sizes(M, N, K));
+  ML_CHECK(x && w && y, "linear: null pointer");
+  ML_CHECK(act >= kActNone && act <= kActGeluTanh, "linear: bad activation %d", act);
+  ML_CHECK(ldx >= K && ldw >= K && ldy >= N && (!residual || ldr >= N), "linear: bad row strides");
+  ML_TRY(ffn::check_kept(keep, z, zscale, "z"));
+  return ffn::dispatch(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    ML_TRY(ffn::Products<T>::check(x, ldx, K, "x"));
+    ML_TRY(ffn::Products<T>::check(w, ldw, K, "weight"));
+    ffn::Arena ws{static_cast<char*>(workspace)};
+    const size_t need = ml_linear_fwd_workspace_bytes(M, N, K, dtype);
+    ML_CHECK(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
+             "linear: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    const ffn::LinearStep<T> step{static_cast<const T*>(bias), static_cast<const T*>(residual),
+                                  static_cast<T*>(y), ldr, ldy, act,
+                                  ffn::make_kept<T>(keep, z, zscale, N)};
+    return ffn::linear_fwd<T>(x, ldx, w, ldw, step, M, N, K, ws, true, (hipStream_t)stream);
+  });
+}
+
+extern "C" size_t ml_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int act,
+                                                int dtype) {
+  if (ffn::check_sizes(M, N, K)) return 0;
+  ffn::LinearBwd p{};
+  p.act = act;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  ffn::Arena ws{nullptr};
+  ffn::dispatch(dtype, [&](auto t) { return ffn::linear_bwd<decltype(t)>(p, ws, false, nullptr); });
+  return ws.used;
+}
+
+extern "C" int ml_linear_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                             const void* dy, int64_t ldy, int act, int keep, const void* z,
+                             const void* zscale, void* dx, void* dw, void* db, int64_t M,
+                             int64_t N, int64_t K, void* workspace, size_t workspace_bytes,
+                             int dtype, void* stream) {
+  ML_TRY(ffn::check_sizes(M, N, K));
+  ML_CHECK(act >= kActNone && act <= kActGeluTanh, "linear backward: bad activation %d", act);
+  ML_CHECK(dy && (!dx || w) && (!dw || x), "linear backward: null pointer");
+  ML_CHECK(ldy >= N && (!dx || ldw >= K) && (!dw || ldx >= K), "linear backward: bad row strides");
+  ML_CHECK(act == kActNone || keep != ffn::kKeepNone, "linear backward: no z was kept");
+  ML_TRY(ffn::check_kept(act == kActNone ? ffn::kKeepNone : keep, z, zscale, "z"));
+  if (!dx && !dw && !db) return ML_OK;
+  return ffn::dispatch(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    if (dx || dw) ML_TRY(ffn::Products<T>::check(act == kActNone ? dy : nullptr, act == kActNone ? ldy : 0, N, "dy"));
+    if (dx) {
+      ML_TRY(ffn::Products<T>::check(w, ldw, K, "weight"));
+      ML_TRY(ffn::Products<T>::check(dx, K, K, "dx"));
+    }
+    if (dw) {
+      ML_TRY(ffn::Products<T>::check(x, ldx, K, "x"));
+      ML_TRY(ffn::Products<T>::check(dw, K, K, "dw"));
+    }
+    ffn::Arena ws{static_cast<char*>(workspace)};
+    const size_t need = ml_linear_bwd_workspace_bytes(M, N, K, act, dtype);
+    ML_CHECK(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
+             "linear backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    const ffn::LinearBwd p{x, w, dy, ldx, ldw, ldy, act, keep, z, zscale, dx, dw, db, M, N, K};
+    return ffn::linear_bwd<T>(p, ws, true, (hipStream_t)stream);
+  });
+}
+
+namespace mla {
+namespace ffn {
+namespace {
+int check_mlp(int64_t M, int64_t H, int64_t I, int64_t O) {
+  ML_TRY(check_sizes(M, H, I));
+  return check_sizes(M, O, 2 * I);
+}
+}  // namespace
+}  // namespace ffn
+}  // namespace mla
+
+extern "C" size_t ml_swiglu_mlp_fwd_workspace_bytes(int64_t M, int64_t H, int64_t I, int64_t O,
+                                                    int dtype) {
+  if (ffn::check_mlp(M, H, I, O)) return 0;
+  ffn::MlpFwd p{};
+  p.M = M;
+  p.H = H;
+  p.I = I;
+  p.O = O;
+  ffn::Arena ws{nullptr};
+  ffn::dispatch(dtype, [&](auto t) { return ffn::mlp_fwd<decltype(t)>(p, ws, false, nullptr); });
+  return ws.used;
+}
+
+extern "C" int ml_swiglu_mlp_fwd(const void* x, int64_t ldx, const void* wg, int64_t ldg,
+                                 const void* wu, int64_t ldu, const void* wd, int64_t ldd,
+                                 const void* residual, int64_t ldr, void* y, int keep, void* gate,
+                                 void* gate_scale, void* up, void* up_scale, int64_t M, int64_t H,
+                                 int64_t I, int64_t O, void* workspace, size_t workspace_bytes,
+                                 int dtype, void* stream) {
+  ML_TRY(ffn::check_mlp(M, H, I, O));
+  ML_CHECK(x && wg && wu && wd && y, "swiglu mlp: null pointer");
+  ML_CHECK(ldx >= H && ldg >= H && ldu >= H && ldd >= I && (!residual || ldr >= O),
+           "swiglu mlp: bad row strides");
+  ML_TRY(ffn::check_kept(keep, gate, gate_scale, "gate"));
+  ML_TRY(ffn::check_kept(keep, up, up_scale, "up"));
+  return ffn::dispatch(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    ML_TRY(ffn::Products<T>::check(x, ldx, H, "x"));
+    ML_TRY(ffn::Products<T>::check(wg, ldg, H, "gate weight"));
+    ML_TRY(ffn::Products<T>::check(wu, ldu, H, "up weight"));
+    ML_TRY(ffn::Products<T>::check(wd, ldd, I, "down weight"));
+    ffn::Arena ws{static_cast<char*>(workspace)};
+    const size_t need = ml_swiglu_mlp_fwd_workspace_bytes(M, H, I, O, dtype);
+    ML_CHECK(workspace_bytes >= need && workspace && aligned16(workspace),
+             "swiglu mlp: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    const ffn::MlpFwd p{x, wg, wu, wd, residual, ldx, ldg, ldu, ldd, ldr, y, keep,
+                        gate, gate_scale, up, up_scale, M, H, I, O};
+    return ffn::mlp_fwd<T>(p, ws, true, (hipStream_t)stream);
+  });
+}
+
+extern "C" size_t ml_swiglu_mlp_bwd_workspace_bytes(int64_t M, int64_t H, int64_t I, int64_t O,
+                                                    int dtype) {
+  if (ffn::check_mlp(M, H, I, O)) return 0;
+  ffn::MlpBwd p{};
+  p.M = M;
+  p.H = H;
+  p.I = I;
+  p.O = O;
+  ffn::Arena ws{nullptr};
+  ffn::dispatch(dtype, [&](auto t) { return ffn::mlp_bwd<decltype(t)>(p, ws, false, nullptr); });
+  return ws.used;
+}
+
+extern "C" int ml_swiglu_mlp_bwd(const void* x, int64_t ldx, const void* wg, int64_t ldg,
+                                 const void* wu, int64_t ldu, const void* wd, int64_t ldd,
+                                 const void* dy, int64_t ldy, int keep, const void* gate,
+                                 const void* gate_scale, const void* up, const void* up_scale,
+                                 void* dx, void* dwg, void* dwu, void* dwd, int64_t M, int64_t H,
+                                 int64_t I, int64_t O, void* workspace, size_t workspace_bytes,
+                                 int dtype, void* stream) {
+  ML_TRY(ffn::check_mlp(M, H, I, O));
+  ML_CHECK(x && wg && wu && wd && dy, "swiglu mlp backward: null pointer");
+  ML_CHECK(ldx >= H && ldg >= H && ldu >= H && ldd >= I && ldy >= O,
+           "swiglu mlp backward: bad row strides");
+  ML_CHECK(keep != ffn::kKeepNone, "swiglu mlp backward: gate and up were not kept");
+  ML_TRY(ffn::check_kept(keep, gate, gate_scale, "gate"));
+  ML_TRY(ffn::check_kept(keep, up, up_scale, "up"));
+  if (!dx && !dwg && !dwu && !dwd) return ML_OK;
+  return ffn::dispatch(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    ML_TRY(ffn::Products<T>::check(x, ldx, H, "x"));
+    ML_TRY(ffn::Products<T>::check(wg, ldg, H, "gate weight"));
+    ML_TRY(ffn::Products<T>::check(wu, ldu, H, "up weight"));
+    ML_TRY(ffn::Products<T>::check(wd, ldd, I, "down weight"));
+    ML_TRY(ffn::Products<T>::check(dy, ldy, O, "dy"));
+    ML_TRY(ffn::Products<T>::check(dx, H, H, "dx"));
+    ML_TRY(ffn::Products<T>::check(dwg, H, H, "gate weight's gradient"));
+    ML_TRY(ffn::Products<T>::check(dwu, H, H, "up weight's gradient"));
+    ML_TRY(ffn::Products<T>::check(dwd, I, I, "down weight's gradient"));
+    ffn::Arena ws{static_cast<char*>(workspace)};
+    const size_t need = ml_swiglu_mlp_bwd_workspace_bytes(M, H, I, O, dtype);
+    ML_CHECK(workspace_bytes >= need && workspace && aligned16(workspace),
+             "swiglu mlp backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    const ffn::MlpBwd p{x, wg, wu, wd, dy, ldx, ldg, ldu, ldd, ldy, keep, gate, gate_scale, up,
+                        up_scale, dx, dwg, dwu, dwd, M, H, I, O};
+    return ffn::mlp_bwd<T>(p, ws, true, (hipStream_t)stream);
+  });
+}
+
+// ------------------------------------------------- SwiGLU kept in 8 bits --
+
+extern "C" int ml_swiglu_kept_fwd(const void* gate, const void* up, void* out, void* gate_q,
+                                  void* gate_scale, void* up_q, void* up_scale, int64_t rows,
+                                  int64_t cols, int dtype, void* stream) {
+  ML_CHECK(rows >= 0 && cols >= 0, "swiglu kept: negative size");
+  if (rows == 0 || cols == 0) return ML_OK;
+  ML_CHECK(gate && up && out, "swiglu kept: null pointer");
+  ML_TRY(ffn::check_kept(ffn::kKeepFp8, gate_q, gate_scale, "gate"));
+  ML_TRY(ffn::check_kept(ffn::kKeepFp8, up_q, up_scale, "up"));
+  return dispatch_dtype(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    const bool vec = cols % 8 == 0 && aligned16(gate) && aligned16(up) && aligned16(out);
+    // whole blocks: one long row
+    const bool flat = cols % held8::kBlock == 0;
+    const int64_t r = flat ? 1 : rows, c = flat ? rows * cols : cols;
+    const ffn::GatedStep<T> step{static_cast<T*>(out), c,
+                                 ffn::make_kept<T>(ffn::kKeepFp8, gate_q, gate_scale, c),
+                                 ffn::make_kept<T>(ffn::kKeepFp8, up_q, up_scale, c)};
+    return ffn::launch_rows(vec, ffn::TypedSource<T>{static_cast<const T*>(gate), c},
+                            ffn::TypedSource<T>{static_cast<const T*>(up), c}, step, r, c,
+                            (hipStream_t)stream);
+  });
+}
+
+extern "C" int ml_swiglu_kept_bwd(const void* gate_q, const void* gate_scale, const void* up_q,
+                                  const void* up_scale, const void* dy, void* dgate, void* dup,
+                                  int64_t rows, int64_t cols, int dtype, void* stream) {
+  ML_CHECK(rows >= 0 && cols >= 0, "swiglu kept backward: negative size");
+  if (rows == 0 || cols == 0) return ML_OK;
+  ML_CHECK(dy && dgate && dup, "swiglu kept backward: null pointer");
+  ML_TRY(ffn::check_kept(ffn::kKeepFp8, gate_q, gate_scale, "gate"));
+  ML_TRY(ffn::check_kept(ffn::kKeepFp8, up_q, up_scale, "up"));
+  return dispatch_dtype(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    const bool vec = cols % 8 == 0 && aligned16(dy) && aligned16(dgate) && aligned16(dup);
+    const bool flat = cols % held8::kBlock == 0;
+    const int64_t r = flat ? 1 : rows, c = flat ? rows * cols : cols;
+    const ffn::GatedGradStep<T> step{static_cast<T*>(dgate), static_cast<T*>(dup), nullptr, c,
+                                     ffn::make_kept<T>(ffn::kKeepFp8, gate_q, gate_scale, c),
+                                     ffn::make_kept<T>(ffn::kKeepFp8, up_q, up_scale, c)};
+    return ffn::launch_rows(vec, ffn::TypedSource<T>{static_cast<const T*>(dy), c}, ffn::NoSource{},
+                            step, r, c, (hipStream_t)stream);
+  });
+}

@@ -1,0 +1,118 @@
+// Tensors kept in 8 bits for a backward pass: rows in blocks of 32 elements (a
+// row's last block may be shorter), each with one scale 2^e, elements as e4m3
+// (3 bits of mantissa, smallest step 2^-9) of v / 2^e:
+//   e = max(floor(log2 m) - 7, -126),  m the largest finite magnitude of the block
+//   (m = 0: e = -126); the scale's byte is e + 127.
+// A block's largest element lands in [128, 256), so nothing saturates (e4m3 ends
+// at 448) and the scale is a matter of m's exponent bits alone: 17 octaves below
+// it still differ from 0. Elements that are not finite are kept as NaN and do not
+// count for m. The scale is a power of two, so that v / 2^e rounds nothing; the
+// rounding to e4m3 (half a step: 2^-4 of the value) is the only one.
+#pragma once
+
+#include "common.h"
+
+namespace mla {
+namespace held8 {
+
+constexpr int kBlock = 32;
+
+inline int64_t blocks(int64_t cols) { return (cols + kBlock - 1) / kBlock; }
+
+// |v|'s bits where v is finite, else 0 (their order is that of the magnitudes)
+__device__ __forceinline__ uint32_t finite_bits(float v) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu;
+  return b < 0x7F800000u ? b : 0u;
+}
+
+// The scale's byte from the bits of m: its exponent field less 7, at least 1.
+__device__ __forceinline__ uint32_t scale_byte(uint32_t max_bits) {
+  const int e = (int)(max_bits >> 23) - 7;
+  return (uint32_t)(e > 1 ? e : 1);
+}
+
+__device__ __forceinline__ float scale_of(uint32_t byte) {
+  return __builtin_bit_cast(float, byte << 23);
+}
+
+__device__ __forceinline__ float inverse_of(uint32_t byte) {  // byte in 1 .. 247
+  return __builtin_bit_cast(float, (254u - byte) << 23);
+}
+
+// Largest value over LANES neighbouring lanes (a power of two, aligned).
+template <int LANES>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t m) {
+#pragma unroll
+  for (int off = 1; off < LANES; off <<= 1) {
+    const uint32_t o = (uint32_t)__shfl_xor((int)m, off, 64);
+    m = m > o ? m : o;
+  }
+  return m;
+}
+
+// The scale's byte of a block that 32 / VEC neighbouring lanes hold VEC elements of.
+template <int VEC>
+__device__ __forceinline__ uint32_t block_byte(const float (&v)[VEC]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) {
+    const uint32_t b = finite_bits(v[k]);
+    m = m > b ? m : b;
+  }
+  return scale_byte(lanes_max<kBlock / VEC>(m));
+}
+
+__device__ __forceinline__ float to_scaled(float v, float inv) {
+  return finite_bits(v) == (__builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu) ? v * inv
+                                                                           : __builtin_nanf("");
+}
+
+// Two elements as bytes 0 and 1 of the result.
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xFFFFu;
+}
+
+// VEC elements to q (VEC bytes, aligned to VEC), by the block's scale.
+template <int VEC>
+__device__ __forceinline__ void store(uint8_t* q, uint32_t byte, const float (&v)[VEC]) {
+  const float inv = inverse_of(byte);
+  if constexpr (VEC == 1) {
+    *q = (uint8_t)pack2(to_scaled(v[0], inv), 0.f);
+  } else {
+    uint32_t w[VEC / 4];
+#pragma unroll
+    for (int k = 0; k < VEC / 4; ++k) {
+      int p = __builtin_amdgcn_cvt_pk_fp8_f32(to_scaled(v[4 * k], inv),
+                                              to_scaled(v[4 * k + 1], inv), 0, false);
+      p = __builtin_amdgcn_cvt_pk_fp8_f32(to_scaled(v[4 * k + 2], inv),
+                                          to_scaled(v[4 * k + 3], inv), p, true);
+      w[k] = (uint32_t)p;
+    }
+    __builtin_memcpy(__builtin_assume_aligned(q, VEC), w, VEC);
+  }
+}
+
+template <int VEC>
+__device__ __forceinline__ void load(const uint8_t* q, uint32_t byte, float (&v)[VEC]) {
+  const float s = scale_of(byte);
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  if constexpr (VEC == 1) {
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)*q, false);
+    v[0] = a[0] * s;
+  } else {
+    uint32_t w[VEC / 4];
+    __builtin_memcpy(w, __builtin_assume_aligned(q, VEC), VEC);
+#pragma unroll
+    for (int k = 0; k < VEC / 4; ++k) {
+      const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[k], false);
+      const f32x2 b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[k], true);
+      v[4 * k] = a[0] * s;
+      v[4 * k + 1] = a[1] * s;
+      v[4 * k + 2] = b[0] * s;
+      v[4 * k + 3] = b[1] * s;
+    }
+  }
+}
+
+}  // namespace held8
+}  // namespace mla

@@ -153,6 +153,163 @@ def swiglu_bwd(gate: torch.Tensor, up: torch.Tensor, dy: torch.Tensor):
     return dg, du
 
 
+# What a backward needs of its forward, kept whole or in 8 bits (ML_KEEP_*).
+KEEP_NONE, KEEP_SAME, KEEP_FP8 = 0, 1, 2
+KEEP_BLOCK = 32  # elements of a row that share a scale
+
+
+def kept_shapes(shape):
+    """Shapes of a tensor's bytes and of their scales (ML_KEEP_FP8): blocks lie in rows
+    of the last dimension."""
+    shape = tuple(shape) or (1,)
+    return shape, (*shape[:-1], -(-shape[-1] // KEEP_BLOCK))
+
+
+def swiglu_kept_fwd(gate: torch.Tensor, up: torch.Tensor):
+    """swiglu_fwd, and gate and up in 8 bits: (out, gate's bytes, scales, up's)."""
+    ensure_rocm_device(gate, up)
+    ct, (g, u) = _swiglu_operands(gate, up)
+    out = torch.empty(g.shape, dtype=ct, device=g.device)
+    bytes_, scales = kept_shapes(g.shape)
+    kept = [torch.empty(s, dtype=torch.uint8, device=g.device)
+            for s in (bytes_, scales, bytes_, scales)]
+    cols = bytes_[-1]
+    if g.numel():
+        call("ml_swiglu_kept_fwd", ptr(g), ptr(u), ptr(out), *map(ptr, kept), g.numel() // cols,
+             cols, dtype_tag(g, "gate"), stream_of(g))
+    return (out if out.dtype == gate.dtype else out.to(gate.dtype), *kept)
+
+
+def swiglu_kept_bwd(gate_q, gate_scale, up_q, up_scale, dy, gate_dtype, up_dtype):
+    """(dgate, dup) in the given dtypes, of dy's shape."""
+    ensure_rocm_device(gate_q, gate_scale, up_q, up_scale, dy)
+    shape = tuple(dy.shape)
+    if kept_shapes(shape) != (tuple(gate_q.shape), tuple(gate_scale.shape)) or \
+            kept_shapes(shape) != (tuple(up_q.shape), tuple(up_scale.shape)):
+        raise ValueError("swiglu backward: grad shape does not match what was kept")
+    ct = dy.dtype if dy.dtype == gate_dtype == up_dtype else torch.float32
+    y = dy.to(ct).contiguous()
+    dg, du = torch.empty_like(y), torch.empty_like(y)
+    cols = gate_q.shape[-1]
+    if y.numel():
+        kept = [t.contiguous() for t in (gate_q, gate_scale, up_q, up_scale)]
+        call("ml_swiglu_kept_bwd", *map(ptr, kept), ptr(y), ptr(dg), ptr(du), y.numel() // cols,
+             cols, dtype_tag(y, "grad"), stream_of(y))
+    return dg.to(gate_dtype), du.to(up_dtype)
+
+
+# ------------------------------------------------------------ feed-forward --
+
+
+def _kept_buffers(x: torch.Tensor, cols: int, keep: int):
+    """(values, scales) for x.shape[0] rows of cols; [0] where nothing is kept."""
+    rows = x.shape[0]
+    if keep == KEEP_FP8:
+        return [torch.empty(s, dtype=torch.uint8, device=x.device)
+                for s in kept_shapes((rows, cols))]
+    return [torch.empty((rows, cols) if keep == KEEP_SAME else (0,), dtype=x.dtype, device=x.device),
+            torch.empty((0,), dtype=torch.uint8, device=x.device)]
+
+
+def _product_rows(t: torch.Tensor) -> torch.Tensor:
+    """[rows, cols] as the products of t's dtype read it (a copy only when needed)."""
+    return _al16(_bf16_rows(t)) if t.dtype == torch.bfloat16 else rows_view(t)
+
+
+def _workspace(like: torch.Tensor, query: str, *args) -> tuple:
+    n = _hip.query(query, *args)
+    return (torch.empty(n, dtype=torch.uint8, device=like.device) if n else None), n
+
+
+def _used(t: torch.Tensor | None):
+    """None for a buffer in which nothing is kept."""
+    return None if t is None or t.numel() == 0 else t
+
+
+def linear_fwd(x2, w, bias, residual, act: int, keep: int):
+    """(y, z, zscale) of ml_linear_fwd: x2 [M, K], w [N, K], bias [N] or None, residual
+    [M, N] or None, all bf16 (sizes in multiples of 8) or all fp32."""
+    ensure_rocm_device(x2, w, bias, residual)
+    x2, w = _product_rows(x2), _product_rows(w)
+    (M, K), N = x2.shape, w.shape[0]
+    y = torch.empty(M, N, dtype=x2.dtype, device=x2.device)
+    z, zscale = _kept_buffers(x2, N, keep)
+    if M == 0:
+        return y, z, zscale
+    bias = None if bias is None else bias.contiguous()
+    residual = None if residual is None else rows_view(residual)
+    tag = dtype_tag(x2, "x")
+    ws, wsb = _workspace(x2, "ml_linear_fwd_workspace_bytes", M, N, K, tag)
+    call("ml_linear_fwd", ptr(x2), row_stride(x2), ptr(w), row_stride(w), ptr(bias), ptr(residual),
+         0 if residual is None else row_stride(residual), act, ptr(y), N, keep, ptr(_used(z)),
+         ptr(_used(zscale)), M, N, K, ptr(ws), wsb, tag, stream_of(x2))
+    return y, z, zscale
+
+
+def linear_bwd(x2, w, dy, act: int, keep: int, z, zscale, N: int, K: int, need_dx: bool,
+               need_dw: bool, need_db: bool):
+    """(dx, dw, db) of ml_linear_bwd, [0] where not wanted. x2 only for dw, w only for
+    dx, z and zscale as linear_fwd gave them (act 0: neither is read)."""
+    ensure_rocm_device(x2, w, dy, z, zscale)
+    M = dy.shape[0]
+    new = lambda need, *s: torch.empty(s if need else (0,), dtype=dy.dtype, device=dy.device)  # noqa: E731
+    dx, dw, db = new(need_dx, M, K), new(need_dw, N, K), new(need_db, N)
+    if M == 0:
+        return dx, dw.zero_(), db.zero_()
+    dy = _product_rows(dy)
+    x2 = _product_rows(x2) if need_dw else None
+    w = _product_rows(w) if need_dx else None
+    tag = dtype_tag(dy, "grad")
+    ws, wsb = _workspace(dy, "ml_linear_bwd_workspace_bytes", M, N, K, act, tag)
+    call("ml_linear_bwd", ptr(x2), 0 if x2 is None else row_stride(x2), ptr(w),
+         0 if w is None else row_stride(w), ptr(dy), row_stride(dy), act, keep, ptr(_used(z)),
+         ptr(_used(zscale)), ptr(_used(dx)), ptr(_used(dw)), ptr(_used(db)), M, N, K, ptr(ws), wsb,
+         tag, stream_of(dy))
+    return dx, dw, db
+
+
+def swiglu_mlp_fwd(x2, wg, wu, wd, residual, keep: int):
+    """(y, gate, gate_scale, up, up_scale) of ml_swiglu_mlp_fwd: x2 [M, H], wg and wu
+    [I, H], wd [O, I], residual [M, O] or None; dtypes as linear_fwd."""
+    ensure_rocm_device(x2, wg, wu, wd, residual)
+    x2, wg, wu, wd = map(_product_rows, (x2, wg, wu, wd))
+    (M, H), (O, I) = x2.shape, wd.shape  # noqa: E741
+    y = torch.empty(M, O, dtype=x2.dtype, device=x2.device)
+    kept = _kept_buffers(x2, I, keep) + _kept_buffers(x2, I, keep)
+    if M == 0:
+        return (y, *kept)
+    residual = None if residual is None else rows_view(residual)
+    tag = dtype_tag(x2, "x")
+    ws, wsb = _workspace(x2, "ml_swiglu_mlp_fwd_workspace_bytes", M, H, I, O, tag)
+    call("ml_swiglu_mlp_fwd", *_pairs(x2, wg, wu, wd), ptr(residual),
+         0 if residual is None else row_stride(residual), ptr(y), keep,
+         *(ptr(_used(t)) for t in kept), M, H, I, O, ptr(ws), wsb, tag, stream_of(x2))
+    return (y, *kept)
+
+
+def _pairs(*ts):
+    """pointer, row stride of each"""
+    return [v for t in ts for v in (ptr(t), row_stride(t))]
+
+
+def swiglu_mlp_bwd(x2, wg, wu, wd, dy, keep: int, gate, gate_scale, up, up_scale, need_dx: bool,
+                   need_dwg: bool, need_dwu: bool, need_dwd: bool):
+    """(dx, dwg, dwu, dwd) of ml_swiglu_mlp_bwd, [0] where not wanted."""
+    ensure_rocm_device(x2, wg, wu, wd, dy, gate, gate_scale, up, up_scale)
+    (M, H), (O, I) = x2.shape, wd.shape  # noqa: E741
+    new = lambda need, *s: torch.empty(s if need else (0,), dtype=x2.dtype, device=x2.device)  # noqa: E731
+    outs = [new(need_dx, M, H), new(need_dwg, I, H), new(need_dwu, I, H), new(need_dwd, O, I)]
+    if M == 0:
+        return tuple(t.zero_() for t in outs)
+    x2, wg, wu, wd, dy = map(_product_rows, (x2, wg, wu, wd, dy))
+    tag = dtype_tag(x2, "x")
+    ws, wsb = _workspace(x2, "ml_swiglu_mlp_bwd_workspace_bytes", M, H, I, O, tag)
+    call("ml_swiglu_mlp_bwd", *_pairs(x2, wg, wu, wd, dy), keep,
+         *(ptr(_used(t)) for t in (gate, gate_scale, up, up_scale)), *(ptr(_used(t)) for t in outs),
+         M, H, I, O, ptr(ws), wsb, tag, stream_of(x2))
+    return tuple(outs)
+
+
 # ----------------------------------------------------------------- dropout --
 
 

@@ -1,0 +1,77 @@
+"""Fused gated feed-forward block on MI355X: y = (silu(x Wg^T) * (x Wu^T)) Wd^T
+(+ residual), and its backward (the reference fuses the activation step only,
+ops/fused_swiglu.py:59-75, and its LoRA block needs adapters).
+
+The backward needs gate = x Wg^T and up = x Wu^T: they are kept in x's dtype, or in 8
+bits (checkpoint="fp8": e4m3 with a power of two as scale for every 32 columns of a
+row), formed of the fp32 sums. h = silu(gate) * up is not kept; the backward forms it
+again of what was kept. h and the gradients of gate, up and h are rounded to bf16
+between the products on the bf16 matrix cores. First derivatives only. Types and sizes
+as ops/fused_linear.py.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from metal_liger_amd import _custom_ops as cops
+from metal_liger_amd import hip_ops
+from metal_liger_amd.ops.fused_linear import (check_input, check_residual, compute_dtype, keep_mode,
+                                              rows, wants_grad)
+
+
+def _forward(x, weights, residual, keep: int):
+    O, I = weights[2].shape  # noqa: E741
+    ct = compute_dtype(x, x.shape[-1], I, O)
+    y, *kept = cops.swiglu_mlp_fwd(rows(x, ct), *(rows(w, ct) for w in weights),
+                                   None if residual is None else rows(residual, ct), keep)
+    y = y if y.dtype == x.dtype else y.to(x.dtype)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], O), kept
+
+
+class _FusedSwiGLUMLPFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, wg, wu, wd, residual, keep: int):
+        if not any(ctx.needs_input_grad[:4]):
+            keep = hip_ops.KEEP_NONE
+        y, kept = _forward(x, (wg, wu, wd), residual, keep)
+        ctx.save_for_backward(x, wg, wu, wd, *kept)
+        ctx.keep = keep
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        grads = [None] * 4
+        if any(ctx.needs_input_grad[:4]):
+            x, wg, wu, wd, *kept = ctx.saved_tensors
+            ct = compute_dtype(x, x.shape[-1], *wd.shape)
+            outs = cops.swiglu_mlp_bwd(*(rows(t, ct) for t in (x, wg, wu, wd, dy)), ctx.keep, *kept,
+                                       *ctx.needs_input_grad[:4])
+            grads = [(g if g.dtype == x.dtype else g.to(x.dtype)) if need else None
+                     for g, need in zip(outs, ctx.needs_input_grad)]
+            if grads[0] is not None and x.dim() != 2:
+                grads[0] = grads[0].view(x.shape)
+        return (*grads, dy if ctx.needs_input_grad[4] else None, None)
+
+
+def fused_swiglu_mlp(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torch.Tensor,
+                     down_weight: torch.Tensor, residual: torch.Tensor | None = None,
+                     checkpoint: str | None = None) -> torch.Tensor:
+    """(silu(x gate_weight^T) * (x up_weight^T)) down_weight^T + residual.
+
+    x [..., hidden], gate_weight and up_weight [inter, hidden], down_weight [out, inter],
+    residual [..., out]; all of x's dtype (fp32, bf16 or fp16) and on its device, any
+    strides. checkpoint: None, or "fp8" to keep gate and up in 8 bits for the backward.
+    """
+    keep = keep_mode(checkpoint)
+    check_input("fused_swiglu_mlp", x, gate_weight, up_weight, down_weight)
+    if up_weight.shape != gate_weight.shape or down_weight.shape[1] != gate_weight.shape[0]:
+        raise ValueError(f"fused_swiglu_mlp: weights {tuple(gate_weight.shape)}, "
+                         f"{tuple(up_weight.shape)} and {tuple(down_weight.shape)} do not fit")
+    check_residual("fused_swiglu_mlp", residual, x, down_weight.shape[0])
+    hip_ops.ensure_rocm_device(x, gate_weight, up_weight, down_weight, residual)
+    weights = (gate_weight, up_weight, down_weight)
+    if not wants_grad(x, *weights, residual):
+        with torch.no_grad():
+            return _forward(x, weights, residual, hip_ops.KEEP_NONE)[0]
+    return _FusedSwiGLUMLPFunction.apply(x, *weights, residual, keep)

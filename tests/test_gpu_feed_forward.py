@@ -1,0 +1,278 @@
+"""The feed-forward operators on the GPU against 64 bits on the CPU.
+
+Bounds, elementwise, of the sizes that the inputs themselves give (u = eps / 2 of the
+operators' type, v = 2^-24 of fp32):
+  a product of K terms in fp32: K v |a| |b| (and one v for each term added after it);
+  a value rounded to its type: u |value| (fp16 below its smallest normal number: 2^-25);
+  act at z + d: 1.13 |d| (the largest |act'|), act' at z + d: 0.8 |d| (the largest
+  |act''|); the activations' own fp32 arithmetic: 32 v (|z| + 1) (exp, a reciprocal and
+  at most ten more roundings, and an exponent's rounding error that grows with |z|).
+A value that a formula multiplies carries its bound through it.
+"""
+
+import pytest
+import torch
+
+from oracle import feed_forward as ref
+from tests.parity import seeded
+
+pytestmark = pytest.mark.gpu
+V = 2.0 ** -24
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+ACTS = [None, "silu", "gelu", "gelu_tanh"]
+
+
+def _u(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def _matrix_cores(dtype, *sizes):
+    """Whether the products read bf16 (else everything between input and output is fp32)."""
+    return dtype == torch.bfloat16 and all(s % 8 == 0 for s in sizes)
+
+
+def _cpu(t):
+    return t.detach().double().cpu()
+
+
+def _check(got, want, bound, what):
+    """bound without the output's own rounding."""
+    u = _u(got.dtype)
+    tiny = 2.0 ** -25 if got.dtype == torch.float16 else 0.0
+    total = bound * (1 + u) + want.abs() * u + tiny + 1e-30
+    err = (_cpu(got) - want).abs()
+    assert got.shape == want.shape, what
+    assert bool((err <= total).all()), (what, (err / total).max())
+
+
+def _mm(a, ea, b, eb, K):
+    """a b and its bound, of operands with bounds."""
+    A, B = a.abs(), b.abs()
+    return a @ b, ea @ (B + eb) + A @ eb + (K + 2) * V * (A @ B)
+
+
+def _act_noise(z):
+    return 32 * V * (z.abs() + 1)
+
+
+def _kept(saved, i, checkpoint):
+    """The i-th kept tensor of an autograd node's saved ones, as its backward reads it."""
+    v, s = saved[i:i + 2]
+    if checkpoint is None:
+        return _cpu(v)
+    return ref.held_values(v.cpu(), s.cpu())
+
+
+# ------------------------------------------------------------------- linear --
+
+def _linear_case(M, K, N, dtype, bias, residual, dev, seed=0, scale=1.0):
+    x = seeded((M, K), seed, dtype, scale).to(dev).requires_grad_()
+    w = seeded((N, K), seed + 1, dtype, K ** -0.5).to(dev).requires_grad_()
+    b = seeded((N,), seed + 2, dtype).to(dev).requires_grad_() if bias else None
+    r = seeded((M, N), seed + 3, dtype).to(dev).requires_grad_() if residual else None
+    dy = seeded((M, N), seed + 4, dtype).to(dev)
+    return x, w, b, r, dy
+
+
+def _linear_check(x, w, b, r, dy, act, checkpoint, call):
+    M, K, N = x.shape[0], x.shape[1], w.shape[0]
+    y = call()
+    saved = y.grad_fn.saved_tensors
+    leaves = [t for t in (x, w, b, r) if t is not None]
+    grads = torch.autograd.grad(y, leaves, dy)
+    dtype, low = x.dtype, _matrix_cores(x.dtype, K, N)
+    X, W, D = _cpu(x), _cpu(w), _cpu(dy)
+    zero = torch.zeros(())
+    z, ez = _mm(X, torch.zeros_like(X), W.t(), torch.zeros_like(W.t()), K)
+    if b is not None:
+        z, ez = z + _cpu(b), ez + V * (z + _cpu(b)).abs()
+    want = ref.act(z, act)
+    bound = 1.13 * ez + (_act_noise(z) if act else zero)
+    if r is not None:
+        want = want + _cpu(r)
+        bound = bound + V * want.abs()
+    _check(y, want, bound, "y")
+    # the backward, at z as it was kept
+    if act is None:
+        dz, edz = D, torch.zeros_like(D)
+    else:
+        zk = _kept(saved, 2, checkpoint)
+        err = (zk - z).abs()
+        if checkpoint == "fp8":
+            e = torch.ldexp(torch.ones((), dtype=torch.float64), ref.held_exponents(z))
+            e = e.repeat_interleave(32, -1)[..., :N]
+            # half a step, a smallest step of half 2^-9, where z's own error may move the scale
+            assert bool((err <= 2 * ez + z.abs() * 2.0 ** -4 + 2 * e * 2.0 ** -10).all()), "kept"
+        else:
+            assert bool((err <= ez + z.abs() * (_u(dtype) if low else V) + 1e-30).all()), "kept"
+        d = ref.act_grad(zk, act)
+        dz, edz = D * d, D.abs() * _act_noise(zk)
+        edz = edz + dz.abs() * (_u(dtype) if low else 2 * V)
+    out = [(*_mm(dz, edz, W, torch.zeros_like(W), N), "dx"),
+           (*_mm(dz.t(), edz.t(), X, torch.zeros_like(X), M), "dw")]
+    if b is not None:
+        out.append((dz.sum(0), edz.sum(0) + (M + 2) * V * dz.abs().sum(0), "db"))
+    if r is not None:
+        assert torch.equal(grads[-1], dy)
+    for g, (want, bound, what) in zip(grads, out):
+        assert g.dtype == dtype
+        _check(g, want, bound, what)
+
+
+SIZES = [(1, 64, 64), (3, 72, 8), (37, 128, 96), (129, 264, 136), (300, 200, 520), (5, 13, 7),
+         (64, 33, 65), (257, 100, 31), (1, 1, 1)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("act", ACTS)
+def test_linear(dev, dtype, size, act):
+    from metal_liger_amd.ops.fused_linear import fused_linear
+    M, K, N = size
+    x, w, b, r, dy = _linear_case(M, K, N, dtype, (M + N) % 2 == 0, K % 2 == 0, dev)
+    _linear_check(x, w, b, r, dy, act, None,
+                  lambda: fused_linear(x, w, b, activation=act, residual=r))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("act", ACTS[1:])
+def test_linear_kept_in_8_bits(dev, dtype, size, act):
+    from metal_liger_amd.ops.fused_linear import fused_linear
+    M, K, N = size
+    x, w, b, r, dy = _linear_case(M, K, N, dtype, (M + N) % 2 == 1, K % 2 == 1, dev)
+    _linear_check(x, w, b, r, dy, act, "fp8",
+                  lambda: fused_linear(x, w, b, activation=act, residual=r, checkpoint="fp8"))
+
+
+# ------------------------------------------------------------- gated block --
+
+def _mlp_case(M, H, I, O, dtype, residual, dev, seed=0):  # noqa: E741
+    x = seeded((M, H), seed, dtype).to(dev).requires_grad_()
+    ws = [seeded(s, seed + 1 + i, dtype, s[1] ** -0.5).to(dev).requires_grad_()
+          for i, s in enumerate([(I, H), (I, H), (O, I)])]
+    r = seeded((M, O), seed + 5, dtype).to(dev).requires_grad_() if residual else None
+    return x, ws, r, seeded((M, O), seed + 6, dtype).to(dev)
+
+
+def _gated(g, eg, u, eu):
+    """silu(g) u and its bound."""
+    s = ref.act(g, "silu")
+    es = 1.13 * eg + _act_noise(g)
+    h = s * u
+    return h, es * (u.abs() + eu) + s.abs() * eu + V * h.abs()
+
+
+def _mlp_check(x, ws, r, dy, checkpoint, call):
+    (M, H), (O, I) = x.shape, ws[2].shape  # noqa: E741
+    y = call()
+    saved = y.grad_fn.saved_tensors
+    leaves = [x, *ws] + ([] if r is None else [r])
+    grads = torch.autograd.grad(y, leaves, dy)
+    low = _matrix_cores(x.dtype, H, I, O)
+    u16 = _u(torch.bfloat16) if low else V  # what is rounded between the products
+    X, (Wg, Wu, Wd), D = _cpu(x), map(_cpu, ws), _cpu(dy)
+    zx = torch.zeros_like(X)
+    g, eg = _mm(X, zx, Wg.t(), torch.zeros_like(Wg.t()), H)
+    u, eu = _mm(X, zx, Wu.t(), torch.zeros_like(Wu.t()), H)
+    h, eh = _gated(g, eg, u, eu)
+    want, bound = _mm(h, eh + u16 * h.abs(), Wd.t(), torch.zeros_like(Wd.t()), I)
+    if r is not None:
+        want = want + _cpu(r)
+        bound = bound + V * want.abs()
+    _check(y, want, bound, "y")
+    gk = _kept(saved, 4, checkpoint)
+    uk = _kept(saved, 6, checkpoint)
+    for k, z, e in ((gk, g, eg), (uk, u, eu)):
+        if checkpoint == "fp8":
+            s = torch.ldexp(torch.ones((), dtype=torch.float64), ref.held_exponents(z))
+            s = s.repeat_interleave(32, -1)[..., :I]
+            assert bool(((k - z).abs() <= 2 * e + z.abs() * 2.0 ** -4 + 2 * s * 2.0 ** -10).all())
+        else:
+            assert bool(((k - z).abs() <= e + u16 * z.abs() + 1e-30).all())
+    zero = torch.zeros_like(gk)
+    h, eh = _gated(gk, zero, uk, zero)
+    dh, edh = _mm(D, torch.zeros_like(D), Wd, torch.zeros_like(Wd), O)
+    d, s = ref.act_grad(gk, "silu"), ref.act(gk, "silu")
+    noise = _act_noise(gk) + 3 * V
+    dg, du = dh * uk * d, dh * s
+    edg = (edh * d.abs() + dh.abs() * noise) * uk.abs() + u16 * dg.abs()
+    edu = edh * s.abs() + dh.abs() * noise + u16 * du.abs()
+    a, ea = _mm(dg, edg, Wg, torch.zeros_like(Wg), I)
+    b, eb = _mm(du, edu, Wu, torch.zeros_like(Wu), I)
+    eb = eb + I * V * (a.abs() + b.abs())  # one sum over both
+    eh = eh + u16 * h.abs()
+    out = [(a + b, ea + eb, "dx"), (*_mm(dg.t(), edg.t(), X, zx, M), "dwg"),
+           (*_mm(du.t(), edu.t(), X, zx, M), "dwu"),
+           (*_mm(D.t(), torch.zeros_like(D.t()), h, eh, M), "dwd")]
+    if r is not None:
+        assert torch.equal(grads[-1], dy)
+    for t, (want, bound, what) in zip(grads, out):
+        assert t.dtype == x.dtype
+        _check(t, want, bound, what)
+
+
+MLP_SIZES = [(1, 64, 64, 64), (3, 72, 104, 8), (37, 128, 96, 40), (129, 264, 136, 264),
+             (300, 200, 520, 200), (5, 13, 7, 9), (65, 33, 70, 33), (1, 1, 1, 1)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("size", MLP_SIZES)
+@pytest.mark.parametrize("checkpoint", [None, "fp8"])
+def test_mlp(dev, dtype, size, checkpoint):
+    from metal_liger_amd.ops.fused_swiglu_mlp import fused_swiglu_mlp
+    M, H, I, O = size  # noqa: E741
+    x, ws, r, dy = _mlp_case(M, H, I, O, dtype, M % 2 == 0 or H % 2 == 1, dev)
+    _mlp_check(x, ws, r, dy, checkpoint,
+               lambda: fused_swiglu_mlp(x, *ws, residual=r, checkpoint=checkpoint))
+
+
+# -------------------------------------------------- SwiGLU kept in 8 bits --
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shape", [(1,), (31,), (32,), (33,), (4, 64), (3, 5, 40), (7, 333),
+                                   (129, 96), (2, 8), (5, 0), (0, 8)])
+def test_swiglu_kept(dev, dtype, shape):
+    from metal_liger_amd.ops.fused_swiglu import fused_swiglu
+    gate = seeded(shape, 1, dtype, 3.0).to(dev).requires_grad_()
+    up = (seeded(shape, 2, dtype) * torch.exp(seeded(shape, 3)).to(dtype)).to(dev).requires_grad_()
+    dy = seeded(shape, 4, dtype).to(dev)
+    y = fused_swiglu(gate, up, checkpoint="fp8")
+    assert torch.equal(y, fused_swiglu(gate.detach(), up.detach()))
+    gq, gs, uq, us = y.grad_fn.saved_tensors
+    if y.numel():
+        for t, q, s in ((gate, gq, gs), (up, uq, us)):
+            want = ref.held_bytes(_cpu(t))
+            assert torch.equal(q.cpu(), want[0]) and torch.equal(s.cpu(), want[1])
+    dg, du = torch.autograd.grad(y, [gate, up], dy)
+    if not y.numel():
+        assert dg.shape == du.shape == gate.shape
+        return
+    g, u, D = ref.held_values(gq.cpu(), gs.cpu()), ref.held_values(uq.cpu(), us.cpu()), _cpu(dy)
+    noise = _act_noise(g) + 3 * V
+    _check(dg, D * u * ref.act_grad(g, "silu"), (D * u).abs() * noise, "dgate")
+    _check(du, D * ref.act(g, "silu"), D.abs() * noise, "dup")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_8_bits_of_every_value(dev, dtype):
+    """Every bf16 or fp16 (a spread of fp32) magnitude as an element of a block whose
+    largest one sets the scale, infinities, NaN and zeros among them."""
+    from metal_liger_amd import hip_ops
+    bits = torch.arange(0, 2 ** 16, dtype=torch.int32)
+    v = (bits - 2 ** 15).to(torch.int16).view(torch.float16 if dtype == torch.float16
+                                              else torch.bfloat16).to(dtype)
+    if dtype == torch.float32:
+        g = torch.Generator().manual_seed(3)
+        v = torch.randint(-2 ** 31, 2 ** 31, (2 ** 16,), generator=g).to(torch.int32).view(dtype)
+    scattered = v[torch.randperm(2 ** 16, generator=torch.Generator().manual_seed(1))]
+    top = torch.where((torch.arange(2 ** 16) % 32 == 5) & (v.abs() < 300), v, v * 0.01).to(dtype)
+    for t in (v.view(64, 1024), scattered.view(64, 1024), top.view(-1, 32), v[:65535].view(-1, 15)):
+        out = hip_ops.swiglu_kept_fwd(t.to(dev), t.to(dev))
+        codes, scales = ref.held_bytes(t)
+        got, want = out[1].cpu(), codes
+        nan = ~torch.isfinite(t)
+        assert torch.equal(out[2].cpu(), scales)
+        assert torch.equal(got[~nan], want[~nan])
+        assert bool(((got[nan] & 0x7F) == 0x7F).all())
+        assert torch.equal(out[3].cpu(), got) and torch.equal(out[4].cpu(), scales)
