@@ -645,17 +645,18 @@ int ml_gemm_f32_segments_ws(int64_t M, int64_t N, int nseg, const int64_t* k_len
  * ML_BF16; bf16 operands of a product have 16-byte aligned bases, and columns and
  * row strides in multiples of 8.
  *
- * What a backward needs of its forward's inner tensors is kept as `keep` says:
- * ML_KEEP_SAME, dense in dtype; ML_KEEP_FP8, one byte an element [rows, cols] and
- * one scale byte for every 32 columns of a row [rows, ceil(cols / 32)]: with
- * e = max(floor(log2 m) - 7, -126) for the largest finite magnitude m of the 32
- * (m = 0: -126) the scale's byte is e + 127, an element's is e4m3 of v / 2^e
- * (nearest, ties to even; NaN where v is not finite). The bits are formed of the
- * fp32 values, before any other rounding. Buffers are 16-byte aligned.
+ * What a backward needs of its forward's inner tensors is kept as `keep` says, dense
+ * [rows, cols]: ML_KEEP_F32, in fp32; ML_KEEP_FP16 and ML_KEEP_FP8, in 2 or 1 bytes an
+ * element and one scale byte for every 32 columns of a row [rows, ceil(cols / 32)]: with
+ * e = max(floor(log2 m) - 14, -126) (FP8: - 7) for the largest finite magnitude m of the
+ * 32 (m = 0: -126) the scale's byte is e + 127, an element's bits are fp16 (e4m3) of
+ * v / 2^e (nearest, ties to even; e4m3: NaN where v is not finite). They are formed of
+ * the fp32 values, before any other rounding. Buffers are 16-byte aligned.
  */
 #define ML_KEEP_NONE 0
-#define ML_KEEP_SAME 1
-#define ML_KEEP_FP8 2
+#define ML_KEEP_F32 1
+#define ML_KEEP_FP16 2
+#define ML_KEEP_FP8 3
 
 /* activations: z, z sigmoid(z), z Phi(z), and the latter by tanh */
 #define ML_ACT_NONE 0

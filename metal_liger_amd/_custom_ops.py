@@ -354,11 +354,8 @@ embedding_bwd = _define("embedding_bwd(Tensor ids, Tensor dy, SymInt vocab, SymI
 
 
 def _kept_fake(x2, cols, keep):
-    rows = x2.shape[0]
-    if keep == hip_ops.KEEP_FP8:
-        return [x2.new_empty(s, dtype=torch.uint8) for s in hip_ops.kept_shapes((rows, cols))]
-    return [x2.new_empty((rows, cols) if keep == hip_ops.KEEP_SAME else (0,)),
-            x2.new_empty((0,), dtype=torch.uint8)]
+    return [x2.new_empty(shape, dtype=dtype)
+            for shape, dtype in hip_ops.kept_layout(x2.shape[0], cols, keep)]
 
 
 def _swiglu_kept_fake(gate, up):

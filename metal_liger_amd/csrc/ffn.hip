@@ -1,7 +1,7 @@
 // The feed-forward operators: a linear layer with bias, activation and residual in its
 // epilogue, the gated block (both projections, SiLU, the product, the projection
 // back), SwiGLU with its inputs kept in 8 bits; forward and backward. The mathematics
-// of the steps between the products is in ffn_rows.h, the 8 bits in held8.h.
+// of the steps between the products is in ffn_rows.h, the 8 bits in held.h.
 //
 //   linear  z = x W^T + b, y = act(z) + residual
 //           dz = dy act'(z), dx = dz W, dW = dz^T x, db = column sums of dz
@@ -10,8 +10,7 @@
 //           dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
 //
 // bf16 runs on the bf16 matrix cores (gemm_core.h), fp32 on the fp32 ones.
-#include "ffn_rows.h"
-#include "gemm_core.h"
+#include "ffn_product.h"
 
 namespace mla {
 namespace ffn {
@@ -33,6 +32,8 @@ struct Arena {
     return p;
   }
 };
+
+size_t larger(size_t a, size_t b) { return a > b ? a : b; }
 
 bool aligned_rows(const void* p, int64_t ld) { return !p || (aligned16(p) && ld % 8 == 0); }
 
@@ -80,6 +81,30 @@ struct Products<bf16> {
     const gemm::Plan p = plan(M, N, K);
     return p.tile == 128 ? raw_cfg<gemm::R4SCfg>(M, N, s, b_mn, p.ksplit, out, splits, st)
                          : raw_cfg<gemm::R4Cfg>(M, N, s, b_mn, p.ksplit, out, splits, st);
+  }
+
+  // Whether the product runs its step as its epilogue: where K is not split.
+  static bool fused(int64_t M, int64_t N, int64_t K) { return plan(M, N, K).ksplit == 1; }
+
+  template <int LB, class Step>
+  static int through(int64_t M, int64_t N, int64_t K, const bf16* a, int64_t lda, const bf16* b,
+                     int64_t ldb, const Step& step, hipStream_t st) {
+    const gemm::Segment s{{a, lda}, {b, ldb}, (int)K};
+    return plan(M, N, K).tile == 128
+               ? launch_product<gemm::R4SCfg, LB, false>(M, N, s, gemm::Operand{}, step, st)
+               : launch_product<gemm::R4Cfg, LB, false>(M, N, s, gemm::Operand{}, step, st);
+  }
+
+  // Both of a's products, with b [N, K] and b2 [N, K]: a plan for 2 N columns.
+  template <class Step>
+  static int through_pair(int64_t M, int64_t N, int64_t K, const bf16* a, int64_t lda,
+                          const bf16* b, int64_t ldb, const bf16* b2, int64_t ldb2,
+                          const Step& step, hipStream_t st) {
+    const gemm::Segment s{{a, lda}, {b, ldb}, (int)K};
+    const gemm::Operand o{b2, ldb2};
+    return plan(M, 2 * N, K).tile == 128
+               ? launch_product<gemm::R4SCfg, kKMajor, true>(M, N, s, o, step, st)
+               : launch_product<gemm::R4Cfg, kKMajor, true>(M, N, s, o, step, st);
   }
 
   static size_t store_bytes(int64_t M, int64_t N, int64_t K) {
@@ -144,6 +169,14 @@ struct Products<float> {
                wsb ? out + (size_t)M * N : nullptr, wsb, st);
   }
 
+  static bool fused(int64_t, int64_t, int64_t) { return false; }
+
+  template <int LB, class... Args>
+  static int through(const Args&...) { return ML_ERR_INVALID; }
+
+  template <class... Args>
+  static int through_pair(const Args&...) { return ML_ERR_INVALID; }
+
   static size_t store_bytes(int64_t M, int64_t N, int64_t K) { return split_bytes(M, N, K); }
 
   static int store(int64_t M, int64_t N, int nseg, const int64_t* K, const float* const* a,
@@ -161,6 +194,20 @@ struct Products<float> {
 
   static int check(const void*, int64_t, int64_t, const char*) { return ML_OK; }
 };
+
+template <int KIND>
+using Kind = std::integral_constant<int, KIND>;
+
+// How a tensor may be kept where the products are of type T.
+template <typename T, typename F>
+int dispatch_keep(int keep, F&& f) {
+  constexpr int kWhole = std::is_same_v<T, float> ? kKeepF32 : kKeepFp16;
+  if (keep == kKeepNone) return f(Kind<kKeepNone>{});
+  if (keep == kWhole) return f(Kind<kWhole>{});
+  if (keep == kKeepFp8) return f(Kind<kKeepFp8>{});
+  set_error("ffn: tensors of this dtype are not kept as %d", keep);
+  return ML_ERR_INVALID;
+}
 
 template <typename F>
 int dispatch(int dtype, F&& f) {
@@ -181,21 +228,26 @@ int check_sizes(int64_t M, int64_t N, int64_t K) {
 int check_kept(int keep, const void* v, const void* scale, const char* what) {
   ML_CHECK(keep >= kKeepNone && keep <= kKeepFp8, "ffn: bad way to keep %s (%d)", what, keep);
   ML_CHECK(keep == kKeepNone || v, "ffn: %s is kept but its buffer is null", what);
-  ML_CHECK(keep != kKeepFp8 || scale, "ffn: %s is kept in 8 bits but its scales are null", what);
+  ML_CHECK(keep < kKeepFp16 || scale, "ffn: %s is kept with scales but they are null", what);
   ML_CHECK(!v || aligned16(v), "ffn: the buffer of %s must be 16-byte aligned", what);
   return ML_OK;
 }
 
 // ------------------------------------------------------------------- linear --
 
-template <typename T>
-int linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const LinearStep<T>& step,
+template <typename T, int KIND>
+int linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
+               const LinearStep<T, KIND>& step,
                int64_t M, int64_t N, int64_t K, Arena& ws, bool run, hipStream_t st) {
+  const T* xt = static_cast<const T*>(x);
+  const T* wt = static_cast<const T*>(w);
+  if (Products<T>::fused(M, N, K))
+    return run ? Products<T>::template through<kKMajor>(M, N, K, xt, ldx, wt, ldw, step, st)
+               : (int)ML_OK;
   float* sums = ws.take<float>(Products<T>::raw_floats(M, N, K));
   if (!run) return ML_OK;
   int splits = 1;
-  const int rc = Products<T>::raw(M, N, K, static_cast<const T*>(x), ldx,
-                                  static_cast<const T*>(w), ldw, false, sums, splits, st);
+  const int rc = Products<T>::raw(M, N, K, xt, ldx, wt, ldw, false, sums, splits, st);
   if (rc) return rc;
   const bool vec = N % 8 == 0 && aligned_rows(step.bias, 0) && aligned_rows(step.residual, step.ldr) &&
                    aligned_rows(step.y, step.ldy);
@@ -217,8 +269,8 @@ GradGrid grad_grid(int64_t rows, int64_t cols, bool vec) {
 }
 
 // dz (act) and db; ws counts what the partial sums take.
-template <typename T>
-int linear_grad(const T* dy, int64_t ldy, const Kept<T>& z, int act, T* dz, T* db, int64_t M,
+template <typename T, int KIND>
+int linear_grad(const T* dy, int64_t ldy, const Kept<KIND>& z, int act, T* dz, T* db, int64_t M,
                 int64_t N, Arena& ws, bool run, hipStream_t st) {
   const bool vec = N % 8 == 0 && aligned_rows(dy, ldy) && aligned_rows(dz, 0);
   // (the row ranges of the wider grid: a count that holds for both)
@@ -229,9 +281,9 @@ int linear_grad(const T* dy, int64_t ldy, const Kept<T>& z, int act, T* dz, T* d
   const GradGrid g = grad_grid(M, N, vec);
   const dim3 grid((unsigned)g.x, (unsigned)g.y);
   if (vec)
-    linear_grad_kernel<8, T><<<grid, kThreads, 0, st>>>(dy, ldy, z, act, dz, partial, M, N, g.rows_per);
+    linear_grad_kernel<8, T, KIND><<<grid, kThreads, 0, st>>>(dy, ldy, z, act, dz, partial, M, N, g.rows_per);
   else
-    linear_grad_kernel<1, T><<<grid, kThreads, 0, st>>>(dy, ldy, z, act, dz, partial, M, N, g.rows_per);
+    linear_grad_kernel<1, T, KIND><<<grid, kThreads, 0, st>>>(dy, ldy, z, act, dz, partial, M, N, g.rows_per);
   ML_LAUNCH_CHECK();
   if (db) {
     column_sum_kernel<T><<<dim3((unsigned)((N + kThreads - 1) / kThreads)), kThreads, 0, st>>>(
@@ -250,16 +302,15 @@ struct LinearBwd {
   int64_t M, N, K;
 };
 
-size_t larger(size_t a, size_t b) { return a > b ? a : b; }
-
 template <typename T>
 int linear_bwd(const LinearBwd& p, Arena& ws, bool run, hipStream_t st) {
   const T* dy = static_cast<const T*>(p.dy);
   T* dz = p.act != kActNone ? ws.take<T>((size_t)(p.M * p.N)) : nullptr;
-  const Kept<T> z = make_kept<T>(p.keep, p.z, p.zscale, p.N);
   if (dz || p.db || !run) {
-    const int rc = linear_grad<T>(dy, p.ldy, z, p.act, dz, static_cast<T*>(p.db), p.M, p.N, ws, run,
-                                  st);
+    const int rc = dispatch_keep<T>(dz ? p.keep : (int)kKeepNone, [&](auto kind) {
+      return linear_grad<T>(dy, p.ldy, make_kept<kind.value>(p.z, p.zscale, p.N), p.act, dz,
+                            static_cast<T*>(p.db), p.M, p.N, ws, run, st);
+    });
     if (rc) return rc;
   }
   const size_t wsb = larger(Products<T>::store_bytes(p.M, p.K, p.N),
@@ -293,33 +344,42 @@ struct MlpFwd {
   int64_t M, H, I, O;
 };
 
-template <typename T>
+template <typename T, int KIND>
 int mlp_fwd(const MlpFwd& p, Arena& ws, bool run, hipStream_t st) {
+  using P = Products<T>;
   T* h = ws.take<T>((size_t)(p.M * p.I));
-  const size_t n_in = Products<T>::raw_floats(p.M, p.I, p.H);
-  float* sums = ws.take<float>(larger(2 * n_in, Products<T>::raw_floats(p.M, p.O, p.I)));
+  const LinearStep<T, kKeepNone> out{nullptr, static_cast<const T*>(p.residual),
+                                     static_cast<T*>(p.y), p.ldr, p.O, kActNone, {}};
+  const bool fuse_in = P::fused(p.M, 2 * p.I, p.H), fuse_out = P::fused(p.M, p.O, p.I);
+  const size_t n_in = fuse_in ? 0 : P::raw_floats(p.M, p.I, p.H);
+  const size_t n_out = fuse_out ? 0 : P::raw_floats(p.M, p.O, p.I);
+  float* sums = ws.take<float>(larger(2 * n_in, n_out));
   if (!run) return ML_OK;
   const T* x = static_cast<const T*>(p.x);
-  int splits = 1;
-  int rc = Products<T>::raw(p.M, p.I, p.H, x, p.ldx, static_cast<const T*>(p.wg), p.ldg, false,
-                            sums, splits, st);
+  const T* wg = static_cast<const T*>(p.wg);
+  const T* wu = static_cast<const T*>(p.wu);
+  const T* wd = static_cast<const T*>(p.wd);
+  const GatedStep<T, KIND> step{h, p.I, make_kept<KIND>(p.gate, p.gscale, p.I),
+                                make_kept<KIND>(p.up, p.uscale, p.I)};
+  int splits = 1, rc;
+  if (fuse_in) {
+    rc = P::through_pair(p.M, p.I, p.H, x, p.ldx, wg, p.ldg, wu, p.ldu, step, st);
+  } else {
+    rc = P::raw(p.M, p.I, p.H, x, p.ldx, wg, p.ldg, false, sums, splits, st);
+    if (rc) return rc;
+    rc = P::raw(p.M, p.I, p.H, x, p.ldx, wu, p.ldu, false, sums + n_in, splits, st);
+    if (rc) return rc;
+    const int64_t mi = p.M * p.I;
+    rc = launch_rows(p.I % 8 == 0, PartialSource{sums, splits, mi, p.I},
+                     PartialSource{sums + n_in, splits, mi, p.I}, step, p.M, p.I, st);
+  }
   if (rc) return rc;
-  rc = Products<T>::raw(p.M, p.I, p.H, x, p.ldx, static_cast<const T*>(p.wu), p.ldu, false,
-                        sums + n_in, splits, st);
+  if (fuse_out) return P::template through<kKMajor>(p.M, p.O, p.I, h, p.I, wd, p.ldd, out, st);
+  rc = P::raw(p.M, p.O, p.I, h, p.I, wd, p.ldd, false, sums, splits, st);
   if (rc) return rc;
-  const GatedStep<T> step{h, p.I, make_kept<T>(p.keep, p.gate, p.gscale, p.I),
-                          make_kept<T>(p.keep, p.up, p.uscale, p.I)};
-  const int64_t mi = p.M * p.I;
-  rc = launch_rows(p.I % 8 == 0, PartialSource{sums, splits, mi, p.I},
-                   PartialSource{sums + n_in, splits, mi, p.I}, step, p.M, p.I, st);
-  if (rc) return rc;
-  rc = Products<T>::raw(p.M, p.O, p.I, h, p.I, static_cast<const T*>(p.wd), p.ldd, false, sums,
-                        splits, st);
-  if (rc) return rc;
-  const LinearStep<T> out{nullptr, static_cast<const T*>(p.residual), static_cast<T*>(p.y), p.ldr,
-                          p.O, kActNone, Kept<T>{}};
-  return launch_rows(p.O % 8 == 0 && aligned_rows(p.residual, p.ldr) && aligned_rows(p.y, p.O),
-                     PartialSource{sums, splits, p.M * p.O, p.O}, NoSource{}, out, p.M, p.O, st);
+  const bool vec = p.O % 8 == 0 && aligned_rows(p.residual, p.ldr) && aligned_rows(p.y, p.O);
+  return launch_rows(vec, PartialSource{sums, splits, p.M * p.O, p.O}, NoSource{}, out, p.M,
+                     p.O, st);
 }
 
 struct MlpBwd {
@@ -331,28 +391,33 @@ struct MlpBwd {
   int64_t M, H, I, O;
 };
 
-template <typename T>
+template <typename T, int KIND>
 int mlp_bwd(const MlpBwd& p, Arena& ws, bool run, hipStream_t st) {
   const size_t mi = (size_t)(p.M * p.I);
   T* dg = ws.take<T>(mi);
   T* du = ws.take<T>(mi);
   T* h = ws.take<T>(mi);
-  float* sums = ws.take<float>(Products<T>::raw_floats(p.M, p.I, p.O));
+  const bool fuse = Products<T>::fused(p.M, p.I, p.O);
+  float* sums = ws.take<float>(fuse ? 0 : Products<T>::raw_floats(p.M, p.I, p.O));
   size_t wsb = larger(Products<T>::store_bytes(p.M, p.H, 2 * p.I), Products<T>::wgrad_bytes(p.I, p.H, p.M));
   wsb = larger(wsb, Products<T>::wgrad_bytes(p.O, p.I, p.M));
   char* pws = ws.take<char>(wsb);
   if (!run) return ML_OK;
   const T* x = static_cast<const T*>(p.x);
   const T* dy = static_cast<const T*>(p.dy);
-  int splits = 1;
-  int rc = Products<T>::raw(p.M, p.I, p.O, dy, p.ldy, static_cast<const T*>(p.wd), p.ldd, true,
-                            sums, splits, st);
-  if (rc) return rc;
-  const GatedGradStep<T> step{dg, du, p.dwd ? h : nullptr, p.I,
-                              make_kept<T>(p.keep, p.gate, p.gscale, p.I),
-                              make_kept<T>(p.keep, p.up, p.uscale, p.I)};
-  rc = launch_rows(p.I % 8 == 0, PartialSource{sums, splits, p.M * p.I, p.I}, NoSource{}, step, p.M,
-                   p.I, st);
+  const T* wd = static_cast<const T*>(p.wd);
+  const GatedGradStep<T, KIND> step{dg, du, p.dwd ? h : nullptr, p.I,
+                                    make_kept<KIND>(p.gate, p.gscale, p.I),
+                                    make_kept<KIND>(p.up, p.uscale, p.I)};
+  int splits = 1, rc;
+  if (fuse) {
+    rc = Products<T>::template through<kMNMajor>(p.M, p.I, p.O, dy, p.ldy, wd, p.ldd, step, st);
+  } else {
+    rc = Products<T>::raw(p.M, p.I, p.O, dy, p.ldy, wd, p.ldd, true, sums, splits, st);
+    if (rc) return rc;
+    rc = launch_rows(p.I % 8 == 0, PartialSource{sums, splits, p.M * p.I, p.I}, NoSource{}, step,
+                     p.M, p.I, st);
+  }
   if (rc) return rc;
   if (p.dx) {
     const int64_t ks[2] = {p.I, p.I}, la[2] = {p.I, p.I}, lb[2] = {p.ldg, p.ldu};
@@ -391,7 +456,8 @@ extern "C" size_t ml_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K,
   ffn::Arena ws{nullptr};
   ffn::dispatch(dtype, [&](auto t) {
     using T = decltype(t);
-    return ffn::linear_fwd<T>(nullptr, 0, nullptr, 0, ffn::LinearStep<T>{}, M, N, K, ws, false, nullptr);
+    return ffn::linear_fwd<T>(nullptr, 0, nullptr, 0, ffn::LinearStep<T, ffn::kKeepNone>{}, M, N, K,
+                              ws, false, nullptr);
   });
   return ws.used;
 }
@@ -410,14 +476,19 @@ extern "C" int ml_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t 
     using T = decltype(t);
     ML_TRY(ffn::Products<T>::check(x, ldx, K, "x"));
     ML_TRY(ffn::Products<T>::check(w, ldw, K, "weight"));
+    ML_TRY(ffn::Products<T>::check(y, ldy, N, "y"));
+    ML_TRY(ffn::Products<T>::check(bias, 0, N, "bias"));
+    ML_TRY(ffn::Products<T>::check(residual, residual ? ldr : 0, N, "residual"));
     ffn::Arena ws{static_cast<char*>(workspace)};
     const size_t need = ml_linear_fwd_workspace_bytes(M, N, K, dtype);
     ML_CHECK(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
              "linear: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-    const ffn::LinearStep<T> step{static_cast<const T*>(bias), static_cast<const T*>(residual),
-                                  static_cast<T*>(y), ldr, ldy, act,
-                                  ffn::make_kept<T>(keep, z, zscale, N)};
-    return ffn::linear_fwd<T>(x, ldx, w, ldw, step, M, N, K, ws, true, (hipStream_t)stream);
+    return ffn::dispatch_keep<T>(keep, [&](auto kind) {
+      const ffn::LinearStep<T, kind.value> step{
+          static_cast<const T*>(bias), static_cast<const T*>(residual), static_cast<T*>(y), ldr,
+          ldy, act, ffn::make_kept<kind.value>(z, zscale, N)};
+      return ffn::linear_fwd<T>(x, ldx, w, ldw, step, M, N, K, ws, true, (hipStream_t)stream);
+    });
   });
 }
 
@@ -486,7 +557,7 @@ extern "C" size_t ml_swiglu_mlp_fwd_workspace_bytes(int64_t M, int64_t H, int64_
   p.I = I;
   p.O = O;
   ffn::Arena ws{nullptr};
-  ffn::dispatch(dtype, [&](auto t) { return ffn::mlp_fwd<decltype(t)>(p, ws, false, nullptr); });
+  ffn::dispatch(dtype, [&](auto t) { return ffn::mlp_fwd<decltype(t), ffn::kKeepNone>(p, ws, false, nullptr); });
   return ws.used;
 }
 
@@ -508,13 +579,17 @@ extern "C" int ml_swiglu_mlp_fwd(const void* x, int64_t ldx, const void* wg, int
     ML_TRY(ffn::Products<T>::check(wg, ldg, H, "gate weight"));
     ML_TRY(ffn::Products<T>::check(wu, ldu, H, "up weight"));
     ML_TRY(ffn::Products<T>::check(wd, ldd, I, "down weight"));
+    ML_TRY(ffn::Products<T>::check(y, O, O, "y"));
+    ML_TRY(ffn::Products<T>::check(residual, residual ? ldr : 0, O, "residual"));
     ffn::Arena ws{static_cast<char*>(workspace)};
     const size_t need = ml_swiglu_mlp_fwd_workspace_bytes(M, H, I, O, dtype);
     ML_CHECK(workspace_bytes >= need && workspace && aligned16(workspace),
              "swiglu mlp: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     const ffn::MlpFwd p{x, wg, wu, wd, residual, ldx, ldg, ldu, ldd, ldr, y, keep,
                         gate, gate_scale, up, up_scale, M, H, I, O};
-    return ffn::mlp_fwd<T>(p, ws, true, (hipStream_t)stream);
+    return ffn::dispatch_keep<T>(keep, [&](auto kind) {
+      return ffn::mlp_fwd<T, kind.value>(p, ws, true, (hipStream_t)stream);
+    });
   });
 }
 
@@ -527,7 +602,7 @@ extern "C" size_t ml_swiglu_mlp_bwd_workspace_bytes(int64_t M, int64_t H, int64_
   p.I = I;
   p.O = O;
   ffn::Arena ws{nullptr};
-  ffn::dispatch(dtype, [&](auto t) { return ffn::mlp_bwd<decltype(t)>(p, ws, false, nullptr); });
+  ffn::dispatch(dtype, [&](auto t) { return ffn::mlp_bwd<decltype(t), ffn::kKeepFp8>(p, ws, false, nullptr); });
   return ws.used;
 }
 
@@ -563,7 +638,12 @@ extern "C" int ml_swiglu_mlp_bwd(const void* x, int64_t ldx, const void* wg, int
              "swiglu mlp backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     const ffn::MlpBwd p{x, wg, wu, wd, dy, ldx, ldg, ldu, ldd, ldy, keep, gate, gate_scale, up,
                         up_scale, dx, dwg, dwu, dwd, M, H, I, O};
-    return ffn::mlp_bwd<T>(p, ws, true, (hipStream_t)stream);
+    return ffn::dispatch_keep<T>(keep, [&](auto kind) -> int {
+      if constexpr (kind.value == ffn::kKeepNone)
+        return ML_ERR_INVALID;  // (refused above)
+      else
+        return ffn::mlp_bwd<T, kind.value>(p, ws, true, (hipStream_t)stream);
+    });
   });
 }
 
@@ -581,11 +661,11 @@ extern "C" int ml_swiglu_kept_fwd(const void* gate, const void* up, void* out, v
     using T = decltype(t);
     const bool vec = cols % 8 == 0 && aligned16(gate) && aligned16(up) && aligned16(out);
     // whole blocks: one long row
-    const bool flat = cols % held8::kBlock == 0;
+    const bool flat = cols % held::kBlock == 0;
     const int64_t r = flat ? 1 : rows, c = flat ? rows * cols : cols;
-    const ffn::GatedStep<T> step{static_cast<T*>(out), c,
-                                 ffn::make_kept<T>(ffn::kKeepFp8, gate_q, gate_scale, c),
-                                 ffn::make_kept<T>(ffn::kKeepFp8, up_q, up_scale, c)};
+    const ffn::GatedStep<T, ffn::kKeepFp8> step{
+        static_cast<T*>(out), c, ffn::make_kept<ffn::kKeepFp8>(gate_q, gate_scale, c),
+        ffn::make_kept<ffn::kKeepFp8>(up_q, up_scale, c)};
     return ffn::launch_rows(vec, ffn::TypedSource<T>{static_cast<const T*>(gate), c},
                             ffn::TypedSource<T>{static_cast<const T*>(up), c}, step, r, c,
                             (hipStream_t)stream);
@@ -603,11 +683,12 @@ extern "C" int ml_swiglu_kept_bwd(const void* gate_q, const void* gate_scale, co
   return dispatch_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
     const bool vec = cols % 8 == 0 && aligned16(dy) && aligned16(dgate) && aligned16(dup);
-    const bool flat = cols % held8::kBlock == 0;
+    const bool flat = cols % held::kBlock == 0;
     const int64_t r = flat ? 1 : rows, c = flat ? rows * cols : cols;
-    const ffn::GatedGradStep<T> step{static_cast<T*>(dgate), static_cast<T*>(dup), nullptr, c,
-                                     ffn::make_kept<T>(ffn::kKeepFp8, gate_q, gate_scale, c),
-                                     ffn::make_kept<T>(ffn::kKeepFp8, up_q, up_scale, c)};
+    const ffn::GatedGradStep<T, ffn::kKeepFp8> step{
+        static_cast<T*>(dgate), static_cast<T*>(dup), nullptr, c,
+        ffn::make_kept<ffn::kKeepFp8>(gate_q, gate_scale, c),
+        ffn::make_kept<ffn::kKeepFp8>(up_q, up_scale, c)};
     return ffn::launch_rows(vec, ffn::TypedSource<T>{static_cast<const T*>(dy), c}, ffn::NoSource{},
                             step, r, c, (hipStream_t)stream);
   });

@@ -2,24 +2,26 @@
 // on VEC neighbouring columns of a row at a time (8, as 16-byte accesses of 16-bit
 // elements; 1 where sizes, strides or bases rule those out). 32 / VEC neighbouring
 // lanes hold a block of 32 columns, so that a step can keep a tensor in 8 bits
-// (held8.h). The same steps run in a product's epilogue and over arrays in memory.
+// (held.h). The same steps run in a product's epilogue and over arrays in memory.
 #pragma once
 
 #include "act_math.h"
-#include "held8.h"
+#include "held.h"
 
 namespace mla {
 namespace ffn {
 
-enum : int { kKeepNone = 0, kKeepSame = 1, kKeepFp8 = 2 };
+enum : int { kKeepNone = ML_KEEP_NONE, kKeepF32 = ML_KEEP_F32, kKeepFp16 = ML_KEEP_FP16,
+             kKeepFp8 = ML_KEEP_FP8 };
 
-// A [rows, cols] tensor kept for the backward, dense: in T, or its bytes with
-// ceil(cols / 32) scale bytes a row.
-template <typename T>
+// A [rows, cols] tensor kept for the backward, dense: in fp32, or in 16 or 8 bits an
+// element with ceil(cols / 32) scale bytes a row (held.h); or not at all. (KIND is a
+// template parameter so that fetch's loads stand in no branch.)
+template <int KIND>
 struct Kept {
-  int kind;
-  T* v;
-  uint8_t* q;
+  using Elem = std::conditional_t<KIND == kKeepF32, float,
+                                  std::conditional_t<KIND == kKeepFp16, f16, uint8_t>>;
+  Elem* v;
   uint8_t* scale;
   int64_t cols, nblocks;
 
@@ -27,36 +29,68 @@ struct Kept {
   template <int VEC>
   __device__ __forceinline__ void put(int64_t m, int64_t n, const float (&x)[VEC],
                                       bool live) const {
-    if (kind == kKeepSame) {
-      if (live) store_n<T, VEC>(v + m * cols + n, x);
-    } else if (kind == kKeepFp8) {
-      const uint32_t b = held8::block_byte<VEC>(x);
-      if (live) {
-        held8::store<VEC>(q + m * cols + n, b, x);
-        if (n % held8::kBlock == 0) scale[m * nblocks + n / held8::kBlock] = (uint8_t)b;
-      }
+    const int64_t at = m * cols + n;
+    if constexpr (KIND == kKeepF32) {
+      if (live) store_n<float, VEC>(v + at, x);
+    } else if constexpr (KIND != kKeepNone) {
+      const uint32_t b = held::block_byte<KIND == kKeepFp16 ? held::kTop16 : held::kTop8, VEC>(x);
+      if (!live) return;
+      if (n % held::kBlock == 0) scale[m * nblocks + n / held::kBlock] = (uint8_t)b;
+      if constexpr (KIND == kKeepFp16)
+        held::store16<VEC>(v + at, b, x);
+      else
+        held::store<VEC>(v + at, b, x);
     }
   }
 
+  // Bits of VEC elements as they lie in memory, and their scale's byte: fetched
+  // first, decoded when they are needed, so that several are in flight.
   template <int VEC>
-  __device__ __forceinline__ void get(int64_t m, int64_t n, float (&x)[VEC]) const {
-    if (kind == kKeepSame)
-      load_n<T, VEC>(v + m * cols + n, x);
+  struct Raw {
+    uint32_t w[(VEC * sizeof(Elem) + 3) / 4];
+    uint32_t byte;
+  };
+
+  template <int VEC>
+  __device__ __forceinline__ Raw<VEC> fetch(int64_t m, int64_t n) const {
+    Raw<VEC> r;
+    constexpr int N = VEC * (int)sizeof(Elem);
+    const Elem* p = v + m * cols + n;
+    if constexpr (N < 4)
+      r.w[0] = N == 1 ? *reinterpret_cast<const uint8_t*>(p) : *reinterpret_cast<const uint16_t*>(p);
     else
-      held8::load<VEC>(q + m * cols + n, scale[m * nblocks + n / held8::kBlock], x);
+      __builtin_memcpy(r.w, __builtin_assume_aligned(p, N < 16 ? N : 16), N);
+    r.byte = KIND == kKeepF32 ? 0 : scale[m * nblocks + n / held::kBlock];
+    return r;
+  }
+
+  template <int VEC>
+  __device__ __forceinline__ void decode(const Raw<VEC>& r, float (&x)[VEC]) const {
+    if constexpr (KIND == kKeepF32)
+      __builtin_memcpy(x, r.w, sizeof(x));
+    else if constexpr (KIND == kKeepFp16)
+      held::load16<VEC>(r.w, r.byte, x);
+    else
+      held::load<VEC>(r.w, r.byte, x);
   }
 };
 
-template <typename T>
-inline Kept<T> make_kept(int kind, const void* v, const void* scale, int64_t cols) {
-  Kept<T> k{};
-  k.kind = v ? kind : kKeepNone;
-  k.v = kind == kKeepSame ? static_cast<T*>(const_cast<void*>(v)) : nullptr;
-  k.q = kind == kKeepFp8 ? static_cast<uint8_t*>(const_cast<void*>(v)) : nullptr;
-  k.scale = static_cast<uint8_t*>(const_cast<void*>(scale));
-  k.cols = cols;
-  k.nblocks = held8::blocks(cols);
-  return k;
+template <int KIND>
+inline Kept<KIND> make_kept(const void* v, const void* scale, int64_t cols) {
+  return Kept<KIND>{static_cast<typename Kept<KIND>::Elem*>(const_cast<void*>(v)),
+                    static_cast<uint8_t*>(const_cast<void*>(scale)), cols, held::blocks(cols)};
+}
+
+// VEC elements of T as they are (16-byte transactions where that is their size or more).
+template <typename T, int VEC>
+__device__ __forceinline__ void load_pack(const T* p, Pack<T, VEC>& r) {
+  constexpr int P = VEC * (int)sizeof(T) >= 16 ? 16 / (int)sizeof(T) : VEC;
+#pragma unroll
+  for (int i = 0; i < VEC; i += P) {
+    const Pack<T, P> q = *reinterpret_cast<const Pack<T, P>*>(p + i);
+#pragma unroll
+    for (int k = 0; k < P; ++k) r.v[i + k] = q.v[k];
+  }
 }
 
 template <int VEC>
@@ -99,48 +133,89 @@ __device__ __forceinline__ void act_grad_vec(int act, float (&x)[VEC]) {
   }
 }
 
+// A step: column(n) gives what it needs of a lane's columns, fetch(m, n) issues its
+// loads for a position, and finish(...) does the work. Every lane of a block takes part
+// in finish; live says whether this lane's position exists (else what column and fetch
+// gave is not used).
+
 // z = x + bias; y = act(z) + residual; z kept.
-template <typename T>
+template <typename T, int KIND>
 struct LinearStep {
   const T* bias;      // or null
   const T* residual;  // or null
   T* y;
   int64_t ldr, ldy;
   int act;
-  Kept<T> z;
+  Kept<KIND> z;
 
   template <int VEC>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&x)[VEC],
-                                             bool live) const {
-    if (bias && live) {
-      float b[VEC];
-      load_n<T, VEC>(bias + n, b);
+  struct Column {
+    float b[VEC];
+  };
+  template <int VEC>
+  struct Fetched {
+    Pack<T, VEC> r;
+  };
+
+  template <int VEC>
+  __device__ __forceinline__ Column<VEC> column(int64_t n) const {
+    Column<VEC> c;
+    if (bias) {
+      load_n<T, VEC>(bias + n, c.b);
+    } else {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] += b[k];
+      for (int k = 0; k < VEC; ++k) c.b[k] = 0.f;
+    }
+    return c;
+  }
+
+  template <int VEC>
+  __device__ __forceinline__ Fetched<VEC> fetch(int64_t m, int64_t n) const {
+    Fetched<VEC> f;
+    if (residual) load_pack<T, VEC>(residual + m * ldr + n, f.r);
+    return f;
+  }
+
+  template <int VEC>
+  __device__ __forceinline__ void finish(int64_t m, int64_t n, float (&x)[VEC],
+                                         const Column<VEC>& c, const Fetched<VEC>& f,
+                                         bool live) const {
+    if (live) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) x[k] += c.b[k];
     }
     z.template put<VEC>(m, n, x, live);
     if (!live) return;
     act_fwd_vec<VEC>(act, x);
     if (residual) {
-      float r[VEC];
-      load_n<T, VEC>(residual + m * ldr + n, r);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] += r[k];
+      for (int k = 0; k < VEC; ++k) x[k] += to_f32(f.r.v[k]);
     }
     store_n<T, VEC>(y + m * ldy + n, x);
   }
 };
 
 // h = silu(g) u; g and u kept.
-template <typename T>
+template <typename T, int KIND>
 struct GatedStep {
   T* h;  // dense
   int64_t cols;
-  Kept<T> gate, up;
+  Kept<KIND> gate, up;
 
   template <int VEC>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&g)[VEC],
-                                             float (&u)[VEC], bool live) const {
+  struct Column {};
+  template <int VEC>
+  struct Fetched {};
+
+  template <int VEC>
+  __device__ __forceinline__ Column<VEC> column(int64_t) const { return {}; }
+  template <int VEC>
+  __device__ __forceinline__ Fetched<VEC> fetch(int64_t, int64_t) const { return {}; }
+
+  template <int VEC>
+  __device__ __forceinline__ void finish(int64_t m, int64_t n, float (&g)[VEC], float (&u)[VEC],
+                                         const Column<VEC>&, const Fetched<VEC>&,
+                                         bool live) const {
     gate.template put<VEC>(m, n, g, live);
     up.template put<VEC>(m, n, u, live);
     if (!live) return;
@@ -151,21 +226,36 @@ struct GatedStep {
 };
 
 // dg, du and (h not null) h again from dh and the kept g, u.
-template <typename T>
+template <typename T, int KIND>
 struct GatedGradStep {
   T* dg;
   T* du;
   T* h;  // or null
   int64_t cols;
-  Kept<T> gate, up;
+  Kept<KIND> gate, up;
 
   template <int VEC>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, float (&dh)[VEC],
-                                             bool live) const {
+  struct Column {};
+  template <int VEC>
+  struct Fetched {
+    typename Kept<KIND>::template Raw<VEC> g, u;
+  };
+
+  template <int VEC>
+  __device__ __forceinline__ Column<VEC> column(int64_t) const { return {}; }
+  template <int VEC>
+  __device__ __forceinline__ Fetched<VEC> fetch(int64_t m, int64_t n) const {
+    return {gate.template fetch<VEC>(m, n), up.template fetch<VEC>(m, n)};
+  }
+
+  template <int VEC>
+  __device__ __forceinline__ void finish(int64_t m, int64_t n, float (&dh)[VEC],
+                                         const Column<VEC>&, const Fetched<VEC>& f,
+                                         bool live) const {
     if (!live) return;
     float g[VEC], u[VEC], hv[VEC];
-    gate.template get<VEC>(m, n, g);
-    up.template get<VEC>(m, n, u);
+    gate.template decode<VEC>(f.g, g);
+    up.template decode<VEC>(f.u, u);
 #pragma unroll
     for (int k = 0; k < VEC; ++k)
       swiglu_bwd_fwd_elem(g[k], u[k], dh[k], g[k], u[k], hv[k]);
@@ -217,28 +307,34 @@ template <int VEC, class Src, class Src2, class Step>
 __global__ __launch_bounds__(kThreads) void rows_kernel(const Src src, const Src2 src2,
                                                         const Step step, int64_t rows,
                                                         int64_t cols) {
-  constexpr int L = held8::kBlock / VEC;
-  const int64_t nb = (cols + held8::kBlock - 1) / held8::kBlock;
+  constexpr int L = held::kBlock / VEC;
+  const int64_t nb = (cols + held::kBlock - 1) / held::kBlock;
   const int64_t groups = rows * nb;
   const int64_t step_groups = (int64_t)gridDim.x * (kThreads / L);
   const int l = threadIdx.x % L;
   for (int64_t g = (int64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L; g < groups;
        g += step_groups) {
     const int64_t m = rows == 1 ? 0 : g / nb;
-    const int64_t n = (g - m * nb) * held8::kBlock + l * VEC;
+    const int64_t n = (g - m * nb) * held::kBlock + l * VEC;
     const bool live = n < cols;
     float x[VEC];
 #pragma unroll
     for (int k = 0; k < VEC; ++k) x[k] = 0.f;
     if (live) src.template load<VEC>(m, n, x);
+    typename Step::template Column<VEC> c;
+    typename Step::template Fetched<VEC> f;
+    if (live) {
+      c = step.template column<VEC>(n);
+      f = step.template fetch<VEC>(m, n);
+    }
     if constexpr (std::is_same_v<Src2, NoSource>) {
-      step.template operator()<VEC>(m, n, x, live);
+      step.template finish<VEC>(m, n, x, c, f, live);
     } else {
       float u[VEC];
 #pragma unroll
       for (int k = 0; k < VEC; ++k) u[k] = 0.f;
       if (live) src2.template load<VEC>(m, n, u);
-      step.template operator()<VEC>(m, n, x, u, live);
+      step.template finish<VEC>(m, n, x, u, c, f, live);
     }
   }
 }
@@ -247,8 +343,8 @@ template <class Src, class Src2, class Step>
 inline int launch_rows(bool vec, const Src& src, const Src2& src2, const Step& step, int64_t rows,
                        int64_t cols, hipStream_t st) {
   if (rows == 0 || cols == 0) return ML_OK;
-  const int64_t groups = rows * held8::blocks(cols);
-  const int per = kThreads / (held8::kBlock / (vec ? 8 : 1));
+  const int64_t groups = rows * held::blocks(cols);
+  const int per = kThreads / (held::kBlock / (vec ? 8 : 1));
   int64_t blocks = (groups + per - 1) / per;
   blocks = blocks < (1 << 20) ? blocks : (1 << 20);
   if (vec)
@@ -262,14 +358,14 @@ inline int launch_rows(bool vec, const Src& src, const Src2& src2, const Step& s
 }
 
 // ------------------------------------------- the linear layer's backward step --
-// dz = dy act'(z) (dz null: not written, as where there is no activation) and the
+// dz = dy act'(z) (KIND none: dy, where there is no activation; dz null: not written) and the
 // column sums of dz: a workgroup takes 32 VEC columns and a range of rows, its 8
 // row lanes' sums are joined in LDS, and the ranges' partial rows are summed in
 // their order by a second kernel. fp32 sums; dz is summed as it was before its
 // rounding.
-template <int VEC, typename T>
+template <int VEC, typename T, int KIND>
 __global__ __launch_bounds__(kThreads) void linear_grad_kernel(
-    const T* __restrict__ dy, int64_t ldy, const Kept<T> z, int act, T* __restrict__ dz,
+    const T* __restrict__ dy, int64_t ldy, const Kept<KIND> z, int act, T* __restrict__ dz,
     float* __restrict__ partial, int64_t rows, int64_t cols, int64_t rows_per) {
   const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
   const int64_t n = ((int64_t)blockIdx.x * 32 + cl) * VEC;
@@ -283,9 +379,9 @@ __global__ __launch_bounds__(kThreads) void linear_grad_kernel(
     for (int64_t m = r0 + rl; m < r1; m += 8) {
       float d[VEC];
       load_n<T, VEC>(dy + m * ldy + n, d);
-      if (act != kActNone) {
+      if constexpr (KIND != kKeepNone) {
         float v[VEC];
-        z.template get<VEC>(m, n, v);
+        z.template decode<VEC>(z.template fetch<VEC>(m, n), v);
         act_grad_vec<VEC>(act, v);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) d[k] *= v[k];

@@ -1199,10 +1199,22 @@ struct R4Frags {
 // block tile; acc[h][i][j] is MFMA tile (i, 4 h + j).
 // SPLIT: the kernel may take part of K (its epilogue writes partials);
 // otherwise the prologue holds no code for it.
-template <int LA, int LB, int T, bool SPLIT>
+// PAIR (one segment, B K-major): two B operands of N rows each, b2 the second; a
+// wave's first 8 T columns are rows of the first, its last 8 T the same rows of the
+// second, so that it holds both products of its rows (the gated block's gate and
+// up). The tile covers half as many rows of each: group g of 8 rows of the LDS tile
+// comes from operand g / T % 2, rows 8 T (g / 2 T) + 8 (g % T). A wave's load i is
+// group wave + 4 i, whose operand and offset depend on i alone.
+template <int T>
+constexpr int pair_which(int i) { return i / (T / 4) % 2; }
+template <int T>
+constexpr int pair_step(int i) { return i % (T / 4) + T / 4 * (i / (T / 2)); }
+
+template <int LA, int LB, int T, bool SPLIT, bool PAIR = false>
 __device__ __forceinline__ void r4_mainloop(const Problem& pb, int tm, int tn, int split,
                                             int ksplit, int kps, char* lds,
-                                            f32x4_t (&acc)[T / 4][T][4]) {
+                                            f32x4_t (&acc)[T / 4][T][4], Operand b2 = {}) {
+  static_assert(!PAIR || (LB == kKMajor && !SPLIT), "a pair: K-major rows, K not split");
   using G = r4::Geom<T>;
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -1210,7 +1222,7 @@ __device__ __forceinline__ void r4_mainloop(const Problem& pb, int tm, int tn, i
   const int wm = (wave >> 1) * G::W;
   const int wn = (wave & 1) * G::W;
   const int m0 = tm * G::TILE;
-  const int n0 = tn * G::TILE;
+  const int n0 = tn * (PAIR ? G::TILE / 2 : G::TILE);
 #pragma unroll
   for (int h = 0; h < T / 4; ++h)
 #pragma unroll
@@ -1238,13 +1250,15 @@ __device__ __forceinline__ void r4_mainloop(const Problem& pb, int tm, int tn, i
   R4Load<LB> ib;
   r4_setup<LA, T>(ia, pb.seg[seg].a, m0, pb.M, kc, klen, wave, lane);
   r4_setup<LB, T>(ib, pb.seg[seg].b, n0, pb.N, kc, klen, wave, lane);
+  R4Load<LB> ic;  // PAIR: the second operand's
+  if constexpr (PAIR) r4_setup<LB, T>(ic, b2, n0, pb.N, kc, klen, wave, lane);
   R4Frag<LA, T> fa;
   R4Frag<LB, T> fb;
   r4_frag_setup<LA, T>(fa, wm, lane);
   r4_frag_setup<LB, T>(fb, wn, lane);
 
-  rsrc_t rsa, rsb;
-  uint32_t va[2], vb[2], sa, sb;
+  rsrc_t rsa, rsb, rsc;
+  uint32_t va[2], vb[2], vc[2], sa, sb;
   // Resources of the cursor's k-tile (with its segment's group stride: the
   // cursor may move to the next segment before the loads are issued), then
   // advance the cursor.
@@ -1252,6 +1266,7 @@ __device__ __forceinline__ void r4_mainloop(const Problem& pb, int tm, int tn, i
     const bool live = loaded < nk;
     r4_tile_rsrc<LA>(ia, kc, klen, live, rsa, va);
     r4_tile_rsrc<LB>(ib, kc, klen, live, rsb, vb);
+    if constexpr (PAIR) r4_tile_rsrc<LB>(ic, kc, klen, live, rsc, vc);
     sa = ia.istride;
     sb = ib.istride;
     ++loaded;
@@ -1268,6 +1283,10 @@ __device__ __forceinline__ void r4_mainloop(const Problem& pb, int tm, int tn, i
         ia.range -= ia.kstep;
         ib.base += ib.kstep;
         ib.range -= ib.kstep;
+        if constexpr (PAIR) {
+          ic.base += ic.kstep;
+          ic.range -= ic.kstep;
+        }
       }
     }
   };
@@ -1275,7 +1294,12 @@ __device__ __forceinline__ void r4_mainloop(const Problem& pb, int tm, int tn, i
   // into the operand slot `slot`.
   auto load = [&](auto opb, char* slot, int i) __attribute__((always_inline)) {
     char* dst = slot + (wave + 4 * i) * 1024;
-    if constexpr (decltype(opb)::value)
+    if constexpr (decltype(opb)::value && PAIR) {
+      if (pair_which<T>(i))
+        buf_load_lds(rsc, vc[0] + (uint32_t)pair_step<T>(i) * ic.istride, dst);
+      else
+        buf_load_lds(rsb, vb[0] + (uint32_t)pair_step<T>(i) * sb, dst);
+    } else if constexpr (decltype(opb)::value)
       buf_load_lds(rsb, vb[i & 1] + (uint32_t)i * sb, dst);
     else
       buf_load_lds(rsa, va[i & 1] + (uint32_t)i * sa, dst);

@@ -1,19 +1,24 @@
-// Tensors kept in 8 bits for a backward pass: rows in blocks of 32 elements (a
-// row's last block may be shorter), each with one scale 2^e, elements as e4m3
-// (3 bits of mantissa, smallest step 2^-9) of v / 2^e:
-//   e = max(floor(log2 m) - 7, -126),  m the largest finite magnitude of the block
-//   (m = 0: e = -126); the scale's byte is e + 127.
-// A block's largest element lands in [128, 256), so nothing saturates (e4m3 ends
-// at 448) and the scale is a matter of m's exponent bits alone: 17 octaves below
-// it still differ from 0. Elements that are not finite are kept as NaN and do not
-// count for m. The scale is a power of two, so that v / 2^e rounds nothing; the
-// rounding to e4m3 (half a step: 2^-4 of the value) is the only one.
+// Tensors kept in 8 or 16 bits for a backward pass: rows in blocks of 32 elements (a
+// row's last block may be shorter), each with one scale 2^e, elements as v / 2^e in
+//   8 bits   e4m3 (3 bits of mantissa, smallest step 2^-9), e = floor(log2 m) - 7
+//   16 bits  fp16 (10 bits of mantissa),                    e = floor(log2 m) - 14
+// for the largest finite magnitude m of the block; e is at least -126, and -126 where
+// m = 0; the scale's byte is e + 127. A block's largest element lands in [128, 256) or
+// [2^14, 2^15), so nothing saturates (e4m3 ends at 448, fp16 at 65504), and the scale
+// is a matter of m's exponent bits alone: 17 octaves below it (fp16: 39) still differ
+// from 0. Elements that are not finite do not count for m; e4m3 keeps them as NaN. The
+// scale is a power of two, so that v / 2^e rounds nothing; the rounding to e4m3 (half a
+// step: 2^-4 of the value) or fp16 (2^-11) is the only one.
+// The 16 bits are fp16 with a scale rather than bf16 because a backward multiplies what
+// it reads: gate and up in bf16 (2^-8) took the weights' gradients of the gated block
+// from 2.4e-3 to 3.5e-3 of their norm off 64 bits, 1.7e-3 being the rounding of the
+// result alone; 33 bytes more for 1024 elements.
 #pragma once
 
 #include "common.h"
 
 namespace mla {
-namespace held8 {
+namespace held {
 
 constexpr int kBlock = 32;
 
@@ -25,9 +30,12 @@ __device__ __forceinline__ uint32_t finite_bits(float v) {
   return b < 0x7F800000u ? b : 0u;
 }
 
-// The scale's byte from the bits of m: its exponent field less 7, at least 1.
+// The scale's byte from the bits of m: its exponent field less TOP, at least 1.
+constexpr int kTop8 = 7, kTop16 = 14;
+
+template <int TOP>
 __device__ __forceinline__ uint32_t scale_byte(uint32_t max_bits) {
-  const int e = (int)(max_bits >> 23) - 7;
+  const int e = (int)(max_bits >> 23) - TOP;
   return (uint32_t)(e > 1 ? e : 1);
 }
 
@@ -51,7 +59,7 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t m) {
 }
 
 // The scale's byte of a block that 32 / VEC neighbouring lanes hold VEC elements of.
-template <int VEC>
+template <int TOP, int VEC>
 __device__ __forceinline__ uint32_t block_byte(const float (&v)[VEC]) {
   uint32_t m = 0;
 #pragma unroll
@@ -59,7 +67,7 @@ __device__ __forceinline__ uint32_t block_byte(const float (&v)[VEC]) {
     const uint32_t b = finite_bits(v[k]);
     m = m > b ? m : b;
   }
-  return scale_byte(lanes_max<kBlock / VEC>(m));
+  return scale_byte<TOP>(lanes_max<kBlock / VEC>(m));
 }
 
 __device__ __forceinline__ float to_scaled(float v, float inv) {
@@ -92,16 +100,15 @@ __device__ __forceinline__ void store(uint8_t* q, uint32_t byte, const float (&v
   }
 }
 
+// VEC elements of the bytes in w.
 template <int VEC>
-__device__ __forceinline__ void load(const uint8_t* q, uint32_t byte, float (&v)[VEC]) {
+__device__ __forceinline__ void load(const uint32_t* w, uint32_t byte, float (&v)[VEC]) {
   const float s = scale_of(byte);
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   if constexpr (VEC == 1) {
-    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)*q, false);
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[0], false);
     v[0] = a[0] * s;
   } else {
-    uint32_t w[VEC / 4];
-    __builtin_memcpy(w, __builtin_assume_aligned(q, VEC), VEC);
 #pragma unroll
     for (int k = 0; k < VEC / 4; ++k) {
       const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[k], false);
@@ -114,5 +121,23 @@ __device__ __forceinline__ void load(const uint8_t* q, uint32_t byte, float (&v)
   }
 }
 
-}  // namespace held8
+// The same in 16 bits (q aligned to 2 VEC bytes).
+template <int VEC>
+__device__ __forceinline__ void store16(f16* q, uint32_t byte, const float (&v)[VEC]) {
+  const float inv = inverse_of(byte);
+  float w[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) w[k] = v[k] * inv;
+  store_n<f16, VEC>(q, w);
+}
+
+template <int VEC>
+__device__ __forceinline__ void load16(const uint32_t* w, uint32_t byte, float (&v)[VEC]) {
+  const float s = scale_of(byte);
+#pragma unroll
+  for (int k = 0; k < VEC; ++k)
+    v[k] = static_cast<float>(__builtin_bit_cast(f16, (uint16_t)(w[k / 2] >> (k % 2 * 16)))) * s;
+}
+
+}  // namespace held
 }  // namespace mla

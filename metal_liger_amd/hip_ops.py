@@ -153,16 +153,26 @@ def swiglu_bwd(gate: torch.Tensor, up: torch.Tensor, dy: torch.Tensor):
     return dg, du
 
 
-# What a backward needs of its forward, kept whole or in 8 bits (ML_KEEP_*).
-KEEP_NONE, KEEP_SAME, KEEP_FP8 = 0, 1, 2
+# What a backward needs of its forward, kept in fp32 or in 16 or 8 bits with scales
+# (ML_KEEP_*).
+KEEP_NONE, KEEP_F32, KEEP_FP16, KEEP_FP8 = 0, 1, 2, 3
+KEEP_DTYPE = {KEEP_F32: torch.float32, KEEP_FP16: torch.float16, KEEP_FP8: torch.uint8}
 KEEP_BLOCK = 32  # elements of a row that share a scale
 
 
 def kept_shapes(shape):
-    """Shapes of a tensor's bytes and of their scales (ML_KEEP_FP8): blocks lie in rows
-    of the last dimension."""
+    """Shapes of a kept tensor's elements and of their scales: blocks lie in rows of the
+    last dimension."""
     shape = tuple(shape) or (1,)
     return shape, (*shape[:-1], -(-shape[-1] // KEEP_BLOCK))
+
+
+def kept_layout(rows, cols, keep: int):
+    """(shape, dtype) of a [rows, cols] tensor's elements and scales as `keep` says; [0]
+    where there are none."""
+    values, scales = kept_shapes((rows, cols))
+    return ((values if keep else (0,), KEEP_DTYPE.get(keep, torch.uint8)),
+            (scales if keep >= KEEP_FP16 else (0,), torch.uint8))
 
 
 def swiglu_kept_fwd(gate: torch.Tensor, up: torch.Tensor):
@@ -203,12 +213,8 @@ def swiglu_kept_bwd(gate_q, gate_scale, up_q, up_scale, dy, gate_dtype, up_dtype
 
 def _kept_buffers(x: torch.Tensor, cols: int, keep: int):
     """(values, scales) for x.shape[0] rows of cols; [0] where nothing is kept."""
-    rows = x.shape[0]
-    if keep == KEEP_FP8:
-        return [torch.empty(s, dtype=torch.uint8, device=x.device)
-                for s in kept_shapes((rows, cols))]
-    return [torch.empty((rows, cols) if keep == KEEP_SAME else (0,), dtype=x.dtype, device=x.device),
-            torch.empty((0,), dtype=torch.uint8, device=x.device)]
+    return [torch.empty(shape, dtype=dtype, device=x.device)
+            for shape, dtype in kept_layout(x.shape[0], cols, keep)]
 
 
 def _product_rows(t: torch.Tensor) -> torch.Tensor:
@@ -236,8 +242,8 @@ def linear_fwd(x2, w, bias, residual, act: int, keep: int):
     z, zscale = _kept_buffers(x2, N, keep)
     if M == 0:
         return y, z, zscale
-    bias = None if bias is None else bias.contiguous()
-    residual = None if residual is None else rows_view(residual)
+    bias = None if bias is None else _al16(bias.contiguous())
+    residual = None if residual is None else _product_rows(residual)
     tag = dtype_tag(x2, "x")
     ws, wsb = _workspace(x2, "ml_linear_fwd_workspace_bytes", M, N, K, tag)
     call("ml_linear_fwd", ptr(x2), row_stride(x2), ptr(w), row_stride(w), ptr(bias), ptr(residual),
@@ -278,7 +284,7 @@ def swiglu_mlp_fwd(x2, wg, wu, wd, residual, keep: int):
     kept = _kept_buffers(x2, I, keep) + _kept_buffers(x2, I, keep)
     if M == 0:
         return (y, *kept)
-    residual = None if residual is None else rows_view(residual)
+    residual = None if residual is None else _product_rows(residual)
     tag = dtype_tag(x2, "x")
     ws, wsb = _workspace(x2, "ml_swiglu_mlp_fwd_workspace_bytes", M, H, I, O, tag)
     call("ml_swiglu_mlp_fwd", *_pairs(x2, wg, wu, wd), ptr(residual),

@@ -4,8 +4,9 @@ nn.Linear around their activations and residual adds).
 
 The sum over K, the bias, the activation and the residual are added up in fp32 and y is
 rounded once. The backward needs z = x W^T + bias where there is an activation: it is
-kept in x's dtype, or in 8 bits (checkpoint="fp8": e4m3 with a power of two as scale for
-every 32 columns of a row), formed of the fp32 sums. What is not needed (x where the
+kept in 16 bits (fp16 with a power of two as scale for every 32 columns of a row, which
+rounds finer than bf16; in fp32 where the products run in fp32), or in 8 (checkpoint=
+"fp8": e4m3 with such scales), formed of the fp32 sums. What is not needed (x where the
 weight is frozen, W where x needs no gradient) is not kept. First derivatives only.
 
 bf16 with sizes in multiples of 8 runs on the bf16 matrix cores, everything else on the
@@ -24,11 +25,16 @@ ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3}
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 
 
-def keep_mode(checkpoint: str | None) -> int:
-    """How a backward's tensors are kept: in their own type, or in 8 bits."""
+def check_checkpoint(checkpoint: str | None) -> None:
     if checkpoint not in (None, "fp8"):
         raise ValueError(f'checkpoint must be None or "fp8" (got {checkpoint!r})')
-    return hip_ops.KEEP_SAME if checkpoint is None else hip_ops.KEEP_FP8
+
+
+def keep_mode(checkpoint: str | None, dtype: torch.dtype) -> int:
+    """How a backward's tensors are kept where the products are of `dtype`."""
+    if checkpoint == "fp8":
+        return hip_ops.KEEP_FP8
+    return hip_ops.KEEP_FP16 if dtype == torch.bfloat16 else hip_ops.KEEP_F32
 
 
 def compute_dtype(x: torch.Tensor, *features: int) -> torch.dtype:
@@ -121,7 +127,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     if activation not in ACTIVATIONS:
         raise ValueError(f"fused_linear: activation {activation!r} is not one of "
                          f"{list(ACTIVATIONS)}")
-    act, keep = ACTIVATIONS[activation], keep_mode(checkpoint)
+    act = ACTIVATIONS[activation]
+    check_checkpoint(checkpoint)
     check_input("fused_linear", x, weight)
     if bias is not None and (tuple(bias.shape) != (weight.shape[0],) or bias.dtype != x.dtype):
         raise ValueError(f"fused_linear: bias {tuple(bias.shape)} {bias.dtype}, needed is "
@@ -131,6 +138,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     if not wants_grad(x, weight, bias, residual):
         with torch.no_grad():
             return _forward(x, weight, bias, residual, act, hip_ops.KEEP_NONE)[0]
+    keep = keep_mode(checkpoint, compute_dtype(x, *weight.shape))
     return _FusedLinearFunction.apply(x, weight, bias, residual, act, keep)
 
 
@@ -146,7 +154,7 @@ class MetalLigerLinear(nn.Module):
         if activation not in ACTIVATIONS:
             raise ValueError(f"MetalLigerLinear: activation {activation!r} is not one of "
                              f"{list(ACTIVATIONS)}")
-        keep_mode(checkpoint)
+        check_checkpoint(checkpoint)
         self.weight, self.bias = original.weight, original.bias
         self.activation, self.checkpoint = activation, checkpoint
 

@@ -14,7 +14,7 @@ import torch
 import torch.nn as nn
 
 from metal_liger_amd import _custom_ops as cops
-from metal_liger_amd.ops.fused_linear import keep_mode
+from metal_liger_amd.ops.fused_linear import check_checkpoint
 
 
 class _FusedSwiGLUFunction(torch.autograd.Function):
@@ -54,11 +54,10 @@ def fused_swiglu(gate: torch.Tensor, up: torch.Tensor,
     """Functional: SiLU(gate) * up in a single fused op (ops/fused_swiglu.py:54-56).
     checkpoint: None, or "fp8" to keep gate and up in 8 bits for the backward, whose
     gradients are then those at the values that the 8 bits stand for."""
+    check_checkpoint(checkpoint)
     if checkpoint is None or not (torch.is_grad_enabled()
                                   and (gate.requires_grad or up.requires_grad)):
-        keep_mode(checkpoint)
         return _FusedSwiGLUFunction.apply(gate, up)
-    keep_mode(checkpoint)
     return _FusedSwiGLUKeptFunction.apply(gate, up)
 
 

@@ -2,9 +2,9 @@
 (+ residual), and its backward (the reference fuses the activation step only,
 ops/fused_swiglu.py:59-75, and its LoRA block needs adapters).
 
-The backward needs gate = x Wg^T and up = x Wu^T: they are kept in x's dtype, or in 8
-bits (checkpoint="fp8": e4m3 with a power of two as scale for every 32 columns of a
-row), formed of the fp32 sums. h = silu(gate) * up is not kept; the backward forms it
+The backward needs gate = x Wg^T and up = x Wu^T: they are kept in 16 bits (fp16 with a
+power of two as scale for every 32 columns of a row; in fp32 where the products run in
+fp32), or in 8 (checkpoint="fp8": e4m3 with such scales), formed of the fp32 sums. h = silu(gate) * up is not kept; the backward forms it
 again of what was kept. h and the gradients of gate, up and h are rounded to bf16
 between the products on the bf16 matrix cores. First derivatives only. Types and sizes
 as ops/fused_linear.py.
@@ -16,8 +16,8 @@ import torch
 
 from metal_liger_amd import _custom_ops as cops
 from metal_liger_amd import hip_ops
-from metal_liger_amd.ops.fused_linear import (check_input, check_residual, compute_dtype, keep_mode,
-                                              rows, wants_grad)
+from metal_liger_amd.ops.fused_linear import (check_checkpoint, check_input, check_residual,
+                                              compute_dtype, keep_mode, rows, wants_grad)
 
 
 def _forward(x, weights, residual, keep: int):
@@ -63,7 +63,7 @@ def fused_swiglu_mlp(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torc
     residual [..., out]; all of x's dtype (fp32, bf16 or fp16) and on its device, any
     strides. checkpoint: None, or "fp8" to keep gate and up in 8 bits for the backward.
     """
-    keep = keep_mode(checkpoint)
+    check_checkpoint(checkpoint)
     check_input("fused_swiglu_mlp", x, gate_weight, up_weight, down_weight)
     if up_weight.shape != gate_weight.shape or down_weight.shape[1] != gate_weight.shape[0]:
         raise ValueError(f"fused_swiglu_mlp: weights {tuple(gate_weight.shape)}, "
@@ -74,4 +74,5 @@ def fused_swiglu_mlp(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torc
     if not wants_grad(x, *weights, residual):
         with torch.no_grad():
             return _forward(x, weights, residual, hip_ops.KEEP_NONE)[0]
+    keep = keep_mode(checkpoint, compute_dtype(x, x.shape[-1], *down_weight.shape))
     return _FusedSwiGLUMLPFunction.apply(x, *weights, residual, keep)

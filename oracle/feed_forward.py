@@ -40,7 +40,10 @@ def held_bytes(v):
 
 
 def held_values(codes, scales):
-    """What the bytes stand for, in 64 bits."""
+    """What the bytes (or fp16 elements) stand for, in 64 bits."""
+    if codes.dtype == torch.float16:
+        s = torch.ldexp(torch.ones((), dtype=torch.float64), scales.long() - 127)
+        return codes.double() * s.repeat_interleave(BLOCK, -1)[..., :codes.shape[-1]]
     c = codes.long()
     mag, sign = c & 0x7F, 1.0 - 2.0 * (c >> 7).double()
     k, f = mag >> 3, (mag & 7).double()
