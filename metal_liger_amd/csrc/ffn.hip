@@ -11,6 +11,7 @@
 //
 // bf16 runs on the bf16 matrix cores (gemm_core.h), fp32 on the fp32 ones.
 #include "ffn_product.h"
+#include "ffn_wgrad.h"
 
 namespace mla {
 namespace ffn {
@@ -42,7 +43,7 @@ int ktiles(int64_t k) { return (int)((k + gemm::kBK - 1) / gemm::kBK); }
 // The products of each type.
 //   raw:    fp32 sums [splits][M][N] of A B^T (B [N, K]) or A B (B [K, N], b_mn)
 //   store:  sum over segments of A_s B_s (B [K_s, N]), rounded to T
-//   wgrad:  A^T B (A [K, M], B [K, N]), rounded to T
+//   wgrads: A^T B (A [K, M], B [K, N]) of up to three products of one K, rounded to T
 template <typename T>
 struct Products;
 
@@ -120,15 +121,13 @@ struct Products<bf16> {
                              wsb ? static_cast<float*>(ws) : nullptr, wsb, st);
   }
 
-  static size_t wgrad_bytes(int64_t, int64_t, int64_t) { return 0; }
+  static size_t wgrads_bytes(int count, const Wgrad<bf16>* p, int64_t K) {
+    return plan_wgrads(count, p, K).floats * sizeof(float);
+  }
 
-  static int wgrad(int64_t M, int64_t N, int64_t K, const bf16* a, int64_t lda, const bf16* b,
-                   int64_t ldb, bf16* out, void*, size_t, hipStream_t st) {
-    const gemm::Segment s{{a, lda}, {b, ldb}, (int)K};
-    gemm::Problem pb;
-    const int rc = gemm::make_problem<gemm::BigCfg>(pb, (int)M, (int)N, 1, &s, kMNMajor, kMNMajor, 0);
-    if (rc) return rc;
-    return gemm::launch_store<bf16>(pb, kMNMajor, kMNMajor, out, N, 1.f, 0.f, st);
+  static int wgrads(int count, const Wgrad<bf16>* p, int64_t K, void* ws, size_t wsb,
+                    hipStream_t st) {
+    return launch_wgrads(count, p, K, ws, wsb, st);
   }
 
   static int check(const void* a, int64_t lda, int64_t cols, const char* what) {
@@ -185,11 +184,20 @@ struct Products<float> {
     return run(M, N, nseg, K, a, lda, b, ldb, kKMajor, kMNMajor, out, ws, wsb, st);
   }
 
-  static size_t wgrad_bytes(int64_t M, int64_t N, int64_t K) { return split_bytes(M, N, K); }
+  static size_t wgrads_bytes(int count, const Wgrad<float>* p, int64_t K) {
+    size_t n = 0;
+    for (int g = 0; g < count; ++g) n = larger(n, split_bytes(p[g].M, p[g].N, K));
+    return n;
+  }
 
-  static int wgrad(int64_t M, int64_t N, int64_t K, const float* a, int64_t lda, const float* b,
-                   int64_t ldb, float* out, void* ws, size_t wsb, hipStream_t st) {
-    return run(M, N, 1, &K, &a, &lda, &b, &ldb, kMNMajor, kMNMajor, out, ws, wsb, st);
+  static int wgrads(int count, const Wgrad<float>* p, int64_t K, void* ws, size_t wsb,
+                    hipStream_t st) {
+    for (int g = 0; g < count; ++g) {
+      const int rc = run(p[g].M, p[g].N, 1, &K, &p[g].a, &p[g].lda, &p[g].b, &p[g].ldb, kMNMajor,
+                         kMNMajor, p[g].c, ws, wsb, st);
+      if (rc) return rc;
+    }
+    return ML_OK;
   }
 
   static int check(const void*, int64_t, int64_t, const char*) { return ML_OK; }
@@ -286,8 +294,8 @@ int linear_grad(const T* dy, int64_t ldy, const Kept<KIND>& z, int act, T* dz, T
     linear_grad_kernel<1, T, KIND><<<grid, kThreads, 0, st>>>(dy, ldy, z, act, dz, partial, M, N, g.rows_per);
   ML_LAUNCH_CHECK();
   if (db) {
-    column_sum_kernel<T><<<dim3((unsigned)((N + kThreads - 1) / kThreads)), kThreads, 0, st>>>(
-        partial, (int)g.y, N, db);
+    column_sum_kernel<T><<<dim3((unsigned)((N + 31) / 32)), kThreads, 0, st>>>(partial, (int)g.y, N,
+                                                                               db);
     ML_LAUNCH_CHECK();
   }
   return ML_OK;
@@ -313,24 +321,20 @@ int linear_bwd(const LinearBwd& p, Arena& ws, bool run, hipStream_t st) {
     });
     if (rc) return rc;
   }
-  const size_t wsb = larger(Products<T>::store_bytes(p.M, p.K, p.N),
-                            Products<T>::wgrad_bytes(p.N, p.K, p.M));
-  char* pws = ws.take<char>(wsb);
-  if (!run) return ML_OK;
   const T* g = dz ? dz : dy;
   const int64_t ldg = dz ? p.N : p.ldy;
+  const Wgrad<T> wgrad{p.N, p.K, g, static_cast<const T*>(p.x), ldg, p.ldx, static_cast<T*>(p.dw)};
+  const size_t wsb = larger(Products<T>::store_bytes(p.M, p.K, p.N),
+                            Products<T>::wgrads_bytes(1, &wgrad, p.M));
+  char* pws = ws.take<char>(wsb);
+  if (!run) return ML_OK;
   const T* w = static_cast<const T*>(p.w);
   if (p.dx) {
     const int rc = Products<T>::store(p.M, p.K, 1, &p.N, &g, &ldg, &w, &p.ldw, static_cast<T*>(p.dx),
                                       pws, wsb, st);
     if (rc) return rc;
   }
-  if (p.dw) {
-    const int rc = Products<T>::wgrad(p.N, p.K, p.M, g, ldg, static_cast<const T*>(p.x), p.ldx,
-                                      static_cast<T*>(p.dw), pws, wsb, st);
-    if (rc) return rc;
-  }
-  return ML_OK;
+  return p.dw ? Products<T>::wgrads(1, &wgrad, p.M, pws, wsb, st) : (int)ML_OK;
 }
 
 // -------------------------------------------------------------- gated block --
@@ -399,12 +403,27 @@ int mlp_bwd(const MlpBwd& p, Arena& ws, bool run, hipStream_t st) {
   T* h = ws.take<T>(mi);
   const bool fuse = Products<T>::fused(p.M, p.I, p.O);
   float* sums = ws.take<float>(fuse ? 0 : Products<T>::raw_floats(p.M, p.I, p.O));
-  size_t wsb = larger(Products<T>::store_bytes(p.M, p.H, 2 * p.I), Products<T>::wgrad_bytes(p.I, p.H, p.M));
-  wsb = larger(wsb, Products<T>::wgrad_bytes(p.O, p.I, p.M));
-  char* pws = ws.take<char>(wsb);
-  if (!run) return ML_OK;
   const T* x = static_cast<const T*>(p.x);
   const T* dy = static_cast<const T*>(p.dy);
+  // the weights' gradients that are wanted (counted for any of them: all three)
+  Wgrad<T> wgrad[3];
+  int wanted = 0;
+  if (p.dwg || !run) wgrad[wanted++] = {p.I, p.H, dg, x, p.I, p.ldx, static_cast<T*>(p.dwg)};
+  if (p.dwu || !run) wgrad[wanted++] = {p.I, p.H, du, x, p.I, p.ldx, static_cast<T*>(p.dwu)};
+  if (p.dwd || !run) wgrad[wanted++] = {p.O, p.I, dy, h, p.ldy, p.I, static_cast<T*>(p.dwd)};
+  size_t wsb = Products<T>::store_bytes(p.M, p.H, 2 * p.I);
+  if (run) {
+    wsb = larger(wsb, Products<T>::wgrads_bytes(wanted, wgrad, p.M));
+  } else {
+    // (fewer products may split more)
+    for (int first = 0; first < 3; ++first)
+      for (int n = 1; first + n <= 3; ++n)
+        wsb = larger(wsb, Products<T>::wgrads_bytes(n, wgrad + first, p.M));
+    const Wgrad<T> outer[2] = {wgrad[0], wgrad[2]};
+    wsb = larger(wsb, Products<T>::wgrads_bytes(2, outer, p.M));
+  }
+  char* pws = ws.take<char>(wsb);
+  if (!run) return ML_OK;
   const T* wd = static_cast<const T*>(p.wd);
   const GatedGradStep<T, KIND> step{dg, du, p.dwd ? h : nullptr, p.I,
                                     make_kept<KIND>(p.gate, p.gscale, p.I),
@@ -426,17 +445,7 @@ int mlp_bwd(const MlpBwd& p, Arena& ws, bool run, hipStream_t st) {
     rc = Products<T>::store(p.M, p.H, 2, ks, a, la, b, lb, static_cast<T*>(p.dx), pws, wsb, st);
     if (rc) return rc;
   }
-  auto wgrad = [&](int64_t rows, int64_t cols, const T* a, int64_t lda, const T* b, int64_t ldb,
-                   void* out) {
-    return out ? Products<T>::wgrad(rows, cols, p.M, a, lda, b, ldb, static_cast<T*>(out), pws, wsb,
-                                    st)
-               : (int)ML_OK;
-  };
-  rc = wgrad(p.I, p.H, dg, p.I, x, p.ldx, p.dwg);
-  if (rc) return rc;
-  rc = wgrad(p.I, p.H, du, p.I, x, p.ldx, p.dwu);
-  if (rc) return rc;
-  return wgrad(p.O, p.I, dy, p.ldy, h, p.I, p.dwd);
+  return wanted ? Products<T>::wgrads(wanted, wgrad, p.M, pws, wsb, st) : (int)ML_OK;
 }
 
 }  // namespace

@@ -33,13 +33,14 @@ struct Kept {
     if constexpr (KIND == kKeepF32) {
       if (live) store_n<float, VEC>(v + at, x);
     } else if constexpr (KIND != kKeepNone) {
-      const uint32_t b = held::block_byte<KIND == kKeepFp16 ? held::kTop16 : held::kTop8, VEC>(x);
+      const held::Scale s =
+          held::block_scale<KIND == kKeepFp16 ? held::kTop16 : held::kTop8, VEC>(x);
       if (!live) return;
-      if (n % held::kBlock == 0) scale[m * nblocks + n / held::kBlock] = (uint8_t)b;
+      if (n % held::kBlock == 0) scale[m * nblocks + n / held::kBlock] = (uint8_t)s.byte;
       if constexpr (KIND == kKeepFp16)
-        held::store16<VEC>(v + at, b, x);
+        held::store16<VEC>(v + at, s, x);
       else
-        held::store<VEC>(v + at, b, x);
+        held::store<VEC>(v + at, s, x);
     }
   }
 
@@ -405,14 +406,25 @@ __global__ __launch_bounds__(kThreads) void linear_grad_kernel(
   }
 }
 
+// A workgroup sums 32 columns: 8 lanes a column take every eighth partial row each, and
+// are joined in order. (One thread a column, 205 rows of 1152 columns: 48 us.)
 template <typename T>
 __global__ __launch_bounds__(kThreads) void column_sum_kernel(const float* __restrict__ partial,
                                                               int parts, int64_t cols,
                                                               T* __restrict__ out) {
-  const int64_t c = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (c >= cols) return;
+  const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + cl;
   float s = 0.f;
-  for (int p = 0; p < parts; ++p) s += partial[(int64_t)p * cols + c];
+  if (c < cols) {
+#pragma unroll 8
+    for (int p = rl; p < parts; p += 8) s += partial[(int64_t)p * cols + c];
+  }
+  __shared__ float lds[8][32];
+  lds[rl][cl] = s;
+  __syncthreads();
+  if (rl || c >= cols) return;
+#pragma unroll
+  for (int r = 1; r < 8; ++r) s += lds[r][cl];
   out[c] = from_f32<T>(s);
 }
 

@@ -852,11 +852,12 @@ __device__ __forceinline__ void big_barrier() {
 // Main loop of the big tile; lds holds STAGES stages of STAGE_BYTES (A tile,
 // then B tile). Wave w = 4 g + s computes rows 128 g .. 128 g + 127 and
 // columns 64 s .. 64 s + 63 of the block tile.
-// KLIVE: K (one segment, not split) ends at klive instead.
+// KLIVE: K (one segment, not split) ends at klive instead. ksplit, kps: a work
+// item's own split of K, the problem's where ksplit is 0.
 template <int LA, int LB, bool KLIVE = false>
 __device__ __forceinline__ void big_mainloop(const Problem& pb, int tm, int tn, int split,
                                              char* lds, f32x4_t (&acc)[big::TM][big::TN],
-                                             int klive = 0) {
+                                             int klive = 0, int ksplit = 0, int kps = 0) {
   const int tid = threadIdx.x;
   const int lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -873,10 +874,11 @@ __device__ __forceinline__ void big_mainloop(const Problem& pb, int tm, int tn, 
   int nk, k0 = 0;
   if (KLIVE) {
     nk = (klive + big::BK - 1) / big::BK;
-  } else if (pb.ksplit > 1) {  // splits are counted in 64-wide k units
+  } else if ((ksplit ? ksplit : pb.ksplit) > 1) {  // splits are counted in 64-wide k units
+    const int per = ksplit ? kps : pb.kps;
     const int total = (pb.seg[0].k_len + kBK - 1) / kBK;
-    const int first = split * pb.kps;
-    const int n64 = total - first < pb.kps ? total - first : pb.kps;
+    const int first = split * per;
+    const int n64 = total - first < per ? total - first : per;
     k0 = first * kBK;
     const int kend = k0 + n64 * kBK < pb.seg[0].k_len ? k0 + n64 * kBK : pb.seg[0].k_len;
     nk = (kend - k0 + big::BK - 1) / big::BK;

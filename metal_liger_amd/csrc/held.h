@@ -58,21 +58,36 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t m) {
   return m;
 }
 
-// The scale's byte of a block that 32 / VEC neighbouring lanes hold VEC elements of.
+// A block's scale, as the 32 / VEC neighbouring lanes that hold VEC elements of it each
+// find it, and whether all of a lane's own elements are finite (they nearly always are:
+// the search for the largest finite one is then 1.5 operations an element).
+struct Scale {
+  uint32_t byte;
+  bool finite;
+};
+
 template <int TOP, int VEC>
-__device__ __forceinline__ uint32_t block_byte(const float (&v)[VEC]) {
+__device__ __forceinline__ Scale block_scale(const float (&v)[VEC]) {
   uint32_t m = 0;
 #pragma unroll
   for (int k = 0; k < VEC; ++k) {
-    const uint32_t b = finite_bits(v[k]);
+    const uint32_t b = __builtin_bit_cast(uint32_t, v[k]) & 0x7FFFFFFFu;
     m = m > b ? m : b;
   }
-  return scale_byte<TOP>(lanes_max<kBlock / VEC>(m));
+  const bool finite = m < 0x7F800000u;
+  if (!finite) {
+    m = 0;
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      const uint32_t b = finite_bits(v[k]);
+      m = m > b ? m : b;
+    }
+  }
+  return {scale_byte<TOP>(lanes_max<kBlock / VEC>(m)), finite};
 }
 
-__device__ __forceinline__ float to_scaled(float v, float inv) {
-  return finite_bits(v) == (__builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu) ? v * inv
-                                                                           : __builtin_nanf("");
+__device__ __forceinline__ float finite_or_nan(float v) {
+  return finite_bits(v) == (__builtin_bit_cast(uint32_t, v) & 0x7FFFFFFFu) ? v : __builtin_nanf("");
 }
 
 // Two elements as bytes 0 and 1 of the result.
@@ -82,19 +97,23 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 
 // VEC elements to q (VEC bytes, aligned to VEC), by the block's scale.
 template <int VEC>
-__device__ __forceinline__ void store(uint8_t* q, uint32_t byte, const float (&v)[VEC]) {
-  const float inv = inverse_of(byte);
+__device__ __forceinline__ void store(uint8_t* q, const Scale& s, const float (&v)[VEC]) {
+  const float inv = inverse_of(s.byte);
+  float x[VEC];
+#pragma unroll
+  for (int k = 0; k < VEC; ++k) x[k] = v[k] * inv;
+  if (!s.finite) {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) x[k] = finite_or_nan(v[k]) * inv;
+  }
   if constexpr (VEC == 1) {
-    *q = (uint8_t)pack2(to_scaled(v[0], inv), 0.f);
+    *q = (uint8_t)pack2(x[0], 0.f);
   } else {
     uint32_t w[VEC / 4];
 #pragma unroll
     for (int k = 0; k < VEC / 4; ++k) {
-      int p = __builtin_amdgcn_cvt_pk_fp8_f32(to_scaled(v[4 * k], inv),
-                                              to_scaled(v[4 * k + 1], inv), 0, false);
-      p = __builtin_amdgcn_cvt_pk_fp8_f32(to_scaled(v[4 * k + 2], inv),
-                                          to_scaled(v[4 * k + 3], inv), p, true);
-      w[k] = (uint32_t)p;
+      const int p = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * k], x[4 * k + 1], 0, false);
+      w[k] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[4 * k + 2], x[4 * k + 3], p, true);
     }
     __builtin_memcpy(__builtin_assume_aligned(q, VEC), w, VEC);
   }
@@ -123,8 +142,8 @@ __device__ __forceinline__ void load(const uint32_t* w, uint32_t byte, float (&v
 
 // The same in 16 bits (q aligned to 2 VEC bytes).
 template <int VEC>
-__device__ __forceinline__ void store16(f16* q, uint32_t byte, const float (&v)[VEC]) {
-  const float inv = inverse_of(byte);
+__device__ __forceinline__ void store16(f16* q, const Scale& s, const float (&v)[VEC]) {
+  const float inv = inverse_of(s.byte);
   float w[VEC];
 #pragma unroll
   for (int k = 0; k < VEC; ++k) w[k] = v[k] * inv;

@@ -305,3 +305,37 @@ def test_mlp_tiles(dev, size, checkpoint):
     x, ws, r, dy = _mlp_case(*size, torch.bfloat16, True, dev)
     _mlp_check(x, ws, r, dy, checkpoint,
                lambda: fused_swiglu_mlp(x, *ws, residual=r, checkpoint=checkpoint))
+
+
+@pytest.mark.parametrize("tokens,hidden,inter,out", [(1100, 264, 520, 264), (4097, 72, 264, 136),
+                                                     (1600, 1032, 4104, 520)])
+@pytest.mark.parametrize("frozen", ["", "gate", "up", "down", "gate up", "gate down", "up down"])
+def test_weight_gradients_together(dev, tokens, hidden, inter, out, frozen):
+    """Weights' gradients of one launch, tiles of a partial round split over the tokens,
+    whichever of them are wanted: the same as each alone, up to the sums' order."""
+    from metal_liger_amd import hip_ops
+    x, ws, _, dy = _mlp_case(tokens, hidden, inter, out, torch.bfloat16, False, dev)
+    x, ws = x.detach(), [w.detach() for w in ws]
+    y, *kept = hip_ops.swiglu_mlp_fwd(x, *ws, None, hip_ops.KEEP_FP16)
+    need = [name not in frozen.split() for name in ("gate", "up", "down")]
+    got = hip_ops.swiglu_mlp_bwd(x, *ws, dy, hip_ops.KEEP_FP16, *kept, False, *need)
+    g = ref.held_values(kept[0].cpu(), kept[1].cpu())
+    u = ref.held_values(kept[2].cpu(), kept[3].cpu())
+    dh = _cpu(dy) @ _cpu(ws[2])
+    X, D, U = _cpu(x), _cpu(dy), _u(torch.bfloat16)
+    noise = _act_noise(g) + (out + 6) * V
+    dg, du = dh * u * ref.act_grad(g, "silu"), dh * ref.act(g, "silu")
+    h = ref.act(g, "silu") * u
+    big = D.abs() @ _cpu(ws[2]).abs()  # dh's error: (out + 2) V of this
+    want = [(dg, U * dg.abs() + 1.2 * noise * big * u.abs(), X),
+            (du, U * du.abs() + noise * big * (g.abs() + 1), X), None]
+    for i in range(2):
+        if need[i]:
+            a, ea, b = want[i]
+            _check(got[1 + i], *_mm(a.t(), ea.t(), b, torch.zeros_like(b), tokens), f"weight {i}")
+        else:
+            assert got[1 + i].numel() == 0
+    if need[2]:
+        eh = U * h.abs() + noise * u.abs()
+        _check(got[3], *_mm(D.t(), torch.zeros_like(D.t()), h, eh, tokens), "down")
+    assert got[0].numel() == 0
