@@ -9,8 +9,12 @@
 //           dh = dy Wd, dg = dh u silu'(g), du = dh silu(g),
 //           dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
 //
-// bf16 runs on the bf16 matrix cores (gemm_core.h), fp32 on the fp32 ones.
+// bf16 runs on the bf16 matrix cores (gemm_core.h), fp32 on the fp32 ones; forwards of
+// up to 64 rows on kernels of their own (ffn_skinny.h), which take fp16 as well.
+#include <initializer_list>
+
 #include "ffn_product.h"
+#include "ffn_skinny.h"
 #include "ffn_wgrad.h"
 
 namespace mla {
@@ -37,6 +41,28 @@ struct Arena {
 size_t larger(size_t a, size_t b) { return a > b ? a : b; }
 
 bool aligned_rows(const void* p, int64_t ld) { return !p || (aligned16(p) && ld % 8 == 0); }
+
+struct Checked {
+  const void* p;
+  int64_t ld, cols;
+  const char* what;
+};
+
+// 16-bit operands of a product and its step.
+int check_operands(std::initializer_list<Checked> list) {
+  for (const Checked& c : list)
+    ML_CHECK(aligned16(c.p) && c.ld % 8 == 0 && c.cols % 8 == 0,
+             "ffn: 16-bit %s needs a 16-byte aligned base, and columns and row stride in multiples "
+             "of 8 (%lld, %lld)", c.what, (long long)c.cols, (long long)c.ld);
+  return ML_OK;
+}
+
+int check_half(int64_t M, int keep) {
+  ML_CHECK(M <= kSkinnyRows && keep == kKeepNone,
+           "ffn: fp16 runs for up to %d rows with nothing kept (got %lld, keep %d)", kSkinnyRows,
+           (long long)M, keep);
+  return ML_OK;
+}
 
 int ktiles(int64_t k) { return (int)((k + gemm::kBK - 1) / gemm::kBK); }
 
@@ -83,6 +109,9 @@ struct Products<bf16> {
     return p.tile == 128 ? raw_cfg<gemm::R4SCfg>(M, N, s, b_mn, p.ksplit, out, splits, st)
                          : raw_cfg<gemm::R4Cfg>(M, N, s, b_mn, p.ksplit, out, splits, st);
   }
+
+  // Whether a product of M rows needs no workspace: it runs as one of few rows.
+  static bool few(int64_t M) { return M <= kSkinnyRows; }
 
   // Whether the product runs its step as its epilogue: where K is not split.
   static bool fused(int64_t M, int64_t N, int64_t K) { return plan(M, N, K).ksplit == 1; }
@@ -131,10 +160,7 @@ struct Products<bf16> {
   }
 
   static int check(const void* a, int64_t lda, int64_t cols, const char* what) {
-    ML_CHECK(aligned16(a) && lda % 8 == 0 && cols % 8 == 0,
-             "ffn: bf16 %s needs a 16-byte aligned base, and columns and row stride in multiples "
-             "of 8 (%lld, %lld)", what, (long long)cols, (long long)lda);
-    return ML_OK;
+    return check_operands({{a, lda, cols, what}});
   }
 };
 
@@ -168,6 +194,7 @@ struct Products<float> {
                wsb ? out + (size_t)M * N : nullptr, wsb, st);
   }
 
+  static bool few(int64_t) { return false; }  // (widths and bases may rule it out)
   static bool fused(int64_t, int64_t, int64_t) { return false; }
 
   template <int LB, class... Args>
@@ -217,6 +244,15 @@ int dispatch_keep(int keep, F&& f) {
   return ML_ERR_INVALID;
 }
 
+// Whether a forward's product runs as one of few rows: any of 16-bit elements (whose
+// operands qualify as they are checked), those of fp32 whose widths and bases do.
+template <typename T>
+bool few_rows(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* w,
+              int64_t ldw) {
+  return M <= kSkinnyRows && N % 8 == 0 && K % 8 == 0 && aligned16(x) && aligned16(w) &&
+         ldx % 4 == 0 && ldw % 4 == 0;
+}
+
 template <typename F>
 int dispatch(int dtype, F&& f) {
   if (dtype == ML_F32) return f(float{});
@@ -249,6 +285,12 @@ int linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
                int64_t M, int64_t N, int64_t K, Arena& ws, bool run, hipStream_t st) {
   const T* xt = static_cast<const T*>(x);
   const T* wt = static_cast<const T*>(w);
+  const bool vec = N % 8 == 0 && aligned_rows(step.bias, 0) && aligned_rows(step.residual, step.ldr) &&
+                   aligned_rows(step.y, step.ldy);
+  if (run && vec && few_rows<T>(M, N, K, x, ldx, w, ldw))
+    return launch_skinny<KIND == kKeepNone ? 1 : 2, false>(
+        SkinnyProduct<T, T>{xt, wt, nullptr, ldx, ldw, 0, (int)M, (int)N, (int)K}, step, st);
+  if (Products<T>::few(M) && !run) return ML_OK;
   if (Products<T>::fused(M, N, K))
     return run ? Products<T>::template through<kKMajor>(M, N, K, xt, ldx, wt, ldw, step, st)
                : (int)ML_OK;
@@ -257,8 +299,6 @@ int linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
   int splits = 1;
   const int rc = Products<T>::raw(M, N, K, xt, ldx, wt, ldw, false, sums, splits, st);
   if (rc) return rc;
-  const bool vec = N % 8 == 0 && aligned_rows(step.bias, 0) && aligned_rows(step.residual, step.ldr) &&
-                   aligned_rows(step.y, step.ldy);
   return launch_rows(vec, PartialSource{sums, splits, M * N, N}, NoSource{}, step, M, N, st);
 }
 
@@ -348,23 +388,43 @@ struct MlpFwd {
   int64_t M, H, I, O;
 };
 
+// The block of few rows: weights of T, h of TH (fp32 where T is fp16, whose range h may
+// leave).
+template <typename T, typename TH, int KIND>
+int few_mlp(const MlpFwd& p, const TH* h, const GatedStep<TH, KIND>& step,
+            const LinearStep<T, kKeepNone>& out, hipStream_t st) {
+  const T *wg = static_cast<const T*>(p.wg), *wu = static_cast<const T*>(p.wu);
+  const int rc = launch_skinny<KIND == kKeepNone ? 1 : 2, true>(
+      SkinnyProduct<T, T>{static_cast<const T*>(p.x), wg, wu, p.ldx, p.ldg, p.ldu, (int)p.M,
+                          (int)p.I, (int)p.H}, step, st);
+  if (rc) return rc;
+  return launch_skinny<1, false>(
+      SkinnyProduct<TH, T>{h, static_cast<const T*>(p.wd), nullptr, p.I, p.ldd, 0, (int)p.M,
+                           (int)p.O, (int)p.I}, out, st);
+}
+
 template <typename T, int KIND>
 int mlp_fwd(const MlpFwd& p, Arena& ws, bool run, hipStream_t st) {
   using P = Products<T>;
   T* h = ws.take<T>((size_t)(p.M * p.I));
-  const LinearStep<T, kKeepNone> out{nullptr, static_cast<const T*>(p.residual),
-                                     static_cast<T*>(p.y), p.ldr, p.O, kActNone, {}};
-  const bool fuse_in = P::fused(p.M, 2 * p.I, p.H), fuse_out = P::fused(p.M, p.O, p.I);
-  const size_t n_in = fuse_in ? 0 : P::raw_floats(p.M, p.I, p.H);
-  const size_t n_out = fuse_out ? 0 : P::raw_floats(p.M, p.O, p.I);
-  float* sums = ws.take<float>(larger(2 * n_in, n_out));
-  if (!run) return ML_OK;
   const T* x = static_cast<const T*>(p.x);
   const T* wg = static_cast<const T*>(p.wg);
   const T* wu = static_cast<const T*>(p.wu);
   const T* wd = static_cast<const T*>(p.wd);
   const GatedStep<T, KIND> step{h, p.I, make_kept<KIND>(p.gate, p.gscale, p.I),
                                 make_kept<KIND>(p.up, p.uscale, p.I)};
+  const LinearStep<T, kKeepNone> out{nullptr, static_cast<const T*>(p.residual),
+                                     static_cast<T*>(p.y), p.ldr, p.O, kActNone, {}};
+  const bool vec = p.O % 8 == 0 && aligned_rows(p.residual, p.ldr) && aligned_rows(p.y, p.O);
+  if (run && vec && few_rows<T>(p.M, p.I, p.H, x, p.ldx, wg, p.ldg) && aligned16(wu) &&
+      p.ldu % 4 == 0 && few_rows<T>(p.M, p.O, p.I, h, p.I, wd, p.ldd))
+    return few_mlp<T, T>(p, h, step, out, st);
+  if (P::few(p.M) && !run) return ML_OK;
+  const bool fuse_in = P::fused(p.M, 2 * p.I, p.H), fuse_out = P::fused(p.M, p.O, p.I);
+  const size_t n_in = fuse_in ? 0 : P::raw_floats(p.M, p.I, p.H);
+  const size_t n_out = fuse_out ? 0 : P::raw_floats(p.M, p.O, p.I);
+  float* sums = ws.take<float>(larger(2 * n_in, n_out));
+  if (!run) return ML_OK;
   int splits = 1, rc;
   if (fuse_in) {
     rc = P::through_pair(p.M, p.I, p.H, x, p.ldx, wg, p.ldg, wu, p.ldu, step, st);
@@ -381,7 +441,6 @@ int mlp_fwd(const MlpFwd& p, Arena& ws, bool run, hipStream_t st) {
   if (fuse_out) return P::template through<kKMajor>(p.M, p.O, p.I, h, p.I, wd, p.ldd, out, st);
   rc = P::raw(p.M, p.O, p.I, h, p.I, wd, p.ldd, false, sums, splits, st);
   if (rc) return rc;
-  const bool vec = p.O % 8 == 0 && aligned_rows(p.residual, p.ldr) && aligned_rows(p.y, p.O);
   return launch_rows(vec, PartialSource{sums, splits, p.M * p.O, p.O}, NoSource{}, out, p.M,
                      p.O, st);
 }
@@ -461,7 +520,7 @@ using namespace mla;
   } while (0)
 
 extern "C" size_t ml_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
-  if (ffn::check_sizes(M, N, K)) return 0;
+  if (ffn::check_sizes(M, N, K) || dtype == ML_F16) return 0;
   ffn::Arena ws{nullptr};
   ffn::dispatch(dtype, [&](auto t) {
     using T = decltype(t);
@@ -481,6 +540,18 @@ extern "C" int ml_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t 
   ML_CHECK(act >= kActNone && act <= kActGeluTanh, "linear: bad activation %d", act);
   ML_CHECK(ldx >= K && ldw >= K && ldy >= N && (!residual || ldr >= N), "linear: bad row strides");
   ML_TRY(ffn::check_kept(keep, z, zscale, "z"));
+  if (dtype == ML_F16) {
+    ML_TRY(ffn::check_half(M, keep));
+    ML_TRY(ffn::check_operands({{x, ldx, K, "x"}, {w, ldw, K, "weight"}, {y, ldy, N, "y"},
+                                {bias, 0, N, "bias"}, {residual, residual ? ldr : 0, N, "residual"}}));
+    const ffn::LinearStep<f16, ffn::kKeepNone> step{
+        static_cast<const f16*>(bias), static_cast<const f16*>(residual), static_cast<f16*>(y), ldr,
+        ldy, act, {}};
+    return ffn::launch_skinny<1, false>(
+        ffn::SkinnyProduct<f16, f16>{static_cast<const f16*>(x), static_cast<const f16*>(w), nullptr,
+                                     ldx, ldw, 0, (int)M, (int)N, (int)K},
+        step, (hipStream_t)stream);
+  }
   return ffn::dispatch(dtype, [&](auto t) -> int {
     using T = decltype(t);
     ML_TRY(ffn::Products<T>::check(x, ldx, K, "x"));
@@ -560,6 +631,7 @@ int check_mlp(int64_t M, int64_t H, int64_t I, int64_t O) {
 extern "C" size_t ml_swiglu_mlp_fwd_workspace_bytes(int64_t M, int64_t H, int64_t I, int64_t O,
                                                     int dtype) {
   if (ffn::check_mlp(M, H, I, O)) return 0;
+  if (dtype == ML_F16) return (size_t)(M * I) * sizeof(float);  // h
   ffn::MlpFwd p{};
   p.M = M;
   p.H = H;
@@ -582,6 +654,22 @@ extern "C" int ml_swiglu_mlp_fwd(const void* x, int64_t ldx, const void* wg, int
            "swiglu mlp: bad row strides");
   ML_TRY(ffn::check_kept(keep, gate, gate_scale, "gate"));
   ML_TRY(ffn::check_kept(keep, up, up_scale, "up"));
+  if (dtype == ML_F16) {
+    ML_TRY(ffn::check_half(M, keep));
+    ML_TRY(ffn::check_operands({{x, ldx, H, "x"}, {wg, ldg, H, "gate weight"},
+                                {wu, ldu, H, "up weight"}, {wd, ldd, I, "down weight"},
+                                {y, O, O, "y"}, {residual, residual ? ldr : 0, O, "residual"}}));
+    const size_t need = ml_swiglu_mlp_fwd_workspace_bytes(M, H, I, O, dtype);
+    ML_CHECK(workspace_bytes >= need && workspace && aligned16(workspace),
+             "swiglu mlp: workspace of %zu bytes, %zu needed", workspace_bytes, need);
+    const ffn::MlpFwd p{x, wg, wu, wd, residual, ldx, ldg, ldu, ldd, ldr, y, keep,
+                        gate, gate_scale, up, up_scale, M, H, I, O};
+    float* h = static_cast<float*>(workspace);
+    const ffn::LinearStep<f16, ffn::kKeepNone> out{nullptr, static_cast<const f16*>(residual),
+                                                   static_cast<f16*>(y), ldr, O, kActNone, {}};
+    return ffn::few_mlp<f16, float>(p, h, ffn::GatedStep<float, ffn::kKeepNone>{h, I, {}, {}}, out,
+                                    (hipStream_t)stream);
+  }
   return ffn::dispatch(dtype, [&](auto t) -> int {
     using T = decltype(t);
     ML_TRY(ffn::Products<T>::check(x, ldx, H, "x"));

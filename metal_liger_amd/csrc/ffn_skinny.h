@@ -1,0 +1,204 @@
+// Products of few rows (single tokens, short prompts) through the steps of ffn_rows.h:
+//   C [M, N] = x [M, K] W [N, K]^T, M up to 64, W read once.
+//
+// Bound by W's bytes and by latency: [1, 2048] x 6144 in bf16 are 25 MB, 5 us at the
+// rate of a large copy. A workgroup takes 16 NT rows of W and all of K, its 8 waves every
+// eighth 64-wide k-chunk each, so that some 8 MB are in flight over the GPU; their sums
+// are joined in LDS in wave order (nothing is left to a second launch, and no atomics).
+// Per chunk a lane loads 16 neighbouring elements of one row of W (four lanes a row:
+// whole 128-byte lines of 16-bit elements) and of x, straight into the operands of
+// 16 x 16 MFMAs: which k an operand slot holds does not matter as long as both operands
+// agree, so the lane's 16 elements feed the chunk's steps in order.
+//   bf16 and fp16 by bf16 or fp16: v_mfma_f32_16x16x32 (exact products, fp32 sums)
+//   fp32 by fp32 or fp16: v_mfma_f32_16x16x4_f32, W upcast in registers
+// With PAIR a second W of the same shape beside it (gate and up).
+#pragma once
+
+#include "ffn_rows.h"
+
+namespace mla {
+namespace ffn {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kSkinnyWaves = 8;
+constexpr int kSkinnyRows = 64;  // most rows of x
+constexpr int kChunk = 64;       // k a chunk
+
+// A lane's 16 elements of a chunk (of one row, from k = 16 (lane / 16)): two halves of 8.
+template <typename T>
+struct Strip {
+  Pack<T, 8> h[2];
+
+  // k0: of the lane; whole: both halves are within K
+  __device__ __forceinline__ void load(const T* row, int k0, int K, bool whole) {
+    if (whole) {
+      load_pack<T, 8>(row + k0, h[0]);
+      load_pack<T, 8>(row + k0 + 8, h[1]);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const bool in = k0 + 8 * i < K;
+      load_pack<T, 8>(row + (in ? k0 + 8 * i : 0), h[i]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[i].v[e] = in ? h[i].v[e] : (T)0.f;
+    }
+  }
+};
+
+template <typename TX, typename TW>
+__device__ __forceinline__ void strip_mma(f32x4& acc, const Strip<TW>& w, const Strip<TX>& x) {
+  typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+  typedef f16 f16x8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (std::is_same_v<TX, bf16>) {
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, w.h[i]),
+                                                    __builtin_bit_cast(bf16x8, x.h[i]), acc, 0, 0, 0);
+    } else if constexpr (std::is_same_v<TX, f16>) {
+      acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, w.h[i]),
+                                                   __builtin_bit_cast(f16x8, x.h[i]), acc, 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(to_f32(w.h[i].v[e]), x.h[i].v[e], acc, 0, 0, 0);
+    }
+  }
+}
+
+template <typename TX, typename TW>
+struct SkinnyProduct {
+  const TX* x;
+  const TW *w, *w2;  // w2: PAIR
+  int64_t ldx, ldw, ldw2;
+  int M, N, K;
+};
+
+// MT: tiles of 16 rows of x; NT: of W (2 where the step keeps a tensor: a block of 32
+// columns).
+template <typename TX, typename TW, int MT, int NT, bool PAIR, class Step>
+__global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(
+    const SkinnyProduct<TX, TW> p, const Step step) {
+  constexpr int kOps = PAIR ? 2 : 1;
+  constexpr int kTiles = kOps * NT * MT;
+  constexpr int kPitch = 16 * NT + 4;
+  __shared__ __attribute__((aligned(16))) float red[kSkinnyWaves][kTiles][64][4];
+  __shared__ __attribute__((aligned(16))) float fin[kOps][16 * MT][kPitch];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int r = lane & 15, G = lane >> 4;
+  const int n0 = blockIdx.x * 16 * NT;
+  // rows past the ends read the last one (their results are not used)
+  const TW* wr[kOps][NT];
+  const TX* xr[MT];
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int n = n0 + 16 * j + r < p.N ? n0 + 16 * j + r : p.N - 1;
+    wr[0][j] = p.w + n * p.ldw;
+    if constexpr (PAIR) wr[1][j] = p.w2 + n * p.ldw2;
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const int m = 16 * i + r < p.M ? 16 * i + r : p.M - 1;
+    xr[i] = p.x + m * p.ldx;
+  }
+  f32x4 acc[kOps][NT][MT];
+#pragma unroll
+  for (int o = 0; o < kOps; ++o)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[o][j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  // chunks c, c + 8, .. of a batch: every load before the first product (as many chunks
+  // as about 128 registers hold)
+  constexpr int kRegs = 4 * (kOps * NT * (int)sizeof(TW) + MT * (int)sizeof(TX));
+  constexpr int kBatch = kRegs <= 16 ? 8 : kRegs <= 32 ? 4 : kRegs <= 64 ? 2 : 1;
+  const int chunks = (p.K + kChunk - 1) / kChunk;
+  for (int c0 = wave; c0 < chunks; c0 += kSkinnyWaves * kBatch) {
+    Strip<TW> ws[kBatch][kOps][NT];
+    Strip<TX> xs[kBatch][MT];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int c = c0 + u * kSkinnyWaves;  // (wave-uniform, as the branches on it are)
+      if (c >= chunks) break;
+      const int k0 = c * kChunk + 16 * G;
+      const bool whole = (c + 1) * kChunk <= p.K;
+#pragma unroll
+      for (int o = 0; o < kOps; ++o)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) ws[u][o][j].load(wr[o][j], k0, p.K, whole);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) xs[u][i].load(xr[i], k0, p.K, whole);
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (c0 + u * kSkinnyWaves >= chunks) break;
+#pragma unroll
+      for (int o = 0; o < kOps; ++o)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int i = 0; i < MT; ++i) strip_mma<TX, TW>(acc[o][j][i], ws[u][o][j], xs[u][i]);
+    }
+  }
+
+#pragma unroll
+  for (int o = 0; o < kOps; ++o)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+        *reinterpret_cast<f32x4*>(red[wave][(o * NT + j) * MT + i][lane]) = acc[o][j][i];
+  __syncthreads();
+  // element v of a lane of tile (o, j, i): row 16 i + lane % 16 of x, row 16 j + 4 (lane /
+  // 16) + v of W
+  for (int q = threadIdx.x; q < kTiles * 64; q += 64 * kSkinnyWaves) {
+    const int t = q >> 6, l = q & 63;
+    f32x4 s = *reinterpret_cast<const f32x4*>(red[0][t][l]);
+#pragma unroll
+    for (int w = 1; w < kSkinnyWaves; ++w) s += *reinterpret_cast<const f32x4*>(red[w][t][l]);
+    const int i = t % MT, j = t / MT % NT, o = t / MT / NT;
+    *reinterpret_cast<f32x4*>(&fin[o][16 * i + (l & 15)][16 * j + 4 * (l >> 4)]) = s;
+  }
+  __syncthreads();
+  // 2 NT neighbouring lanes a row (whole waves: 16 MT rows of 2 or 4 lanes)
+  constexpr int kPositions = 16 * MT * 2 * NT;
+  for (int q = threadIdx.x; q < (kPositions + 63) / 64 * 64; q += 64 * kSkinnyWaves) {
+    const int m = q / (2 * NT), c = 8 * (q % (2 * NT)), n = n0 + c;
+    const bool live = m < p.M && n < p.N && q < kPositions;
+    const int row = q < kPositions ? m : 0;
+    typename Step::template Column<8> column;
+    typename Step::template Fetched<8> f;
+    if (live) {
+      column = step.template column<8>(n);
+      f = step.template fetch<8>(m, n);
+    }
+    float x[8];
+    load_n<float, 8>(&fin[0][row][c], x);
+    if constexpr (PAIR) {
+      float u[8];
+      load_n<float, 8>(&fin[1][row][c], u);
+      step.template finish<8>(m, n, x, u, column, f, live);
+    } else {
+      step.template finish<8>(m, n, x, column, f, live);
+    }
+  }
+}
+
+template <int NT, bool PAIR, typename TX, typename TW, class Step>
+inline int launch_skinny(const SkinnyProduct<TX, TW>& p, const Step& step, hipStream_t st) {
+  const dim3 grid((p.N + 16 * NT - 1) / (16 * NT)), block(64 * kSkinnyWaves);
+  if (p.M <= 16)
+    skinny_kernel<TX, TW, 1, NT, PAIR, Step><<<grid, block, 0, st>>>(p, step);
+  else if (p.M <= 32)
+    skinny_kernel<TX, TW, 2, NT, PAIR, Step><<<grid, block, 0, st>>>(p, step);
+  else
+    skinny_kernel<TX, TW, 4, NT, PAIR, Step><<<grid, block, 0, st>>>(p, step);
+  ML_LAUNCH_CHECK();
+  return ML_OK;
+}
+
+}  // namespace ffn
+}  // namespace mla

@@ -217,13 +217,25 @@ def _kept_buffers(x: torch.Tensor, cols: int, keep: int):
             for shape, dtype in kept_layout(x.shape[0], cols, keep)]
 
 
+FEW_ROWS = 64  # rows up to which a forward's products take fp16 (with nothing kept)
+
+
 def _product_rows(t: torch.Tensor) -> torch.Tensor:
     """[rows, cols] as the products of t's dtype read it (a copy only when needed)."""
-    return _al16(_bf16_rows(t)) if t.dtype == torch.bfloat16 else rows_view(t)
+    if t.dtype == torch.float32:
+        return rows_view(t)
+    if t.stride(1) != 1 or t.stride(0) % 8 != 0 or t.stride(0) < t.shape[1]:
+        t = _dense(t)
+    return _al16(t)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(query: str, *args) -> int:
+    return _hip.query(query, *args)
 
 
 def _workspace(like: torch.Tensor, query: str, *args) -> tuple:
-    n = _hip.query(query, *args)
+    n = _workspace_bytes(query, *args)
     return (torch.empty(n, dtype=torch.uint8, device=like.device) if n else None), n
 
 
@@ -234,7 +246,8 @@ def _used(t: torch.Tensor | None):
 
 def linear_fwd(x2, w, bias, residual, act: int, keep: int):
     """(y, z, zscale) of ml_linear_fwd: x2 [M, K], w [N, K], bias [N] or None, residual
-    [M, N] or None, all bf16 (sizes in multiples of 8) or all fp32."""
+    [M, N] or None, all bf16 (sizes in multiples of 8), all fp32, or all fp16 (as bf16, up
+    to FEW_ROWS rows with nothing kept)."""
     ensure_rocm_device(x2, w, bias, residual)
     x2, w = _product_rows(x2), _product_rows(w)
     (M, K), N = x2.shape, w.shape[0]

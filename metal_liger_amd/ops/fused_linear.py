@@ -9,8 +9,9 @@ rounds finer than bf16; in fp32 where the products run in fp32), or in 8 (checkp
 "fp8": e4m3 with such scales), formed of the fp32 sums. What is not needed (x where the
 weight is frozen, W where x needs no gradient) is not kept. First derivatives only.
 
-bf16 with sizes in multiples of 8 runs on the bf16 matrix cores, everything else on the
-fp32 ones (fp16 and other bf16 sizes are upcast, and rounded once at the end).
+bf16 with sizes in multiples of 8 runs on the bf16 matrix cores, as fp16 does in forwards
+of up to 64 rows that keep nothing, everything else on the fp32 ones (fp16 and other bf16
+sizes are upcast, and rounded once at the end).
 """
 
 from __future__ import annotations
@@ -37,10 +38,15 @@ def keep_mode(checkpoint: str | None, dtype: torch.dtype) -> int:
     return hip_ops.KEEP_FP16 if dtype == torch.bfloat16 else hip_ops.KEEP_F32
 
 
-def compute_dtype(x: torch.Tensor, *features: int) -> torch.dtype:
-    """bf16 where its matrix-core kernels take the sizes, else fp32."""
-    bf16 = x.dtype == torch.bfloat16 and all(f % 8 == 0 for f in features)
-    return torch.bfloat16 if bf16 else torch.float32
+def compute_dtype(x: torch.Tensor, *features: int, infer: bool = False) -> torch.dtype:
+    """bf16 where its matrix-core kernels take the sizes, fp16 in forwards of few rows
+    with nothing to keep (infer), else fp32."""
+    if x.dtype != torch.float32 and all(f % 8 == 0 for f in features):
+        if x.dtype == torch.bfloat16:
+            return x.dtype
+        if infer and x.numel() <= hip_ops.FEW_ROWS * x.shape[-1]:
+            return x.dtype
+    return torch.float32
 
 
 def rows(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
@@ -74,7 +80,7 @@ def wants_grad(*tensors) -> bool:
 
 
 def _forward(x, weight, bias, residual, act: int, keep: int):
-    ct = compute_dtype(x, *weight.shape)
+    ct = compute_dtype(x, *weight.shape, infer=keep == hip_ops.KEEP_NONE)
     cast = lambda t: t if t is None or t.dtype == ct else t.to(ct)  # noqa: E731
     y, z, zscale = cops.linear_fwd(rows(x, ct), cast(weight), cast(bias),
                                    None if residual is None else rows(residual, ct), act, keep)

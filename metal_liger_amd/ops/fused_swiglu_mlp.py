@@ -22,7 +22,7 @@ from metal_liger_amd.ops.fused_linear import (check_checkpoint, check_input, che
 
 def _forward(x, weights, residual, keep: int):
     O, I = weights[2].shape  # noqa: E741
-    ct = compute_dtype(x, x.shape[-1], I, O)
+    ct = compute_dtype(x, x.shape[-1], I, O, infer=keep == hip_ops.KEEP_NONE)
     y, *kept = cops.swiglu_mlp_fwd(rows(x, ct), *(rows(w, ct) for w in weights),
                                    None if residual is None else rows(residual, ct), keep)
     y = y if y.dtype == x.dtype else y.to(x.dtype)

@@ -339,3 +339,52 @@ def test_weight_gradients_together(dev, tokens, hidden, inter, out, frozen):
         eh = U * h.abs() + noise * u.abs()
         _check(got[3], *_mm(D.t(), torch.zeros_like(D.t()), h, eh, tokens), "down")
     assert got[0].numel() == 0
+
+
+# ------------------------------------------------- few rows, nothing to keep --
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 33, 64, 65])
+@pytest.mark.parametrize("K,N", [(8, 8), (72, 40), (512, 264), (2056, 16), (1000, 1000)])
+def test_linear_few_rows(dev, dtype, M, K, N):
+    from metal_liger_amd.ops.fused_linear import fused_linear
+    x, w, b, r, _ = _linear_case(M, K, N, dtype, K != 72, N != 16, dev)
+    with torch.no_grad():
+        y = fused_linear(x, w, b, "silu", r)
+    X, W = _cpu(x), _cpu(w)
+    z, ez = _mm(X, torch.zeros_like(X), W.t(), torch.zeros_like(W.t()), K)
+    if b is not None:
+        z = z + _cpu(b)
+        ez = ez + V * z.abs()
+    want, bound = ref.act(z, "silu"), 1.13 * ez + _act_noise(z)
+    if r is not None:
+        want = want + _cpu(r)
+        bound = bound + V * want.abs()
+    assert y.dtype == dtype
+    _check(y, want, bound, "y")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M", [1, 16, 31, 64, 65])
+@pytest.mark.parametrize("H,I,O", [(64, 8, 8), (264, 520, 72), (520, 1032, 1000), (33, 40, 50)])
+def test_mlp_few_rows(dev, dtype, M, H, I, O):  # noqa: E741
+    """Without gradients; h past fp16's range (gate weights of one sign and size)."""
+    from metal_liger_amd.ops.fused_swiglu_mlp import fused_swiglu_mlp
+    x, ws, r, _ = _mlp_case(M, H, I, O, dtype, M != 16, dev)
+    with torch.no_grad():
+        ws[0].mul_(100.0)
+        ws[1].mul_(2000.0)
+        ws[2].mul_(1e-3)
+        y = fused_swiglu_mlp(x, *ws, residual=r)
+    X, (Wg, Wu, Wd) = _cpu(x), map(_cpu, ws)
+    zx, low = torch.zeros_like(X), _matrix_cores(dtype, H, I, O)
+    g, eg = _mm(X, zx, Wg.t(), torch.zeros_like(Wg.t()), H)
+    u, eu = _mm(X, zx, Wu.t(), torch.zeros_like(Wu.t()), H)
+    h, eh = _gated(g, eg, u, eu)
+    assert h.abs().max() > 65504 or H * I < 4000
+    want, bound = _mm(h, eh + (_u(dtype) if low else V) * h.abs(), Wd.t(), torch.zeros_like(Wd.t()), I)
+    if r is not None:
+        want = want + _cpu(r)
+        bound = bound + V * want.abs()
+    keep = want.abs() < 65000
+    _check(torch.where(keep.to(dev), y, 0), torch.where(keep, want, 0.0), torch.where(keep, bound, 0.0), "y")
