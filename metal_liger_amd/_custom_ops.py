@@ -393,12 +393,19 @@ swiglu_kept_bwd = _define("swiglu_kept_bwd(Tensor gate_q, Tensor gate_scale, Ten
                                                               dy.new_empty(dy.shape, dtype=ut)))
 linear_fwd = _define("linear_fwd(Tensor x2, Tensor w, Tensor? bias, Tensor? residual, int act, "
                      "int keep) -> (Tensor, Tensor, Tensor)", hip_ops.linear_fwd, _linear_fwd_fake)
-linear_bwd = _define("linear_bwd(Tensor? x2, Tensor? w, Tensor dy, int act, int keep, Tensor z, "
-                     "Tensor zscale, SymInt N, SymInt K, bool need_dx, bool need_dw, bool need_db)"
+linear_bwd = _define("linear_bwd(Tensor? x2, Tensor? w, Tensor dy, int act, int keep, Tensor? z, "
+                     "Tensor? zscale, SymInt N, SymInt K, bool need_dx, bool need_dw, bool need_db)"
                      " -> (Tensor, Tensor, Tensor)", hip_ops.linear_bwd, _linear_bwd_fake)
 swiglu_mlp_fwd = _define("swiglu_mlp_fwd(Tensor x2, Tensor wg, Tensor wu, Tensor wd, "
                          "Tensor? residual, int keep) -> (Tensor, Tensor, Tensor, Tensor, Tensor)",
                          hip_ops.swiglu_mlp_fwd, _swiglu_mlp_fwd_fake)
+linear_infer = _define("linear_infer(Tensor x2, Tensor w, Tensor? bias, Tensor? residual, int act) "
+                       "-> Tensor", hip_ops.linear_infer, lambda x2, w, bias, residual, act:
+                       x2.new_empty((x2.shape[0], w.shape[0])))
+swiglu_mlp_infer = _define("swiglu_mlp_infer(Tensor x2, Tensor wg, Tensor wu, Tensor wd, "
+                           "Tensor? residual) -> Tensor", hip_ops.swiglu_mlp_infer,
+                           lambda x2, wg, wu, wd, residual:
+                           x2.new_empty((x2.shape[0], wd.shape[0])))
 swiglu_mlp_bwd = _define("swiglu_mlp_bwd(Tensor x2, Tensor wg, Tensor wu, Tensor wd, Tensor dy, "
                          "int keep, Tensor gate, Tensor gate_scale, Tensor up, Tensor up_scale, "
                          "bool need_dx, bool need_dwg, bool need_dwu, bool need_dwd) -> "

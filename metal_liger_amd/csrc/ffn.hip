@@ -16,6 +16,7 @@
 #include "ffn_product.h"
 #include "ffn_skinny.h"
 #include "ffn_wgrad.h"
+#include "gemm_f32.h"
 
 namespace mla {
 namespace ffn {
@@ -171,7 +172,7 @@ struct Products<float> {
   }
 
   static size_t raw_floats(int64_t M, int64_t N, int64_t K) {
-    return (size_t)M * N + (split_bytes(M, N, K) + 3) / 4;
+    return (size_t)gemmf32::sums_splits(M, N, K) * M * N;
   }
 
   static int run(int64_t M, int64_t N, int nseg, const int64_t* K, const float* const* a,
@@ -188,10 +189,7 @@ struct Products<float> {
 
   static int raw(int64_t M, int64_t N, int64_t K, const float* a, int64_t lda, const float* b,
                  int64_t ldb, bool b_mn, float* out, int& splits, hipStream_t st) {
-    splits = 1;
-    const size_t wsb = split_bytes(M, N, K);
-    return run(M, N, 1, &K, &a, &lda, &b, &ldb, kKMajor, b_mn ? kMNMajor : kKMajor, out,
-               wsb ? out + (size_t)M * N : nullptr, wsb, st);
+    return gemmf32::sums(M, N, K, a, lda, b, ldb, b_mn ? kMNMajor : kKMajor, out, splits, st);
   }
 
   static bool few(int64_t) { return false; }  // (widths and bases may rule it out)
@@ -288,7 +286,7 @@ int linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
   const bool vec = N % 8 == 0 && aligned_rows(step.bias, 0) && aligned_rows(step.residual, step.ldr) &&
                    aligned_rows(step.y, step.ldy);
   if (run && vec && few_rows<T>(M, N, K, x, ldx, w, ldw))
-    return launch_skinny<KIND == kKeepNone ? 1 : 2, false>(
+    return launch_skinny<KIND != kKeepNone, false>(
         SkinnyProduct<T, T>{xt, wt, nullptr, ldx, ldw, 0, (int)M, (int)N, (int)K}, step, st);
   if (Products<T>::few(M) && !run) return ML_OK;
   if (Products<T>::fused(M, N, K))
@@ -394,11 +392,11 @@ template <typename T, typename TH, int KIND>
 int few_mlp(const MlpFwd& p, const TH* h, const GatedStep<TH, KIND>& step,
             const LinearStep<T, kKeepNone>& out, hipStream_t st) {
   const T *wg = static_cast<const T*>(p.wg), *wu = static_cast<const T*>(p.wu);
-  const int rc = launch_skinny<KIND == kKeepNone ? 1 : 2, true>(
+  const int rc = launch_skinny<KIND != kKeepNone, true>(
       SkinnyProduct<T, T>{static_cast<const T*>(p.x), wg, wu, p.ldx, p.ldg, p.ldu, (int)p.M,
                           (int)p.I, (int)p.H}, step, st);
   if (rc) return rc;
-  return launch_skinny<1, false>(
+  return launch_skinny<false, false>(
       SkinnyProduct<TH, T>{h, static_cast<const T*>(p.wd), nullptr, p.I, p.ldd, 0, (int)p.M,
                            (int)p.O, (int)p.I}, out, st);
 }
@@ -547,7 +545,7 @@ extern "C" int ml_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t 
     const ffn::LinearStep<f16, ffn::kKeepNone> step{
         static_cast<const f16*>(bias), static_cast<const f16*>(residual), static_cast<f16*>(y), ldr,
         ldy, act, {}};
-    return ffn::launch_skinny<1, false>(
+    return ffn::launch_skinny<false, false>(
         ffn::SkinnyProduct<f16, f16>{static_cast<const f16*>(x), static_cast<const f16*>(w), nullptr,
                                      ldx, ldw, 0, (int)M, (int)N, (int)K},
         step, (hipStream_t)stream);

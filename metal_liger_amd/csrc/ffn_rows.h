@@ -288,72 +288,95 @@ struct PartialSource {
 };
 
 template <typename T>
-struct TypedSource {
+struct TypedSource {  // read once
   const T* p;
   int64_t ld;
 
   template <int VEC>
   __device__ __forceinline__ void load(int64_t m, int64_t n, float (&x)[VEC]) const {
-    load_n<T, VEC>(p + m * ld + n, x);
+    load_n_nt<T, VEC>(p + m * ld + n, x);
   }
 };
 
 constexpr int kThreads = 256;
 
-// One or two sources (Src2 void: one) through a step, a block of 32 columns by 32 / VEC
-// lanes at a time.
+// One or two sources through a step, a block of 32 columns by 32 / VEC lanes at a time.
+// A thread issues the loads of kInFlight positions before it works on the first. The
+// index arithmetic is 32-bit where the blocks can be counted in 32 bits (a 64-bit
+// division costs more than the rest of a step).
 struct NoSource {};
+constexpr int kInFlight = 2;
 
-template <int VEC, class Src, class Src2, class Step>
+template <int VEC, class Src, class Src2, class Step, typename Index>
 __global__ __launch_bounds__(kThreads) void rows_kernel(const Src src, const Src2 src2,
-                                                        const Step step, int64_t rows,
-                                                        int64_t cols) {
+                                                        const Step step, Index rows, int64_t cols,
+                                                        Index nb) {
   constexpr int L = held::kBlock / VEC;
-  const int64_t nb = (cols + held::kBlock - 1) / held::kBlock;
-  const int64_t groups = rows * nb;
-  const int64_t step_groups = (int64_t)gridDim.x * (kThreads / L);
+  constexpr bool kTwo = !std::is_same_v<Src2, NoSource>;
+  const Index groups = rows * nb;
+  const Index stride = (Index)gridDim.x * (kThreads / L) * kInFlight;
   const int l = threadIdx.x % L;
-  for (int64_t g = (int64_t)blockIdx.x * (kThreads / L) + threadIdx.x / L; g < groups;
-       g += step_groups) {
-    const int64_t m = rows == 1 ? 0 : g / nb;
-    const int64_t n = (g - m * nb) * held::kBlock + l * VEC;
-    const bool live = n < cols;
-    float x[VEC];
+  for (Index g0 = (Index)blockIdx.x * (kThreads / L) * kInFlight + threadIdx.x / L; g0 < groups;
+       g0 += stride) {
+    int64_t m[kInFlight], n[kInFlight];
+    bool live[kInFlight];
+    float x[kInFlight][VEC], u[kInFlight][VEC];
+    typename Step::template Column<VEC> c[kInFlight];
+    typename Step::template Fetched<VEC> f[kInFlight];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) x[k] = 0.f;
-    if (live) src.template load<VEC>(m, n, x);
-    typename Step::template Column<VEC> c;
-    typename Step::template Fetched<VEC> f;
-    if (live) {
-      c = step.template column<VEC>(n);
-      f = step.template fetch<VEC>(m, n);
+    for (int k = 0; k < kInFlight; ++k) {
+      // (positions past the last block fetch the last one's; they are not live)
+      const Index at = g0 + k * (kThreads / L);
+      const Index g = at < groups ? at : groups - 1;
+      const Index row = rows == 1 ? 0 : g / nb;
+      m[k] = row;
+      n[k] = (int64_t)(g - row * nb) * held::kBlock + l * VEC;
+      live[k] = n[k] < cols;
+      const int64_t nc = live[k] ? n[k] : 0;
+      src.template load<VEC>(m[k], nc, x[k]);
+      if constexpr (kTwo) src2.template load<VEC>(m[k], nc, u[k]);
+      c[k] = step.template column<VEC>(nc);
+      f[k] = step.template fetch<VEC>(m[k], nc);
+      if (!live[k]) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) x[k][e] = u[k][e] = 0.f;
+      }
+      live[k] = live[k] && at < groups;
     }
-    if constexpr (std::is_same_v<Src2, NoSource>) {
-      step.template finish<VEC>(m, n, x, c, f, live);
-    } else {
-      float u[VEC];
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) u[k] = 0.f;
-      if (live) src2.template load<VEC>(m, n, u);
-      step.template finish<VEC>(m, n, x, u, c, f, live);
+    for (int k = 0; k < kInFlight; ++k) {
+      if constexpr (kTwo)
+        step.template finish<VEC>(m[k], n[k], x[k], u[k], c[k], f[k], live[k]);
+      else
+        step.template finish<VEC>(m[k], n[k], x[k], c[k], f[k], live[k]);
     }
   }
+}
+
+template <int VEC, class Src, class Src2, class Step>
+inline void rows_launch(const Src& src, const Src2& src2, const Step& step, int64_t rows,
+                        int64_t cols, hipStream_t st) {
+  const int64_t nb = held::blocks(cols), groups = rows * nb;
+  const int per = kThreads / (held::kBlock / VEC) * kInFlight;
+  int64_t blocks = (groups + per - 1) / per;
+  blocks = blocks < (1 << 20) ? blocks : (1 << 20);
+  // (the last stride must not wrap)
+  if (groups + blocks * per < (1LL << 32))
+    rows_kernel<VEC, Src, Src2, Step, uint32_t><<<dim3((unsigned)blocks), kThreads, 0, st>>>(
+        src, src2, step, (uint32_t)rows, cols, (uint32_t)nb);
+  else
+    rows_kernel<VEC, Src, Src2, Step, int64_t><<<dim3((unsigned)blocks), kThreads, 0, st>>>(
+        src, src2, step, rows, cols, nb);
 }
 
 template <class Src, class Src2, class Step>
 inline int launch_rows(bool vec, const Src& src, const Src2& src2, const Step& step, int64_t rows,
                        int64_t cols, hipStream_t st) {
   if (rows == 0 || cols == 0) return ML_OK;
-  const int64_t groups = rows * held::blocks(cols);
-  const int per = kThreads / (held::kBlock / (vec ? 8 : 1));
-  int64_t blocks = (groups + per - 1) / per;
-  blocks = blocks < (1 << 20) ? blocks : (1 << 20);
   if (vec)
-    rows_kernel<8, Src, Src2, Step><<<dim3((unsigned)blocks), kThreads, 0, st>>>(src, src2, step,
-                                                                                 rows, cols);
+    rows_launch<8>(src, src2, step, rows, cols, st);
   else
-    rows_kernel<1, Src, Src2, Step><<<dim3((unsigned)blocks), kThreads, 0, st>>>(src, src2, step,
-                                                                                 rows, cols);
+    rows_launch<1>(src, src2, step, rows, cols, st);
   ML_LAUNCH_CHECK();
   return ML_OK;
 }

@@ -76,8 +76,9 @@ struct SkinnyProduct {
 };
 
 // MT: tiles of 16 rows of x; NT: of W (2 where the step keeps a tensor: a block of 32
-// columns).
-template <typename TX, typename TW, int MT, int NT, bool PAIR, class Step>
+// columns); REGS: registers for loads in flight. (8 rows of W a workgroup, so that 2048
+// of them lie on 256 CUs instead of 128, gained nothing, and cost 17% at 6144 pairs.)
+template <typename TX, typename TW, int MT, int NT, bool PAIR, int REGS, class Step>
 __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(
     const SkinnyProduct<TX, TW> p, const Step step) {
   constexpr int kOps = PAIR ? 2 : 1;
@@ -111,10 +112,9 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(
 #pragma unroll
       for (int i = 0; i < MT; ++i) acc[o][j][i] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // chunks c, c + 8, .. of a batch: every load before the first product (as many chunks
-  // as about 128 registers hold)
+  // chunks c, c + 8, .. of a batch: every load before the first product
   constexpr int kRegs = 4 * (kOps * NT * (int)sizeof(TW) + MT * (int)sizeof(TX));
-  constexpr int kBatch = kRegs <= 16 ? 8 : kRegs <= 32 ? 4 : kRegs <= 64 ? 2 : 1;
+  constexpr int kBatch = REGS / kRegs > 0 ? REGS / kRegs : 1;
   const int chunks = (p.K + kChunk - 1) / kChunk;
   for (int c0 = wave; c0 < chunks; c0 += kSkinnyWaves * kBatch) {
     Strip<TW> ws[kBatch][kOps][NT];
@@ -163,10 +163,11 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(
     *reinterpret_cast<f32x4*>(&fin[o][16 * i + (l & 15)][16 * j + 4 * (l >> 4)]) = s;
   }
   __syncthreads();
-  // 2 NT neighbouring lanes a row (whole waves: 16 MT rows of 2 or 4 lanes)
-  constexpr int kPositions = 16 * MT * 2 * NT;
+  // 2 NT neighbouring lanes a row
+  constexpr int kLanes = 2 * NT;
+  constexpr int kPositions = 16 * MT * kLanes;
   for (int q = threadIdx.x; q < (kPositions + 63) / 64 * 64; q += 64 * kSkinnyWaves) {
-    const int m = q / (2 * NT), c = 8 * (q % (2 * NT)), n = n0 + c;
+    const int m = q / kLanes, c = 8 * (q % kLanes), n = n0 + c;
     const bool live = m < p.M && n < p.N && q < kPositions;
     const int row = q < kPositions ? m : 0;
     typename Step::template Column<8> column;
@@ -187,15 +188,29 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(
   }
 }
 
-template <int NT, bool PAIR, typename TX, typename TW, class Step>
-inline int launch_skinny(const SkinnyProduct<TX, TW>& p, const Step& step, hipStream_t st) {
-  const dim3 grid((p.N + 16 * NT - 1) / (16 * NT)), block(64 * kSkinnyWaves);
-  if (p.M <= 16)
-    skinny_kernel<TX, TW, 1, NT, PAIR, Step><<<grid, block, 0, st>>>(p, step);
-  else if (p.M <= 32)
-    skinny_kernel<TX, TW, 2, NT, PAIR, Step><<<grid, block, 0, st>>>(p, step);
+template <int MT, bool KEEPS, bool PAIR, typename TX, typename TW, class Step>
+inline void skinny_launch(const SkinnyProduct<TX, TW>& p, const Step& step, hipStream_t st) {
+  constexpr int NT = KEEPS ? 2 : 1, kThreads = 64 * kSkinnyWaves;
+  const int blocks = (p.N + 16 * NT - 1) / (16 * NT);
+  // One workgroup a CU may fill its registers with loads (K = 6144 in one or two
+  // batches); where there are more, two share a CU.
+  constexpr int kOne = MT > 2 || KEEPS ? 96 : 160;
+  if (blocks <= num_cus())
+    skinny_kernel<TX, TW, MT, NT, PAIR, kOne, Step><<<dim3(blocks), kThreads, 0, st>>>(p, step);
   else
-    skinny_kernel<TX, TW, 4, NT, PAIR, Step><<<grid, block, 0, st>>>(p, step);
+    skinny_kernel<TX, TW, MT, NT, PAIR, 96, Step><<<dim3(blocks), kThreads, 0, st>>>(p, step);
+}
+
+template <bool KEEPS, bool PAIR, typename TX, typename TW, class Step>
+inline int launch_skinny(const SkinnyProduct<TX, TW>& p, const Step& step, hipStream_t st) {
+  if (p.M <= 16)
+    skinny_launch<1, KEEPS, PAIR>(p, step, st);
+  else if (p.M <= 32)
+    skinny_launch<2, KEEPS, PAIR>(p, step, st);
+  else if (p.M <= 48)
+    skinny_launch<3, KEEPS, PAIR>(p, step, st);
+  else
+    skinny_launch<4, KEEPS, PAIR>(p, step, st);
   ML_LAUNCH_CHECK();
   return ML_OK;
 }

@@ -35,7 +35,7 @@
 // GPU time as 128 x 128 tiles without a split, 278 us.
 #include <algorithm>
 
-#include "common.h"
+#include "gemm_f32.h"
 
 namespace mla {
 namespace gemmf32 {
@@ -274,7 +274,51 @@ Choice choose(int64_t M, int64_t N, int64_t k_len) {
   return {false, (int)std::max<int64_t>(want, 1)};
 }
 
+int launch(const Prob& pb, bool big, int a_layout, int b_layout, hipStream_t st) {
+  const int64_t bt = big ? 128 : 64;
+  const int64_t tiles = ((pb.M + bt - 1) / bt) * ((pb.N + bt - 1) / bt);
+  ML_CHECK(tiles <= 0x7fffffffLL, "gemm f32: too many tiles");
+  const dim3 grid((unsigned)tiles, (unsigned)pb.nsplit);
+#define ML_GF(LA, LB)                                                              \
+  if (big)                                                                         \
+    gemm_f32_kernel<128, 128, 16, LA, LB><<<grid, kThreads, 0, st>>>(pb);          \
+  else                                                                             \
+    gemm_f32_kernel<64, 64, 32, LA, LB><<<grid, kThreads, 0, st>>>(pb)
+  if (a_layout == kKMajor && b_layout == kKMajor) {
+    ML_GF(kKMajor, kKMajor);
+  } else if (a_layout == kKMajor) {
+    ML_GF(kKMajor, kMNMajor);
+  } else if (b_layout == kKMajor) {
+    ML_GF(kMNMajor, kKMajor);
+  } else {
+    ML_GF(kMNMajor, kMNMajor);
+  }
+#undef ML_GF
+  ML_LAUNCH_CHECK();
+  return ML_OK;
+}
+
 }  // namespace
+
+int sums(int64_t M, int64_t N, int64_t K, const float* a, int64_t lda, const float* b, int64_t ldb,
+         int b_layout, float* out, int& splits, hipStream_t st) {
+  const Choice ch = choose(M, N, K);
+  splits = ch.nsplit;
+  Prob pb{};
+  pb.M = (int)M;
+  pb.N = (int)N;
+  pb.nseg = 1;
+  pb.seg[0] = Seg{a, b, lda, ldb, (int)K};
+  pb.C = out;
+  pb.ldc = N;
+  pb.alpha = 1.f;
+  pb.partial = out;
+  pb.nsplit = splits;
+  return launch(pb, ch.big, kKMajor, b_layout, st);
+}
+
+int sums_splits(int64_t M, int64_t N, int64_t K) { return choose(M, N, K).nsplit; }
+
 }  // namespace gemmf32
 }  // namespace mla
 
@@ -332,27 +376,9 @@ extern "C" int ml_gemm_f32_segments_ws(int64_t M, int64_t N, int nseg, const int
                      workspace_bytes >= (size_t)ch.nsplit * M * N * sizeof(float);
   pb.nsplit = split ? ch.nsplit : 1;
   pb.partial = static_cast<float*>(workspace);
-  const int64_t bt = ch.big ? 128 : 64;
-  const int64_t tiles = ((M + bt - 1) / bt) * ((N + bt - 1) / bt);
-  ML_CHECK(tiles <= 0x7fffffffLL, "gemm f32: too many tiles");
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)tiles, (unsigned)pb.nsplit);
-#define ML_GF(LA, LB)                                                              \
-  if (ch.big)                                                                      \
-    gemm_f32_kernel<128, 128, 16, LA, LB><<<grid, kThreads, 0, st>>>(pb);          \
-  else                                                                             \
-    gemm_f32_kernel<64, 64, 32, LA, LB><<<grid, kThreads, 0, st>>>(pb)
-  if (a_layout == kKMajor && b_layout == kKMajor) {
-    ML_GF(kKMajor, kKMajor);
-  } else if (a_layout == kKMajor) {
-    ML_GF(kKMajor, kMNMajor);
-  } else if (b_layout == kKMajor) {
-    ML_GF(kMNMajor, kKMajor);
-  } else {
-    ML_GF(kMNMajor, kMNMajor);
-  }
-#undef ML_GF
-  ML_LAUNCH_CHECK();
+  const int rc = launch(pb, ch.big, a_layout, b_layout, st);
+  if (rc) return rc;
   if (split) {
     const int64_t blocks = std::min<int64_t>((M * N + kThreads - 1) / kThreads, 8 * num_cus());
     reduce_f32_kernel<<<dim3((unsigned)blocks), kThreads, 0, st>>>(pb.partial, pb.nsplit, M, N, C,

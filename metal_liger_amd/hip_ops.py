@@ -244,17 +244,13 @@ def _used(t: torch.Tensor | None):
     return None if t is None or t.numel() == 0 else t
 
 
-def linear_fwd(x2, w, bias, residual, act: int, keep: int):
-    """(y, z, zscale) of ml_linear_fwd: x2 [M, K], w [N, K], bias [N] or None, residual
-    [M, N] or None, all bf16 (sizes in multiples of 8), all fp32, or all fp16 (as bf16, up
-    to FEW_ROWS rows with nothing kept)."""
+def _linear(x2, w, bias, residual, act: int, keep: int, z, zscale):
     ensure_rocm_device(x2, w, bias, residual)
     x2, w = _product_rows(x2), _product_rows(w)
     (M, K), N = x2.shape, w.shape[0]
     y = torch.empty(M, N, dtype=x2.dtype, device=x2.device)
-    z, zscale = _kept_buffers(x2, N, keep)
     if M == 0:
-        return y, z, zscale
+        return y
     bias = None if bias is None else _al16(bias.contiguous())
     residual = None if residual is None else _product_rows(residual)
     tag = dtype_tag(x2, "x")
@@ -262,7 +258,19 @@ def linear_fwd(x2, w, bias, residual, act: int, keep: int):
     call("ml_linear_fwd", ptr(x2), row_stride(x2), ptr(w), row_stride(w), ptr(bias), ptr(residual),
          0 if residual is None else row_stride(residual), act, ptr(y), N, keep, ptr(_used(z)),
          ptr(_used(zscale)), M, N, K, ptr(ws), wsb, tag, stream_of(x2))
-    return y, z, zscale
+    return y
+
+
+def linear_fwd(x2, w, bias, residual, act: int, keep: int):
+    """(y, z, zscale) of ml_linear_fwd: x2 [M, K], w [N, K], bias [N] or None, residual
+    [M, N] or None, all bf16 (sizes in multiples of 8) or all fp32."""
+    kept = _kept_buffers(x2, w.shape[0], keep)
+    return (_linear(x2, w, bias, residual, act, keep, *kept), *kept)
+
+
+def linear_infer(x2, w, bias, residual, act: int):
+    """linear_fwd's y with nothing kept; also all fp16 (as bf16, up to FEW_ROWS rows)."""
+    return _linear(x2, w, bias, residual, act, KEEP_NONE, None, None)
 
 
 def linear_bwd(x2, w, dy, act: int, keep: int, z, zscale, N: int, K: int, need_dx: bool,
@@ -287,23 +295,32 @@ def linear_bwd(x2, w, dy, act: int, keep: int, z, zscale, N: int, K: int, need_d
     return dx, dw, db
 
 
-def swiglu_mlp_fwd(x2, wg, wu, wd, residual, keep: int):
-    """(y, gate, gate_scale, up, up_scale) of ml_swiglu_mlp_fwd: x2 [M, H], wg and wu
-    [I, H], wd [O, I], residual [M, O] or None; dtypes as linear_fwd."""
+def _swiglu_mlp(x2, wg, wu, wd, residual, keep: int, kept):
     ensure_rocm_device(x2, wg, wu, wd, residual)
     x2, wg, wu, wd = map(_product_rows, (x2, wg, wu, wd))
     (M, H), (O, I) = x2.shape, wd.shape  # noqa: E741
     y = torch.empty(M, O, dtype=x2.dtype, device=x2.device)
-    kept = _kept_buffers(x2, I, keep) + _kept_buffers(x2, I, keep)
     if M == 0:
-        return (y, *kept)
+        return y
     residual = None if residual is None else _product_rows(residual)
     tag = dtype_tag(x2, "x")
     ws, wsb = _workspace(x2, "ml_swiglu_mlp_fwd_workspace_bytes", M, H, I, O, tag)
     call("ml_swiglu_mlp_fwd", *_pairs(x2, wg, wu, wd), ptr(residual),
          0 if residual is None else row_stride(residual), ptr(y), keep,
          *(ptr(_used(t)) for t in kept), M, H, I, O, ptr(ws), wsb, tag, stream_of(x2))
-    return (y, *kept)
+    return y
+
+
+def swiglu_mlp_fwd(x2, wg, wu, wd, residual, keep: int):
+    """(y, gate, gate_scale, up, up_scale) of ml_swiglu_mlp_fwd: x2 [M, H], wg and wu
+    [I, H], wd [O, I], residual [M, O] or None; dtypes as linear_fwd."""
+    kept = _kept_buffers(x2, wd.shape[1], keep) + _kept_buffers(x2, wd.shape[1], keep)
+    return (_swiglu_mlp(x2, wg, wu, wd, residual, keep, kept), *kept)
+
+
+def swiglu_mlp_infer(x2, wg, wu, wd, residual):
+    """swiglu_mlp_fwd's y with nothing kept; dtypes as linear_infer."""
+    return _swiglu_mlp(x2, wg, wu, wd, residual, KEEP_NONE, (None,) * 4)
 
 
 def _pairs(*ts):

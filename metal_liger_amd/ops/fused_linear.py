@@ -80,12 +80,17 @@ def wants_grad(*tensors) -> bool:
 
 
 def _forward(x, weight, bias, residual, act: int, keep: int):
-    ct = compute_dtype(x, *weight.shape, infer=keep == hip_ops.KEEP_NONE)
-    cast = lambda t: t if t is None or t.dtype == ct else t.to(ct)  # noqa: E731
-    y, z, zscale = cops.linear_fwd(rows(x, ct), cast(weight), cast(bias),
-                                   None if residual is None else rows(residual, ct), act, keep)
-    y = y if y.dtype == x.dtype else y.to(x.dtype)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0]), z, zscale
+    """(y, z, zscale), or y alone where nothing is kept."""
+    none = keep == hip_ops.KEEP_NONE
+    ct = compute_dtype(x, *weight.shape, infer=none)
+    args = (rows(x, ct), rows(weight, ct), bias if bias is None or bias.dtype == ct else bias.to(ct),
+            None if residual is None else rows(residual, ct), act)
+    y, *kept = (cops.linear_infer(*args),) if none else cops.linear_fwd(*args, keep)
+    if y.dtype != x.dtype:
+        y = y.to(x.dtype)
+    if x.dim() != 2:
+        y = y.view(*x.shape[:-1], weight.shape[0])
+    return y, *kept
 
 
 class _FusedLinearFunction(torch.autograd.Function):
@@ -94,8 +99,8 @@ class _FusedLinearFunction(torch.autograd.Function):
         need_dx, need_dw, need_db = ctx.needs_input_grad[:3]
         if act == 0 or not (need_dx or need_dw or need_db):
             keep = hip_ops.KEEP_NONE
-        y, z, zscale = _forward(x, weight, bias, residual, act, keep)
-        ctx.save_for_backward(x if need_dw else None, weight if need_dx else None, z, zscale)
+        y, *kept = _forward(x, weight, bias, residual, act, keep)
+        ctx.save_for_backward(x if need_dw else None, weight if need_dx else None, *kept)
         ctx.act, ctx.keep, ctx.sizes = act, keep, tuple(weight.shape)
         ctx.x_shape, ctx.dtype = x.shape, x.dtype
         return y
@@ -105,7 +110,8 @@ class _FusedLinearFunction(torch.autograd.Function):
         need_dx, need_dw, need_db, need_dr = ctx.needs_input_grad[:4]
         grads = [None, None, None]
         if need_dx or need_dw or need_db:
-            x, weight, z, zscale = ctx.saved_tensors
+            x, weight, *kept = ctx.saved_tensors
+            z, zscale = kept or (None, None)
             N, K = ctx.sizes
             g = rows(dy, compute_dtype(dy, N, K))
             out = cops.linear_bwd(None if x is None else rows(x, g.dtype),
@@ -140,10 +146,8 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
         raise ValueError(f"fused_linear: bias {tuple(bias.shape)} {bias.dtype}, needed is "
                          f"({weight.shape[0]},) {x.dtype}")
     check_residual("fused_linear", residual, x, weight.shape[0])
-    hip_ops.ensure_rocm_device(x, weight, bias, residual)
     if not wants_grad(x, weight, bias, residual):
-        with torch.no_grad():
-            return _forward(x, weight, bias, residual, act, hip_ops.KEEP_NONE)[0]
+        return _forward(x, weight, bias, residual, act, hip_ops.KEEP_NONE)[0]
     keep = keep_mode(checkpoint, compute_dtype(x, *weight.shape))
     return _FusedLinearFunction.apply(x, weight, bias, residual, act, keep)
 

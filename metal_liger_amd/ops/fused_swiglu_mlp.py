@@ -21,12 +21,16 @@ from metal_liger_amd.ops.fused_linear import (check_checkpoint, check_input, che
 
 
 def _forward(x, weights, residual, keep: int):
+    """(y, gate, its scales, up, its scales), or y alone where nothing is kept."""
     O, I = weights[2].shape  # noqa: E741
-    ct = compute_dtype(x, x.shape[-1], I, O, infer=keep == hip_ops.KEEP_NONE)
-    y, *kept = cops.swiglu_mlp_fwd(rows(x, ct), *(rows(w, ct) for w in weights),
-                                   None if residual is None else rows(residual, ct), keep)
-    y = y if y.dtype == x.dtype else y.to(x.dtype)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], O), kept
+    none = keep == hip_ops.KEEP_NONE
+    ct = compute_dtype(x, x.shape[-1], I, O, infer=none)
+    args = (rows(x, ct), *(rows(w, ct) for w in weights),
+            None if residual is None else rows(residual, ct))
+    y, *kept = (cops.swiglu_mlp_infer(*args),) if none else cops.swiglu_mlp_fwd(*args, keep)
+    if y.dtype != x.dtype:
+        y = y.to(x.dtype)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], O), *kept
 
 
 class _FusedSwiGLUMLPFunction(torch.autograd.Function):
@@ -34,7 +38,7 @@ class _FusedSwiGLUMLPFunction(torch.autograd.Function):
     def forward(ctx, x, wg, wu, wd, residual, keep: int):
         if not any(ctx.needs_input_grad[:4]):
             keep = hip_ops.KEEP_NONE
-        y, kept = _forward(x, (wg, wu, wd), residual, keep)
+        y, *kept = _forward(x, (wg, wu, wd), residual, keep)
         ctx.save_for_backward(x, wg, wu, wd, *kept)
         ctx.keep = keep
         return y
@@ -69,10 +73,8 @@ def fused_swiglu_mlp(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torc
         raise ValueError(f"fused_swiglu_mlp: weights {tuple(gate_weight.shape)}, "
                          f"{tuple(up_weight.shape)} and {tuple(down_weight.shape)} do not fit")
     check_residual("fused_swiglu_mlp", residual, x, down_weight.shape[0])
-    hip_ops.ensure_rocm_device(x, gate_weight, up_weight, down_weight, residual)
     weights = (gate_weight, up_weight, down_weight)
     if not wants_grad(x, *weights, residual):
-        with torch.no_grad():
-            return _forward(x, weights, residual, hip_ops.KEEP_NONE)[0]
+        return _forward(x, weights, residual, hip_ops.KEEP_NONE)[0]
     keep = keep_mode(checkpoint, compute_dtype(x, x.shape[-1], *down_weight.shape))
     return _FusedSwiGLUMLPFunction.apply(x, *weights, residual, keep)
