@@ -725,6 +725,11 @@ int ml_swiglu_kept_bwd(const void* gate_q, const void* gate_scale, const void* u
                        const void* up_scale, const void* dy, void* dgate, void* dup, int64_t rows,
                        int64_t cols, int dtype, void* stream);
 
+/* What a tensor [rows, cols] kept as ML_KEEP_FP8 stands for, in any dtype (dense): for a
+ * backward that reads it whole (the LoRA MLP's). */
+int ml_held_values(const void* q, const void* scale, void* out, int64_t rows, int64_t cols,
+                   int dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,8 @@ _SUBMODULES = (
     "ops.fused_lora",
     "ops.fused_dropout",
     "ops.fused_embedding",
+    "ops.fused_linear",
+    "ops.fused_swiglu_mlp",
     "patch",
     "_torch_library",
     "_compile",

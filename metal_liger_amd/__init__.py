@@ -16,6 +16,8 @@ from metal_liger_amd.ops.fused_rope import MetalLigerRoPE  # noqa: E402
 from metal_liger_amd.ops.fused_linear_cross_entropy import MetalLigerFusedLinearCrossEntropy  # noqa: E402
 from metal_liger_amd.ops.fused_dropout import MetalLigerDropout, fused_dropout  # noqa: E402
 from metal_liger_amd.ops.fused_embedding import MetalLigerEmbedding, fused_embedding  # noqa: E402
+from metal_liger_amd.ops.fused_linear import MetalLigerLinear, fused_linear  # noqa: E402
+from metal_liger_amd.ops.fused_swiglu_mlp import MetalLigerSwiGLUMLP, fused_swiglu_mlp  # noqa: E402
 from metal_liger_amd.ops.fused_lora import (  # noqa: E402
     apply_fused_lora_mlp,
     apply_fused_lora_qkv,
@@ -34,6 +36,10 @@ __all__ = [
     "MetalLigerFusedLinearCrossEntropy",
     "MetalLigerDropout",
     "MetalLigerEmbedding",
+    "MetalLigerLinear",
+    "MetalLigerSwiGLUMLP",
+    "fused_linear",
+    "fused_swiglu_mlp",
     "fused_dropout",
     "fused_embedding",
     "apply_metal_liger_to_qwen3vl",

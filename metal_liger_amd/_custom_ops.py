@@ -391,6 +391,9 @@ swiglu_kept_bwd = _define("swiglu_kept_bwd(Tensor gate_q, Tensor gate_scale, Ten
                           " -> (Tensor, Tensor)", hip_ops.swiglu_kept_bwd,
                           lambda gq, gs, uq, us, dy, gt, ut: (dy.new_empty(dy.shape, dtype=gt),
                                                               dy.new_empty(dy.shape, dtype=ut)))
+held_values = _define("held_values(Tensor q, Tensor scale, ScalarType dtype) -> Tensor",
+                      hip_ops.held_values,
+                      lambda q, scale, dtype: q.new_empty(q.shape, dtype=dtype))
 linear_fwd = _define("linear_fwd(Tensor x2, Tensor w, Tensor? bias, Tensor? residual, int act, "
                      "int keep) -> (Tensor, Tensor, Tensor)", hip_ops.linear_fwd, _linear_fwd_fake)
 linear_bwd = _define("linear_bwd(Tensor? x2, Tensor? w, Tensor dy, int act, int keep, Tensor? z, "

@@ -54,6 +54,7 @@ SIGNATURES: dict[str, tuple] = {
     "ml_swiglu_bwd": (_i32, [_p, _p, _p, _p, _p, _i64, _i32, _p]),
     "ml_swiglu_kept_fwd": (_i32, [_p] * 7 + [_i64, _i64, _i32, _p]),
     "ml_swiglu_kept_bwd": (_i32, [_p] * 7 + [_i64, _i64, _i32, _p]),
+    "ml_held_values": (_i32, [_p, _p, _p, _i64, _i64, _i32, _p]),
     "ml_linear_fwd_workspace_bytes": (_sz, [_i64, _i64, _i64, _i32]),
     "ml_linear_fwd": (
         _i32,

@@ -788,3 +788,20 @@ extern "C" int ml_swiglu_kept_bwd(const void* gate_q, const void* gate_scale, co
                             step, r, c, (hipStream_t)stream);
   });
 }
+
+extern "C" int ml_held_values(const void* q, const void* scale, void* out, int64_t rows,
+                              int64_t cols, int dtype, void* stream) {
+  ML_CHECK(rows >= 0 && cols >= 0, "held values: negative size");
+  if (rows == 0 || cols == 0) return ML_OK;
+  ML_CHECK(out, "held values: null pointer");
+  ML_TRY(ffn::check_kept(ffn::kKeepFp8, q, scale, "the tensor"));
+  return dispatch_dtype(dtype, [&](auto t) -> int {
+    using T = decltype(t);
+    const bool flat = cols % held::kBlock == 0;
+    const int64_t r = flat ? 1 : rows, c = flat ? rows * cols : cols;
+    const ffn::ValuesStep<T, ffn::kKeepFp8> step{static_cast<T*>(out), c,
+                                                 ffn::make_kept<ffn::kKeepFp8>(q, scale, c)};
+    return ffn::launch_rows(cols % 8 == 0 && aligned16(out), ffn::ZeroSource{}, ffn::NoSource{},
+                            step, r, c, (hipStream_t)stream);
+  });
+}

@@ -266,7 +266,44 @@ struct GatedGradStep {
   }
 };
 
+// What a kept tensor stands for.
+template <typename T, int KIND>
+struct ValuesStep {
+  T* out;  // dense
+  int64_t cols;
+  Kept<KIND> v;
+
+  template <int VEC>
+  struct Column {};
+  template <int VEC>
+  using Fetched = typename Kept<KIND>::template Raw<VEC>;
+
+  template <int VEC>
+  __device__ __forceinline__ Column<VEC> column(int64_t) const { return {}; }
+  template <int VEC>
+  __device__ __forceinline__ Fetched<VEC> fetch(int64_t m, int64_t n) const {
+    return v.template fetch<VEC>(m, n);
+  }
+
+  template <int VEC>
+  __device__ __forceinline__ void finish(int64_t m, int64_t n, float (&x)[VEC],
+                                         const Column<VEC>&, const Fetched<VEC>& f,
+                                         bool live) const {
+    if (!live) return;
+    v.template decode<VEC>(f, x);
+    store_n<T, VEC>(out + m * cols + n, x);
+  }
+};
+
 // ------------------------------------------------------- over arrays in memory --
+
+struct ZeroSource {  // of a step that reads all by itself
+  template <int VEC>
+  __device__ __forceinline__ void load(int64_t, int64_t, float (&x)[VEC]) const {
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) x[k] = 0.f;
+  }
+};
 
 // The sum of S fp32 partials [S][rows][ld], in their order.
 struct PartialSource {

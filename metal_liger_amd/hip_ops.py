@@ -208,6 +208,18 @@ def swiglu_kept_bwd(gate_q, gate_scale, up_q, up_scale, dy, gate_dtype, up_dtype
     return dg.to(gate_dtype), du.to(up_dtype)
 
 
+def held_values(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """What a tensor kept in 8 bits stands for, in dtype."""
+    ensure_rocm_device(q, scale)
+    if kept_shapes(q.shape) != (tuple(q.shape), tuple(scale.shape)):
+        raise ValueError(f"held values: scales {tuple(scale.shape)} do not fit {tuple(q.shape)}")
+    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    if q.numel():
+        call("ml_held_values", ptr(q.contiguous()), ptr(scale.contiguous()), ptr(out),
+             q.numel() // q.shape[-1], q.shape[-1], dtype_tag(out, "out"), stream_of(q))
+    return out
+
+
 # ------------------------------------------------------------ feed-forward --
 
 

@@ -16,11 +16,17 @@ sizes are upcast, and rounded once at the end).
 
 from __future__ import annotations
 
+import dis
+import inspect
+import logging
+
 import torch
 import torch.nn as nn
 
 from metal_liger_amd import _custom_ops as cops
 from metal_liger_amd import hip_ops
+
+logger = logging.getLogger(__name__)
 
 ACTIVATIONS = {None: 0, "silu": 1, "gelu": 2, "gelu_tanh": 3}
 DTYPES = (torch.float32, torch.bfloat16, torch.float16)
@@ -175,3 +181,137 @@ class MetalLigerLinear(nn.Module):
     def extra_repr(self) -> str:
         out, ins = self.weight.shape
         return f"{ins}, {out}, bias={self.bias is not None}, activation={self.activation}"
+
+
+# ------------------------------------------------------------------ patching --
+
+_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+
+
+def plain_linear(module) -> bool:
+    """An nn.Linear as it is: an adapter's wrapper or a subclass may compute something
+    else, and hooks (or a replaced forward) want the module to be called."""
+    return (type(module) is nn.Linear and "forward" not in module.__dict__
+            and not any(getattr(module, name, None) for name in _HOOKS))
+
+
+def runs_fused(x, *linears) -> bool:
+    """Whether a routed module's forward may run the fused op for x: its linear layers
+    are plain ones of x's dtype, and autocast would not cast them."""
+    return (all(plain_linear(m) and m.weight.dtype == x.dtype for m in linears)
+            and x.dtype in DTYPES and x.dim() > 0 and not torch.is_autocast_enabled("cuda"))
+
+
+def activation_name(module) -> str | None:
+    """The name in ACTIVATIONS of an activation module (nn's, or transformers' by its
+    class name), None for any other."""
+    if isinstance(module, nn.SiLU):
+        return "silu"
+    if isinstance(module, nn.GELU):
+        return "gelu" if module.approximate == "none" else "gelu_tanh"
+    # GELUTanh is gelu by tanh; GELUActivation is gelu, by torch or in Python
+    return {"SiLUActivation": "silu", "GELUActivation": "gelu",
+            "GELUTanh": "gelu_tanh", "PytorchGELUTanh": "gelu_tanh"}.get(type(module).__name__)
+
+
+class _FusedVisionMLPForward:
+    """Forward of a vision block's MLP, linear_fc2(act_fn(linear_fc1(x))), with the
+    activation and (residual given) the block's addition in the products' epilogues.
+    Where runs_fused does not hold, the module's own forward."""
+
+    def __init__(self, mlp: nn.Module, original, checkpoint: str | None):
+        self.mlp, self.original, self.checkpoint = mlp, original, checkpoint
+        self.activation = activation_name(mlp.act_fn)
+
+    def __call__(self, hidden_state, residual=None):
+        fc1, fc2 = self.mlp.linear_fc1, self.mlp.linear_fc2
+        if not runs_fused(hidden_state, fc1, fc2):
+            out = self.original(hidden_state)
+            return out if residual is None else residual + out
+        fused = residual is not None and residual.dtype == hidden_state.dtype and \
+            residual.shape == (*hidden_state.shape[:-1], fc2.weight.shape[0])
+        h = fused_linear(hidden_state, fc1.weight, fc1.bias, self.activation,
+                         checkpoint=self.checkpoint)
+        out = fused_linear(h, fc2.weight, fc2.bias, residual=residual if fused else None)
+        return out if fused or residual is None else residual + out
+
+
+_BLOCK_PARTS = ("norm1", "attn", "norm2", "mlp")
+
+
+def _block_structure(fn) -> tuple:
+    """(the block's parts in the order in which a forward's bytecode loads them, its
+    additions, whether it returns a local variable and keeps no tuple or list)."""
+    parts, adds, single, prev = [], 0, True, None
+    for ins in dis.get_instructions(fn):
+        if ins.opname in ("LOAD_ATTR", "LOAD_METHOD") and ins.argval in _BLOCK_PARTS:
+            parts.append(ins.argval)
+        elif ins.opname in ("BINARY_ADD", "INPLACE_ADD") or (
+                ins.opname == "BINARY_OP" and ins.argrepr in ("+", "+=")):
+            adds += 1
+        elif ins.opname in ("BUILD_LIST", "LIST_APPEND", "LIST_EXTEND") or (
+                ins.opname == "STORE_FAST" and prev is not None and prev.opname == "BUILD_TUPLE"):
+            single = False  # (a call with ** builds a tuple of its arguments)
+        elif ins.opname == "RETURN_VALUE" and (prev is None or prev.opname != "LOAD_FAST"):
+            single = False
+        prev = ins
+    return tuple(parts), adds, single
+
+
+def _fusable_block(block: nn.Module) -> bool:
+    """A vision block whose forward is h + attn(norm1(h), ...), then + mlp(norm2(h))."""
+    if not all(hasattr(block, p) for p in _BLOCK_PARTS) or \
+            not isinstance(block.mlp.__dict__.get("forward"), _FusedVisionMLPForward):
+        return False
+    fn = inspect.unwrap(getattr(type(block).forward, "__func__", type(block).forward))
+    try:
+        first = list(inspect.signature(fn).parameters)[1]
+    except (TypeError, ValueError, IndexError):
+        return False
+    # (attn stands before norm1: the method is looked up before its arguments are)
+    return first == "hidden_states" and _block_structure(fn) == (("attn", "norm1", "mlp", "norm2"),
+                                                                 2, True)
+
+
+class _FusedVisionBlockForward:
+    """Forward of a vision block, whose second addition its MLP makes. Every argument but
+    hidden_states goes to attn, as the replaced forward passes them."""
+
+    def __init__(self, block: nn.Module, original):
+        self.block, self.signature = block, inspect.signature(original)
+        self.var_kw = next((p.name for p in self.signature.parameters.values()
+                            if p.kind is p.VAR_KEYWORD), None)
+
+    def __call__(self, *args, **kwargs):
+        bound = self.signature.bind(*args, **kwargs)
+        bound.apply_defaults()
+        rest = dict(bound.arguments)
+        extra = rest.pop(self.var_kw, {}) if self.var_kw else {}
+        h, b = rest.pop("hidden_states"), self.block
+        h = h + b.attn(b.norm1(h), **rest, **extra)
+        return b.mlp(b.norm2(h), residual=h)
+
+
+def patch_vision_mlp(model: nn.Module, checkpoint: str | None = None) -> int:
+    """Routes the MLPs of a vision tower (modules with linear_fc1, act_fn and linear_fc2
+    as Qwen3-VL's blocks have them, whose forward is linear_fc2(act_fn(linear_fc1(x))))
+    through the fused linear layers, and the additions around them where a block's
+    forward has transformers' structure. Returns how many MLPs were routed; only the
+    instances' ``forward`` changes, modules already routed are left as they are."""
+    check_checkpoint(checkpoint)
+    routed = 0
+    for module in model.modules():
+        if not all(hasattr(module, n) for n in ("linear_fc1", "act_fn", "linear_fc2")) or \
+                hasattr(module, "norm") or getattr(module, "_metal_liger_vision_mlp", False):
+            continue
+        if not (plain_linear(module.linear_fc1) and plain_linear(module.linear_fc2)
+                and activation_name(module.act_fn)):
+            continue
+        module.forward = _FusedVisionMLPForward(module, module.forward, checkpoint)
+        module._metal_liger_vision_mlp = True
+        routed += 1
+    for module in model.modules():
+        if "forward" not in module.__dict__ and _fusable_block(module):
+            module.forward = _FusedVisionBlockForward(module, module.forward)
+    logger.info(f"MetalLiger vision MLP: activated on {routed} modules.")
+    return routed

@@ -40,6 +40,7 @@ from metal_liger_amd import _custom_ops as cops
 from metal_liger_amd import hip_ops
 from metal_liger_amd._model_walk import find_layers, shadowed
 from metal_liger_amd.ops.fused_dropout import MetalLigerDropout, seed_tensor
+from metal_liger_amd.ops.fused_linear import check_checkpoint
 from metal_liger_amd.ops.fused_swiglu import fused_swiglu
 
 logger = logging.getLogger(__name__)
@@ -300,17 +301,23 @@ class _LoRA_MLP(torch.autograd.Function):
                 X,
                 GW, GA, GB, GS,   # gate projection
                 UW, UA, UB, US,   # up projection
-                DW, DA, DB, DS):  # down projection
+                DW, DA, DB, DS,   # down projection
+                checkpoint=None):  # "fp8": gate and up are kept in 8 bits
         _check_float(X, "LoRA MLP")
         shape = X.shape
+        ctx.held = checkpoint is not None
+        swiglu = cops.swiglu_kept_fwd if ctx.held else lambda g, u: (cops.swiglu_fwd(g, u), g, u)
         ctx.fp32 = _fp32_path(X, X.shape[-1], GW.shape[0])
         if ctx.fp32:
             X2 = _rows_f32(X)
             gate, xa_g = _lora_out_f32(X2, GW, GA, GB, GS)
             up, xa_u = _lora_out_f32(X2, UW, UA, UB, US)
-            h = cops.swiglu_fwd(gate, up)                          # silu(gate) * up, fp32
+            h, *kept = swiglu(gate, up)                            # silu(gate) * up, fp32
             out, ha = _lora_out_f32(h, DW, DA, DB, DS)
-            ctx.save_for_backward(X2, gate, up, h, xa_g, xa_u, ha,
+            if not ctx.held:
+                kept.append(h)
+            ctx.n_kept = len(kept)
+            ctx.save_for_backward(*kept, X2, xa_g, xa_u, ha,
                                   *(t.detach() for t in (GW, UW, DW, GA, UA, DA, GB, UB, DB)))
             ctx.scales = [float(GS), float(US), float(DS)]
             ctx.orig_shape, ctx.x_dtype = shape, X.dtype
@@ -327,12 +334,13 @@ class _LoRA_MLP(torch.autograd.Function):
         xa_gu = cops.lora_xa(Xf, a_gu)                            # [N, 2 rp]
         gate = cops.lora_linear_out(Xf, GWc, xa_gu[:, :rp], sG)
         up = cops.lora_linear_out(Xf, UWc, xa_gu[:, rp:], sU)
-        h = cops.swiglu_fwd(gate, up)                             # silu(gate) * up, bf16
+        h, *kept = swiglu(gate, up)                               # silu(gate) * up, bf16
         ha_d = cops.lora_xa(h, a_d)                               # [N, rp]
         out = cops.lora_linear_out(h, DWc, ha_d, sD)
         # h is not saved: the backward recomputes it from gate and up (the
         # same kernel math, so the same bits), one [N, inter] tensor less
-        ctx.save_for_backward(Xf, gate, up, xa_gu, ha_d, a_gu, a_d, GWc, UWc, DWc, BG, BU, BD)
+        ctx.n_kept = len(kept)
+        ctx.save_for_backward(*kept, Xf, xa_gu, ha_d, a_gu, a_d, GWc, UWc, DWc, BG, BU, BD)
         ctx.scales = scales
         ctx.param_dtypes = [t.dtype for t in (GA, UA, DA, GB, UB, DB)]
         ctx.ranks, ctx.rank_p = ranks, rp
@@ -341,8 +349,15 @@ class _LoRA_MLP(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dY):
+        kept, rest = ctx.saved_tensors[:ctx.n_kept], ctx.saved_tensors[ctx.n_kept:]
+        if ctx.held:
+            dtype = torch.float32 if ctx.fp32 else torch.bfloat16
+            gate, up = cops.held_values(*kept[:2], dtype), cops.held_values(*kept[2:], dtype)
+        else:
+            gate, up = kept[:2]
         if ctx.fp32:
-            (X2, gate, up, h, xa_g, xa_u, ha, *params) = ctx.saved_tensors
+            h = cops.swiglu_fwd(gate, up) if ctx.held else kept[2]
+            (X2, xa_g, xa_u, ha, *params) = rest
             GW, UW, DW, GA, UA, DA, GB, UB, DB = (_f32(t) for t in params)
             sg, su, sd = ctx.scales
             dy = _rows_f32(dY)
@@ -356,8 +371,8 @@ class _LoRA_MLP(torch.autograd.Function):
             return (dX,
                     None, dA_G, dB_G, None,
                     None, dA_U, dB_U, None,
-                    None, dA_D, dB_D, None)
-        (Xf, gate, up, xa_gu, ha_d, a_gu, a_d, GW, UW, DW, BG, BU, BD) = ctx.saved_tensors
+                    None, dA_D, dB_D, None, *((None,) if ctx.held else ()))
+        (Xf, xa_gu, ha_d, a_gu, a_d, GW, UW, DW, BG, BU, BD) = rest
         (rg, ru, rd), rp = ctx.ranks, ctx.rank_p
         shape = ctx.orig_shape
         dy = hip_ops._bf16_rows(dY.reshape(-1, dY.shape[-1]))
@@ -372,7 +387,8 @@ class _LoRA_MLP(torch.autograd.Function):
         return (dX,
                 None, dA_G, dB_G, None,   # GW, GA, GB, GS
                 None, dA_U, dB_U, None,   # UW, UA, UB, US
-                None, dA_D, dB_D, None)   # DW, DA, DB, DS
+                None, dA_D, dB_D, None,   # DW, DA, DB, DS
+                *((None,) if ctx.held else ()))
 
 
 class _LoRA_W(torch.autograd.Function):
@@ -651,12 +667,14 @@ def apply_fused_lora_qkv(attn_module, X: torch.Tensor, lora_dropout: bool = Fals
 
 
 def apply_fused_lora_mlp(mlp_module, X: torch.Tensor, lora_dropout: bool = False,
-                         seed=None) -> torch.Tensor:
+                         seed=None, checkpoint: str | None = None) -> torch.Tensor:
     """Fused gate+up+down LoRA MLP (ops/fused_lora.py:298-320); the module's
     own forward when any projection has no LoRA adapter.
 
     lora_dropout, seed: as in apply_fused_lora_qkv (streams 0, 1, 2 for gate, up,
-    down)."""
+    down). checkpoint: None, or "fp8" to keep gate and up in 8 bits for the backward
+    (ops/fused_swiglu.py), not where dropout is applied."""
+    check_checkpoint(checkpoint)
     GW, GA, GB, GS = _get_lora_params(mlp_module.gate_proj)
     UW, UA, UB, US = _get_lora_params(mlp_module.up_proj)
     DW, DA, DB, DS = _get_lora_params(mlp_module.down_proj)
@@ -668,6 +686,8 @@ def apply_fused_lora_mlp(mlp_module, X: torch.Tensor, lora_dropout: bool = False
         projections = [mlp_module.gate_proj, mlp_module.up_proj, mlp_module.down_proj]
         thresholds = tuple(_drop_threshold(m) for m in projections)
         if any(thresholds):
+            if checkpoint:
+                raise ValueError("LoRA MLP: checkpoint does not go with lora_dropout")
             _check_float(X, "LoRA MLP")
             hip_ops.ensure_rocm_device(X)
             seed = seed_tensor(seed, X.device)
@@ -688,6 +708,7 @@ def apply_fused_lora_mlp(mlp_module, X: torch.Tensor, lora_dropout: bool = False
         GW, GA, GB, GS,
         UW, UA, UB, US,
         DW, DA, DB, DS,
+        *(() if checkpoint is None else (checkpoint,)),
     )
 
 
@@ -740,15 +761,17 @@ class _FusedMLPForward:
     """Forward of an MLP whose gate/up/down projections all carry LoRA: the
     whole block is one _LoRA_MLP call."""
 
-    def __init__(self, mlp: nn.Module, lora_dropout: bool = False):
+    def __init__(self, mlp: nn.Module, lora_dropout: bool = False, checkpoint: str | None = None):
         self.mlp = mlp
         self.lora_dropout = lora_dropout
+        self.checkpoint = checkpoint
 
     def __call__(self, x):
-        return apply_fused_lora_mlp(self.mlp, x, self.lora_dropout)
+        return apply_fused_lora_mlp(self.mlp, x, self.lora_dropout, checkpoint=self.checkpoint)
 
 
-def patch_fused_lora(model: nn.Module, lora_dropout: bool = False) -> int:
+def patch_fused_lora(model: nn.Module, lora_dropout: bool = False,
+                     mlp_checkpoint: str | None = None) -> int:
     """Routes every decoder layer's attention and MLP whose three
     projections all carry LoRA through _LoRA_QKV / _LoRA_MLP and returns how
     many modules were routed (ops/fused_lora.py:323-421).
@@ -761,7 +784,9 @@ def patch_fused_lora(model: nn.Module, lora_dropout: bool = False) -> int:
     are left as they are, so a second call returns 0.
 
     lora_dropout: in training mode the adapters read their input through their
-    lora_dropout modules, as PEFT's own forward does (the reference ignores it)."""
+    lora_dropout modules, as PEFT's own forward does (the reference ignores it).
+    mlp_checkpoint: apply_fused_lora_mlp's checkpoint."""
+    check_checkpoint(mlp_checkpoint)
     layers = find_layers(model)
     if layers is None:
         logger.warning("MetalLiger fused LoRA: could not find transformer layers")
@@ -771,7 +796,8 @@ def patch_fused_lora(model: nn.Module, lora_dropout: bool = False) -> int:
         for attr, names, make in (
                 ("self_attn", _QKV_PROJ,
                  lambda m: _FusedAttentionForward(m, m.forward, lora_dropout)),
-                ("mlp", _MLP_PROJ, lambda m: _FusedMLPForward(m, lora_dropout))):
+                ("mlp", _MLP_PROJ,
+                 lambda m: _FusedMLPForward(m, lora_dropout, mlp_checkpoint))):
             mod = getattr(layer, attr, None)
             if mod is None or getattr(mod, "_metal_liger_fused_lora", False):
                 continue

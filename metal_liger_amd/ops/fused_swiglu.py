@@ -64,10 +64,15 @@ def fused_swiglu(gate: torch.Tensor, up: torch.Tensor,
 class MetalLigerSwiGLU(nn.Module):
     """Drop-in for a SwiGLU MLP block; fuses the activation step only
     (ops/fused_swiglu.py:59-75). Keeps gate_proj / up_proj / down_proj under
-    their original names so state_dict keys are unchanged."""
+    their original names so state_dict keys are unchanged. checkpoint: as
+    fused_swiglu's."""
 
-    def __init__(self, original_mlp: nn.Module):
+    checkpoint = None
+
+    def __init__(self, original_mlp: nn.Module, checkpoint: str | None = None):
         super().__init__()
+        check_checkpoint(checkpoint)
+        self.checkpoint = checkpoint
         self.gate_proj = original_mlp.gate_proj
         self.up_proj = original_mlp.up_proj
         self.down_proj = original_mlp.down_proj
@@ -75,7 +80,7 @@ class MetalLigerSwiGLU(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         gate = self.gate_proj(x)
         up = self.up_proj(x)
-        activated = _FusedSwiGLUFunction.apply(gate, up)
+        activated = fused_swiglu(gate, up, self.checkpoint)
         return self.down_proj(activated)
 
     def extra_repr(self) -> str:

@@ -12,12 +12,20 @@ as ops/fused_linear.py.
 
 from __future__ import annotations
 
+import logging
+
 import torch
+import torch.nn as nn
 
 from metal_liger_amd import _custom_ops as cops
 from metal_liger_amd import hip_ops
+from metal_liger_amd._model_walk import find_layers
 from metal_liger_amd.ops.fused_linear import (check_checkpoint, check_input, check_residual,
-                                              compute_dtype, keep_mode, rows, wants_grad)
+                                              compute_dtype, keep_mode, plain_linear, rows,
+                                              runs_fused, wants_grad)
+from metal_liger_amd.ops.fused_swiglu import MetalLigerSwiGLU
+
+logger = logging.getLogger(__name__)
 
 
 def _forward(x, weights, residual, keep: int):
@@ -78,3 +86,75 @@ def fused_swiglu_mlp(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torc
         return _forward(x, weights, residual, hip_ops.KEEP_NONE)[0]
     keep = keep_mode(checkpoint, compute_dtype(x, x.shape[-1], *down_weight.shape))
     return _FusedSwiGLUMLPFunction.apply(x, *weights, residual, keep)
+
+
+_PROJECTIONS = ("gate_proj", "up_proj", "down_proj")
+
+
+def _fusable(mlp: nn.Module) -> bool:
+    """A gated MLP of three plain linear layers without bias, on SiLU."""
+    projections = [getattr(mlp, name, None) for name in _PROJECTIONS]
+    if not all(plain_linear(m) and m.bias is None for m in projections):
+        return False
+    act = getattr(mlp, "act_fn", None)  # MetalLigerSwiGLU has none: SiLU
+    return isinstance(mlp, MetalLigerSwiGLU) if act is None else \
+        isinstance(act, nn.SiLU) or type(act).__name__ == "SiLUActivation"
+
+
+class MetalLigerSwiGLUMLP(nn.Module):
+    """Drop-in for a gated MLP (gate_proj, up_proj, down_proj without bias, SiLU), whose
+    projections it keeps under their names (state_dict keys are unchanged); forward also
+    takes a residual to add."""
+
+    def __init__(self, original_mlp: nn.Module, checkpoint: str | None = None):
+        super().__init__()
+        check_checkpoint(checkpoint)
+        if not _fusable(original_mlp):
+            raise ValueError("MetalLigerSwiGLUMLP: gate_proj, up_proj and down_proj must be plain "
+                             f"nn.Linear layers without bias, on SiLU (got {original_mlp})")
+        self.gate_proj = original_mlp.gate_proj
+        self.up_proj = original_mlp.up_proj
+        self.down_proj = original_mlp.down_proj
+        self.checkpoint = checkpoint
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
+        return fused_swiglu_mlp(x, self.gate_proj.weight, self.up_proj.weight,
+                                self.down_proj.weight, residual, self.checkpoint)
+
+    def extra_repr(self) -> str:
+        return f"checkpoint={self.checkpoint}"
+
+
+class _FusedMLPForward:
+    """Forward of a routed MLP: the fused block, or the module's own forward where a
+    projection is no longer a plain linear layer (an adapter was added since, a hook),
+    under autocast and for inputs of another dtype."""
+
+    def __init__(self, mlp: nn.Module, original, checkpoint: str | None):
+        self.mlp, self.original, self.checkpoint = mlp, original, checkpoint
+
+    def __call__(self, x):
+        gate, up, down = (getattr(self.mlp, name) for name in _PROJECTIONS)
+        if not runs_fused(x, gate, up, down):
+            return self.original(x)
+        return fused_swiglu_mlp(x, gate.weight, up.weight, down.weight, checkpoint=self.checkpoint)
+
+
+def patch_swiglu_mlp(model: nn.Module, checkpoint: str | None = None) -> int:
+    """Routes the decoder layers' gated MLPs without adapters through the fused block and
+    returns how many were routed. Only the instances' ``forward`` changes; modules
+    already routed (here or to the LoRA block) are left as they are."""
+    check_checkpoint(checkpoint)
+    layers = find_layers(model)
+    if layers is None:
+        logger.warning("MetalLiger fused MLP: could not find transformer layers")
+        return 0
+    routed = 0
+    for layer in layers:
+        mlp = getattr(layer, "mlp", None)
+        if mlp is None or "forward" in mlp.__dict__ or not _fusable(mlp):
+            continue
+        mlp.forward = _FusedMLPForward(mlp, mlp.forward, checkpoint)
+        routed += 1
+    logger.info(f"MetalLiger fused MLP: activated on {routed} modules.")
+    return routed

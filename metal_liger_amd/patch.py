@@ -17,11 +17,13 @@ import torch.nn as nn
 from metal_liger_amd._model_walk import find_final_norm, find_layers
 from metal_liger_amd.ops.fused_add_rms_norm import patch_residual_add_norm
 from metal_liger_amd.ops.fused_embedding import patch_embedding
+from metal_liger_amd.ops.fused_linear import check_checkpoint, patch_vision_mlp
 from metal_liger_amd.ops.fused_linear_cross_entropy import patch_causal_lm_loss
 from metal_liger_amd.ops.fused_lora import patch_fused_lora
 from metal_liger_amd.ops.fused_qk_norm_rope import patch_qk_norm_rope
 from metal_liger_amd.ops.fused_rms_norm import MetalLigerRMSNorm
 from metal_liger_amd.ops.fused_swiglu import MetalLigerSwiGLU
+from metal_liger_amd.ops.fused_swiglu_mlp import patch_swiglu_mlp
 from metal_liger_amd.ops.gqa_attention import patch_efficient_attention
 
 logger = logging.getLogger(__name__)
@@ -58,7 +60,7 @@ def _replace_rms_norms(model: nn.Module) -> int:
     return count
 
 
-def _replace_mlps(model: nn.Module) -> int:
+def _replace_mlps(model: nn.Module, checkpoint: str | None = None) -> int:
     """Wraps every layer MLP that has gate_proj in MetalLigerSwiGLU (patch.py:162-178)."""
     layers = _find_layers(model)
     if layers is None:
@@ -66,7 +68,7 @@ def _replace_mlps(model: nn.Module) -> int:
     count = 0
     for layer in layers:
         if hasattr(layer, "mlp") and hasattr(layer.mlp, "gate_proj"):
-            layer.mlp = MetalLigerSwiGLU(layer.mlp)
+            layer.mlp = MetalLigerSwiGLU(layer.mlp, checkpoint)
             count += 1
     return count
 
@@ -85,6 +87,9 @@ def apply_metal_liger_to_qwen3vl(
     efficient_attention: bool = False,
     lora_dropout: bool = False,
     fuse_embedding: bool = False,
+    fuse_mlp: bool = False,
+    fuse_vision_mlp: bool = False,
+    mlp_checkpoint: str | None = None,
 ) -> nn.Module:
     """Apply the fused operations to a Qwen3 / Qwen3-VL model in place and
     return it (patch.py:181-240).
@@ -114,15 +119,26 @@ def apply_metal_liger_to_qwen3vl(
     (ops/fused_lora.py, ops/fused_dropout.py).
     fuse_embedding: the token embedding and the gradient of its table
     (ops/fused_embedding.py).
+    fuse_mlp: gated MLPs without adapters run as one block, the projections'
+    products with the activation in their epilogue (ops/fused_swiglu_mlp.py).
+    fuse_vision_mlp: the MLPs of Qwen3-VL's vision tower, with the activation
+    and the block's addition in the products' epilogues (ops/fused_linear.py).
+    mlp_checkpoint: "fp8" keeps what the MLPs' backward needs of the
+    activation's inputs in 8 bits: in MLPs that this call routes or replaces
+    (fuse_swiglu, fuse_mlp, fuse_vision_mlp, and fuse_lora without
+    lora_dropout).
     use_optimized_generator is not part of metal_liger_amd (inference path).
     """
+    check_checkpoint(mlp_checkpoint)
+    if mlp_checkpoint and lora_dropout and fuse_lora:
+        raise ValueError("mlp_checkpoint does not go with lora_dropout")
     stats = {}
     if fuse_rms_norm:
         n = _replace_rms_norms(model)
         stats["rms_norm"] = n
         logger.info(f"MetalLiger: replaced {n} RMSNorm layers with fused versions")
     if fuse_swiglu:
-        n = _replace_mlps(model)
+        n = _replace_mlps(model, mlp_checkpoint)
         stats["swiglu"] = n
         logger.info(f"MetalLiger: replaced {n} MLP layers with fused SwiGLU")
     if fuse_residual_norm:
@@ -135,9 +151,18 @@ def apply_metal_liger_to_qwen3vl(
         stats["qk_norm_rope"] = n
         logger.info(f"MetalLiger: fused q/k norm + RoPE on {n} attention modules")
     if fuse_lora:
-        n = patch_fused_lora(model, lora_dropout)
+        n = patch_fused_lora(model, lora_dropout, mlp_checkpoint)
         stats["fused_lora"] = n
         logger.info(f"MetalLiger: fused LoRA QKV+MLP marked {n} modules")
+    if fuse_mlp:
+        # after the LoRA patch, which takes the MLPs with adapters
+        n = patch_swiglu_mlp(model, mlp_checkpoint)
+        stats["mlp"] = n
+        logger.info(f"MetalLiger: fused {n} gated MLPs")
+    if fuse_vision_mlp:
+        n = patch_vision_mlp(model, mlp_checkpoint)
+        stats["vision_mlp"] = n
+        logger.info(f"MetalLiger: fused {n} vision MLPs")
     if fuse_lm_loss:
         n = patch_causal_lm_loss(model)
         stats["lm_loss"] = n
