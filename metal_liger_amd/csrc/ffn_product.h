@@ -32,7 +32,8 @@ struct Stager {
   static_assert(4 * kWaveBytes <= gemm::r4::Geom<T>::LDS_BYTES, "within the operand slots");
 
   // Rows m0 .. m0 + W - 1, columns n0 .. n0 + kCols - 1 of this wave (lds: its own).
-  template <class Step>
+  // ALL: all of them are within M and N.
+  template <bool ALL, class Step>
   static __device__ __forceinline__ void run(gemm::f32x4_t (&acc)[T / 4][T][4], float* lds, int m0,
                                              int n0, int lane, int M, int N, const Step& step) {
     const int G = lane >> 4, c = lane & 15;
@@ -41,9 +42,8 @@ struct Stager {
     const float* rd = lds + row * kPitch + col;
     const int n = n0 + col;
     using Fetched = typename Step::template Fetched<8>;
-    typename Step::template Column<8> column;
-    const int nc = n < N ? n : 0;  // positions past the edges fetch others, in range
-    column = step.template column<8>(nc);
+    const int nc = ALL || n < N ? n : 0;  // positions past the edges fetch others, in range
+    const typename Step::template Column<8> column = step.template column<8>(nc);
     Fetched next[kBatch];
     auto fetch = [&](Fetched(&f)[kBatch], int m) __attribute__((always_inline)) {
 #pragma unroll
@@ -74,20 +74,21 @@ struct Stager {
         for (int k = 0; k < kBatch; ++k) now[k] = next[k];
         const int m1 = mh + (s0 + kBatch) * kStepRows;  // the next batch: of this half, then the next
         fetch(next, s0 + kBatch < kSteps ? m1 : mh + kRows);
+        int64_t m[kBatch];
+        bool live[kBatch];
+        float x[kBatch][8], u[PAIR ? kBatch : 1][8];
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
           const int r = (s0 + k) * kStepRows;
-          const int m = mh + r;
-          float x[8];
-          load_n<float, 8>(rd + r * kPitch, x);
-          if constexpr (PAIR) {
-            float u[8];
-            load_n<float, 8>(rd + r * kPitch + kCols, u);
-            step.template finish<8>(m, n, x, u, column, now[k], m < M && n < N);
-          } else {
-            step.template finish<8>(m, n, x, column, now[k], m < M && n < N);
-          }
+          m[k] = mh + r;
+          live[k] = ALL || (mh + r < M && n < N);
+          load_n<float, 8>(rd + r * kPitch, x[k]);
+          if constexpr (PAIR) load_n<float, 8>(rd + r * kPitch + kCols, u[k]);
         }
+        if constexpr (PAIR)
+          step.template finish<ALL, 8, kBatch>(m, n, x, u, column, now, live);
+        else
+          step.template finish<ALL, 8, kBatch>(m, n, x, column, now, live);
       }
       __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
       __builtin_amdgcn_wave_barrier();
@@ -111,8 +112,12 @@ __global__ __launch_bounds__(C::THREADS) void product_kernel(const gemm::Problem
   gemm::r4_mainloop<gemm::kKMajor, LB, T, false, PAIR>(pb, tm, tn, 0, 1, 0, lds, acc, b2);
   const int w = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   constexpr int kTileN = PAIR ? C::BN / 2 : C::BN;
-  S::run(acc, reinterpret_cast<float*>(lds + w * S::kWaveBytes), tm * C::BM + (w >> 1) * S::W,
-         tn * kTileN + (w & 1) * S::kCols, threadIdx.x & 63, pb.M, pb.N, step);
+  float* wl = reinterpret_cast<float*>(lds + w * S::kWaveBytes);
+  const int m0 = tm * C::BM + (w >> 1) * S::W, n0 = tn * kTileN + (w & 1) * S::kCols;
+  if (m0 + S::W <= pb.M && n0 + S::kCols <= pb.N)  // (wave-uniform)
+    S::template run<true>(acc, wl, m0, n0, threadIdx.x & 63, pb.M, pb.N, step);
+  else
+    S::template run<false>(acc, wl, m0, n0, threadIdx.x & 63, pb.M, pb.N, step);
 }
 
 // The product of a [M, K] and b ([N, K], or with LB kMNMajor [K, N]) through the step.

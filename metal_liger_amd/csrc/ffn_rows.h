@@ -25,22 +25,52 @@ struct Kept {
   uint8_t* scale;
   int64_t cols, nblocks;
 
-  // every lane of a block takes part; live: this lane's columns exist
-  template <int VEC>
-  __device__ __forceinline__ void put(int64_t m, int64_t n, const float (&x)[VEC],
-                                      bool live) const {
-    const int64_t at = m * cols + n;
+  // B positions (rows m[q], columns n on); every lane of a block takes part; live[q]:
+  // this lane's position exists (ALL: every one does).
+  template <bool ALL, int VEC, int B>
+  __device__ __forceinline__ void put(const int64_t (&m)[B], int64_t n, const float (&x)[B][VEC],
+                                      const bool (&live)[B]) const {
     if constexpr (KIND == kKeepF32) {
-      if (live) store_n<float, VEC>(v + at, x);
+#pragma unroll
+      for (int q = 0; q < B; ++q)
+        if (ALL || live[q]) store_n<float, VEC>(v + m[q] * cols + n, x[q]);
     } else if constexpr (KIND != kKeepNone) {
-      const held::Scale s =
-          held::block_scale<KIND == kKeepFp16 ? held::kTop16 : held::kTop8, VEC>(x);
-      if (!live) return;
-      if (n % held::kBlock == 0) scale[m * nblocks + n / held::kBlock] = (uint8_t)s.byte;
-      if constexpr (KIND == kKeepFp16)
-        held::store16<VEC>(v + at, s, x);
-      else
-        held::store<VEC>(v + at, s, x);
+      // (a block's columns past the tensor's do not count for its scale)
+      float w[B][VEC];
+#pragma unroll
+      for (int q = 0; q < B; ++q)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) w[q][k] = ALL || live[q] ? x[q][k] : 0.f;
+      const held::Scales<B> s =
+          held::block_scales<KIND == kKeepFp16 ? held::kTop16 : held::kTop8, VEC, B>(w);
+#pragma unroll
+      for (int q = 0; q < B; ++q) {
+        const float inv = held::inverse_of(s.byte[q]);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) w[q][k] = x[q][k] * inv;
+      }
+      if (KIND == kKeepFp8 && !s.finite) {
+#pragma unroll
+        for (int q = 0; q < B; ++q)
+#pragma unroll
+          for (int k = 0; k < VEC; ++k)
+            w[q][k] = held::finite_or_nan(x[q][k]) * held::inverse_of(s.byte[q]);
+      }
+      const int64_t block = n / held::kBlock;
+      const bool first = n % held::kBlock == 0;
+#pragma unroll
+      for (int q = 0; q < B; ++q) {
+        if (!(ALL || live[q])) continue;
+        if constexpr (KIND == kKeepFp16)
+          store_n<f16, VEC>(v + m[q] * cols + n, w[q]);
+        else
+          held::store<VEC>(v + m[q] * cols + n, w[q]);
+      }
+      if (first) {
+#pragma unroll
+        for (int q = 0; q < B; ++q)
+          if (ALL || live[q]) scale[m[q] * nblocks + block] = (uint8_t)s.byte[q];
+      }
     }
   }
 
@@ -94,21 +124,20 @@ __device__ __forceinline__ void load_pack(const T* p, Pack<T, VEC>& r) {
   }
 }
 
-template <int VEC>
-__device__ __forceinline__ void act_fwd_vec(int act, float (&x)[VEC]) {
+template <int ACT, int VEC, int B>
+__device__ __forceinline__ void act_fwd_all(float (&x)[B][VEC]) {
+#pragma unroll
+  for (int q = 0; q < B; ++q)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) x[q][k] = act_fwd<ACT>(x[q][k]);
+}
+
+template <int VEC, int B>
+__device__ __forceinline__ void act_fwd_vec(int act, float (&x)[B][VEC]) {
   switch (act) {  // uniform
-    case kActSilu:
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] = act_fwd<kActSilu>(x[k]);
-      break;
-    case kActGelu:
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] = act_fwd<kActGelu>(x[k]);
-      break;
-    case kActGeluTanh:
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] = act_fwd<kActGeluTanh>(x[k]);
-      break;
+    case kActSilu: act_fwd_all<kActSilu>(x); break;
+    case kActGelu: act_fwd_all<kActGelu>(x); break;
+    case kActGeluTanh: act_fwd_all<kActGeluTanh>(x); break;
     default: break;
   }
 }
@@ -135,9 +164,11 @@ __device__ __forceinline__ void act_grad_vec(int act, float (&x)[VEC]) {
 }
 
 // A step: column(n) gives what it needs of a lane's columns, fetch(m, n) issues its
-// loads for a position, and finish(...) does the work. Every lane of a block takes part
-// in finish; live says whether this lane's position exists (else what column and fetch
-// gave is not used).
+// loads for a position, and finish(...) does the work for B positions of these columns
+// at once: straight through, so that a wave on its own has B chains of operations to
+// hide latencies in. Every lane of a block takes part in finish; live says whether a
+// lane's position exists (ALL: every one does), else what column and fetch gave of it is
+// not used.
 
 // z = x + bias; y = act(z) + residual; z kept.
 template <typename T, int KIND>
@@ -177,22 +208,25 @@ struct LinearStep {
     return f;
   }
 
-  template <int VEC>
-  __device__ __forceinline__ void finish(int64_t m, int64_t n, float (&x)[VEC],
-                                         const Column<VEC>& c, const Fetched<VEC>& f,
-                                         bool live) const {
-    if (live) {
+  template <bool ALL, int VEC, int B>
+  __device__ __forceinline__ void finish(const int64_t (&m)[B], int64_t n, float (&x)[B][VEC],
+                                         const Column<VEC>& c, const Fetched<VEC> (&f)[B],
+                                         const bool (&live)[B]) const {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] += c.b[k];
-    }
-    z.template put<VEC>(m, n, x, live);
-    if (!live) return;
-    act_fwd_vec<VEC>(act, x);
+    for (int q = 0; q < B; ++q)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) x[q][k] += c.b[k];
+    z.template put<ALL, VEC, B>(m, n, x, live);
+    act_fwd_vec<VEC, B>(act, x);
     if (residual) {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] += to_f32(f.r.v[k]);
+      for (int q = 0; q < B; ++q)
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) x[q][k] += to_f32(f[q].r.v[k]);
     }
-    store_n<T, VEC>(y + m * ldy + n, x);
+#pragma unroll
+    for (int q = 0; q < B; ++q)
+      if (ALL || live[q]) store_n<T, VEC>(y + m[q] * ldy + n, x[q]);
   }
 };
 
@@ -213,16 +247,19 @@ struct GatedStep {
   template <int VEC>
   __device__ __forceinline__ Fetched<VEC> fetch(int64_t, int64_t) const { return {}; }
 
-  template <int VEC>
-  __device__ __forceinline__ void finish(int64_t m, int64_t n, float (&g)[VEC], float (&u)[VEC],
-                                         const Column<VEC>&, const Fetched<VEC>&,
-                                         bool live) const {
-    gate.template put<VEC>(m, n, g, live);
-    up.template put<VEC>(m, n, u, live);
-    if (!live) return;
+  template <bool ALL, int VEC, int B>
+  __device__ __forceinline__ void finish(const int64_t (&m)[B], int64_t n, float (&g)[B][VEC],
+                                         float (&u)[B][VEC], const Column<VEC>&,
+                                         const Fetched<VEC> (&)[B], const bool (&live)[B]) const {
+    gate.template put<ALL, VEC, B>(m, n, g, live);
+    up.template put<ALL, VEC, B>(m, n, u, live);
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) g[k] = swiglu_fwd_elem(g[k], u[k]);
-    store_n<T, VEC>(h + m * cols + n, g);
+    for (int q = 0; q < B; ++q)
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) g[q][k] = swiglu_fwd_elem(g[q][k], u[q][k]);
+#pragma unroll
+    for (int q = 0; q < B; ++q)
+      if (ALL || live[q]) store_n<T, VEC>(h + m[q] * cols + n, g[q]);
   }
 };
 
@@ -249,20 +286,26 @@ struct GatedGradStep {
     return {gate.template fetch<VEC>(m, n), up.template fetch<VEC>(m, n)};
   }
 
-  template <int VEC>
-  __device__ __forceinline__ void finish(int64_t m, int64_t n, float (&dh)[VEC],
-                                         const Column<VEC>&, const Fetched<VEC>& f,
-                                         bool live) const {
-    if (!live) return;
-    float g[VEC], u[VEC], hv[VEC];
-    gate.template decode<VEC>(f.g, g);
-    up.template decode<VEC>(f.u, u);
+  template <bool ALL, int VEC, int B>
+  __device__ __forceinline__ void finish(const int64_t (&m)[B], int64_t n, float (&dh)[B][VEC],
+                                         const Column<VEC>&, const Fetched<VEC> (&f)[B],
+                                         const bool (&live)[B]) const {
+    float g[B][VEC], u[B][VEC];
 #pragma unroll
-    for (int k = 0; k < VEC; ++k)
-      swiglu_bwd_fwd_elem(g[k], u[k], dh[k], g[k], u[k], hv[k]);
-    store_n<T, VEC>(dg + m * cols + n, g);
-    store_n<T, VEC>(du + m * cols + n, u);
-    if (h) store_n<T, VEC>(h + m * cols + n, hv);
+    for (int q = 0; q < B; ++q) {
+      gate.template decode<VEC>(f[q].g, g[q]);
+      up.template decode<VEC>(f[q].u, u[q]);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k)
+        swiglu_bwd_fwd_elem(g[q][k], u[q][k], dh[q][k], g[q][k], u[q][k], dh[q][k]);
+    }
+#pragma unroll
+    for (int q = 0; q < B; ++q) {
+      if (!(ALL || live[q])) continue;
+      store_n<T, VEC>(dg + m[q] * cols + n, g[q]);
+      store_n<T, VEC>(du + m[q] * cols + n, u[q]);
+      if (h) store_n<T, VEC>(h + m[q] * cols + n, dh[q]);
+    }
   }
 };
 
@@ -285,13 +328,15 @@ struct ValuesStep {
     return v.template fetch<VEC>(m, n);
   }
 
-  template <int VEC>
-  __device__ __forceinline__ void finish(int64_t m, int64_t n, float (&x)[VEC],
-                                         const Column<VEC>&, const Fetched<VEC>& f,
-                                         bool live) const {
-    if (!live) return;
-    v.template decode<VEC>(f, x);
-    store_n<T, VEC>(out + m * cols + n, x);
+  template <bool ALL, int VEC, int B>
+  __device__ __forceinline__ void finish(const int64_t (&m)[B], int64_t n, float (&x)[B][VEC],
+                                         const Column<VEC>&, const Fetched<VEC> (&f)[B],
+                                         const bool (&live)[B]) const {
+#pragma unroll
+    for (int q = 0; q < B; ++q) {
+      v.template decode<VEC>(f[q], x[q]);
+      if (ALL || live[q]) store_n<T, VEC>(out + m[q] * cols + n, x[q]);
+    }
   }
 };
 
@@ -382,10 +427,15 @@ __global__ __launch_bounds__(kThreads) void rows_kernel(const Src src, const Src
     }
 #pragma unroll
     for (int k = 0; k < kInFlight; ++k) {
+      const int64_t mk[1] = {m[k]};
+      const bool lk[1] = {live[k]};
+      float(&xk)[1][VEC] = reinterpret_cast<float(&)[1][VEC]>(x[k]);
+      typename Step::template Fetched<VEC> fk[1] = {f[k]};
       if constexpr (kTwo)
-        step.template finish<VEC>(m[k], n[k], x[k], u[k], c[k], f[k], live[k]);
+        step.template finish<false, VEC, 1>(mk, n[k], xk, reinterpret_cast<float(&)[1][VEC]>(u[k]),
+                                            c[k], fk, lk);
       else
-        step.template finish<VEC>(m[k], n[k], x[k], c[k], f[k], live[k]);
+        step.template finish<false, VEC, 1>(mk, n[k], xk, c[k], fk, lk);
     }
   }
 }

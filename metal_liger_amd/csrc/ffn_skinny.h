@@ -171,19 +171,21 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(
     const bool live = m < p.M && n < p.N && q < kPositions;
     const int row = q < kPositions ? m : 0;
     typename Step::template Column<8> column;
-    typename Step::template Fetched<8> f;
+    typename Step::template Fetched<8> f[1];
     if (live) {
       column = step.template column<8>(n);
-      f = step.template fetch<8>(m, n);
+      f[0] = step.template fetch<8>(m, n);
     }
-    float x[8];
-    load_n<float, 8>(&fin[0][row][c], x);
+    float x[1][8];
+    load_n<float, 8>(&fin[0][row][c], x[0]);
+    const int64_t ms[1] = {m};
+    const bool lives[1] = {live};
     if constexpr (PAIR) {
-      float u[8];
-      load_n<float, 8>(&fin[1][row][c], u);
-      step.template finish<8>(m, n, x, u, column, f, live);
+      float u[1][8];
+      load_n<float, 8>(&fin[1][row][c], u[0]);
+      step.template finish<false, 8, 1>(ms, n, x, u, column, f, lives);
     } else {
-      step.template finish<8>(m, n, x, column, f, live);
+      step.template finish<false, 8, 1>(ms, n, x, column, f, lives);
     }
   }
 }

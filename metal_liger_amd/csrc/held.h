@@ -58,32 +58,45 @@ __device__ __forceinline__ uint32_t lanes_max(uint32_t m) {
   return m;
 }
 
-// A block's scale, as the 32 / VEC neighbouring lanes that hold VEC elements of it each
-// find it, and whether all of a lane's own elements are finite (they nearly always are:
-// the search for the largest finite one is then 1.5 operations an element).
-struct Scale {
-  uint32_t byte;
+// Scales of B blocks, as the 32 / VEC neighbouring lanes that hold VEC elements of each
+// find them, and whether all of a lane's own elements are finite. They nearly always
+// are: the search for the largest finite one is then 1.5 operations an element, and one
+// branch for all B blocks.
+template <int B>
+struct Scales {
+  uint32_t byte[B];
   bool finite;
 };
 
-template <int TOP, int VEC>
-__device__ __forceinline__ Scale block_scale(const float (&v)[VEC]) {
-  uint32_t m = 0;
+template <int TOP, int VEC, int B>
+__device__ __forceinline__ Scales<B> block_scales(const float (&v)[B][VEC]) {
+  uint32_t m[B], all = 0;
 #pragma unroll
-  for (int k = 0; k < VEC; ++k) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, v[k]) & 0x7FFFFFFFu;
-    m = m > b ? m : b;
-  }
-  const bool finite = m < 0x7F800000u;
-  if (!finite) {
-    m = 0;
+  for (int q = 0; q < B; ++q) {
+    m[q] = 0;
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
-      const uint32_t b = finite_bits(v[k]);
-      m = m > b ? m : b;
+      const uint32_t b = __builtin_bit_cast(uint32_t, v[q][k]) & 0x7FFFFFFFu;
+      m[q] = m[q] > b ? m[q] : b;
+    }
+    all = all > m[q] ? all : m[q];
+  }
+  Scales<B> s;
+  s.finite = all < 0x7F800000u;
+  if (!s.finite) {
+#pragma unroll
+    for (int q = 0; q < B; ++q) {
+      m[q] = 0;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        const uint32_t b = finite_bits(v[q][k]);
+        m[q] = m[q] > b ? m[q] : b;
+      }
     }
   }
-  return {scale_byte<TOP>(lanes_max<kBlock / VEC>(m)), finite};
+#pragma unroll
+  for (int q = 0; q < B; ++q) s.byte[q] = scale_byte<TOP>(lanes_max<kBlock / VEC>(m[q]));
+  return s;
 }
 
 __device__ __forceinline__ float finite_or_nan(float v) {
@@ -95,17 +108,10 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xFFFFu;
 }
 
-// VEC elements to q (VEC bytes, aligned to VEC), by the block's scale.
+// VEC elements to q (VEC bytes, aligned to VEC), already divided by their scale and with
+// NaN for what is not finite.
 template <int VEC>
-__device__ __forceinline__ void store(uint8_t* q, const Scale& s, const float (&v)[VEC]) {
-  const float inv = inverse_of(s.byte);
-  float x[VEC];
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) x[k] = v[k] * inv;
-  if (!s.finite) {
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) x[k] = finite_or_nan(v[k]) * inv;
-  }
+__device__ __forceinline__ void store(uint8_t* q, const float (&x)[VEC]) {
   if constexpr (VEC == 1) {
     *q = (uint8_t)pack2(x[0], 0.f);
   } else {
@@ -140,16 +146,7 @@ __device__ __forceinline__ void load(const uint32_t* w, uint32_t byte, float (&v
   }
 }
 
-// The same in 16 bits (q aligned to 2 VEC bytes).
-template <int VEC>
-__device__ __forceinline__ void store16(f16* q, const Scale& s, const float (&v)[VEC]) {
-  const float inv = inverse_of(s.byte);
-  float w[VEC];
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) w[k] = v[k] * inv;
-  store_n<f16, VEC>(q, w);
-}
-
+// VEC elements of the fp16 bits in w.
 template <int VEC>
 __device__ __forceinline__ void load16(const uint32_t* w, uint32_t byte, float (&v)[VEC]) {
   const float s = scale_of(byte);

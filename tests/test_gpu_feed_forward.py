@@ -388,3 +388,22 @@ def test_mlp_few_rows(dev, dtype, M, H, I, O):  # noqa: E741
         bound = bound + V * want.abs()
     keep = want.abs() < 65000
     _check(torch.where(keep.to(dev), y, 0), torch.where(keep, want, 0.0), torch.where(keep, bound, 0.0), "y")
+
+
+@pytest.mark.parametrize("M", [5, 200])
+@pytest.mark.parametrize("N", [8, 40, 72, 136])
+def test_scales_of_short_blocks(dev, M, N):
+    """A bias that cancels most of the sums: the scales of a row's last, short block go by
+    its own columns alone."""
+    from metal_liger_amd import hip_ops
+    K = 64
+    x, w, b, _, _ = _linear_case(M, K, N, torch.bfloat16, True, False, dev)
+    x, w = torch.ones_like(x), torch.ones_like(w)
+    b = torch.full_like(b, -float(K)) + b.detach() * 2.0 ** -6
+    for keep in (hip_ops.KEEP_FP16, hip_ops.KEEP_FP8):
+        _, v, s = hip_ops.linear_fwd(x, w, b, None, 1, keep)
+        z = K + _cpu(b).expand(M, N)  # exact in fp32
+        e = ref.held_exponents(z) - (7 if keep == hip_ops.KEEP_FP16 else 0)
+        assert torch.equal(s.cpu().long() - 127, e.clamp_min(-126))
+        half = z.abs() * (2.0 ** -11 if keep == hip_ops.KEEP_FP16 else 2.0 ** -4) + 2.0 ** -30
+        assert bool(((ref.held_values(v.cpu(), s.cpu()) - z).abs() <= half).all())
