@@ -121,19 +121,19 @@ struct Products<bf16> {
   static int through(int64_t M, int64_t N, int64_t K, const bf16* a, int64_t lda, const bf16* b,
                      int64_t ldb, const Step& step, hipStream_t st) {
     const gemm::Segment s{{a, lda}, {b, ldb}, (int)K};
-    return plan(M, N, K).tile == 128
+    return step_tile(step.cost(), M, N, K) == 128
                ? launch_product<gemm::R4SCfg, LB, false>(M, N, s, gemm::Operand{}, step, st)
                : launch_product<gemm::R4Cfg, LB, false>(M, N, s, gemm::Operand{}, step, st);
   }
 
-  // Both of a's products, with b [N, K] and b2 [N, K]: a plan for 2 N columns.
+  // Both of a's products, with b [N, K] and b2 [N, K].
   template <class Step>
   static int through_pair(int64_t M, int64_t N, int64_t K, const bf16* a, int64_t lda,
                           const bf16* b, int64_t ldb, const bf16* b2, int64_t ldb2,
                           const Step& step, hipStream_t st) {
     const gemm::Segment s{{a, lda}, {b, ldb}, (int)K};
     const gemm::Operand o{b2, ldb2};
-    return plan(M, 2 * N, K).tile == 128
+    return step_tile(step.cost(), M, 2 * N, K) == 128
                ? launch_product<gemm::R4SCfg, kKMajor, true>(M, N, s, o, step, st)
                : launch_product<gemm::R4Cfg, kKMajor, true>(M, N, s, o, step, st);
   }

@@ -97,6 +97,49 @@ struct Stager {
   }
 };
 
+// The tile of a product that carries a step: 256 x 256, or 128 x 128, of which two
+// workgroups share a CU, so that one's epilogue runs beside the other's products. Which
+// is faster goes by the rounds of tiles, K and the step. Times in us on one MI355X,
+// fitted to 152 products each way (rows 130 .. 8192, columns and K 1024 .. 6144; off by
+// 2.5-8%; the choice it makes was at most 6% slower than the better tile, 0.2% on
+// average, that of the plain products' estimate up to 31%: [8192, 1152] x 4304 with
+// gelu_tanh 134 us as 256 x 256 tiles, 102 as 128 x 128; [8192, 2048] x 6144 with both
+// of the gated block's products 338 and 436):
+//   256: a whole round of 256 tiles of kt 64-wide k-tiles c0 + c1 kt, a partial one of r
+//        c2 + c3 kt + (c4 + c5 kt) r / 256
+//   128: a whole round of 512 c0 + c1 kt, a partial one c2 + c3 kt, and where it has
+//        more than one tile a CU c4 + c5 kt besides
+inline double step_us(int tile, int kind, int64_t items, int kt) {
+  static const double k256[4][6] = {{12.4, 1.40, 13.3, 1.05, 7.1, 0.11},
+                                    {22.7, 1.37, 21.4, 1.11, 8.9, 0.01},
+                                    {10.7, 1.40, 14.3, 1.10, 3.9, 0.21},
+                                    {38.8, 1.27, 21.9, 1.11, 0.3, 0.38}};
+  static const double k128[4][6] = {{0.0, 0.99, 5.6, 0.49, 1.4, 0.32},
+                                    {4.5, 0.95, 8.2, 0.49, 1.4, 0.37},
+                                    {4.2, 0.88, 7.1, 0.50, 2.1, 0.32},
+                                    {17.2, 0.81, 9.2, 0.49, 7.3, 0.17}};
+  const double* c = tile == 256 ? k256[kind] : k128[kind];
+  const int64_t round = tile == 256 ? 256 : 512, full = items / round, rem = items % round;
+  double t = full * (c[0] + c[1] * kt);
+  if (rem) {
+    t += c[2] + c[3] * kt;
+    if (tile == 256) t += (c[4] + c[5] * kt) * rem / 256;
+    else if (rem > 256) t += c[4] + c[5] * kt;
+  }
+  return t;
+}
+
+// columns: of both products of a pair together
+inline int step_tile(int kind, int64_t M, int64_t columns, int64_t K) {
+  const int kt = (int)((K + gemm::kBK - 1) / gemm::kBK);
+  double us[2];
+  for (int i = 0; i < 2; ++i) {
+    const int64_t t = i ? 128 : 256;
+    us[i] = step_us((int)t, kind, ((M + t - 1) / t) * ((columns + t - 1) / t), kt);
+  }
+  return us[0] <= us[1] ? 256 : 128;
+}
+
 // C: R4Cfg or R4SCfg; b2: the second operand of a pair.
 template <class C, int LB, bool PAIR, class Step>
 __global__ __launch_bounds__(C::THREADS) void product_kernel(const gemm::Problem pb,

@@ -142,24 +142,20 @@ __device__ __forceinline__ void act_fwd_vec(int act, float (&x)[B][VEC]) {
   }
 }
 
-template <int VEC>
-__device__ __forceinline__ void act_grad_vec(int act, float (&x)[VEC]) {
+template <int ACT, int VEC, int B>
+__device__ __forceinline__ void act_grad_all(float (&x)[B][VEC]) {
+#pragma unroll
+  for (int q = 0; q < B; ++q)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) x[q][k] = act_grad<ACT>(x[q][k]);
+}
+
+template <int VEC, int B>
+__device__ __forceinline__ void act_grad_vec(int act, float (&x)[B][VEC]) {
   switch (act) {
-    case kActSilu:
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] = act_grad<kActSilu>(x[k]);
-      break;
-    case kActGelu:
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] = act_grad<kActGelu>(x[k]);
-      break;
-    case kActGeluTanh:
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] = act_grad<kActGeluTanh>(x[k]);
-      break;
-    default:
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) x[k] = 1.f;
+    case kActSilu: act_grad_all<kActSilu>(x); break;
+    case kActGelu: act_grad_all<kActGelu>(x); break;
+    default: act_grad_all<kActGeluTanh>(x); break;
   }
 }
 
@@ -170,6 +166,9 @@ __device__ __forceinline__ void act_grad_vec(int act, float (&x)[VEC]) {
 // lane's position exists (ALL: every one does), else what column and fetch gave of it is
 // not used.
 
+// cost: which of the times measured with products it goes by (ffn_product.h).
+enum : int { kPlainStep, kActStep, kPairStep, kGradStep };
+
 // z = x + bias; y = act(z) + residual; z kept.
 template <typename T, int KIND>
 struct LinearStep {
@@ -179,6 +178,8 @@ struct LinearStep {
   int64_t ldr, ldy;
   int act;
   Kept<KIND> z;
+
+  int cost() const { return act == kActNone && KIND == kKeepNone ? kPlainStep : kActStep; }
 
   template <int VEC>
   struct Column {
@@ -237,6 +238,8 @@ struct GatedStep {
   int64_t cols;
   Kept<KIND> gate, up;
 
+  int cost() const { return kPairStep; }
+
   template <int VEC>
   struct Column {};
   template <int VEC>
@@ -271,6 +274,8 @@ struct GatedGradStep {
   T* h;  // or null
   int64_t cols;
   Kept<KIND> gate, up;
+
+  int cost() const { return kGradStep; }
 
   template <int VEC>
   struct Column {};
@@ -487,19 +492,32 @@ __global__ __launch_bounds__(kThreads) void linear_grad_kernel(
 #pragma unroll
   for (int k = 0; k < VEC; ++k) sum[k] = 0.f;
   if (live) {
-    for (int64_t m = r0 + rl; m < r1; m += 8) {
-      float d[VEC];
-      load_n<T, VEC>(dy + m * ldy + n, d);
-      if constexpr (KIND != kKeepNone) {
-        float v[VEC];
-        z.template decode<VEC>(z.template fetch<VEC>(m, n), v);
-        act_grad_vec<VEC>(act, v);
+    constexpr int B = VEC == 8 && sizeof(T) == 2 ? 4 : 2;  // rows of a lane in flight
+    for (int64_t m0 = r0 + rl; m0 < r1; m0 += 8 * B) {
+      float d[B][VEC], v[B][VEC];
+      typename Kept<KIND>::template Raw<VEC> raw[B];
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) d[k] *= v[k];
+      for (int q = 0; q < B; ++q) {  // (rows past the range: the first one's again)
+        const int64_t m = m0 + 8 * q < r1 ? m0 + 8 * q : m0;
+        load_n_nt<T, VEC>(dy + m * ldy + n, d[q]);
+        if constexpr (KIND != kKeepNone) raw[q] = z.template fetch<VEC>(m, n);
       }
-      if (dz) store_n<T, VEC>(dz + m * cols + n, d);
+      if constexpr (KIND != kKeepNone) {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) sum[k] += d[k];
+        for (int q = 0; q < B; ++q) z.template decode<VEC>(raw[q], v[q]);
+        act_grad_vec<VEC, B>(act, v);
+      }
+#pragma unroll
+      for (int q = 0; q < B; ++q) {
+        if (m0 + 8 * q >= r1) break;
+        if constexpr (KIND != kKeepNone) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) d[q][k] *= v[q][k];
+        }
+        if (dz) store_n<T, VEC>(dz + (m0 + 8 * q) * cols + n, d[q]);
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) sum[k] += d[q][k];
+      }
     }
   }
   if (!partial) return;
