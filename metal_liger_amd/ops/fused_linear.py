@@ -9,9 +9,10 @@ rounds finer than bf16; in fp32 where the products run in fp32), or in 8 (checkp
 "fp8": e4m3 with such scales), formed of the fp32 sums. What is not needed (x where the
 weight is frozen, W where x needs no gradient) is not kept. First derivatives only.
 
-bf16 with sizes in multiples of 8 runs on the bf16 matrix cores, as fp16 does in forwards
-of up to 64 rows that keep nothing, everything else on the fp32 ones (fp16 and other bf16
-sizes are upcast, and rounded once at the end).
+bf16 runs on the bf16 matrix cores (whose kernels take sizes in multiples of 8: others are
+padded with zeros, which add nothing), as fp16 with such sizes does in forwards of up to
+64 rows that keep nothing; fp32, and fp16 elsewhere (upcast, and rounded once at the end),
+on the fp32 ones.
 """
 
 from __future__ import annotations
@@ -45,20 +46,45 @@ def keep_mode(checkpoint: str | None, dtype: torch.dtype) -> int:
 
 
 def compute_dtype(x: torch.Tensor, *features: int, infer: bool = False) -> torch.dtype:
-    """bf16 where its matrix-core kernels take the sizes, fp16 in forwards of few rows
-    with nothing to keep (infer), else fp32."""
-    if x.dtype != torch.float32 and all(f % 8 == 0 for f in features):
-        if x.dtype == torch.bfloat16:
-            return x.dtype
-        if infer and x.numel() <= hip_ops.FEW_ROWS * x.shape[-1]:
-            return x.dtype
+    """bf16 for bf16, fp16 in forwards of few rows with nothing to keep (infer) and sizes
+    in multiples of 8, else fp32."""
+    if x.dtype == torch.bfloat16 or (
+            infer and x.dtype == torch.float16 and x.numel() <= hip_ops.FEW_ROWS * x.shape[-1]
+            and all(f % 8 == 0 for f in features)):
+        return x.dtype
     return torch.float32
 
 
+def padded(n: int, dtype: torch.dtype) -> int:
+    """A feature size as the products of dtype take it."""
+    return n if dtype == torch.float32 else -(-n // 8) * 8
+
+
+def pad(t, dim: int, dtype: torch.dtype):
+    """t's dimension at the size padded gives, with zeros."""
+    if t is None or t.shape[dim] % 8 == 0 or dtype == torch.float32:
+        return t
+    shape = list(t.shape)
+    shape[dim] = padded(shape[dim], dtype)
+    out = t.new_zeros(shape)
+    out.narrow(dim, 0, t.shape[dim]).copy_(t)
+    return out
+
+
+def cut(t: torch.Tensor, *sizes: int) -> torch.Tensor:
+    """A result at its sizes without the padding, dense."""
+    return t if tuple(t.shape) == sizes else t[tuple(slice(n) for n in sizes)].contiguous()
+
+
 def rows(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """[..., C] -> [R, C] in dtype."""
+    """[..., C] -> [R, C] in dtype, C padded."""
     t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    return t if t.dtype == dtype else t.to(dtype)
+    return pad(t if t.dtype == dtype else t.to(dtype), 1, dtype)
+
+
+def weight_as(t, dtype: torch.dtype):
+    """A weight in dtype, both sizes padded."""
+    return None if t is None else pad(rows(t, dtype), 0, dtype)
 
 
 def check_input(what: str, x: torch.Tensor, *weights: torch.Tensor) -> None:
@@ -89,9 +115,11 @@ def _forward(x, weight, bias, residual, act: int, keep: int):
     """(y, z, zscale), or y alone where nothing is kept."""
     none = keep == hip_ops.KEEP_NONE
     ct = compute_dtype(x, *weight.shape, infer=none)
-    args = (rows(x, ct), rows(weight, ct), bias if bias is None or bias.dtype == ct else bias.to(ct),
+    bias = bias if bias is None or bias.dtype == ct else bias.to(ct)
+    args = (rows(x, ct), weight_as(weight, ct), pad(bias, 0, ct),
             None if residual is None else rows(residual, ct), act)
     y, *kept = (cops.linear_infer(*args),) if none else cops.linear_fwd(*args, keep)
+    y = cut(y, y.shape[0], weight.shape[0])
     if y.dtype != x.dtype:
         y = y.to(x.dtype)
     if x.dim() != 2:
@@ -119,13 +147,15 @@ class _FusedLinearFunction(torch.autograd.Function):
             x, weight, *kept = ctx.saved_tensors
             z, zscale = kept or (None, None)
             N, K = ctx.sizes
-            g = rows(dy, compute_dtype(dy, N, K))
-            out = cops.linear_bwd(None if x is None else rows(x, g.dtype),
-                                  None if weight is None else rows(weight, g.dtype), g, ctx.act,
-                                  ctx.keep, z, zscale, N, K, need_dx, need_dw, need_db)
+            ct = compute_dtype(dy, N, K)
+            out = cops.linear_bwd(None if x is None else rows(x, ct), weight_as(weight, ct),
+                                  rows(dy, ct), ctx.act, ctx.keep, z, zscale, padded(N, ct),
+                                  padded(K, ct), need_dx, need_dw, need_db)
+            sizes = ((ctx.x_shape.numel() // K, K), (N, K), (N,))
             for i, need in enumerate((need_dx, need_dw, need_db)):
                 if need:
-                    grads[i] = out[i] if out[i].dtype == ctx.dtype else out[i].to(ctx.dtype)
+                    g = cut(out[i], *sizes[i])
+                    grads[i] = g if g.dtype == ctx.dtype else g.to(ctx.dtype)
             if need_dx and len(ctx.x_shape) != 2:
                 grads[0] = grads[0].view(ctx.x_shape)
         return (*grads, dy if need_dr else None, None, None)

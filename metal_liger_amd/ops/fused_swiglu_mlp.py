@@ -21,8 +21,8 @@ from metal_liger_amd import _custom_ops as cops
 from metal_liger_amd import hip_ops
 from metal_liger_amd._model_walk import find_layers
 from metal_liger_amd.ops.fused_linear import (check_checkpoint, check_input, check_residual,
-                                              compute_dtype, keep_mode, plain_linear, rows,
-                                              runs_fused, wants_grad)
+                                              compute_dtype, cut, keep_mode, plain_linear, rows,
+                                              runs_fused, wants_grad, weight_as)
 from metal_liger_amd.ops.fused_swiglu import MetalLigerSwiGLU
 
 logger = logging.getLogger(__name__)
@@ -33,9 +33,10 @@ def _forward(x, weights, residual, keep: int):
     O, I = weights[2].shape  # noqa: E741
     none = keep == hip_ops.KEEP_NONE
     ct = compute_dtype(x, x.shape[-1], I, O, infer=none)
-    args = (rows(x, ct), *(rows(w, ct) for w in weights),
+    args = (rows(x, ct), *(weight_as(w, ct) for w in weights),
             None if residual is None else rows(residual, ct))
     y, *kept = (cops.swiglu_mlp_infer(*args),) if none else cops.swiglu_mlp_fwd(*args, keep)
+    y = cut(y, y.shape[0], O)
     if y.dtype != x.dtype:
         y = y.to(x.dtype)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], O), *kept
@@ -57,10 +58,11 @@ class _FusedSwiGLUMLPFunction(torch.autograd.Function):
         if any(ctx.needs_input_grad[:4]):
             x, wg, wu, wd, *kept = ctx.saved_tensors
             ct = compute_dtype(x, x.shape[-1], *wd.shape)
-            outs = cops.swiglu_mlp_bwd(*(rows(t, ct) for t in (x, wg, wu, wd, dy)), ctx.keep, *kept,
-                                       *ctx.needs_input_grad[:4])
-            grads = [(g if g.dtype == x.dtype else g.to(x.dtype)) if need else None
-                     for g, need in zip(outs, ctx.needs_input_grad)]
+            outs = cops.swiglu_mlp_bwd(rows(x, ct), *(weight_as(w, ct) for w in (wg, wu, wd)),
+                                       rows(dy, ct), ctx.keep, *kept, *ctx.needs_input_grad[:4])
+            sizes = ((x.numel() // x.shape[-1], x.shape[-1]), wg.shape, wu.shape, wd.shape)
+            grads = [cut(g, *n).to(x.dtype) if need else None
+                     for g, n, need in zip(outs, sizes, ctx.needs_input_grad)]
             if grads[0] is not None and x.dim() != 2:
                 grads[0] = grads[0].view(x.shape)
         return (*grads, dy if ctx.needs_input_grad[4] else None, None)

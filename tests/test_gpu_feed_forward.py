@@ -30,7 +30,7 @@ def _u(dtype):
 
 def _matrix_cores(dtype, *sizes):
     """Whether the products read bf16 (else everything between input and output is fp32)."""
-    return dtype == torch.bfloat16 and all(s % 8 == 0 for s in sizes)
+    return dtype == torch.bfloat16
 
 
 def _cpu(t):
@@ -57,12 +57,13 @@ def _act_noise(z):
     return 32 * V * (z.abs() + 1)
 
 
-def _kept(saved, i, checkpoint):
-    """The i-th kept tensor of an autograd node's saved ones, as its backward reads it."""
+def _kept(saved, i, checkpoint, cols):
+    """The i-th kept tensor of an autograd node's saved ones, as its backward reads it
+    (without the columns that pad it)."""
     v, s = saved[i:i + 2]
     if checkpoint is None and v.dtype == torch.float32:
-        return _cpu(v)
-    return ref.held_values(v.cpu(), s.cpu())
+        return _cpu(v)[:, :cols]
+    return ref.held_values(v.cpu(), s.cpu())[:, :cols]
 
 
 # ------------------------------------------------------------------- linear --
@@ -98,7 +99,7 @@ def _linear_check(x, w, b, r, dy, act, checkpoint, call):
     if act is None:
         dz, edz = D, torch.zeros_like(D)
     else:
-        zk = _kept(saved, 2, checkpoint)
+        zk = _kept(saved, 2, checkpoint, N)
         err = (zk - z).abs()
         if checkpoint == "fp8":
             e = torch.ldexp(torch.ones((), dtype=torch.float64), ref.held_exponents(z))
@@ -184,8 +185,8 @@ def _mlp_check(x, ws, r, dy, checkpoint, call):
         want = want + _cpu(r)
         bound = bound + V * want.abs()
     _check(y, want, bound, "y")
-    gk = _kept(saved, 4, checkpoint)
-    uk = _kept(saved, 6, checkpoint)
+    gk = _kept(saved, 4, checkpoint, I)
+    uk = _kept(saved, 6, checkpoint, I)
     for k, z, e in ((gk, g, eg), (uk, u, eu)):
         if checkpoint == "fp8":
             s = torch.ldexp(torch.ones((), dtype=torch.float64), ref.held_exponents(z))
