@@ -641,12 +641,14 @@ int ml_gemm_f32_segments_ws(int64_t M, int64_t N, int nseg, const int64_t* k_len
 /* ------------------------------------------------------------ feed-forward
  * Linear layers with what surrounds them, and the gated block, forward and
  * backward (no reference counterpart: its models keep nn.Linear, and its SwiGLU
- * fuses the activation step only, ops/fused_swiglu.py:59-75). dtype ML_F32 or
- * ML_BF16; bf16 operands of a product have 16-byte aligned bases, and columns and
- * row strides in multiples of 8.
+ * fuses the activation step only, ops/fused_swiglu.py:59-75). bf16 and fp16 operands
+ * have 16-byte aligned bases, and columns and row strides in multiples of 8, strides up
+ * to 2^21; fp32 ones may have any (and run fastest with these). bf16 is rounded to bf16
+ * between two products, fp16 to fp32.
  *
  * What a backward needs of its forward's inner tensors is kept as `keep` says, dense
- * [rows, cols]: ML_KEEP_F32, in fp32; ML_KEEP_FP16 and ML_KEEP_FP8, in 2 or 1 bytes an
+ * [rows, cols]: ML_KEEP_F32 (fp32 alone), in fp32; ML_KEEP_FP16 (bf16 and fp16) and
+ * ML_KEEP_FP8, in 2 or 1 bytes an
  * element and one scale byte for every 32 columns of a row [rows, ceil(cols / 32)]: with
  * e = max(floor(log2 m) - 14, -126) (FP8: - 7) for the largest finite magnitude m of the
  * 32 (m = 0: -126) the scale's byte is e + 127, an element's bits are fp16 (e4m3) of
@@ -690,7 +692,7 @@ int ml_linear_bwd(const void* x, int64_t ldx, const void* w, int64_t ldw, const 
 /*
  *   g = x Wg^T, u = x Wu^T, h = silu(g) u, y = h Wd^T + residual
  * x [M, H], Wg and Wu [I, H], Wd [O, I], residual [M, O] or NULL, y [M, O] dense;
- * g and u kept as keep says. h is rounded to dtype between the products.
+ * g and u kept as keep says.
  */
 size_t ml_swiglu_mlp_fwd_workspace_bytes(int64_t M, int64_t H, int64_t I, int64_t O, int dtype);
 int ml_swiglu_mlp_fwd(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu,
@@ -702,7 +704,7 @@ int ml_swiglu_mlp_fwd(const void* x, int64_t ldx, const void* wg, int64_t ldg, c
 /*
  * Its backward, of dy [M, O] (ldy) and the kept g and u: dx [M, H], dwg and dwu
  * [I, H], dwd [O, I], each dense, or NULL where it is not wanted. h is formed again
- * of the kept g and u; dg, du and h are rounded to dtype between the products.
+ * of the kept g and u.
  */
 size_t ml_swiglu_mlp_bwd_workspace_bytes(int64_t M, int64_t H, int64_t I, int64_t O, int dtype);
 int ml_swiglu_mlp_bwd(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu,

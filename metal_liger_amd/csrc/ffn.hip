@@ -9,10 +9,12 @@
 //           dh = dy Wd, dg = dh u silu'(g), du = dh silu(g),
 //           dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
 //
-// bf16 runs on the bf16 matrix cores (gemm_core.h), fp32 on the fp32 ones; forwards of
-// up to 64 rows on kernels of their own (ffn_skinny.h), which take fp16 as well.
+// bf16 runs on the bf16 matrix cores (gemm_core.h), fp32 and fp16 on the fp32 ones
+// (ffn_f32.h; what lies between fp16's products is fp32); forwards of up to 64 rows on
+// kernels of their own (ffn_skinny.h).
 #include <initializer_list>
 
+#include "ffn_f32.h"
 #include "ffn_product.h"
 #include "ffn_skinny.h"
 #include "ffn_wgrad.h"
@@ -43,6 +45,9 @@ size_t larger(size_t a, size_t b) { return a > b ? a : b; }
 
 bool aligned_rows(const void* p, int64_t ld) { return !p || (aligned16(p) && ld % 8 == 0); }
 
+// A tile's rows are addressed by 32-bit offsets: at most 256 rows of bf16 or 128 of fp32.
+constexpr int64_t kMaxStride = 1 << 21;
+
 struct Checked {
   const void* p;
   int64_t ld, cols;
@@ -52,25 +57,35 @@ struct Checked {
 // 16-bit operands of a product and its step.
 int check_operands(std::initializer_list<Checked> list) {
   for (const Checked& c : list)
-    ML_CHECK(aligned16(c.p) && c.ld % 8 == 0 && c.cols % 8 == 0,
+    ML_CHECK(aligned16(c.p) && c.ld % 8 == 0 && c.cols % 8 == 0 && c.ld <= kMaxStride,
              "ffn: 16-bit %s needs a 16-byte aligned base, and columns and row stride in multiples "
-             "of 8 (%lld, %lld)", c.what, (long long)c.cols, (long long)c.ld);
-  return ML_OK;
-}
-
-int check_half(int64_t M, int keep) {
-  ML_CHECK(M <= kSkinnyRows && keep == kKeepNone,
-           "ffn: fp16 runs for up to %d rows with nothing kept (got %lld, keep %d)", kSkinnyRows,
-           (long long)M, keep);
+             "of 8, up to %lld (%lld, %lld)", c.what, (long long)kMaxStride, (long long)c.cols,
+             (long long)c.ld);
   return ML_OK;
 }
 
 int ktiles(int64_t k) { return (int)((k + gemm::kBK - 1) / gemm::kBK); }
 
+// What lies between two products: bf16 as it is, fp32 for fp32 and fp16 (whose range h
+// and the gradients of gate, up and z may leave).
+template <typename T>
+using Inner = std::conditional_t<std::is_same_v<T, bf16>, bf16, float>;
+
+// A weight's gradient C = A^T B, A [K, M], B [K, N]; either may be of the inner type.
+struct Wgrad {
+  int64_t M, N;
+  const void *a, *b;
+  int64_t lda, ldb;
+  void* c;  // dense
+  bool a_inner, b_inner;
+};
+
 // The products of each type.
-//   raw:    fp32 sums [splits][M][N] of A B^T (B [N, K]) or A B (B [K, N], b_mn)
-//   store:  sum over segments of A_s B_s (B [K_s, N]), rounded to T
-//   wgrads: A^T B (A [K, M], B [K, N]) of up to three products of one K, rounded to T
+//   raw:     fp32 sums [splits][M][N] of A B^T (B [N, K]) or A B (LB kMNMajor: B [K, N])
+//   store:   sum over segments of A_s B_s (B [K_s, N]), rounded to T
+//   wgrads:  A^T B of up to three products of one K, rounded to T
+// and, where K is not split, a product with its step as its epilogue:
+//   through, through_pair
 template <typename T>
 struct Products;
 
@@ -85,36 +100,28 @@ struct Products<bf16> {
     return (size_t)plan(M, N, K).ksplit * M * N;
   }
 
-  template <class CF>
-  static int raw_cfg(int64_t M, int64_t N, const gemm::Segment& s, bool b_mn, int ksplit,
-                     float* out, int& splits, hipStream_t st) {
+  template <class CF, int LB>
+  static int raw_cfg(int64_t M, int64_t N, const gemm::Segment& s, int ksplit, float* out,
+                     int& splits, hipStream_t st) {
     gemm::Problem pb;
-    const int rc = gemm::make_problem<CF>(pb, (int)M, (int)N, 1, &s, kKMajor,
-                                          b_mn ? kMNMajor : kKMajor, 0, ksplit);
+    const int rc = gemm::make_problem<CF>(pb, (int)M, (int)N, 1, &s, kKMajor, LB, 0, ksplit);
     if (rc) return rc;
     splits = pb.ksplit;
-    const gemm::EpiPartial epi{out, pb.M, pb.N};
-    const dim3 grid(gemm::grid_blocks(pb));
-    if (b_mn)
-      gemm::gemm_kernel<CF, kKMajor, kMNMajor, gemm::EpiPartial><<<grid, CF::THREADS, 0, st>>>(pb, epi);
-    else
-      gemm::gemm_kernel<CF, kKMajor, kKMajor, gemm::EpiPartial><<<grid, CF::THREADS, 0, st>>>(pb, epi);
+    gemm::gemm_kernel<CF, kKMajor, LB, gemm::EpiPartial>
+        <<<dim3(gemm::grid_blocks(pb)), CF::THREADS, 0, st>>>(pb, gemm::EpiPartial{out, pb.M, pb.N});
     ML_LAUNCH_CHECK();
     return ML_OK;
   }
 
+  template <int LB>
   static int raw(int64_t M, int64_t N, int64_t K, const bf16* a, int64_t lda, const bf16* b,
-                 int64_t ldb, bool b_mn, float* out, int& splits, hipStream_t st) {
+                 int64_t ldb, float* out, int& splits, hipStream_t st) {
     const gemm::Segment s{{a, lda}, {b, ldb}, (int)K};
     const gemm::Plan p = plan(M, N, K);
-    return p.tile == 128 ? raw_cfg<gemm::R4SCfg>(M, N, s, b_mn, p.ksplit, out, splits, st)
-                         : raw_cfg<gemm::R4Cfg>(M, N, s, b_mn, p.ksplit, out, splits, st);
+    return p.tile == 128 ? raw_cfg<gemm::R4SCfg, LB>(M, N, s, p.ksplit, out, splits, st)
+                         : raw_cfg<gemm::R4Cfg, LB>(M, N, s, p.ksplit, out, splits, st);
   }
 
-  // Whether a product of M rows needs no workspace: it runs as one of few rows.
-  static bool few(int64_t M) { return M <= kSkinnyRows; }
-
-  // Whether the product runs its step as its epilogue: where K is not split.
   static bool fused(int64_t M, int64_t N, int64_t K) { return plan(M, N, K).ksplit == 1; }
 
   template <int LB, class Step>
@@ -138,8 +145,10 @@ struct Products<bf16> {
                : launch_product<gemm::R4Cfg, kKMajor, true>(M, N, s, o, step, st);
   }
 
-  static size_t store_bytes(int64_t M, int64_t N, int64_t K) {
-    return gemm::product_ws_bytes((int)M, (int)N, ktiles(K));
+  static size_t store_bytes(int64_t M, int64_t N, int nseg, const int64_t* K) {
+    int kt = 0;
+    for (int i = 0; i < nseg; ++i) kt += ktiles(K[i]);
+    return gemm::product_ws_bytes((int)M, (int)N, kt);
   }
 
   static int store(int64_t M, int64_t N, int nseg, const int64_t* K, const bf16* const* a,
@@ -151,48 +160,76 @@ struct Products<bf16> {
                              wsb ? static_cast<float*>(ws) : nullptr, wsb, st);
   }
 
-  static size_t wgrads_bytes(int count, const Wgrad<bf16>* p, int64_t K) {
-    return plan_wgrads(count, p, K).floats * sizeof(float);
+  static size_t wgrads_bytes(int count, const Wgrad* p, int64_t K) {
+    WgradTiles t[kMaxWgrads];
+    for (int g = 0; g < count; ++g) t[g] = {p[g].M, p[g].N};
+    return plan_wgrads(count, t, K).floats * sizeof(float);
   }
 
-  static int wgrads(int count, const Wgrad<bf16>* p, int64_t K, void* ws, size_t wsb,
-                    hipStream_t st) {
-    return launch_wgrads(count, p, K, ws, wsb, st);
-  }
-
-  static int check(const void* a, int64_t lda, int64_t cols, const char* what) {
-    return check_operands({{a, lda, cols, what}});
+  static int wgrads(int count, const Wgrad* p, int64_t K, void* ws, size_t wsb, hipStream_t st) {
+    WgradProduct q[kMaxWgrads];
+    for (int g = 0; g < count; ++g)
+      q[g] = {{p[g].M, p[g].N}, static_cast<const bf16*>(p[g].a), static_cast<const bf16*>(p[g].b),
+              p[g].lda, p[g].ldb, static_cast<bf16*>(p[g].c)};
+    return launch_wgrads(count, q, K, ws, wsb, st);
   }
 };
 
-template <>
-struct Products<float> {
-  static size_t split_bytes(int64_t M, int64_t N, int64_t K) {
-    return ml_gemm_f32_workspace_bytes(M, N, K);
+// fp32 and fp16: fp32 sums on the fp32 matrix cores (ffn_f32.h), joined by the step that
+// reads them. fp32 operands whose sizes, strides or bases are not multiples of 8 elements
+// and 16 bytes go through the kernels that take any (gemm_f32.hip).
+template <typename T>
+struct Products {
+  using In = float;
+
+  template <typename E>
+  static bool regular(const E* p, int64_t ld, int64_t cols) {
+    return aligned16(p) && ld % 8 == 0 && cols % 8 == 0 && ld <= kMaxStride;
+  }
+
+  static F32Plan plan(int64_t M, int64_t N, int nseg, const int64_t* K) {
+    return plan_f32(M, N, f32_ktiles(nseg, K));
+  }
+
+  static size_t splits_of(int64_t M, int64_t N, int nseg, const int64_t* K) {
+    size_t n = plan(M, N, nseg, K).splits;
+    if constexpr (std::is_same_v<T, float>) {
+      int64_t sum = 0;
+      for (int i = 0; i < nseg; ++i) sum += K[i];
+      n = larger(n, gemmf32::sums_splits(M, N, sum));
+    }
+    return n;
   }
 
   static size_t raw_floats(int64_t M, int64_t N, int64_t K) {
-    return (size_t)gemmf32::sums_splits(M, N, K) * M * N;
+    return splits_of(M, N, 1, &K) * M * N;
   }
 
-  static int run(int64_t M, int64_t N, int nseg, const int64_t* K, const float* const* a,
-                 const int64_t* lda, const float* const* b, const int64_t* ldb, int la, int lb,
-                 float* out, void* ws, size_t wsb, hipStream_t st) {
-    const void *ap[2], *bp[2];
-    for (int i = 0; i < nseg; ++i) {
-      ap[i] = a[i];
-      bp[i] = b[i];
+  template <typename EA, typename EB, int LA, int LB>
+  static int sums(int64_t M, int64_t N, int nseg, const int64_t* K, const EA* const* a,
+                  const int64_t* lda, const EB* const* b, const int64_t* ldb, float* out,
+                  int& splits, hipStream_t st) {
+    F32Problem p{};
+    p.nseg = nseg;
+    p.M = (int)M;
+    p.N = (int)N;
+    p.out = out;
+    for (int i = 0; i < nseg; ++i) p.seg[i] = F32Segment{a[i], b[i], lda[i], ldb[i], (int)K[i]};
+    const F32Plan pl = plan(M, N, nseg, K);
+    splits = pl.splits;
+    return launch_f32<EA, EB, LA, LB>(p, pl, st);
+  }
+
+  template <int LB, typename EA, typename EB>
+  static int raw(int64_t M, int64_t N, int64_t K, const EA* a, int64_t lda, const EB* b,
+                 int64_t ldb, float* out, int& splits, hipStream_t st) {
+    if constexpr (std::is_same_v<T, float>) {
+      if (!regular(a, lda, K) || !regular(b, ldb, LB == kMNMajor ? N : K) || K % 8)
+        return gemmf32::sums(M, N, K, a, lda, b, ldb, LB, out, splits, st);
     }
-    return ml_gemm_f32_segments_ws(M, N, nseg, K, ap, lda, bp, ldb, la, lb, out, N, 1.f, 0.f, ws,
-                                   wsb, st);
+    return sums<EA, EB, kRowsK, LB>(M, N, 1, &K, &a, &lda, &b, &ldb, out, splits, st);
   }
 
-  static int raw(int64_t M, int64_t N, int64_t K, const float* a, int64_t lda, const float* b,
-                 int64_t ldb, bool b_mn, float* out, int& splits, hipStream_t st) {
-    return gemmf32::sums(M, N, K, a, lda, b, ldb, b_mn ? kMNMajor : kKMajor, out, splits, st);
-  }
-
-  static bool few(int64_t) { return false; }  // (widths and bases may rule it out)
   static bool fused(int64_t, int64_t, int64_t) { return false; }
 
   template <int LB, class... Args>
@@ -201,32 +238,97 @@ struct Products<float> {
   template <class... Args>
   static int through_pair(const Args&...) { return ML_ERR_INVALID; }
 
-  static size_t store_bytes(int64_t M, int64_t N, int64_t K) { return split_bytes(M, N, K); }
-
-  static int store(int64_t M, int64_t N, int nseg, const int64_t* K, const float* const* a,
-                   const int64_t* lda, const float* const* b, const int64_t* ldb, float* out,
-                   void* ws, size_t wsb, hipStream_t st) {
-    return run(M, N, nseg, K, a, lda, b, ldb, kKMajor, kMNMajor, out, ws, wsb, st);
+  // parts of sums to out, in order
+  static int join(const float* sums, int splits, int64_t M, int64_t N, T* out, hipStream_t st) {
+    const LinearStep<T, kKeepNone> step{nullptr, nullptr, out, 0, N, kActNone, {}};
+    return launch_rows(N % 8 == 0 && aligned16(out), PartialSource{sums, splits, M * N, N},
+                       NoSource{}, step, M, N, st);
   }
 
-  static size_t wgrads_bytes(int count, const Wgrad<float>* p, int64_t K) {
+  static size_t store_bytes(int64_t M, int64_t N, int nseg, const int64_t* K) {
+    return splits_of(M, N, nseg, K) * M * N * sizeof(float);
+  }
+
+  template <typename EA>
+  static int store(int64_t M, int64_t N, int nseg, const int64_t* K, const EA* const* a,
+                   const int64_t* lda, const T* const* b, const int64_t* ldb, T* out, void* ws,
+                   size_t wsb, hipStream_t st) {
+    if constexpr (std::is_same_v<T, float>) {
+      bool any = false;
+      for (int i = 0; i < nseg; ++i)
+        any = any || !regular(a[i], lda[i], K[i]) || !regular(b[i], ldb[i], N);
+      if (any) return any_size(M, N, nseg, K, a, lda, b, ldb, kKMajor, kMNMajor, out, ws, wsb, st);
+    }
+    return joined<EA, T, kRowsK, kRowsMN>(M, N, nseg, K, a, lda, b, ldb, out, ws, st);
+  }
+
+  static size_t wgrads_bytes(int count, const Wgrad* p, int64_t K) {
     size_t n = 0;
-    for (int g = 0; g < count; ++g) n = larger(n, split_bytes(p[g].M, p[g].N, K));
+    for (int g = 0; g < count; ++g) n = larger(n, store_bytes(p[g].M, p[g].N, 1, &K));
     return n;
   }
 
-  static int wgrads(int count, const Wgrad<float>* p, int64_t K, void* ws, size_t wsb,
-                    hipStream_t st) {
+  static int wgrads(int count, const Wgrad* p, int64_t K, void* ws, size_t wsb, hipStream_t st) {
     for (int g = 0; g < count; ++g) {
-      const int rc = run(p[g].M, p[g].N, 1, &K, &p[g].a, &p[g].lda, &p[g].b, &p[g].ldb, kMNMajor,
-                         kMNMajor, p[g].c, ws, wsb, st);
+      const Wgrad& w = p[g];
+      T* out = static_cast<T*>(w.c);
+      int rc;
+      if constexpr (std::is_same_v<T, float>) {
+        const float *a = static_cast<const float*>(w.a), *b = static_cast<const float*>(w.b);
+        rc = regular(a, w.lda, w.M) && regular(b, w.ldb, w.N)
+                 ? joined<float, float, kRowsMN, kRowsMN>(w.M, w.N, 1, &K, &a, &w.lda, &b, &w.ldb,
+                                                          out, ws, st)
+                 : any_size(w.M, w.N, 1, &K, &a, &w.lda, &b, &w.ldb, kMNMajor, kMNMajor, out, ws,
+                            wsb, st);
+      } else {
+        rc = w.a_inner ? wgrad<float, T>(w, K, out, ws, st)
+             : w.b_inner ? wgrad<T, float>(w, K, out, ws, st) : wgrad<T, T>(w, K, out, ws, st);
+      }
       if (rc) return rc;
     }
     return ML_OK;
   }
 
-  static int check(const void*, int64_t, int64_t, const char*) { return ML_OK; }
+ private:
+  template <typename EA, typename EB>
+  static int wgrad(const Wgrad& w, int64_t K, T* out, void* ws, hipStream_t st) {
+    const EA* a = static_cast<const EA*>(w.a);
+    const EB* b = static_cast<const EB*>(w.b);
+    return joined<EA, EB, kRowsMN, kRowsMN>(w.M, w.N, 1, &K, &a, &w.lda, &b, &w.ldb, out, ws, st);
+  }
+
+  template <typename EA, typename EB, int LA, int LB>
+  static int joined(int64_t M, int64_t N, int nseg, const int64_t* K, const EA* const* a,
+                    const int64_t* lda, const EB* const* b, const int64_t* ldb, T* out, void* ws,
+                    hipStream_t st) {
+    int splits = 1;
+    float* to = static_cast<float*>(ws);
+    if constexpr (std::is_same_v<T, float>)
+      if (plan(M, N, nseg, K).splits == 1) to = out;
+    const int rc = sums<EA, EB, LA, LB>(M, N, nseg, K, a, lda, b, ldb, to, splits, st);
+    if (rc || (const void*)to == (const void*)out) return rc;
+    return join(to, splits, M, N, out, st);
+  }
+
+  static int any_size(int64_t M, int64_t N, int nseg, const int64_t* K, const float* const* a,
+                      const int64_t* lda, const float* const* b, const int64_t* ldb, int la, int lb,
+                      float* out, void* ws, size_t wsb, hipStream_t st) {
+    const void *ap[2], *bp[2];
+    for (int i = 0; i < nseg; ++i) {
+      ap[i] = a[i];
+      bp[i] = b[i];
+    }
+    return ml_gemm_f32_segments_ws(M, N, nseg, K, ap, lda, bp, ldb, la, lb, out, N, 1.f, 0.f, ws,
+                                   wsb, st);
+  }
 };
+
+// Operands of the 16-bit forms (fp32 takes any).
+template <typename T>
+int check(const void* a, int64_t lda, int64_t cols, const char* what) {
+  if constexpr (std::is_same_v<T, float>) return ML_OK;
+  return check_operands({{a, lda, cols, what}});
+}
 
 template <int KIND>
 using Kind = std::integral_constant<int, KIND>;
@@ -244,19 +346,17 @@ int dispatch_keep(int keep, F&& f) {
 
 // Whether a forward's product runs as one of few rows: any of 16-bit elements (whose
 // operands qualify as they are checked), those of fp32 whose widths and bases do.
-template <typename T>
 bool few_rows(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* w,
               int64_t ldw) {
   return M <= kSkinnyRows && N % 8 == 0 && K % 8 == 0 && aligned16(x) && aligned16(w) &&
          ldx % 4 == 0 && ldw % 4 == 0;
 }
 
-template <typename F>
-int dispatch(int dtype, F&& f) {
-  if (dtype == ML_F32) return f(float{});
-  if (dtype == ML_BF16) return f(bf16{});
-  set_error("ffn: dtype tag %d not supported (fp32 or bf16)", dtype);
-  return ML_ERR_INVALID;
+// Whether a forward of M rows needs no workspace for its sums: fp32 may yet run as one of
+// any size.
+template <typename T>
+bool few(int64_t M) {
+  return !std::is_same_v<T, float> && M <= kSkinnyRows;
 }
 
 int check_sizes(int64_t M, int64_t N, int64_t K) {
@@ -285,17 +385,17 @@ int linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
   const T* wt = static_cast<const T*>(w);
   const bool vec = N % 8 == 0 && aligned_rows(step.bias, 0) && aligned_rows(step.residual, step.ldr) &&
                    aligned_rows(step.y, step.ldy);
-  if (run && vec && few_rows<T>(M, N, K, x, ldx, w, ldw))
+  if (run && vec && few_rows(M, N, K, x, ldx, w, ldw))
     return launch_skinny<KIND != kKeepNone, false>(
         SkinnyProduct<T, T>{xt, wt, nullptr, ldx, ldw, 0, (int)M, (int)N, (int)K}, step, st);
-  if (Products<T>::few(M) && !run) return ML_OK;
+  if (few<T>(M) && !run) return ML_OK;
   if (Products<T>::fused(M, N, K))
     return run ? Products<T>::template through<kKMajor>(M, N, K, xt, ldx, wt, ldw, step, st)
                : (int)ML_OK;
   float* sums = ws.take<float>(Products<T>::raw_floats(M, N, K));
   if (!run) return ML_OK;
   int splits = 1;
-  const int rc = Products<T>::raw(M, N, K, xt, ldx, wt, ldw, false, sums, splits, st);
+  const int rc = Products<T>::template raw<kKMajor>(M, N, K, xt, ldx, wt, ldw, sums, splits, st);
   if (rc) return rc;
   return launch_rows(vec, PartialSource{sums, splits, M * N, N}, NoSource{}, step, M, N, st);
 }
@@ -316,8 +416,8 @@ GradGrid grad_grid(int64_t rows, int64_t cols, bool vec) {
 
 // dz (act) and db; ws counts what the partial sums take.
 template <typename T, int KIND>
-int linear_grad(const T* dy, int64_t ldy, const Kept<KIND>& z, int act, T* dz, T* db, int64_t M,
-                int64_t N, Arena& ws, bool run, hipStream_t st) {
+int linear_grad(const T* dy, int64_t ldy, const Kept<KIND>& z, int act, Inner<T>* dz, T* db,
+                int64_t M, int64_t N, Arena& ws, bool run, hipStream_t st) {
   const bool vec = N % 8 == 0 && aligned_rows(dy, ldy) && aligned_rows(dz, 0);
   // (the row ranges of the wider grid: a count that holds for both)
   const int64_t most = grad_grid(M, N, true).y > grad_grid(M, N, false).y
@@ -327,9 +427,9 @@ int linear_grad(const T* dy, int64_t ldy, const Kept<KIND>& z, int act, T* dz, T
   const GradGrid g = grad_grid(M, N, vec);
   const dim3 grid((unsigned)g.x, (unsigned)g.y);
   if (vec)
-    linear_grad_kernel<8, T, KIND><<<grid, kThreads, 0, st>>>(dy, ldy, z, act, dz, partial, M, N, g.rows_per);
+    linear_grad_kernel<8, T, Inner<T>, KIND><<<grid, kThreads, 0, st>>>(dy, ldy, z, act, dz, partial, M, N, g.rows_per);
   else
-    linear_grad_kernel<1, T, KIND><<<grid, kThreads, 0, st>>>(dy, ldy, z, act, dz, partial, M, N, g.rows_per);
+    linear_grad_kernel<1, T, Inner<T>, KIND><<<grid, kThreads, 0, st>>>(dy, ldy, z, act, dz, partial, M, N, g.rows_per);
   ML_LAUNCH_CHECK();
   if (db) {
     column_sum_kernel<T><<<dim3((unsigned)((N + 31) / 32)), kThreads, 0, st>>>(partial, (int)g.y, N,
@@ -350,8 +450,10 @@ struct LinearBwd {
 
 template <typename T>
 int linear_bwd(const LinearBwd& p, Arena& ws, bool run, hipStream_t st) {
+  using P = Products<T>;
   const T* dy = static_cast<const T*>(p.dy);
-  T* dz = p.act != kActNone ? ws.take<T>((size_t)(p.M * p.N)) : nullptr;
+  const bool act = p.act != kActNone;
+  Inner<T>* dz = act ? ws.take<Inner<T>>((size_t)(p.M * p.N)) : nullptr;
   if (dz || p.db || !run) {
     const int rc = dispatch_keep<T>(dz ? p.keep : (int)kKeepNone, [&](auto kind) {
       return linear_grad<T>(dy, p.ldy, make_kept<kind.value>(p.z, p.zscale, p.N), p.act, dz,
@@ -359,20 +461,20 @@ int linear_bwd(const LinearBwd& p, Arena& ws, bool run, hipStream_t st) {
     });
     if (rc) return rc;
   }
-  const T* g = dz ? dz : dy;
-  const int64_t ldg = dz ? p.N : p.ldy;
-  const Wgrad<T> wgrad{p.N, p.K, g, static_cast<const T*>(p.x), ldg, p.ldx, static_cast<T*>(p.dw)};
-  const size_t wsb = larger(Products<T>::store_bytes(p.M, p.K, p.N),
-                            Products<T>::wgrads_bytes(1, &wgrad, p.M));
+  const Wgrad wgrad{p.N, p.K, act ? (const void*)dz : p.dy, p.x, act ? p.N : p.ldy, p.ldx, p.dw, act,
+                    false};
+  const size_t wsb = larger(P::store_bytes(p.M, p.K, 1, &p.N), P::wgrads_bytes(1, &wgrad, p.M));
   char* pws = ws.take<char>(wsb);
   if (!run) return ML_OK;
-  const T* w = static_cast<const T*>(p.w);
   if (p.dx) {
-    const int rc = Products<T>::store(p.M, p.K, 1, &p.N, &g, &ldg, &w, &p.ldw, static_cast<T*>(p.dx),
-                                      pws, wsb, st);
+    const T* w = static_cast<const T*>(p.w);
+    T* dx = static_cast<T*>(p.dx);
+    const Inner<T>* z = dz;
+    const int rc = act ? P::store(p.M, p.K, 1, &p.N, &z, &p.N, &w, &p.ldw, dx, pws, wsb, st)
+                       : P::store(p.M, p.K, 1, &p.N, &dy, &p.ldy, &w, &p.ldw, dx, pws, wsb, st);
     if (rc) return rc;
   }
-  return p.dw ? Products<T>::wgrads(1, &wgrad, p.M, pws, wsb, st) : (int)ML_OK;
+  return p.dw ? P::wgrads(1, &wgrad, p.M, pws, wsb, st) : (int)ML_OK;
 }
 
 // -------------------------------------------------------------- gated block --
@@ -404,20 +506,21 @@ int few_mlp(const MlpFwd& p, const TH* h, const GatedStep<TH, KIND>& step,
 template <typename T, int KIND>
 int mlp_fwd(const MlpFwd& p, Arena& ws, bool run, hipStream_t st) {
   using P = Products<T>;
-  T* h = ws.take<T>((size_t)(p.M * p.I));
+  using In = Inner<T>;
+  In* h = ws.take<In>((size_t)(p.M * p.I));
   const T* x = static_cast<const T*>(p.x);
   const T* wg = static_cast<const T*>(p.wg);
   const T* wu = static_cast<const T*>(p.wu);
   const T* wd = static_cast<const T*>(p.wd);
-  const GatedStep<T, KIND> step{h, p.I, make_kept<KIND>(p.gate, p.gscale, p.I),
+  const GatedStep<In, KIND> step{h, p.I, make_kept<KIND>(p.gate, p.gscale, p.I),
                                 make_kept<KIND>(p.up, p.uscale, p.I)};
   const LinearStep<T, kKeepNone> out{nullptr, static_cast<const T*>(p.residual),
                                      static_cast<T*>(p.y), p.ldr, p.O, kActNone, {}};
   const bool vec = p.O % 8 == 0 && aligned_rows(p.residual, p.ldr) && aligned_rows(p.y, p.O);
-  if (run && vec && few_rows<T>(p.M, p.I, p.H, x, p.ldx, wg, p.ldg) && aligned16(wu) &&
-      p.ldu % 4 == 0 && few_rows<T>(p.M, p.O, p.I, h, p.I, wd, p.ldd))
-    return few_mlp<T, T>(p, h, step, out, st);
-  if (P::few(p.M) && !run) return ML_OK;
+  if (run && vec && few_rows(p.M, p.I, p.H, x, p.ldx, wg, p.ldg) && aligned16(wu) &&
+      p.ldu % 4 == 0 && few_rows(p.M, p.O, p.I, h, p.I, wd, p.ldd))
+    return few_mlp<T, In>(p, h, step, out, st);
+  if (few<T>(p.M) && !run) return ML_OK;
   const bool fuse_in = P::fused(p.M, 2 * p.I, p.H), fuse_out = P::fused(p.M, p.O, p.I);
   const size_t n_in = fuse_in ? 0 : P::raw_floats(p.M, p.I, p.H);
   const size_t n_out = fuse_out ? 0 : P::raw_floats(p.M, p.O, p.I);
@@ -427,9 +530,9 @@ int mlp_fwd(const MlpFwd& p, Arena& ws, bool run, hipStream_t st) {
   if (fuse_in) {
     rc = P::through_pair(p.M, p.I, p.H, x, p.ldx, wg, p.ldg, wu, p.ldu, step, st);
   } else {
-    rc = P::raw(p.M, p.I, p.H, x, p.ldx, wg, p.ldg, false, sums, splits, st);
+    rc = P::template raw<kKMajor>(p.M, p.I, p.H, x, p.ldx, wg, p.ldg, sums, splits, st);
     if (rc) return rc;
-    rc = P::raw(p.M, p.I, p.H, x, p.ldx, wu, p.ldu, false, sums + n_in, splits, st);
+    rc = P::template raw<kKMajor>(p.M, p.I, p.H, x, p.ldx, wu, p.ldu, sums + n_in, splits, st);
     if (rc) return rc;
     const int64_t mi = p.M * p.I;
     rc = launch_rows(p.I % 8 == 0, PartialSource{sums, splits, mi, p.I},
@@ -437,7 +540,7 @@ int mlp_fwd(const MlpFwd& p, Arena& ws, bool run, hipStream_t st) {
   }
   if (rc) return rc;
   if (fuse_out) return P::template through<kKMajor>(p.M, p.O, p.I, h, p.I, wd, p.ldd, out, st);
-  rc = P::raw(p.M, p.O, p.I, h, p.I, wd, p.ldd, false, sums, splits, st);
+  rc = P::template raw<kKMajor>(p.M, p.O, p.I, h, p.I, wd, p.ldd, sums, splits, st);
   if (rc) return rc;
   return launch_rows(vec, PartialSource{sums, splits, p.M * p.O, p.O}, NoSource{}, out, p.M,
                      p.O, st);
@@ -454,55 +557,57 @@ struct MlpBwd {
 
 template <typename T, int KIND>
 int mlp_bwd(const MlpBwd& p, Arena& ws, bool run, hipStream_t st) {
+  using P = Products<T>;
+  using In = Inner<T>;
   const size_t mi = (size_t)(p.M * p.I);
-  T* dg = ws.take<T>(mi);
-  T* du = ws.take<T>(mi);
-  T* h = ws.take<T>(mi);
-  const bool fuse = Products<T>::fused(p.M, p.I, p.O);
-  float* sums = ws.take<float>(fuse ? 0 : Products<T>::raw_floats(p.M, p.I, p.O));
-  const T* x = static_cast<const T*>(p.x);
+  In* dg = ws.take<In>(mi);
+  In* du = ws.take<In>(mi);
+  In* h = ws.take<In>(mi);
+  const bool fuse = P::fused(p.M, p.I, p.O);
+  float* sums = ws.take<float>(fuse ? 0 : P::raw_floats(p.M, p.I, p.O));
   const T* dy = static_cast<const T*>(p.dy);
   // the weights' gradients that are wanted (counted for any of them: all three)
-  Wgrad<T> wgrad[3];
+  Wgrad wgrad[3];
   int wanted = 0;
-  if (p.dwg || !run) wgrad[wanted++] = {p.I, p.H, dg, x, p.I, p.ldx, static_cast<T*>(p.dwg)};
-  if (p.dwu || !run) wgrad[wanted++] = {p.I, p.H, du, x, p.I, p.ldx, static_cast<T*>(p.dwu)};
-  if (p.dwd || !run) wgrad[wanted++] = {p.O, p.I, dy, h, p.ldy, p.I, static_cast<T*>(p.dwd)};
-  size_t wsb = Products<T>::store_bytes(p.M, p.H, 2 * p.I);
+  if (p.dwg || !run) wgrad[wanted++] = {p.I, p.H, dg, p.x, p.I, p.ldx, p.dwg, true, false};
+  if (p.dwu || !run) wgrad[wanted++] = {p.I, p.H, du, p.x, p.I, p.ldx, p.dwu, true, false};
+  if (p.dwd || !run) wgrad[wanted++] = {p.O, p.I, p.dy, h, p.ldy, p.I, p.dwd, false, true};
+  const int64_t ks[2] = {p.I, p.I};
+  size_t wsb = P::store_bytes(p.M, p.H, 2, ks);
   if (run) {
-    wsb = larger(wsb, Products<T>::wgrads_bytes(wanted, wgrad, p.M));
+    wsb = larger(wsb, P::wgrads_bytes(wanted, wgrad, p.M));
   } else {
     // (fewer products may split more)
     for (int first = 0; first < 3; ++first)
       for (int n = 1; first + n <= 3; ++n)
-        wsb = larger(wsb, Products<T>::wgrads_bytes(n, wgrad + first, p.M));
-    const Wgrad<T> outer[2] = {wgrad[0], wgrad[2]};
-    wsb = larger(wsb, Products<T>::wgrads_bytes(2, outer, p.M));
+        wsb = larger(wsb, P::wgrads_bytes(n, wgrad + first, p.M));
+    const Wgrad outer[2] = {wgrad[0], wgrad[2]};
+    wsb = larger(wsb, P::wgrads_bytes(2, outer, p.M));
   }
   char* pws = ws.take<char>(wsb);
   if (!run) return ML_OK;
   const T* wd = static_cast<const T*>(p.wd);
-  const GatedGradStep<T, KIND> step{dg, du, p.dwd ? h : nullptr, p.I,
+  const GatedGradStep<In, KIND> step{dg, du, p.dwd ? h : nullptr, p.I,
                                     make_kept<KIND>(p.gate, p.gscale, p.I),
                                     make_kept<KIND>(p.up, p.uscale, p.I)};
   int splits = 1, rc;
   if (fuse) {
-    rc = Products<T>::template through<kMNMajor>(p.M, p.I, p.O, dy, p.ldy, wd, p.ldd, step, st);
+    rc = P::template through<kMNMajor>(p.M, p.I, p.O, dy, p.ldy, wd, p.ldd, step, st);
   } else {
-    rc = Products<T>::raw(p.M, p.I, p.O, dy, p.ldy, wd, p.ldd, true, sums, splits, st);
+    rc = P::template raw<kMNMajor>(p.M, p.I, p.O, dy, p.ldy, wd, p.ldd, sums, splits, st);
     if (rc) return rc;
     rc = launch_rows(p.I % 8 == 0, PartialSource{sums, splits, p.M * p.I, p.I}, NoSource{}, step,
                      p.M, p.I, st);
   }
   if (rc) return rc;
   if (p.dx) {
-    const int64_t ks[2] = {p.I, p.I}, la[2] = {p.I, p.I}, lb[2] = {p.ldg, p.ldu};
-    const T* a[2] = {dg, du};
+    const int64_t la[2] = {p.I, p.I}, lb[2] = {p.ldg, p.ldu};
+    const In* a[2] = {dg, du};
     const T* b[2] = {static_cast<const T*>(p.wg), static_cast<const T*>(p.wu)};
-    rc = Products<T>::store(p.M, p.H, 2, ks, a, la, b, lb, static_cast<T*>(p.dx), pws, wsb, st);
+    rc = P::store(p.M, p.H, 2, ks, a, la, b, lb, static_cast<T*>(p.dx), pws, wsb, st);
     if (rc) return rc;
   }
-  return wanted ? Products<T>::wgrads(wanted, wgrad, p.M, pws, wsb, st) : (int)ML_OK;
+  return wanted ? P::wgrads(wanted, wgrad, p.M, pws, wsb, st) : (int)ML_OK;
 }
 
 }  // namespace
@@ -518,9 +623,9 @@ using namespace mla;
   } while (0)
 
 extern "C" size_t ml_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int dtype) {
-  if (ffn::check_sizes(M, N, K) || dtype == ML_F16) return 0;
+  if (ffn::check_sizes(M, N, K)) return 0;
   ffn::Arena ws{nullptr};
-  ffn::dispatch(dtype, [&](auto t) {
+  dispatch_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     return ffn::linear_fwd<T>(nullptr, 0, nullptr, 0, ffn::LinearStep<T, ffn::kKeepNone>{}, M, N, K,
                               ws, false, nullptr);
@@ -538,25 +643,13 @@ extern "C" int ml_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t 
   ML_CHECK(act >= kActNone && act <= kActGeluTanh, "linear: bad activation %d", act);
   ML_CHECK(ldx >= K && ldw >= K && ldy >= N && (!residual || ldr >= N), "linear: bad row strides");
   ML_TRY(ffn::check_kept(keep, z, zscale, "z"));
-  if (dtype == ML_F16) {
-    ML_TRY(ffn::check_half(M, keep));
-    ML_TRY(ffn::check_operands({{x, ldx, K, "x"}, {w, ldw, K, "weight"}, {y, ldy, N, "y"},
-                                {bias, 0, N, "bias"}, {residual, residual ? ldr : 0, N, "residual"}}));
-    const ffn::LinearStep<f16, ffn::kKeepNone> step{
-        static_cast<const f16*>(bias), static_cast<const f16*>(residual), static_cast<f16*>(y), ldr,
-        ldy, act, {}};
-    return ffn::launch_skinny<false, false>(
-        ffn::SkinnyProduct<f16, f16>{static_cast<const f16*>(x), static_cast<const f16*>(w), nullptr,
-                                     ldx, ldw, 0, (int)M, (int)N, (int)K},
-        step, (hipStream_t)stream);
-  }
-  return ffn::dispatch(dtype, [&](auto t) -> int {
+  return dispatch_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    ML_TRY(ffn::Products<T>::check(x, ldx, K, "x"));
-    ML_TRY(ffn::Products<T>::check(w, ldw, K, "weight"));
-    ML_TRY(ffn::Products<T>::check(y, ldy, N, "y"));
-    ML_TRY(ffn::Products<T>::check(bias, 0, N, "bias"));
-    ML_TRY(ffn::Products<T>::check(residual, residual ? ldr : 0, N, "residual"));
+    ML_TRY(ffn::check<T>(x, ldx, K, "x"));
+    ML_TRY(ffn::check<T>(w, ldw, K, "weight"));
+    ML_TRY(ffn::check<T>(y, ldy, N, "y"));
+    ML_TRY(ffn::check<T>(bias, 0, N, "bias"));
+    ML_TRY(ffn::check<T>(residual, residual ? ldr : 0, N, "residual"));
     ffn::Arena ws{static_cast<char*>(workspace)};
     const size_t need = ml_linear_fwd_workspace_bytes(M, N, K, dtype);
     ML_CHECK(workspace_bytes >= need && (need == 0 || (workspace && aligned16(workspace))),
@@ -579,7 +672,7 @@ extern "C" size_t ml_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K,
   p.N = N;
   p.K = K;
   ffn::Arena ws{nullptr};
-  ffn::dispatch(dtype, [&](auto t) { return ffn::linear_bwd<decltype(t)>(p, ws, false, nullptr); });
+  dispatch_dtype(dtype, [&](auto t) { return ffn::linear_bwd<decltype(t)>(p, ws, false, nullptr); });
   return ws.used;
 }
 
@@ -595,16 +688,16 @@ extern "C" int ml_linear_bwd(const void* x, int64_t ldx, const void* w, int64_t 
   ML_CHECK(act == kActNone || keep != ffn::kKeepNone, "linear backward: no z was kept");
   ML_TRY(ffn::check_kept(act == kActNone ? ffn::kKeepNone : keep, z, zscale, "z"));
   if (!dx && !dw && !db) return ML_OK;
-  return ffn::dispatch(dtype, [&](auto t) -> int {
+  return dispatch_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    if (dx || dw) ML_TRY(ffn::Products<T>::check(act == kActNone ? dy : nullptr, act == kActNone ? ldy : 0, N, "dy"));
+    if (dx || dw) ML_TRY(ffn::check<T>(act == kActNone ? dy : nullptr, act == kActNone ? ldy : 0, N, "dy"));
     if (dx) {
-      ML_TRY(ffn::Products<T>::check(w, ldw, K, "weight"));
-      ML_TRY(ffn::Products<T>::check(dx, K, K, "dx"));
+      ML_TRY(ffn::check<T>(w, ldw, K, "weight"));
+      ML_TRY(ffn::check<T>(dx, K, K, "dx"));
     }
     if (dw) {
-      ML_TRY(ffn::Products<T>::check(x, ldx, K, "x"));
-      ML_TRY(ffn::Products<T>::check(dw, K, K, "dw"));
+      ML_TRY(ffn::check<T>(x, ldx, K, "x"));
+      ML_TRY(ffn::check<T>(dw, K, K, "dw"));
     }
     ffn::Arena ws{static_cast<char*>(workspace)};
     const size_t need = ml_linear_bwd_workspace_bytes(M, N, K, act, dtype);
@@ -629,14 +722,13 @@ int check_mlp(int64_t M, int64_t H, int64_t I, int64_t O) {
 extern "C" size_t ml_swiglu_mlp_fwd_workspace_bytes(int64_t M, int64_t H, int64_t I, int64_t O,
                                                     int dtype) {
   if (ffn::check_mlp(M, H, I, O)) return 0;
-  if (dtype == ML_F16) return (size_t)(M * I) * sizeof(float);  // h
   ffn::MlpFwd p{};
   p.M = M;
   p.H = H;
   p.I = I;
   p.O = O;
   ffn::Arena ws{nullptr};
-  ffn::dispatch(dtype, [&](auto t) { return ffn::mlp_fwd<decltype(t), ffn::kKeepNone>(p, ws, false, nullptr); });
+  dispatch_dtype(dtype, [&](auto t) { return ffn::mlp_fwd<decltype(t), ffn::kKeepNone>(p, ws, false, nullptr); });
   return ws.used;
 }
 
@@ -652,30 +744,14 @@ extern "C" int ml_swiglu_mlp_fwd(const void* x, int64_t ldx, const void* wg, int
            "swiglu mlp: bad row strides");
   ML_TRY(ffn::check_kept(keep, gate, gate_scale, "gate"));
   ML_TRY(ffn::check_kept(keep, up, up_scale, "up"));
-  if (dtype == ML_F16) {
-    ML_TRY(ffn::check_half(M, keep));
-    ML_TRY(ffn::check_operands({{x, ldx, H, "x"}, {wg, ldg, H, "gate weight"},
-                                {wu, ldu, H, "up weight"}, {wd, ldd, I, "down weight"},
-                                {y, O, O, "y"}, {residual, residual ? ldr : 0, O, "residual"}}));
-    const size_t need = ml_swiglu_mlp_fwd_workspace_bytes(M, H, I, O, dtype);
-    ML_CHECK(workspace_bytes >= need && workspace && aligned16(workspace),
-             "swiglu mlp: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-    const ffn::MlpFwd p{x, wg, wu, wd, residual, ldx, ldg, ldu, ldd, ldr, y, keep,
-                        gate, gate_scale, up, up_scale, M, H, I, O};
-    float* h = static_cast<float*>(workspace);
-    const ffn::LinearStep<f16, ffn::kKeepNone> out{nullptr, static_cast<const f16*>(residual),
-                                                   static_cast<f16*>(y), ldr, O, kActNone, {}};
-    return ffn::few_mlp<f16, float>(p, h, ffn::GatedStep<float, ffn::kKeepNone>{h, I, {}, {}}, out,
-                                    (hipStream_t)stream);
-  }
-  return ffn::dispatch(dtype, [&](auto t) -> int {
+  return dispatch_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    ML_TRY(ffn::Products<T>::check(x, ldx, H, "x"));
-    ML_TRY(ffn::Products<T>::check(wg, ldg, H, "gate weight"));
-    ML_TRY(ffn::Products<T>::check(wu, ldu, H, "up weight"));
-    ML_TRY(ffn::Products<T>::check(wd, ldd, I, "down weight"));
-    ML_TRY(ffn::Products<T>::check(y, O, O, "y"));
-    ML_TRY(ffn::Products<T>::check(residual, residual ? ldr : 0, O, "residual"));
+    ML_TRY(ffn::check<T>(x, ldx, H, "x"));
+    ML_TRY(ffn::check<T>(wg, ldg, H, "gate weight"));
+    ML_TRY(ffn::check<T>(wu, ldu, H, "up weight"));
+    ML_TRY(ffn::check<T>(wd, ldd, I, "down weight"));
+    ML_TRY(ffn::check<T>(y, O, O, "y"));
+    ML_TRY(ffn::check<T>(residual, residual ? ldr : 0, O, "residual"));
     ffn::Arena ws{static_cast<char*>(workspace)};
     const size_t need = ml_swiglu_mlp_fwd_workspace_bytes(M, H, I, O, dtype);
     ML_CHECK(workspace_bytes >= need && workspace && aligned16(workspace),
@@ -697,7 +773,7 @@ extern "C" size_t ml_swiglu_mlp_bwd_workspace_bytes(int64_t M, int64_t H, int64_
   p.I = I;
   p.O = O;
   ffn::Arena ws{nullptr};
-  ffn::dispatch(dtype, [&](auto t) { return ffn::mlp_bwd<decltype(t), ffn::kKeepFp8>(p, ws, false, nullptr); });
+  dispatch_dtype(dtype, [&](auto t) { return ffn::mlp_bwd<decltype(t), ffn::kKeepFp8>(p, ws, false, nullptr); });
   return ws.used;
 }
 
@@ -716,17 +792,17 @@ extern "C" int ml_swiglu_mlp_bwd(const void* x, int64_t ldx, const void* wg, int
   ML_TRY(ffn::check_kept(keep, gate, gate_scale, "gate"));
   ML_TRY(ffn::check_kept(keep, up, up_scale, "up"));
   if (!dx && !dwg && !dwu && !dwd) return ML_OK;
-  return ffn::dispatch(dtype, [&](auto t) -> int {
+  return dispatch_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    ML_TRY(ffn::Products<T>::check(x, ldx, H, "x"));
-    ML_TRY(ffn::Products<T>::check(wg, ldg, H, "gate weight"));
-    ML_TRY(ffn::Products<T>::check(wu, ldu, H, "up weight"));
-    ML_TRY(ffn::Products<T>::check(wd, ldd, I, "down weight"));
-    ML_TRY(ffn::Products<T>::check(dy, ldy, O, "dy"));
-    ML_TRY(ffn::Products<T>::check(dx, H, H, "dx"));
-    ML_TRY(ffn::Products<T>::check(dwg, H, H, "gate weight's gradient"));
-    ML_TRY(ffn::Products<T>::check(dwu, H, H, "up weight's gradient"));
-    ML_TRY(ffn::Products<T>::check(dwd, I, I, "down weight's gradient"));
+    ML_TRY(ffn::check<T>(x, ldx, H, "x"));
+    ML_TRY(ffn::check<T>(wg, ldg, H, "gate weight"));
+    ML_TRY(ffn::check<T>(wu, ldu, H, "up weight"));
+    ML_TRY(ffn::check<T>(wd, ldd, I, "down weight"));
+    ML_TRY(ffn::check<T>(dy, ldy, O, "dy"));
+    ML_TRY(ffn::check<T>(dx, H, H, "dx"));
+    ML_TRY(ffn::check<T>(dwg, H, H, "gate weight's gradient"));
+    ML_TRY(ffn::check<T>(dwu, H, H, "up weight's gradient"));
+    ML_TRY(ffn::check<T>(dwd, I, I, "down weight's gradient"));
     ffn::Arena ws{static_cast<char*>(workspace)};
     const size_t need = ml_swiglu_mlp_bwd_workspace_bytes(M, H, I, O, dtype);
     ML_CHECK(workspace_bytes >= need && workspace && aligned16(workspace),

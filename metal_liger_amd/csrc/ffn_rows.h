@@ -479,9 +479,9 @@ inline int launch_rows(bool vec, const Src& src, const Src2& src2, const Step& s
 // row lanes' sums are joined in LDS, and the ranges' partial rows are summed in
 // their order by a second kernel. fp32 sums; dz is summed as it was before its
 // rounding.
-template <int VEC, typename T, int KIND>
+template <int VEC, typename T, typename TZ, int KIND>
 __global__ __launch_bounds__(kThreads) void linear_grad_kernel(
-    const T* __restrict__ dy, int64_t ldy, const Kept<KIND> z, int act, T* __restrict__ dz,
+    const T* __restrict__ dy, int64_t ldy, const Kept<KIND> z, int act, TZ* __restrict__ dz,
     float* __restrict__ partial, int64_t rows, int64_t cols, int64_t rows_per) {
   const int cl = threadIdx.x & 31, rl = threadIdx.x >> 5;
   const int64_t n = ((int64_t)blockIdx.x * 32 + cl) * VEC;
@@ -514,7 +514,7 @@ __global__ __launch_bounds__(kThreads) void linear_grad_kernel(
 #pragma unroll
           for (int k = 0; k < VEC; ++k) d[q][k] *= v[q][k];
         }
-        if (dz) store_n<T, VEC>(dz + (m0 + 8 * q) * cols + n, d[q]);
+        if (dz) store_n<TZ, VEC>(dz + (m0 + 8 * q) * cols + n, d[q]);
 #pragma unroll
         for (int k = 0; k < VEC; ++k) sum[k] += d[q][k];
       }

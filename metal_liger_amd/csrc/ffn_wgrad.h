@@ -18,12 +18,15 @@
 namespace mla {
 namespace ffn {
 
-template <typename T>
-struct Wgrad {
+struct WgradTiles {
   int64_t M, N;
-  const T *a, *b;
+};
+
+struct WgradProduct {
+  WgradTiles size;
+  const bf16 *a, *b;
   int64_t lda, ldb;
-  T* c;  // dense
+  bf16* c;  // dense
 };
 
 constexpr int kMaxWgrads = 3;
@@ -38,7 +41,7 @@ struct WgradPlan {
 
 // Times on one MI355X: a tile of kt 64-wide k-tiles 10 + 1.6 kt us in a round of 256;
 // partials are written and read once (262 KB each way at 4.5 TB/s).
-inline WgradPlan plan_wgrads(int count, const Wgrad<bf16>* p, int64_t K) {
+inline WgradPlan plan_wgrads(int count, const WgradTiles* p, int64_t K) {
   WgradPlan w{};
   for (int g = 0; g < count; ++g)
     w.tiles += (int)(((p[g].M + 255) / 256) * ((p[g].N + 255) / 256));
@@ -165,18 +168,20 @@ __global__ __launch_bounds__(256) void wgrad_join_kernel(const WgradArgs w) {
       });
 }
 
-inline int launch_wgrads(int count, const Wgrad<bf16>* p, int64_t K, void* ws, size_t wsb,
+inline int launch_wgrads(int count, const WgradProduct* p, int64_t K, void* ws, size_t wsb,
                          hipStream_t st) {
-  const WgradPlan plan = plan_wgrads(count, p, K);
+  WgradTiles sizes[kMaxWgrads];
+  for (int g = 0; g < count; ++g) sizes[g] = p[g].size;
+  const WgradPlan plan = plan_wgrads(count, sizes, K);
   ML_CHECK(plan.floats * sizeof(float) <= wsb, "ffn: weight gradients' workspace too small");
   WgradArgs w{};
   w.count = count;
   for (int g = 0; g < count; ++g) {
     const gemm::Segment s{{p[g].a, p[g].lda}, {p[g].b, p[g].ldb}, (int)K};
-    const int rc = gemm::make_problem<gemm::BigCfg>(w.pb[g], (int)p[g].M, (int)p[g].N, 1, &s,
+    const int rc = gemm::make_problem<gemm::BigCfg>(w.pb[g], (int)p[g].size.M, (int)p[g].size.N, 1, &s,
                                                     gemm::kMNMajor, gemm::kMNMajor, 0);
     if (rc) return rc;
-    w.epi[g] = gemm::EpiStore<bf16>{p[g].c, p[g].N, (int)p[g].M, (int)p[g].N, 1.f, 0.f};
+    w.epi[g] = gemm::EpiStore<bf16>{p[g].c, p[g].size.N, (int)p[g].size.M, (int)p[g].size.N, 1.f, 0.f};
     w.first[g + 1] = w.first[g] + w.pb[g].tiles_m * w.pb[g].tiles_n;
   }
   w.tiles = plan.tiles;

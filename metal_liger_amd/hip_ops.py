@@ -229,14 +229,15 @@ def _kept_buffers(x: torch.Tensor, cols: int, keep: int):
             for shape, dtype in kept_layout(x.shape[0], cols, keep)]
 
 
-FEW_ROWS = 64  # rows up to which a forward's products take fp16 (with nothing kept)
+MAX_STRIDE = 1 << 21  # of an operand's rows (ml_linear_fwd)
 
 
 def _product_rows(t: torch.Tensor) -> torch.Tensor:
     """[rows, cols] as the products of t's dtype read it (a copy only when needed)."""
-    if t.dtype == torch.float32:
-        return rows_view(t)
-    if t.stride(1) != 1 or t.stride(0) % 8 != 0 or t.stride(0) < t.shape[1]:
+    if t.dtype == torch.float32 and t.shape[1] % 8:
+        return rows_view(t)  # (the kernels that take any size)
+    s = t.stride(0)
+    if t.stride(1) != 1 or s % 8 != 0 or s < t.shape[1] or s > MAX_STRIDE:
         t = _dense(t)
     return _al16(t)
 
@@ -275,13 +276,13 @@ def _linear(x2, w, bias, residual, act: int, keep: int, z, zscale):
 
 def linear_fwd(x2, w, bias, residual, act: int, keep: int):
     """(y, z, zscale) of ml_linear_fwd: x2 [M, K], w [N, K], bias [N] or None, residual
-    [M, N] or None, all bf16 (sizes in multiples of 8) or all fp32."""
+    [M, N] or None, all fp32, or all bf16 or fp16 (sizes in multiples of 8)."""
     kept = _kept_buffers(x2, w.shape[0], keep)
     return (_linear(x2, w, bias, residual, act, keep, *kept), *kept)
 
 
 def linear_infer(x2, w, bias, residual, act: int):
-    """linear_fwd's y with nothing kept; also all fp16 (as bf16, up to FEW_ROWS rows)."""
+    """linear_fwd's y with nothing kept."""
     return _linear(x2, w, bias, residual, act, KEEP_NONE, None, None)
 
 
@@ -331,7 +332,7 @@ def swiglu_mlp_fwd(x2, wg, wu, wd, residual, keep: int):
 
 
 def swiglu_mlp_infer(x2, wg, wu, wd, residual):
-    """swiglu_mlp_fwd's y with nothing kept; dtypes as linear_infer."""
+    """swiglu_mlp_fwd's y with nothing kept."""
     return _swiglu_mlp(x2, wg, wu, wd, residual, KEEP_NONE, (None,) * 4)
 
 

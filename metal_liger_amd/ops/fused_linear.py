@@ -5,14 +5,13 @@ nn.Linear around their activations and residual adds).
 The sum over K, the bias, the activation and the residual are added up in fp32 and y is
 rounded once. The backward needs z = x W^T + bias where there is an activation: it is
 kept in 16 bits (fp16 with a power of two as scale for every 32 columns of a row, which
-rounds finer than bf16; in fp32 where the products run in fp32), or in 8 (checkpoint=
-"fp8": e4m3 with such scales), formed of the fp32 sums. What is not needed (x where the
+rounds finer than bf16; fp32 in fp32), or in 8 (checkpoint="fp8": e4m3 with such
+scales), formed of the fp32 sums. What is not needed (x where the
 weight is frozen, W where x needs no gradient) is not kept. First derivatives only.
 
-bf16 runs on the bf16 matrix cores (whose kernels take sizes in multiples of 8: others are
-padded with zeros, which add nothing), as fp16 with such sizes does in forwards of up to
-64 rows that keep nothing; fp32, and fp16 elsewhere (upcast, and rounded once at the end),
-on the fp32 ones.
+bf16 runs on the bf16 matrix cores; fp32 and fp16 on the fp32 ones, with everything
+between input and output in fp32. The kernels take 16-bit sizes in multiples of 8, and
+fp32 ones faster: others are padded with zeros, which add nothing.
 """
 
 from __future__ import annotations
@@ -39,35 +38,40 @@ def check_checkpoint(checkpoint: str | None) -> None:
 
 
 def keep_mode(checkpoint: str | None, dtype: torch.dtype) -> int:
-    """How a backward's tensors are kept where the products are of `dtype`."""
+    """How a backward's tensors are kept where the inputs are of `dtype`."""
     if checkpoint == "fp8":
         return hip_ops.KEEP_FP8
-    return hip_ops.KEEP_FP16 if dtype == torch.bfloat16 else hip_ops.KEEP_F32
+    return hip_ops.KEEP_F32 if dtype == torch.float32 else hip_ops.KEEP_FP16
 
 
-def compute_dtype(x: torch.Tensor, *features: int, infer: bool = False) -> torch.dtype:
-    """bf16 for bf16, fp16 in forwards of few rows with nothing to keep (infer) and sizes
-    in multiples of 8, else fp32."""
-    if x.dtype == torch.bfloat16 or (
-            infer and x.dtype == torch.float16 and x.numel() <= hip_ops.FEW_ROWS * x.shape[-1]
-            and all(f % 8 == 0 for f in features)):
-        return x.dtype
-    return torch.float32
+# Multiply-adds of a product from which fp32 sizes are padded: [517, 1001] x 777 (4e8)
+# takes 180 us a training pass as it is and 215 padded, [1024, 1001] x 4001 (4e9) 600 and
+# 470.
+_PAD_F32 = 1 << 30
 
 
-def padded(n: int, dtype: torch.dtype) -> int:
-    """A feature size as the products of dtype take it."""
-    return n if dtype == torch.float32 else -(-n // 8) * 8
+def pads(dtype: torch.dtype, rows: int, *features: int) -> bool:
+    """Whether an operator of these sizes pads its feature sizes to multiples of 8."""
+    if dtype != torch.float32:
+        return True
+    for f in features:
+        rows *= f
+    return rows >= _PAD_F32
 
 
-def pad(t, dim: int, dtype: torch.dtype):
-    """t's dimension at the size padded gives, with zeros."""
-    if t is None or t.shape[dim] % 8 == 0 or dtype == torch.float32:
+def padded(n: int) -> int:
+    return -(-n // 8) * 8
+
+
+def pad(t, *dims: int):
+    """t with these dimensions' sizes padded by zeros."""
+    if t is None or all(t.shape[d] % 8 == 0 for d in dims):
         return t
     shape = list(t.shape)
-    shape[dim] = padded(shape[dim], dtype)
+    for d in dims:
+        shape[d] = padded(shape[d])
     out = t.new_zeros(shape)
-    out.narrow(dim, 0, t.shape[dim]).copy_(t)
+    out[tuple(slice(n) for n in t.shape)].copy_(t)
     return out
 
 
@@ -76,15 +80,12 @@ def cut(t: torch.Tensor, *sizes: int) -> torch.Tensor:
     return t if tuple(t.shape) == sizes else t[tuple(slice(n) for n in sizes)].contiguous()
 
 
-def rows(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """[..., C] -> [R, C] in dtype, C padded."""
+def rows(t, padding: bool = False):
+    """[..., C] -> [R, C], C padded if wanted."""
+    if t is None:
+        return None
     t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    return pad(t if t.dtype == dtype else t.to(dtype), 1, dtype)
-
-
-def weight_as(t, dtype: torch.dtype):
-    """A weight in dtype, both sizes padded."""
-    return None if t is None else pad(rows(t, dtype), 0, dtype)
+    return pad(t, 1) if padding else t
 
 
 def check_input(what: str, x: torch.Tensor, *weights: torch.Tensor) -> None:
@@ -113,18 +114,15 @@ def wants_grad(*tensors) -> bool:
 
 def _forward(x, weight, bias, residual, act: int, keep: int):
     """(y, z, zscale), or y alone where nothing is kept."""
-    none = keep == hip_ops.KEEP_NONE
-    ct = compute_dtype(x, *weight.shape, infer=none)
-    bias = bias if bias is None or bias.dtype == ct else bias.to(ct)
-    args = (rows(x, ct), weight_as(weight, ct), pad(bias, 0, ct),
-            None if residual is None else rows(residual, ct), act)
-    y, *kept = (cops.linear_infer(*args),) if none else cops.linear_fwd(*args, keep)
-    y = cut(y, y.shape[0], weight.shape[0])
-    if y.dtype != x.dtype:
-        y = y.to(x.dtype)
-    if x.dim() != 2:
-        y = y.view(*x.shape[:-1], weight.shape[0])
-    return y, *kept
+    N, K = weight.shape
+    p = pads(x.dtype, x.numel() // K, N, K)
+    w, b = (pad(weight, 0, 1), pad(bias, 0)) if p else (weight, bias)
+    args = (rows(x, p), w, b, rows(residual, p), act)
+    y, *kept = (cops.linear_infer(*args),) if keep == hip_ops.KEEP_NONE else \
+        cops.linear_fwd(*args, keep)
+    if p:
+        y = cut(y, y.shape[0], N)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], N), *kept
 
 
 class _FusedLinearFunction(torch.autograd.Function):
@@ -136,7 +134,7 @@ class _FusedLinearFunction(torch.autograd.Function):
         y, *kept = _forward(x, weight, bias, residual, act, keep)
         ctx.save_for_backward(x if need_dw else None, weight if need_dx else None, *kept)
         ctx.act, ctx.keep, ctx.sizes = act, keep, tuple(weight.shape)
-        ctx.x_shape, ctx.dtype = x.shape, x.dtype
+        ctx.x_shape = x.shape
         return y
 
     @staticmethod
@@ -147,15 +145,14 @@ class _FusedLinearFunction(torch.autograd.Function):
             x, weight, *kept = ctx.saved_tensors
             z, zscale = kept or (None, None)
             N, K = ctx.sizes
-            ct = compute_dtype(dy, N, K)
-            out = cops.linear_bwd(None if x is None else rows(x, ct), weight_as(weight, ct),
-                                  rows(dy, ct), ctx.act, ctx.keep, z, zscale, padded(N, ct),
-                                  padded(K, ct), need_dx, need_dw, need_db)
-            sizes = ((ctx.x_shape.numel() // K, K), (N, K), (N,))
-            for i, need in enumerate((need_dx, need_dw, need_db)):
-                if need:
-                    g = cut(out[i], *sizes[i])
-                    grads[i] = g if g.dtype == ctx.dtype else g.to(ctx.dtype)
+            M = ctx.x_shape.numel() // K
+            p = pads(dy.dtype, M, N, K)
+            size = padded if p else int
+            out = cops.linear_bwd(rows(x, p), pad(weight, 0, 1) if p else weight, rows(dy, p),
+                                  ctx.act, ctx.keep, z, zscale, size(N), size(K), need_dx, need_dw,
+                                  need_db)
+            grads = [cut(g, *sizes) if need else None
+                     for g, sizes, need in zip(out, ((M, K), (N, K), (N,)), ctx.needs_input_grad)]
             if need_dx and len(ctx.x_shape) != 2:
                 grads[0] = grads[0].view(ctx.x_shape)
         return (*grads, dy if need_dr else None, None, None)
@@ -184,7 +181,7 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     check_residual("fused_linear", residual, x, weight.shape[0])
     if not wants_grad(x, weight, bias, residual):
         return _forward(x, weight, bias, residual, act, hip_ops.KEEP_NONE)[0]
-    keep = keep_mode(checkpoint, compute_dtype(x, *weight.shape))
+    keep = keep_mode(checkpoint, x.dtype)
     return _FusedLinearFunction.apply(x, weight, bias, residual, act, keep)
 
 

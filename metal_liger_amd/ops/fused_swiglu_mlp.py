@@ -3,8 +3,7 @@
 ops/fused_swiglu.py:59-75, and its LoRA block needs adapters).
 
 The backward needs gate = x Wg^T and up = x Wu^T: they are kept in 16 bits (fp16 with a
-power of two as scale for every 32 columns of a row; in fp32 where the products run in
-fp32), or in 8 (checkpoint="fp8": e4m3 with such scales), formed of the fp32 sums. h = silu(gate) * up is not kept; the backward forms it
+power of two as scale for every 32 columns of a row; fp32 in fp32), or in 8 (checkpoint="fp8": e4m3 with such scales), formed of the fp32 sums. h = silu(gate) * up is not kept; the backward forms it
 again of what was kept. h and the gradients of gate, up and h are rounded to bf16
 between the products on the bf16 matrix cores. First derivatives only. Types and sizes
 as ops/fused_linear.py.
@@ -20,9 +19,9 @@ import torch.nn as nn
 from metal_liger_amd import _custom_ops as cops
 from metal_liger_amd import hip_ops
 from metal_liger_amd._model_walk import find_layers
-from metal_liger_amd.ops.fused_linear import (check_checkpoint, check_input, check_residual,
-                                              compute_dtype, cut, keep_mode, plain_linear, rows,
-                                              runs_fused, wants_grad, weight_as)
+from metal_liger_amd.ops.fused_linear import (check_checkpoint, check_input, check_residual, cut,
+                                              keep_mode, pad, pads, plain_linear, rows, runs_fused,
+                                              wants_grad)
 from metal_liger_amd.ops.fused_swiglu import MetalLigerSwiGLU
 
 logger = logging.getLogger(__name__)
@@ -31,14 +30,14 @@ logger = logging.getLogger(__name__)
 def _forward(x, weights, residual, keep: int):
     """(y, gate, its scales, up, its scales), or y alone where nothing is kept."""
     O, I = weights[2].shape  # noqa: E741
-    none = keep == hip_ops.KEEP_NONE
-    ct = compute_dtype(x, x.shape[-1], I, O, infer=none)
-    args = (rows(x, ct), *(weight_as(w, ct) for w in weights),
-            None if residual is None else rows(residual, ct))
-    y, *kept = (cops.swiglu_mlp_infer(*args),) if none else cops.swiglu_mlp_fwd(*args, keep)
-    y = cut(y, y.shape[0], O)
-    if y.dtype != x.dtype:
-        y = y.to(x.dtype)
+    p = pads(x.dtype, x.numel() // x.shape[-1], x.shape[-1], I)
+    if p:
+        weights = [pad(w, 0, 1) for w in weights]
+    args = (rows(x, p), *weights, rows(residual, p))
+    y, *kept = (cops.swiglu_mlp_infer(*args),) if keep == hip_ops.KEEP_NONE else \
+        cops.swiglu_mlp_fwd(*args, keep)
+    if p:
+        y = cut(y, y.shape[0], O)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], O), *kept
 
 
@@ -57,12 +56,13 @@ class _FusedSwiGLUMLPFunction(torch.autograd.Function):
         grads = [None] * 4
         if any(ctx.needs_input_grad[:4]):
             x, wg, wu, wd, *kept = ctx.saved_tensors
-            ct = compute_dtype(x, x.shape[-1], *wd.shape)
-            outs = cops.swiglu_mlp_bwd(rows(x, ct), *(weight_as(w, ct) for w in (wg, wu, wd)),
-                                       rows(dy, ct), ctx.keep, *kept, *ctx.needs_input_grad[:4])
-            sizes = ((x.numel() // x.shape[-1], x.shape[-1]), wg.shape, wu.shape, wd.shape)
-            grads = [cut(g, *n).to(x.dtype) if need else None
-                     for g, n, need in zip(outs, sizes, ctx.needs_input_grad)]
+            M, H = x.numel() // x.shape[-1], x.shape[-1]
+            p = pads(x.dtype, M, H, wd.shape[1])
+            weights = [pad(w, 0, 1) for w in (wg, wu, wd)] if p else (wg, wu, wd)
+            outs = cops.swiglu_mlp_bwd(rows(x, p), *weights, rows(dy, p), ctx.keep, *kept,
+                                       *ctx.needs_input_grad[:4])
+            grads = [cut(g, *sizes) if need else None for g, sizes, need in
+                     zip(outs, ((M, H), wg.shape, wu.shape, wd.shape), ctx.needs_input_grad)]
             if grads[0] is not None and x.dim() != 2:
                 grads[0] = grads[0].view(x.shape)
         return (*grads, dy if ctx.needs_input_grad[4] else None, None)
@@ -86,7 +86,7 @@ def fused_swiglu_mlp(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torc
     weights = (gate_weight, up_weight, down_weight)
     if not wants_grad(x, *weights, residual):
         return _forward(x, weights, residual, hip_ops.KEEP_NONE)[0]
-    keep = keep_mode(checkpoint, compute_dtype(x, x.shape[-1], *down_weight.shape))
+    keep = keep_mode(checkpoint, x.dtype)
     return _FusedSwiGLUMLPFunction.apply(x, *weights, residual, keep)
 
 

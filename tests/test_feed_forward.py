@@ -141,8 +141,9 @@ def test_host_side_argument_errors():
     refused(linear(bias=p + 2), b"bias")
     refused(linear(res=p, ldr=68), b"residual")
     refused(linear(M=1000, wsb=0, N=8, ldy=8, K=4096, ldx=4096, ldw=4096), b"workspace")
-    refused(linear(dtype=2, M=65), b"fp16")
-    refused(linear(dtype=2, M=4, keep=3, z=p, zs=p), b"fp16")
+    refused(linear(dtype=2, keep=1, z=p), b"not kept as 1")
+    refused(linear(dtype=2, x=p + 2), b"16-byte aligned")
+    refused(linear(ldx=(1 << 21) + 8), b"up to")
     refused(linear(dtype=7), b"dtype tag 7")
 
     def linear_bwd(x=p, w=p, dy=p, ldy=64, act=0, keep=0, z=None, zs=None, dx=q, dw=q, db=q, M=100, N=64,
@@ -157,7 +158,7 @@ def test_host_side_argument_errors():
     refused(linear_bwd(ldy=72, dy=p + 4), b"dy")
     refused(linear_bwd(dx=q + 8), b"dx")
     refused(linear_bwd(wsb=0), b"workspace")
-    refused(linear_bwd(dtype=2), b"dtype tag 2")
+    refused(linear_bwd(dtype=9), b"dtype tag 9")
     assert linear_bwd(dx=None, dw=None, db=None) == 0
 
     def mlp(fn, *args, keep=0, kept=(None,) * 4, M=100, H=64, I=128, O=64, wsb=1 << 40, dtype=1):  # noqa: E741
@@ -169,7 +170,7 @@ def test_host_side_argument_errors():
     refused(mlp(L.ml_swiglu_mlp_fwd, *fwd, I=136), b"row strides")
     refused(mlp(L.ml_swiglu_mlp_fwd, *fwd, keep=3, kept=(p, p, None, None)), b"up")
     refused(mlp(L.ml_swiglu_mlp_fwd, *fwd, wsb=0), b"workspace")
-    refused(mlp(L.ml_swiglu_mlp_fwd, *fwd, dtype=2), b"fp16")
+    refused(mlp(L.ml_swiglu_mlp_fwd, *fwd, dtype=-1), b"dtype tag -1")
     refused(mlp(L.ml_swiglu_mlp_fwd, *fwd[:-1], None), b"null pointer")
 
     def mlp_bwd(dx=q, keep=3, kept=(p,) * 4, dy=p, wsb=1 << 40, dtype=1):

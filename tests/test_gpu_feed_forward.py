@@ -107,7 +107,7 @@ def _linear_check(x, w, b, r, dy, act, checkpoint, call):
             # half a step, a smallest step of half 2^-9, where z's own error may move the scale
             assert bool((err <= 2 * ez + z.abs() * 2.0 ** -4 + 2 * e * 2.0 ** -10).all()), "kept"
         else:
-            assert bool((err <= ez + z.abs() * (_u(torch.float16) if low else V)
+            assert bool((err <= ez + z.abs() * (V if dtype == torch.float32 else _u(torch.float16))
                         + 2.0 ** -38 * z.abs().max()).all()), "kept"
         d = ref.act_grad(zk, act)
         dz, edz = D * d, D.abs() * _act_noise(zk)
@@ -193,7 +193,7 @@ def _mlp_check(x, ws, r, dy, checkpoint, call):
             s = s.repeat_interleave(32, -1)[..., :I]
             assert bool(((k - z).abs() <= 2 * e + z.abs() * 2.0 ** -4 + 2 * s * 2.0 ** -10).all())
         else:
-            v = _u(torch.float16) if low else V
+            v = V if x.dtype == torch.float32 else _u(torch.float16)
             assert bool(((k - z).abs() <= e + v * z.abs()
                         + 2.0 ** -38 * z.abs().max()).all())
     zero = torch.zeros_like(gk)
@@ -408,3 +408,40 @@ def test_scales_of_short_blocks(dev, M, N):
         assert torch.equal(s.cpu().long() - 127, e.clamp_min(-126))
         half = z.abs() * (2.0 ** -11 if keep == hip_ops.KEEP_FP16 else 2.0 ** -4) + 2.0 ** -30
         assert bool(((ref.held_values(v.cpu(), s.cpu()) - z).abs() <= half).all())
+
+
+# fp32 and fp16: 128 x 128 and 64 x 64 tiles, K whole and split, sizes that pad
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("size", [(1025, 72, 2056), (300, 1000, 264), (70, 2056, 136), (2100, 64, 520),
+                                  (1030, 1001, 1043), (129, 40, 8)])
+def test_linear_fp32_tiles(dev, dtype, size):
+    from metal_liger_amd.ops.fused_linear import fused_linear
+    for act in ("silu", None):
+        x, w, b, r, dy = _linear_case(*size, dtype, True, act is None, dev)
+        _linear_check(x, w, b, r, dy, act, None, lambda: fused_linear(x, w, b, act, r))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+@pytest.mark.parametrize("size", [(1025, 72, 2056, 136), (520, 264, 1000, 264), (70, 1000, 1501, 999),
+                                  (1100, 999, 1001, 64)])
+@pytest.mark.parametrize("checkpoint", [None, "fp8"])
+def test_mlp_fp32_tiles(dev, dtype, size, checkpoint):
+    from metal_liger_amd.ops.fused_swiglu_mlp import fused_swiglu_mlp
+    x, ws, r, dy = _mlp_case(*size, dtype, True, dev)
+    _mlp_check(x, ws, r, dy, checkpoint,
+               lambda: fused_swiglu_mlp(x, *ws, residual=r, checkpoint=checkpoint))
+
+
+def test_wide_strides(dev):
+    """Rows further apart than the kernels address."""
+    from metal_liger_amd.ops.fused_linear import fused_linear
+    wide = 5 * (1 << 20)
+    w = seeded((40, 64), 1, torch.bfloat16).to(dev)
+    big = torch.zeros(300, wide, dtype=torch.bfloat16, device=dev)
+    x = big[:, 8:72]
+    x.copy_(seeded((300, 64), 2, torch.bfloat16))
+    assert torch.equal(fused_linear(x, w), fused_linear(x.contiguous(), w))
+    big = torch.zeros(150, wide, device=dev)
+    x = big[:, 8:72]
+    x.copy_(seeded((150, 64), 2))
+    assert torch.equal(fused_linear(x, w.float()), fused_linear(x.contiguous(), w.float()))
