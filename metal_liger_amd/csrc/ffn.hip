@@ -123,6 +123,7 @@ struct Products<bf16> {
   }
 
   static bool fused(int64_t M, int64_t N, int64_t K) { return plan(M, N, K).ksplit == 1; }
+  static bool fused_pair(int64_t M, int64_t N, int64_t K) { return fused(M, 2 * N, K); }
 
   template <int LB, class Step>
   static int through(int64_t M, int64_t N, int64_t K, const bf16* a, int64_t lda, const bf16* b,
@@ -205,10 +206,12 @@ struct Products {
     return splits_of(M, N, 1, &K) * M * N;
   }
 
-  template <typename EA, typename EB, int LA, int LB>
+  // out: the sums, in as many parts as splits says; a step (with plan().splits 1) takes
+  // them instead
+  template <typename EA, typename EB, int LA, int LB, class Step = SumsOnly>
   static int sums(int64_t M, int64_t N, int nseg, const int64_t* K, const EA* const* a,
                   const int64_t* lda, const EB* const* b, const int64_t* ldb, float* out,
-                  int& splits, hipStream_t st) {
+                  int& splits, hipStream_t st, const Step& step = {}) {
     F32Problem p{};
     p.nseg = nseg;
     p.M = (int)M;
@@ -217,7 +220,7 @@ struct Products {
     for (int i = 0; i < nseg; ++i) p.seg[i] = F32Segment{a[i], b[i], lda[i], ldb[i], (int)K[i]};
     const F32Plan pl = plan(M, N, nseg, K);
     splits = pl.splits;
-    return launch_f32<EA, EB, LA, LB>(p, pl, st);
+    return launch_f32<EA, EB, LA, LB>(p, pl, step, st);
   }
 
   template <int LB, typename EA, typename EB>
@@ -230,17 +233,32 @@ struct Products {
     return sums<EA, EB, kRowsK, LB>(M, N, 1, &K, &a, &lda, &b, &ldb, out, splits, st);
   }
 
-  static bool fused(int64_t, int64_t, int64_t) { return false; }
+  // Only steps that keep nothing: those of 128 x 128 tiles that keep a tensor did not fit
+  // in two workgroups' registers. (fp32 operands may yet turn out to be of any size:
+  // whether a product runs its step itself is known when they are.)
+  static bool fused(int64_t M, int64_t N, int64_t K) {
+    return !std::is_same_v<T, float> && plan(M, N, 1, &K).splits == 1;
+  }
 
-  template <int LB, class... Args>
-  static int through(const Args&...) { return ML_ERR_INVALID; }
+  template <int LB, typename EA, class Step>
+  static int through(int64_t M, int64_t N, int64_t K, const EA* a, int64_t lda, const T* b,
+                     int64_t ldb, const Step& step, hipStream_t st) {
+    int splits;
+    return sums<EA, T, kRowsK, LB>(M, N, 1, &K, &a, &lda, &b, &ldb, nullptr, splits, st, step);
+  }
+
+  static bool fused_pair(int64_t, int64_t, int64_t) { return false; }
 
   template <class... Args>
   static int through_pair(const Args&...) { return ML_ERR_INVALID; }
 
+  static LinearStep<T, kKeepNone> store_step(T* out, int64_t N) {
+    return {nullptr, nullptr, out, 0, N, kActNone, {}};
+  }
+
   // parts of sums to out, in order
   static int join(const float* sums, int splits, int64_t M, int64_t N, T* out, hipStream_t st) {
-    const LinearStep<T, kKeepNone> step{nullptr, nullptr, out, 0, N, kActNone, {}};
+    const LinearStep<T, kKeepNone> step = store_step(out, N);
     return launch_rows(N % 8 == 0 && aligned16(out), PartialSource{sums, splits, M * N, N},
                        NoSource{}, step, M, N, st);
   }
@@ -302,12 +320,12 @@ struct Products {
                     const int64_t* lda, const EB* const* b, const int64_t* ldb, T* out, void* ws,
                     hipStream_t st) {
     int splits = 1;
-    float* to = static_cast<float*>(ws);
-    if constexpr (std::is_same_v<T, float>)
-      if (plan(M, N, nseg, K).splits == 1) to = out;
-    const int rc = sums<EA, EB, LA, LB>(M, N, nseg, K, a, lda, b, ldb, to, splits, st);
-    if (rc || (const void*)to == (const void*)out) return rc;
-    return join(to, splits, M, N, out, st);
+    float* parts = static_cast<float*>(ws);
+    if (plan(M, N, nseg, K).splits == 1)
+      return sums<EA, EB, LA, LB>(M, N, nseg, K, a, lda, b, ldb, parts, splits, st,
+                                  store_step(out, N));
+    const int rc = sums<EA, EB, LA, LB>(M, N, nseg, K, a, lda, b, ldb, parts, splits, st);
+    return rc ? rc : join(parts, splits, M, N, out, st);
   }
 
   static int any_size(int64_t M, int64_t N, int nseg, const int64_t* K, const float* const* a,
@@ -389,9 +407,17 @@ int linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
     return launch_skinny<KIND != kKeepNone, false>(
         SkinnyProduct<T, T>{xt, wt, nullptr, ldx, ldw, 0, (int)M, (int)N, (int)K}, step, st);
   if (few<T>(M) && !run) return ML_OK;
-  if (Products<T>::fused(M, N, K))
-    return run ? Products<T>::template through<kKMajor>(M, N, K, xt, ldx, wt, ldw, step, st)
-               : (int)ML_OK;
+  if constexpr (std::is_same_v<T, bf16> || KIND == kKeepNone) {
+    if (run && Products<T>::fused(M, N, K))
+      return Products<T>::template through<kKMajor>(M, N, K, xt, ldx, wt, ldw, step, st);
+  }
+  if (std::is_same_v<T, bf16> && Products<T>::fused(M, N, K)) return ML_OK;
+  if constexpr (std::is_same_v<T, float> && KIND == kKeepNone) {
+    using P = Products<float>;
+    if (run && P::regular(xt, ldx, K) && P::regular(wt, ldw, K) &&
+        P::plan(M, N, 1, &K).splits == 1)
+      return P::through<kKMajor>(M, N, K, xt, ldx, wt, ldw, step, st);
+  }
   float* sums = ws.take<float>(Products<T>::raw_floats(M, N, K));
   if (!run) return ML_OK;
   int splits = 1;
@@ -521,7 +547,7 @@ int mlp_fwd(const MlpFwd& p, Arena& ws, bool run, hipStream_t st) {
       p.ldu % 4 == 0 && few_rows(p.M, p.O, p.I, h, p.I, wd, p.ldd))
     return few_mlp<T, In>(p, h, step, out, st);
   if (few<T>(p.M) && !run) return ML_OK;
-  const bool fuse_in = P::fused(p.M, 2 * p.I, p.H), fuse_out = P::fused(p.M, p.O, p.I);
+  const bool fuse_in = P::fused_pair(p.M, p.I, p.H), fuse_out = P::fused(p.M, p.O, p.I);
   const size_t n_in = fuse_in ? 0 : P::raw_floats(p.M, p.I, p.H);
   const size_t n_out = fuse_out ? 0 : P::raw_floats(p.M, p.O, p.I);
   float* sums = ws.take<float>(larger(2 * n_in, n_out));
@@ -563,7 +589,8 @@ int mlp_bwd(const MlpBwd& p, Arena& ws, bool run, hipStream_t st) {
   In* dg = ws.take<In>(mi);
   In* du = ws.take<In>(mi);
   In* h = ws.take<In>(mi);
-  const bool fuse = P::fused(p.M, p.I, p.O);
+  constexpr bool kMayFuse = std::is_same_v<T, bf16>;
+  const bool fuse = kMayFuse && P::fused(p.M, p.I, p.O);
   float* sums = ws.take<float>(fuse ? 0 : P::raw_floats(p.M, p.I, p.O));
   const T* dy = static_cast<const T*>(p.dy);
   // the weights' gradients that are wanted (counted for any of them: all three)
@@ -590,9 +617,10 @@ int mlp_bwd(const MlpBwd& p, Arena& ws, bool run, hipStream_t st) {
   const GatedGradStep<In, KIND> step{dg, du, p.dwd ? h : nullptr, p.I,
                                     make_kept<KIND>(p.gate, p.gscale, p.I),
                                     make_kept<KIND>(p.up, p.uscale, p.I)};
-  int splits = 1, rc;
+  int splits = 1, rc = ML_OK;
   if (fuse) {
-    rc = P::template through<kMNMajor>(p.M, p.I, p.O, dy, p.ldy, wd, p.ldd, step, st);
+    if constexpr (kMayFuse)
+      rc = P::template through<kMNMajor>(p.M, p.I, p.O, dy, p.ldy, wd, p.ldd, step, st);
   } else {
     rc = P::template raw<kMNMajor>(p.M, p.I, p.O, dy, p.ldy, wd, p.ldd, sums, splits, st);
     if (rc) return rc;

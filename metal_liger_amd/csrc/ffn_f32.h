@@ -20,8 +20,9 @@
 // rows, c ^ (r / 2 & 3)); MN-major tile [32 k][rows]. Rows past the operand's end and
 // k-rows past K read zeros by the buffer's range, K-major chunks past K by an offset past
 // every range: sizes and strides are multiples of 8, so that no chunk lies across an end.
-// Measured against one and the same library product: [1024, 4352] x 4352 448 -> 307 us
-// (its own 327), [2048, 2048] x 2048 162 -> 124 (118).
+// Measured (fp32, forward; a plain library product of the same): [1024, 4352] x 4352 378
+// us (318; with an any-size kernel's register tiles 448), [2048, 2048] x 2048 147 (121),
+// [8192, 2048] x 2048 527, 130 TFLOP/s (468).
 #pragma once
 
 #include "ffn_rows.h"
@@ -130,8 +131,12 @@ struct F32Operand {
   }
 };
 
-template <typename EA, typename EB, int LA, int LB, int T>
-__global__ __launch_bounds__(256) void f32_kernel(const F32Problem p) {
+// Step SumsOnly: the sums (or a split's part of them) to p.out; otherwise, K not split,
+// the step takes them from the accumulators: 32 lanes hold a row's 32 columns.
+struct SumsOnly {};
+
+template <typename EA, typename EB, int LA, int LB, int T, class Step>
+__global__ __launch_bounds__(256, 2) void f32_kernel(const F32Problem p, const Step step) {
   constexpr int TILE = 64 * T, W = 32 * T;
   using OA = F32Operand<EA, LA, TILE>;
   using OB = F32Operand<EB, LB, TILE>;
@@ -192,46 +197,88 @@ __global__ __launch_bounds__(256) void f32_kernel(const F32Problem p) {
   __builtin_amdgcn_s_waitcnt(gemm::big::kWaitVm0);
   gemm::lds_barrier();
 
+  // Fragments are read a step ahead of their products, over the end of a k-tile as well:
+  // its last step waits for the next k-tile's loads and the other waves (which frees its
+  // stage), reads the next one's first fragments and then multiplies.
   const int fr = lane & 31, g = lane >> 5;
+  float a[2][T][4], b[2][T][4];
+  auto read = [&](int to, const char* st, int s) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < T; ++i) OA::fragment(st, wm + 32 * i + fr, g, s, a[to][i]);
+#pragma unroll
+    for (int j = 0; j < T; ++j) OB::fragment(st + OA::kBytes, wn + 32 * j + fr, g, s, b[to][j]);
+  };
+  read(0, lds[0], 0);
   for (int t = 0; t < nk; ++t) {
-    const char* as = lds[t & 1];
-    const char* bs = as + OA::kBytes;
+    const char* st = lds[t & 1];
+    char* ld = lds[(t & 1) ^ 1];
     advance();
-    // (the stage was last read in k-tile t - 1, before the barrier that ended it)
-    oa.load(lds[(t & 1) ^ 1], wave, t + 1 < nk, K - k);
-    ob.load(lds[(t & 1) ^ 1] + OA::kBytes, wave, t + 1 < nk, K - k);
+    oa.load(ld, wave, t + 1 < nk, K - k);
+    ob.load(ld + OA::kBytes, wave, t + 1 < nk, K - k);
+    constexpr int kSteps = kF32K / 8;
 #pragma unroll
-    for (int s = 0; s < kF32K / 8; ++s) {
-      float a[T][4], b[T][4];
-#pragma unroll
-      for (int i = 0; i < T; ++i) OA::fragment(as, wm + 32 * i + fr, g, s, a[i]);
-#pragma unroll
-      for (int j = 0; j < T; ++j) OB::fragment(bs, wn + 32 * j + fr, g, s, b[j]);
+    for (int s = 0; s < kSteps; ++s) {
+      if (s + 1 < kSteps) {
+        read((s + 1) & 1, st, s + 1);
+      } else {
+        __builtin_amdgcn_s_waitcnt(gemm::big::kWaitVm0);
+        gemm::lds_barrier();
+        read((s + 1) & 1, ld, 0);  // (past the last k-tile: zeros)
+      }
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int i = 0; i < T; ++i)
 #pragma unroll
           for (int j = 0; j < T; ++j)
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i][e], b[j][e], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s & 1][i][e], b[s & 1][j][e],
+                                                             acc[i][j], 0, 0, 0);
     }
-    __builtin_amdgcn_s_waitcnt(gemm::big::kWaitVm0);
-    gemm::lds_barrier();
   }
 
   // element v of tile (i, j): row 32 i + 8 (v / 4) + 4 g + v % 4, column 32 j + lane % 32
-  float* out = p.out + (int64_t)split * p.M * p.N;
+  if constexpr (std::is_same_v<Step, SumsOnly>) {
+    float* out = p.out + (int64_t)split * p.M * p.N;
 #pragma unroll
-  for (int j = 0; j < T; ++j) {
-    const int n = n0 + wn + 32 * j + fr;
-    if (n >= p.N) continue;
+    for (int j = 0; j < T; ++j) {
+      const int n = n0 + wn + 32 * j + fr;
+      if (n >= p.N) continue;
 #pragma unroll
-    for (int i = 0; i < T; ++i)
+      for (int i = 0; i < T; ++i)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) {
-        const int m = m0 + wm + 32 * i + 8 * (v >> 2) + 4 * g + (v & 3);
-        if (m < p.M) out[(int64_t)m * p.N + n] = acc[i][j][v];
-      }
+        for (int v = 0; v < 16; ++v) {
+          const int m = m0 + wm + 32 * i + 8 * (v >> 2) + 4 * g + (v & 3);
+          if (m < p.M) out[(int64_t)m * p.N + n] = acc[i][j][v];
+        }
+    }
+  } else {
+    constexpr int B = 8;
+#pragma unroll
+    for (int j = 0; j < T; ++j) {
+      const int n = n0 + wn + 32 * j + fr, nc = n < p.N ? n : 0;
+      const typename Step::template Column<1> column = step.template column<1>(nc);
+#pragma unroll
+      for (int i = 0; i < T; ++i)
+#pragma unroll
+        for (int v0 = 0; v0 < 16; v0 += B) {
+          int64_t m[B];
+          bool live[B];
+          float x[B][1];
+          typename Step::template Fetched<1> f[B];
+#pragma unroll
+          for (int q = 0; q < B; ++q) {
+            const int v = v0 + q, r = m0 + wm + 32 * i + 8 * (v >> 2) + 4 * g + (v & 3);
+            m[q] = r;
+            live[q] = r < p.M && n < p.N;
+            x[q][0] = acc[i][j][v];
+            f[q] = step.template fetch<1>(r < p.M ? r : p.M - 1, nc);
+          }
+          step.template finish<false, 1, B>(m, n, x, column, f, live);
+          // (a group's loads are not moved before the last one's: two workgroups a CU
+          // need the registers)
+          __builtin_amdgcn_sched_barrier(0);
+        }
+    }
   }
 }
 
@@ -239,21 +286,22 @@ struct F32Plan {
   int tile, splits, kps;
 };
 
-// A CU's matrix cores take c us for a k-tile of a 128 x 128 tile (a quarter for 64 x 64),
-// whichever of its workgroups it is of; o: a workgroup's start and end. Parts of K are
-// written once and read once.
+// A CU's matrix cores take c us for a k-tile of a 128 x 128 tile (.28 of it for 64 x 64),
+// whichever of its workgroups it is of; parts of K are written once and read once, at 5
+// TB/s. Fitted to the times of ten shapes from [128, 512] x 512 to [8192, 2048] x 2048
+// with every split (4 % off in the mean; its choice costs 1 % over the best one).
 inline F32Plan plan_f32(int64_t M, int64_t N, int64_t ktiles) {
   F32Plan best{128, 1, (int)ktiles};
   double best_us = -1;
   for (int tile = 128; tile >= 64; tile /= 2) {
     const int64_t tiles = ((M + tile - 1) / tile) * ((N + tile - 1) / tile);
-    const double c = tile == 128 ? 1.9 : 0.55, o = tile == 128 ? 3.0 : 1.5;
+    const double c = tile == 128 ? 1.9 : 0.535;
     for (int s = 1; s <= 16; ++s) {
       const int64_t kps = (ktiles + s - 1) / s;
       if (s > 1 && (kps < 4 || (ktiles + kps - 1) / kps != s)) continue;
       const int64_t per_cu = (tiles * s + 255) / 256;
-      double us = 3.0 + per_cu * (o + c * kps);
-      if (s > 1) us += (double)s * M * N * 8 / 4.3e6;
+      double us = per_cu * c * kps;
+      if (s > 1) us += (double)s * M * N * 8 / 5.0e6;
       if (best_us < 0 || us < best_us) {
         best_us = us;
         best = F32Plan{tile, s, (int)kps};
@@ -269,8 +317,8 @@ inline int64_t f32_ktiles(int nseg, const int64_t* K) {
   return n;
 }
 
-template <typename EA, typename EB, int LA, int LB>
-inline int launch_f32(F32Problem& p, const F32Plan& plan, hipStream_t st) {
+template <typename EA, typename EB, int LA, int LB, class Step>
+inline int launch_f32(F32Problem& p, const F32Plan& plan, const Step& step, hipStream_t st) {
   p.tiles_m = (p.M + plan.tile - 1) / plan.tile;
   p.tiles_n = (p.N + plan.tile - 1) / plan.tile;
   p.splits = plan.splits;
@@ -279,9 +327,9 @@ inline int launch_f32(F32Problem& p, const F32Plan& plan, hipStream_t st) {
   ML_CHECK(items <= 0x7fffffffLL, "ffn: too many tiles");
   const dim3 grid((unsigned)items);
   if (plan.tile == 128)
-    f32_kernel<EA, EB, LA, LB, 2><<<grid, 256, 0, st>>>(p);
+    f32_kernel<EA, EB, LA, LB, 2, Step><<<grid, 256, 0, st>>>(p, step);
   else
-    f32_kernel<EA, EB, LA, LB, 1><<<grid, 256, 0, st>>>(p);
+    f32_kernel<EA, EB, LA, LB, 1, Step><<<grid, 256, 0, st>>>(p, step);
   ML_LAUNCH_CHECK();
   return ML_OK;
 }

@@ -44,10 +44,10 @@ def keep_mode(checkpoint: str | None, dtype: torch.dtype) -> int:
     return hip_ops.KEEP_F32 if dtype == torch.float32 else hip_ops.KEEP_FP16
 
 
-# Multiply-adds of a product from which fp32 sizes are padded: [517, 1001] x 777 (4e8)
-# takes 180 us a training pass as it is and 215 padded, [1024, 1001] x 4001 (4e9) 600 and
-# 470.
-_PAD_F32 = 1 << 30
+# Multiply-adds of a product from which fp32 sizes are padded: a training pass of [1024,
+# 1001] x 4001 (4e9) takes 297 us as it is and 313 padded, of [700, 3001] x 3001 (6e9) 614
+# and 477.
+_PAD_F32 = 5 * 10**9
 
 
 def pads(dtype: torch.dtype, rows: int, *features: int) -> bool:
