@@ -704,7 +704,8 @@ int ml_swiglu_mlp_fwd(const void* x, int64_t ldx, const void* wg, int64_t ldg, c
 /*
  * Its backward, of dy [M, O] (ldy) and the kept g and u: dx [M, H], dwg and dwu
  * [I, H], dwd [O, I], each dense, or NULL where it is not wanted. h is formed again
- * of the kept g and u.
+ * of the kept g and u. x is read only for dwg and dwu (NULL otherwise), wg and wu only
+ * for dx.
  */
 size_t ml_swiglu_mlp_bwd_workspace_bytes(int64_t M, int64_t H, int64_t I, int64_t O, int dtype);
 int ml_swiglu_mlp_bwd(const void* x, int64_t ldx, const void* wg, int64_t ldg, const void* wu,

@@ -379,8 +379,11 @@ def _swiglu_mlp_fwd_fake(x2, wg, wu, wd, residual, keep):
 
 
 def _swiglu_mlp_bwd_fake(x2, wg, wu, wd, dy, keep, gate, gate_scale, up, up_scale, *needs):
-    shapes = (x2.shape, wg.shape, wu.shape, wd.shape)
-    return tuple(x2.new_empty(s if need else (0,)) for s, need in zip(shapes, needs))
+    I = wd.shape[1]  # noqa: E741
+    H = hip_ops.mlp_hidden(x2, wg, I)
+    into = (I, H)
+    shapes = ((dy.shape[0], H), into, into, wd.shape)
+    return tuple(dy.new_empty(s if need else (0,)) for s, need in zip(shapes, needs))
 
 
 swiglu_kept_fwd = _define("swiglu_kept_fwd(Tensor gate, Tensor up) -> "
@@ -409,7 +412,7 @@ swiglu_mlp_infer = _define("swiglu_mlp_infer(Tensor x2, Tensor wg, Tensor wu, Te
                            "Tensor? residual) -> Tensor", hip_ops.swiglu_mlp_infer,
                            lambda x2, wg, wu, wd, residual:
                            x2.new_empty((x2.shape[0], wd.shape[0])))
-swiglu_mlp_bwd = _define("swiglu_mlp_bwd(Tensor x2, Tensor wg, Tensor wu, Tensor wd, Tensor dy, "
+swiglu_mlp_bwd = _define("swiglu_mlp_bwd(Tensor? x2, Tensor? wg, Tensor? wu, Tensor wd, Tensor dy, "
                          "int keep, Tensor gate, Tensor gate_scale, Tensor up, Tensor up_scale, "
                          "bool need_dx, bool need_dwg, bool need_dwu, bool need_dwd) -> "
                          "(Tensor, Tensor, Tensor, Tensor)", hip_ops.swiglu_mlp_bwd,

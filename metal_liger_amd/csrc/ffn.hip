@@ -378,7 +378,7 @@ bool few(int64_t M) {
 }
 
 int check_sizes(int64_t M, int64_t N, int64_t K) {
-  constexpr int64_t kMax = 1LL << 31;
+  constexpr int64_t kMax = (1LL << 31) - 1024;  // (a last tile's rows are counted in 32 bits)
   ML_CHECK(M > 0 && N > 0 && K > 0 && M < kMax && N < kMax && K < kMax,
            "ffn: bad sizes (rows %lld, columns %lld, %lld)", (long long)M, (long long)N,
            (long long)K);
@@ -556,13 +556,14 @@ int mlp_fwd(const MlpFwd& p, Arena& ws, bool run, hipStream_t st) {
   if (fuse_in) {
     rc = P::through_pair(p.M, p.I, p.H, x, p.ldx, wg, p.ldg, wu, p.ldu, step, st);
   } else {
+    int splits_up = 1;  // (the two weights may lie so that their products split differently)
     rc = P::template raw<kKMajor>(p.M, p.I, p.H, x, p.ldx, wg, p.ldg, sums, splits, st);
     if (rc) return rc;
-    rc = P::template raw<kKMajor>(p.M, p.I, p.H, x, p.ldx, wu, p.ldu, sums + n_in, splits, st);
+    rc = P::template raw<kKMajor>(p.M, p.I, p.H, x, p.ldx, wu, p.ldu, sums + n_in, splits_up, st);
     if (rc) return rc;
     const int64_t mi = p.M * p.I;
     rc = launch_rows(p.I % 8 == 0, PartialSource{sums, splits, mi, p.I},
-                     PartialSource{sums + n_in, splits, mi, p.I}, step, p.M, p.I, st);
+                     PartialSource{sums + n_in, splits_up, mi, p.I}, step, p.M, p.I, st);
   }
   if (rc) return rc;
   if (fuse_out) return P::template through<kKMajor>(p.M, p.O, p.I, h, p.I, wd, p.ldd, out, st);
@@ -813,8 +814,9 @@ extern "C" int ml_swiglu_mlp_bwd(const void* x, int64_t ldx, const void* wg, int
                                  int64_t I, int64_t O, void* workspace, size_t workspace_bytes,
                                  int dtype, void* stream) {
   ML_TRY(ffn::check_mlp(M, H, I, O));
-  ML_CHECK(x && wg && wu && wd && dy, "swiglu mlp backward: null pointer");
-  ML_CHECK(ldx >= H && ldg >= H && ldu >= H && ldd >= I && ldy >= O,
+  ML_CHECK(wd && dy && (!dx || (wg && wu)) && (!(dwg || dwu) || x),
+           "swiglu mlp backward: null pointer");
+  ML_CHECK((!x || ldx >= H) && (!wg || ldg >= H) && (!wu || ldu >= H) && ldd >= I && ldy >= O,
            "swiglu mlp backward: bad row strides");
   ML_CHECK(keep != ffn::kKeepNone, "swiglu mlp backward: gate and up were not kept");
   ML_TRY(ffn::check_kept(keep, gate, gate_scale, "gate"));
@@ -822,9 +824,9 @@ extern "C" int ml_swiglu_mlp_bwd(const void* x, int64_t ldx, const void* wg, int
   if (!dx && !dwg && !dwu && !dwd) return ML_OK;
   return dispatch_dtype(dtype, [&](auto t) -> int {
     using T = decltype(t);
-    ML_TRY(ffn::check<T>(x, ldx, H, "x"));
-    ML_TRY(ffn::check<T>(wg, ldg, H, "gate weight"));
-    ML_TRY(ffn::check<T>(wu, ldu, H, "up weight"));
+    ML_TRY(ffn::check<T>(x, x ? ldx : 0, H, "x"));
+    ML_TRY(ffn::check<T>(wg, wg ? ldg : 0, H, "gate weight"));
+    ML_TRY(ffn::check<T>(wu, wu ? ldu : 0, H, "up weight"));
     ML_TRY(ffn::check<T>(wd, ldd, I, "down weight"));
     ML_TRY(ffn::check<T>(dy, ldy, O, "dy"));
     ML_TRY(ffn::check<T>(dx, H, H, "dx"));

@@ -153,6 +153,19 @@ def swiglu_bwd(gate: torch.Tensor, up: torch.Tensor, dy: torch.Tensor):
     return dg, du
 
 
+def _on_device(fn):
+    """fn with its tensors' device as the current one (launches and properties of the
+    device go by it), however the caller's stands."""
+    @functools.wraps(fn)
+    def on_device(*args):
+        t = next((a for a in args if isinstance(a, torch.Tensor)), None)
+        if t is None or not t.is_cuda or t.get_device() == torch.cuda.current_device():
+            return fn(*args)
+        with torch.cuda.device(t.get_device()):
+            return fn(*args)
+    return on_device
+
+
 # What a backward needs of its forward, kept in fp32 or in 16 or 8 bits with scales
 # (ML_KEEP_*).
 KEEP_NONE, KEEP_F32, KEEP_FP16, KEEP_FP8 = 0, 1, 2, 3
@@ -175,6 +188,7 @@ def kept_layout(rows, cols, keep: int):
             (scales if keep >= KEEP_FP16 else (0,), torch.uint8))
 
 
+@_on_device
 def swiglu_kept_fwd(gate: torch.Tensor, up: torch.Tensor):
     """swiglu_fwd, and gate and up in 8 bits: (out, gate's bytes, scales, up's)."""
     ensure_rocm_device(gate, up)
@@ -190,6 +204,7 @@ def swiglu_kept_fwd(gate: torch.Tensor, up: torch.Tensor):
     return (out if out.dtype == gate.dtype else out.to(gate.dtype), *kept)
 
 
+@_on_device
 def swiglu_kept_bwd(gate_q, gate_scale, up_q, up_scale, dy, gate_dtype, up_dtype):
     """(dgate, dup) in the given dtypes, of dy's shape."""
     ensure_rocm_device(gate_q, gate_scale, up_q, up_scale, dy)
@@ -208,6 +223,7 @@ def swiglu_kept_bwd(gate_q, gate_scale, up_q, up_scale, dy, gate_dtype, up_dtype
     return dg.to(gate_dtype), du.to(up_dtype)
 
 
+@_on_device
 def held_values(q: torch.Tensor, scale: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
     """What a tensor kept in 8 bits stands for, in dtype."""
     ensure_rocm_device(q, scale)
@@ -274,6 +290,7 @@ def _linear(x2, w, bias, residual, act: int, keep: int, z, zscale):
     return y
 
 
+@_on_device
 def linear_fwd(x2, w, bias, residual, act: int, keep: int):
     """(y, z, zscale) of ml_linear_fwd: x2 [M, K], w [N, K], bias [N] or None, residual
     [M, N] or None, all fp32, or all bf16 or fp16 (sizes in multiples of 8)."""
@@ -281,11 +298,13 @@ def linear_fwd(x2, w, bias, residual, act: int, keep: int):
     return (_linear(x2, w, bias, residual, act, keep, *kept), *kept)
 
 
+@_on_device
 def linear_infer(x2, w, bias, residual, act: int):
     """linear_fwd's y with nothing kept."""
     return _linear(x2, w, bias, residual, act, KEEP_NONE, None, None)
 
 
+@_on_device
 def linear_bwd(x2, w, dy, act: int, keep: int, z, zscale, N: int, K: int, need_dx: bool,
                need_dw: bool, need_db: bool):
     """(dx, dw, db) of ml_linear_bwd, [0] where not wanted. x2 only for dw, w only for
@@ -324,6 +343,7 @@ def _swiglu_mlp(x2, wg, wu, wd, residual, keep: int, kept):
     return y
 
 
+@_on_device
 def swiglu_mlp_fwd(x2, wg, wu, wd, residual, keep: int):
     """(y, gate, gate_scale, up, up_scale) of ml_swiglu_mlp_fwd: x2 [M, H], wg and wu
     [I, H], wd [O, I], residual [M, O] or None; dtypes as linear_fwd."""
@@ -331,31 +351,42 @@ def swiglu_mlp_fwd(x2, wg, wu, wd, residual, keep: int):
     return (_swiglu_mlp(x2, wg, wu, wd, residual, keep, kept), *kept)
 
 
+@_on_device
 def swiglu_mlp_infer(x2, wg, wu, wd, residual):
     """swiglu_mlp_fwd's y with nothing kept."""
     return _swiglu_mlp(x2, wg, wu, wd, residual, KEEP_NONE, (None,) * 4)
 
 
 def _pairs(*ts):
-    """pointer, row stride of each"""
-    return [v for t in ts for v in (ptr(t), row_stride(t))]
+    """pointer, row stride of each; None and 0 of None"""
+    return [v for t in ts for v in (ptr(t), 0 if t is None else row_stride(t))]
 
 
+def mlp_hidden(x2, wg, default: int) -> int:
+    """The block's input width; any where no gradient has it."""
+    return x2.shape[1] if x2 is not None else wg.shape[1] if wg is not None else default
+
+
+@_on_device
 def swiglu_mlp_bwd(x2, wg, wu, wd, dy, keep: int, gate, gate_scale, up, up_scale, need_dx: bool,
                    need_dwg: bool, need_dwu: bool, need_dwd: bool):
-    """(dx, dwg, dwu, dwd) of ml_swiglu_mlp_bwd, [0] where not wanted."""
+    """(dx, dwg, dwu, dwd) of ml_swiglu_mlp_bwd, [0] where not wanted. x2 only for dwg and
+    dwu, wg and wu only for dx."""
     ensure_rocm_device(x2, wg, wu, wd, dy, gate, gate_scale, up, up_scale)
-    (M, H), (O, I) = x2.shape, wd.shape  # noqa: E741
-    new = lambda need, *s: torch.empty(s if need else (0,), dtype=x2.dtype, device=x2.device)  # noqa: E731
+    M, (O, I) = dy.shape[0], wd.shape  # noqa: E741
+    H = mlp_hidden(x2, wg, I)
+    new = lambda need, *s: torch.empty(s if need else (0,), dtype=dy.dtype, device=dy.device)  # noqa: E731
     outs = [new(need_dx, M, H), new(need_dwg, I, H), new(need_dwu, I, H), new(need_dwd, O, I)]
     if M == 0:
         return tuple(t.zero_() for t in outs)
-    x2, wg, wu, wd, dy = map(_product_rows, (x2, wg, wu, wd, dy))
-    tag = dtype_tag(x2, "x")
-    ws, wsb = _workspace(x2, "ml_swiglu_mlp_bwd_workspace_bytes", M, H, I, O, tag)
+    x2 = _product_rows(x2) if need_dwg or need_dwu else None
+    wg, wu = (_product_rows(wg), _product_rows(wu)) if need_dx else (None, None)
+    wd, dy = _product_rows(wd), _product_rows(dy)
+    tag = dtype_tag(dy, "grad")
+    ws, wsb = _workspace(dy, "ml_swiglu_mlp_bwd_workspace_bytes", M, H, I, O, tag)
     call("ml_swiglu_mlp_bwd", *_pairs(x2, wg, wu, wd, dy), keep,
          *(ptr(_used(t)) for t in (gate, gate_scale, up, up_scale)), *(ptr(_used(t)) for t in outs),
-         M, H, I, O, ptr(ws), wsb, tag, stream_of(x2))
+         M, H, I, O, ptr(ws), wsb, tag, stream_of(dy))
     return tuple(outs)
 
 

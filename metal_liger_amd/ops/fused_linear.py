@@ -164,10 +164,11 @@ def fused_linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | Non
     """act(x weight^T + bias) + residual.
 
     x [..., in], weight [out, in] (nn.Linear's), bias [out], residual [..., out]; all of
-    x's dtype (fp32, bf16 or fp16) and on its device, any strides. activation: None,
-    "silu", "gelu" (by the error function, nn.GELU's default) or "gelu_tanh" (nn.GELU's
-    approximate="tanh"); the residual is added after it. checkpoint: None, or "fp8" to
-    keep what the activation's backward needs in 8 bits (module docstring).
+    x's dtype (fp32, bf16 or fp16; autocast casts none of them) and on its device, any
+    strides. activation: None, "silu", "gelu" (by the error function, nn.GELU's default)
+    or "gelu_tanh" (nn.GELU's approximate="tanh"); the residual is added after it.
+    checkpoint: None, or "fp8" to keep what the activation's backward needs in 8 bits
+    (module docstring).
     """
     if activation not in ACTIVATIONS:
         raise ValueError(f"fused_linear: activation {activation!r} is not one of "
@@ -215,11 +216,16 @@ class MetalLigerLinear(nn.Module):
 _HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
 
 
+def hooked(module) -> bool:
+    """Whether hooks want the module to be called, and to see what it returns."""
+    return any(getattr(module, name, None) for name in _HOOKS)
+
+
 def plain_linear(module) -> bool:
     """An nn.Linear as it is: an adapter's wrapper or a subclass may compute something
     else, and hooks (or a replaced forward) want the module to be called."""
     return (type(module) is nn.Linear and "forward" not in module.__dict__
-            and not any(getattr(module, name, None) for name in _HOOKS))
+            and not hooked(module))
 
 
 def runs_fused(x, *linears) -> bool:
@@ -252,7 +258,7 @@ class _FusedVisionMLPForward:
 
     def __call__(self, hidden_state, residual=None):
         fc1, fc2 = self.mlp.linear_fc1, self.mlp.linear_fc2
-        if not runs_fused(hidden_state, fc1, fc2):
+        if hooked(self.mlp.act_fn) or not runs_fused(hidden_state, fc1, fc2):
             out = self.original(hidden_state)
             return out if residual is None else residual + out
         fused = residual is not None and residual.dtype == hidden_state.dtype and \
@@ -316,6 +322,8 @@ class _FusedVisionBlockForward:
         extra = rest.pop(self.var_kw, {}) if self.var_kw else {}
         h, b = rest.pop("hidden_states"), self.block
         h = h + b.attn(b.norm1(h), **rest, **extra)
+        if hooked(b.mlp):  # (they see the MLP's own output)
+            return h + b.mlp(b.norm2(h))
         return b.mlp(b.norm2(h), residual=h)
 
 

@@ -3,10 +3,12 @@
 ops/fused_swiglu.py:59-75, and its LoRA block needs adapters).
 
 The backward needs gate = x Wg^T and up = x Wu^T: they are kept in 16 bits (fp16 with a
-power of two as scale for every 32 columns of a row; fp32 in fp32), or in 8 (checkpoint="fp8": e4m3 with such scales), formed of the fp32 sums. h = silu(gate) * up is not kept; the backward forms it
-again of what was kept. h and the gradients of gate, up and h are rounded to bf16
-between the products on the bf16 matrix cores. First derivatives only. Types and sizes
-as ops/fused_linear.py.
+power of two as scale for every 32 columns of a row; fp32 in fp32), or in 8
+(checkpoint="fp8": e4m3 with such scales), formed of the fp32 sums. h = silu(gate) * up
+is not kept; the backward forms it again of what was kept. What is not needed (x where
+gate's and up's weights are frozen) is not kept. h and the gradients of gate, up and h
+are rounded to bf16 between the products on the bf16 matrix cores. First derivatives
+only. Types and sizes as ops/fused_linear.py.
 """
 
 from __future__ import annotations
@@ -20,8 +22,8 @@ from metal_liger_amd import _custom_ops as cops
 from metal_liger_amd import hip_ops
 from metal_liger_amd._model_walk import find_layers
 from metal_liger_amd.ops.fused_linear import (check_checkpoint, check_input, check_residual, cut,
-                                              keep_mode, pad, pads, plain_linear, rows, runs_fused,
-                                              wants_grad)
+                                              hooked, keep_mode, pad, pads, plain_linear, rows,
+                                              runs_fused, wants_grad)
 from metal_liger_amd.ops.fused_swiglu import MetalLigerSwiGLU
 
 logger = logging.getLogger(__name__)
@@ -47,8 +49,10 @@ class _FusedSwiGLUMLPFunction(torch.autograd.Function):
         if not any(ctx.needs_input_grad[:4]):
             keep = hip_ops.KEEP_NONE
         y, *kept = _forward(x, (wg, wu, wd), residual, keep)
-        ctx.save_for_backward(x, wg, wu, wd, *kept)
-        ctx.keep = keep
+        need_dx, need_dwg, need_dwu = ctx.needs_input_grad[:3]
+        ctx.save_for_backward(x if need_dwg or need_dwu else None, *((wg, wu) if need_dx else
+                              (None, None)), wd, *kept)
+        ctx.keep, ctx.x_shape = keep, x.shape
         return y
 
     @staticmethod
@@ -56,15 +60,16 @@ class _FusedSwiGLUMLPFunction(torch.autograd.Function):
         grads = [None] * 4
         if any(ctx.needs_input_grad[:4]):
             x, wg, wu, wd, *kept = ctx.saved_tensors
-            M, H = x.numel() // x.shape[-1], x.shape[-1]
-            p = pads(x.dtype, M, H, wd.shape[1])
+            H, (O, I) = ctx.x_shape[-1], wd.shape  # noqa: E741
+            M = ctx.x_shape.numel() // H
+            p = pads(dy.dtype, M, H, I)
             weights = [pad(w, 0, 1) for w in (wg, wu, wd)] if p else (wg, wu, wd)
             outs = cops.swiglu_mlp_bwd(rows(x, p), *weights, rows(dy, p), ctx.keep, *kept,
                                        *ctx.needs_input_grad[:4])
             grads = [cut(g, *sizes) if need else None for g, sizes, need in
-                     zip(outs, ((M, H), wg.shape, wu.shape, wd.shape), ctx.needs_input_grad)]
-            if grads[0] is not None and x.dim() != 2:
-                grads[0] = grads[0].view(x.shape)
+                     zip(outs, ((M, H), (I, H), (I, H), (O, I)), ctx.needs_input_grad)]
+            if grads[0] is not None and len(ctx.x_shape) != 2:
+                grads[0] = grads[0].view(ctx.x_shape)
         return (*grads, dy if ctx.needs_input_grad[4] else None, None)
 
 
@@ -74,8 +79,9 @@ def fused_swiglu_mlp(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torc
     """(silu(x gate_weight^T) * (x up_weight^T)) down_weight^T + residual.
 
     x [..., hidden], gate_weight and up_weight [inter, hidden], down_weight [out, inter],
-    residual [..., out]; all of x's dtype (fp32, bf16 or fp16) and on its device, any
-    strides. checkpoint: None, or "fp8" to keep gate and up in 8 bits for the backward.
+    residual [..., out]; all of x's dtype (fp32, bf16 or fp16; autocast casts none of
+    them) and on its device, any strides. checkpoint: None, or "fp8" to keep gate and up in
+    8 bits for the backward.
     """
     check_checkpoint(checkpoint)
     check_input("fused_swiglu_mlp", x, gate_weight, up_weight, down_weight)
@@ -137,7 +143,7 @@ class _FusedMLPForward:
 
     def __call__(self, x):
         gate, up, down = (getattr(self.mlp, name) for name in _PROJECTIONS)
-        if not runs_fused(x, gate, up, down):
+        if hooked(getattr(self.mlp, "act_fn", None)) or not runs_fused(x, gate, up, down):
             return self.original(x)
         return fused_swiglu_mlp(x, gate.weight, up.weight, down.weight, checkpoint=self.checkpoint)
 

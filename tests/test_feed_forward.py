@@ -125,6 +125,7 @@ def test_host_side_argument_errors():
 
     refused(linear(M=0), b"bad sizes")
     refused(linear(M=1 << 31), b"bad sizes")
+    refused(linear(M=(1 << 31) - 1), b"bad sizes")
     refused(linear(x=None), b"null pointer")
     refused(linear(act=4), b"bad activation")
     refused(linear(ldx=56), b"row strides")
@@ -326,6 +327,64 @@ def test_patcher_routes_vision_mlps(monkeypatch):
         m.setattr(torch, "is_autocast_enabled", lambda device=None: True)
         assert torch.equal(block.mlp(x), want)
         assert torch.equal(block.mlp(x, residual=r), r + want)
+
+
+def test_hooks_see_what_their_module_returns(monkeypatch):
+    """A hook on an activation is called, one on an MLP sees its output alone."""
+    model = qwen_tiny.build_vl()
+    apply_metal_liger_to_qwen3vl(model, fuse_vision_mlp=True)
+    block = model.model.visual.blocks[0]
+    x, seen = seeded((4, 64), 1), []
+    own = block.mlp.linear_fc2(block.mlp.act_fn(block.mlp.linear_fc1(x)))
+    handle = block.mlp.act_fn.register_forward_hook(lambda *a: seen.append("act"))
+    assert torch.equal(block.mlp(x), own) and seen == ["act"]
+    handle.remove()
+    block.mlp.register_forward_hook(lambda module, args, out: seen.append(out))
+    monkeypatch.setattr(torch, "is_autocast_enabled", lambda device=None: True)
+    block.attn.forward = lambda h, **kw: torch.zeros_like(h)
+    out = block(x, cu_seqlens=None)
+    want = block.mlp.linear_fc2(block.mlp.act_fn(block.mlp.linear_fc1(block.norm2(x))))
+    assert torch.equal(seen[-1], want) and torch.equal(out, x + want)
+
+    decoder = qwen_tiny.build_vl()
+    mlp = next(m for m in decoder.modules() if hasattr(m, "gate_proj"))
+    routed = fm._FusedMLPForward(mlp, mlp.forward, None)
+    x = seeded((4, mlp.gate_proj.weight.shape[1]), 2)
+    mlp.act_fn.register_forward_hook(lambda *a: seen.append("act"))
+    assert torch.equal(routed(x), mlp(x)) and seen[-2:] == ["act", "act"]
+
+
+def test_current_device(monkeypatch):
+    """Tensors on another device than the current one: the call is made under theirs."""
+    entered = []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            entered.append(self.index)
+
+        def __exit__(self, *exc):
+            entered.append("out")
+
+    class OnDevice(torch.Tensor):
+        is_cuda = True
+
+        def get_device(self):
+            return 1
+
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    x = torch.ones(2).as_subclass(OnDevice)
+    f = hip_ops._on_device(lambda *args: list(entered))
+    for current, want in ((1, []), (0, [1])):
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: current)
+        assert f(None, x) == want
+    assert entered == [1, "out"]
+    assert f(None, 3) == [1, "out"]
+    for name in ("swiglu_kept_fwd", "swiglu_kept_bwd", "held_values", "linear_fwd", "linear_infer",
+                 "linear_bwd", "swiglu_mlp_fwd", "swiglu_mlp_infer", "swiglu_mlp_bwd"):
+        assert hasattr(getattr(hip_ops, name), "__wrapped__")
 
 
 def test_activation_names():

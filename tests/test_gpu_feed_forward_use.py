@@ -171,6 +171,41 @@ def test_what_is_kept(dev):
     assert kept(_swiglu(g, u, checkpoint="fp8"), ()) == 2 * (M * N + M * N // 32)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+def test_what_a_frozen_block_keeps(dev, dtype):
+    """x is kept for the gradients of gate's and up's weights alone, these weights for x's."""
+    M, H, I, O = 100, 72, 104, 40  # noqa: E741
+    make = [((M, H), 1.0), ((I, H), 0.1), ((I, H), 0.1), ((O, I), 0.1), ((M, O), 1.0)]
+    for mask in range(1, 32):
+        ts = [seeded(s, i, dtype, c).to(dev).requires_grad_(bool(mask >> i & 1))
+              for i, (s, c) in enumerate(make)]
+        y = _mlp(*ts)
+        saved = {t.data_ptr() for t in y.grad_fn.saved_tensors if t is not None}
+        for t, needed in zip(ts, (mask & 6, mask & 1, mask & 1, True, False)):
+            assert (t.data_ptr() in saved) == bool(needed)
+
+
+def test_c_entry_of_weights_that_lie_differently(dev):
+    """fp32 weights of which one is 16-byte aligned and one is not: their products run on
+    different kernels, which may split K differently."""
+    from metal_liger_amd import _hip
+    M, H, I, O = 200, 2048, 264, 64  # noqa: E741
+    x, wd = seeded((M, H), 1).to(dev), seeded((O, I), 4, scale=0.1).to(dev)
+    wg = seeded((I, H), 2, scale=0.1).to(dev)
+    wu = torch.empty(I * H + 1, device=dev)[1:].view(I, H).copy_(seeded((I, H), 3, scale=0.1))
+    n = _hip.query("ml_swiglu_mlp_fwd_workspace_bytes", M, H, I, O, 0)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    for a, b in ((wg, wu), (wu, wg)):
+        y = torch.empty(M, O, device=dev)
+        _hip.call("ml_swiglu_mlp_fwd", x.data_ptr(), H, a.data_ptr(), H, b.data_ptr(), H,
+                  wd.data_ptr(), I, None, 0, y.data_ptr(), 0, None, None, None, None, M, H, I, O,
+                  ws.data_ptr(), n, 0, torch.cuda.current_stream().cuda_stream)
+        g, u, d = (t.double().cpu() for t in (a, b, wd))
+        want = (F.silu(x.double().cpu() @ g.t()) * (x.double().cpu() @ u.t())) @ d.t()
+        # (2048 roundings of a sum of 2048 products, and fewer after them)
+        assert rel_fro(y, want) < 2048 * 2**-24
+
+
 def test_repeatable(dev):
     """The same bits at every call (no sum depends on the order of workgroups)."""
     x, w, b = _leaf((3000, 264), 1, dev), _leaf((1160, 264), 2, dev), _leaf((1160,), 3, dev)
