@@ -10,8 +10,8 @@
 //           dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T h
 //
 // bf16 runs on the bf16 matrix cores (gemm_core.h), fp32 and fp16 on the fp32 ones
-// (ffn_f32.h; what lies between fp16's products is fp32); forwards of up to 64 rows on
-// kernels of their own (ffn_skinny.h).
+// (ffn_f32.h; what lies between fp16's products is fp32); forwards of few rows (up to
+// 128) on kernels of their own (ffn_skinny.h).
 #include <initializer_list>
 
 #include "ffn_f32.h"
@@ -362,19 +362,45 @@ int dispatch_keep(int keep, F&& f) {
   return ML_ERR_INVALID;
 }
 
-// Whether a forward's product runs as one of few rows: any of 16-bit elements (whose
-// operands qualify as they are checked), those of fp32 whose widths and bases do.
-bool few_rows(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* w,
-              int64_t ldw) {
-  return M <= kSkinnyRows && N % 8 == 0 && K % 8 == 0 && aligned16(x) && aligned16(w) &&
-         ldx % 4 == 0 && ldw % 4 == 0;
+// Time in us of a product of up to 128 rows on the tiles (ops: 2 for the gated block's
+// pair): latency in bf16, the fp32 matrix cores' time otherwise. Fitted to 96 and 128 rows
+// by plan_skinny's shapes. What the two estimates choose, against workgroups for all of up
+// to 64 rows and tiles above: [80, 1024] to 1024 through 2816, the gated block in bf16, 44
+// -> 21 us, [64, 2048] x 16384 39 -> 19, [96, 4304] x 1152 24 -> 11, in fp16 26 -> 11.
+template <typename T>
+double tiles_us(int64_t M, int64_t N, int64_t K, int ops) {
+  const double all = (double)ops * N;
+  return std::is_same_v<T, bf16> ? (ops > 1 ? 19.5 : 11.5) + 1.5e-3 * K + 0.33e-3 * all
+                                 : 14 + (M > 64 ? 2e-6 : 1e-6) * all * K;
 }
 
-// Whether a forward of M rows needs no workspace for its sums: fp32 may yet run as one of
-// any size.
+// Whether a forward's product is one of few rows. (Kept tensors do not count, so that a
+// workspace goes by the sizes alone.)
 template <typename T>
-bool few(int64_t M) {
-  return !std::is_same_v<T, float> && M <= kSkinnyRows;
+bool few(int64_t M, int64_t N, int64_t K) {
+  return M <= kSkinnyRows &&
+         plan_skinny(sizeof(T), sizeof(T), 1, 1, M, N, K).us <= tiles_us<T>(M, N, K, 1);
+}
+
+template <typename T>
+bool few_mlp(int64_t M, int64_t H, int64_t I, int64_t O) {
+  return M <= kSkinnyRows &&
+         plan_skinny(sizeof(T), sizeof(T), 2, 1, M, I, H).us +
+                 plan_skinny(sizeof(Inner<T>), sizeof(T), 1, 1, M, O, I).us <=
+             tiles_us<T>(M, I, H, 2) + tiles_us<T>(M, O, I, 1);
+}
+
+// Whether such a product's operands can be read so: 16-bit ones always (they qualify as
+// they are checked), fp32 ones may not.
+bool few_operands(int64_t N, int64_t K, const void* x, int64_t ldx, const void* w, int64_t ldw) {
+  return N % 8 == 0 && K % 8 == 0 && aligned16(x) && aligned16(w) && ldx % 4 == 0 && ldw % 4 == 0;
+}
+
+// A product of few rows of 16-bit operands needs no workspace, and never comes to run
+// on another kernel.
+int few_checked(bool run) {
+  ML_CHECK(!run, "ffn: operands of few rows that were not checked");
+  return ML_OK;
 }
 
 int check_sizes(int64_t M, int64_t N, int64_t K) {
@@ -403,10 +429,11 @@ int linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
   const T* wt = static_cast<const T*>(w);
   const bool vec = N % 8 == 0 && aligned_rows(step.bias, 0) && aligned_rows(step.residual, step.ldr) &&
                    aligned_rows(step.y, step.ldy);
-  if (run && vec && few_rows(M, N, K, x, ldx, w, ldw))
+  const bool rows_few = few<T>(M, N, K);
+  if (run && vec && rows_few && few_operands(N, K, x, ldx, w, ldw))
     return launch_skinny<KIND != kKeepNone, false>(
         SkinnyProduct<T, T>{xt, wt, nullptr, ldx, ldw, 0, (int)M, (int)N, (int)K}, step, st);
-  if (few<T>(M) && !run) return ML_OK;
+  if (!std::is_same_v<T, float> && rows_few) return few_checked(run);
   if constexpr (std::is_same_v<T, bf16> || KIND == kKeepNone) {
     if (run && Products<T>::fused(M, N, K))
       return Products<T>::template through<kKMajor>(M, N, K, xt, ldx, wt, ldw, step, st);
@@ -517,7 +544,7 @@ struct MlpFwd {
 // The block of few rows: weights of T, h of TH (fp32 where T is fp16, whose range h may
 // leave).
 template <typename T, typename TH, int KIND>
-int few_mlp(const MlpFwd& p, const TH* h, const GatedStep<TH, KIND>& step,
+int launch_few_mlp(const MlpFwd& p, const TH* h, const GatedStep<TH, KIND>& step,
             const LinearStep<T, kKeepNone>& out, hipStream_t st) {
   const T *wg = static_cast<const T*>(p.wg), *wu = static_cast<const T*>(p.wu);
   const int rc = launch_skinny<KIND != kKeepNone, true>(
@@ -543,10 +570,11 @@ int mlp_fwd(const MlpFwd& p, Arena& ws, bool run, hipStream_t st) {
   const LinearStep<T, kKeepNone> out{nullptr, static_cast<const T*>(p.residual),
                                      static_cast<T*>(p.y), p.ldr, p.O, kActNone, {}};
   const bool vec = p.O % 8 == 0 && aligned_rows(p.residual, p.ldr) && aligned_rows(p.y, p.O);
-  if (run && vec && few_rows(p.M, p.I, p.H, x, p.ldx, wg, p.ldg) && aligned16(wu) &&
-      p.ldu % 4 == 0 && few_rows(p.M, p.O, p.I, h, p.I, wd, p.ldd))
-    return few_mlp<T, In>(p, h, step, out, st);
-  if (few<T>(p.M) && !run) return ML_OK;
+  const bool rows_few = few_mlp<T>(p.M, p.H, p.I, p.O);
+  if (run && vec && rows_few && few_operands(p.I, p.H, x, p.ldx, wg, p.ldg) && aligned16(wu) &&
+      p.ldu % 4 == 0 && few_operands(p.O, p.I, h, p.I, wd, p.ldd))
+    return launch_few_mlp<T, In>(p, h, step, out, st);
+  if (!std::is_same_v<T, float> && rows_few) return few_checked(run);
   const bool fuse_in = P::fused_pair(p.M, p.I, p.H), fuse_out = P::fused(p.M, p.O, p.I);
   const size_t n_in = fuse_in ? 0 : P::raw_floats(p.M, p.I, p.H);
   const size_t n_out = fuse_out ? 0 : P::raw_floats(p.M, p.O, p.I);

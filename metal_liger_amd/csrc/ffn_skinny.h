@@ -1,5 +1,5 @@
 // Products of few rows (single tokens, short prompts) through the steps of ffn_rows.h:
-//   C [M, N] = x [M, K] W [N, K]^T, M up to 64, W read once.
+//   C [M, N] = x [M, K] W [N, K]^T, M up to 128.
 //
 // Bound by W's bytes and by latency: [1, 2048] x 6144 in bf16 are 25 MB, 5 us at the
 // rate of a large copy. A workgroup takes 16 NT rows of W and all of K, its 8 waves every
@@ -12,6 +12,10 @@
 //   bf16 and fp16 by bf16 or fp16: v_mfma_f32_16x16x32 (exact products, fp32 sums)
 //   fp32 by fp32 or fp16: v_mfma_f32_16x16x4_f32, W upcast in registers
 // With PAIR a second W of the same shape beside it (gate and up).
+// Tiles of 16 rows of x are shared out over workgroups where that gives the CUs more to do
+// (plan_skinny); W then comes from the caches again. A workgroup for all of x's rows and
+// so: [64, 2048] to 512 columns in bf16 11.0 and 5.8 us, [64, 4304] to 1152 15.7 and 10.6,
+// [64, 6144] to 2048 29.4 and 19.2.
 #pragma once
 
 #include "ffn_rows.h"
@@ -22,7 +26,7 @@ namespace ffn {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kSkinnyWaves = 8;
-constexpr int kSkinnyRows = 64;  // most rows of x
+constexpr int kSkinnyRows = 128;  // most rows of x
 constexpr int kChunk = 64;       // k a chunk
 
 // A lane's 16 elements of a chunk (of one row, from k = 16 (lane / 16)): two halves of 8.
@@ -89,7 +93,7 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int r = lane & 15, G = lane >> 4;
-  const int n0 = blockIdx.x * 16 * NT;
+  const int n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
   // rows past the ends read the last one (their results are not used)
   const TW* wr[kOps][NT];
   const TX* xr[MT];
@@ -101,7 +105,7 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(
   }
 #pragma unroll
   for (int i = 0; i < MT; ++i) {
-    const int m = 16 * i + r < p.M ? 16 * i + r : p.M - 1;
+    const int m = m0 + 16 * i + r < p.M ? m0 + 16 * i + r : p.M - 1;
     xr[i] = p.x + m * p.ldx;
   }
   f32x4 acc[kOps][NT][MT];
@@ -167,9 +171,9 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(
   constexpr int kLanes = 2 * NT;
   constexpr int kPositions = 16 * MT * kLanes;
   for (int q = threadIdx.x; q < (kPositions + 63) / 64 * 64; q += 64 * kSkinnyWaves) {
-    const int m = q / kLanes, c = 8 * (q % kLanes), n = n0 + c;
+    const int row = q < kPositions ? q / kLanes : 0, c = 8 * (q % kLanes);
+    const int m = m0 + row, n = n0 + c;
     const bool live = m < p.M && n < p.N && q < kPositions;
-    const int row = q < kPositions ? m : 0;
     typename Step::template Column<8> column;
     typename Step::template Fetched<8> f[1];
     if (live) {
@@ -190,29 +194,51 @@ __global__ __launch_bounds__(64 * kSkinnyWaves) void skinny_kernel(
   }
 }
 
+// How many tiles of 16 rows a workgroup takes (mt, up to 4), and the time in us: a round of
+// 256 workgroups (one a CU; two that share one take as long as one after the other) goes
+// by K and the bytes that they read of W and x. nt: tiles of 16 rows of W; ops: 2 for a
+// pair. Fitted to 17 .. 256 rows by six shapes of W, 1152 x 4304 to 16384 x 2048, with
+// mt 1, 2 and 4, in bf16 and fp32, with and without a kept tensor.
+struct SkinnyPlan {
+  int mt;
+  double us;
+};
+
+inline SkinnyPlan plan_skinny(int x_size, int w_size, int ops, int nt, int64_t M, int64_t N,
+                              int64_t K) {
+  const int64_t blocks = (N + 16 * nt - 1) / (16 * nt), tiles = (M + 15) / 16;
+  SkinnyPlan best{1, -1};
+  for (int mt = 1; mt <= 4 && mt <= tiles; ++mt) {
+    const int64_t rounds = (blocks * ((tiles + mt - 1) / mt) + 255) / 256;
+    const double x_cost = ops * nt > 1 ? 1.2 : 1.0;
+    const double us = 2.4 + rounds * 0.43e-3 * K * (ops * nt * w_size + x_cost * mt * x_size);
+    if (best.us < 0 || us < best.us) best = {mt, us};
+  }
+  return best;
+}
+
 template <int MT, bool KEEPS, bool PAIR, typename TX, typename TW, class Step>
 inline void skinny_launch(const SkinnyProduct<TX, TW>& p, const Step& step, hipStream_t st) {
   constexpr int NT = KEEPS ? 2 : 1, kThreads = 64 * kSkinnyWaves;
-  const int blocks = (p.N + 16 * NT - 1) / (16 * NT);
+  const int blocks = (p.N + 16 * NT - 1) / (16 * NT), parts = (p.M + 16 * MT - 1) / (16 * MT);
   // One workgroup a CU may fill its registers with loads (K = 6144 in one or two
   // batches); where there are more, two share a CU.
   constexpr int kOne = MT > 2 || KEEPS ? 96 : 160;
-  if (blocks <= num_cus())
-    skinny_kernel<TX, TW, MT, NT, PAIR, kOne, Step><<<dim3(blocks), kThreads, 0, st>>>(p, step);
+  const dim3 grid(blocks, parts);
+  if (blocks * parts <= num_cus())
+    skinny_kernel<TX, TW, MT, NT, PAIR, kOne, Step><<<grid, kThreads, 0, st>>>(p, step);
   else
-    skinny_kernel<TX, TW, MT, NT, PAIR, 96, Step><<<dim3(blocks), kThreads, 0, st>>>(p, step);
+    skinny_kernel<TX, TW, MT, NT, PAIR, 96, Step><<<grid, kThreads, 0, st>>>(p, step);
 }
 
 template <bool KEEPS, bool PAIR, typename TX, typename TW, class Step>
 inline int launch_skinny(const SkinnyProduct<TX, TW>& p, const Step& step, hipStream_t st) {
-  if (p.M <= 16)
-    skinny_launch<1, KEEPS, PAIR>(p, step, st);
-  else if (p.M <= 32)
-    skinny_launch<2, KEEPS, PAIR>(p, step, st);
-  else if (p.M <= 48)
-    skinny_launch<3, KEEPS, PAIR>(p, step, st);
-  else
-    skinny_launch<4, KEEPS, PAIR>(p, step, st);
+  switch (plan_skinny(sizeof(TX), sizeof(TW), PAIR ? 2 : 1, KEEPS ? 2 : 1, p.M, p.N, p.K).mt) {
+    case 1: skinny_launch<1, KEEPS, PAIR>(p, step, st); break;
+    case 2: skinny_launch<2, KEEPS, PAIR>(p, step, st); break;
+    case 3: skinny_launch<3, KEEPS, PAIR>(p, step, st); break;
+    default: skinny_launch<4, KEEPS, PAIR>(p, step, st); break;
+  }
   ML_LAUNCH_CHECK();
   return ML_OK;
 }

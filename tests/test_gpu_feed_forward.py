@@ -391,6 +391,31 @@ def test_mlp_few_rows(dev, dtype, M, H, I, O):  # noqa: E741
     _check(torch.where(keep.to(dev), y, 0), torch.where(keep, want, 0.0), torch.where(keep, bound, 0.0), "y")
 
 
+# (rows shared out over workgroups by one tile of 16 and by two to four, the last
+# workgroup's not full; on both sides of where the tiles take over)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,K,N", [(40, 264, 2056), (72, 136, 5000), (100, 520, 264), (113, 264, 4104),
+                                   (128, 72, 8200), (128, 1000, 512), (129, 264, 264)])
+@pytest.mark.parametrize("checkpoint", [None, "fp8"])
+def test_linear_shared_rows(dev, dtype, M, K, N, checkpoint):
+    from metal_liger_amd.ops.fused_linear import fused_linear
+    case = _linear_case(M, K, N, dtype, True, True, dev, seed=7)
+    _linear_check(*case, "gelu_tanh", checkpoint,
+                  lambda: fused_linear(*case[:3], "gelu_tanh", case[3], checkpoint))
+    test_linear_few_rows(dev, dtype, M, K, N)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("M,H,I,O", [(33, 72, 2056, 264), (80, 264, 1032, 520), (97, 136, 4104, 72),
+                                     (128, 264, 520, 1000)])
+def test_mlp_shared_rows(dev, dtype, M, H, I, O):  # noqa: E741
+    from metal_liger_amd.ops.fused_swiglu_mlp import fused_swiglu_mlp
+    for checkpoint in (None, "fp8"):
+        case = _mlp_case(M, H, I, O, dtype, True, dev, seed=7)
+        _mlp_check(*case, checkpoint, lambda: fused_swiglu_mlp(case[0], *case[1], case[2], checkpoint))
+    test_mlp_few_rows(dev, dtype, M, H, I, O)
+
+
 @pytest.mark.parametrize("M", [5, 200])
 @pytest.mark.parametrize("N", [8, 40, 72, 136])
 def test_scales_of_short_blocks(dev, M, N):
