@@ -716,6 +716,17 @@ int ml_swiglu_mlp_bwd(const void* x, int64_t ldx, const void* wg, int64_t ldg, c
                       int dtype, void* stream);
 
 /*
+ * Up to 8 matrices copied into dense ones padded with zeros (to_wide), or out of them
+ * without the padding. Matrix j: sizes[2j] x sizes[2j + 1] elements at strides[2j],
+ * strides[2j + 1] of any[j]; wide[j] of wide_sizes[2j] x wide_sizes[2j + 1], no smaller,
+ * columns in multiples of 8, 16-byte aligned. All of one dtype; the arrays are read on the
+ * host, before the call returns. No reference interface (its kernels take any size).
+ */
+int ml_pad_matrices(int count, void* const* any, const int64_t* strides, const int64_t* sizes,
+                    void* const* wide, const int64_t* wide_sizes, int to_wide, int dtype,
+                    void* stream);
+
+/*
  * SwiGLU whose backward reads gate and up as 8 bits hold them (ops/fused_swiglu.py:
  * 26-50 keeps them whole): out = silu(gate) up of the inputs themselves, gate and up
  * [rows, cols] written to *_q and *_scale as ML_KEEP_FP8; all dense, any dtype and

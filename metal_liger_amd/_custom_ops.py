@@ -364,8 +364,8 @@ def _swiglu_kept_fake(gate, up):
 
 
 def _linear_fwd_fake(x2, w, bias, residual, act, keep):
-    N = w.shape[0]
-    return (x2.new_empty((x2.shape[0], N)), *_kept_fake(x2, N, keep))
+    M, K, N = *x2.shape, w.shape[0]
+    return (x2.new_empty((M, N)), *_kept_fake(x2, hip_ops.kept_cols(x2.dtype, M, N, K), keep))
 
 
 def _linear_bwd_fake(x2, w, dy, act, keep, z, zscale, N, K, need_dx, need_dw, need_db):
@@ -374,8 +374,9 @@ def _linear_bwd_fake(x2, w, dy, act, keep, z, zscale, N, K, need_dx, need_dw, ne
 
 
 def _swiglu_mlp_fwd_fake(x2, wg, wu, wd, residual, keep):
-    return (x2.new_empty((x2.shape[0], wd.shape[0])), *_kept_fake(x2, wd.shape[1], keep),
-            *_kept_fake(x2, wd.shape[1], keep))
+    (M, H), (O, I) = x2.shape, wd.shape  # noqa: E741
+    cols = hip_ops.kept_cols(x2.dtype, M, I, H, O)
+    return x2.new_empty((M, O)), *_kept_fake(x2, cols, keep), *_kept_fake(x2, cols, keep)
 
 
 def _swiglu_mlp_bwd_fake(x2, wg, wu, wd, dy, keep, gate, gate_scale, up, up_scale, *needs):

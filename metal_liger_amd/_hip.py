@@ -79,6 +79,9 @@ SIGNATURES: dict[str, tuple] = {
         [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _p, _p, _p, _p, _p, _p, _p, _p,
          _i64, _i64, _i64, _i64, _p, _sz, _i32, _p],
     ),
+    "ml_pad_matrices": (
+        _i32, [_i32, ctypes.POINTER(_p), _i64p, _i64p, ctypes.POINTER(_p), _i64p, _i32, _i32, _p],
+    ),
     "ml_dropout": (_i32, [_p, _p, _p, _i64, _i64, _f32, _p, _i64, _i32, _p]),
     "ml_embedding_fwd": (_i32, [_p, _i32, _i64, _p, _i64, _p, _i64, _i64, _f32, _i32, _p]),
     "ml_embedding_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64]),

@@ -15,6 +15,7 @@
 #include <initializer_list>
 
 #include "ffn_f32.h"
+#include "ffn_pad.h"
 #include "ffn_product.h"
 #include "ffn_skinny.h"
 #include "ffn_wgrad.h"
@@ -873,6 +874,39 @@ extern "C" int ml_swiglu_mlp_bwd(const void* x, int64_t ldx, const void* wg, int
       else
         return ffn::mlp_bwd<T, kind.value>(p, ws, true, (hipStream_t)stream);
     });
+  });
+}
+
+// ----------------------------------------------------------------- padding --
+
+extern "C" int ml_pad_matrices(int count, void* const* any, const int64_t* strides,
+                               const int64_t* sizes, void* const* wide, const int64_t* wide_sizes,
+                               int to_wide, int dtype, void* stream) {
+  ML_CHECK(count >= 1 && count <= ffn::kMaxPads, "pad: %d matrices, 1 to %d at a time", count,
+           ffn::kMaxPads);
+  ML_CHECK(any && strides && sizes && wide && wide_sizes, "pad: null pointer");
+  ffn::PadJobs jobs{};
+  jobs.count = count;
+  for (int j = 0; j < count; ++j) {
+    ffn::PadJob& p = jobs.job[j];
+    p.any = any[j];
+    p.wide = wide[j];
+    p.s0 = strides[2 * j];
+    p.s1 = strides[2 * j + 1];
+    p.rows = sizes[2 * j];
+    p.cols = sizes[2 * j + 1];
+    p.wrows = wide_sizes[2 * j];
+    p.wcols = wide_sizes[2 * j + 1];
+    ML_CHECK(p.rows >= 0 && p.cols >= 0 && p.wrows >= p.rows && p.wcols >= p.cols &&
+                 p.wcols % 8 == 0 && p.wrows < (1LL << 31) && p.wcols < (1LL << 31),
+             "pad: [%lld, %lld] in [%lld, %lld]", (long long)p.rows, (long long)p.cols,
+             (long long)p.wrows, (long long)p.wcols);
+    ML_CHECK((p.any || p.rows == 0 || p.cols == 0) && (p.wide || p.wrows == 0 || p.wcols == 0),
+             "pad: null pointer");
+    ML_CHECK(aligned16(p.wide), "pad: the padded matrix must be 16-byte aligned");
+  }
+  return dispatch_dtype(dtype, [&](auto t) {
+    return ffn::launch_pads(jobs, (int)sizeof(t), to_wide != 0, (hipStream_t)stream);
   });
 }
 

@@ -273,28 +273,131 @@ def _used(t: torch.Tensor | None):
     return None if t is None or t.numel() == 0 else t
 
 
+# Multiply-adds of a product from which fp32 sizes are padded: a training pass of [1024,
+# 1001] x 4001 (4e9) takes 297 us as it is and 313 padded, of [700, 3001] x 3001 (6e9) 614
+# and 477.
+PAD_F32 = 5 * 10**9
+
+
+def padded8(n: int) -> int:
+    return -(-n // 8) * 8
+
+
+def pads(dtype: torch.dtype, rows: int, *features: int) -> bool:
+    """Whether a feed-forward operator of these sizes pads its feature sizes to multiples of
+    8: the 16-bit kernels take no others, large fp32 products are faster so."""
+    if all(f % 8 == 0 for f in features):
+        return False
+    if dtype == torch.float32:
+        for f in features[:2]:
+            rows *= f
+        return rows >= PAD_F32
+    return True
+
+
+def kept_cols(dtype: torch.dtype, rows: int, cols: int, *features: int) -> int:
+    """The width at which an operator of these sizes keeps a tensor of cols columns."""
+    return padded8(cols) if pads(dtype, rows, cols, *features) else cols
+
+
+class _Wide:
+    """Operands of a call padded with zeros, and its results with room for the padding:
+    one allocation, one launch before the call and one after it."""
+
+    def __init__(self, like: torch.Tensor):
+        self.like, self.size, self.rooms, self.ins, self.outs = like, 0, [], [], []
+
+    def _room(self, rows: int, cols: int) -> int:
+        self.rooms.append((self.size, rows, cols))
+        self.size += (rows * cols * self.like.element_size() + 255) // 256 * 256
+        return len(self.rooms) - 1
+
+    def operand(self, t: torch.Tensor | None, rows: int, cols: int):
+        """t as the call reads it, for at(): itself where it has that size."""
+        if t is None:
+            return None
+        if t.shape[-1] == cols and (t.dim() == 1 or t.shape[0] == rows):
+            return _product_rows(t) if t.dim() == 2 else _al16(t.contiguous())
+        self.ins.append((t, self._room(rows, cols)))
+        return self.ins[-1][1]
+
+    def result(self, t: torch.Tensor, rows: int, cols: int):
+        """Where the call writes t (empty: not wanted)."""
+        if t.numel() == 0:
+            return None
+        if t.numel() == rows * cols:
+            return t
+        self.outs.append((t, self._room(rows, cols)))
+        return self.outs[-1][1]
+
+    def _copy(self, which, to_wide: int) -> None:
+        if which:
+            strides, sizes, wide, wide_sizes = [], [], [], []
+            for t, room in which:
+                first = () if t.dim() == 2 else (1,)  # (a vector: one row)
+                strides += (*first, *t.stride())
+                sizes += (*first, *t.shape)
+                at, rows, cols = self.rooms[room]
+                wide.append(self.base + at)
+                wide_sizes += (rows, cols)
+            call("ml_pad_matrices", len(which), _hip.ptrs([ptr(t) for t, _ in which]), geom(strides),
+                 geom(sizes), _hip.ptrs(wide), geom(wide_sizes), to_wide,
+                 dtype_tag(self.like, "operand"), stream_of(self.like))
+
+    def begin(self) -> None:
+        self.buffer = torch.empty(self.size, dtype=torch.uint8, device=self.like.device)
+        self.base = self.buffer.data_ptr()
+        self._copy(self.ins, 1)
+
+    def end(self) -> None:
+        self._copy(self.outs, 0)
+
+    def at(self, what):
+        """(pointer, row stride) of an operand or a result."""
+        if what is None:
+            return None, 0
+        if isinstance(what, int):
+            at, _, cols = self.rooms[what]
+            return self.base + at, cols
+        return what.data_ptr(), row_stride(what) if what.dim() == 2 else 0
+
+
 def _linear(x2, w, bias, residual, act: int, keep: int, z, zscale):
     ensure_rocm_device(x2, w, bias, residual)
-    x2, w = _product_rows(x2), _product_rows(w)
     (M, K), N = x2.shape, w.shape[0]
     y = torch.empty(M, N, dtype=x2.dtype, device=x2.device)
     if M == 0:
         return y
+    kept = (keep, ptr(_used(z)), ptr(_used(zscale)))
+    tag = dtype_tag(x2, "x")
+    if pads(x2.dtype, M, N, K):
+        wide, Np, Kp = _Wide(x2), padded8(N), padded8(K)
+        ins = (wide.operand(x2, M, Kp), wide.operand(w, Np, Kp), wide.operand(bias, 1, Np),
+               wide.operand(residual, M, Np))
+        out = wide.result(y, M, Np)
+        wide.begin()
+        (px, ldx), (pw, ldw), (pb, _), (pr, ldr), (py, ldy) = map(wide.at, (*ins, out))
+        ws, wsb = _workspace(x2, "ml_linear_fwd_workspace_bytes", M, Np, Kp, tag)
+        call("ml_linear_fwd", px, ldx, pw, ldw, pb, pr, ldr, act, py, ldy, *kept, M, Np, Kp, ptr(ws),
+             wsb, tag, stream_of(x2))
+        wide.end()
+        return y
+    x2, w = _product_rows(x2), _product_rows(w)
     bias = None if bias is None else _al16(bias.contiguous())
     residual = None if residual is None else _product_rows(residual)
-    tag = dtype_tag(x2, "x")
     ws, wsb = _workspace(x2, "ml_linear_fwd_workspace_bytes", M, N, K, tag)
     call("ml_linear_fwd", ptr(x2), row_stride(x2), ptr(w), row_stride(w), ptr(bias), ptr(residual),
-         0 if residual is None else row_stride(residual), act, ptr(y), N, keep, ptr(_used(z)),
-         ptr(_used(zscale)), M, N, K, ptr(ws), wsb, tag, stream_of(x2))
+         0 if residual is None else row_stride(residual), act, ptr(y), N, *kept, M, N, K, ptr(ws), wsb,
+         tag, stream_of(x2))
     return y
 
 
 @_on_device
 def linear_fwd(x2, w, bias, residual, act: int, keep: int):
     """(y, z, zscale) of ml_linear_fwd: x2 [M, K], w [N, K], bias [N] or None, residual
-    [M, N] or None, all fp32, or all bf16 or fp16 (sizes in multiples of 8)."""
-    kept = _kept_buffers(x2, w.shape[0], keep)
+    [M, N] or None, all of one dtype; z of kept_cols columns."""
+    M, K, N = *x2.shape, w.shape[0]
+    kept = _kept_buffers(x2, kept_cols(x2.dtype, M, N, K), keep)
     return (_linear(x2, w, bias, residual, act, keep, *kept), *kept)
 
 
@@ -312,42 +415,70 @@ def linear_bwd(x2, w, dy, act: int, keep: int, z, zscale, N: int, K: int, need_d
     ensure_rocm_device(x2, w, dy, z, zscale)
     M = dy.shape[0]
     new = lambda need, *s: torch.empty(s if need else (0,), dtype=dy.dtype, device=dy.device)  # noqa: E731
-    dx, dw, db = new(need_dx, M, K), new(need_dw, N, K), new(need_db, N)
+    outs = dx, dw, db = new(need_dx, M, K), new(need_dw, N, K), new(need_db, N)
     if M == 0:
         return dx, dw.zero_(), db.zero_()
-    dy = _product_rows(dy)
-    x2 = _product_rows(x2) if need_dw else None
-    w = _product_rows(w) if need_dx else None
+    kept = (act, keep, ptr(_used(z)), ptr(_used(zscale)))
     tag = dtype_tag(dy, "grad")
+    x2, w = x2 if need_dw else None, w if need_dx else None
+    if pads(dy.dtype, M, N, K):
+        wide, Np, Kp = _Wide(dy), padded8(N), padded8(K)
+        ins = wide.operand(x2, M, Kp), wide.operand(w, Np, Kp), wide.operand(dy, M, Np)
+        to = wide.result(dx, M, Kp), wide.result(dw, Np, Kp), wide.result(db, 1, Np)
+        wide.begin()
+        ws, wsb = _workspace(dy, "ml_linear_bwd_workspace_bytes", M, Np, Kp, act, tag)
+        call("ml_linear_bwd", *wide.at(ins[0]), *wide.at(ins[1]), *wide.at(ins[2]), *kept,
+             *(wide.at(t)[0] for t in to), M, Np, Kp, ptr(ws), wsb, tag, stream_of(dy))
+        wide.end()
+        return outs
+    x2, w = (None if t is None else _product_rows(t) for t in (x2, w))
+    dy = _product_rows(dy)
     ws, wsb = _workspace(dy, "ml_linear_bwd_workspace_bytes", M, N, K, act, tag)
-    call("ml_linear_bwd", ptr(x2), 0 if x2 is None else row_stride(x2), ptr(w),
-         0 if w is None else row_stride(w), ptr(dy), row_stride(dy), act, keep, ptr(_used(z)),
-         ptr(_used(zscale)), ptr(_used(dx)), ptr(_used(dw)), ptr(_used(db)), M, N, K, ptr(ws), wsb,
-         tag, stream_of(dy))
-    return dx, dw, db
+    call("ml_linear_bwd", *_pairs(x2, w, dy), *kept, *(ptr(_used(t)) for t in outs), M, N, K, ptr(ws),
+         wsb, tag, stream_of(dy))
+    return outs
+
+
+def _pairs(*ts):
+    """pointer, row stride of each; None and 0 of None"""
+    return [v for t in ts for v in (ptr(t), 0 if t is None else row_stride(t))]
 
 
 def _swiglu_mlp(x2, wg, wu, wd, residual, keep: int, kept):
     ensure_rocm_device(x2, wg, wu, wd, residual)
-    x2, wg, wu, wd = map(_product_rows, (x2, wg, wu, wd))
     (M, H), (O, I) = x2.shape, wd.shape  # noqa: E741
     y = torch.empty(M, O, dtype=x2.dtype, device=x2.device)
     if M == 0:
         return y
-    residual = None if residual is None else _product_rows(residual)
+    kept = (keep, *(ptr(_used(t)) for t in kept))
     tag = dtype_tag(x2, "x")
+    if pads(x2.dtype, M, I, H, O):
+        wide, Hp, Ip, Op = _Wide(x2), padded8(H), padded8(I), padded8(O)
+        ins = (wide.operand(x2, M, Hp), wide.operand(wg, Ip, Hp), wide.operand(wu, Ip, Hp),
+               wide.operand(wd, Op, Ip), wide.operand(residual, M, Op))
+        out = wide.result(y, M, Op)
+        wide.begin()
+        ws, wsb = _workspace(x2, "ml_swiglu_mlp_fwd_workspace_bytes", M, Hp, Ip, Op, tag)
+        call("ml_swiglu_mlp_fwd", *(v for t in ins for v in wide.at(t)), wide.at(out)[0], *kept, M, Hp,
+             Ip, Op, ptr(ws), wsb, tag, stream_of(x2))
+        wide.end()
+        return y
+    x2, wg, wu, wd = map(_product_rows, (x2, wg, wu, wd))
+    residual = None if residual is None else _product_rows(residual)
     ws, wsb = _workspace(x2, "ml_swiglu_mlp_fwd_workspace_bytes", M, H, I, O, tag)
-    call("ml_swiglu_mlp_fwd", *_pairs(x2, wg, wu, wd), ptr(residual),
-         0 if residual is None else row_stride(residual), ptr(y), keep,
-         *(ptr(_used(t)) for t in kept), M, H, I, O, ptr(ws), wsb, tag, stream_of(x2))
+    call("ml_swiglu_mlp_fwd", *_pairs(x2, wg, wu, wd, residual), ptr(y), *kept, M, H, I, O, ptr(ws),
+         wsb, tag, stream_of(x2))
     return y
 
 
 @_on_device
 def swiglu_mlp_fwd(x2, wg, wu, wd, residual, keep: int):
     """(y, gate, gate_scale, up, up_scale) of ml_swiglu_mlp_fwd: x2 [M, H], wg and wu
-    [I, H], wd [O, I], residual [M, O] or None; dtypes as linear_fwd."""
-    kept = _kept_buffers(x2, wd.shape[1], keep) + _kept_buffers(x2, wd.shape[1], keep)
+    [I, H], wd [O, I], residual [M, O] or None, all of one dtype; gate and up of kept_cols
+    columns."""
+    (M, H), (O, I) = x2.shape, wd.shape  # noqa: E741
+    cols = kept_cols(x2.dtype, M, I, H, O)
+    kept = _kept_buffers(x2, cols, keep) + _kept_buffers(x2, cols, keep)
     return (_swiglu_mlp(x2, wg, wu, wd, residual, keep, kept), *kept)
 
 
@@ -355,11 +486,6 @@ def swiglu_mlp_fwd(x2, wg, wu, wd, residual, keep: int):
 def swiglu_mlp_infer(x2, wg, wu, wd, residual):
     """swiglu_mlp_fwd's y with nothing kept."""
     return _swiglu_mlp(x2, wg, wu, wd, residual, KEEP_NONE, (None,) * 4)
-
-
-def _pairs(*ts):
-    """pointer, row stride of each; None and 0 of None"""
-    return [v for t in ts for v in (ptr(t), 0 if t is None else row_stride(t))]
 
 
 def mlp_hidden(x2, wg, default: int) -> int:
@@ -376,18 +502,32 @@ def swiglu_mlp_bwd(x2, wg, wu, wd, dy, keep: int, gate, gate_scale, up, up_scale
     M, (O, I) = dy.shape[0], wd.shape  # noqa: E741
     H = mlp_hidden(x2, wg, I)
     new = lambda need, *s: torch.empty(s if need else (0,), dtype=dy.dtype, device=dy.device)  # noqa: E731
-    outs = [new(need_dx, M, H), new(need_dwg, I, H), new(need_dwu, I, H), new(need_dwd, O, I)]
+    outs = (new(need_dx, M, H), new(need_dwg, I, H), new(need_dwu, I, H), new(need_dwd, O, I))
     if M == 0:
         return tuple(t.zero_() for t in outs)
-    x2 = _product_rows(x2) if need_dwg or need_dwu else None
-    wg, wu = (_product_rows(wg), _product_rows(wu)) if need_dx else (None, None)
-    wd, dy = _product_rows(wd), _product_rows(dy)
+    kept = (keep, *(ptr(_used(t)) for t in (gate, gate_scale, up, up_scale)))
     tag = dtype_tag(dy, "grad")
+    x2 = x2 if need_dwg or need_dwu else None
+    wg, wu = (wg, wu) if need_dx else (None, None)
+    # (an odd I: as the forward did; else the choice is free, and H may not be known)
+    if gate.shape[1] != I if I % 8 else pads(dy.dtype, M, I, H, O):
+        wide, Hp, Ip, Op = _Wide(dy), padded8(H), padded8(I), padded8(O)
+        ins = (wide.operand(x2, M, Hp), wide.operand(wg, Ip, Hp), wide.operand(wu, Ip, Hp),
+               wide.operand(wd, Op, Ip), wide.operand(dy, M, Op))
+        to = (wide.result(outs[0], M, Hp), wide.result(outs[1], Ip, Hp), wide.result(outs[2], Ip, Hp),
+              wide.result(outs[3], Op, Ip))
+        wide.begin()
+        ws, wsb = _workspace(dy, "ml_swiglu_mlp_bwd_workspace_bytes", M, Hp, Ip, Op, tag)
+        call("ml_swiglu_mlp_bwd", *(v for t in ins for v in wide.at(t)), *kept,
+             *(wide.at(t)[0] for t in to), M, Hp, Ip, Op, ptr(ws), wsb, tag, stream_of(dy))
+        wide.end()
+        return outs
+    x2, wg, wu = (None if t is None else _product_rows(t) for t in (x2, wg, wu))
+    wd, dy = _product_rows(wd), _product_rows(dy)
     ws, wsb = _workspace(dy, "ml_swiglu_mlp_bwd_workspace_bytes", M, H, I, O, tag)
-    call("ml_swiglu_mlp_bwd", *_pairs(x2, wg, wu, wd, dy), keep,
-         *(ptr(_used(t)) for t in (gate, gate_scale, up, up_scale)), *(ptr(_used(t)) for t in outs),
-         M, H, I, O, ptr(ws), wsb, tag, stream_of(dy))
-    return tuple(outs)
+    call("ml_swiglu_mlp_bwd", *_pairs(x2, wg, wu, wd, dy), *kept, *(ptr(_used(t)) for t in outs), M, H,
+         I, O, ptr(ws), wsb, tag, stream_of(dy))
+    return outs
 
 
 # ----------------------------------------------------------------- dropout --

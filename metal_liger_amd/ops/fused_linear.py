@@ -44,48 +44,9 @@ def keep_mode(checkpoint: str | None, dtype: torch.dtype) -> int:
     return hip_ops.KEEP_F32 if dtype == torch.float32 else hip_ops.KEEP_FP16
 
 
-# Multiply-adds of a product from which fp32 sizes are padded: a training pass of [1024,
-# 1001] x 4001 (4e9) takes 297 us as it is and 313 padded, of [700, 3001] x 3001 (6e9) 614
-# and 477.
-_PAD_F32 = 5 * 10**9
-
-
-def pads(dtype: torch.dtype, rows: int, *features: int) -> bool:
-    """Whether an operator of these sizes pads its feature sizes to multiples of 8."""
-    if dtype != torch.float32:
-        return True
-    for f in features:
-        rows *= f
-    return rows >= _PAD_F32
-
-
-def padded(n: int) -> int:
-    return -(-n // 8) * 8
-
-
-def pad(t, *dims: int):
-    """t with these dimensions' sizes padded by zeros."""
-    if t is None or all(t.shape[d] % 8 == 0 for d in dims):
-        return t
-    shape = list(t.shape)
-    for d in dims:
-        shape[d] = padded(shape[d])
-    out = t.new_zeros(shape)
-    out[tuple(slice(n) for n in t.shape)].copy_(t)
-    return out
-
-
-def cut(t: torch.Tensor, *sizes: int) -> torch.Tensor:
-    """A result at its sizes without the padding, dense."""
-    return t if tuple(t.shape) == sizes else t[tuple(slice(n) for n in sizes)].contiguous()
-
-
-def rows(t, padding: bool = False):
-    """[..., C] -> [R, C], C padded if wanted."""
-    if t is None:
-        return None
-    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    return pad(t, 1) if padding else t
+def rows(t):
+    """[..., C] -> [R, C]."""
+    return t if t is None or t.dim() == 2 else t.reshape(-1, t.shape[-1])
 
 
 def check_input(what: str, x: torch.Tensor, *weights: torch.Tensor) -> None:
@@ -114,15 +75,10 @@ def wants_grad(*tensors) -> bool:
 
 def _forward(x, weight, bias, residual, act: int, keep: int):
     """(y, z, zscale), or y alone where nothing is kept."""
-    N, K = weight.shape
-    p = pads(x.dtype, x.numel() // K, N, K)
-    w, b = (pad(weight, 0, 1), pad(bias, 0)) if p else (weight, bias)
-    args = (rows(x, p), w, b, rows(residual, p), act)
+    args = (rows(x), weight, bias, rows(residual), act)
     y, *kept = (cops.linear_infer(*args),) if keep == hip_ops.KEEP_NONE else \
         cops.linear_fwd(*args, keep)
-    if p:
-        y = cut(y, y.shape[0], N)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], N), *kept
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.shape[0]), *kept
 
 
 class _FusedLinearFunction(torch.autograd.Function):
@@ -144,15 +100,9 @@ class _FusedLinearFunction(torch.autograd.Function):
         if need_dx or need_dw or need_db:
             x, weight, *kept = ctx.saved_tensors
             z, zscale = kept or (None, None)
-            N, K = ctx.sizes
-            M = ctx.x_shape.numel() // K
-            p = pads(dy.dtype, M, N, K)
-            size = padded if p else int
-            out = cops.linear_bwd(rows(x, p), pad(weight, 0, 1) if p else weight, rows(dy, p),
-                                  ctx.act, ctx.keep, z, zscale, size(N), size(K), need_dx, need_dw,
-                                  need_db)
-            grads = [cut(g, *sizes) if need else None
-                     for g, sizes, need in zip(out, ((M, K), (N, K), (N,)), ctx.needs_input_grad)]
+            out = cops.linear_bwd(rows(x), weight, rows(dy), ctx.act, ctx.keep, z, zscale, *ctx.sizes,
+                                  need_dx, need_dw, need_db)
+            grads = [g if need else None for g, need in zip(out, ctx.needs_input_grad)]
             if need_dx and len(ctx.x_shape) != 2:
                 grads[0] = grads[0].view(ctx.x_shape)
         return (*grads, dy if need_dr else None, None, None)

@@ -21,9 +21,9 @@ import torch.nn as nn
 from metal_liger_amd import _custom_ops as cops
 from metal_liger_amd import hip_ops
 from metal_liger_amd._model_walk import find_layers
-from metal_liger_amd.ops.fused_linear import (check_checkpoint, check_input, check_residual, cut,
-                                              hooked, keep_mode, pad, pads, plain_linear, rows,
-                                              runs_fused, wants_grad)
+from metal_liger_amd.ops.fused_linear import (check_checkpoint, check_input, check_residual,
+                                              hooked, keep_mode, plain_linear, rows, runs_fused,
+                                              wants_grad)
 from metal_liger_amd.ops.fused_swiglu import MetalLigerSwiGLU
 
 logger = logging.getLogger(__name__)
@@ -31,16 +31,10 @@ logger = logging.getLogger(__name__)
 
 def _forward(x, weights, residual, keep: int):
     """(y, gate, its scales, up, its scales), or y alone where nothing is kept."""
-    O, I = weights[2].shape  # noqa: E741
-    p = pads(x.dtype, x.numel() // x.shape[-1], x.shape[-1], I)
-    if p:
-        weights = [pad(w, 0, 1) for w in weights]
-    args = (rows(x, p), *weights, rows(residual, p))
+    args = (rows(x), *weights, rows(residual))
     y, *kept = (cops.swiglu_mlp_infer(*args),) if keep == hip_ops.KEEP_NONE else \
         cops.swiglu_mlp_fwd(*args, keep)
-    if p:
-        y = cut(y, y.shape[0], O)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], O), *kept
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], weights[2].shape[0]), *kept
 
 
 class _FusedSwiGLUMLPFunction(torch.autograd.Function):
@@ -60,14 +54,9 @@ class _FusedSwiGLUMLPFunction(torch.autograd.Function):
         grads = [None] * 4
         if any(ctx.needs_input_grad[:4]):
             x, wg, wu, wd, *kept = ctx.saved_tensors
-            H, (O, I) = ctx.x_shape[-1], wd.shape  # noqa: E741
-            M = ctx.x_shape.numel() // H
-            p = pads(dy.dtype, M, H, I)
-            weights = [pad(w, 0, 1) for w in (wg, wu, wd)] if p else (wg, wu, wd)
-            outs = cops.swiglu_mlp_bwd(rows(x, p), *weights, rows(dy, p), ctx.keep, *kept,
+            outs = cops.swiglu_mlp_bwd(rows(x), wg, wu, wd, rows(dy), ctx.keep, *kept,
                                        *ctx.needs_input_grad[:4])
-            grads = [cut(g, *sizes) if need else None for g, sizes, need in
-                     zip(outs, ((M, H), (I, H), (I, H), (O, I)), ctx.needs_input_grad)]
+            grads = [g if need else None for g, need in zip(outs, ctx.needs_input_grad)]
             if grads[0] is not None and len(ctx.x_shape) != 2:
                 grads[0] = grads[0].view(ctx.x_shape)
         return (*grads, dy if ctx.needs_input_grad[4] else None, None)

@@ -184,6 +184,22 @@ def test_host_side_argument_errors():
     refused(mlp_bwd(dx=q + 2), b"dx")
     refused(mlp_bwd(wsb=16), b"workspace")
 
+    def pads(n=1, any_=p, strides=(16, 1), sizes=(3, 5), wide=q, wide_sizes=(8, 8), dtype=1):
+        return L.ml_pad_matrices(n, _hip.ptrs([any_]), _hip.geom(strides), _hip.geom(sizes),
+                                 _hip.ptrs([wide]), _hip.geom(wide_sizes), 1, dtype, None)
+
+    refused(pads(n=0), b"0 matrices")
+    refused(pads(n=9), b"9 matrices")
+    refused(pads(sizes=(3, 9)), b"[3, 9] in [8, 8]")
+    refused(pads(sizes=(9, 5)), b"[9, 5] in [8, 8]")
+    refused(pads(sizes=(-1, 5)), b"[-1, 5]")
+    refused(pads(wide_sizes=(8, 12)), b"[8, 12]")
+    refused(pads(any_=None), b"null pointer")
+    refused(pads(wide=q + 8), b"16-byte aligned")
+    refused(pads(dtype=5), b"dtype tag 5")
+    assert L.ml_pad_matrices(1, _hip.ptrs([None]), _hip.geom((8, 1)), _hip.geom((0, 5)),
+                             _hip.ptrs([None]), _hip.geom((0, 8)), 1, 1, None) == 0
+
     refused(L.ml_swiglu_kept_fwd(p, p, q, p, p, p, p, -1, 8, 1, None), b"negative")
     refused(L.ml_swiglu_kept_fwd(p, p, q, p, None, p, p, 1, 8, 1, None), b"scales")
     refused(L.ml_swiglu_kept_fwd(p, p, q, p + 1, p, p, p, 1, 8, 1, None), b"16-byte aligned")
@@ -240,6 +256,12 @@ def test_fake_kernels():
         assert look([ops.swiglu_mlp_infer(x, *ws, None)]) == [((10, 40), BF)]
         out = ops.swiglu_mlp_bwd(x, *ws, e(10, 40), 3, *y[1:], True, False, True, True)
         assert look(out) == [((10, 64), BF), ((0,), BF), ((96, 64), BF), ((40, 96), BF)]
+        y = ops.linear_fwd(e(10, 33), e(45, 33), None, None, 1, 3)  # (kept at the padded width)
+        assert look(y) == [((10, 45), BF), ((10, 48), U8), ((10, 2), U8)]
+        out = ops.linear_bwd(e(10, 33), e(45, 33), e(10, 45), 1, 3, *y[1:], 45, 33, True, True, True)
+        assert look(out) == [((10, 33), BF), ((45, 33), BF), ((45,), BF)]
+        y = ops.linear_fwd(e(10, 33, dtype=F32), e(45, 33, dtype=F32), None, None, 1, 1)
+        assert look(y) == [((10, 45), F32), ((10, 45), F32), ((0,), U8)]
         y = ops.swiglu_kept_fwd(e(2, 5, 70), e(2, 5, 70))
         assert look(y) == [((2, 5, 70), BF)] + 2 * [((2, 5, 70), U8), ((2, 5, 3), U8)]
         out = ops.swiglu_kept_bwd(*y[1:], e(2, 5, 70), BF, F32)

@@ -470,3 +470,42 @@ def test_wide_strides(dev):
     x = big[:, 8:72]
     x.copy_(seeded((150, 64), 2))
     assert torch.equal(fused_linear(x, w.float()), fused_linear(x.contiguous(), w.float()))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("shapes", [[(1, 1)], [(13,), (7, 9), (0, 5), (8, 16), (1,)],
+                                    [(3000, 1001), (517, 8), (1, 70001), (70001, 1), (4, 7), (9,), (2, 2), (65, 31)]])
+def test_padding(dev, dtype, shapes):
+    """Copies of any sizes and strides, in one launch: the same bits, zeros beside them."""
+    from metal_liger_amd import hip_ops
+    ts = []
+    for i, s in enumerate(shapes):
+        t = seeded(s, i, dtype).to(dev)
+        if i % 3 == 1 and t.dim() == 2:
+            t = t.t().contiguous().t()                            # columns apart
+        elif i % 3 == 2:
+            t = torch.cat([t, t, t], -1)[..., s[-1]:2 * s[-1]]    # a slice of longer rows
+        elif t.dim() == 2 and i:
+            t = t[:1].expand(s)                                   # one row for all
+        ts.append(t)
+    wide = hip_ops._Wide(ts[0])
+    sizes = [(1 if t.dim() == 1 else t.shape[0] + 5 * (i % 2), hip_ops.padded8(t.shape[-1]))
+             for i, t in enumerate(ts)]
+    ins = [wide.operand(t, *s) for t, s in zip(ts, sizes)]
+    wide.begin()
+    for t, s, i in zip(ts, sizes, ins):
+        want = torch.zeros(s, dtype=dtype, device=dev)
+        want[:t.shape[0] if t.dim() == 2 else 1, :t.shape[-1]] = t
+        if not isinstance(i, int):
+            assert torch.equal(i.view(s), want)
+            continue
+        at = wide.rooms[i][0]
+        n = s[0] * s[1] * t.element_size()
+        assert wide.at(i) == (wide.base + at, s[1])
+        assert torch.equal(wide.buffer[at:at + n].view(dtype).view(s), want)
+    # back: each room into a result of the matrix's size
+    outs = [torch.full(t.shape, 7.0, dtype=dtype, device=dev) for t in ts]
+    wide.outs = [(o, i) for o, i in zip(outs, ins) if isinstance(i, int)]
+    wide.end()
+    for t, o, i in zip(ts, outs, ins):
+        assert torch.equal(o, t) or not isinstance(i, int)

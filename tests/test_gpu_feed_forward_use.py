@@ -448,6 +448,12 @@ def test_opcheck(dev):
     check(ops.swiglu_mlp_fwd, (x, *ws, None, hip_ops.KEEP_FP16))
     kept = ops.swiglu_mlp_fwd(x, *ws, r, hip_ops.KEEP_FP8)[1:]
     check(ops.swiglu_mlp_bwd, (x, *ws, r, hip_ops.KEEP_FP8, *kept, True, True, False, True))
+    odd = (x[:, :61], w[:70, :61], b[:70], None, 2, hip_ops.KEEP_FP8)
+    check(ops.linear_fwd, odd)
+    z = ops.linear_fwd(*odd)[1:]
+    check(ops.linear_bwd, (*odd[:2], r[:, :70], 2, hip_ops.KEEP_FP8, *z, 70, 61, True, True, True))
+    check(ops.swiglu_mlp_bwd, (None, *ws, r, hip_ops.KEEP_FP8, *kept, True, False, False, True))
+    check(ops.swiglu_mlp_bwd, (None, None, None, ws[2], r, hip_ops.KEEP_FP8, *kept, False, False, False, True))
     out = ops.swiglu_kept_fwd(x, x)
     check(ops.swiglu_kept_fwd, (x, x))
     check(ops.swiglu_kept_bwd, (*out[1:], x, BF, BF))
