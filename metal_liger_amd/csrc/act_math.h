@@ -8,8 +8,8 @@
 // degree 8 fitted to it by reweighted least squares in t (largest relative error
 // 1.5e-8 up to a = 14.8, past which the product underflows). One exponential, which the
 // derivative's density shares, one reciprocal and ten multiplications; with the math
-// library's erfc, whose branches a wave takes both of, the epilogue of [8192, 1152] x
-// 4304 took 62 us more.
+// library's erfc, whose branches a wave takes both of, the product of [8192, 1152] x 4304
+// with this epilogue takes 150 us instead of 123 (110 without an activation).
 #pragma once
 
 #include "swiglu_math.h"

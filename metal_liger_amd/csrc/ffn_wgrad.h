@@ -9,8 +9,8 @@
 // their fp32 partials lie in the workspace as the accumulators lie in the lanes (16
 // bytes a lane, whatever the tile's edges) and a second kernel sums them in split
 // order, one workgroup a tile. Bound by the matrix cores; [8192, 4304]^T [8192, 1152]:
-// 188 us as 85 tiles, 87 us split three ways; the gated block's three at 8192 tokens
-// 660 us one by one, 545 together.
+// 188 us as 85 tiles, 90 split three ways and 17 to join; the gated block's three at 8192
+// tokens 660 us one by one, 546 and 16 together.
 #pragma once
 
 #include "gemm_core.h"

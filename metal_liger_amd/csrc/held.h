@@ -12,7 +12,7 @@
 // The 16 bits are fp16 with a scale rather than bf16 because a backward multiplies what
 // it reads: gate and up in bf16 (2^-8) took the weights' gradients of the gated block
 // from 2.4e-3 to 3.5e-3 of their norm off 64 bits, 1.7e-3 being the rounding of the
-// result alone; 33 bytes more for 1024 elements.
+// result alone; the scales are 32 bytes for 1024 elements.
 #pragma once
 
 #include "common.h"
