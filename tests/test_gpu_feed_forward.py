@@ -509,3 +509,30 @@ def test_padding(dev, dtype, shapes):
     wide.end()
     for t, o, i in zip(ts, outs, ins):
         assert torch.equal(o, t) or not isinstance(i, int)
+
+
+@pytest.mark.parametrize("checkpoint", [None, "fp8"])
+@pytest.mark.parametrize("M,K,N", [(5, 13, 7), (70, 33, 65), (300, 201, 521), (129, 264, 131), (129, 131, 264)])
+def test_fp32_padded(dev, monkeypatch, checkpoint, M, K, N):
+    """fp32 sizes padded as large ones are."""
+    from metal_liger_amd import hip_ops
+    from metal_liger_amd.ops.fused_linear import fused_linear
+    from metal_liger_amd.ops.fused_swiglu_mlp import fused_swiglu_mlp
+    monkeypatch.setattr(hip_ops, "PAD_F32", 1)
+    case = _linear_case(M, K, N, torch.float32, True, True, dev, seed=3)
+    _linear_check(*case, "silu", checkpoint,
+                  lambda: fused_linear(*case[:3], "silu", case[3], checkpoint))
+    x, ws, r, dy = _mlp_case(M, K, N, K + 3, torch.float32, True, dev, seed=3)
+    _mlp_check(x, ws, r, dy, checkpoint, lambda: fused_swiglu_mlp(x, *ws, r, checkpoint))
+    for frozen in range(15):  # (the padding of what is left)
+        for i, t in enumerate((x, *ws)):
+            t.requires_grad_(not frozen >> i & 1)
+        leaves = [t for t in (x, *ws) if t.requires_grad]
+        got = torch.autograd.grad(fused_swiglu_mlp(x, *ws, r, checkpoint), leaves, dy)
+        for g, t in zip(got, leaves):
+            assert g.shape == t.shape and bool(g.isfinite().all())
+        if frozen == 0:
+            full = dict(zip(map(id, leaves), got))
+        # (fewer gradients may split K otherwise)
+        for g, t in zip(got, leaves):
+            assert torch.allclose(g, full[id(t)], rtol=0, atol=N * M * V * float(full[id(t)].abs().max()))

@@ -362,6 +362,56 @@ def test_captured_step(dev, tokens, held):
         torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, BF, torch.float16])
+def test_captured_padded_step(dev, dtype):
+    """Sizes that are no multiples of 8: the padding belongs to the graph."""
+    x, w, b = (_leaf(s, i, dev, dtype) for i, s in enumerate(((70, 61), (75, 61), (75,))))
+    ws = [_leaf(s, 5, dev, dtype, 0.1) for s in ((45, 75), (45, 75), (61, 45))]
+    dy, leaves = seeded((70, 61), 6, dtype).to(dev), [x, w, b, *ws]
+
+    def step():
+        y = _mlp(_linear(x, w, b, "gelu", checkpoint="fp8"), *ws, residual=x)
+        return [y, *_grads(y, leaves, dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = step()
+    for i in range(3):
+        with torch.no_grad():
+            x.copy_(seeded((70, 61), 20 + i, dtype))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.detach().clone() for t in outs]
+        assert all(torch.equal(a, b) for a, b in zip(got, step())), i
+        torch.cuda.synchronize()
+
+
+def test_two_threads(dev):
+    """Calls of two threads at once, each on a stream of its own: a call's bits alone."""
+    from concurrent.futures import ThreadPoolExecutor
+    sizes = [(300, 264, 136), (33, 61, 75)]
+    cases = [[seeded(s, i, BF).to(dev) for i, s in enumerate(((M, K), (N, K), (N,), (M, N)))]
+             for M, K, N in sizes]
+    want = [_linear(c[0], c[1], c[2], "gelu", c[3]) for c in cases]
+    torch.cuda.synchronize()
+
+    def run(j):
+        stream, same = torch.cuda.Stream(), True
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                c = cases[j]
+                same &= torch.equal(_linear(c[0], c[1], c[2], "gelu", c[3]), want[j])
+        return same
+
+    with ThreadPoolExecutor(2) as pool:
+        assert all(pool.map(run, (0, 1)))
+
+
 def test_two_captured_graphs(dev):
     """Two graphs of the same shapes, replayed in turn and on two streams at once: each
     has workspaces of its own."""
