@@ -11,7 +11,8 @@ weight is frozen, W where x needs no gradient) is not kept. First derivatives on
 
 bf16 runs on the bf16 matrix cores; fp32 and fp16 on the fp32 ones, with everything
 between input and output in fp32. The kernels take 16-bit sizes in multiples of 8, and
-fp32 ones faster: others are padded with zeros, which add nothing.
+fp32 ones faster: others are padded with zeros, which add nothing (but a row of x that
+holds infinities then has NaN for its gradient, where the formula may have numbers).
 """
 
 from __future__ import annotations
