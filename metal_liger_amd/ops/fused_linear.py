@@ -7,7 +7,8 @@ rounded once. The backward needs z = x W^T + bias where there is an activation: 
 kept in 16 bits (fp16 with a power of two as scale for every 32 columns of a row, which
 rounds finer than bf16; fp32 in fp32), or in 8 (checkpoint="fp8": e4m3 with such
 scales), formed of the fp32 sums. What is not needed (x where the
-weight is frozen, W where x needs no gradient) is not kept. First derivatives only.
+weight is frozen, W where x needs no gradient) is not kept. First derivatives only, in
+reverse mode (forward mode is refused).
 
 bf16 runs on the bf16 matrix cores; fp32 and fp16 on the fp32 ones, with everything
 between input and output in fp32. The kernels take 16-bit sizes in multiples of 8, and
@@ -23,6 +24,7 @@ import logging
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from metal_liger_amd import _custom_ops as cops
 from metal_liger_amd import hip_ops
@@ -70,8 +72,17 @@ def check_residual(what: str, residual, x: torch.Tensor, out: int) -> None:
                          f"{shape} {x.dtype}")
 
 
+def forward_mode() -> bool:
+    """Whether forward-mode differentiation is at work (told by a private name; where
+    torch has none, it is taken to be)."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
+
+
 def wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    """Whether a call goes through its autograd Function: for a backward, or to have
+    forward mode refused there (the ops alone would drop the tangents)."""
+    return forward_mode() or torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in tensors)
 
 
 def _forward(x, weight, bias, residual, act: int, keep: int):
@@ -181,9 +192,11 @@ def plain_linear(module) -> bool:
 
 def runs_fused(x, *linears) -> bool:
     """Whether a routed module's forward may run the fused op for x: its linear layers
-    are plain ones of x's dtype, and autocast would not cast them."""
+    are plain ones of x's dtype, autocast would not cast them, and no forward-mode
+    derivative is wanted."""
     return (all(plain_linear(m) and m.weight.dtype == x.dtype for m in linears)
-            and x.dtype in DTYPES and x.dim() > 0 and not torch.is_autocast_enabled("cuda"))
+            and x.dtype in DTYPES and x.dim() > 0 and not torch.is_autocast_enabled("cuda")
+            and not forward_mode())
 
 
 def activation_name(module) -> str | None:

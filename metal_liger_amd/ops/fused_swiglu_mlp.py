@@ -8,7 +8,7 @@ power of two as scale for every 32 columns of a row; fp32 in fp32), or in 8
 is not kept; the backward forms it again of what was kept. What is not needed (x where
 gate's and up's weights are frozen) is not kept. h and the gradients of gate, up and h
 are rounded to bf16 between the products on the bf16 matrix cores. First derivatives
-only. Types and sizes as ops/fused_linear.py.
+only, in reverse mode (forward mode is refused). Types and sizes as ops/fused_linear.py.
 """
 
 from __future__ import annotations
@@ -125,7 +125,7 @@ class MetalLigerSwiGLUMLP(nn.Module):
 class _FusedMLPForward:
     """Forward of a routed MLP: the fused block, or the module's own forward where a
     projection is no longer a plain linear layer (an adapter was added since, a hook),
-    under autocast and for inputs of another dtype."""
+    under autocast, in forward mode and for inputs of another dtype."""
 
     def __init__(self, mlp: nn.Module, original, checkpoint: str | None):
         self.mlp, self.original, self.checkpoint = mlp, original, checkpoint
