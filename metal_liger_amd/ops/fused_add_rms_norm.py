@@ -19,15 +19,13 @@ bit-identical to the unfused pair; the backward rounds once where autograd
 rounds the norm's dx and the sum of the two gradients separately.
 
 ``patch_residual_add_norm(model)`` swaps the forward of each decoder layer
-whose forward has exactly that structure (checked on its bytecode: the four
-submodules in order and two additions) and whose post_attention_layernorm is
-a MetalLigerRMSNorm (so the numerics are the reference's fused norm's).
+whose forward computes exactly that (read from its source, _forward_form.py)
+and whose post_attention_layernorm is a MetalLigerRMSNorm (so the numerics are the reference's fused norm's).
 Modules and state_dict keys are unchanged.
 """
 
 from __future__ import annotations
 
-import dis
 import inspect
 import logging
 
@@ -35,6 +33,7 @@ import torch
 import torch.nn as nn
 
 from metal_liger_amd import _custom_ops as cops
+from metal_liger_amd._forward_form import add, arg, call, form, item, passed_on
 from metal_liger_amd.ops.fused_rms_norm import MetalLigerRMSNorm
 
 logger = logging.getLogger(__name__)
@@ -77,30 +76,20 @@ def fused_add_rms_norm(x: torch.Tensor, residual: torch.Tensor, norm: nn.Module)
 _LAYER_PARTS = ("input_layernorm", "self_attn", "post_attention_layernorm", "mlp")
 
 
-_CONTAINER_OPS = ("BUILD_TUPLE", "BUILD_LIST", "LIST_APPEND", "LIST_EXTEND", "LIST_TO_TUPLE")
-
-
 def _structure(fn) -> tuple:
-    """(attribute loads of the layer parts in order, number of additions
-    (in-place ones included), whether every return hands back one local
-    variable and no tuple or list is built) of a forward's bytecode. The
-    fused forward returns one tensor, so a layer that returns an outputs
-    tuple (older transformers: ``outputs = (hidden_states,)`` with attention
-    weights appended by ``+=``) does not match."""
-    parts, adds, single = [], 0, True
-    prev = None
-    for ins in dis.get_instructions(fn):
-        if ins.opname in ("LOAD_ATTR", "LOAD_METHOD") and ins.argval in _LAYER_PARTS:
-            parts.append(ins.argval)
-        elif ins.opname in ("BINARY_ADD", "INPLACE_ADD") or (
-                ins.opname == "BINARY_OP" and ins.argrepr in ("+", "+=")):
-            adds += 1
-        elif ins.opname in _CONTAINER_OPS:
-            single = False
-        elif ins.opname == "RETURN_VALUE" and (prev is None or prev.opname != "LOAD_FAST"):
-            single = False
-        prev = ins
-    return tuple(parts), adds, single
+    """(the layer parts that a forward calls, in order, its number of additions, whether
+    it returns h + mlp(post_attention_layernorm(h)) of h = hidden_states + the first of
+    the two results of self_attn(input_layernorm(hidden_states), every other argument)).
+    A layer that scales a branch, returns an outputs tuple (older transformers) or does
+    anything else besides does not match."""
+    f = form(fn)
+    if f is None or "hidden_states" not in f.params:
+        return (), 0, False
+    h = arg("hidden_states")
+    rest = passed_on(f, "hidden_states")
+    rest["kwargs"]["hidden_states"] = call("input_layernorm", h)
+    h = add(h, item(0, 2, call("self_attn", **rest)))
+    return f.calls, f.adds, f.value == add(h, call("mlp", call("post_attention_layernorm", h)))
 
 
 def _eligible(layer: nn.Module) -> bool:
@@ -108,12 +97,7 @@ def _eligible(layer: nn.Module) -> bool:
         return False
     if not isinstance(layer.post_attention_layernorm, MetalLigerRMSNorm):
         return False
-    fwd = getattr(type(layer).forward, "__func__", type(layer).forward)
-    try:
-        params = inspect.signature(fwd).parameters
-    except (TypeError, ValueError):
-        return False
-    return "hidden_states" in params and _structure(fwd) == (_LAYER_PARTS, 2, True)
+    return _structure(type(layer).forward) == (_LAYER_PARTS, 2, True)
 
 
 def _make_forward(layer: nn.Module, orig_fwd):

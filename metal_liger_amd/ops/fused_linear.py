@@ -18,7 +18,6 @@ holds infinities then has NaN for its gradient, where the formula may have numbe
 
 from __future__ import annotations
 
-import dis
 import inspect
 import logging
 
@@ -28,6 +27,7 @@ from torch.autograd import forward_ad
 
 from metal_liger_amd import _custom_ops as cops
 from metal_liger_amd import hip_ops
+from metal_liger_amd._forward_form import add, arg, call, form, passed_on
 
 logger = logging.getLogger(__name__)
 
@@ -236,38 +236,18 @@ class _FusedVisionMLPForward:
 _BLOCK_PARTS = ("norm1", "attn", "norm2", "mlp")
 
 
-def _block_structure(fn) -> tuple:
-    """(the block's parts in the order in which a forward's bytecode loads them, its
-    additions, whether it returns a local variable and keeps no tuple or list)."""
-    parts, adds, single, prev = [], 0, True, None
-    for ins in dis.get_instructions(fn):
-        if ins.opname in ("LOAD_ATTR", "LOAD_METHOD") and ins.argval in _BLOCK_PARTS:
-            parts.append(ins.argval)
-        elif ins.opname in ("BINARY_ADD", "INPLACE_ADD") or (
-                ins.opname == "BINARY_OP" and ins.argrepr in ("+", "+=")):
-            adds += 1
-        elif ins.opname in ("BUILD_LIST", "LIST_APPEND", "LIST_EXTEND") or (
-                ins.opname == "STORE_FAST" and prev is not None and prev.opname == "BUILD_TUPLE"):
-            single = False  # (a call with ** builds a tuple of its arguments)
-        elif ins.opname == "RETURN_VALUE" and (prev is None or prev.opname != "LOAD_FAST"):
-            single = False
-        prev = ins
-    return tuple(parts), adds, single
-
-
 def _fusable_block(block: nn.Module) -> bool:
-    """A vision block whose forward is h + attn(norm1(h), ...), then + mlp(norm2(h))."""
+    """A vision block whose forward is h + attn(norm1(h), ...), then + mlp(norm2(h)), with
+    every argument but h handed to attn."""
     if not all(hasattr(block, p) for p in _BLOCK_PARTS) or \
             not isinstance(block.mlp.__dict__.get("forward"), _FusedVisionMLPForward):
         return False
-    fn = inspect.unwrap(getattr(type(block).forward, "__func__", type(block).forward))
-    try:
-        first = list(inspect.signature(fn).parameters)[1]
-    except (TypeError, ValueError, IndexError):
+    f = form(type(block).forward)
+    if f is None or f.calls != _BLOCK_PARTS or f.params[:1] != ("hidden_states",):
         return False
-    # (attn stands before norm1: the method is looked up before its arguments are)
-    return first == "hidden_states" and _block_structure(fn) == (("attn", "norm1", "mlp", "norm2"),
-                                                                 2, True)
+    h = arg("hidden_states")
+    h = add(h, call("attn", call("norm1", h), **passed_on(f, "hidden_states")))
+    return f.value == add(h, call("mlp", call("norm2", h)))
 
 
 class _FusedVisionBlockForward:
@@ -295,7 +275,7 @@ def patch_vision_mlp(model: nn.Module, checkpoint: str | None = None) -> int:
     """Routes the MLPs of a vision tower (modules with linear_fc1, act_fn and linear_fc2
     as Qwen3-VL's blocks have them, whose forward is linear_fc2(act_fn(linear_fc1(x))))
     through the fused linear layers, and the additions around them where a block's
-    forward has transformers' structure. Returns how many MLPs were routed; only the
+    forward is transformers' (read from its source, _forward_form.py). Returns how many MLPs were routed; only the
     instances' ``forward`` changes, modules already routed are left as they are."""
     check_checkpoint(checkpoint)
     routed = 0
