@@ -201,14 +201,34 @@ def runs_fused(x, *linears) -> bool:
 
 def activation_name(module) -> str | None:
     """The name in ACTIVATIONS of an activation module (nn's, or transformers' by its
-    class name), None for any other."""
-    if isinstance(module, nn.SiLU):
+    class name) as it is, None for any other: a subclass or a replaced forward may
+    compute something else."""
+    if "forward" in getattr(module, "__dict__", ()):
+        return None
+    if type(module) is nn.SiLU:
         return "silu"
-    if isinstance(module, nn.GELU):
+    if type(module) is nn.GELU:
         return "gelu" if module.approximate == "none" else "gelu_tanh"
+    if type(module).__module__ != "transformers.activations":
+        return None
     # GELUTanh is gelu by tanh; GELUActivation is gelu, by torch or in Python
     return {"SiLUActivation": "silu", "GELUActivation": "gelu",
             "GELUTanh": "gelu_tanh", "PytorchGELUTanh": "gelu_tanh"}.get(type(module).__name__)
+
+
+def computes(module: nn.Module, value, *parts: str) -> bool:
+    """Whether a module's own forward has one argument x, returns value(x) and calls each
+    of the parts once (_forward_form.py)."""
+    f = form(type(module).forward) if "forward" not in module.__dict__ else None
+    return (f is not None and len(f.params) == 1 and f.var_kw is None
+            and sorted(f.calls) == sorted(parts) and f.value == value(arg(f.params[0])))
+
+
+_VISION_PARTS = ("linear_fc1", "act_fn", "linear_fc2")
+
+
+def _vision_formula(x):
+    return call("linear_fc2", call("act_fn", call("linear_fc1", x)))
 
 
 class _FusedVisionMLPForward:
@@ -220,7 +240,8 @@ class _FusedVisionMLPForward:
         self.mlp, self.original, self.checkpoint = mlp, original, checkpoint
         self.activation = activation_name(mlp.act_fn)
 
-    def __call__(self, hidden_state, residual=None):
+    def __call__(self, *args, residual=None, **kwargs):
+        hidden_state, = (*args, *kwargs.values())  # (by whatever name)
         fc1, fc2 = self.mlp.linear_fc1, self.mlp.linear_fc2
         if hooked(self.mlp.act_fn) or not runs_fused(hidden_state, fc1, fc2):
             out = self.original(hidden_state)
@@ -273,18 +294,19 @@ class _FusedVisionBlockForward:
 
 def patch_vision_mlp(model: nn.Module, checkpoint: str | None = None) -> int:
     """Routes the MLPs of a vision tower (modules with linear_fc1, act_fn and linear_fc2
-    as Qwen3-VL's blocks have them, whose forward is linear_fc2(act_fn(linear_fc1(x))))
-    through the fused linear layers, and the additions around them where a block's
+    as Qwen3-VL's blocks have them, whose own forward computes linear_fc2(act_fn(
+    linear_fc1(x))) and nothing else) through the fused linear layers, and the additions around them where a block's
     forward is transformers' (read from its source, _forward_form.py). Returns how many MLPs were routed; only the
     instances' ``forward`` changes, modules already routed are left as they are."""
     check_checkpoint(checkpoint)
     routed = 0
     for module in model.modules():
-        if not all(hasattr(module, n) for n in ("linear_fc1", "act_fn", "linear_fc2")) or \
-                hasattr(module, "norm") or getattr(module, "_metal_liger_vision_mlp", False):
+        if not all(hasattr(module, n) for n in _VISION_PARTS) or \
+                getattr(module, "_metal_liger_vision_mlp", False):
             continue
         if not (plain_linear(module.linear_fc1) and plain_linear(module.linear_fc2)
-                and activation_name(module.act_fn)):
+                and activation_name(module.act_fn)
+                and computes(module, _vision_formula, *_VISION_PARTS)):
             continue
         module.forward = _FusedVisionMLPForward(module, module.forward, checkpoint)
         module._metal_liger_vision_mlp = True

@@ -20,10 +20,11 @@ import torch.nn as nn
 
 from metal_liger_amd import _custom_ops as cops
 from metal_liger_amd import hip_ops
+from metal_liger_amd._forward_form import call, mul
 from metal_liger_amd._model_walk import find_layers
-from metal_liger_amd.ops.fused_linear import (check_checkpoint, check_input, check_residual,
-                                              hooked, keep_mode, plain_linear, rows, runs_fused,
-                                              wants_grad)
+from metal_liger_amd.ops.fused_linear import (activation_name, check_checkpoint, check_input,
+                                              check_residual, computes, hooked, keep_mode,
+                                              plain_linear, rows, runs_fused, wants_grad)
 from metal_liger_amd.ops.fused_swiglu import MetalLigerSwiGLU
 
 logger = logging.getLogger(__name__)
@@ -88,14 +89,24 @@ def fused_swiglu_mlp(x: torch.Tensor, gate_weight: torch.Tensor, up_weight: torc
 _PROJECTIONS = ("gate_proj", "up_proj", "down_proj")
 
 
-def _fusable(mlp: nn.Module) -> bool:
-    """A gated MLP of three plain linear layers without bias, on SiLU."""
+def _gated_formula(x):
+    return call("down_proj", mul(call("act_fn", call("gate_proj", x)), call("up_proj", x)))
+
+
+def _gated(mlp: nn.Module) -> bool:
+    """Three plain linear layers without bias, and SiLU."""
     projections = [getattr(mlp, name, None) for name in _PROJECTIONS]
     if not all(plain_linear(m) and m.bias is None for m in projections):
         return False
     act = getattr(mlp, "act_fn", None)  # MetalLigerSwiGLU has none: SiLU
-    return isinstance(mlp, MetalLigerSwiGLU) if act is None else \
-        isinstance(act, nn.SiLU) or type(act).__name__ == "SiLUActivation"
+    return type(mlp) is MetalLigerSwiGLU if act is None else activation_name(act) == "silu"
+
+
+def _fusable(mlp: nn.Module) -> bool:
+    """A gated MLP of such parts whose own forward computes their formula and nothing
+    else."""
+    return _gated(mlp) and (type(mlp) is MetalLigerSwiGLU and "forward" not in mlp.__dict__
+                            or computes(mlp, _gated_formula, *_PROJECTIONS, "act_fn"))
 
 
 class MetalLigerSwiGLUMLP(nn.Module):
@@ -106,9 +117,13 @@ class MetalLigerSwiGLUMLP(nn.Module):
     def __init__(self, original_mlp: nn.Module, checkpoint: str | None = None):
         super().__init__()
         check_checkpoint(checkpoint)
-        if not _fusable(original_mlp):
+        # (a routed module is one already; one without a forward only holds the parts)
+        if not (_fusable(original_mlp) or _gated(original_mlp) and
+                (type(original_mlp).forward is nn.Module.forward or
+                 isinstance(original_mlp.__dict__.get("forward"), _FusedMLPForward))):
             raise ValueError("MetalLigerSwiGLUMLP: gate_proj, up_proj and down_proj must be plain "
-                             f"nn.Linear layers without bias, on SiLU (got {original_mlp})")
+                             "nn.Linear layers without bias, on SiLU, in a forward of nothing else "
+                             f"(got {original_mlp})")
         self.gate_proj = original_mlp.gate_proj
         self.up_proj = original_mlp.up_proj
         self.down_proj = original_mlp.down_proj
@@ -130,7 +145,8 @@ class _FusedMLPForward:
     def __init__(self, mlp: nn.Module, original, checkpoint: str | None):
         self.mlp, self.original, self.checkpoint = mlp, original, checkpoint
 
-    def __call__(self, x):
+    def __call__(self, *args, **kwargs):
+        x, = (*args, *kwargs.values())  # (by whatever name)
         gate, up, down = (getattr(self.mlp, name) for name in _PROJECTIONS)
         if hooked(getattr(self.mlp, "act_fn", None)) or not runs_fused(x, gate, up, down):
             return self.original(x)
@@ -149,7 +165,7 @@ def patch_swiglu_mlp(model: nn.Module, checkpoint: str | None = None) -> int:
     routed = 0
     for layer in layers:
         mlp = getattr(layer, "mlp", None)
-        if mlp is None or "forward" in mlp.__dict__ or not _fusable(mlp):
+        if mlp is None or not _fusable(mlp):
             continue
         mlp.forward = _FusedMLPForward(mlp, mlp.forward, checkpoint)
         routed += 1
