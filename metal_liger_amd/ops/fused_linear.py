@@ -190,13 +190,11 @@ def plain_linear(module) -> bool:
             and not hooked(module))
 
 
-def runs_fused(x, *linears) -> bool:
-    """Whether a routed module's forward may run the fused op for x: its linear layers
-    are plain ones of x's dtype, autocast would not cast them, and no forward-mode
-    derivative is wanted."""
-    return (all(plain_linear(m) and m.weight.dtype == x.dtype for m in linears)
-            and x.dtype in DTYPES and x.dim() > 0 and not torch.is_autocast_enabled("cuda")
-            and not forward_mode())
+def takes(x, *linears) -> bool:
+    """Whether a routed module's forward may run the fused op for x: its linear layers are
+    of x's dtype, autocast would not cast them, and no forward-mode derivative is wanted."""
+    return (all(m.weight.dtype == x.dtype for m in linears) and x.dtype in DTYPES and x.dim() > 0
+            and not torch.is_autocast_enabled("cuda") and not forward_mode())
 
 
 def activation_name(module) -> str | None:
@@ -233,22 +231,27 @@ def _vision_formula(x):
 
 class _FusedVisionMLPForward:
     """Forward of a vision block's MLP, linear_fc2(act_fn(linear_fc1(x))), with the
-    activation and (residual given) the block's addition in the products' epilogues.
-    Where runs_fused does not hold, the module's own forward."""
+    activation and (residual given) the block's addition in the products' epilogues. The
+    module's own forward where its parts, looked at in every call, are no longer plain
+    linear layers and an activation as it is, or takes() does not hold."""
 
     def __init__(self, mlp: nn.Module, original, checkpoint: str | None):
         self.mlp, self.original, self.checkpoint = mlp, original, checkpoint
-        self.activation = activation_name(mlp.act_fn)
+
+    @property
+    def activation(self) -> str | None:
+        return activation_name(self.mlp.act_fn)
 
     def __call__(self, *args, residual=None, **kwargs):
         hidden_state, = (*args, *kwargs.values())  # (by whatever name)
-        fc1, fc2 = self.mlp.linear_fc1, self.mlp.linear_fc2
-        if hooked(self.mlp.act_fn) or not runs_fused(hidden_state, fc1, fc2):
+        fc1, fc2, activation = self.mlp.linear_fc1, self.mlp.linear_fc2, self.activation
+        if activation is None or hooked(self.mlp.act_fn) or \
+                not (plain_linear(fc1) and plain_linear(fc2) and takes(hidden_state, fc1, fc2)):
             out = self.original(hidden_state)
             return out if residual is None else residual + out
         fused = residual is not None and residual.dtype == hidden_state.dtype and \
             residual.shape == (*hidden_state.shape[:-1], fc2.weight.shape[0])
-        h = fused_linear(hidden_state, fc1.weight, fc1.bias, self.activation,
+        h = fused_linear(hidden_state, fc1.weight, fc1.bias, activation,
                          checkpoint=self.checkpoint)
         out = fused_linear(h, fc2.weight, fc2.bias, residual=residual if fused else None)
         return out if fused or residual is None else residual + out

@@ -24,7 +24,7 @@ from metal_liger_amd._forward_form import call, mul
 from metal_liger_amd._model_walk import find_layers
 from metal_liger_amd.ops.fused_linear import (activation_name, check_checkpoint, check_input,
                                               check_residual, computes, hooked, keep_mode,
-                                              plain_linear, rows, runs_fused, wants_grad)
+                                              plain_linear, rows, takes, wants_grad)
 from metal_liger_amd.ops.fused_swiglu import MetalLigerSwiGLU
 
 logger = logging.getLogger(__name__)
@@ -138,17 +138,20 @@ class MetalLigerSwiGLUMLP(nn.Module):
 
 
 class _FusedMLPForward:
-    """Forward of a routed MLP: the fused block, or the module's own forward where a
-    projection is no longer a plain linear layer (an adapter was added since, a hook),
-    under autocast, in forward mode and for inputs of another dtype."""
+    """Forward of a routed MLP: the fused block, or the module's own forward where its
+    parts, looked at in every call, are no longer what _gated asks for (an adapter was
+    added since, a bias, a hook, another activation), under autocast, in forward mode and
+    for inputs of another dtype."""
 
     def __init__(self, mlp: nn.Module, original, checkpoint: str | None):
         self.mlp, self.original, self.checkpoint = mlp, original, checkpoint
 
     def __call__(self, *args, **kwargs):
         x, = (*args, *kwargs.values())  # (by whatever name)
+        if not _gated(self.mlp) or hooked(getattr(self.mlp, "act_fn", None)):
+            return self.original(x)
         gate, up, down = (getattr(self.mlp, name) for name in _PROJECTIONS)
-        if hooked(getattr(self.mlp, "act_fn", None)) or not runs_fused(x, gate, up, down):
+        if not takes(x, gate, up, down):
             return self.original(x)
         return fused_swiglu_mlp(x, gate.weight, up.weight, down.weight, checkpoint=self.checkpoint)
 

@@ -181,3 +181,53 @@ def test_a_module_that_only_holds_the_parts():
     assert fm.MetalLigerSwiGLUMLP(parts).up_proj is own.up_proj
     assert fm.patch_swiglu_mlp(_layers(own)) == 1
     assert fm.MetalLigerSwiGLUMLP(own).up_proj is own.up_proj  # a routed one
+
+
+# ------------------------------------------------- parts that change afterwards --
+
+def _biased(linear):
+    new = nn.Linear(linear.in_features, linear.out_features)
+    new.weight = linear.weight
+    return new
+
+
+CHANGES = {
+    "another layer, with a bias": lambda m: setattr(m, "up_proj", _biased(m.up_proj)),
+    "a bias": lambda m: setattr(m.down_proj, "bias", nn.Parameter(torch.ones(24))),
+    "another activation": lambda m: setattr(m, "act_fn", nn.GELU()),
+    "an activation's forward": lambda m: setattr(m.act_fn, "forward", lambda x: x),
+    "a subclass": lambda m: setattr(m, "act_fn", Doubled()),
+    "another dtype": lambda m: m.double(),
+}
+
+
+@pytest.mark.parametrize("change", list(CHANGES))
+def test_a_gated_mlp_changed_after_it_was_routed(formulas, change):
+    mlp, own = Gated(), Gated()
+    own.load_state_dict(mlp.state_dict())
+    assert fm.patch_swiglu_mlp(_layers(mlp)) == 1
+    x = seeded((3, 24), 1)
+    mlp(x)
+    with torch.random.fork_rng():
+        for m in (mlp, own):
+            torch.manual_seed(0)
+            CHANGES[change](m)
+    x = x.to(mlp.up_proj.weight.dtype)
+    if change == "another dtype":  # (fp64 is none of the operator's)
+        assert formulas == ["mlp"]
+    assert torch.equal(mlp(x), own(x)) and formulas == ["mlp"]
+
+
+def test_a_vision_mlp_changed_after_it_was_routed(formulas):
+    x = seeded((3, 24), 1)
+    for change, same_op in ((lambda m: setattr(m, "act_fn", nn.ReLU()), False),
+                            (lambda m: setattr(m, "act_fn", Doubled()), False),
+                            (lambda m: setattr(m, "act_fn", nn.SiLU()), True),
+                            (lambda m: setattr(m.act_fn, "approximate", "tanh"), True)):
+        mlp, own = Vision(), Vision()
+        own.load_state_dict(mlp.state_dict())
+        assert fl.patch_vision_mlp(mlp) == 1 and mlp.forward.activation == "gelu"
+        change(mlp)
+        change(own)
+        del formulas[:]
+        assert torch.allclose(mlp(x), own(x), atol=1e-6) and (formulas == 2 * ["linear"]) == same_op
