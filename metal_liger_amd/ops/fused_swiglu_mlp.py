@@ -17,6 +17,7 @@ import logging
 
 import torch
 import torch.nn as nn
+import torch.nn.functional as F
 
 from metal_liger_amd import _custom_ops as cops
 from metal_liger_amd import hip_ops
@@ -93,10 +94,15 @@ def _gated_formula(x):
     return call("down_proj", mul(call("act_fn", call("gate_proj", x)), call("up_proj", x)))
 
 
+def _plain_projections(mlp: nn.Module) -> bool:
+    """Three plain linear layers without bias."""
+    projections = [getattr(mlp, name, None) for name in _PROJECTIONS]
+    return all(plain_linear(m) and m.bias is None for m in projections)
+
+
 def _gated(mlp: nn.Module) -> bool:
     """Three plain linear layers without bias, and SiLU."""
-    projections = [getattr(mlp, name, None) for name in _PROJECTIONS]
-    if not all(plain_linear(m) and m.bias is None for m in projections):
+    if not _plain_projections(mlp):
         return False
     act = getattr(mlp, "act_fn", None)  # MetalLigerSwiGLU has none: SiLU
     return type(mlp) is MetalLigerSwiGLU if act is None else activation_name(act) == "silu"
@@ -112,7 +118,9 @@ def _fusable(mlp: nn.Module) -> bool:
 class MetalLigerSwiGLUMLP(nn.Module):
     """Drop-in for a gated MLP (gate_proj, up_proj, down_proj without bias, SiLU), whose
     projections it keeps under their names (state_dict keys are unchanged); forward also
-    takes a residual to add."""
+    takes a residual to add. Where a projection has become something else since (an
+    adapter's wrapper, a hook, a bias), under autocast, in forward mode and for inputs of
+    another dtype, forward calls the projections themselves."""
 
     def __init__(self, original_mlp: nn.Module, checkpoint: str | None = None):
         super().__init__()
@@ -130,8 +138,12 @@ class MetalLigerSwiGLUMLP(nn.Module):
         self.checkpoint = checkpoint
 
     def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None) -> torch.Tensor:
-        return fused_swiglu_mlp(x, self.gate_proj.weight, self.up_proj.weight,
-                                self.down_proj.weight, residual, self.checkpoint)
+        gate, up, down = self.gate_proj, self.up_proj, self.down_proj
+        if _plain_projections(self) and takes(x, gate, up, down):
+            return fused_swiglu_mlp(x, gate.weight, up.weight, down.weight, residual,
+                                    self.checkpoint)
+        y = down(F.silu(gate(x)) * up(x))
+        return y if residual is None else y + residual
 
     def extra_repr(self) -> str:
         return f"checkpoint={self.checkpoint}"

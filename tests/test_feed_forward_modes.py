@@ -8,7 +8,8 @@ from torch.autograd import forward_ad
 
 from metal_liger_amd import _custom_ops as cops
 from metal_liger_amd.ops.fused_linear import fused_linear, patch_vision_mlp
-from metal_liger_amd.ops.fused_swiglu_mlp import fused_swiglu_mlp, patch_swiglu_mlp
+from metal_liger_amd.ops.fused_swiglu_mlp import (MetalLigerSwiGLUMLP, fused_swiglu_mlp,
+                                                  patch_swiglu_mlp)
 from tests import qwen_tiny
 from tests.parity import seeded
 
@@ -65,3 +66,15 @@ def test_compiled_whole(call):
     step = torch.compile(call, fullgraph=True, backend="eager")
     with pytest.raises(Exception, match="ROCm GPU"):
         step(seeded((3, 8), 1), seeded((4, 8), 2))
+
+
+def test_compiled_modules():
+    """Modules too, their checks in each call included."""
+    model = qwen_tiny.build_vl()
+    mlp, vision = model.model.language_model.layers[0].mlp, model.model.visual.blocks[0].mlp
+    own = MetalLigerSwiGLUMLP(mlp)
+    assert patch_swiglu_mlp(model) == 2 and patch_vision_mlp(model) == 1
+    for m, width in ((own, 128), (mlp, 128), (vision, 64)):
+        step = torch.compile(lambda x: m(x), fullgraph=True, backend="eager")
+        with pytest.raises(Exception, match="ROCm GPU"):
+            step(seeded((3, width), 1))

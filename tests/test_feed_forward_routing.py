@@ -9,8 +9,8 @@ import torch.nn.functional as F
 from metal_liger_amd.ops import fused_linear as fl
 from metal_liger_amd.ops import fused_swiglu_mlp as fm
 from metal_liger_amd.ops.fused_swiglu import MetalLigerSwiGLU
-from tests import qwen_tiny
 from tests.parity import seeded
+from tests.peft_shim import LoraLinear, init_lora
 
 ACTS = {None: lambda z: z, "silu": F.silu, "gelu": F.gelu,
         "gelu_tanh": lambda z: F.gelu(z, approximate="tanh")}
@@ -231,3 +231,38 @@ def test_a_vision_mlp_changed_after_it_was_routed(formulas):
         change(own)
         del formulas[:]
         assert torch.allclose(mlp(x), own(x), atol=1e-6) and (formulas == 2 * ["linear"]) == same_op
+
+
+def _with_adapter(m):
+    m.gate_proj = LoraLinear(m.gate_proj, r=4, alpha=8)
+    init_lora(m.gate_proj, 3, b_std=0.3)
+
+
+def _with_hook(m):
+    m.up_proj.register_forward_hook(lambda module, args, out: 2 * out)
+
+
+@pytest.mark.parametrize("change", [None, _with_adapter, _with_hook, CHANGES["a bias"],
+                                    CHANGES["another layer, with a bias"], CHANGES["another dtype"]])
+def test_the_module_after_its_projections_changed(formulas, change):
+    """What the projections have become counts, in the output and for the gradients."""
+    own = Gated()
+    m = fm.MetalLigerSwiGLUMLP(own)  # (the same projections)
+    x, fused = seeded((3, 24), 1), ["mlp", "mlp"] if change is None else []
+    if change is not None:
+        with torch.random.fork_rng():
+            torch.manual_seed(0)
+            change(m)
+        own.gate_proj, own.up_proj, own.down_proj = m.gate_proj, m.up_proj, m.down_proj
+    x = x.to(own.up_proj.weight.dtype)
+    for y, want in ((m(x), own(x)), (m(x, x), own(x) + x)):
+        assert torch.allclose(y, want, atol=1e-6)
+        y.sum().backward()
+    assert formulas == fused and all(p.grad is not None for p in m.parameters())
+
+
+def test_the_module_under_autocast(formulas, monkeypatch):
+    m, x = fm.MetalLigerSwiGLUMLP(Gated()), seeded((3, 24), 1)
+    monkeypatch.setattr(torch, "is_autocast_enabled", lambda device=None: True)
+    m(x)
+    assert formulas == []
