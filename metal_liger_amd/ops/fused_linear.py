@@ -290,7 +290,8 @@ class _FusedVisionBlockForward:
         extra = rest.pop(self.var_kw, {}) if self.var_kw else {}
         h, b = rest.pop("hidden_states"), self.block
         h = h + b.attn(b.norm1(h), **rest, **extra)
-        if hooked(b.mlp):  # (they see the MLP's own output)
+        # (hooks see the MLP's own output; another MLP adds nothing)
+        if hooked(b.mlp) or not isinstance(b.mlp.__dict__.get("forward"), _FusedVisionMLPForward):
             return h + b.mlp(b.norm2(h))
         return b.mlp(b.norm2(h), residual=h)
 

@@ -212,6 +212,20 @@ def test_blocks_that_compute_the_same_are_routed(monkeypatch):
     assert type(fl_block.forward) is fl._FusedVisionBlockForward
 
 
+def test_a_block_whose_mlp_was_replaced(monkeypatch):
+    """After the block was routed, its MLP is wrapped or given another forward."""
+    monkeypatch.setattr(torch, "is_autocast_enabled", lambda device=None: True)
+    x = seeded((4, 64), 1)
+    for change in (lambda b: setattr(b, "mlp", nn.Sequential(b.mlp)),
+                   lambda b: setattr(b.mlp, "forward", lambda t: 2 * t)):
+        model, block = _tower(Same)
+        own = copy.deepcopy(block)
+        assert fl.patch_vision_mlp(model) == 1
+        change(block)
+        change(own)
+        assert torch.equal(block(x, None), own(x, None))
+
+
 # ------------------------------------------------------------ decoder layers --
 
 class DecoderLayer(nn.Module):
