@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define ML_ABI_VERSION 14
+#define ML_ABI_VERSION 15
 
 /* dtype tags */
 #define ML_F32 0
@@ -714,6 +714,31 @@ int ml_swiglu_mlp_bwd(const void* x, int64_t ldx, const void* wg, int64_t ldg, c
                       const void* up_scale, void* dx, void* dwg, void* dwu, void* dwd, int64_t M,
                       int64_t H, int64_t I, int64_t O, void* workspace, size_t workspace_bytes,
                       int dtype, void* stream);
+
+/*
+ * The same on operands padded with zeros: columns data_n .. N - 1 of z, and data_i .. I - 1
+ * of gate, up, h and their gradients, are padding and are taken as zeros (a padded zero
+ * times an infinity of x or dy would make them NaN, and every result that reads them). A
+ * z that was kept so needs nothing more in ml_linear_bwd.
+ */
+int ml_linear_fwd_padded(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias,
+                         const void* residual, int64_t ldr, int act, void* y, int64_t ldy,
+                         int keep, void* z, void* zscale, int64_t M, int64_t N, int64_t K,
+                         int64_t data_n, void* workspace, size_t workspace_bytes, int dtype,
+                         void* stream);
+int ml_swiglu_mlp_fwd_padded(const void* x, int64_t ldx, const void* wg, int64_t ldg,
+                             const void* wu, int64_t ldu, const void* wd, int64_t ldd,
+                             const void* residual, int64_t ldr, void* y, int keep, void* gate,
+                             void* gate_scale, void* up, void* up_scale, int64_t M, int64_t H,
+                             int64_t I, int64_t O, int64_t data_i, void* workspace,
+                             size_t workspace_bytes, int dtype, void* stream);
+int ml_swiglu_mlp_bwd_padded(const void* x, int64_t ldx, const void* wg, int64_t ldg,
+                             const void* wu, int64_t ldu, const void* wd, int64_t ldd,
+                             const void* dy, int64_t ldy, int keep, const void* gate,
+                             const void* gate_scale, const void* up, const void* up_scale,
+                             void* dx, void* dwg, void* dwu, void* dwd, int64_t M, int64_t H,
+                             int64_t I, int64_t O, int64_t data_i, void* workspace,
+                             size_t workspace_bytes, int dtype, void* stream);
 
 /*
  * Up to 8 matrices copied into dense ones padded with zeros (to_wide), or out of them

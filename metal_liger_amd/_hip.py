@@ -79,6 +79,21 @@ SIGNATURES: dict[str, tuple] = {
         [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _p, _p, _p, _p, _p, _p, _p, _p,
          _i64, _i64, _i64, _i64, _p, _sz, _i32, _p],
     ),
+    "ml_linear_fwd_padded": (
+        _i32,
+        [_p, _i64, _p, _i64, _p, _p, _i64, _i32, _p, _i64, _i32, _p, _p, _i64, _i64, _i64, _i64, _p,
+         _sz, _i32, _p],
+    ),
+    "ml_swiglu_mlp_fwd_padded": (
+        _i32,
+        [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i32, _p, _p, _p, _p, _i64, _i64,
+         _i64, _i64, _i64, _p, _sz, _i32, _p],
+    ),
+    "ml_swiglu_mlp_bwd_padded": (
+        _i32,
+        [_p, _i64, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i32, _p, _p, _p, _p, _p, _p, _p, _p,
+         _i64, _i64, _i64, _i64, _i64, _p, _sz, _i32, _p],
+    ),
     "ml_pad_matrices": (
         _i32, [_i32, ctypes.POINTER(_p), _i64p, _i64p, ctypes.POINTER(_p), _i64p, _i32, _i32, _p],
     ),
@@ -221,7 +236,7 @@ SIGNATURES: dict[str, tuple] = {
     ),
 }
 
-ABI_VERSION = 14
+ABI_VERSION = 15
 
 _lib = None
 _lock = threading.Lock()

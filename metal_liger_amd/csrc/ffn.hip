@@ -412,6 +412,12 @@ int check_sizes(int64_t M, int64_t N, int64_t K) {
   return ML_OK;
 }
 
+int check_data(int64_t data, int64_t cols) {
+  ML_CHECK(data > 0 && data <= cols, "ffn: %lld of %lld columns are not padding", (long long)data,
+           (long long)cols);
+  return ML_OK;
+}
+
 int check_kept(int keep, const void* v, const void* scale, const char* what) {
   ML_CHECK(keep >= kKeepNone && keep <= kKeepFp8, "ffn: bad way to keep %s (%d)", what, keep);
   ML_CHECK(keep == kKeepNone || v, "ffn: %s is kept but its buffer is null", what);
@@ -539,7 +545,7 @@ struct MlpFwd {
   void* y;
   int keep;
   void *gate, *gscale, *up, *uscale;
-  int64_t M, H, I, O;
+  int64_t M, H, I, O, data;
 };
 
 // The block of few rows: weights of T, h of TH (fp32 where T is fp16, whose range h may
@@ -567,7 +573,7 @@ int mlp_fwd(const MlpFwd& p, Arena& ws, bool run, hipStream_t st) {
   const T* wu = static_cast<const T*>(p.wu);
   const T* wd = static_cast<const T*>(p.wd);
   const GatedStep<In, KIND> step{h, p.I, make_kept<KIND>(p.gate, p.gscale, p.I),
-                                make_kept<KIND>(p.up, p.uscale, p.I)};
+                                make_kept<KIND>(p.up, p.uscale, p.I), p.data};
   const LinearStep<T, kKeepNone> out{nullptr, static_cast<const T*>(p.residual),
                                      static_cast<T*>(p.y), p.ldr, p.O, kActNone, {}};
   const bool vec = p.O % 8 == 0 && aligned_rows(p.residual, p.ldr) && aligned_rows(p.y, p.O);
@@ -608,7 +614,7 @@ struct MlpBwd {
   int keep;
   const void *gate, *gscale, *up, *uscale;
   void *dx, *dwg, *dwu, *dwd;
-  int64_t M, H, I, O;
+  int64_t M, H, I, O, data;
 };
 
 template <typename T, int KIND>
@@ -646,7 +652,7 @@ int mlp_bwd(const MlpBwd& p, Arena& ws, bool run, hipStream_t st) {
   const T* wd = static_cast<const T*>(p.wd);
   const GatedGradStep<In, KIND> step{dg, du, p.dwd ? h : nullptr, p.I,
                                     make_kept<KIND>(p.gate, p.gscale, p.I),
-                                    make_kept<KIND>(p.up, p.uscale, p.I)};
+                                    make_kept<KIND>(p.up, p.uscale, p.I), p.data};
   int splits = 1, rc = ML_OK;
   if (fuse) {
     if constexpr (kMayFuse)
@@ -691,12 +697,14 @@ extern "C" size_t ml_linear_fwd_workspace_bytes(int64_t M, int64_t N, int64_t K,
   return ws.used;
 }
 
-extern "C" int ml_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
-                             const void* bias, const void* residual, int64_t ldr, int act,
-                             void* y, int64_t ldy, int keep, void* z, void* zscale, int64_t M,
-                             int64_t N, int64_t K, void* workspace, size_t workspace_bytes,
-                             int dtype, void* stream) {
+extern "C" int ml_linear_fwd_padded(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                                    const void* bias, const void* residual, int64_t ldr, int act,
+                                    void* y, int64_t ldy, int keep, void* z, void* zscale,
+                                    int64_t M, int64_t N, int64_t K, int64_t data_n,
+                                    void* workspace, size_t workspace_bytes, int dtype,
+                                    void* stream) {
   ML_TRY(ffn::check_sizes(M, N, K));
+  ML_TRY(ffn::check_data(data_n, N));
   ML_CHECK(x && w && y, "linear: null pointer");
   ML_CHECK(act >= kActNone && act <= kActGeluTanh, "linear: bad activation %d", act);
   ML_CHECK(ldx >= K && ldw >= K && ldy >= N && (!residual || ldr >= N), "linear: bad row strides");
@@ -715,10 +723,19 @@ extern "C" int ml_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t 
     return ffn::dispatch_keep<T>(keep, [&](auto kind) {
       const ffn::LinearStep<T, kind.value> step{
           static_cast<const T*>(bias), static_cast<const T*>(residual), static_cast<T*>(y), ldr,
-          ldy, act, ffn::make_kept<kind.value>(z, zscale, N)};
+          ldy, act, ffn::make_kept<kind.value>(z, zscale, N), data_n};
       return ffn::linear_fwd<T>(x, ldx, w, ldw, step, M, N, K, ws, true, (hipStream_t)stream);
     });
   });
+}
+
+extern "C" int ml_linear_fwd(const void* x, int64_t ldx, const void* w, int64_t ldw,
+                             const void* bias, const void* residual, int64_t ldr, int act,
+                             void* y, int64_t ldy, int keep, void* z, void* zscale, int64_t M,
+                             int64_t N, int64_t K, void* workspace, size_t workspace_bytes,
+                             int dtype, void* stream) {
+  return ml_linear_fwd_padded(x, ldx, w, ldw, bias, residual, ldr, act, y, ldy, keep, z, zscale, M,
+                              N, K, N, workspace, workspace_bytes, dtype, stream);
 }
 
 extern "C" size_t ml_linear_bwd_workspace_bytes(int64_t M, int64_t N, int64_t K, int act,
@@ -790,13 +807,15 @@ extern "C" size_t ml_swiglu_mlp_fwd_workspace_bytes(int64_t M, int64_t H, int64_
   return ws.used;
 }
 
-extern "C" int ml_swiglu_mlp_fwd(const void* x, int64_t ldx, const void* wg, int64_t ldg,
-                                 const void* wu, int64_t ldu, const void* wd, int64_t ldd,
-                                 const void* residual, int64_t ldr, void* y, int keep, void* gate,
-                                 void* gate_scale, void* up, void* up_scale, int64_t M, int64_t H,
-                                 int64_t I, int64_t O, void* workspace, size_t workspace_bytes,
-                                 int dtype, void* stream) {
+extern "C" int ml_swiglu_mlp_fwd_padded(const void* x, int64_t ldx, const void* wg, int64_t ldg,
+                                        const void* wu, int64_t ldu, const void* wd, int64_t ldd,
+                                        const void* residual, int64_t ldr, void* y, int keep,
+                                        void* gate, void* gate_scale, void* up, void* up_scale,
+                                        int64_t M, int64_t H, int64_t I, int64_t O, int64_t data_i,
+                                        void* workspace, size_t workspace_bytes, int dtype,
+                                        void* stream) {
   ML_TRY(ffn::check_mlp(M, H, I, O));
+  ML_TRY(ffn::check_data(data_i, I));
   ML_CHECK(x && wg && wu && wd && y, "swiglu mlp: null pointer");
   ML_CHECK(ldx >= H && ldg >= H && ldu >= H && ldd >= I && (!residual || ldr >= O),
            "swiglu mlp: bad row strides");
@@ -815,11 +834,22 @@ extern "C" int ml_swiglu_mlp_fwd(const void* x, int64_t ldx, const void* wg, int
     ML_CHECK(workspace_bytes >= need && workspace && aligned16(workspace),
              "swiglu mlp: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     const ffn::MlpFwd p{x, wg, wu, wd, residual, ldx, ldg, ldu, ldd, ldr, y, keep,
-                        gate, gate_scale, up, up_scale, M, H, I, O};
+                        gate, gate_scale, up, up_scale, M, H, I, O, data_i};
     return ffn::dispatch_keep<T>(keep, [&](auto kind) {
       return ffn::mlp_fwd<T, kind.value>(p, ws, true, (hipStream_t)stream);
     });
   });
+}
+
+extern "C" int ml_swiglu_mlp_fwd(const void* x, int64_t ldx, const void* wg, int64_t ldg,
+                                 const void* wu, int64_t ldu, const void* wd, int64_t ldd,
+                                 const void* residual, int64_t ldr, void* y, int keep, void* gate,
+                                 void* gate_scale, void* up, void* up_scale, int64_t M, int64_t H,
+                                 int64_t I, int64_t O, void* workspace, size_t workspace_bytes,
+                                 int dtype, void* stream) {
+  return ml_swiglu_mlp_fwd_padded(x, ldx, wg, ldg, wu, ldu, wd, ldd, residual, ldr, y, keep, gate,
+                                  gate_scale, up, up_scale, M, H, I, O, I, workspace,
+                                  workspace_bytes, dtype, stream);
 }
 
 extern "C" size_t ml_swiglu_mlp_bwd_workspace_bytes(int64_t M, int64_t H, int64_t I, int64_t O,
@@ -835,14 +865,16 @@ extern "C" size_t ml_swiglu_mlp_bwd_workspace_bytes(int64_t M, int64_t H, int64_
   return ws.used;
 }
 
-extern "C" int ml_swiglu_mlp_bwd(const void* x, int64_t ldx, const void* wg, int64_t ldg,
-                                 const void* wu, int64_t ldu, const void* wd, int64_t ldd,
-                                 const void* dy, int64_t ldy, int keep, const void* gate,
-                                 const void* gate_scale, const void* up, const void* up_scale,
-                                 void* dx, void* dwg, void* dwu, void* dwd, int64_t M, int64_t H,
-                                 int64_t I, int64_t O, void* workspace, size_t workspace_bytes,
-                                 int dtype, void* stream) {
+extern "C" int ml_swiglu_mlp_bwd_padded(const void* x, int64_t ldx, const void* wg, int64_t ldg,
+                                        const void* wu, int64_t ldu, const void* wd, int64_t ldd,
+                                        const void* dy, int64_t ldy, int keep, const void* gate,
+                                        const void* gate_scale, const void* up,
+                                        const void* up_scale, void* dx, void* dwg, void* dwu,
+                                        void* dwd, int64_t M, int64_t H, int64_t I, int64_t O,
+                                        int64_t data_i, void* workspace, size_t workspace_bytes,
+                                        int dtype, void* stream) {
   ML_TRY(ffn::check_mlp(M, H, I, O));
+  ML_TRY(ffn::check_data(data_i, I));
   ML_CHECK(wd && dy && (!dx || (wg && wu)) && (!(dwg || dwu) || x),
            "swiglu mlp backward: null pointer");
   ML_CHECK((!x || ldx >= H) && (!wg || ldg >= H) && (!wu || ldu >= H) && ldd >= I && ldy >= O,
@@ -867,7 +899,7 @@ extern "C" int ml_swiglu_mlp_bwd(const void* x, int64_t ldx, const void* wg, int
     ML_CHECK(workspace_bytes >= need && workspace && aligned16(workspace),
              "swiglu mlp backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
     const ffn::MlpBwd p{x, wg, wu, wd, dy, ldx, ldg, ldu, ldd, ldy, keep, gate, gate_scale, up,
-                        up_scale, dx, dwg, dwu, dwd, M, H, I, O};
+                        up_scale, dx, dwg, dwu, dwd, M, H, I, O, data_i};
     return ffn::dispatch_keep<T>(keep, [&](auto kind) -> int {
       if constexpr (kind.value == ffn::kKeepNone)
         return ML_ERR_INVALID;  // (refused above)
@@ -875,6 +907,18 @@ extern "C" int ml_swiglu_mlp_bwd(const void* x, int64_t ldx, const void* wg, int
         return ffn::mlp_bwd<T, kind.value>(p, ws, true, (hipStream_t)stream);
     });
   });
+}
+
+extern "C" int ml_swiglu_mlp_bwd(const void* x, int64_t ldx, const void* wg, int64_t ldg,
+                                 const void* wu, int64_t ldu, const void* wd, int64_t ldd,
+                                 const void* dy, int64_t ldy, int keep, const void* gate,
+                                 const void* gate_scale, const void* up, const void* up_scale,
+                                 void* dx, void* dwg, void* dwu, void* dwd, int64_t M, int64_t H,
+                                 int64_t I, int64_t O, void* workspace, size_t workspace_bytes,
+                                 int dtype, void* stream) {
+  return ml_swiglu_mlp_bwd_padded(x, ldx, wg, ldg, wu, ldu, wd, ldd, dy, ldy, keep, gate,
+                                  gate_scale, up, up_scale, dx, dwg, dwu, dwd, M, H, I, O, I,
+                                  workspace, workspace_bytes, dtype, stream);
 }
 
 // ----------------------------------------------------------------- padding --

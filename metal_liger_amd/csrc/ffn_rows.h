@@ -166,6 +166,19 @@ __device__ __forceinline__ void act_grad_vec(int act, float (&x)[B][VEC]) {
 // lane's position exists (ALL: every one does), else what column and fetch gave of it is
 // not used.
 
+// data (of the steps whose outputs a product or a backward reads): columns from it on are
+// padding beside the operands' own and are written as zeros. The sums there are zeros
+// already, unless an infinity met a padded zero: that NaN would reach every column of the
+// next product.
+template <int VEC, int B>
+__device__ __forceinline__ void zero_padding(int64_t n, int64_t data, float (&x)[B][VEC]) {
+  if (n + VEC <= data) return;
+#pragma unroll
+  for (int q = 0; q < B; ++q)
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) x[q][k] = n + k < data ? x[q][k] : 0.f;
+}
+
 // cost: which of the times measured with products it goes by (ffn_product.h).
 enum : int { kPlainStep, kActStep, kPairStep, kGradStep };
 
@@ -178,6 +191,7 @@ struct LinearStep {
   int64_t ldr, ldy;
   int act;
   Kept<KIND> z;
+  int64_t data = INT64_MAX;
 
   int cost() const { return act == kActNone && KIND == kKeepNone ? kPlainStep : kActStep; }
 
@@ -217,6 +231,7 @@ struct LinearStep {
     for (int q = 0; q < B; ++q)
 #pragma unroll
       for (int k = 0; k < VEC; ++k) x[q][k] += c.b[k];
+    if constexpr (KIND != kKeepNone) zero_padding<VEC, B>(n, data, x);
     z.template put<ALL, VEC, B>(m, n, x, live);
     act_fwd_vec<VEC, B>(act, x);
     if (residual) {
@@ -237,6 +252,7 @@ struct GatedStep {
   T* h;  // dense
   int64_t cols;
   Kept<KIND> gate, up;
+  int64_t data = INT64_MAX;
 
   int cost() const { return kPairStep; }
 
@@ -254,6 +270,8 @@ struct GatedStep {
   __device__ __forceinline__ void finish(const int64_t (&m)[B], int64_t n, float (&g)[B][VEC],
                                          float (&u)[B][VEC], const Column<VEC>&,
                                          const Fetched<VEC> (&)[B], const bool (&live)[B]) const {
+    zero_padding<VEC, B>(n, data, g);
+    zero_padding<VEC, B>(n, data, u);
     gate.template put<ALL, VEC, B>(m, n, g, live);
     up.template put<ALL, VEC, B>(m, n, u, live);
 #pragma unroll
@@ -274,6 +292,7 @@ struct GatedGradStep {
   T* h;  // or null
   int64_t cols;
   Kept<KIND> gate, up;
+  int64_t data = INT64_MAX;
 
   int cost() const { return kGradStep; }
 
@@ -296,6 +315,7 @@ struct GatedGradStep {
                                          const Column<VEC>&, const Fetched<VEC> (&f)[B],
                                          const bool (&live)[B]) const {
     float g[B][VEC], u[B][VEC];
+    zero_padding<VEC, B>(n, data, dh);  // (g and u were kept as zeros there)
 #pragma unroll
     for (int q = 0; q < B; ++q) {
       gate.template decode<VEC>(f[q].g, g[q]);

@@ -378,8 +378,8 @@ def _linear(x2, w, bias, residual, act: int, keep: int, z, zscale):
         wide.begin()
         (px, ldx), (pw, ldw), (pb, _), (pr, ldr), (py, ldy) = map(wide.at, (*ins, out))
         ws, wsb = _workspace(x2, "ml_linear_fwd_workspace_bytes", M, Np, Kp, tag)
-        call("ml_linear_fwd", px, ldx, pw, ldw, pb, pr, ldr, act, py, ldy, *kept, M, Np, Kp, ptr(ws),
-             wsb, tag, stream_of(x2))
+        call("ml_linear_fwd_padded", px, ldx, pw, ldw, pb, pr, ldr, act, py, ldy, *kept, M, Np, Kp, N,
+             ptr(ws), wsb, tag, stream_of(x2))
         wide.end()
         return y
     x2, w = _product_rows(x2), _product_rows(w)
@@ -459,8 +459,8 @@ def _swiglu_mlp(x2, wg, wu, wd, residual, keep: int, kept):
         out = wide.result(y, M, Op)
         wide.begin()
         ws, wsb = _workspace(x2, "ml_swiglu_mlp_fwd_workspace_bytes", M, Hp, Ip, Op, tag)
-        call("ml_swiglu_mlp_fwd", *(v for t in ins for v in wide.at(t)), wide.at(out)[0], *kept, M, Hp,
-             Ip, Op, ptr(ws), wsb, tag, stream_of(x2))
+        call("ml_swiglu_mlp_fwd_padded", *(v for t in ins for v in wide.at(t)), wide.at(out)[0], *kept,
+             M, Hp, Ip, Op, I, ptr(ws), wsb, tag, stream_of(x2))
         wide.end()
         return y
     x2, wg, wu, wd = map(_product_rows, (x2, wg, wu, wd))
@@ -518,8 +518,8 @@ def swiglu_mlp_bwd(x2, wg, wu, wd, dy, keep: int, gate, gate_scale, up, up_scale
               wide.result(outs[3], Op, Ip))
         wide.begin()
         ws, wsb = _workspace(dy, "ml_swiglu_mlp_bwd_workspace_bytes", M, Hp, Ip, Op, tag)
-        call("ml_swiglu_mlp_bwd", *(v for t in ins for v in wide.at(t)), *kept,
-             *(wide.at(t)[0] for t in to), M, Hp, Ip, Op, ptr(ws), wsb, tag, stream_of(dy))
+        call("ml_swiglu_mlp_bwd_padded", *(v for t in ins for v in wide.at(t)), *kept,
+             *(wide.at(t)[0] for t in to), M, Hp, Ip, Op, I, ptr(ws), wsb, tag, stream_of(dy))
         wide.end()
         return outs
     x2, wg, wu = (None if t is None else _product_rows(t) for t in (x2, wg, wu))

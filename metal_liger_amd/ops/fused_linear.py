@@ -12,8 +12,7 @@ reverse mode (forward mode is refused).
 
 bf16 runs on the bf16 matrix cores; fp32 and fp16 on the fp32 ones, with everything
 between input and output in fp32. The kernels take 16-bit sizes in multiples of 8, and
-fp32 ones faster: others are padded with zeros, which add nothing (but a row of x that
-holds infinities then has NaN for its gradient, where the formula may have numbers).
+fp32 ones faster: others are padded with zeros, which add nothing.
 """
 
 from __future__ import annotations
