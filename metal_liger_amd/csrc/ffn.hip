@@ -11,7 +11,8 @@
 //
 // bf16 runs on the bf16 matrix cores (gemm_core.h), fp32 and fp16 on the fp32 ones
 // (ffn_f32.h; what lies between fp16's products is fp32); forwards of few rows (up to
-// 128) on kernels of their own (ffn_skinny.h).
+// 128) on kernels of their own (ffn_skinny.h), where products of two fp16 operands run on
+// the fp16 matrix cores.
 #include <initializer_list>
 
 #include "ffn_f32.h"

@@ -8,7 +8,7 @@
 // last, partial round are split over K, as many ways as the estimate below finds best;
 // their fp32 partials lie in the workspace as the accumulators lie in the lanes (16
 // bytes a lane, whatever the tile's edges) and a second kernel sums them in split
-// order, one workgroup a tile. Bound by the matrix cores; [8192, 4304]^T [8192, 1152]:
+// order, eight workgroups a tile. Bound by the matrix cores; [8192, 4304]^T [8192, 1152]:
 // 188 us as 85 tiles, 90 split three ways and 17 to join; the gated block's three at 8192
 // tokens 660 us one by one, 546 and 16 together.
 #pragma once

@@ -10,8 +10,10 @@ scales), formed of the fp32 sums. What is not needed (x where the
 weight is frozen, W where x needs no gradient) is not kept. First derivatives only, in
 reverse mode (forward mode is refused).
 
-bf16 runs on the bf16 matrix cores; fp32 and fp16 on the fp32 ones, with everything
-between input and output in fp32. The kernels take 16-bit sizes in multiples of 8, and
+bf16 runs on the bf16 matrix cores, and dz is rounded to bf16 before its products (not in
+db's sum); fp32 and fp16 run on the fp32 ones, with everything between input and output in
+fp32 (fp16 forwards of up to 128 rows on the fp16 ones: the same products and sums, exact
+and in fp32). The kernels take 16-bit sizes in multiples of 8, and
 fp32 ones faster: others are padded with zeros, which add nothing.
 """
 

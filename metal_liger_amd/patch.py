@@ -123,6 +123,7 @@ def apply_metal_liger_to_qwen3vl(
     products with the activation in their epilogue (ops/fused_swiglu_mlp.py).
     fuse_vision_mlp: the MLPs of Qwen3-VL's vision tower, with the activation
     and the block's addition in the products' epilogues (ops/fused_linear.py).
+    Both take only modules whose own forward computes that and nothing else.
     mlp_checkpoint: "fp8" keeps what the MLPs' backward needs of the
     activation's inputs in 8 bits: in MLPs that this call routes or replaces
     (fuse_swiglu, fuse_mlp, fuse_vision_mlp, and fuse_lora without
