@@ -191,10 +191,15 @@ def plain_linear(module) -> bool:
             and not hooked(module))
 
 
+_PLAIN = (torch.Tensor, nn.Parameter)
+
+
 def takes(x, *linears) -> bool:
     """Whether a routed module's forward may run the fused op for x: its linear layers are
-    of x's dtype, autocast would not cast them, and no forward-mode derivative is wanted."""
-    return (all(m.weight.dtype == x.dtype for m in linears) and x.dtype in DTYPES and x.dim() > 0
+    of x's dtype, all are plain tensors (a subclass, sharded or quantized, has products of
+    its own), autocast would not cast them, and no forward-mode derivative is wanted."""
+    return (all(m.weight.dtype == x.dtype and type(m.weight) in _PLAIN for m in linears)
+            and type(x) in _PLAIN and x.dtype in DTYPES and x.dim() > 0
             and not torch.is_autocast_enabled("cuda") and not forward_mode())
 
 

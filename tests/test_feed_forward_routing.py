@@ -266,3 +266,24 @@ def test_the_module_under_autocast(formulas, monkeypatch):
     monkeypatch.setattr(torch, "is_autocast_enabled", lambda device=None: True)
     m(x)
     assert formulas == []
+
+
+class Sharded(torch.Tensor):
+    """A tensor subclass: what its products are is its own matter."""
+
+
+@pytest.mark.parametrize("part", ["x", "weight"])
+def test_tensor_subclasses(formulas, part):
+    x = seeded((3, 24), 1)
+    mlp, vision, own = Gated(), Vision(), Gated()
+    module = fm.MetalLigerSwiGLUMLP(own)
+    wants = [m(x) for m in (mlp, vision, own)]
+    assert fm.patch_swiglu_mlp(_layers(mlp)) == fl.patch_vision_mlp(vision) == 1
+    if part == "x":
+        x = x.as_subclass(Sharded)
+    else:
+        for m in (mlp.down_proj, vision.linear_fc2, module.gate_proj):
+            m.weight = nn.Parameter(m.weight.detach().as_subclass(Sharded))
+    for m, want in zip((mlp, vision, module), wants):
+        assert torch.equal(m(x).as_subclass(torch.Tensor), want)
+    assert formulas == []
